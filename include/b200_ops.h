@@ -754,6 +754,53 @@ int b200_conv_qknorm_store(const void* proj, long long ld, const float* bias, co
 int b200_moe_gather(const void* h, const long long* dest, const long long* tok, void* xs, long long assignments, long long row_bytes,
                     void* stream);
 
+/* Attention of a decode batch over a paged cache whose sequences share their first keys (csrc/prefix_attn.cu): out [T, H * D], token t over keys
+ * 0 .. pos[t] of row slot[t] of the block table (int32, rows of table_stride entries, `width` of them used). groups int32 [n_groups, 4] = (first token,
+ * tokens, shared keys, -): consecutive tokens whose sequences hold the same first keys; those are read once, from the first token's row. of
+ * int32 [T]: the group of a token, -1 for none. longest: tokens of the largest group. sinks fp32 [H] or NULL: a logit per head that only takes
+ * part in the sum. part: fp32 [T * H * nsplit * (D + 2)] scratch, nsplit = b200_prefix_attn_splits(...). Pools [n_pages, G, block_size, D];
+ * 16-bit types, D a multiple of 16 up to 128, block_size a power of two, scale > 0. A token with pos < 0, or a slot outside the table, sees no key:
+ * zero. Pages outside the pools are not read. */
+int b200_prefix_attn_splits(int n_groups, int longest, int max_shared, int H, int G);
+int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const void* cv, int n_pages, const int* pos, const int* slot,
+                     const int* table, long long table_stride, int table_rows, int width, const int* groups, const int* of, int n_groups,
+                     int longest, const float* sinks, void* out, float* part, int nsplit, int T, int H, int G, int D, int block_size,
+                     float scale, int dtype, void* stream);
+
+/* Block tables and maps of a serving step (csrc/step_maps.cu), from the requests' lengths on the device: rows, cached, lens / fresh int32 [n]
+ * (row of the block table, tokens in the cache, tokens after / new in the step); table int32, rows of table_stride entries of which
+ * width are used. extend: row i gets blocks ceil(cached / bs) .. ceil(lens / bs) - 1 off the list `blocks` in request order; used (int32, may be
+ * NULL): how many they need. Entries outside the table or beyond the list are left alone. maps: cu int32 [n + 1], pos / slot int32 [total], place
+ * int64 [total] (block * bs + offset, -1 where none is listed), last int64 [n]; with n_tiles > 0 tiles / tile_of int32 [n_tiles, 4] and runs /
+ * run_tiles int32 [n, 4], 16-byte aligned. */
+int b200_extend_block_tables(void* table, long long table_stride, int table_rows, int width, const void* rows, const void* cached,
+                             const void* lens, const void* blocks, int n_blocks, void* used, int n, int block_size, void* stream);
+int b200_step_maps(const void* table, long long table_stride, int table_rows, int width, const void* rows, const void* cached, const void* fresh,
+                   int n, int block_size, int total, int n_tiles, void* cu, void* pos, void* slot, void* place, void* last, void* tiles,
+                   void* tile_of, void* runs, void* run_tiles, void* stream);
+
+/* Rules on logits (csrc/logits.cu). Batch row b follows row slot[b] (NULL: b) of these tables; a slot outside 0 .. rows - 1 has no rules. */
+#ifndef B200_LOGIT_RULES
+#define B200_LOGIT_RULES
+typedef struct {
+  const int32_t *tokens, *length, *prompt_length;  /* [rows, width], [rows]: history, the first prompt_length of it the prompt */
+  const float *repetition, *presence, *frequency, *temperature;  /* [rows] */
+  const int32_t *bias_ids, *bias_length;           /* [rows, bias_width], [rows] */
+  const float* bias_values;                        /* [rows, bias_width] */
+  const int32_t* mask;                             /* [rows, words]: bit v % 32 of word v / 32 set = v allowed; NULL: no masks */
+  const uint8_t* masked;                           /* [rows]: nonzero = the row's mask holds */
+  int32_t rows, width, bias_width, words;
+} b200_logit_rules;
+#endif
+/* out fp32 [B, ldo]: seen: y < 0 ? y r : y / r; in the output c times: y -= f c, y -= p; y += bias; y /= T; not allowed: -inf. */
+int b200_process_logits(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, float* out, long long ldo, int dtype, void* stream);
+/* The best token of each row under these rules, the lowest of equals, NaN above all. workspace: b200_greedy_workspace(B, V) bytes. */
+long long b200_greedy_workspace(int B, int V);
+int b200_greedy_tokens(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, void* workspace, long long* ids, int dtype,
+                       void* stream);
+/* ids int64 [n] behind the histories of rows slot[i] (NULL: i), whose lengths go up by one; full rows and slots outside the table keep theirs. */
+int b200_append_tokens(int* tokens, int rows, int width, int* length, const int* slot, const long long* ids, int n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,14 @@ def stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def call_on(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` with the tensors' device as the current one, on its current stream."""
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args, stream())
+    with torch.cuda.device(device):
+        return fn(*args, stream())
+
+
 def ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 

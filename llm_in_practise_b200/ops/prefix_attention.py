@@ -1,0 +1,99 @@
+"""Attention of a decode batch whose sequences share their first keys (``csrc/prefix_attn.cu``): the keys and values of the shared part
+are read once for the whole group instead of once a sequence.
+
+The sequences of a serving batch often start alike: a system prompt, a few-shot preamble, one long document with many questions. A paged
+cache holds such a part once (the engine's prefix cache lists its blocks in every sequence's row), and ``paged_attention`` reads it
+once for every sequence. ``prefix_attention`` is told the groups (``make_prefix_groups``) and gives the same result.
+
+The reference's deployments turn on vLLM's prefix caching for this kind of traffic (Deployment/Ray/serve_run_examples/deepseek.py:29-34).
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import torch
+
+from . import _native as nv
+from .paged_attention import paged_attention
+
+vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+
+
+@dataclass
+class PrefixGroups:
+    """Which tokens of a step share their first keys. ``groups`` int32 [n_groups, 4] = (first token, tokens, shared keys, 0); ``of`` int32
+    [tokens]: the group of every token, -1 for none. ``longest`` (tokens of the largest group) and ``max_shared`` (shared keys of the group with
+    the most) are bounds known on the host; a plan that a captured graph replays may be rewritten on the device within them: tokens of a
+    group behind the ``longest``-th read all their keys by themselves, and ``max_shared`` only chooses how the work is cut."""
+    groups: torch.Tensor
+    of: torch.Tensor
+    n_groups: int
+    longest: int
+    max_shared: int
+
+
+def make_prefix_groups(groups: Sequence[Sequence[int]], tokens: int, device) -> PrefixGroups:
+    """The plan of a step of ``tokens`` tokens from its groups ``(first token, tokens, shared keys)``: runs of consecutive tokens, none of them in
+    two groups, whose sequences hold the same keys and values at positions ``0 .. shared - 1`` (in the same pages, or in copies)."""
+    rows, of = [], [-1] * tokens
+    for first, n, shared in ([int(v) for v in g] for g in groups):
+        if n < 0 or shared < 0 or first < 0 or first + n > tokens:
+            raise ValueError(f"make_prefix_groups: group ({first}, {n}, {shared}) is not within {tokens} tokens")
+        if n == 0 or shared == 0:
+            continue
+        if any(j >= 0 for j in of[first:first + n]):
+            raise ValueError("make_prefix_groups: a token is in two groups")
+        of[first:first + n] = [len(rows)] * n
+        rows.append([first, n, shared, 0])
+    host = torch.tensor([v for r in rows for v in r] + of, dtype=torch.int32)
+    dev = torch.device(device)
+    host = host.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else host
+    return PrefixGroups(host[:4 * len(rows)].view(-1, 4), host[4 * len(rows):], len(rows), max((r[1] for r in rows), default=0),
+                        max((r[2] for r in rows), default=0))
+
+
+def _int32(name, t, device, shape):
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"prefix_attention: {name} must be a contiguous int32 {list(shape)} tensor on the queries' device")
+
+
+def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
+                     groups: Optional[PrefixGroups], n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+                     sinks: Optional[torch.Tensor] = None, max_pos: int = 0) -> torch.Tensor:
+    """Context [T, H * D] of token t over keys ``0 .. pos[t]`` of cache row ``slot[t]``, as ``paged_attention`` gives it (same arguments; no
+    window), with the shared keys of ``groups`` read once. Tokens of a group whose position is before its last shared key, and tokens of no
+    group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. Caches of 16 bits with head sizes that
+    are multiples of 16 up to 128, pages of a power of two and a positive scale; others go through ``paged_attention``, as does a step without
+    groups. Captured into a graph, each call keeps a workspace of its own."""
+    T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
+    BS = cache_k.shape[2]
+    if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or q.dtype not in (torch.bfloat16, torch.float16) or D % 16 or D > 128
+            or BS & (BS - 1) or not scale > 0):
+        return paged_attention(q, cache_k, cache_v, table.contiguous(), pos, slot, H, G, D, scale, sinks=sinks, max_pos=max_pos)
+    dev = q.device
+    if cache_k.dtype != q.dtype or cache_v.dtype != q.dtype or cache_k.shape != cache_v.shape or cache_k.shape[1] != G or cache_k.shape[3] != D:
+        raise ValueError(f"prefix_attention: caches must be {q.dtype} [blocks, {G}, block_size, {D}], both of one shape")
+    if not cache_k.is_contiguous() or not cache_v.is_contiguous() or cache_k.device != dev or cache_v.device != dev:
+        raise ValueError("prefix_attention: caches must be contiguous and on the queries' device")
+    if H % G or q.dim() != 2 or q.shape[1] < H * D or (T and q.stride(1) != 1) or q.stride(0) % 8 or q.data_ptr() % 16:
+        raise ValueError(f"prefix_attention: queries must be rows of {H * D} or more contiguous values that start on 16 bytes")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("prefix_attention: the block table is int32 [rows, blocks] with contiguous rows on the queries' device")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous() or sinks.device != dev):
+        raise ValueError(f"prefix_attention: sinks must be contiguous fp32 [{H}] on the queries' device")
+    _int32("pos", pos, dev, (T,))
+    _int32("slot", slot, dev, (T,))
+    _int32("the groups' token table", groups.of, dev, (T,))
+    _int32("the groups' table", groups.groups, dev, (groups.n_groups, 4))
+    out = torch.empty(T, H * D, dtype=q.dtype, device=dev)
+    nsplit = nv.proto("b200_prefix_attn_splits", [i32] * 5)(groups.n_groups, groups.longest, groups.max_shared, H, G)
+    part = torch.empty(T * H * nsplit * (D + 2), dtype=torch.float32, device=dev)
+    fn = nv.proto("b200_prefix_attn", [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32,
+                                       i32, vp])
+    nv.check(nv.call_on(dev, fn, nv.ptr(q), q.stride(0), nv.ptr(cache_k), nv.ptr(cache_v), cache_k.shape[0], nv.ptr(pos), nv.ptr(slot), nv.ptr(table),
+                        table.stride(0), table.shape[0], table.shape[1], nv.ptr(groups.groups), nv.ptr(groups.of), groups.n_groups, groups.longest,
+                        nv.ptr(sinks), nv.ptr(out), nv.ptr(part), nsplit, T, H, G, D, BS, scale, nv.dtype_code(q.dtype)), "prefix_attn")
+    nv.count_launch(2)
+    return out

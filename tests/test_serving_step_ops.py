@@ -1,0 +1,607 @@
+"""Operators of a serving step that shares work between its sequences: attention over shared keys, block tables and maps from the
+requests' lengths, rules on logits. Each against a statement of its own in 64 bits (or in whole numbers), token by token; the plain PyTorch
+path on the CPU, the kernels on the GPU."""
+import itertools
+import math
+
+import pytest
+import torch
+
+from llm_in_practise_b200.ops import _native as nv
+from llm_in_practise_b200.ops.logits import LogitState, greedy_tokens, process_logits
+from llm_in_practise_b200.ops.prefix_attention import make_prefix_groups, prefix_attention
+from llm_in_practise_b200.ops.step_maps import extend_block_tables, step_maps
+
+CPU_AND_GPU = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture
+def entries(monkeypatch):
+    """Names of the entry points that took a call."""
+    names, real = [], nv.proto
+
+    def proto(name, argtypes):
+        fn = real(name, argtypes)
+
+        def call(*args):
+            rc = fn(*args)
+            names.append(name)
+            return rc
+        return call
+    monkeypatch.setattr(nv, "proto", proto)
+    return names
+
+
+# ------------------------------------------------------------------------------------------------ block tables
+def grown(table, rows, cached, lens, blocks, bs):
+    table, at = [list(r) for r in table], 0
+    for row, c, n in zip(rows, cached, lens):
+        for j in range(-(-max(c, 0) // bs), -(-max(n, 0) // bs)):
+            if 0 <= row < len(table) and j < len(table[0]) and at < len(blocks):
+                table[row][j] = blocks[at]
+            at += 1
+    return table, at
+
+
+def requests(n, cached, new, seed, rows=None):
+    g = torch.Generator().manual_seed(seed)
+    c = torch.randint(0, cached + 1, (n,), generator=g).tolist()
+    k = torch.randint(0, new + 1, (n,), generator=g).tolist()
+    return c, k, torch.randperm(rows or n + 2, generator=g)[:n].tolist()
+
+
+def i32(x, device):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("n,cached,new,bs,spare", [(1, 0, 1, 16, 0), (1, 17, 0, 16, 0), (31, 100, 40, 16, 3), (32, 100, 40, 1, 0), (33, 5, 3, 64, -2), (200, 0, 900, 16, 9),
+                                                   (64, 4000, 1, 16, 0), (1000, 30, 70, 8, 0), (4097, 9, 9, 4, -50)])
+def test_block_tables(device, n, cached, new, bs, spare):
+    """Blocks in the order of the requests; a list that ends too early leaves the rest of the rows as they were, and says how many it lacks."""
+    c, k, rows = requests(n, cached, new, n + new)
+    lens = [a + b for a, b in zip(c, k)]
+    need = sum(-(-b // bs) - -(-a // bs) for a, b in zip(c, lens))
+    blocks = list(range(7, 7 + max(0, need + spare)))
+    width = -(-max(lens + [1]) // bs)
+    wide = i32([[-5] * (width + 3)] * (n + 2), device)
+    table = wide[:, :width]                                           # rows of a wider table
+    before = table.tolist()
+    used = extend_block_tables(table, i32(rows, device), i32(c, device), i32(lens, device), i32(blocks, device), bs)
+    want, at = grown(before, rows, c, lens, blocks, bs)
+    assert table.tolist() == want and used.tolist() == [at] and at == need
+    assert bool((wide[:, width:] == -5).all())
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_block_tables_keep_to_their_bounds(device):
+    """Rows outside the table, rows that are too short, lengths that shrink or are negative: what does not fit is left out, nothing else is touched."""
+    rows, c, lens = [-1, 0, 5, 1, 2, 3], [0, 0, 0, 40, 3, -9], [64, 200, 64, 20, 36, 32]
+    table = i32([[0] * 4 for _ in range(4)], device)
+    used = extend_block_tables(table, i32(rows, device), i32(c, device), i32(lens, device), i32(list(range(100, 140)), device), 16)
+    want, at = grown([[0] * 4 for _ in range(4)], rows, c, lens, list(range(100, 140)), 16)
+    assert table.tolist() == want and used.tolist() == [at]
+    none = i32([], device)
+    assert extend_block_tables(table, none, none, none, none, 16).tolist() == [0] and table.tolist() == want
+
+
+def maps_of(table, rows, cached, new, bs):
+    cu, pos, slot, place, tiles, tile_of, run_tiles = [0], [], [], [], [], [], []
+    for i, (row, c, k) in enumerate(zip(rows, cached, new)):
+        run_tiles.append([len(tiles), -(-k // 64), 0, 0])
+        tile_of += [[i, j, -(-k // 64), len(tiles)] for j in range(-(-k // 64))]
+        tiles += [[cu[-1] + a, min(64, k - a), c + a, row] for a in range(0, k, 64)]
+        for p in range(c, c + k):
+            pos.append(p)
+            slot.append(row)
+            place.append(table[row][p // bs] * bs + p % bs if 0 <= row < len(table) and 0 <= p // bs < len(table[0]) else -1)
+        cu.append(cu[-1] + k)
+    runs = [[cu[i], k, c, row] for i, (row, c, k) in enumerate(zip(rows, cached, new))]
+    return dict(cu=cu, pos=pos, slot=slot, place=place, last=[x - 1 for x in cu[1:]], tiles=tiles, tile_of=tile_of, runs=runs, run_tiles=run_tiles)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("n,cached,new,bs", [(1, 0, 1, 16), (1, 3, 0, 16), (1, 9, 5000, 16), (32, 50, 1, 64), (33, 700, 130, 16), (60, 3000, 2000, 16), (300, 40, 3, 1),
+                                             (2000, 100, 20, 32)])
+def test_step_maps(device, n, cached, new, bs):
+    c, k, rows = requests(n, cached, new, n)
+    width = -(-(cached + new) // bs) + 1
+    g = torch.Generator().manual_seed(1)
+    table = torch.randperm((n + 2) * width, generator=g).view(n + 2, width).to(torch.int32)
+    want = maps_of(table.tolist(), rows, c, k, bs)
+    table = table.to(device)
+    bare = step_maps(table, i32(rows, device), i32(c, device), i32(k, device), bs, sum(k))
+    full = step_maps(table, i32(rows, device), i32(c, device), i32(k, device), bs, sum(k), n_tiles=len(want["tiles"]) + 2)
+    assert bare.tiles is None
+    for m in (bare, full):
+        assert all(getattr(m, f).tolist() == want[f] for f in ("cu", "pos", "slot", "place", "last"))
+    for f in ("tiles", "tile_of"):                                    # two tiles more than there are: of no rows
+        assert getattr(full, f).tolist() == want[f] + [[0, 0, 0, 0]] * 2
+    assert full.runs.tolist() == want["runs"] and full.run_tiles.tolist() == want["run_tiles"]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_step_maps_keep_to_their_bounds(device):
+    """A table that does not list a token's block gives no place for it; tables sized for fewer tokens or tiles than there are are not left."""
+    rows, c, k = [0, 7, 1, -2, 2], [0, 0, 30, 4, -2], [70, 3, 8, 2, 5]
+    table = torch.arange(1, 10, dtype=torch.int32).view(3, 3)
+    want = maps_of(table.tolist(), rows, c, k, 16)
+    m = step_maps(table.to(device), i32(rows, device), i32(c, device), i32(k, device), 16, 40, n_tiles=3)
+    assert m.cu.tolist() == want["cu"] and m.pos.tolist() == want["pos"][:40] and m.place.tolist() == want["place"][:40]
+    assert m.tiles.tolist() == want["tiles"][:3]
+    more = step_maps(table.to(device), i32(rows, device), i32(c, device), i32(k, device), 16, 100)
+    assert more.place[:88].tolist() == want["place"] and len(more.place) == 100
+    assert -1 in want["place"][70:73] and -1 in want["place"][-7:]
+
+
+def test_refusals_of_tables():
+    t, r = torch.zeros(4, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for bad in (dict(table=t.long()), dict(rows=r.long()), dict(cached=r[:1]), dict(lens=r.view(1, 2)), dict(block_size=0), dict(table=t.t()),
+                dict(blocks=torch.zeros(8, dtype=torch.int32)[::2])):
+        args = dict(table=t, rows=r, cached=r, lens=r, blocks=r, block_size=16)
+        args.update(bad)
+        with pytest.raises(ValueError, match="extend_block_tables"):
+            extend_block_tables(**args)
+    for bad in (dict(new=r.float()), dict(total=-1), dict(n_tiles=-1), dict(rows=r[:0], cached=r[:0], new=r[:0])):
+        args = dict(table=t, rows=r, cached=r, new=r, block_size=16, total=0)
+        args.update(bad)
+        with pytest.raises(ValueError, match="step_maps"):
+            step_maps(**args)
+
+
+# ------------------------------------------------------------------------------------------------ rules on logits
+def exact_rules(x, rows):
+    """One row after another in 64 bits. rows: dicts as for LogitState.set_row, or None for a row without rules. Returns values and, for each, a
+    bound: six roundings to 32 bits, each half a step of what stands there, on values that a subtraction may make small."""
+    out, size = [], []
+    for l, r in zip(x.double(), rows):
+        y, s = l.clone(), l.abs()
+        if r is not None:
+            prompt, said = list(r.get("prompt", ())), list(r.get("output", ()))
+            V = y.shape[0]
+            for t in {t for t in prompt + said if 0 <= t < V}:
+                rep = f32(r.get("repetition_penalty", 1.0))
+                y[t] = y[t] * rep if y[t] < 0 else y[t] / rep
+                s[t] = torch.maximum(s[t], y[t].abs())
+            for t in {t for t in said if 0 <= t < V}:
+                f, p = f32(r.get("frequency_penalty", 0.0)), f32(r.get("presence_penalty", 0.0))
+                y[t] -= f * said.count(t) + p
+                s[t] += abs(f) * said.count(t) + abs(p)
+            for t, v in (r.get("logit_bias") or {}).items():
+                y[t] += f32(v)
+                s[t] += abs(f32(v))
+            T = f32(r.get("temperature", 1.0))
+            y, s = y / T, s / T
+            if r.get("allowed") is not None:
+                keep = torch.zeros(V, dtype=torch.bool)
+                keep[torch.tensor(list(r["allowed"]), dtype=torch.long)] = True
+                y[~keep] = -INF
+        out.append(y)
+        size.append(s)
+    return torch.stack(out), torch.stack(size) * 6 * 2.0 ** -24
+
+
+def f32(v):
+    return float(torch.tensor(v, dtype=torch.float32))
+
+
+def some_rules(V, B, seed, max_len):
+    """Rows of all kinds: no rules, each rule alone, all of them, histories with the same token many times and tokens outside the vocabulary."""
+    g = torch.Generator().manual_seed(seed)
+
+    def toks(n):
+        return torch.where(torch.rand(n, generator=g) < 0.5, torch.randint(0, V, (n,), generator=g), torch.randint(0, min(V, 5), (n,), generator=g)).tolist()
+    rows = []
+    for b in range(B):
+        n = int(torch.randint(0, max_len // 2 + 1, (1,), generator=g))
+        r = dict(prompt=toks(n) + [-1, V, 2 ** 31 - 1][:b % 4], output=toks(max_len // 3))
+        kind = b % 7
+        if kind in (1, 6):
+            r["repetition_penalty"] = 1.3 if b % 2 else 0.7
+        if kind in (2, 6):
+            r["presence_penalty"] = 0.75
+        if kind in (3, 6):
+            r["frequency_penalty"] = -0.31
+        if kind in (4, 6):
+            ids = torch.randperm(V, generator=g)[:5].tolist()
+            r["logit_bias"] = dict(zip(ids, [100.0, -100.0, 0.5, -0.25, 3.0]))
+        if kind in (5, 6):
+            r["allowed"] = torch.randperm(V, generator=g)[:V // 3].tolist()
+            r["temperature"] = 0.6
+        rows.append(r)
+    return rows
+
+
+def state_of(rows, V, max_len, device, max_bias=8):
+    st = LogitState(len(rows), V, max_len, max_bias, device)
+    for b, r in enumerate(rows):
+        if r is not None:
+            st.set_row(b, **r)
+    return st
+
+
+def check_rules(got, want, bound):
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got == -INF, want == -INF) and torch.equal(got == INF, want == INF)
+    fin = torch.isfinite(want)
+    over = ((got - want).abs() - bound)[fin]
+    assert over.numel() == 0 or over.max().item() <= 0, over.max().item()
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V,B,dtype", [(1, 3, torch.float32), (31, 8, torch.float32), (33, 7, torch.bfloat16), (4096, 14, torch.float16), (4097, 7, torch.float32),
+                                       (30522, 9, torch.float32), (50257, 7, torch.bfloat16), (151936, 14, torch.float32)])
+def test_rules_on_logits(device, V, B, dtype):
+    """Each rule and all together, at vocabularies that end in a word of the mask, a slice, a vector; two strided batches; greedy is their argmax."""
+    rows = some_rules(V, B, V + B, 60) if V >= 15 else [dict(prompt=[0], repetition_penalty=2.0), dict(output=[0, 0], frequency_penalty=1.0), dict(allowed=[])]
+    B = len(rows)
+    st = state_of(rows, V, 100, device)
+    wide = (torch.randn(B, V + 5, generator=torch.Generator().manual_seed(V)) * 3).to(dtype)
+    for x in (wide[:, :V].contiguous(), wide[:, :V], wide[:, 5:]):
+        want, bound = exact_rules(x, rows)
+        y = process_logits(x.to(device) if x.is_contiguous() else wide.to(device)[:, x.storage_offset():x.storage_offset() + V], st)
+        check_rules(y, want, bound)
+        assert torch.equal(greedy_tokens(x.to(device), st).cpu(), y.argmax(1).cpu())
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_rules_go_by_slot(device):
+    """Batch rows take the rules of any rows of the state, the same one twice too; a slot outside of it has none."""
+    V = 5000
+    rows = some_rules(V, 9, 3, 40)
+    st = state_of(rows, V, 64, device)
+    slot = [8, 2, 2, -1, 9, 0, 6, 2 ** 31 - 1]
+    x = torch.randn(len(slot), V) * 3
+    want, bound = exact_rules(x, [rows[s] if 0 <= s < 9 else None for s in slot])
+    y = process_logits(x.to(device), st, i32(slot, device))
+    check_rules(y, want, bound)
+    assert torch.equal(y[3].cpu(), x[3]) and torch.equal(greedy_tokens(x.to(device), st, i32(slot, device)).cpu(), y.argmax(1).cpu())
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nan_and_infinity_in_logits(device, dtype):
+    """What stands in a masked place is gone, whatever it was; an allowed NaN stays and is the best token, as in torch; equals give the lowest."""
+    V = 9000
+    x = torch.zeros(7, V, dtype=dtype)
+    x[0, 100] = NAN; x[0, 8000] = INF                          # both masked
+    x[1, 7000] = NAN; x[1, 50] = INF                           # both allowed
+    x[2, 5000], x[2, 4000] = 3.0, 3.0                          # equals in different slices
+    x[3] = -INF
+    x[4, 10] = torch.finfo(dtype).min
+    x[5, :] = torch.finfo(dtype).min
+    x[6, 3], x[6, 2] = 0.0, -0.0
+    x[6, 4:] = -1.0
+    x[6, :2] = -1.0
+    rows = [dict(allowed=range(200, 5000))] + [dict(repetition_penalty=1.5, prompt=[1])] + [None] * 5
+    st = state_of(rows, V, 8, device)
+    y = process_logits(x.to(device), st).cpu()
+    assert not torch.isnan(y[0]).any() and (y[0] == -INF).sum() == V - 4800 and (y[0, 200:5000] == 0).all()
+    assert torch.isnan(y[1]).sum() == 1 and y[1, 50] == INF and torch.equal(y[2:], x[2:].float())
+    assert greedy_tokens(x.to(device), st).tolist() == [200, 7000, 4000, 0, 0, 0, 2] == y.argmax(1).tolist()[:4] + [0, 0, 2]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_masked_to_nothing_and_all_allowed(device):
+    V = 12345
+    st = state_of([dict(allowed=[]), dict(allowed=range(V)), dict(allowed=[V - 1]), dict(allowed=[0])], V, 4, device)
+    x = torch.randn(4, V)
+    y = process_logits(x.to(device), st).cpu()
+    assert (y[0] == -INF).all() and torch.equal(y[1], x[1]) and greedy_tokens(x.to(device), st).tolist()[0] == 0
+    assert greedy_tokens(x.to(device), st).tolist()[2:] == [V - 1, 0] and (y[2] == -INF).sum() == V - 1
+    st.set_mask(0, None)
+    assert torch.equal(process_logits(x.to(device), st).cpu()[0], x[0])
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_biases_that_name_a_token_twice(device):
+    """The last entry for a token counts, in any order that the entries are worked on."""
+    V = 600
+    st = LogitState(2, V, 4, 300, device)
+    st.bias_ids[0, :300] = torch.arange(300, dtype=torch.int32, device=device) % 7
+    st.bias_values[0, :300] = torch.arange(300, dtype=torch.float32, device=device)
+    st.bias_length[0] = 300
+    st.bias_ids[1, :3], st.bias_values[1, :3], st.bias_length[1] = i32([V, -1, 5], device), torch.tensor([9.0, 9.0, 2.0], device=device), 9999
+    y = process_logits(torch.zeros(2, V, device=device), st).cpu()
+    assert y[0, :7].tolist() == [float(max(i for i in range(300) if i % 7 == t)) for t in range(7)] and (y[0, 7:] == 0).all()
+    assert y[1, 5] == 2.0 and y[1].count_nonzero() == 1          # ids outside the vocabulary are passed over, as are entries of id 0 and value 0
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_histories_grow(device):
+    """Tokens come behind their rows' histories and count from the next call on; a full row and slots outside the state keep what they have."""
+    V = 200
+    st = LogitState(4, V, 5, 0, device)
+    st.set_row(0, prompt=[7, 7], output=[8], frequency_penalty=1.0)
+    st.set_row(2, prompt=[1, 2, 3, 4], repetition_penalty=2.0)
+    x = torch.ones(4, V, device=device)
+    st.append(torch.tensor([9, 8, 5, 6], device=device), i32([0, 2, 77, -3], device))
+    st.append(torch.tensor([9, 8], device=device), i32([0, 2], device))      # row 2 is full
+    assert st.length.tolist() == [5, 0, 5, 0] and st.tokens[0].tolist() == [7, 7, 8, 9, 9] and st.tokens[2].tolist() == [1, 2, 3, 4, 8]
+    y = process_logits(x, st).cpu()
+    assert y[0, [7, 8, 9, 10]].tolist() == [1.0, 0.0, -1.0, 1.0] and y[2, [1, 4, 8, 9]].tolist() == [0.5, 0.5, 0.5, 1.0]
+    st.append(torch.tensor([3, 3, 3, 3], device=device))
+    assert st.length.tolist() == [5, 1, 5, 1]
+    st.set_row(0)
+    assert torch.equal(process_logits(x, st).cpu()[0], torch.ones(V))
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_logits_in_place(device):
+    V = 6400
+    rows = some_rules(V, 7, 5, 30)
+    st = state_of(rows, V, 64, device)
+    x = torch.randn(7, V)
+    y = x.clone().to(device)
+    assert process_logits(y, st, out=y) is y
+    check_rules(y, *exact_rules(x, rows))
+    assert process_logits(x[:0].to(device), st).shape == (0, V) and greedy_tokens(x[:0].to(device), st).shape == (0,)
+
+
+def test_refusals_of_rules():
+    st = LogitState(4, 100, 8, 2)
+    x = torch.zeros(4, 100)
+    for bad in (dict(logits=x[0]), dict(logits=x[:, :99]), dict(logits=torch.zeros(5, 100)), dict(slot=torch.zeros(4)), dict(slot=torch.zeros(3, dtype=torch.int32)),
+                dict(logits=torch.zeros(100, 4).t())):
+        for fn in (process_logits, greedy_tokens):
+            with pytest.raises(ValueError, match=fn.__name__):
+                fn(**{**dict(logits=x, state=st), **bad})
+    for out in (x.double(), x[:2], torch.zeros(100, 4).t()):
+        with pytest.raises(ValueError, match="process_logits"):
+            process_logits(x, st, out=out)
+    for bad in (dict(row=4), dict(row=-1), dict(row=0, prompt=range(9)), dict(row=0, logit_bias={1: 1.0, 2: 1.0, 3: 1.0}), dict(row=0, logit_bias={100: 1.0}),
+                dict(row=0, allowed=[-1]), dict(row=0, repetition_penalty=0.0), dict(row=0, temperature=0.0), dict(row=0, temperature=NAN)):
+        with pytest.raises(ValueError, match="LogitState"):
+            st.set_row(**bad)
+    for bad in (dict(rows=0), dict(vocab=0), dict(max_len=0), dict(max_len=(1 << 20) + 1), dict(max_bias=2048), dict(max_bias=-1)):
+        with pytest.raises(ValueError, match="LogitState"):
+            LogitState(**{**dict(rows=2, vocab=9, max_len=4), **bad})
+    for ids, slot in ((torch.zeros(2), None), (torch.zeros(5, dtype=torch.int64), None), (torch.zeros(2, dtype=torch.int64), torch.zeros(2))):
+        with pytest.raises(ValueError, match="append"):
+            st.append(ids, slot)
+
+
+# ------------------------------------------------------------------------------------------------ attention over shared keys
+def batch_of(groups, alone, own, H, G, D, BS, dtype, seed, copies=False, odd=None):
+    """A decode batch on the CPU: groups (tokens, shared keys), then sequences by themselves, ``own`` keys (cyclic) behind the shared ones. Whole pages of
+    the shared part are the same page for all; the page that it ends in is each sequence's copy. All that no sequence holds is NaN."""
+    g = torch.Generator().manual_seed(seed)
+    members, plan, first = [], [], 0
+    for n, shared in groups:
+        plan.append((first, n, shared))
+        members += [(first, shared)] * n
+        first += n
+    members += [(None, 0)] * alone
+    keys = [s + k for (_, s), k in zip(members, itertools.cycle(own))]
+    total = sum(-(-k // BS) for k in keys) + 3
+    pages = (torch.randperm(total, generator=g) + 1).tolist()
+    ck, cv = (torch.full((total + 1, G, BS, D), NAN, dtype=dtype) for _ in range(2))
+    rows = []
+    for i, ((first, s), n) in enumerate(zip(members, keys)):
+        lead = rows[first][:s // BS] if first is not None and first != i and not copies else []
+        rows.append(lead + [pages.pop() for _ in range(-(-n // BS) - len(lead))])
+        own_k, own_v = (torch.randn(n, G, D, generator=g).to(dtype) for _ in range(2))
+        if first is not None and first != i:
+            k0, v0 = keys_of(ck, rows[first], s), keys_of(cv, rows[first], s)
+            own_k[:s], own_v[:s] = k0, v0
+        at = torch.arange(n)
+        blk = torch.tensor(rows[-1])[at // BS]
+        ck[blk, :, at % BS], cv[blk, :, at % BS] = own_k, own_v
+    width = max(map(len, rows)) + 1
+    table = torch.zeros(len(rows), width + 2, dtype=torch.int32)
+    for i, r in enumerate(rows):
+        table[i, :len(r)] = torch.tensor(r, dtype=torch.int32)
+    T = len(rows)
+    q = torch.randn(T, (H + 2 * G) * D, generator=g).to(dtype)
+    return dict(q=q, ck=ck, cv=cv, table=table, pos=torch.tensor([n - 1 for n in keys], dtype=torch.int32), slot=torch.arange(T, dtype=torch.int32), plan=plan,
+                H=H, G=G, D=D, BS=BS)
+
+
+def keys_of(pool, row, n):
+    at = torch.arange(n)
+    return pool[torch.tensor(row)[at // pool.shape[2]], :, at % pool.shape[2]]
+
+
+def exact_attention(b, scale, sinks=None):
+    """Token by token in 64 bits, with a bound for a result of 16 bits. The result and every weight are rounded once, each by half a step; a score is a sum of D
+    products in 32 bits, off by at most D 2^-24 of the sum of their sizes, and a weight by that much twice (it and the sum); 2^-20 more for exponentials
+    (2^-22 each, of the weight and of two joins) and for sums in 32 bits of a few hundred blocks. Numbers below the type's smallest normal one
+    are a fixed step apart (fp16: 2^-24 below 2^-14), so a rounding there is off by half of that, ``tiny``: of the result, and of a weight, which is
+    rounded as a part of the largest one of its range, so by no more than ``tiny`` of the row's largest weight."""
+    H, G, D, BS = b["H"], b["G"], b["D"], b["BS"]
+    half = torch.finfo(b["q"].dtype).eps / 2
+    tiny = torch.finfo(b["q"].dtype).smallest_normal * half
+    out, bound = [], []
+    for t in range(b["q"].shape[0]):
+        n, row = int(b["pos"][t]) + 1, int(b["slot"][t])
+        if n <= 0 or not 0 <= row < b["table"].shape[0]:
+            out.append(torch.zeros(H * D, dtype=torch.float64)); bound.append(torch.zeros(H * D, dtype=torch.float64))
+            continue
+        k, v = (keys_of(b[c], b["table"][row].tolist(), n).double().repeat_interleave(H // G, 1) for c in ("ck", "cv"))
+        q = b["q"][t, :H * D].double().view(H, D)
+        s = torch.einsum("hd,nhd->hn", q, k) * scale
+        err = D * 2.0 ** -24 * scale * torch.einsum("hd,nhd->hn", q.abs(), k.abs()).amax(1)
+        full = s if sinks is None else torch.cat([s, sinks.double()[:, None]], 1)
+        w = full.softmax(1)[:, :n]
+        o, size = torch.einsum("hn,nhd->hd", w, v), torch.einsum("hn,nhd->hd", w, v.abs())
+        out.append(o.reshape(-1))
+        bound.append((half * o.abs() + size * (half + 2 * err[:, None] + 2.0 ** -20) * (1 + half)
+                      + tiny * (1 + w.amax(1)[:, None] * v.abs().sum(0))).reshape(-1))
+    return torch.stack(out), torch.stack(bound)
+
+
+def call(b, device, groups=None, scale=None, sinks=None, **kw):
+    on = {k: v.to(device) for k, v in b.items() if isinstance(v, torch.Tensor)}
+    plan = make_prefix_groups(b["plan"] if groups is None else groups, b["q"].shape[0], device)
+    return prefix_attention(on["q"], on["ck"], on["cv"], on["table"][:, :-2], on["pos"], on["slot"], plan, b["H"], b["G"], b["D"],
+                            b["D"] ** -0.5 if scale is None else scale, sinks=None if sinks is None else sinks.to(device), max_pos=int(b["pos"].max()), **kw)
+
+
+def close(got, b, scale=None, sinks=None):
+    want, bound = exact_attention(b, b["D"] ** -0.5 if scale is None else scale, sinks)
+    got = got.double().cpu()
+    assert got.shape == want.shape and torch.isfinite(got).all()
+    over = ((got - want).abs() - bound).max().item()
+    assert over <= 0, over
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,G,D", [(16, 4, 128), (40, 8, 128), (8, 8, 128), (16, 1, 128), (12, 2, 64), (4, 4, 64), (24, 2, 64), (8, 4, 96), (6, 2, 80), (3, 1, 16), (5, 5, 112)])
+@pytest.mark.parametrize("BS", [1, 8, 16, 64, 256])
+def test_shared_keys(entries, H, G, D, BS):
+    """Groups of 1 to 40 tokens whose shared part ends in and beside pages, tiles and ranges; sequences by themselves between and behind them."""
+    b = batch_of([(3, 64), (1, 1), (40, 257), (2, 63), (17, 640)], 3, [1, 2, 65, 31, 200, 129], H, G, D, BS, torch.bfloat16, H + D + BS)
+    close(call(b, "cuda"), b)
+    assert "b200_prefix_attn" in entries and "b200_paged_attn" not in entries
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 96])
+@pytest.mark.parametrize("groups,own", [([(130, 2000)], [1, 7]), ([(2, 5000)], [3000, 1]), ([(33, 128), (33, 129), (33, 127)], [64]), ([(1, 4096)], [1]), ([(300, 1)], [5])])
+def test_few_and_many_rows(entries, dtype, D, groups, own):
+    """Work cut into many ranges and into none, tiles that are full and all but empty; copies of the shared keys instead of the same pages."""
+    b = batch_of(groups, 0, own, 8, 2, D, 16, dtype, D, copies=len(own) == 1 and groups[0][0] < 40)
+    close(call(b, "cuda"), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 80])
+def test_sinks_and_scales(D):
+    b = batch_of([(5, 300), (9, 77)], 2, [1, 40], 8, 2, D, 16, torch.float16, 3)
+    sinks = torch.tensor([-INF, -50.0, 0.0, 3.0, 40.0, -1.0, 1.0, 10.0])
+    close(call(b, "cuda", sinks=sinks), b, sinks=sinks)
+    for scale in (1e-3, 0.5):
+        close(call(b, "cuda", scale=scale), b, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 64, 48])
+def test_tokens_that_do_not_see_all_of_the_shared_part(D):
+    """A token before the last shared key, one at it, one without any key, slots outside the table: each as by itself; no row of the batch touches
+    another's."""
+    b = batch_of([(8, 200)], 2, [10], 8, 2, D, 16, torch.bfloat16, 5)
+    b["pos"][[1, 2, 3, 4, 9]] = torch.tensor([0, 198, 199, -1, -1], dtype=torch.int32)
+    b["slot"][[6, 8]] = torch.tensor([-1, 10], dtype=torch.int32)
+    got = call(b, "cuda")
+    close(got, b)
+    assert (got[[4, 6, 8, 9]] == 0).all()
+    sinks = torch.zeros(8)
+    got = call(b, "cuda", sinks=sinks)
+    close(got, b, sinks=sinks)
+    assert (got[[4, 6, 8, 9]] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 96])
+def test_values_of_other_sequences_stay_theirs(D):
+    """A NaN or infinity in one sequence's own keys and values reaches that sequence alone; one in the shared part all of the group."""
+    b = batch_of([(6, 100), (3, 50)], 1, [30, 7], 8, 2, D, 64, torch.bfloat16, 8)
+    clean = call(b, "cuda")
+    for pool, bad in (("ck", NAN), ("cv", INF), ("cv", NAN)):
+        c = {**b, "ck": b["ck"].clone(), "cv": b["cv"].clone()}
+        row, p = 2, 110
+        c[pool][int(b["table"][row, p // 64]), :, p % 64] = bad
+        got = call(c, "cuda")
+        assert torch.equal(got[[0, 1, 3, 4, 5, 6, 7, 8, 9]], clean[[0, 1, 3, 4, 5, 6, 7, 8, 9]]) and not torch.isfinite(got[2]).all()
+        c = {**b, "ck": b["ck"].clone(), "cv": b["cv"].clone()}
+        c[pool][int(b["table"][0, 0]), :, 5] = bad
+        got = call(c, "cuda")
+        assert torch.equal(got[6:], clean[6:]) and not torch.isfinite(got[:6]).all(1).any()
+
+
+@pytest.mark.gpu
+def test_pages_outside_the_pool_are_not_read():
+    """A table entry that names no page of the pool: its keys are not read, the other rows have their results."""
+    b = batch_of([(6, 128)], 2, [70], 8, 2, 128, 64, torch.bfloat16, 9)
+    clean = call(b, "cuda")
+    for page in (-1, b["ck"].shape[0], 2 ** 31 - 1, -2 ** 31):
+        c = {**b, "table": b["table"].clone()}
+        c["table"][3, 2] = page
+        got = call(c, "cuda")
+        others = [0, 1, 2, 4, 5, 6, 7]
+        assert torch.equal(got[others], clean[others]) and not torch.equal(got[3], clean[3])
+        c["table"][0, 0] = page
+        assert torch.equal(call(c, "cuda")[6:], clean[6:])
+
+
+@pytest.mark.gpu
+def test_a_pool_that_32_bits_do_not_address():
+    """Pages behind 2^31 elements of a pool."""
+    n_pages = 2 ** 31 // (8 * 64 * 128) + 70
+    if torch.cuda.mem_get_info()[0] < 3 * n_pages * 8 * 64 * 128 * 2:
+        pytest.skip("not enough memory")
+    b = batch_of([(5, 200)], 1, [100], 8, 8, 128, 64, torch.bfloat16, 11)
+    used = b["ck"].shape[0]
+    on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
+    ck, cv = (torch.empty(n_pages, 8, 64, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ck[-used:], cv[-used:] = on["ck"], on["cv"]
+    out = prefix_attention(on["q"], ck, cv, on["table"] + (n_pages - used), on["pos"], on["slot"], make_prefix_groups(b["plan"], 6, "cuda"), 8, 8, 128, 128 ** -0.5)
+    assert torch.equal(out, call(b, "cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 48])
+def test_captured_and_on_another_stream(D):
+    """Two captured calls and an eager one between their replays, on a stream of their own; the plan rewritten on the device within its bounds, and beyond
+    them."""
+    b = batch_of([(20, 300)], 4, [33], 16, 4, D, 16, torch.bfloat16, 13)
+    on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
+    plan = make_prefix_groups([(0, 20, 300)], 24, "cuda")
+    args = (on["q"], on["ck"], on["cv"], on["table"], on["pos"], on["slot"], plan, 16, 4, D, D ** -0.5)
+    want = prefix_attention(*args)
+    close(want, b)
+    stream, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = prefix_attention(*args)
+        graphs.append((graph, out))
+    for rewrite in ([0, 20, 300, 0], [0, 5, 17, 0], [2, 18, 300, 0], [0, 20, 10 ** 6, 0], [-3, 20, 300, 0], [0, 99, 300, 0], [0, 20, 0, 0], [0, 20, -5, 0]):
+        plan.groups.copy_(torch.tensor([rewrite]))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for graph, out in graphs:
+                out.fill_(NAN)
+                graph.replay()
+            eager = prefix_attention(*args)
+        stream.synchronize()
+        close(eager, b)
+        assert torch.equal(graphs[0][1], eager) and torch.equal(graphs[1][1], eager)
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_other_caches_go_through_paged_attention(entries, device):
+    """32-bit caches, head sizes and steps without groups that the kernels are not for."""
+    for dtype, D, groups in ((torch.float32, 64, None), (torch.bfloat16, 24, None), (torch.bfloat16, 160, None), (torch.bfloat16, 64, [])):
+        b = batch_of([(4, 40)], 1, [3, 20], 4, 2, D, 16, dtype, 1)
+        close(call(b, device, groups=groups), b)
+    assert "b200_prefix_attn" not in entries
+
+
+def test_refusals_of_groups():
+    for groups in ([(0, 3, 5), (2, 2, 5)], [(-1, 2, 5)], [(3, 2, 5)], [(0, -1, 5)], [(0, 1, -5)]):
+        with pytest.raises(ValueError, match="make_prefix_groups"):
+            make_prefix_groups(groups, 4, "cpu")
+    p = make_prefix_groups([(0, 2, 7), (2, 0, 9), (2, 1, 0), (3, 1, 4)], 4, "cpu")
+    assert p.of.tolist() == [0, 0, -1, 1] and p.groups.tolist() == [[0, 2, 7, 0], [3, 1, 4, 0]] and (p.n_groups, p.longest, p.max_shared) == (2, 2, 7)
+    assert make_prefix_groups([], 3, "cpu").n_groups == 0
+
+
+@pytest.mark.gpu
+def test_refusals_of_attention():
+    b = batch_of([(4, 40)], 1, [3], 4, 2, 64, 16, torch.bfloat16, 1)
+    for change in (dict(ck=b["ck"].float()), dict(cv=b["cv"][:, :1]), dict(q=b["q"][:, :100]), dict(table=b["table"].long()), dict(pos=b["pos"].long()),
+                   dict(slot=b["slot"][:2]), dict(ck=b["ck"].transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises(ValueError, match="prefix_attention"):
+            call({**b, **change}, "cuda")
+    on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
+    args = [on["q"], on["ck"], on["cv"], on["table"], on["pos"], on["slot"], make_prefix_groups(b["plan"], 5, "cuda"), 4, 2, 64, 0.125]
+    for i, bad in ((0, torch.empty(5, 516, dtype=torch.bfloat16, device="cuda")[:, 1:513]), (7, 3), (6, make_prefix_groups(b["plan"], 4, "cuda")),
+                   (6, make_prefix_groups(b["plan"], 5, "cpu"))):
+        with pytest.raises(ValueError, match="prefix_attention"):
+            prefix_attention(*args[:i], bad, *args[i + 1:])
+    with pytest.raises(ValueError, match="sinks"):
+        prefix_attention(*args, sinks=torch.zeros(4))
