@@ -230,17 +230,29 @@ prefix_shared_mma_kernel(const PrefixParams p) {
 // ------------------------------------------------------------------------------------------------------------------
 // own keys, and both parts together
 // ------------------------------------------------------------------------------------------------------------------
-// A CTA owns one token and up to HB query heads of one KV head. A lane is (key, 16-byte chunk): the CP lanes of a key read its row and the
-// same row of the values with one load each; every lane keeps (max, sum, acc) for the keys it has seen.
-template <typename T, int HB>
-__global__ void __launch_bounds__(128)
-prefix_own_kernel(const PrefixParams p, int CP, int CPR) {
-  extern __shared__ float sm[];                       // [4 warps][HB][D + 2]
-  const int D = p.D, rep = p.H / p.G, passes = ceil_div(rep, HB);
-  const int t = blockIdx.x, g = blockIdx.y / passes, h0 = g * rep + (blockIdx.y % passes) * HB, nh = min(HB, g * rep + rep - h0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int KPI = 32 / CP, kk = lane / CP, c = lane % CP;
-  const bool live = c < CPR;
+// A CTA owns one token and up to eight query heads of one KV head; its warps take blocks of 16 keys in turn. Keys and values go from memory
+// straight into the registers that mma.sync reads, 16 bytes to a load, whole rows side by side: the keys are the first operand of S^T = K Q^T and
+// the values, turned in pairs of rows, that of O^T = V^T P^T, the heads the eight columns of both. For that the dimensions are taken in
+// the order in which they lie in the lanes, the same for Q and K, and undone where O is written; P changes sides by movmatrix. Against a lane per
+// key and chunk with FMAs, which kept two keys in flight per lane and spent 140 instructions on each pair of keys: 64 tokens with 300 own keys each, 32 / 8
+// heads of 128 (78 MB).
+constexpr int kPxOwn = 16;
+
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T, int KC>                         // KC: head size in chunks of 32, rounded up
+__global__ void __launch_bounds__(128, 3)
+prefix_own_kernel(const PrefixParams p) {
+  constexpr int VC = (KC + 1) / 2, LD = 64 * VC + 4;
+  __shared__ __align__(16) float so[4][8][LD];
+  __shared__ float sml[4][8][2], sw[8][36], sinv[8];  // of each head: weights of the four warps and of up to 32 ranges
+  const int D = p.D, rep = p.H / p.G, passes = ceil_div(rep, 8);
+  const int t = blockIdx.x, kvh = blockIdx.y / passes, h0 = kvh * rep + (blockIdx.y % passes) * 8, nh = min(8, kvh * rep + rep - h0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int slot = p.slot[t];
   const bool listed = (unsigned)slot < (unsigned)p.table_rows;
   const int* trow = p.table + (listed ? slot : 0) * p.table_stride;
@@ -252,108 +264,146 @@ prefix_own_kernel(const PrefixParams p, int CP, int CPR) {
     const PrefixGroup grp = prefix_group(p, j);
     if (t >= grp.first && t < grp.first + grp.tokens && k_hi >= grp.shared) { k_lo = grp.shared; used = ranges_used(p, grp.shared); }
   }
-  const T* q = reinterpret_cast<const T*>(p.q);
   const T* ck = reinterpret_cast<const T*>(p.ck);
   const T* cv = reinterpret_cast<const T*>(p.cv);
-  float qv[HB][8], acc[HB][8], m[HB], l[HB];
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 qf[KC];
 #pragma unroll
-  for (int hh = 0; hh < HB; ++hh) {
-    m[hh] = -INFINITY;
-    l[hh] = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      acc[hh][e] = 0.f;
-      qv[hh][e] = (live && hh < nh) ? to_f32<T>(q[(long long)t * p.q_stride + (long long)(h0 + hh) * D + c * 8 + e]) * p.scale_log2 : 0.f;
-    }
+  for (int i = 0; i < KC; ++i) {
+    const int d = i * 32 + c * 8;
+    qf[i] = g < nh && d < D ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (long long)t * p.q_stride + (long long)(h0 + g) * D + d) : zero;
   }
-  const int bs_mask = (1 << p.bs_log2) - 1, stride = 4 * KPI;
-  constexpr int U = HB >= 4 ? 2 : 4;                  // keys in flight per lane
-  for (int kb = k_lo; kb < k_hi; kb += stride * U) {
-    uint4 kr[U], vr[U];
-    bool valid[U];
+  const int bs_mask = (1 << p.bs_log2) - 1;
+  const bool one_page = p.bs_log2 >= 4;               // a block lies in one page
+  auto page_at = [&](int kb) { return kb < k_hi ? page_of(p, trow, kb) : -1; };
+  // row of key k in the pools, -1: not read
+  auto row_of = [&](int k, int page) -> long long {
+    if (k < k_lo || k >= k_hi) return -1;
+    if (!one_page) page = page_of(p, trow, k);
+    return page < 0 ? -1 : (((long long)page * p.G + kvh) << p.bs_log2) + (k & bs_mask);
+  };
+  uint4 kr[KC][2], vr[VC][4];
+  auto load_k = [&](int kb, int page) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k0 = kb + u * stride + warp * KPI + kk;
-      valid[u] = k0 < k_hi;
-      kr[u] = vr[u] = make_uint4(0, 0, 0, 0);
-      if (valid[u] && live) {
-        const int page = page_of(p, trow, k0);
-        if (page >= 0) {
-          const long long off = ((((long long)page * p.G + g) << p.bs_log2) + (k0 & bs_mask)) * D + c * 8;
-          kr[u] = *reinterpret_cast<const uint4*>(ck + off);
-          vr[u] = *reinterpret_cast<const uint4*>(cv + off);
-        }
+    for (int r = 0; r < 2; ++r) {
+      const long long row = row_of(kb + g + 8 * r, page);
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int d = i * 32 + c * 8;
+        kr[i][r] = row >= 0 && d < D ? *reinterpret_cast<const uint4*>(ck + row * D + d) : zero;
       }
     }
+  };
+  auto load_v = [&](int kb, int page) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (kb + u * stride >= k_hi) break;             // uniform over the CTA: no lane has a key in this or a later slot
-      float kf[8], vf[8];
-      const T* kp = reinterpret_cast<const T*>(&kr[u]);
-      const T* vp = reinterpret_cast<const T*>(&vr[u]);
+    for (int r = 0; r < 4; ++r) {
+      const long long row = row_of(kb + 2 * c + (r & 1) + 8 * (r >> 1), page);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { kf[e] = to_f32<T>(kp[e]); vf[e] = to_f32<T>(vp[e]); }
-#pragma unroll
-      for (int hh = 0; hh < HB; ++hh) {
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(qv[hh][e], kf[e], s);
-        for (int o = CP >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (valid[u]) {
-          const float mn = fmaxf(m[hh], s), e0 = mn == -INFINITY ? 0.f : mn;
-          const float r = ex2_approx(m[hh] - e0), pj = ex2_approx(s - e0);
-          m[hh] = mn;
-          l[hh] = l[hh] * r + pj;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[hh][e] = fmaf(pj, vf[e], acc[hh][e] * r);
-        }
+      for (int i = 0; i < VC; ++i) {
+        const int d = i * 64 + g * 8;
+        vr[i][r] = row >= 0 && d < D ? *reinterpret_cast<const uint4*>(cv + row * D + d) : zero;
       }
     }
+  };
+  float o[4 * VC][4];
+#pragma unroll
+  for (int i = 0; i < 4 * VC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;     // heads 2 c and 2 c + 1
+  const float sl2 = p.scale_log2;
+  int kb = (k_lo & ~(kPxOwn - 1)) + warp * kPxOwn;    // blocks start at multiples of 16: with larger pages each lies in one
+  int page = page_at(kb), next = page_at(kb + 4 * kPxOwn);
+  if (kb < k_hi) { load_k(kb, page); load_v(kb, page); }
+  for (; kb < k_hi; kb += 4 * kPxOwn) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const uint32_t a0[4] = {kr[i][0].x, kr[i][1].x, kr[i][0].y, kr[i][1].y}, a1[4] = {kr[i][0].z, kr[i][1].z, kr[i][0].w, kr[i][1].w};
+      mma_16816<T>(s, a0, qf[i].x, qf[i].y);
+      mma_16816<T>(s, a1, qf[i].z, qf[i].w);
+    }
+    const int after = page_at(kb + 8 * kPxOwn);
+    if (kb + 4 * kPxOwn < k_hi) load_k(kb + 4 * kPxOwn, next);   // under way while this block is worked on; V's as soon as its registers are read
+    if (kb < k_lo || kb + kPxOwn > k_hi) {
+      if (kb + g < k_lo || kb + g >= k_hi) s[0] = s[1] = -INFINITY;
+      if (kb + g + 8 < k_lo || kb + g + 8 >= k_hi) s[2] = s[3] = -INFINITY;
+    }
+    float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
+#pragma unroll
+    for (int x = 4; x <= 16; x <<= 1) {
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, x));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, x));
+    }
+    const float n0 = fmaxf(m0, x0 * sl2), n1 = fmaxf(m1, x1 * sl2);
+    const float e0 = n0 == -INFINITY ? 0.f : n0, e1 = n1 == -INFINITY ? 0.f : n1;
+    const float r0 = ex2_approx(m0 - e0), r1 = ex2_approx(m1 - e1);
+    m0 = n0; m1 = n1;
+    const float p0 = ex2_approx(fmaf(s[0], sl2, -e0)), p1 = ex2_approx(fmaf(s[1], sl2, -e1));
+    const float p2 = ex2_approx(fmaf(s[2], sl2, -e0)), p3 = ex2_approx(fmaf(s[3], sl2, -e1));
+    l0 = fmaf(l0, r0, p0 + p2);
+    l1 = fmaf(l1, r1, p1 + p3);
+    const uint32_t b0 = turn8x8(pack_pair<T>(p0, p1)), b1 = turn8x8(pack_pair<T>(p2, p3));
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+      const uint32_t* v[4] = {&vr[i][0].x, &vr[i][1].x, &vr[i][2].x, &vr[i][3].x};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t a[4] = {__byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632),
+                               __byte_perm(v[2][w], v[3][w], 0x5410), __byte_perm(v[2][w], v[3][w], 0x7632)};
+        float (&oo)[4] = o[4 * i + w];
+        oo[0] *= r0; oo[1] *= r1; oo[2] *= r0; oo[3] *= r1;
+        mma_16816<T>(oo, a, b0, b1);
+      }
+    }
+    if (kb + 4 * kPxOwn < k_hi) load_v(kb + 4 * kPxOwn, next);
+    next = after;
   }
-  // the key groups of the warp, then the warps, the ranges of the shared keys and the sink
+  // ---- the warps' parts, the ranges of the shared keys and the sink ----
 #pragma unroll
-  for (int hh = 0; hh < HB; ++hh) {
-    for (int o = CP; o < 32; o <<= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m[hh], o), l2 = __shfl_xor_sync(0xffffffffu, l[hh], o);
-      const float mn = fmaxf(m[hh], m2), e0 = mn == -INFINITY ? 0.f : mn;
-      const float w1 = ex2_approx(m[hh] - e0), w2 = ex2_approx(m2 - e0);
-      l[hh] = l[hh] * w1 + l2 * w2;
+  for (int x = 4; x <= 16; x <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+  }
+  if (g == 0) {
+    sml[warp][2 * c][0] = m0; sml[warp][2 * c][1] = l0;
+    sml[warp][2 * c + 1][0] = m1; sml[warp][2 * c + 1][1] = l1;
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[hh][e] = acc[hh][e] * w1 + __shfl_xor_sync(0xffffffffu, acc[hh][e], o) * w2;
-      m[hh] = mn;
-    }
-    if (kk == 0 && live) {
-      float* w = sm + (warp * HB + hh) * (D + 2);
-      if (c == 0) { w[0] = m[hh]; w[1] = l[hh]; }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[2 + c * 8 + e] = acc[hh][e];
-    }
+  for (int i = 0; i < 4 * VC; ++i) {
+    const int d = (i >> 2) * 64 + g * 8 + (i & 3) * 2;
+    *reinterpret_cast<float2*>(&so[warp][2 * c][d]) = make_float2(o[i][0], o[i][2]);
+    *reinterpret_cast<float2*>(&so[warp][2 * c + 1][d]) = make_float2(o[i][1], o[i][3]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nh * D; i += 128) {
-    const int hh = i / D, d = i % D, h = h0 + hh;
-    const long long at = ((long long)t * p.H + h) * p.nsplit;
-    const float sink = p.sinks ? p.sinks[h] * kPxLog2e : -INFINITY;
-    float mt = sink;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, sm[(w * HB + hh) * (D + 2)]);
-    for (int s = 0; s < used; ++s) mt = fmaxf(mt, p.part_ml[2 * (at + s)]);
-    const float e0 = mt == -INFINITY ? 0.f : mt;
-    float lt = ex2_approx(sink - e0), ot = 0.f;
+  for (int hh = warp; hh < nh; hh += 4) {             // a lane for each range; the first four take a warp's part each as well
+    const long long at = ((long long)t * p.H + h0 + hh) * p.nsplit + lane;
+    const float2 ml = lane < used ? *reinterpret_cast<const float2*>(p.part_ml + 2 * at) : make_float2(-INFINITY, 0.f);
+    const float wm = lane < 4 ? sml[lane][hh][0] : -INFINITY, wl = lane < 4 ? sml[lane][hh][1] : 0.f;
+    const float sink = p.sinks ? p.sinks[h0 + hh] * kPxLog2e : -INFINITY;
+    const float top = fmaxf(warp_max(fmaxf(ml.x, wm)), sink), e = top == -INFINITY ? 0.f : top;
+    const float w1 = ex2_approx(wm - e), w2 = ex2_approx(ml.x - e);
+    const float total = warp_sum(wl * w1 + ml.y * w2) + ex2_approx(sink - e);
+    if (lane < 4) sw[hh][lane] = w1;
+    if (lane < used) sw[hh][4 + lane] = w2;
+    if (lane == 0) sinv[hh] = total == 0.f ? 0.f : 1.f / total;      // a row that sees no key is zero
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nh * (D / 2); i += 128) {
+    const int hh = i / (D / 2), d = i % (D / 2) * 2;
+    float2 a = make_float2(0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float* ws = sm + (w * HB + hh) * (D + 2);
-      const float e = ex2_approx(ws[0] - e0);
-      lt += ws[1] * e;
-      ot += ws[2 + d] * e;
+      const float2 x = *reinterpret_cast<const float2*>(&so[w][hh][d]);
+      a.x = fmaf(x.x, sw[hh][w], a.x);
+      a.y = fmaf(x.y, sw[hh][w], a.y);
     }
-    for (int s = 0; s < used; ++s) {
-      const float e = ex2_approx(p.part_ml[2 * (at + s)] - e0);
-      lt += p.part_ml[2 * (at + s) + 1] * e;
-      ot += p.part_o[(at + s) * D + d] * e;
+    const float2* part = reinterpret_cast<const float2*>(p.part_o + ((long long)t * p.H + h0 + hh) * p.nsplit * D + d);
+#pragma unroll 4
+    for (int r = 0; r < used; ++r) {
+      const float2 x = part[(long long)r * (D / 2)];
+      a.x = fmaf(x.x, sw[hh][4 + r], a.x);
+      a.y = fmaf(x.y, sw[hh][4 + r], a.y);
     }
-    // a row that sees no key is zero
-    reinterpret_cast<T*>(p.out)[((long long)t * p.H + h) * D + d] = from_f32<T>(lt == 0.f ? 0.f : ot / lt);
+    *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + ((long long)t * p.H + h0 + hh) * D + d) = pack_pair<T>(a.x * sinv[hh], a.y * sinv[hh]);
   }
 }
 
@@ -379,15 +429,13 @@ static int prefix_attn(const PrefixParams& p, cudaStream_t st) {
 #undef SHARED
     if (rc) return rc;
   }
-  const int CPR = p.D / 8;
-  int CP = 1;
-  while (CP < CPR) CP <<= 1;
-  const int HB = rep >= 4 ? 4 : rep >= 2 ? 2 : 1;
-  const dim3 grid(p.T, p.G * ceil_div(rep, HB));
-  const size_t smem = (size_t)4 * HB * (p.D + 2) * sizeof(float);
-  if (HB == 4) prefix_own_kernel<T, 4><<<grid, 128, smem, st>>>(p, CP, CPR);
-  else if (HB == 2) prefix_own_kernel<T, 2><<<grid, 128, smem, st>>>(p, CP, CPR);
-  else prefix_own_kernel<T, 1><<<grid, 128, smem, st>>>(p, CP, CPR);
+  const dim3 grid(p.T, p.G * ceil_div(rep, 8));
+  switch ((p.D + 31) / 32) {
+    case 1: prefix_own_kernel<T, 1><<<grid, 128, 0, st>>>(p); break;
+    case 2: prefix_own_kernel<T, 2><<<grid, 128, 0, st>>>(p); break;
+    case 3: prefix_own_kernel<T, 3><<<grid, 128, 0, st>>>(p); break;
+    default: prefix_own_kernel<T, 4><<<grid, 128, 0, st>>>(p); break;
+  }
   B200_LAUNCH_CHECK();
   return 0;
 }
