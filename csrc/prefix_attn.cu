@@ -17,48 +17,13 @@
 // 17 MB of shared keys and 78 MB of own ones (15 us at 6.5 TB/s), 4.6 GFLOP (3 us); read once a sequence they were 1.15 GB.
 #include "common.cuh"
 #include "mma_sync.cuh"
+#include "prefix_attn.cuh"
+#include <type_traits>
 #include "../include/b200_ops.h"
 
 namespace b200 {
 
-constexpr int kPxRows = 64, kPxKeys = 64;
-constexpr float kPxLog2e = 1.4426950408889634f;
-
-struct PrefixParams {
-  const void *q, *ck, *cv;
-  long long q_stride;
-  const int *pos, *slot, *table;
-  long long table_stride;
-  int table_rows, width, n_pages;               // block table [table_rows, width], pages in the pools
-  const int *groups, *of;                       // [n_groups, 4] = (first token, tokens, shared keys, -), [T] group of a token or -1
-  int n_groups, longest;                        // tokens of a group that the shared part takes; those behind them see to all keys by themselves
-  const float* sinks;
-  void* out;
-  float *part_o, *part_ml;                      // [T, H, nsplit, D], [T, H, nsplit, 2] (maximum in powers of two, sum)
-  int T, H, G, D, bs_log2, nsplit;
-  float scale_log2;
-};
-
-// A group as the kernels use it; nothing in it reaches outside the batch or the table
-struct PrefixGroup { int first, tokens, shared; };
-__device__ __forceinline__ PrefixGroup prefix_group(const PrefixParams& p, int j) {
-  PrefixGroup g;
-  g.first = p.groups[4 * j]; g.tokens = p.groups[4 * j + 1]; g.shared = p.groups[4 * j + 2];
-  if (g.first < 0 || g.first >= p.T) g.tokens = g.first = 0;
-  g.tokens = min(max(g.tokens, 0), min(p.T - g.first, p.longest));
-  g.shared = (int)min((long long)max(g.shared, 0), (long long)p.width << p.bs_log2);
-  return g;
-}
-// ranges of the shared keys, in blocks of kPxKeys: how many each takes, and how many there are
-__device__ __forceinline__ int range_blocks(const PrefixParams& p, int shared) { return (ceil_div(shared, kPxKeys) + p.nsplit - 1) / p.nsplit; }
-__device__ __forceinline__ int ranges_used(const PrefixParams& p, int shared) {
-  return shared > 0 ? ceil_div(ceil_div(shared, kPxKeys), range_blocks(p, shared)) : 0;
-}
-// the page of key k in a table row, or -1: pages outside the pool are not read
-__device__ __forceinline__ int page_of(const PrefixParams& p, const int* row, int k) {
-  const int page = row[k >> p.bs_log2];
-  return (unsigned)page < (unsigned)p.n_pages ? page : -1;
-}
+constexpr int kPxRows = 64;
 
 template <typename T> __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -419,13 +384,14 @@ static int launch_shared_mma(const PrefixParams& p, dim3 grid, cudaStream_t st) 
 }
 
 template <typename T>
-static int prefix_attn(const PrefixParams& p, cudaStream_t st) {
+static int prefix_attn(const PrefixParams& p, bool tc, cudaStream_t st) {
   const int rep = p.H / p.G;
   if (p.n_groups > 0 && p.longest > 0) {
-    const dim3 grid(p.nsplit, p.G * ceil_div(p.longest * rep, kPxRows), p.n_groups);
     int rc = B200_ERR_UNSUPPORTED;
+    const dim3 grid(p.nsplit, p.G * ceil_div(p.longest * rep, kPxRows), p.n_groups);
 #define SHARED(DK) case DK: rc = launch_shared_mma<T, DK>(p, grid, st); break
-    switch (p.D / 16) { SHARED(1); SHARED(2); SHARED(3); SHARED(4); SHARED(5); SHARED(6); SHARED(7); SHARED(8); }
+    if (tc) rc = prefix_shared_tc(p, std::is_same<T, __nv_bfloat16>::value ? B200_DT_BF16 : B200_DT_FP16, st);
+    else switch (p.D / 16) { SHARED(1); SHARED(2); SHARED(3); SHARED(4); SHARED(5); SHARED(6); SHARED(7); SHARED(8); }
 #undef SHARED
     if (rc) return rc;
   }
@@ -443,23 +409,28 @@ static int prefix_attn(const PrefixParams& p, cudaStream_t st) {
 }  // namespace b200
 using namespace b200;
 
-// Ranges that the shared keys of a call are cut into: enough CTAs for three on every SM, of no fewer than 256 keys each
-B200_API int b200_prefix_attn_splits(int n_groups, int longest, int max_shared, int H, int G) {
-  if (n_groups < 1 || longest < 1 || max_shared < 1 || H < 1 || G < 1 || H % G) return 1;
-  const long long items = (long long)n_groups * G * ceil_div64((int64_t)longest * (H / G), kPxRows);
-  long long n = ceil_div64(3 * kNumSMs, items);
+// How the shared keys of a call are worked on: the number of ranges (1 .. 32), plus kPxTc where tcgen05 does it.
+constexpr int kPxTc = 256;
+B200_API int b200_prefix_attn_plan(int n_groups, int longest, int max_shared, int H, int G, int D, int block_size, int n_pages) {
+  if (n_groups < 1 || longest < 1 || max_shared < 1 || H < 1 || G < 1 || H % G || block_size < 1 || n_pages < 0) return 1;
+  const int rep = H / G, tokens = prefix_tc_tokens(H, G, D, block_size);
+  const bool tc = tokens > 0 && (long long)longest * rep > 32 && (long long)n_pages * G * block_size < 0x7fffff00LL;
+  const long long items = (long long)n_groups * G * (tc ? ceil_div(longest, tokens) : ceil_div64((int64_t)longest * rep, kPxRows));
+  long long n = ceil_div64(tc ? 2 * kNumSMs : 3 * kNumSMs, items);
   const long long most = ceil_div64(max_shared, 256);
   if (n > most) n = most;
-  return (int)(n > 32 ? 32 : n);
+  return (int)(n > 32 ? 32 : n) + (tc ? kPxTc : 0);
 }
 
 B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const void* cv, int n_pages, const int* pos, const int* slot,
                               const int* table, long long table_stride, int table_rows, int width, const int* groups, const int* of, int n_groups,
-                              int longest, const float* sinks, void* out, float* part, int nsplit, int T, int H, int G, int D, int block_size,
+                              int longest, const float* sinks, void* out, float* part, int plan, int T, int H, int G, int D, int block_size,
                               float scale, int dtype, void* stream) {
   if (T <= 0) return 0;
   if ((dtype != B200_DT_BF16 && dtype != B200_DT_FP16) || D % 16 || D < 16 || D > 128 || !(scale > 0.f)) return B200_ERR_UNSUPPORTED;
-  if (H < 1 || G < 1 || H % G || n_pages < 0 || table_rows < 1 || width < 1 || n_groups < 0 || nsplit < 1 || block_size < 1) return B200_ERR_BAD_SHAPE;
+  const bool tc = plan >= kPxTc;
+  const int nsplit = tc ? plan - kPxTc : plan;
+  if (H < 1 || G < 1 || H % G || n_pages < 0 || table_rows < 1 || width < 1 || n_groups < 0 || nsplit < 1 || nsplit > 32 || block_size < 1) return B200_ERR_BAD_SHAPE;
   if (n_groups > 65535 || (long long)G * ceil_div64((int64_t)(longest < 1 ? 1 : longest) * (H / G), kPxRows) > 65535 || H > 65535) return B200_ERR_TOO_LARGE;
   if (q_stride % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(ck) | reinterpret_cast<uintptr_t>(cv) |
                         reinterpret_cast<uintptr_t>(part)) & 15)) return B200_ERR_BAD_ALIGN;
@@ -467,10 +438,11 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
   while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
   if ((1 << p.bs_log2) != block_size) return B200_ERR_UNSUPPORTED;
   if (n_groups > 0 && longest > 0 && !part) return B200_ERR_BAD_SHAPE;
+  if (tc && (prefix_tc_tokens(H, G, D, block_size) < 1 || n_pages < 1 || (long long)n_pages * G * block_size >= 0x7fffff00LL)) return B200_ERR_UNSUPPORTED;
   p.q = q; p.ck = ck; p.cv = cv; p.q_stride = q_stride; p.pos = pos; p.slot = slot; p.table = table; p.table_stride = table_stride;
   p.table_rows = table_rows; p.width = width; p.n_pages = n_pages; p.groups = groups; p.of = of; p.n_groups = n_groups;
   p.longest = longest; p.sinks = sinks; p.out = out; p.T = T; p.H = H; p.G = G; p.D = D; p.nsplit = nsplit;
   p.part_o = part; p.part_ml = part ? part + (long long)T * H * nsplit * D : nullptr;
   p.scale_log2 = scale * kPxLog2e;
-  return dtype == B200_DT_BF16 ? prefix_attn<__nv_bfloat16>(p, (cudaStream_t)stream) : prefix_attn<__half>(p, (cudaStream_t)stream);
+  return dtype == B200_DT_BF16 ? prefix_attn<__nv_bfloat16>(p, tc, (cudaStream_t)stream) : prefix_attn<__half>(p, tc, (cudaStream_t)stream);
 }

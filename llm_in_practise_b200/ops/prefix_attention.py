@@ -61,12 +61,13 @@ def _int32(name, t, device, shape):
 
 def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
                      groups: Optional[PrefixGroups], n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
-                     sinks: Optional[torch.Tensor] = None, max_pos: int = 0) -> torch.Tensor:
+                     sinks: Optional[torch.Tensor] = None, max_pos: int = 0, plan: int = 0) -> torch.Tensor:
     """Context [T, H * D] of token t over keys ``0 .. pos[t]`` of cache row ``slot[t]``, as ``paged_attention`` gives it (same arguments; no
     window), with the shared keys of ``groups`` read once. Tokens of a group whose position is before its last shared key, and tokens of no
     group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. Caches of 16 bits with head sizes that
     are multiples of 16 up to 128, pages of a power of two and a positive scale; others go through ``paged_attention``, as does a step without
-    groups. Captured into a graph, each call keeps a workspace of its own."""
+    groups. Captured into a graph, each call keeps a workspace of its own. ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it
+    (include/b200_ops.h); 0: chosen by the sizes."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
     BS = cache_k.shape[2]
     if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or q.dtype not in (torch.bfloat16, torch.float16) or D % 16 or D > 128
@@ -88,12 +89,13 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     _int32("the groups' token table", groups.of, dev, (T,))
     _int32("the groups' table", groups.groups, dev, (groups.n_groups, 4))
     out = torch.empty(T, H * D, dtype=q.dtype, device=dev)
-    nsplit = nv.proto("b200_prefix_attn_splits", [i32] * 5)(groups.n_groups, groups.longest, groups.max_shared, H, G)
-    part = torch.empty(T * H * nsplit * (D + 2), dtype=torch.float32, device=dev)
+    if not plan:
+        plan = nv.proto("b200_prefix_attn_plan", [i32] * 8)(groups.n_groups, groups.longest, groups.max_shared, H, G, D, BS, cache_k.shape[0])
+    part = torch.empty(T * H * (plan % 256) * (D + 2), dtype=torch.float32, device=dev)
     fn = nv.proto("b200_prefix_attn", [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32,
                                        i32, vp])
     nv.check(nv.call_on(dev, fn, nv.ptr(q), q.stride(0), nv.ptr(cache_k), nv.ptr(cache_v), cache_k.shape[0], nv.ptr(pos), nv.ptr(slot), nv.ptr(table),
                         table.stride(0), table.shape[0], table.shape[1], nv.ptr(groups.groups), nv.ptr(groups.of), groups.n_groups, groups.longest,
-                        nv.ptr(sinks), nv.ptr(out), nv.ptr(part), nsplit, T, H, G, D, BS, scale, nv.dtype_code(q.dtype)), "prefix_attn")
+                        nv.ptr(sinks), nv.ptr(out), nv.ptr(part), plan, T, H, G, D, BS, scale, nv.dtype_code(q.dtype)), "prefix_attn")
     nv.count_launch(2)
     return out

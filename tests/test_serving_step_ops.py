@@ -466,6 +466,19 @@ def test_few_and_many_rows(entries, dtype, D, groups, own):
     close(call(b, "cuda"), b)
 
 
+TC = 256                      # plan: the tcgen05 kernel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,G,D,BS", [(8, 2, 128, 8), (5, 1, 64, 16), (40, 8, 128, 16), (24, 2, 64, 64), (16, 16, 128, 128), (128, 1, 64, 32)])
+def test_every_cut_of_the_shared_keys(dtype, H, G, D, BS):
+    """Both kernels of the shared keys, from one range to more than there are keys for; each result by the same bound."""
+    b = batch_of([(3, 64), (1, 1), (70, 257), (9, 1030)], 2, [1, 65, 31], H, G, D, BS, dtype, H + D)
+    for plan in (1, 2, 5, 32, TC + 1, TC + 2, TC + 3, TC + 7, TC + 32):
+        close(call(b, "cuda", plan=plan), b)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [128, 80])
 def test_sinks_and_scales(D):
@@ -498,16 +511,21 @@ def test_tokens_that_do_not_see_all_of_the_shared_part(D):
 def test_values_of_other_sequences_stay_theirs(D):
     """A NaN or infinity in one sequence's own keys and values reaches that sequence alone; one in the shared part all of the group."""
     b = batch_of([(6, 100), (3, 50)], 1, [30, 7], 8, 2, D, 64, torch.bfloat16, 8)
-    clean = call(b, "cuda")
+    for plan in (0, 2, TC + 2) if D == 128 else (0, 2):
+        nan_and_infinity(b, plan)
+
+
+def nan_and_infinity(b, plan):
+    clean = call(b, "cuda", plan=plan)
     for pool, bad in (("ck", NAN), ("cv", INF), ("cv", NAN)):
         c = {**b, "ck": b["ck"].clone(), "cv": b["cv"].clone()}
         row, p = 2, 110
         c[pool][int(b["table"][row, p // 64]), :, p % 64] = bad
-        got = call(c, "cuda")
+        got = call(c, "cuda", plan=plan)
         assert torch.equal(got[[0, 1, 3, 4, 5, 6, 7, 8, 9]], clean[[0, 1, 3, 4, 5, 6, 7, 8, 9]]) and not torch.isfinite(got[2]).all()
         c = {**b, "ck": b["ck"].clone(), "cv": b["cv"].clone()}
         c[pool][int(b["table"][0, 0]), :, 5] = bad
-        got = call(c, "cuda")
+        got = call(c, "cuda", plan=plan)
         assert torch.equal(got[6:], clean[6:]) and not torch.isfinite(got[:6]).all(1).any()
 
 
@@ -515,15 +533,15 @@ def test_values_of_other_sequences_stay_theirs(D):
 def test_pages_outside_the_pool_are_not_read():
     """A table entry that names no page of the pool: its keys are not read, the other rows have their results."""
     b = batch_of([(6, 128)], 2, [70], 8, 2, 128, 64, torch.bfloat16, 9)
-    clean = call(b, "cuda")
-    for page in (-1, b["ck"].shape[0], 2 ** 31 - 1, -2 ** 31):
+    for plan, page in itertools.product((2, TC + 2), (-1, b["ck"].shape[0], 2 ** 31 - 1, -2 ** 31)):
+        clean = call(b, "cuda", plan=plan)
         c = {**b, "table": b["table"].clone()}
         c["table"][3, 2] = page
-        got = call(c, "cuda")
+        got = call(c, "cuda", plan=plan)
         others = [0, 1, 2, 4, 5, 6, 7]
         assert torch.equal(got[others], clean[others]) and not torch.equal(got[3], clean[3])
         c["table"][0, 0] = page
-        assert torch.equal(call(c, "cuda")[6:], clean[6:])
+        assert torch.equal(call(c, "cuda", plan=plan)[6:], clean[6:])
 
 
 @pytest.mark.gpu
