@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "mma_sync.cuh"
 #include "prefix_attn.cuh"
+#include "tma_host.h"
 #include <type_traits>
 #include "../include/b200_ops.h"
 
@@ -51,6 +52,7 @@ prefix_shared_mma_kernel(const PrefixParams p) {
   T* sk = reinterpret_cast<T*>(smem_raw);             // [2][64][LD]
   T* sv = sk + 2 * kPxKeys * LD;                      // [2][64][LD]
   T* sq = sk + kPxKeys * LD;                          // Q is staged in K buffer 1 until its fragments are read
+  pdl_launch_dependents();
   const PrefixGroup grp = prefix_group(p, blockIdx.z);
   const int rep = p.H / p.G, tiles = gridDim.y / p.G;
   const int g = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * kPxRows, nrows = min(kPxRows, grp.tokens * rep - row0);
@@ -195,13 +197,10 @@ prefix_shared_mma_kernel(const PrefixParams p) {
 // ------------------------------------------------------------------------------------------------------------------
 // own keys, and both parts together
 // ------------------------------------------------------------------------------------------------------------------
-// A CTA owns one token and up to eight query heads of one KV head; its warps take blocks of 16 keys in turn. Keys and values go from memory
-// straight into the registers that mma.sync reads, 16 bytes to a load, whole rows side by side: the keys are the first operand of S^T = K Q^T and
-// the values, turned in pairs of rows, that of O^T = V^T P^T, the heads the eight columns of both. For that the dimensions are taken in
-// the order in which they lie in the lanes, the same for Q and K, and undone where O is written; P changes sides by movmatrix. Against a lane per
-// key and chunk with FMAs, which kept two keys in flight per lane and spent 140 instructions on each pair of keys: 64 tokens with 300 own keys each, 32 / 8
-// heads of 128 (78 MB).
-constexpr int kPxOwn = 16;
+// A CTA owns one token and up to eight query heads of one KV head; its warps take blocks of 16 keys in turn, each with a ring of its own that its
+// first lane refills by TMA (one box per page and 64 dimensions, 128-byte swizzle). On mma.sync: S^T = K Q^T, the keys the first operand and the
+// heads the eight columns, then O^T = V^T P^T with V turned by ldmatrix; P changes sides by movmatrix.
+constexpr int kPxOwn = 16, kPxWarps = 4, kPxStages = 2;
 
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   uint32_t y;
@@ -209,88 +208,104 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   return y;
 }
 
-template <typename T, int KC>                         // KC: head size in chunks of 32, rounded up
-__global__ void __launch_bounds__(128, 3)
-prefix_own_kernel(const PrefixParams p) {
-  constexpr int VC = (KC + 1) / 2, LD = 64 * VC + 4;
-  __shared__ __align__(16) float so[4][8][LD];
-  __shared__ float sml[4][8][2], sw[8][36], sinv[8];  // of each head: weights of the four warps and of up to 32 ranges
-  const int D = p.D, rep = p.H / p.G, passes = ceil_div(rep, 8);
+template <int DK> struct OwnSmem {
+  static constexpr int kHalves = (DK + 3) / 4, LD = 64 * kHalves + 4;       // LD: floats of a row of O
+  static constexpr int kBlock = kHalves * 2048, kStage = 2 * kBlock;        // 16 keys, 16 keys and their values
+  static constexpr int kRing = kPxStages * kStage, kBytes = kPxWarps * kRing + 8 * kPxWarps * kPxStages;
+  static_assert(8 * LD * 4 <= kRing, "a warp's O is joined where its ring was");
+};
+
+template <typename T, int DK>                         // head size = 16 * DK
+__global__ void __launch_bounds__(32 * kPxWarps)
+prefix_own_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PrefixParams p) {
+  using L = OwnSmem<DK>;
+  constexpr int D = 16 * DK, LD = L::LD;
+  extern __shared__ __align__(1024) uint8_t smem_own[];
+  __shared__ float sml[kPxWarps][8][2], sw[8][kPxWarps + 32], sinv[8];  // of each head: weights of the warps and of up to 32 ranges
+  const int rep = p.H / p.G, passes = ceil_div(rep, 8);
   const int t = blockIdx.x, kvh = blockIdx.y / passes, h0 = kvh * rep + (blockIdx.y % passes) * 8, nh = min(8, kvh * rep + rep - h0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int slot = p.slot[t];
+  const uint32_t ring = smem_u32(smem_own) + warp * L::kRing, bars = smem_u32(smem_own) + kPxWarps * L::kRing + warp * kPxStages * 8;
+  if (lane == 0) {
+    for (int s = 0; s < kPxStages; ++s) mbar_init(bars + 8 * s, 1);
+    fence_mbar_init();
+  }
+  const int slot = p.slot[t], j = p.of[t], pos = p.pos[t];
   const bool listed = (unsigned)slot < (unsigned)p.table_rows;
   const int* trow = p.table + (listed ? slot : 0) * p.table_stride;
-  const int k_hi = listed ? (int)min((long long)p.pos[t] + 1, (long long)p.width << p.bs_log2) : 0;
+  const int k_hi = listed ? (int)min((long long)pos + 1, (long long)p.width << p.bs_log2) : 0;
   // the shared part holds for this token if it is one of the group's and sees all of it
-  const int j = p.of[t];
   int k_lo = 0, used = 0;
   if ((unsigned)j < (unsigned)p.n_groups) {
     const PrefixGroup grp = prefix_group(p, j);
     if (t >= grp.first && t < grp.first + grp.tokens && k_hi >= grp.shared) { k_lo = grp.shared; used = ranges_used(p, grp.shared); }
   }
-  const T* ck = reinterpret_cast<const T*>(p.ck);
-  const T* cv = reinterpret_cast<const T*>(p.cv);
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  uint4 qf[KC];
+  // this warp's blocks: n of them, the i-th at key_at(i). They start at multiples of 16, so that each lies in one page (pages of 8: in two)
+  const int base = (k_lo & ~(kPxOwn - 1)) + warp * kPxOwn, n = base < k_hi ? (k_hi - base + kPxWarps * kPxOwn - 1) / (kPxWarps * kPxOwn) : 0;
+  auto key_at = [&](int i) { return base + i * kPxWarps * kPxOwn; };
+  const int psl = min(p.bs_log2, 4), pieces = kPxOwn >> psl, pool_rows = (p.n_pages * p.G) << p.bs_log2;
+  // Lane x holds the pool row of piece x % pieces of block (first of a set) + x / pieces. A piece behind the token's keys, or on a page outside the
+  // pools, is asked for behind the pools' last row: zeros
+  const int set = 32 / pieces;
+  auto rows_of = [&](int first) {
+    const int i = first + lane / pieces, k = key_at(i) + (lane % pieces << psl);
+    const int page = i < n && k < k_hi ? page_of(p, trow, k) : -1;
+    return page >= 0 ? ((page * p.G + kvh) << p.bs_log2) + (k & ((1 << p.bs_log2) - 1)) : pool_rows;
+  };
+  int rows = rows_of(0), have = 0;                    // for blocks have .. have + set - 1
+  auto fetch = [&](int i) {                           // whole warp
+    if (i >= n) return;
+    if (i - have >= set) { have += set; rows = rows_of(have); }
+    const int s = i % kPxStages;
+    const uint32_t bar = bars + 8 * s, at = ring + s * L::kStage;
+    if (lane == 0) mbar_arrive_expect_tx(bar, L::kStage);
+    __syncwarp();
+    for (int x = 0; x < pieces; ++x) {
+      const int row = __shfl_sync(0xffffffffu, rows, (i - have) * pieces + x);
+      if (lane < L::kHalves) tma_load_2d(at + lane * 2048 + (x << psl) * 128, &tk, bar, lane * 64, row);
+      else if (lane < 2 * L::kHalves) tma_load_2d(at + lane * 2048 + (x << psl) * 128, &tv, bar, (lane - L::kHalves) * 64, row);
+    }
+  };
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < KC; ++i) {
-    const int d = i * 32 + c * 8;
-    qf[i] = g < nh && d < D ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (long long)t * p.q_stride + (long long)(h0 + g) * D + d) : zero;
+  for (int i = 0; i < kPxStages; ++i) fetch(i);
+  // Q^T as the second operand of S^T
+  uint32_t qf[DK][2];
+  {
+    const T* q = reinterpret_cast<const T*>(p.q) + (long long)t * p.q_stride + (long long)(h0 + min(g, nh - 1)) * D + 2 * c;
+#pragma unroll
+    for (int i = 0; i < DK; ++i) {
+      qf[i][0] = g < nh ? *reinterpret_cast<const uint32_t*>(q + 16 * i) : 0u;
+      qf[i][1] = g < nh ? *reinterpret_cast<const uint32_t*>(q + 16 * i + 8) : 0u;
+    }
   }
-  const int bs_mask = (1 << p.bs_log2) - 1;
-  const bool one_page = p.bs_log2 >= 4;               // a block lies in one page
-  auto page_at = [&](int kb) { return kb < k_hi ? page_of(p, trow, kb) : -1; };
-  // row of key k in the pools, -1: not read
-  auto row_of = [&](int k, int page) -> long long {
-    if (k < k_lo || k >= k_hi) return -1;
-    if (!one_page) page = page_of(p, trow, k);
-    return page < 0 ? -1 : (((long long)page * p.G + kvh) << p.bs_log2) + (k & bs_mask);
-  };
-  uint4 kr[KC][2], vr[VC][4];
-  auto load_k = [&](int kb, int page) {
+  float o[DK][4];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const long long row = row_of(kb + g + 8 * r, page);
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int d = i * 32 + c * 8;
-        kr[i][r] = row >= 0 && d < D ? *reinterpret_cast<const uint4*>(ck + row * D + d) : zero;
-      }
-    }
-  };
-  auto load_v = [&](int kb, int page) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long long row = row_of(kb + 2 * c + (r & 1) + 8 * (r >> 1), page);
-#pragma unroll
-      for (int i = 0; i < VC; ++i) {
-        const int d = i * 64 + g * 8;
-        vr[i][r] = row >= 0 && d < D ? *reinterpret_cast<const uint4*>(cv + row * D + d) : zero;
-      }
-    }
-  };
-  float o[4 * VC][4];
-#pragma unroll
-  for (int i = 0; i < 4 * VC; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < DK; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;     // heads 2 c and 2 c + 1
   const float sl2 = p.scale_log2;
-  int kb = (k_lo & ~(kPxOwn - 1)) + warp * kPxOwn;    // blocks start at multiples of 16: with larger pages each lies in one
-  int page = page_at(kb), next = page_at(kb + 4 * kPxOwn);
-  if (kb < k_hi) { load_k(kb, page); load_v(kb, page); }
-  for (; kb < k_hi; kb += 4 * kPxOwn) {
+  // where a lane's rows of ldmatrix are: keys by rows of 16 and chunk, values (turned) by groups of 8 keys and chunk
+  const int kr = lane & 15, kc = lane >> 4, vr = (lane & 7) + 8 * (lane >> 4), vc = (lane >> 3) & 1;
+  for (int i = 0; i < n; ++i) {
+    const int st = i % kPxStages, kb = key_at(i);
+    const uint32_t ka = ring + st * L::kStage + kr * 128, va = ring + st * L::kStage + L::kBlock + vr * 128;
+    mbar_wait_warp(bars + 8 * st, (uint32_t)(i / kPxStages) & 1u);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      const uint32_t a0[4] = {kr[i][0].x, kr[i][1].x, kr[i][0].y, kr[i][1].y}, a1[4] = {kr[i][0].z, kr[i][1].z, kr[i][0].w, kr[i][1].w};
-      mma_16816<T>(s, a0, qf[i].x, qf[i].y);
-      mma_16816<T>(s, a1, qf[i].z, qf[i].w);
+    for (int x = 0; x < DK; ++x) {
+      uint32_t a[4];
+      ldsm_x4(ka + (x >> 2) * 2048 + ((((x & 3) * 2 + kc) ^ (kr & 7)) << 4), a[0], a[1], a[2], a[3]);
+      mma_16816<T>(s, a, qf[x][0], qf[x][1]);
     }
-    const int after = page_at(kb + 8 * kPxOwn);
-    if (kb + 4 * kPxOwn < k_hi) load_k(kb + 4 * kPxOwn, next);   // under way while this block is worked on; V's as soon as its registers are read
-    if (kb < k_lo || kb + kPxOwn > k_hi) {
-      if (kb + g < k_lo || kb + g >= k_hi) s[0] = s[1] = -INFINITY;
-      if (kb + g + 8 < k_lo || kb + g + 8 >= k_hi) s[2] = s[3] = -INFINITY;
+    uint32_t keep0 = ~0u, keep1 = ~0u;                // pairs of values of this lane's keys
+    const bool ragged = kb < k_lo || kb + kPxOwn > k_hi;
+    if (ragged) {
+      auto out = [&](int k) { return kb + k < k_lo || kb + k >= k_hi; };
+      if (out(g)) s[0] = s[1] = -INFINITY;
+      if (out(g + 8)) s[2] = s[3] = -INFINITY;
+      // values of keys that are not the token's own become zeros: a weight of zero does not undo a NaN
+      keep0 = (out(2 * c) ? 0u : 0xffffu) | (out(2 * c + 1) ? 0u : 0xffff0000u);
+      keep1 = (out(2 * c + 8) ? 0u : 0xffffu) | (out(2 * c + 9) ? 0u : 0xffff0000u);
     }
     float x0 = fmaxf(s[0], s[2]), x1 = fmaxf(s[1], s[3]);
 #pragma unroll
@@ -308,19 +323,15 @@ prefix_own_kernel(const PrefixParams p) {
     l1 = fmaf(l1, r1, p1 + p3);
     const uint32_t b0 = turn8x8(pack_pair<T>(p0, p1)), b1 = turn8x8(pack_pair<T>(p2, p3));
 #pragma unroll
-    for (int i = 0; i < VC; ++i) {
-      const uint32_t* v[4] = {&vr[i][0].x, &vr[i][1].x, &vr[i][2].x, &vr[i][3].x};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t a[4] = {__byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632),
-                               __byte_perm(v[2][w], v[3][w], 0x5410), __byte_perm(v[2][w], v[3][w], 0x7632)};
-        float (&oo)[4] = o[4 * i + w];
-        oo[0] *= r0; oo[1] *= r1; oo[2] *= r0; oo[3] *= r1;
-        mma_16816<T>(oo, a, b0, b1);
-      }
+    for (int x = 0; x < DK; ++x) {
+      uint32_t a[4];
+      ldsm_x4_trans(va + (x >> 2) * 2048 + ((((x & 3) * 2 + vc) ^ (vr & 7)) << 4), a[0], a[1], a[2], a[3]);
+      if (ragged) { a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1; }
+      o[x][0] *= r0; o[x][1] *= r1; o[x][2] *= r0; o[x][3] *= r1;
+      mma_16816<T>(o[x], a, b0, b1);
     }
-    if (kb + 4 * kPxOwn < k_hi) load_v(kb + 4 * kPxOwn, next);
-    next = after;
+    __syncwarp();                                     // every lane has read the stage
+    fetch(i + kPxStages);
   }
   // ---- the warps' parts, the ranges of the shared keys and the sink ----
 #pragma unroll
@@ -332,43 +343,41 @@ prefix_own_kernel(const PrefixParams p) {
     sml[warp][2 * c][0] = m0; sml[warp][2 * c][1] = l0;
     sml[warp][2 * c + 1][0] = m1; sml[warp][2 * c + 1][1] = l1;
   }
+  float* so = reinterpret_cast<float*>(smem_own + warp * L::kRing);
 #pragma unroll
-  for (int i = 0; i < 4 * VC; ++i) {
-    const int d = (i >> 2) * 64 + g * 8 + (i & 3) * 2;
-    *reinterpret_cast<float2*>(&so[warp][2 * c][d]) = make_float2(o[i][0], o[i][2]);
-    *reinterpret_cast<float2*>(&so[warp][2 * c + 1][d]) = make_float2(o[i][1], o[i][3]);
+  for (int i = 0; i < DK; ++i) {
+    so[2 * c * LD + 16 * i + g] = o[i][0];
+    so[(2 * c + 1) * LD + 16 * i + g] = o[i][1];
+    so[2 * c * LD + 16 * i + g + 8] = o[i][2];
+    so[(2 * c + 1) * LD + 16 * i + g + 8] = o[i][3];
   }
+  pdl_wait();
   __syncthreads();
-  for (int hh = warp; hh < nh; hh += 4) {             // a lane for each range; the first four take a warp's part each as well
+  for (int hh = warp; hh < nh; hh += kPxWarps) {      // a lane for each range; the first lanes take a warp's part each as well
     const long long at = ((long long)t * p.H + h0 + hh) * p.nsplit + lane;
     const float2 ml = lane < used ? *reinterpret_cast<const float2*>(p.part_ml + 2 * at) : make_float2(-INFINITY, 0.f);
-    const float wm = lane < 4 ? sml[lane][hh][0] : -INFINITY, wl = lane < 4 ? sml[lane][hh][1] : 0.f;
+    const float wm = lane < kPxWarps ? sml[lane][hh][0] : -INFINITY, wl = lane < kPxWarps ? sml[lane][hh][1] : 0.f;
     const float sink = p.sinks ? p.sinks[h0 + hh] * kPxLog2e : -INFINITY;
     const float top = fmaxf(warp_max(fmaxf(ml.x, wm)), sink), e = top == -INFINITY ? 0.f : top;
     const float w1 = ex2_approx(wm - e), w2 = ex2_approx(ml.x - e);
     const float total = warp_sum(wl * w1 + ml.y * w2) + ex2_approx(sink - e);
-    if (lane < 4) sw[hh][lane] = w1;
-    if (lane < used) sw[hh][4 + lane] = w2;
+    if (lane < kPxWarps) sw[hh][lane] = w1;
+    if (lane < used) sw[hh][kPxWarps + lane] = w2;
     if (lane == 0) sinv[hh] = total == 0.f ? 0.f : 1.f / total;      // a row that sees no key is zero
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nh * (D / 2); i += 128) {
-    const int hh = i / (D / 2), d = i % (D / 2) * 2;
-    float2 a = make_float2(0.f, 0.f);
+  for (int i = threadIdx.x; i < nh * (D / 4); i += 32 * kPxWarps) {
+    const int hh = i / (D / 4), d = i % (D / 4) * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto take = [&](const float4 x, float w) { a.x = fmaf(x.x, w, a.x); a.y = fmaf(x.y, w, a.y); a.z = fmaf(x.z, w, a.z); a.w = fmaf(x.w, w, a.w); };
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float2 x = *reinterpret_cast<const float2*>(&so[w][hh][d]);
-      a.x = fmaf(x.x, sw[hh][w], a.x);
-      a.y = fmaf(x.y, sw[hh][w], a.y);
-    }
-    const float2* part = reinterpret_cast<const float2*>(p.part_o + ((long long)t * p.H + h0 + hh) * p.nsplit * D + d);
-#pragma unroll 4
-    for (int r = 0; r < used; ++r) {
-      const float2 x = part[(long long)r * (D / 2)];
-      a.x = fmaf(x.x, sw[hh][4 + r], a.x);
-      a.y = fmaf(x.y, sw[hh][4 + r], a.y);
-    }
-    *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + ((long long)t * p.H + h0 + hh) * D + d) = pack_pair<T>(a.x * sinv[hh], a.y * sinv[hh]);
+    for (int w = 0; w < kPxWarps; ++w) take(*reinterpret_cast<const float4*>(smem_own + w * L::kRing + (hh * LD + d) * 4), sw[hh][w]);
+    const float4* part = reinterpret_cast<const float4*>(p.part_o + ((long long)t * p.H + h0 + hh) * p.nsplit * D + d);
+#pragma unroll 8
+    for (int r = 0; r < used; ++r) take(part[(long long)r * (D / 4)], sw[hh][kPxWarps + r]);
+    const float inv = sinv[hh];
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + ((long long)t * p.H + h0 + hh) * D + d) =
+        make_uint2(pack_pair<T>(a.x * inv, a.y * inv), pack_pair<T>(a.z * inv, a.w * inv));
   }
 }
 
@@ -383,6 +392,29 @@ static int launch_shared_mma(const PrefixParams& p, dim3 grid, cudaStream_t st) 
   return 0;
 }
 
+// The second kernel starts while the first one ends: it waits for it (griddepcontrol.wait) before it takes up the ranges, its own keys, queries and
+// tables are of launches that were complete when the first one began.
+template <typename T, int DK>
+static int launch_own(const PrefixParams& p, dim3 grid, cudaStream_t st) {
+  // rows of the pools, boxes of 64 dimensions (those behind the head size come as zeros) and up to 16 keys
+  const uint64_t dims[2] = {16 * DK, (uint64_t)((p.n_pages * p.G) << p.bs_log2)}, str[1] = {32 * DK};
+  const uint32_t box[2] = {64, (uint32_t)(p.bs_log2 < 4 ? 1 << p.bs_log2 : kPxOwn)};
+  CUtensorMap tk, tv;
+  if (int rc = make_tensor_map(&tk, p.ck, 2, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = make_tensor_map(&tv, p.cv, 2, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  auto kern = prefix_own_kernel<T, DK>;
+  // per call: the attribute belongs to the current device, and a process may use several
+  B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnSmem<DK>::kBytes));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid; cfg.blockDim = dim3(32 * kPxWarps); cfg.dynamicSmemBytes = OwnSmem<DK>::kBytes; cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.n_groups > 0 && p.longest > 0 ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, p);
+}
+
 template <typename T>
 static int prefix_attn(const PrefixParams& p, bool tc, cudaStream_t st) {
   const int rep = p.H / p.G;
@@ -395,31 +427,42 @@ static int prefix_attn(const PrefixParams& p, bool tc, cudaStream_t st) {
 #undef SHARED
     if (rc) return rc;
   }
-  const dim3 grid(p.T, p.G * ceil_div(rep, 8));
-  switch ((p.D + 31) / 32) {
-    case 1: prefix_own_kernel<T, 1><<<grid, 128, 0, st>>>(p); break;
-    case 2: prefix_own_kernel<T, 2><<<grid, 128, 0, st>>>(p); break;
-    case 3: prefix_own_kernel<T, 3><<<grid, 128, 0, st>>>(p); break;
-    default: prefix_own_kernel<T, 4><<<grid, 128, 0, st>>>(p); break;
-  }
-  B200_LAUNCH_CHECK();
-  return 0;
+#define OWN(DK) case DK: return launch_own<T, DK>(p, dim3(p.T, p.G * ceil_div(rep, 8)), st)
+  switch (p.D / 16) { OWN(1); OWN(2); OWN(3); OWN(4); OWN(5); OWN(6); OWN(7); OWN(8); }
+#undef OWN
+  return B200_ERR_UNSUPPORTED;
 }
 
 }  // namespace b200
 using namespace b200;
 
 // How the shared keys of a call are worked on: the number of ranges (1 .. 32), plus kPxTc where tcgen05 does it.
+// Which kernel: tcgen05 for the head sizes that it has, but for up to 32 rows a group and 1024 keys (32 / 8 heads of 128, one token, 600 keys: 15.4 us, 13.3 on
+// mma.sync; 4096 keys: 19.1 and 19.4, 16000: 29.7 and 37.9; 64 rows, 16000 keys: 30 and 42; 128 rows: 30 and 52).
+// How many ranges: those that a cost makes cheapest, in us: the blocks of a CTA, each of which takes longer where an SM has more CTAs (0.72 and 1.15
+// for one and two on tcgen05, 1.7 for each on mma.sync), rounds of CTAs, and the ranges' way through L2, written and read at 4 TB/s. 64 x 4096 keys with 32 / 8 heads:
+// 4, 8, 9, 18 ranges 44, 38, 39, 40 us (chosen: 8); 128 x 16384: 4, 8, 9, 12 ranges 92, 75.5, 75.3, 91 (9); 100 x 8000, 12 / 2 heads of 64: 4, 9, 12, 18 ranges
+// 36, 25.7, 23.7, 26.2 (14).
 constexpr int kPxTc = 256;
-B200_API int b200_prefix_attn_plan(int n_groups, int longest, int max_shared, int H, int G, int D, int block_size, int n_pages) {
-  if (n_groups < 1 || longest < 1 || max_shared < 1 || H < 1 || G < 1 || H % G || block_size < 1 || n_pages < 0) return 1;
-  const int rep = H / G, tokens = prefix_tc_tokens(H, G, D, block_size);
-  const bool tc = tokens > 0 && (long long)longest * rep > 32 && (long long)n_pages * G * block_size < 0x7fffff00LL;
-  const long long items = (long long)n_groups * G * (tc ? ceil_div(longest, tokens) : ceil_div64((int64_t)longest * rep, kPxRows));
-  long long n = ceil_div64(tc ? 2 * kNumSMs : 3 * kNumSMs, items);
-  const long long most = ceil_div64(max_shared, 256);
-  if (n > most) n = most;
-  return (int)(n > 32 ? 32 : n) + (tc ? kPxTc : 0);
+B200_API int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int H, int G, int D) {
+  if (T < 1 || n_groups < 1 || longest < 1 || max_shared < 1 || H < 1 || G < 1 || H % G) return 1;
+  const int rep = H / G, tokens = prefix_tc_tokens(H, G, D);
+  const bool tc = tokens > 0 && !((long long)longest * rep <= 32 && max_shared <= 1024);
+  // tiles: those of the longest group for each, but no more than the batch can fill
+  const long long of_longest = tc ? ceil_div(longest, tokens) : ceil_div64((int64_t)longest * rep, kPxRows);
+  const long long of_batch = (tc ? T / tokens : (long long)T * rep / kPxRows) + n_groups;
+  const long long items = G * (n_groups * of_longest < of_batch ? n_groups * of_longest : of_batch), blocks = ceil_div64(max_shared, kPxKeys);
+  const int resident = tc ? 2 : 3;
+  const double pass = (double)T * H * D * 8 / 4e6;
+  int best = 1;
+  double least = 0;
+  for (int n = 1; n <= 32 && n <= blocks; ++n) {
+    const long long ctas = items * n, rounds = ceil_div64(ctas, resident * kNumSMs);
+    const int beside = ctas > resident * kNumSMs ? resident : (int)ceil_div64(ctas, kNumSMs);
+    const double cost = rounds * ceil_div64(blocks, n) * (tc ? 0.29 + 0.43 * beside : 1.7 * beside) + n * pass;
+    if (n == 1 || cost < least) { best = n; least = cost; }
+  }
+  return best + (tc ? kPxTc : 0);
 }
 
 B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const void* cv, int n_pages, const int* pos, const int* slot,
@@ -436,9 +479,10 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
                         reinterpret_cast<uintptr_t>(part)) & 15)) return B200_ERR_BAD_ALIGN;
   PrefixParams p = {};
   while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
-  if ((1 << p.bs_log2) != block_size) return B200_ERR_UNSUPPORTED;
+  // a swizzled box starts on a group of eight rows, and rows of the pools are counted in 32 bits
+  if ((1 << p.bs_log2) != block_size || block_size < 8 || n_pages < 1 || (long long)n_pages * G * block_size >= 0x7fffff00LL) return B200_ERR_UNSUPPORTED;
   if (n_groups > 0 && longest > 0 && !part) return B200_ERR_BAD_SHAPE;
-  if (tc && (prefix_tc_tokens(H, G, D, block_size) < 1 || n_pages < 1 || (long long)n_pages * G * block_size >= 0x7fffff00LL)) return B200_ERR_UNSUPPORTED;
+  if (tc && prefix_tc_tokens(H, G, D) < 1) return B200_ERR_UNSUPPORTED;
   p.q = q; p.ck = ck; p.cv = cv; p.q_stride = q_stride; p.pos = pos; p.slot = slot; p.table = table; p.table_stride = table_stride;
   p.table_rows = table_rows; p.width = width; p.n_pages = n_pages; p.groups = groups; p.of = of; p.n_groups = n_groups;
   p.longest = longest; p.sinks = sinks; p.out = out; p.T = T; p.H = H; p.G = G; p.D = D; p.nsplit = nsplit;

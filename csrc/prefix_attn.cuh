@@ -46,7 +46,7 @@ __device__ __forceinline__ int page_of(const PrefixParams& p, const int* row, in
 
 // The shared keys on tcgen05 (prefix_attn_tc.cu): part_o and part_ml of every row and range, as the mma.sync kernel leaves them. Tokens of a tile, 0 where the
 // kernel does not take the call.
-int prefix_tc_tokens(int H, int G, int D, int block_size);
+int prefix_tc_tokens(int H, int G, int D);
 int prefix_shared_tc(const PrefixParams& p, int dtype, cudaStream_t st);
 
 }  // namespace b200

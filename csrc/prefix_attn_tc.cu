@@ -19,6 +19,10 @@ namespace b200 {
 
 constexpr int kPtRows = 128, kPtThreads = 192;
 constexpr uint32_t kPtCols = 256, kPtO = 128;
+// How far a row's maximum may run ahead of the number that its weights refer to before O is scaled (an exponent of two). With 32 rows to a warp one of
+// them has a new maximum in almost every block: with no slack 128 x 16384 keys, 32 / 8 heads of 128, take 88 us, with 2^8 75. A weight of up to 256 is rounded
+// like one of up to 1, relative to itself, and sums are in 32 bits.
+constexpr float kPtSlack = 8.f;
 
 template <int D> struct PtSmem {
   static constexpr uint32_t kHalves = D / 64, kStage = 8192 * kHalves;
@@ -77,6 +81,7 @@ prefix_shared_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_con
   extern __shared__ __align__(1024) uint8_t smem_pt[];
   const uint32_t sbase = smem_u32(smem_pt);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
   const PrefixGroup grp = prefix_group(p, blockIdx.z);
   const int rep = p.H / p.G, tiles = gridDim.y / p.G, kvh = blockIdx.y / tiles, tok0 = blockIdx.y % tiles * tile_tokens;
   const int nrows = min(tile_tokens, grp.tokens - tok0) * rep;
@@ -224,9 +229,9 @@ prefix_shared_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_con
 #pragma unroll
         for (int c = 0; c < 4; ++c) m4[c] = pt_max3(m4[c], __uint_as_float(v[i + 2 * c]), __uint_as_float(v[i + 2 * c + 1]));
       const float mn = fmaxf(m, fmaxf(pt_max3(m4[0], m4[1], m4[2]), m4[3]) * sl);      // the scale is above zero (checked by the launcher)
-      const bool raise = mn > m;
+      const bool raise = mn > m + kPtSlack;
       const float alpha = raise ? pt_ex2(m - mn) : 1.f;
-      m = mn;
+      if (raise) m = mn;
       const float e = m == -INFINITY ? 0.f : m;
       const bool any_raise = j > 0 && __any_sync(0xffffffffu, raise);
       // The product of block j - 1 is complete: O may be read. A parity tells phase c from c + 1, not from c + 2; S(j) proves that the product
@@ -309,10 +314,9 @@ prefix_shared_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_con
   }
 }
 
-int prefix_tc_tokens(int H, int G, int D, int block_size) {
+int prefix_tc_tokens(int H, int G, int D) {
   const int rep = H / G;
-  // a swizzled box starts on a group of eight rows
-  return (D == 64 || D == 128) && rep <= kPtRows && block_size >= 8 ? kPtRows / rep : 0;
+  return (D == 64 || D == 128) && rep <= kPtRows ? kPtRows / rep : 0;
 }
 
 template <int D, bool BF16>

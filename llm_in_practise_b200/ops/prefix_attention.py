@@ -65,13 +65,13 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     """Context [T, H * D] of token t over keys ``0 .. pos[t]`` of cache row ``slot[t]``, as ``paged_attention`` gives it (same arguments; no
     window), with the shared keys of ``groups`` read once. Tokens of a group whose position is before its last shared key, and tokens of no
     group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. Caches of 16 bits with head sizes that
-    are multiples of 16 up to 128, pages of a power of two and a positive scale; others go through ``paged_attention``, as does a step without
+    are multiples of 16 up to 128, pages of a power of two from 8 on (fewer than 2^31 - 256 rows of a pool in all) and a positive scale; others go through ``paged_attention``, as does a step without
     groups. Captured into a graph, each call keeps a workspace of its own. ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it
     (include/b200_ops.h); 0: chosen by the sizes."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
     BS = cache_k.shape[2]
     if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or q.dtype not in (torch.bfloat16, torch.float16) or D % 16 or D > 128
-            or BS & (BS - 1) or not scale > 0):
+            or BS < 8 or BS & (BS - 1) or cache_k.shape[0] * G * BS >= 2 ** 31 - 256 or not scale > 0):
         return paged_attention(q, cache_k, cache_v, table.contiguous(), pos, slot, H, G, D, scale, sinks=sinks, max_pos=max_pos)
     dev = q.device
     if cache_k.dtype != q.dtype or cache_v.dtype != q.dtype or cache_k.shape != cache_v.shape or cache_k.shape[1] != G or cache_k.shape[3] != D:
@@ -90,7 +90,7 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     _int32("the groups' table", groups.groups, dev, (groups.n_groups, 4))
     out = torch.empty(T, H * D, dtype=q.dtype, device=dev)
     if not plan:
-        plan = nv.proto("b200_prefix_attn_plan", [i32] * 8)(groups.n_groups, groups.longest, groups.max_shared, H, G, D, BS, cache_k.shape[0])
+        plan = nv.proto("b200_prefix_attn_plan", [i32] * 7)(T, groups.n_groups, groups.longest, groups.max_shared, H, G, D)
     part = torch.empty(T * H * (plan % 256) * (D + 2), dtype=torch.float32, device=dev)
     fn = nv.proto("b200_prefix_attn", [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32,
                                        i32, vp])

@@ -448,7 +448,7 @@ def close(got, b, scale=None, sinks=None):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,G,D", [(16, 4, 128), (40, 8, 128), (8, 8, 128), (16, 1, 128), (12, 2, 64), (4, 4, 64), (24, 2, 64), (8, 4, 96), (6, 2, 80), (3, 1, 16), (5, 5, 112)])
-@pytest.mark.parametrize("BS", [1, 8, 16, 64, 256])
+@pytest.mark.parametrize("BS", [8, 16, 64, 256])
 def test_shared_keys(entries, H, G, D, BS):
     """Groups of 1 to 40 tokens whose shared part ends in and beside pages, tiles and ranges; sequences by themselves between and behind them."""
     b = batch_of([(3, 64), (1, 1), (40, 257), (2, 63), (17, 640)], 3, [1, 2, 65, 31, 200, 129], H, G, D, BS, torch.bfloat16, H + D + BS)
@@ -592,9 +592,10 @@ def test_captured_and_on_another_stream(D):
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_other_caches_go_through_paged_attention(entries, device):
-    """32-bit caches, head sizes and steps without groups that the kernels are not for."""
-    for dtype, D, groups in ((torch.float32, 64, None), (torch.bfloat16, 24, None), (torch.bfloat16, 160, None), (torch.bfloat16, 64, [])):
-        b = batch_of([(4, 40)], 1, [3, 20], 4, 2, D, 16, dtype, 1)
+    """32-bit caches, head sizes, small pages and steps without groups that the kernels are not for."""
+    for dtype, D, groups, BS in ((torch.float32, 64, None, 16), (torch.bfloat16, 24, None, 16), (torch.bfloat16, 160, None, 16), (torch.bfloat16, 64, [], 16),
+                                 (torch.bfloat16, 64, None, 4), (torch.bfloat16, 64, None, 1)):
+        b = batch_of([(4, 40)], 1, [3, 20], 4, 2, D, BS, dtype, 1)
         close(call(b, device, groups=groups), b)
     assert "b200_prefix_attn" not in entries
 
