@@ -794,10 +794,12 @@ typedef struct {
   int32_t rows, width, bias_width, words;
 } b200_logit_rules;
 #endif
-/* out fp32 [B, ldo]: seen: y < 0 ? y r : y / r; in the output c times: y -= f c, y -= p; y += bias; y /= T; not allowed: -inf. */
-int b200_process_logits(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, float* out, long long ldo, int dtype, void* stream);
-/* The best token of each row under these rules, the lowest of equals, NaN above all. workspace: b200_greedy_workspace(B, V) bytes. */
-long long b200_greedy_workspace(int B, int V);
+/* out fp32 [B, ldo] (x itself, if that is fp32 with the same rows): seen: y < 0 ? y r : y / r; in the output c times: y -= f c, y -= p; y += bias; y /= T;
+ * not allowed: -inf. V up to 2^19. workspace: b200_logits_workspace(B, V, greedy) bytes, 16-byte aligned, of this call alone while it runs. */
+long long b200_logits_workspace(int B, int V, int greedy);
+int b200_process_logits(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, void* workspace, float* out, long long ldo,
+                        int dtype, void* stream);
+/* The best token of each row under these rules, the lowest of equals, NaN above all. */
 int b200_greedy_tokens(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, void* workspace, long long* ids, int dtype,
                        void* stream);
 /* ids int64 [n] behind the histories of rows slot[i] (NULL: i), whose lengths go up by one; full rows and slots outside the table keep theirs. */

@@ -20,8 +20,9 @@ import torch
 from . import _native as nv
 
 vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+MAX_VOCAB = 1 << 19
 MAX_BIAS = 2047          # biases of one row
-MAX_HISTORY = 1 << 20    # tokens of one row's history
+MAX_HISTORY = (1 << 20) - 1      # tokens of one row's history
 
 
 class _Rules(ctypes.Structure):
@@ -40,8 +41,8 @@ class LogitState:
     nobody writes the rows that another call reads."""
 
     def __init__(self, rows: int, vocab: int, max_len: int, max_bias: int = 0, device=None):
-        if rows < 1 or vocab < 1 or not 1 <= max_len <= MAX_HISTORY or not 0 <= max_bias <= MAX_BIAS:
-            raise ValueError(f"LogitState: rows and vocab must be positive, max_len 1 .. {MAX_HISTORY}, max_bias 0 .. {MAX_BIAS}")
+        if rows < 1 or not 1 <= vocab <= MAX_VOCAB or not 1 <= max_len <= MAX_HISTORY or not 0 <= max_bias <= MAX_BIAS:
+            raise ValueError(f"LogitState: rows must be positive, vocab 1 .. {MAX_VOCAB}, max_len 1 .. {MAX_HISTORY}, max_bias 0 .. {MAX_BIAS}")
         self.rows, self.vocab, self.max_len, self.max_bias = rows, vocab, max_len, max_bias
         self.words = -(-vocab // 32)
 
@@ -53,6 +54,7 @@ class LogitState:
         self.bias_ids, self.bias_values = of(torch.int32, rows, max_bias), of(torch.float32, rows, max_bias)
         self.bias_length = of(torch.int32, rows)
         self.mask = self.masked = None
+        self._work = {}                                  # bytes of a workspace by batch size and form
         self.device = self.tokens.device
 
     def allow_masks(self) -> "LogitState":
@@ -129,7 +131,7 @@ class LogitState:
 
 
 def _check_slot(what, state, n, slot):
-    if slot is not None and (slot.dtype != torch.int32 or slot.shape != (n,) or not slot.is_contiguous() or slot.device != state.device):
+    if slot is not None and (slot.dtype is not torch.int32 or slot.shape != (n,) or not slot.is_contiguous() or slot.device != state.device):
         raise ValueError(f"{what}: slot must be a contiguous int32 [{n}] tensor on the state's device")
     if slot is None and n > state.rows:
         raise ValueError(f"{what}: {n} rows, and the state has {state.rows}: name them with slot")
@@ -138,7 +140,7 @@ def _check_slot(what, state, n, slot):
 def _check(what, logits, state, slot):
     if logits.dim() != 2 or logits.shape[1] != state.vocab or logits.device != state.device:
         raise ValueError(f"{what}: logits must be [rows, {state.vocab}] on {state.device}, like the state")
-    if logits.stride(1) != 1:
+    if logits.stride(1) != 1 and state.vocab > 1:
         raise ValueError(f"{what}: the logits of a row must be contiguous")
     _check_slot(what, state, logits.shape[0], slot)
 
@@ -154,11 +156,23 @@ def process_logits(logits: torch.Tensor, state: LogitState, slot: Optional[torch
         raise ValueError("process_logits: out must be fp32, like the logits in shape, with contiguous rows")
     if not nv.use_native(logits):
         return out.copy_(_rules_torch(logits, state, slot))
-    fn = nv.proto("b200_process_logits", [vp, i64, i32, i32, vp, vp, vp, i64, i32, vp])
-    nv.check(nv.call_on(logits.device, fn, nv.ptr(logits), logits.stride(0), logits.shape[0], state.vocab, nv.ptr(slot), state._address(), nv.ptr(out),
-                        out.stride(0), nv.dtype_code(logits.dtype)), "process_logits")
-    nv.count_launch()
+    if logits.shape[0] == 0:
+        return out
+    work = _workspace(state, logits.shape[0], 0)
+    fn = nv.proto("b200_process_logits", [vp, i64, i32, i32, vp, vp, vp, vp, i64, i32, vp])
+    nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), logits.shape[0], state.vocab, nv.ptr(slot), state._address(),
+                        work.data_ptr(), out.data_ptr(), out.stride(0), nv.dtype_code(logits.dtype)), "process_logits")
+    nv.count_launch(2)
     return out
+
+
+def _workspace(state, B, greedy):
+    size = state._work.get((B, greedy))
+    if size is None:
+        fn = nv.lib().b200_logits_workspace
+        fn.argtypes, fn.restype = [i32] * 3, i64
+        size = state._work[B, greedy] = fn(B, state.vocab, greedy)
+    return torch.empty(size, dtype=torch.uint8, device=state.device)
 
 
 def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -169,11 +183,13 @@ def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.
         return _rules_torch(logits, state, slot).argmax(1)
     B = logits.shape[0]
     ids = torch.empty(B, dtype=torch.int64, device=logits.device)
-    work = torch.empty(B * -(-state.vocab // 4096), dtype=torch.int64, device=logits.device)
+    if B == 0:
+        return ids
+    work = _workspace(state, B, 1)
     fn = nv.proto("b200_greedy_tokens", [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp])
-    nv.check(nv.call_on(logits.device, fn, nv.ptr(logits), logits.stride(0), B, state.vocab, nv.ptr(slot), state._address(), nv.ptr(work), nv.ptr(ids),
-                        nv.dtype_code(logits.dtype)), "greedy_tokens")
-    nv.count_launch(2)
+    nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), B, state.vocab, nv.ptr(slot), state._address(), work.data_ptr(),
+                        ids.data_ptr(), nv.dtype_code(logits.dtype)), "greedy_tokens")
+    nv.count_launch(3)
     return ids
 
 

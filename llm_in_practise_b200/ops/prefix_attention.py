@@ -19,6 +19,7 @@ from . import _native as nv
 from .paged_attention import paged_attention
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_ARGS = [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp]
 
 
 @dataclass
@@ -54,9 +55,10 @@ def make_prefix_groups(groups: Sequence[Sequence[int]], tokens: int, device) -> 
                         max((r[2] for r in rows), default=0))
 
 
-def _int32(name, t, device, shape):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"prefix_attention: {name} must be a contiguous int32 {list(shape)} tensor on the queries' device")
+def _ints(device, **tensors):
+    for name, (t, shape) in tensors.items():
+        if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+            raise ValueError(f"prefix_attention: {name} must be a contiguous int32 {list(shape)} tensor on the queries' device")
 
 
 def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
@@ -69,33 +71,30 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     groups. Captured into a graph, each call keeps a workspace of its own. ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it
     (include/b200_ops.h); 0: chosen by the sizes."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
-    BS = cache_k.shape[2]
-    if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or q.dtype not in (torch.bfloat16, torch.float16) or D % 16 or D > 128
+    BS, dt = cache_k.shape[2], q.dtype
+    if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or (dt is not torch.bfloat16 and dt is not torch.float16) or D % 16 or D > 128
             or BS < 8 or BS & (BS - 1) or cache_k.shape[0] * G * BS >= 2 ** 31 - 256 or not scale > 0):
         return paged_attention(q, cache_k, cache_v, table.contiguous(), pos, slot, H, G, D, scale, sinks=sinks, max_pos=max_pos)
-    dev = q.device
-    if cache_k.dtype != q.dtype or cache_v.dtype != q.dtype or cache_k.shape != cache_v.shape or cache_k.shape[1] != G or cache_k.shape[3] != D:
-        raise ValueError(f"prefix_attention: caches must be {q.dtype} [blocks, {G}, block_size, {D}], both of one shape")
+    dev, pools = q.device, cache_k.shape
+    if cache_k.dtype is not dt or cache_v.dtype is not dt or cache_v.shape != pools or pools[1] != G or pools[3] != D:
+        raise ValueError(f"prefix_attention: caches must be {dt} [blocks, {G}, block_size, {D}], both of one shape")
     if not cache_k.is_contiguous() or not cache_v.is_contiguous() or cache_k.device != dev or cache_v.device != dev:
         raise ValueError("prefix_attention: caches must be contiguous and on the queries' device")
-    if H % G or q.dim() != 2 or q.shape[1] < H * D or (T and q.stride(1) != 1) or q.stride(0) % 8 or q.data_ptr() % 16:
+    q_ptr, stride = q.data_ptr(), q.stride()
+    if H % G or len(stride) != 2 or q.shape[1] < H * D or (T and stride[1] != 1) or stride[0] % 8 or q_ptr % 16:
         raise ValueError(f"prefix_attention: queries must be rows of {H * D} or more contiguous values that start on 16 bytes")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev or (table.stride(1) != 1 and table.shape[1] > 1):
         raise ValueError("prefix_attention: the block table is int32 [rows, blocks] with contiguous rows on the queries' device")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous() or sinks.device != dev):
+    if sinks is not None and (sinks.dtype is not torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous() or sinks.device != dev):
         raise ValueError(f"prefix_attention: sinks must be contiguous fp32 [{H}] on the queries' device")
-    _int32("pos", pos, dev, (T,))
-    _int32("slot", slot, dev, (T,))
-    _int32("the groups' token table", groups.of, dev, (T,))
-    _int32("the groups' table", groups.groups, dev, (groups.n_groups, 4))
-    out = torch.empty(T, H * D, dtype=q.dtype, device=dev)
+    _ints(dev, pos=(pos, (T,)), slot=(slot, (T,)), of=(groups.of, (T,)), groups=(groups.groups, (groups.n_groups, 4)))
     if not plan:
         plan = nv.proto("b200_prefix_attn_plan", [i32] * 7)(T, groups.n_groups, groups.longest, groups.max_shared, H, G, D)
+    out = torch.empty(T, H * D, dtype=dt, device=dev)
     part = torch.empty(T * H * (plan % 256) * (D + 2), dtype=torch.float32, device=dev)
-    fn = nv.proto("b200_prefix_attn", [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32,
-                                       i32, vp])
-    nv.check(nv.call_on(dev, fn, nv.ptr(q), q.stride(0), nv.ptr(cache_k), nv.ptr(cache_v), cache_k.shape[0], nv.ptr(pos), nv.ptr(slot), nv.ptr(table),
-                        table.stride(0), table.shape[0], table.shape[1], nv.ptr(groups.groups), nv.ptr(groups.of), groups.n_groups, groups.longest,
-                        nv.ptr(sinks), nv.ptr(out), nv.ptr(part), plan, T, H, G, D, BS, scale, nv.dtype_code(q.dtype)), "prefix_attn")
+    fn = nv.proto("b200_prefix_attn", _ARGS)
+    nv.check(nv.call_on(dev, fn, q_ptr, stride[0], cache_k.data_ptr(), cache_v.data_ptr(), pools[0], pos.data_ptr(), slot.data_ptr(), table.data_ptr(),
+                        table.stride(0), *table.shape, groups.groups.data_ptr(), groups.of.data_ptr(), groups.n_groups, groups.longest, nv.ptr(sinks),
+                        out.data_ptr(), part.data_ptr(), plan, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
     nv.count_launch(2)
     return out

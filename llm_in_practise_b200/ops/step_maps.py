@@ -39,18 +39,21 @@ class StepMaps:
     run_tiles: Optional[torch.Tensor] = None
 
 
-def _lengths(what, device, n, **tensors):
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device or (n is not None and t.shape[0] != n):
-            raise ValueError(f"{what}: {name} must be a contiguous int32 [{'n' if n is None else n}] tensor on {device}, like rows and the table")
+def _ints(n, device, tensors) -> bool:
+    """All of them contiguous int32 [n] on the device?"""
+    for t in tensors:
+        if t.dtype is not torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
+            return False
+    return True
 
 
-def _check(what, table, rows, block_size, **tensors):
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+def _check(what, table, rows, block_size, *lengths):
+    if table.dtype is not torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
         raise ValueError(f"{what}: the block table is int32 [rows, blocks] with contiguous rows")
     if block_size < 1:
         raise ValueError(f"{what}: block_size must be positive, not {block_size}")
-    _lengths(what, table.device, rows.shape[0], rows=rows, **tensors)
+    if rows.dim() != 1 or not _ints(rows.shape[0], table.device, (rows, *lengths)):
+        raise ValueError(f"{what}: rows and lengths must be contiguous int32 tensors of one size on the table's device, {table.device}")
 
 
 def extend_block_tables(table: torch.Tensor, rows: torch.Tensor, cached: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
@@ -60,14 +63,15 @@ def extend_block_tables(table: torch.Tensor, rows: torch.Tensor, cached: torch.T
     order of the requests (none where a length shrinks). ``rows`` are different rows. Returns the number of blocks that the requests need, int32 [1]
     on the device: where it is more than ``blocks`` holds, entries beyond the list stay as they were, and so do those beyond the table's
     width. With ``block_size`` 1 ``cached`` and ``lens`` count blocks."""
-    _check("extend_block_tables", table, rows, block_size, cached=cached, lens=lens)
-    _lengths("extend_block_tables", table.device, None, blocks=blocks)
+    _check("extend_block_tables", table, rows, block_size, cached, lens)
+    if blocks.dim() != 1 or not _ints(blocks.shape[0], table.device, (blocks,)):
+        raise ValueError(f"extend_block_tables: blocks must be a contiguous int32 tensor on the table's device, {table.device}")
     n = rows.shape[0]
     used = torch.empty(1, dtype=torch.int32, device=table.device)
     if nv.use_native(table):
         fn = nv.proto("b200_extend_block_tables", [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp, i32, i32, vp])
-        nv.check(nv.call_on(table.device, fn, nv.ptr(table), table.stride(0), table.shape[0], table.shape[1], nv.ptr(rows), nv.ptr(cached), nv.ptr(lens),
-                            nv.ptr(blocks), blocks.shape[0], nv.ptr(used), n, block_size), "extend_block_tables")
+        nv.check(nv.call_on(table.device, fn, table.data_ptr(), table.stride(0), *table.shape, rows.data_ptr(), cached.data_ptr(), lens.data_ptr(),
+                            blocks.data_ptr(), blocks.shape[0], used.data_ptr(), n, block_size), "extend_block_tables")
         nv.count_launch()
         return used
     at = 0
@@ -87,7 +91,7 @@ def step_maps(table: torch.Tensor, rows: torch.Tensor, cached: torch.Tensor, new
     int32 [rows, max_blocks] lists their blocks already). ``total``: the step's tokens, as known to the host: rows of the result, which where
     it is larger than the sum of ``new`` are not written behind that sum. ``n_tiles`` > 0: tables of the tiles too, so many of them; where the step
     has fewer, the others are of no rows (where more, they are left out)."""
-    _check("step_maps", table, rows, block_size, cached=cached, new=new)
+    _check("step_maps", table, rows, block_size, cached, new)
     n, dev = rows.shape[0], table.device
     if n < 1 or total < 0 or n_tiles < 0:
         raise ValueError("step_maps: a step has at least one request, and no negative number of tokens or tiles")
@@ -95,18 +99,22 @@ def step_maps(table: torch.Tensor, rows: torch.Tensor, cached: torch.Tensor, new
         return _step_maps_torch(table, rows, cached, new, block_size, total, n_tiles)
     four = 4 * n if n_tiles else 0
     # one allocation for the int32 tables (those of four columns first, so that they start on 16 bytes), one for the int64 ones
-    words = torch.empty(2 * (4 * n_tiles + four) + 2 * total + n + 1, dtype=torch.int32, device=dev)
+    at = 8 * n_tiles + 2 * four
+    words = torch.empty(at + 2 * total + n + 1, dtype=torch.int32, device=dev)
     longs = torch.empty(total + n, dtype=torch.int64, device=dev)
-    tiles, tile_of, runs, run_tiles, pos, slot, cu = words.split_with_sizes([4 * n_tiles, 4 * n_tiles, four, four, total, total, n + 1])
-    place, last = longs.split_with_sizes([total, n])
+    w, g = words.data_ptr(), longs.data_ptr()
+    w_pos = w + 4 * at
     fn = nv.proto("b200_step_maps", [vp, i64, i32, i32, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp])
-    nv.check(nv.call_on(dev, fn, nv.ptr(table), table.stride(0), table.shape[0], table.shape[1], nv.ptr(rows), nv.ptr(cached), nv.ptr(new), n, block_size,
-                        total, n_tiles, nv.ptr(cu), nv.ptr(pos), nv.ptr(slot), nv.ptr(place), nv.ptr(last), nv.ptr(tiles), nv.ptr(tile_of), nv.ptr(runs),
-                        nv.ptr(run_tiles)), "step_maps")
+    nv.check(nv.call_on(dev, fn, table.data_ptr(), table.stride(0), *table.shape, rows.data_ptr(), cached.data_ptr(), new.data_ptr(), n, block_size, total,
+                        n_tiles, w_pos + 8 * total, w_pos, w_pos + 4 * total, g, g + 8 * total, w, w + 16 * n_tiles, w + 32 * n_tiles,
+                        w + 32 * n_tiles + 4 * four), "step_maps")
     nv.count_launch()
+    place, last = longs.split_with_sizes((total, n))
     if not n_tiles:
+        pos, slot, cu = words.split_with_sizes((total, total, n + 1))
         return StepMaps(cu, pos, slot, place, last)
-    return StepMaps(cu, pos, slot, place, last, tiles.view(-1, 4), tile_of.view(-1, 4), runs.view(-1, 4), run_tiles.view(-1, 4))
+    fours, pos, slot, cu = words.split_with_sizes((at, total, total, n + 1))
+    return StepMaps(cu, pos, slot, place, last, *fours.view(-1, 4).split_with_sizes((n_tiles, n_tiles, n, n)))
 
 
 def _step_maps_torch(table, rows, cached, new, bs, total, n_tiles) -> StepMaps:

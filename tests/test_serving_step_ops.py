@@ -1,8 +1,8 @@
 """Operators of a serving step that shares work between its sequences: attention over shared keys, block tables and maps from the
 requests' lengths, rules on logits. Each against a statement of its own in 64 bits (or in whole numbers), token by token; the plain PyTorch
 path on the CPU, the kernels on the GPU."""
+import collections
 import itertools
-import math
 
 import pytest
 import torch
@@ -309,6 +309,42 @@ def test_biases_that_name_a_token_twice(device):
 
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("V,n", [(50257, 12000), (50257, 12300), (50257, 40000), (524288, 20000), (7, 30000)])
+def test_long_histories(device, V, n):
+    """More tokens than the table has room for by their hashes, all different or the same few, in the largest vocabulary too; biases among them."""
+    g = torch.Generator().manual_seed(n)
+    toks = torch.randint(0, V, (n,), generator=g).tolist()
+    rows = [dict(prompt=toks[:n // 2], output=toks[n // 2:], repetition_penalty=1.2, frequency_penalty=0.01, presence_penalty=0.5,
+                 logit_bias={toks[0]: 2.0, toks[-1]: -1.0, V - 1: 0.5}), dict(output=list(range(min(V, n))), frequency_penalty=1.0)]
+    st = state_of(rows, V, n, device)
+    x = torch.randn(2, V, generator=g) * 3
+    said = [collections.Counter(r.get("output", ())) for r in rows]
+    want, bound = exact_counts(x, rows, said)
+    y = process_logits(x.to(device), st)
+    check_rules(y, want, bound)
+    assert torch.equal(greedy_tokens(x.to(device), st).cpu(), y.argmax(1).cpu())
+
+
+def exact_counts(x, rows, said):
+    """As exact_rules for unmasked rows, by vectors: six roundings of numbers no larger than the sum of the sizes."""
+    want, size = x.double().clone(), x.double().abs()
+    for y, s, r, c in zip(want, size, rows, said):
+        count = torch.zeros(y.shape[0], dtype=torch.float64)
+        count[torch.tensor(list(c))] = torch.tensor([float(v) for v in c.values()], dtype=torch.float64)
+        seen = count > 0
+        if r.get("prompt"):
+            seen[torch.tensor(r["prompt"])] = True
+        rep, f, p = (f32(r.get(k, d)) for k, d in (("repetition_penalty", 1.0), ("frequency_penalty", 0.0), ("presence_penalty", 0.0)))
+        y.copy_(torch.where(seen, torch.where(y < 0, y * rep, y / rep), y))
+        y -= f * count + p * (count > 0)
+        s.copy_(torch.maximum(s * max(rep, 1.0), s) + abs(f) * count + abs(p))
+        for t, v in (r.get("logit_bias") or {}).items():
+            y[t] += f32(v)
+            s[t] += abs(f32(v))
+    return want, size * 6 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
 def test_histories_grow(device):
     """Tokens come behind their rows' histories and count from the next call on; a full row and slots outside the state keep what they have."""
     V = 200
@@ -354,7 +390,7 @@ def test_refusals_of_rules():
                 dict(row=0, allowed=[-1]), dict(row=0, repetition_penalty=0.0), dict(row=0, temperature=0.0), dict(row=0, temperature=NAN)):
         with pytest.raises(ValueError, match="LogitState"):
             st.set_row(**bad)
-    for bad in (dict(rows=0), dict(vocab=0), dict(max_len=0), dict(max_len=(1 << 20) + 1), dict(max_bias=2048), dict(max_bias=-1)):
+    for bad in (dict(rows=0), dict(vocab=0), dict(vocab=(1 << 19) + 1), dict(max_len=0), dict(max_len=1 << 20), dict(max_bias=2048), dict(max_bias=-1)):
         with pytest.raises(ValueError, match="LogitState"):
             LogitState(**{**dict(rows=2, vocab=9, max_len=4), **bad})
     for ids, slot in ((torch.zeros(2), None), (torch.zeros(5, dtype=torch.int64), None), (torch.zeros(2, dtype=torch.int64), torch.zeros(2))):
