@@ -15,16 +15,21 @@ from __future__ import annotations
 import os
 
 import ctypes
+import math
 import queue
 import threading
 from dataclasses import dataclass
-from typing import Callable, Iterator, List, Optional, Sequence
+from typing import Callable, Dict, Iterator, List, Optional, Sequence
 
 import torch
 
 from ..ops import _native as nv
 from ..ops import elementwise as ew
 from ..ops import fused_decode
+from ..ops.logits import MAX_BIAS, LogitState, greedy_tokens, process_logits
+from ..ops.paged_attention import rope_paged_store
+from ..ops.prefix_attention import PrefixGroups, make_prefix_groups, prefix_attention
+from ..ops.step_maps import extend_block_tables
 from ..ops.attention import attention
 from ..ops.gemm import ensure_graph_workspace, gemm, gemv16
 from ..ops.norm import rms_norm
@@ -45,6 +50,34 @@ class GenerationConfig:
     eos_token_id: Optional[Sequence[int]] = None
     pad_token_id: int = 0
     ignore_eos: bool = False             # vLLM's sampling parameter: generate max_new_tokens whatever is sampled (benchmarks)
+    # rules on the logits beside the repetition penalty (ops.logits): the OpenAI API's penalties on what was generated, its logit_bias
+    # (token id -> value), and the only tokens that may be generated at all (vLLM's allowed_token_ids)
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None
+    allowed_token_ids: Optional[Sequence[int]] = None
+    # HF's prefix_allowed_tokens_fn(batch row or request id, its tokens so far) -> the tokens that may come next: a grammar, asked before every token
+    prefix_allowed_tokens_fn: Optional[Callable[[int, List[int]], Sequence[int]]] = None
+
+    def has_rules(self) -> bool:
+        """Whether ``LogitRules`` has anything to do for this configuration that ``sample_next`` does not."""
+        return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias or self.allowed_token_ids is not None
+                    or self.prefix_allowed_tokens_fn is not None)
+
+    def check_rules(self, vocab: int) -> None:
+        """Refuse rules that ``vocab`` tokens have no room for, before a step is run with them."""
+        if not self.has_rules():
+            return
+        bias = self.logit_bias or {}
+        if len(bias) > MAX_BIAS:
+            raise ValueError(f"logit_bias has {len(bias)} entries; at most {MAX_BIAS} are taken")
+        for t in [*bias, *(self.allowed_token_ids if self.allowed_token_ids is not None else ())]:
+            if not 0 <= int(t) < vocab:
+                raise ValueError(f"logit_bias and allowed_token_ids name token {t}, which is not one of the vocabulary's {vocab}")
+        if not all(math.isfinite(float(v)) for v in (*bias.values(), self.presence_penalty, self.frequency_penalty)):
+            raise ValueError("logit_bias and penalties must be finite")
+        if not self.repetition_penalty > 0 or (self.do_sample and self.temperature > 0 and not math.isfinite(self.temperature)):
+            raise ValueError("repetition_penalty must be positive and the temperature finite")
 
 
 def sample_next(logits: torch.Tensor, cfg: GenerationConfig, prev: Optional[torch.Tensor] = None,
@@ -58,7 +91,11 @@ def sample_next(logits: torch.Tensor, cfg: GenerationConfig, prev: Optional[torc
         lg = lg.scatter(1, prev, g)
     if not cfg.do_sample or cfg.temperature <= 0:
         return lg.argmax(-1)
-    lg = lg / cfg.temperature
+    return draw_next(lg / cfg.temperature, cfg, generator)
+
+
+def draw_next(lg: torch.Tensor, cfg: GenerationConfig, generator: Optional[torch.Generator] = None) -> torch.Tensor:
+    """fp32 logits [B, V] after penalties and temperature -> next ids [B]: top-k, top-p, multinomial."""
     if cfg.top_k and cfg.top_k > 0:
         kth = lg.topk(min(cfg.top_k, lg.shape[-1])).values[:, -1:]
         lg = lg.masked_fill(lg < kth, float("-inf"))
@@ -69,6 +106,73 @@ def sample_next(logits: torch.Tensor, cfg: GenerationConfig, prev: Optional[torc
         sl = sl.masked_fill(drop, float("-inf"))
         lg = torch.full_like(lg, float("-inf")).scatter(1, si, sl)
     return torch.multinomial(lg.softmax(-1), 1, generator=generator).squeeze(1)
+
+
+class LogitRules:
+    """``sample_next`` for sequences with rules on their logits: a ``LogitState`` with a row each, whose history grows with what is chosen.
+    ``rows`` sequences of up to ``max_len`` tokens."""
+
+    def __init__(self, rows: int, vocab: int, max_len: int, device, max_bias: int = 0):
+        self.state = LogitState(rows, vocab, max_len, max_bias, device)
+        self._tokens: Dict[int, List[int]] = {}          # rows whose grammar is asked before every token: what they hold
+        self._fn: Dict[int, tuple] = {}
+
+    def begin(self, row: int, cfg: GenerationConfig, prompt: Sequence[int], output: Sequence[int] = (), name: Optional[int] = None) -> None:
+        """Row ``row`` starts a sequence (``name``: what its ``prefix_allowed_tokens_fn`` is called with, by default the row)."""
+        warm = cfg.do_sample and cfg.temperature > 0
+        self.state.set_row(row, prompt, output, cfg.repetition_penalty, cfg.presence_penalty, cfg.frequency_penalty, cfg.temperature if warm else 1.0,
+                           cfg.logit_bias, cfg.allowed_token_ids)
+        self._fn.pop(row, None)
+        if cfg.prefix_allowed_tokens_fn is not None:
+            self._fn[row], self._tokens[row] = (cfg, row if name is None else name), [*prompt, *output]
+
+    def next(self, logits: torch.Tensor, rows: Sequence[int], cfgs: Sequence[GenerationConfig], generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """logits [B, V] of sequences ``rows`` (all different) -> next ids [B], which join the rows' histories."""
+        st, dev = self.state, logits.device
+        for row in rows:
+            if row in self._fn:
+                cfg, name = self._fn[row]
+                allowed = cfg.prefix_allowed_tokens_fn(name, list(self._tokens[row]))
+                if cfg.allowed_token_ids is not None:
+                    allowed = [t for t in allowed if t in set(cfg.allowed_token_ids)]
+                st.set_mask(row, [t for t in allowed if 0 <= int(t) < st.vocab])
+        slot = torch.tensor(list(rows), dtype=torch.int32)
+        slot = slot.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else slot
+        draws: Dict[tuple, List[int]] = {}
+        for i, c in enumerate(cfgs):
+            if c.do_sample and c.temperature > 0:
+                draws.setdefault((c.top_k, c.top_p), []).append(i)
+        if not draws:
+            ids = greedy_tokens(logits, st, slot)
+        else:
+            y = process_logits(logits, st, slot)
+            ids = y.argmax(1)
+            for at in draws.values():
+                ids[at] = draw_next(_one_at_least(y[at]), cfgs[at[0]], generator)
+        st.append(ids, slot)
+        if self._fn:
+            for row, t in zip(rows, ids.tolist()):
+                if row in self._fn:
+                    self._tokens[row].append(t)
+        return ids
+
+
+def logit_rules(cfg: GenerationConfig, prompts: torch.Tensor, vocab: int, max_len: int) -> Optional[LogitRules]:
+    """Rules of ``generate`` for prompts [B, S], None where ``sample_next`` does all that ``cfg`` asks for."""
+    if not cfg.has_rules():
+        return None
+    cfg.check_rules(vocab)
+    rules = LogitRules(prompts.shape[0], vocab, max_len, prompts.device, len(cfg.logit_bias or ()))
+    for b, ids in enumerate(prompts.tolist()):
+        rules.begin(b, cfg, ids)
+    return rules
+
+
+def _one_at_least(lg: torch.Tensor) -> torch.Tensor:
+    """Rows that allow no token at all draw token 0, as the greedy choice does, instead of failing the batch."""
+    none = (lg == float("-inf")).all(1)
+    lg[:, 0] = torch.where(none, torch.zeros_like(lg[:, 0]), lg[:, 0])
+    return lg
 
 
 class KVCache:
@@ -130,6 +234,18 @@ class PagedKVCache(KVCache):
         if len(blocks):
             self.table[slot, :len(blocks)] = torch.as_tensor(list(blocks), dtype=torch.int32).to(self.table.device, non_blocking=True)
 
+    def extend_rows(self, updates) -> None:
+        """Blocks behind those that sequences list already: ``updates`` = (slot, blocks listed, the next ones) of different sequences, all in one
+        copy and one launch."""
+        updates = [u for u in updates if len(u[2])]
+        if not updates:
+            return
+        n, flat = len(updates), [b for u in updates for b in u[2]]
+        host = torch.tensor([u[0] for u in updates] + [u[1] for u in updates] + [u[1] + len(u[2]) for u in updates] + flat, dtype=torch.int32)
+        dev = self.table.device
+        t = host.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else host
+        extend_block_tables(self.table, t[:n], t[n:2 * n], t[2 * n:3 * n], t[3 * n:])
+
     def _where(self, rows, pos):
         blk = self.table[rows, pos // self.block_size].long()
         return blk, pos % self.block_size
@@ -146,6 +262,28 @@ class PagedKVCache(KVCache):
         k = self.k[li].index_select(0, blks).permute(1, 0, 2, 3).reshape(Hkv, nb * self.block_size, D)
         v = self.v[li].index_select(0, blks).permute(1, 0, 2, 3).reshape(Hkv, nb * self.block_size, self.v[li].shape[3])
         return k, v
+
+
+MAX_GROUPS = 4           # groups of a captured decode step
+
+
+def group_plan(tokens: int, max_len: int, device) -> PrefixGroups:
+    """A plan that a captured step of ``tokens`` tokens keeps and ``set_group_plan`` rewrites: up to ``MAX_GROUPS`` groups, for now none."""
+    flat = torch.zeros(4 * MAX_GROUPS + tokens, dtype=torch.int32, device=device)
+    flat[4 * MAX_GROUPS:] = -1
+    return PrefixGroups(flat[:4 * MAX_GROUPS].view(-1, 4), flat[4 * MAX_GROUPS:], MAX_GROUPS, tokens, max_len)
+
+
+def set_group_plan(plan: PrefixGroups, groups) -> None:
+    """The groups of the next replay: (first token, tokens, shared keys) each."""
+    if len(groups) > plan.n_groups:
+        raise ValueError(f"a captured step takes {plan.n_groups} groups, not {len(groups)}")
+    new = make_prefix_groups(groups, plan.of.shape[0], "cpu")
+    host = torch.cat([new.groups.reshape(-1), torch.zeros(4 * (plan.n_groups - new.n_groups), dtype=torch.int32), new.of])
+    dev = plan.of.device
+    host = host.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else host
+    plan.groups.copy_(host[:4 * plan.n_groups].view(-1, 4))
+    plan.of.copy_(host[4 * plan.n_groups:])
 
 
 def _decode_attn(qkv, ck, cv, pos, H, Hkv, D, scale, slots=None, table=None):
@@ -284,6 +422,11 @@ class Generator:
         """Paged cache: logical -> physical block list of sequence ``slot``. A generator method so that tensor-parallel
         followers apply the same table update to their slice of the cache."""
         cache.set_row(slot, blocks)
+
+    @torch.no_grad()
+    def extend_block_rows(self, cache: KVCache, updates) -> None:
+        """Paged cache: the next blocks of several sequences (``PagedKVCache.extend_rows``)."""
+        cache.extend_rows(updates)
 
     @torch.no_grad()
     def _prefill_chunk(self, ids: torch.Tensor, cache: KVCache, slot: int, pos0: int) -> torch.Tensor:
@@ -432,11 +575,27 @@ class Generator:
                 self._tail = fused_decode.FusedTail(hid, x.device, None, x.dtype)
         return self._tail
 
+    prefix_groups = True                                 # decode steps take groups of sequences that share their first blocks
+
+    def _attend(self, qkv, cache: KVCache, li: int, pos, slots, groups: Optional[PrefixGroups]) -> torch.Tensor:
+        """Append the step's keys and values of layer ``li`` and attend: each sequence by itself, or with the keys of ``groups`` read once."""
+        c = self.cfg
+        H, Hkv, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+        ck, cv, table = cache.k[li], cache.v[li], getattr(cache, "table", None)
+        if groups is None:
+            return _decode_attn(qkv, ck, cv, pos, H, Hkv, D, D ** -0.5, slots, table)
+        none = self.__dict__.setdefault("_no_angles", {}).get(qkv.device)
+        if none is None:
+            none = self._no_angles[qkv.device] = torch.zeros(1, 1, dtype=torch.float32, device=qkv.device)
+        rope_paged_store(qkv, none, none, pos, slots, ck, cv, table, H, Hkv, D, rot_dims=0)       # rotated already
+        return prefix_attention(qkv, ck, cv, table, pos, slots, groups, H, Hkv, D, D ** -0.5)
+
     @torch.no_grad()
     def _decode(self, tok: torch.Tensor, cache: KVCache, pos: Optional[torch.Tensor] = None,
-                slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+                slots: Optional[torch.Tensor] = None, groups: Optional[PrefixGroups] = None) -> torch.Tensor:
         """One token per sequence. ``pos`` [B] int32 = tokens already cached per sequence (default: cache.len for
-        all); ``slots`` [B] int32 = cache row of each batch row (continuous batching)."""
+        all); ``slots`` [B] int32 = cache row of each batch row (continuous batching). ``groups``: batch rows whose sequences list the same
+        first blocks (a paged cache), so that attention reads those once."""
         m, c = self.model, self.cfg
         B = tok.shape[0]
         dev = tok.device
@@ -453,7 +612,7 @@ class Generator:
             x, res = rms_norm(delta, layers[0].input_layernorm, c.rms_norm_eps, None)
             for li, layer in enumerate(layers):
                 qkv = ew.qknorm_rope(layer.qkv_proj(x), layer.q_norm, layer.k_norm, cos, sin, pos, H, Hkv, D, False, c.rms_norm_eps)
-                ctx = _decode_attn(qkv, cache.k[li], cache.v[li], pos, H, Hkv, D, D ** -0.5, slots, getattr(cache, "table", None))
+                ctx = self._attend(qkv, cache, li, pos, slots, groups)
                 x, res = fused_decode.gemv_fused(layer.o_proj, ctx, res, layer.post_attention_layernorm, c.rms_norm_eps, tail)
                 nw = layers[li + 1].input_layernorm if li + 1 < len(layers) else m.norm
                 x, res = fused_decode.gemv_fused(layer.down_proj, ew.swiglu(layer.gate_up_proj(x)), res, nw, c.rms_norm_eps, tail)
@@ -462,7 +621,7 @@ class Generator:
             for li, layer in enumerate(m.layers):
                 x, res = rms_norm(delta, layer.input_layernorm, c.rms_norm_eps, res)
                 qkv = ew.qknorm_rope(layer.qkv_proj(x), layer.q_norm, layer.k_norm, cos, sin, pos, H, Hkv, D, False, c.rms_norm_eps)
-                ctx = _decode_attn(qkv, cache.k[li], cache.v[li], pos, H, Hkv, D, D ** -0.5, slots, getattr(cache, "table", None))
+                ctx = self._attend(qkv, cache, li, pos, slots, groups)
                 x, res = rms_norm(layer.o_proj(ctx), layer.post_attention_layernorm, c.rms_norm_eps, res)
                 delta = layer.down_proj(ew.swiglu(layer.gate_up_proj(x)))
             h, _ = rms_norm(delta, m.norm, c.rms_norm_eps, res)
@@ -471,12 +630,13 @@ class Generator:
         return logits if logits is not None else gemm(h, m.head_weight(), out_dtype=torch.float32)
 
     @torch.no_grad()
-    def decode_graphed(self, tok: torch.Tensor, cache: KVCache, pos: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    def decode_graphed(self, tok: torch.Tensor, cache: KVCache, pos: torch.Tensor, slots: torch.Tensor, groups=()) -> torch.Tensor:
         """``_decode`` replayed from a CUDA graph (one per batch size and cache): a decode step is ~14 launches per
         layer of a few microseconds each, so eager execution is bound by the Python launch rate, not by the GPU. The
         kernels read token ids, positions and cache slots from device tensors, so one graph serves any set of
         sequences. Falls back to the eager path on CPU and under tensor parallelism (the peer all-reduce takes a host
-        epoch). Inside a capture the GEMMs run without stream-K and 4-bit weights are expanded in line."""
+        epoch). Inside a capture the GEMMs run without stream-K and 4-bit weights are expanded in line. ``groups``: up to ``MAX_GROUPS`` of
+        (first batch row, rows, shared keys), as for ``make_prefix_groups``: sequences of a paged cache that list the same first blocks."""
         B = tok.shape[0]
         L = cache.len                                   # ``cache.len`` is the caller's to advance, never this method's
         tp = getattr(self.model, "tp", None)
@@ -484,25 +644,27 @@ class Generator:
         tp_eager = tp is not None and tp.world > 1 and not (getattr(tp, "fused", False) and getattr(tp, "oneshot", False)
                                                             and B * self.cfg.hidden_size <= getattr(tp, "half16", 0))
         if not tok.is_cuda or B > 512 or tp_eager:
-            out = self._decode(tok, cache, pos, slots)
+            out = self._decode(tok, cache, pos, slots, make_prefix_groups(groups, B, tok.device) if groups else None)
             cache.len = L
             return out
-        key = (B, id(cache))
+        key = (B, id(cache), "groups") if groups else (B, id(cache))
         g = self._graphs.get(key)
         if g is None:
-            st = {"tok": tok.clone(), "pos": pos.clone(), "slots": slots.clone()}
+            st = {"tok": tok.clone(), "pos": pos.clone(), "slots": slots.clone(), "plan": group_plan(B, cache.max_len, tok.device) if groups else None}
             ensure_graph_workspace(tok.device)                              # stream-K scratch of captured GEMMs
-            self._decode(st["tok"], cache, st["pos"], st["slots"])          # warm-up: allocates every lazily built buffer
+            self._decode(st["tok"], cache, st["pos"], st["slots"], st["plan"])          # warm-up: allocates every lazily built buffer
             torch.cuda.synchronize()
             graph = torch.cuda.CUDAGraph()
             with no_gc(), torch.cuda.graph(graph):
-                st["logits"] = self._decode(st["tok"], cache, st["pos"], st["slots"])
+                st["logits"] = self._decode(st["tok"], cache, st["pos"], st["slots"], st["plan"])
             g = self._graphs[key] = (graph, st)
             cache.len = L
         graph, st = g
         st["tok"].copy_(tok)
         st["pos"].copy_(pos)
         st["slots"].copy_(slots)
+        if groups:
+            set_group_plan(st["plan"], groups)
         graph.replay()
         return st["logits"]
 
@@ -543,8 +705,9 @@ class Generator:
         out = input_ids
         done = torch.zeros(B, dtype=torch.bool, device=dev)
         logprobs: List[torch.Tensor] = []
+        rules = logit_rules(cfg, input_ids, logits.shape[1], total)
         for _ in range(total - S):
-            nxt = sample_next(logits, cfg, out, gen)
+            nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen)
             if return_logprobs:
                 logprobs.append(logits.float().log_softmax(-1).gather(1, nxt[:, None]).squeeze(1))
             nxt = torch.where(done, torch.full_like(nxt, cfg.pad_token_id), nxt)

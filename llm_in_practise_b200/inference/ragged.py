@@ -20,9 +20,10 @@ import numpy as np
 import torch
 
 from ..ops.gemm import ensure_graph_workspace
+from ..ops.step_maps import step_maps
 from ..utils.graph_step import no_gc
 
-from .generate import GenerationConfig, Generator, PagedKVCache, sample_next
+from .generate import GenerationConfig, Generator, PagedKVCache, group_plan, logit_rules, sample_next, set_group_plan
 
 TILE_Q = 64          # query rows per tile of the tensor-core attention kernel
 
@@ -117,14 +118,14 @@ class RaggedGenerator(Generator):
 
     # ------------------------------------------------------------------ the step
     @torch.no_grad()
-    def step(self, entries: Sequence[Entry], cache: PagedKVCache, layer_outputs: Optional[list] = None) -> Optional[torch.Tensor]:
+    def step(self, entries: Sequence[Entry], cache: PagedKVCache, layer_outputs: Optional[list] = None, groups=()) -> Optional[torch.Tensor]:
         """Run the tokens of ``entries`` as one batch; their cache rows must already list blocks for the positions they
         write. Returns the fp32 logits of the wanted tokens in entry order [n_wanted, vocab], or None if nothing is wanted
-        (the K/V of the tokens are stored all the same)."""
+        (the K/V of the tokens are stored all the same). ``groups``: entries of a decode step that share their first blocks (``decode``)."""
         dev = self.model.embed_tokens.device
         if (dev.type == "cuda" and layer_outputs is None and self._graph_decode and entries
                 and all(len(e[2]) == 1 and list(e[3]) == [0] for e in entries)):
-            return self.decode([e[2][0] for e in entries], [e[1] for e in entries], [e[0] for e in entries], cache)
+            return self.decode([e[2][0] for e in entries], [e[1] for e in entries], [e[0] for e in entries], cache, groups)
         ids: List[int] = []
         want: List[int] = []
         runs: List[List[int]] = []
@@ -143,26 +144,32 @@ class RaggedGenerator(Generator):
             max_pos = max(max_pos, pos0 + n - 1)
         if not ids:
             return None
-        # token t of a run is at its first position + (t - its first row): built by numpy, not token by token, and what goes to the device
-        # goes in two copies from pinned memory (a copy from pageable memory waits for the work queued before it)
+        # what goes to the device goes in two copies from pinned memory (a copy from pageable memory waits for the work queued before it); positions,
+        # rows and tiles of the tokens follow from the runs' lengths and are built there
         first, count, start, rows = np.asarray(runs, dtype=np.int64).T
-        meta = torch.from_numpy(np.stack([np.arange(len(ids)) + np.repeat(start - first, count), np.repeat(rows, count)]).astype(np.int32))
         long = torch.from_numpy(np.asarray(ids + (want or [0]), dtype=np.int64))
         if dev.type == "cuda":
-            meta = meta.pin_memory().to(dev, non_blocking=True)
+            lens = torch.from_numpy(np.stack([rows, start, count]).astype(np.int32)).pin_memory().to(dev, non_blocking=True)
             long = long.pin_memory().to(dev, non_blocking=True)
+            nt = int((-(-count // TILE_Q)).sum())
+            m = step_maps(cache.table, lens[0], lens[1], lens[2], cache.block_size, len(ids), n_tiles=nt)
+            pos, slot, pieces = m.pos, m.slot, Pieces(m.tiles, nt, int(count.max()), m.runs, len(runs), m.tile_of, m.run_tiles)
+        else:
+            # token t of a run is at its first position + (t - its first row)
+            meta = torch.from_numpy(np.stack([np.arange(len(ids)) + np.repeat(start - first, count), np.repeat(rows, count)]).astype(np.int32))
+            pos, slot, pieces = meta[0], meta[1], make_pieces(runs, dev)
         ids_t, want_t = long[:len(ids)], long[len(ids):]
-        pieces = make_pieces(runs, dev)
-        logits = self.model.forward_ragged(ids_t, meta[0], meta[1], cache, want_t, max_pos=max_pos, pieces=pieces,
+        logits = self.model.forward_ragged(ids_t, pos, slot, cache, want_t, max_pos=max_pos, pieces=pieces,
                                            layer_outputs=layer_outputs)
         return logits if want else None
 
     @torch.no_grad()
-    def decode(self, tokens: Sequence[int], positions: Sequence[int], rows: Sequence[int], cache: PagedKVCache) -> torch.Tensor:
+    def decode(self, tokens: Sequence[int], positions: Sequence[int], rows: Sequence[int], cache: PagedKVCache, groups=()) -> torch.Tensor:
         """One token per sequence (``tokens[i]`` at ``positions[i]`` of cache row ``rows[i]``), replayed from a CUDA graph: a
         decode step is ~10 short launches per layer, so eager execution is bound by the launch rate. One graph per
         (batch bucket, context bucket, cache); token ids, positions and rows are read from device tensors, padding rows of
-        the bucket write to the cache's scratch row. Returns fp32 logits [len(tokens), vocab]."""
+        the bucket write to the cache's scratch row. ``groups``: up to ``MAX_GROUPS`` of (first sequence, sequences, shared keys) that list the same
+        first blocks, for models whose step takes them (``prefix_groups``). Returns fp32 logits [len(tokens), vocab]."""
         dev = self.model.embed_tokens.device
         n = len(tokens)
         self._check_position(max(positions))
@@ -178,23 +185,29 @@ class RaggedGenerator(Generator):
         # the graphs live on the cache they were captured against (they hold its addresses): they go when it goes, and a new
         # cache that happens to get the old one's id() cannot pick them up
         graphs = cache.__dict__.setdefault("_decode_graphs", {})
-        key = (nb, mp)
+        if groups and not getattr(self.model, "prefix_groups", False):
+            raise ValueError(f"{type(self.model).__name__}: its decode step takes no groups of sequences")
+        key = (nb, mp, "groups") if groups else (nb, mp)
         g = graphs.get(key)
         if g is None:
+            plan = group_plan(nb, mp, dev) if groups else None
+            kw = {"groups": plan} if groups else {}
             st = {"ids": torch.zeros(nb, dtype=torch.long, device=dev), "pos": torch.zeros(nb, dtype=torch.int32, device=dev),
-                  "slot": torch.full((nb,), cache.scratch_row, dtype=torch.int32, device=dev)}
+                  "slot": torch.full((nb,), cache.scratch_row, dtype=torch.int32, device=dev), "plan": plan}
             ensure_graph_workspace(dev)
-            self.model.forward_ragged(st["ids"], st["pos"], st["slot"], cache, None, max_pos=mp - 1)       # warm-up: lazily built buffers
+            self.model.forward_ragged(st["ids"], st["pos"], st["slot"], cache, None, max_pos=mp - 1, **kw)       # warm-up: lazily built buffers
             torch.cuda.synchronize()
             graph = torch.cuda.CUDAGraph()
             with no_gc(), torch.cuda.graph(graph):
-                st["logits"] = self.model.forward_ragged(st["ids"], st["pos"], st["slot"], cache, None, max_pos=mp - 1)
+                st["logits"] = self.model.forward_ragged(st["ids"], st["pos"], st["slot"], cache, None, max_pos=mp - 1, **kw)
             g = graphs[key] = (graph, st)
         graph, st = g
         hd = host.pin_memory().to(dev, non_blocking=True)
         st["ids"].copy_(hd[0])
         st["pos"].copy_(hd[1])
         st["slot"].copy_(hd[2])
+        if groups:
+            set_group_plan(st["plan"], groups)
         graph.replay()
         return st["logits"][:n].clone()          # the graph's output buffer is rewritten by the next replay
 
@@ -224,8 +237,9 @@ class RaggedGenerator(Generator):
         out = input_ids
         done = torch.zeros(B, dtype=torch.bool, device=dev)
         logprobs: List[torch.Tensor] = []
+        rules = logit_rules(cfg, input_ids, logits.shape[1], total)
         for n in range(S, total):
-            nxt = sample_next(logits, cfg, out, gen)
+            nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen)
             if return_logprobs:
                 logprobs.append(logits.float().log_softmax(-1).gather(1, nxt[:, None]).squeeze(1))
             nxt = torch.where(done, torch.full_like(nxt, cfg.pad_token_id), nxt)

@@ -36,6 +36,7 @@ from ..ops.linear import FusedLinear
 from ..ops.moe import ROUTE_SOFTMAX_SELECTED, gated_moe_ffn, route_topk
 from ..ops.norm import sandwich_norm
 from ..ops.paged_attention import paged_attention, rope_paged_store
+from ..ops.prefix_attention import prefix_attention
 
 GELU_SIGMOID_ALPHA = 1.702        # g * sigmoid(1.702 g): the sigmoid approximation of GELU, fixed by the design
 
@@ -163,6 +164,7 @@ class GorozenLayer(nn.Module):
 class GorozenForCausalLM(nn.Module):
     """``forward_ragged`` is the serving step; ``forward(input_ids)`` runs whole sequences through the same step."""
     ragged = True                                   # served by inference.ragged.RaggedGenerator
+    prefix_groups = True                            # decode steps take groups of sequences that share their first blocks
 
     def __init__(self, cfg: GorozenConfig, dtype=torch.bfloat16, device=None, init_std: float = 0.02):
         super().__init__()
@@ -197,11 +199,12 @@ class GorozenForCausalLM(nn.Module):
 
     @torch.no_grad()
     def forward_ragged(self, ids: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor, cache, want: Optional[torch.Tensor] = None,
-                       max_pos: int = 0, pieces=None, layer_outputs: Optional[list] = None) -> torch.Tensor:
+                       max_pos: int = 0, pieces=None, layer_outputs: Optional[list] = None, groups=None) -> torch.Tensor:
         """One serving step over a flat token list: ``ids`` long [T], ``pos`` / ``slot`` int32 [T] (position in its sequence
         and cache row of every token), ``cache`` a ``PagedKVCache`` whose table rows cover those positions. Returns fp32
         logits of the rows ``want`` (long [n]; default all). ``max_pos`` >= every position (host-side bound that sizes the
-        rotary tables). ``layer_outputs``: a list that receives the residual stream after every layer."""
+        rotary tables). ``layer_outputs``: a list that receives the residual stream after every layer. ``groups``: tokens of a decode step whose
+        sequences share their first keys (``ops.prefix_attention.PrefixGroups``), which are then read once for each group."""
         cfg = self.config
         dt = self.embed_tokens.dtype
         eps = cfg.norm_eps
@@ -219,8 +222,12 @@ class GorozenForCausalLM(nn.Module):
                 cos = sin = torch.zeros(1, 1, dtype=torch.float32, device=dev)
             rope_paged_store(qk, cos, sin, pos, slot, cache.k[li], cache.v[li], cache.table, a.heads, a.kv_heads, a.dim,
                              a.rot_dims, interleaved=True, v_from_k=True)
-            ctx = paged_attention(qk, cache.k[li], cache.v[li], cache.table, pos, slot, a.heads, a.kv_heads, a.dim, a.scale,
-                                  sinks=layer.sink, max_pos=max_pos, pieces=pieces)
+            if groups is not None and pieces is None:
+                ctx = prefix_attention(qk, cache.k[li], cache.v[li], cache.table, pos, slot, groups, a.heads, a.kv_heads, a.dim, a.scale,
+                                       sinks=layer.sink, max_pos=max_pos)
+            else:
+                ctx = paged_attention(qk, cache.k[li], cache.v[li], cache.table, pos, slot, a.heads, a.kv_heads, a.dim, a.scale,
+                                      sinks=layer.sink, max_pos=max_pos, pieces=pieces)
             y = linear_exact(ctx, layer.o_proj.weight, out_dtype=torch.float32)
             if layer.spec.mlp is None:
                 h, x = sandwich_norm(y, layer.norm1b, x, nxt, eps, 1.0, dt)

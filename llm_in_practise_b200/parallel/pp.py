@@ -116,6 +116,7 @@ def shard_qwen3_pipeline(model, stages: Optional[int] = None, tp: int = 1, max_t
 class PipelineGenerator(Generator):
     """``Generator`` whose model is one pipeline stage. Same call surface and results; every rank of the grid makes the
     same calls in the same order (serve/tp_engine.py announces rank 0's calls to the others)."""
+    prefix_groups = False
 
     def __init__(self, model, tokenizer=None, max_len: int = 4096):
         super().__init__(model, tokenizer, max_len)

@@ -26,7 +26,8 @@ from typing import Deque, Dict, Iterator, List, Optional, Sequence, Tuple
 
 import torch
 
-from ..inference.generate import GenerationConfig, Generator, KVCache, PagedKVCache, sample_next
+from ..inference.generate import MAX_GROUPS, GenerationConfig, Generator, KVCache, LogitRules, PagedKVCache, sample_next
+from ..ops.logits import MAX_BIAS
 
 
 @dataclass
@@ -51,6 +52,11 @@ class EngineArgs:
     # 07-L1-Cache/LMCache): > 0 keeps the K/V of cached prefixes that lose their HBM row in this many GB of pinned host
     # memory (LRU) and copies them back on a later prefix hit instead of recomputing the prompt
     kv_offload_gb: float = 0.0
+    # decode steps read the K/V blocks that running sequences share (their cached prefix) once for all of them instead of once each; a paged
+    # cache with prefix caching, one GPU. Sums are then in another order: a logit may differ in its last bits. Groups of at least two
+    # sequences and shared_prefix_min keys count
+    shared_prefix_attention: bool = False
+    shared_prefix_min: int = 256
 
 
 @dataclass
@@ -72,6 +78,7 @@ class Request:
     cached_tokens: int = 0                                   # ... of which came from the prefix cache
     aborted: bool = False                                    # set by LLMEngine.abort(): dropped at the next scheduler iteration
     reserved_blocks: int = 0                                 # paged cache: blocks promised to this request but not handed out yet
+    rules_row: int = -1                                      # row of the engine's logit rules that was set up for this request
 
     @property
     def ttft(self) -> Optional[float]:
@@ -192,6 +199,11 @@ class LLMEngine:
         self._host_pin = -1
         self._kv_token_bytes = (self.gen.kv_token_bytes() if self.ragged else
                                 2 * c.num_hidden_layers * c.num_key_value_heads * c.head_dim * self.model.embed_tokens.element_size())
+        self._rules: Optional[LogitRules] = None             # made for the first request with rules on its logits: a row for every slot
+        self._groups_of: Tuple[Optional[tuple], tuple] = (None, ())       # running requests, and the groups among them
+        if self.args.shared_prefix_attention and not (self.paged and self.args.enable_prefix_caching
+                                                      and getattr(self.model if self.ragged else self.gen, "prefix_groups", False)):
+            raise ValueError("shared_prefix_attention needs a paged cache (block_size), prefix caching and a model whose decode step takes groups")
         self._ids = itertools.count()
         self._cv = threading.Condition()
         self._stop = False
@@ -242,6 +254,7 @@ class LLMEngine:
             raise ValueError("empty prompt")
         if len(ids) >= self.args.max_model_len:
             raise ValueError(f"prompt of {len(ids)} tokens does not fit max_model_len={self.args.max_model_len}")
+        cfg.check_rules(self.model.embed_tokens.shape[0])
         if self.paged:
             pool = len(self._block_ref) - 1
             if self._nblocks(len(ids) + 1) > pool:
@@ -362,24 +375,27 @@ class LLMEngine:
 
     def _grow(self, r: Request, n_tokens: int) -> None:
         """Make sure ``r``'s row has blocks for ``n_tokens`` positions (taken out of its reservation)."""
-        blocks = self._slot_blocks.setdefault(r.slot, [])
-        want = self._nblocks(n_tokens)
-        if len(blocks) >= want:
-            return
-        first_new = len(blocks)
-        while len(blocks) < want:
-            if not self._free_blocks:
-                raise RuntimeError("KV block pool exhausted (reservation accounting is broken)")
-            b = self._free_blocks.pop()
-            self._block_ref[b] = 1
-            blocks.append(b)
-            if r.reserved_blocks > 0:
-                r.reserved_blocks -= 1
-                self._reserved -= 1
-        self.gen.set_block_row(self.cache, r.slot, blocks) if first_new == 0 else self._set_row_tail(r.slot, blocks, first_new)
+        self._grow_all([(r, n_tokens)])
 
-    def _set_row_tail(self, slot: int, blocks: List[int], first_new: int) -> None:
-        self.gen.set_block_row(self.cache, slot, blocks)          # rows are short (max_model_len / block_size ints)
+    def _grow_all(self, wanted: Sequence[Tuple[Request, int]]) -> None:
+        """``_grow`` for several requests; the blocks of all of them reach the table in one update."""
+        updates = []
+        for r, n_tokens in wanted:
+            blocks = self._slot_blocks.setdefault(r.slot, [])
+            want, first_new = self._nblocks(n_tokens), len(blocks)
+            while len(blocks) < want:
+                if not self._free_blocks:
+                    raise RuntimeError("KV block pool exhausted (reservation accounting is broken)")
+                b = self._free_blocks.pop()
+                self._block_ref[b] = 1
+                blocks.append(b)
+                if r.reserved_blocks > 0:
+                    r.reserved_blocks -= 1
+                    self._reserved -= 1
+            if len(blocks) > first_new:
+                updates.append((r.slot, first_new, blocks[first_new:]))
+        if updates:
+            self.gen.extend_block_rows(self.cache, updates)
 
     def _unreserve(self, r: Request) -> None:
         self._reserved -= r.reserved_blocks
@@ -567,11 +583,65 @@ class LLMEngine:
             return True
         return False
 
+    def _shared_groups(self, reqs: List[Request]) -> Tuple[tuple, tuple]:
+        """Running requests whose rows list the same first blocks: (the order of ``reqs`` that puts them side by side, (first, number, shared
+        keys) of up to ``MAX_GROUPS`` groups, those that save most). Found anew only when other requests run: a row's shared blocks never change."""
+        if not self.args.shared_prefix_attention or len(reqs) < 2:
+            return (), ()
+        key = tuple((r.rid, r.slot) for r in reqs)
+        if self._groups_of[0] == key:
+            return self._groups_of[1]
+        by_first: Dict[int, List[int]] = {}
+        for i, r in enumerate(reqs):
+            blocks = self._slot_blocks.get(r.slot)
+            if blocks:
+                by_first.setdefault(blocks[0], []).append(i)
+        found = []
+        for members in by_first.values():
+            if len(members) > 1:
+                lists = [self._slot_blocks[reqs[i].slot] for i in members]
+                n = next((j for j, same in enumerate(zip(*lists)) if len(set(same)) > 1), min(map(len, lists)))
+                shared = min(n * self.args.block_size, *(len(reqs[i].prompt_ids) for i in members))
+                if shared >= self.args.shared_prefix_min:
+                    found.append((shared * (len(members) - 1), shared, members))
+        found = sorted(found, key=lambda f: -f[0])[:MAX_GROUPS]
+        order, groups = [], []
+        for _, shared, members in found:
+            groups.append((len(order), len(members), shared))
+            order += members
+        taken = set(order)
+        order += [i for i in range(len(reqs)) if i not in taken]
+        self._groups_of = (key, (tuple(order), tuple(groups)))
+        return self._groups_of[1]
+
+    def _places(self, order: Sequence[int]) -> torch.Tensor:
+        """Where each request is in a batch that was put in this order."""
+        at = [0] * len(order)
+        for place, i in enumerate(order):
+            at[i] = place
+        return torch.tensor(at, device=self.device)
+
+    def _sample_ruled(self, logits: torch.Tensor, reqs: List[Request]) -> List[int]:
+        """Requests with rules on their logits (``GenerationConfig.has_rules``): their rows' rules and histories are on the device."""
+        if self._rules is None:
+            self._rules = LogitRules(self.args.max_num_seqs, logits.shape[1], self.args.max_model_len, self.device, MAX_BIAS)
+        for r in reqs:
+            if r.rules_row != r.slot:
+                r.rules_row = r.slot
+                self._rules.begin(r.slot, r.cfg, r.prompt_ids, r.output_ids, name=r.rid)
+        return self._rules.next(logits, [r.slot for r in reqs], [r.cfg for r in reqs], self._rng).tolist()
+
     def _sample(self, logits: torch.Tensor, reqs: List[Request]) -> List[int]:
         """Per-request sampling parameters: requests sharing a config are sampled together."""
         out = [0] * len(reqs)
+        ruled = [i for i, r in enumerate(reqs) if r.cfg.has_rules()]
+        if ruled:
+            for i, t in zip(ruled, self._sample_ruled(logits if len(ruled) == len(reqs) else logits[ruled], [reqs[i] for i in ruled])):
+                out[i] = t
         groups: Dict[tuple, List[int]] = {}
         for i, r in enumerate(reqs):
+            if r.cfg.has_rules():
+                continue
             c = r.cfg
             groups.setdefault((c.do_sample, c.temperature, c.top_p, c.top_k, c.repetition_penalty), []).append(i)
         for key, idx in groups.items():
@@ -744,8 +814,9 @@ class LLMEngine:
         reqs = self.running
         n = len(reqs)
         if self.paged:
-            for r in reqs:
-                self._grow(r, len(r.prompt_ids) + len(r.output_ids))
+            self._grow_all([(r, len(r.prompt_ids) + len(r.output_ids)) for r in reqs])
+        order, groups = self._shared_groups(reqs)
+        reqs = [reqs[i] for i in order] if groups else reqs
         nb = n
         if self.device.type == "cuda":          # pad to a power-of-two bucket: one captured graph per bucket, not per batch size
             nb = 1
@@ -756,7 +827,11 @@ class LLMEngine:
         last = torch.tensor([r.output_ids[-1] for r in reqs] + [0] * pad, device=self.device)
         pos = torch.tensor([len(r.prompt_ids) + len(r.output_ids) - 1 for r in reqs] + [0] * pad, device=self.device, dtype=torch.int32)
         slots = torch.tensor([r.slot for r in reqs] + [scratch] * pad, device=self.device, dtype=torch.int32)
-        logits = self.gen.decode_graphed(last, self.cache, pos, slots)[:n]
+        if groups:
+            logits = self.gen.decode_graphed(last, self.cache, pos, slots, groups=groups)
+            logits, reqs = logits[self._places(order)], self.running          # back in the order in which requests are sampled
+        else:
+            logits = self.gen.decode_graphed(last, self.cache, pos, slots)[:n]
         toks = self._sample(logits, reqs)
         self.running = [r for r, t in zip(reqs, toks) if not self._emit(r, t)]
         self.metrics.steps += 1
@@ -792,10 +867,10 @@ class LLMEngine:
                 self.metrics.prefix_hits += P
             self.prefilling.append(r)
             budget -= (L - P) if not chunked else min(L - P, budget)
-        entries, owners = [], []
+        entries, owners, grown = [], [], []
         for r in self.running:
             n = len(r.prompt_ids) + len(r.output_ids)
-            self._grow(r, n)
+            grown.append((r, n))
             entries.append((r.slot, n - 1, [r.output_ids[-1]], [0]))
             owners.append(r)
         budget = self.args.max_prefill_tokens
@@ -807,7 +882,7 @@ class LLMEngine:
             if n <= 0:
                 continue
             budget -= n
-            self._grow(r, r.prefilled + n)
+            grown.append((r, r.prefilled + n))
             last = r.prefilled + n >= L
             entries.append((r.slot, r.prefilled, r.prompt_ids[r.prefilled:r.prefilled + n], [n - 1] if last else []))
             r.prefilled += n
@@ -817,7 +892,12 @@ class LLMEngine:
                 owners.append(r)
         if not entries:
             return
-        logits = self.gen.step(entries, self.cache)
+        self._grow_all(grown)
+        order, groups = self._shared_groups(self.running) if len(entries) == len(self.running) else ((), ())
+        if groups and self.device.type == "cuda":
+            logits = self.gen.step([entries[i] for i in order], self.cache, groups=groups)[self._places(order)]
+        else:
+            logits = self.gen.step(entries, self.cache)
         if owners:
             toks = self._sample(logits, owners)
             for r, t in zip(owners, toks):

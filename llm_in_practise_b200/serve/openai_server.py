@@ -43,6 +43,10 @@ class ChatCompletionRequest(BaseModel):
     stream: Optional[bool] = False
     top_k: Optional[int] = 0
     repetition_penalty: Optional[float] = 1.0
+    presence_penalty: Optional[float] = Field(0.0, ge=-2.0, le=2.0)
+    frequency_penalty: Optional[float] = Field(0.0, ge=-2.0, le=2.0)
+    logit_bias: Optional[Dict[str, float]] = None   # OpenAI: token id -> value added to its logit
+    allowed_token_ids: Optional[List[int]] = None   # vLLM: the only tokens that may be generated
     stop: Optional[Union[str, List[str]]] = None    # vLLM / OpenAI stop strings (not in the reference's FastAPI schema)
     ignore_eos: Optional[bool] = False              # vLLM extension (``vllm bench serve --ignore-eos``)
     stream_options: Optional[Dict[str, Any]] = None  # {"include_usage": true}: one more chunk with the token counts
@@ -55,6 +59,10 @@ class CompletionRequest(BaseModel):
     top_p: Optional[float] = 1.0
     max_tokens: Optional[int] = 16
     stream: Optional[bool] = False
+    presence_penalty: Optional[float] = Field(0.0, ge=-2.0, le=2.0)
+    frequency_penalty: Optional[float] = Field(0.0, ge=-2.0, le=2.0)
+    logit_bias: Optional[Dict[str, float]] = None
+    allowed_token_ids: Optional[List[int]] = None
     stop: Optional[Union[str, List[str]]] = None
     ignore_eos: Optional[bool] = False
     stream_options: Optional[Dict[str, Any]] = None
@@ -150,11 +158,15 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         except TypeError:
             return eng.tokenizer.decode(ids)
 
-    def gen_cfg(temperature, top_p, max_tokens, top_k=0, rep=1.0, ignore_eos=False) -> GenerationConfig:
+    def gen_cfg(temperature, top_p, max_tokens, top_k=0, rep=1.0, ignore_eos=False, req=None) -> GenerationConfig:
+        """``req``: the request that rules on logits are taken from (OpenAI's penalties and logit_bias, vLLM's allowed_token_ids)."""
+        rules = {} if req is None else {"presence_penalty": float(req.presence_penalty or 0.0), "frequency_penalty": float(req.frequency_penalty or 0.0),
+                                        "logit_bias": {int(k): float(v) for k, v in (req.logit_bias or {}).items()} or None,
+                                        "allowed_token_ids": req.allowed_token_ids}
         t = 0.0 if temperature is None else float(temperature)
         return GenerationConfig(max_new_tokens=int(max_tokens or 16), do_sample=t > 0.0, temperature=max(t, 1e-5),
                                 top_p=1.0 if top_p is None else float(top_p), top_k=int(top_k or 0),
-                                repetition_penalty=float(rep or 1.0), ignore_eos=bool(ignore_eos))
+                                repetition_penalty=float(rep or 1.0), ignore_eos=bool(ignore_eos), **rules)
 
     def usage_chunk(head, n_p, n_c) -> str:
         return "data: " + json.dumps({**head, "choices": [], "usage": {"prompt_tokens": n_p, "completion_tokens": n_c,
@@ -184,7 +196,7 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         prompt = render(req.messages)
         ids = eng.tokenizer.encode(prompt)
         try:
-            r = eng.submit(ids, gen_cfg(req.temperature, req.top_p, req.max_tokens, req.top_k, req.repetition_penalty, req.ignore_eos))
+            r = eng.submit(ids, gen_cfg(req.temperature, req.top_p, req.max_tokens, req.top_k, req.repetition_penalty, req.ignore_eos, req))
         except ValueError as e:
             raise HTTPException(status_code=400, detail=str(e))
         cid, created = f"chatcmpl-{uuid.uuid4().hex}", int(time.time())
@@ -232,10 +244,10 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         if req.stream and not allow_stream:
             raise HTTPException(status_code=501, detail="Streaming is not yet implemented.")
         prompts = [req.prompt] if isinstance(req.prompt, str) else list(req.prompt)
-        cfg = gen_cfg(req.temperature, req.top_p, req.max_tokens, ignore_eos=req.ignore_eos)
         if req.stream and len(prompts) != 1:
             raise HTTPException(status_code=400, detail="streaming takes one prompt per request")
         try:
+            cfg = gen_cfg(req.temperature, req.top_p, req.max_tokens, ignore_eos=req.ignore_eos, req=req)
             reqs = [eng.submit(eng.tokenizer.encode(p), cfg) for p in prompts]
         except ValueError as e:
             raise HTTPException(status_code=400, detail=str(e))

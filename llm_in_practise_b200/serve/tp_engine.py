@@ -21,7 +21,7 @@ import torch.distributed as dist
 from ..parallel.pp import PipelineGenerator
 from .engine import EngineArgs, LLMEngine
 
-_CALLS = ("_prefill_packed", "_prefill", "_prefill_chunk", "decode_graphed", "copy_prefix", "set_block_row",
+_CALLS = ("_prefill_packed", "_prefill", "_prefill_chunk", "decode_graphed", "copy_prefix", "set_block_row", "extend_block_rows",
           "offload_row", "restore_row", "drop_host_row")
 
 
@@ -68,6 +68,8 @@ class TensorParallelEngine(LLMEngine):
     def __init__(self, model, tokenizer=None, args: Optional[EngineArgs] = None, model_name: str = "b200-model"):
         if not (dist.is_available() and dist.is_initialized()):
             raise RuntimeError("TensorParallelEngine needs an initialised process group (launch with torchrun)")
+        if args is not None and args.shared_prefix_attention:
+            raise ValueError("shared_prefix_attention is for engines on one GPU")
         super().__init__(model, tokenizer, args, model_name)
         self.rank = dist.get_rank()
         if self.rank == 0:
