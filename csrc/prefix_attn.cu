@@ -200,7 +200,7 @@ prefix_shared_mma_kernel(const PrefixParams p) {
 // A CTA owns one token and up to eight query heads of one KV head; its warps take blocks of 16 keys in turn, each with a ring of its own that its
 // first lane refills by TMA (one box per page and 64 dimensions, 128-byte swizzle). On mma.sync: S^T = K Q^T, the keys the first operand and the
 // heads the eight columns, then O^T = V^T P^T with V turned by ldmatrix; P changes sides by movmatrix.
-constexpr int kPxOwn = 16, kPxWarps = 4, kPxStages = 2;
+constexpr int kPxOwn = 16, kPxStages = 2, kPxCluster = 4, kPxClusterWarps = 8 * kPxCluster;
 
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   uint32_t y;
@@ -208,24 +208,25 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   return y;
 }
 
-template <int DK> struct OwnSmem {
+template <int DK, int W> struct OwnSmem {
   static constexpr int kHalves = (DK + 3) / 4, LD = 64 * kHalves + 4;       // LD: floats of a row of O
   static constexpr int kBlock = kHalves * 2048, kStage = 2 * kBlock;        // 16 keys, 16 keys and their values
-  static constexpr int kRing = kPxStages * kStage, kBytes = kPxWarps * kRing + 8 * kPxWarps * kPxStages;
+  static constexpr int kRing = kPxStages * kStage, kBytes = W * kRing + 8 * W * kPxStages;
   static_assert(8 * LD * 4 <= kRing, "a warp's O is joined where its ring was");
 };
 
-template <typename T, int DK>                         // head size = 16 * DK
-__global__ void __launch_bounds__(32 * kPxWarps)
-prefix_own_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PrefixParams p) {
-  using L = OwnSmem<DK>;
+template <typename T, int DK, int W>                  // head size = 16 * DK, warps
+__global__ void __launch_bounds__(32 * W)
+prefix_own_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PrefixParams p, const int cl) {
+  using L = OwnSmem<DK, W>;
   constexpr int D = 16 * DK, LD = L::LD;
   extern __shared__ __align__(1024) uint8_t smem_own[];
-  __shared__ float sml[kPxWarps][8][2], sw[8][kPxWarps + 32], sinv[8];  // of each head: weights of the warps and of up to 32 ranges
+  __shared__ float sml[W][8][2], sw[8][kPxClusterWarps + 32], sinv[8];  // of each head: weights of the cluster's warps and of up to 32 ranges
   const int rep = p.H / p.G, passes = ceil_div(rep, 8);
-  const int t = blockIdx.x, kvh = blockIdx.y / passes, h0 = kvh * rep + (blockIdx.y % passes) * 8, nh = min(8, kvh * rep + rep - h0);
+  // cl CTAs, a cluster, share the keys of a token
+  const int t = blockIdx.x / cl, rank = blockIdx.x % cl, kvh = blockIdx.y / passes, h0 = kvh * rep + (blockIdx.y % passes) * 8, nh = min(8, kvh * rep + rep - h0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t ring = smem_u32(smem_own) + warp * L::kRing, bars = smem_u32(smem_own) + kPxWarps * L::kRing + warp * kPxStages * 8;
+  const uint32_t ring = smem_u32(smem_own) + warp * L::kRing, bars = smem_u32(smem_own) + W * L::kRing + warp * kPxStages * 8;
   if (lane == 0) {
     for (int s = 0; s < kPxStages; ++s) mbar_init(bars + 8 * s, 1);
     fence_mbar_init();
@@ -241,8 +242,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (t >= grp.first && t < grp.first + grp.tokens && k_hi >= grp.shared) { k_lo = grp.shared; used = ranges_used(p, grp.shared); }
   }
   // this warp's blocks: n of them, the i-th at key_at(i). They start at multiples of 16, so that each lies in one page (pages of 8: in two)
-  const int base = (k_lo & ~(kPxOwn - 1)) + warp * kPxOwn, n = base < k_hi ? (k_hi - base + kPxWarps * kPxOwn - 1) / (kPxWarps * kPxOwn) : 0;
-  auto key_at = [&](int i) { return base + i * kPxWarps * kPxOwn; };
+  const int stride = W * cl * kPxOwn, base = (k_lo & ~(kPxOwn - 1)) + (rank * W + warp) * kPxOwn, n = base < k_hi ? (k_hi - base + stride - 1) / stride : 0;
+  auto key_at = [&](int i) { return base + i * stride; };
   const int psl = min(p.bs_log2, 4), pieces = kPxOwn >> psl, pool_rows = (p.n_pages * p.G) << p.bs_log2;
   // Lane x holds the pool row of piece x % pieces of block (first of a set) + x / pieces. A piece behind the token's keys, or on a page outside the
   // pools, is asked for behind the pools' last row: zeros
@@ -352,33 +353,43 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     so[(2 * c + 1) * LD + 16 * i + g + 8] = o[i][3];
   }
   pdl_wait();
-  __syncthreads();
-  for (int hh = warp; hh < nh; hh += kPxWarps) {      // a lane for each range; the first lanes take a warp's part each as well
+  if (cl > 1) cluster_sync_all();
+  else __syncthreads();
+  const int warps = cl * W;                           // up to 32: one to a lane
+  auto of_warp = [&](int w, const void* mine) { return mapa_shared(smem_u32(mine), w / W); };
+  auto load2 = [](uint32_t at) { float2 x; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory"); return x; };
+  auto load4 = [](uint32_t at) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+    return x;
+  };
+  for (int hh = warp; hh < nh; hh += W) {             // a lane for each range and each warp's part
     const long long at = ((long long)t * p.H + h0 + hh) * p.nsplit + lane;
     const float2 ml = lane < used ? *reinterpret_cast<const float2*>(p.part_ml + 2 * at) : make_float2(-INFINITY, 0.f);
-    const float wm = lane < kPxWarps ? sml[lane][hh][0] : -INFINITY, wl = lane < kPxWarps ? sml[lane][hh][1] : 0.f;
+    const float2 own = lane < warps ? load2(of_warp(lane, &sml[lane % W][hh][0])) : make_float2(-INFINITY, 0.f);
     const float sink = p.sinks ? p.sinks[h0 + hh] * kPxLog2e : -INFINITY;
-    const float top = fmaxf(warp_max(fmaxf(ml.x, wm)), sink), e = top == -INFINITY ? 0.f : top;
-    const float w1 = ex2_approx(wm - e), w2 = ex2_approx(ml.x - e);
-    const float total = warp_sum(wl * w1 + ml.y * w2) + ex2_approx(sink - e);
-    if (lane < kPxWarps) sw[hh][lane] = w1;
-    if (lane < used) sw[hh][kPxWarps + lane] = w2;
+    const float top = fmaxf(warp_max(fmaxf(ml.x, own.x)), sink), e = top == -INFINITY ? 0.f : top;
+    const float w1 = ex2_approx(own.x - e), w2 = ex2_approx(ml.x - e);
+    const float total = warp_sum(own.y * w1 + ml.y * w2) + ex2_approx(sink - e);
+    if (lane < warps) sw[hh][lane] = w1;
+    if (lane < used) sw[hh][kPxClusterWarps + lane] = w2;
     if (lane == 0) sinv[hh] = total == 0.f ? 0.f : 1.f / total;      // a row that sees no key is zero
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nh * (D / 4); i += 32 * kPxWarps) {
+  for (int i = rank * (32 * W) + threadIdx.x; i < nh * (D / 4); i += cl * (32 * W)) {
     const int hh = i / (D / 4), d = i % (D / 4) * 4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     auto take = [&](const float4 x, float w) { a.x = fmaf(x.x, w, a.x); a.y = fmaf(x.y, w, a.y); a.z = fmaf(x.z, w, a.z); a.w = fmaf(x.w, w, a.w); };
-#pragma unroll
-    for (int w = 0; w < kPxWarps; ++w) take(*reinterpret_cast<const float4*>(smem_own + w * L::kRing + (hh * LD + d) * 4), sw[hh][w]);
+#pragma unroll 4
+    for (int w = 0; w < warps; ++w) take(load4(of_warp(w, smem_own + (w % W) * L::kRing + (hh * LD + d) * 4)), sw[hh][w]);
     const float4* part = reinterpret_cast<const float4*>(p.part_o + ((long long)t * p.H + h0 + hh) * p.nsplit * D + d);
 #pragma unroll 8
-    for (int r = 0; r < used; ++r) take(part[(long long)r * (D / 4)], sw[hh][kPxWarps + r]);
+    for (int r = 0; r < used; ++r) take(part[(long long)r * (D / 4)], sw[hh][kPxClusterWarps + r]);
     const float inv = sinv[hh];
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + ((long long)t * p.H + h0 + hh) * D + d) =
         make_uint2(pack_pair<T>(a.x * inv, a.y * inv), pack_pair<T>(a.z * inv, a.w * inv));
   }
+  if (cl > 1) cluster_sync_all();                     // its shared memory has been read by the others
 }
 
 template <typename T, int DK>
@@ -394,25 +405,47 @@ static int launch_shared_mma(const PrefixParams& p, dim3 grid, cudaStream_t st) 
 
 // The second kernel starts while the first one ends: it waits for it (griddepcontrol.wait) before it takes up the ranges, its own keys, queries and
 // tables are of launches that were complete when the first one began.
-template <typename T, int DK>
-static int launch_own(const PrefixParams& p, dim3 grid, cudaStream_t st) {
+template <typename T, int DK, int W>
+static int launch_own_by(const PrefixParams& p, dim3 grid, int cl, cudaStream_t st) {
+  using L = OwnSmem<DK, W>;
   // rows of the pools, boxes of 64 dimensions (those behind the head size come as zeros) and up to 16 keys
   const uint64_t dims[2] = {16 * DK, (uint64_t)((p.n_pages * p.G) << p.bs_log2)}, str[1] = {32 * DK};
   const uint32_t box[2] = {64, (uint32_t)(p.bs_log2 < 4 ? 1 << p.bs_log2 : kPxOwn)};
   CUtensorMap tk, tv;
   if (int rc = make_tensor_map(&tk, p.ck, 2, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   if (int rc = make_tensor_map(&tv, p.cv, 2, 2, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-  auto kern = prefix_own_kernel<T, DK>;
+  auto kern = prefix_own_kernel<T, DK, W>;
   // per call: the attribute belongs to the current device, and a process may use several
-  B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnSmem<DK>::kBytes));
+  B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid; cfg.blockDim = dim3(32 * kPxWarps); cfg.dynamicSmemBytes = OwnSmem<DK>::kBytes; cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid; cfg.blockDim = dim3(32 * W); cfg.dynamicSmemBytes = L::kBytes; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  if (cl > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = cl; attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  if (p.n_groups > 0 && p.longest > 0) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = p.n_groups > 0 && p.longest > 0 ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, p);
+  cfg.numAttrs = na;
+  return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, p, cl);
+}
+template <typename T, int DK>
+static int launch_own(const PrefixParams& p, dim3 grid, cudaStream_t st) {
+  // Where there are fewer CTAs than SMs, eight warps to each (four otherwise: then three CTAs fit an SM), and up to four CTAs to a token, while each warp has
+  // two blocks. 32 / 8 heads of 128, own keys of up to 3000 for 2 tokens 37.9 -> 12.9 us (with eight CTAs to a token 21.9), of 2000 for 8 30.7 -> 21.5; 16 / 4
+  // heads, 8000 keys for 4 tokens 99 -> 22; 64 tokens by eight warps 29.7 -> 37.5, 4 tokens with 40 keys 7.7 -> 7.9.
+  const long long ctas = (long long)grid.x * grid.y;
+  if (ctas > kNumSMs || p.most_own <= 256) return launch_own_by<T, DK, 4>(p, grid, 1, st);
+  int cl = 1;
+  while (cl < kPxCluster && ctas * cl * 2 <= kNumSMs && p.most_own >= 256 * cl) cl *= 2;
+  grid.x *= cl;
+  return launch_own_by<T, DK, 8>(p, grid, cl, st);
 }
 
 template <typename T>
@@ -467,7 +500,7 @@ B200_API int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_sha
 
 B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const void* cv, int n_pages, const int* pos, const int* slot,
                               const int* table, long long table_stride, int table_rows, int width, const int* groups, const int* of, int n_groups,
-                              int longest, const float* sinks, void* out, float* part, int plan, int T, int H, int G, int D, int block_size,
+                              int longest, const float* sinks, void* out, float* part, int plan, int most_own, int T, int H, int G, int D, int block_size,
                               float scale, int dtype, void* stream) {
   if (T <= 0) return 0;
   if ((dtype != B200_DT_BF16 && dtype != B200_DT_FP16) || D % 16 || D < 16 || D > 128 || !(scale > 0.f)) return B200_ERR_UNSUPPORTED;
@@ -487,6 +520,7 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
   p.table_rows = table_rows; p.width = width; p.n_pages = n_pages; p.groups = groups; p.of = of; p.n_groups = n_groups;
   p.longest = longest; p.sinks = sinks; p.out = out; p.T = T; p.H = H; p.G = G; p.D = D; p.nsplit = nsplit;
   p.part_o = part; p.part_ml = part ? part + (long long)T * H * nsplit * D : nullptr;
+  p.most_own = most_own > 0 ? most_own : 0x7fffffff;
   p.scale_log2 = scale * kPxLog2e;
   return dtype == B200_DT_BF16 ? prefix_attn<__nv_bfloat16>(p, tc, (cudaStream_t)stream) : prefix_attn<__half>(p, tc, (cudaStream_t)stream);
 }

@@ -759,14 +759,15 @@ int b200_moe_gather(const void* h, const long long* dest, const long long* tok, 
  * tokens, shared keys, -): consecutive tokens whose sequences hold the same first keys; those are read once, from the first token's row. of
  * int32 [T]: the group of a token, -1 for none. longest: tokens of the largest group. sinks fp32 [H] or NULL: a logit per head that only takes
  * part in the sum. plan = b200_prefix_attn_plan(...), or any number of ranges of the shared keys (1 .. 32), plus 256
- * for the tcgen05 kernel (D 64 or 128, at most 128 heads to a KV head); part: fp32 [T * H * (plan % 256) * (D + 2)] scratch. Pools [n_pages, G, block_size, D];
+ * for the tcgen05 kernel (D 64 or 128, at most 128 heads to a KV head); part: fp32 [T * H * (plan % 256) * (D + 2)] scratch.
+ * most_own: keys behind the shared ones that a token has, at most (0: not known); it only chooses how they are cut. Pools [n_pages, G, block_size, D];
  * 16-bit types, D a multiple of 16 up to 128, block_size a power of two from 8 on, n_pages * G * block_size below 2^31 - 256, scale > 0.
  * A token with pos < 0, or a slot outside the table, sees no key:
  * zero. Pages outside the pools are not read. */
 int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int H, int G, int D);
 int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const void* cv, int n_pages, const int* pos, const int* slot,
                      const int* table, long long table_stride, int table_rows, int width, const int* groups, const int* of, int n_groups,
-                     int longest, const float* sinks, void* out, float* part, int plan, int T, int H, int G, int D, int block_size,
+                     int longest, const float* sinks, void* out, float* part, int plan, int most_own, int T, int H, int G, int D, int block_size,
                      float scale, int dtype, void* stream);
 
 /* Block tables and maps of a serving step (csrc/step_maps.cu), from the requests' lengths on the device: rows, cached, lens / fresh int32 [n]

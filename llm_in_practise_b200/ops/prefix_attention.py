@@ -19,20 +19,21 @@ from . import _native as nv
 from .paged_attention import paged_attention
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-_ARGS = [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, i32, vp]
+_ARGS = [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp]
 
 
 @dataclass
 class PrefixGroups:
     """Which tokens of a step share their first keys. ``groups`` int32 [n_groups, 4] = (first token, tokens, shared keys, 0); ``of`` int32
     [tokens]: the group of every token, -1 for none. ``longest`` (tokens of the largest group) and ``max_shared`` (shared keys of the group with
-    the most) are bounds known on the host; a plan that a captured graph replays may be rewritten on the device within them: tokens of a
-    group behind the ``longest``-th read all their keys by themselves, and ``max_shared`` only chooses how the work is cut."""
+    the most) are bounds known on the host, ``min_shared`` what every token shares at least; a plan that a captured graph replays may be rewritten on the device within them: tokens of a
+    group behind the ``longest``-th read all their keys by themselves, and the last two only choose how the work is cut."""
     groups: torch.Tensor
     of: torch.Tensor
     n_groups: int
     longest: int
     max_shared: int
+    min_shared: int = 0
 
 
 def make_prefix_groups(groups: Sequence[Sequence[int]], tokens: int, device) -> PrefixGroups:
@@ -52,7 +53,7 @@ def make_prefix_groups(groups: Sequence[Sequence[int]], tokens: int, device) -> 
     dev = torch.device(device)
     host = host.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else host
     return PrefixGroups(host[:4 * len(rows)].view(-1, 4), host[4 * len(rows):], len(rows), max((r[1] for r in rows), default=0),
-                        max((r[2] for r in rows), default=0))
+                        max((r[2] for r in rows), default=0), min((r[2] for r in rows), default=0) if -1 not in of else 0)
 
 
 def _ints(device, **tensors):
@@ -68,7 +69,7 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     window), with the shared keys of ``groups`` read once. Tokens of a group whose position is before its last shared key, and tokens of no
     group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. Caches of 16 bits with head sizes that
     are multiples of 16 up to 128, pages of a power of two from 8 on (fewer than 2^31 - 256 rows of a pool in all) and a positive scale; others go through ``paged_attention``, as does a step without
-    groups. Captured into a graph, each call keeps a workspace of its own. ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it
+    groups. ``max_pos``: an upper bound of ``pos`` known on the host (0: unknown). Captured into a graph, each call keeps a workspace of its own. ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it
     (include/b200_ops.h); 0: chosen by the sizes."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
     BS, dt = cache_k.shape[2], q.dtype
@@ -95,6 +96,6 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     fn = nv.proto("b200_prefix_attn", _ARGS)
     nv.check(nv.call_on(dev, fn, q_ptr, stride[0], cache_k.data_ptr(), cache_v.data_ptr(), pools[0], pos.data_ptr(), slot.data_ptr(), table.data_ptr(),
                         table.stride(0), *table.shape, groups.groups.data_ptr(), groups.of.data_ptr(), groups.n_groups, groups.longest, nv.ptr(sinks),
-                        out.data_ptr(), part.data_ptr(), plan, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
+                        out.data_ptr(), part.data_ptr(), plan, max(1, max_pos + 1 - groups.min_shared) if max_pos else 0, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
     nv.count_launch(2)
     return out
