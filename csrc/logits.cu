@@ -14,8 +14,8 @@
 //
 // Bound: memory. 128 x 151936 in 32 bits, histories of up to 6000 tokens, 300 biases, half of the rows masked (158 MB): 24 us; here 52, 30 of them the second
 // kernel (29 in all without histories) and the rest the first: 4800 single logits of a row lie in half of the memory of its 152 000. One
-// kernel with the counts of a slice in shared memory was kept waiting by its own steps (rules, history, counts, logits): 100 us in slices of 4096
-// tokens, 69 to 78 in slices of 20480 with the history counted once for clusters of 2 to 8 CTAs (8 rows: 8.8 and 6.5 us, here 9.7). The rules applied in
+// kernel with the counts of a slice in shared memory is kept waiting by its own steps (rules, history, counts, logits): 100 us in slices of 4096
+// tokens (which small batches keep, see kLmSlices), 69 to 78 in slices of 20480 with the history counted once for clusters of 2 to 8 CTAs (8 rows: 8.8 and 6.5 us, here 9.7). The rules applied in
 // the second kernel, from records in token order, took 64: almost every warp had a lane with one.
 #include "common.cuh"
 #include "../include/b200_ops.h"
@@ -377,9 +377,75 @@ logits_stream_kernel(const T* x, long long ldx, int V, const int* __restrict__ m
   }
 }
 
+// Small batches: one kernel, a CTA for a slice of kLmTokens tokens of a row, its counts and biases in shared memory. Every slice goes through the whole history.
+constexpr int kLmTokens = 4096, kLmSlices = 800;
+template <typename T, bool GREEDY>
+__global__ void __launch_bounds__(256)
+logits_small_kernel(const T* x, long long ldx, int V, const LogitRules L, float* out, long long ldo, unsigned long long* __restrict__ best) {
+  __shared__ uint32_t word[kLmTokens];
+  __shared__ unsigned long long red[8];
+  const int b = blockIdx.y, v0 = blockIdx.x * kLmTokens, nv = min(kLmTokens, V - v0), tid = threadIdx.x;
+  const T* xr = x + (long long)b * ldx + v0;
+  constexpr int kEach = kLmTokens / 256;
+  T l[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (tid + i * 256 < nv) l[i] = xr[tid + i * 256];
+  for (int i = tid; i < kLmTokens; i += 256) word[i] = 0;
+  const int row = L.slot ? L.slot[b] : b;
+  RowRules R = {1.f, 0.f, 0.f, 1.f, 1.f, 0, 0, 0, false};
+  const long long r0 = (unsigned)row < (unsigned)L.rows ? row : 0;
+  if ((unsigned)row < (unsigned)L.rows) R = row_rules(L, row);
+  const float* values = L.bias_values + r0 * L.bias_width;
+  const int* mask = R.masked ? L.mask + r0 * L.words + (v0 >> 5) : nullptr;
+  if (R.n_hist > 0 || R.n_bias > 0) {
+    __syncthreads();
+    if (R.n_bias > 0) {                                       // while the words hold nothing else: the last bias of a token is the largest
+      const int* ids = L.bias_ids + r0 * L.bias_width;
+      for (int i = tid; i < R.n_bias; i += 256) {
+        const int v = ids[i] - v0;
+        if ((unsigned)v < (unsigned)nv) atomicMax(word + v, (uint32_t)(i + 1) << kLgBias);
+      }
+      __syncthreads();
+    }
+    const int* hist = L.tokens + r0 * L.width;
+#pragma unroll 4
+    for (int i = tid; i < R.n_hist; i += 256) {
+      const int v = hist[i] - v0;
+      if ((unsigned)v >= (unsigned)nv) continue;
+      if (i < R.n_prompt) atomicOr(word + v, kLgSeen);
+      else atomicAdd(word + v, 1u);
+    }
+  }
+  __syncthreads();
+  unsigned long long mine = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int at = tid + i * 256;
+    if (at >= nv) break;
+    float y = to_f32<T>(l[i]);
+    const uint32_t w = word[at];
+    y = w ? apply_word(y, R, w, values) : quotient(y, R.T, R.inv_T);
+    if (mask && !(mask[at >> 5] >> (at & 31) & 1)) y = -INFINITY;
+    if (GREEDY) mine = max(mine, rank_of(y, v0 + at));
+    else out[(long long)b * ldo + v0 + at] = y;
+  }
+  if (GREEDY) {
+    pdl_launch_dependents();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if ((tid & 31) == 0) red[tid >> 5] = mine;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < 8; ++w) mine = max(mine, red[w]);
+      best[(long long)b * gridDim.x + blockIdx.x] = mine;
+    }
+  }
+}
+
 // the best of a row's CTAs: a warp to a row
 __global__ void __launch_bounds__(128) greedy_pick_kernel(const unsigned long long* __restrict__ best, int parts, long long* __restrict__ ids, int B) {
-  pdl_wait();                                                 // (the first kernel too: the second one waited for it)
+  pdl_wait();
   const int b = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (b >= B) return;
   unsigned long long m = 0;
@@ -423,7 +489,22 @@ static int launch_logits_as(const void* x, long long ldx, int B, int V, const Lo
   RowPlan* plan = (RowPlan*)work;
   uint32_t* bitmap = (uint32_t*)(plan + B);
   unsigned long long* best = GREEDY ? (unsigned long long*)(bitmap + (long long)B * bitmap_words(V)) : nullptr;
-  const int parts = ceil_div(V, kLgTokens);
+  const int parts = ceil_div(V, kLgTokens), slices = ceil_div(V, kLmTokens);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // Up to so many slices one kernel is faster: 8 x 151936, histories of 1500: 7.2 us on the device against 9.6 (and a launch less for the host), 16 rows 8.2
+  // against 11.1, 24 rows (912 slices) 12.4 against 13.8, but greedy 17.3 against 15.9; 48 rows 20.6 against 18.5, 128 with all rules 100 against 52
+  if ((long long)B * slices <= kLmSlices) {
+    logits_small_kernel<T, GREEDY><<<dim3(slices, B), 256, 0, st>>>((const T*)x, ldx, V, L, out, ldo, best);
+    B200_LAUNCH_CHECK();
+    if (!GREEDY) return 0;
+    cfg.gridDim = dim3(ceil_div(B, 4)); cfg.blockDim = dim3(128); cfg.stream = st;
+    return (int)cudaLaunchKernelEx(&cfg, greedy_pick_kernel, (const unsigned long long*)best, slices, ids, B);
+  }
   int slots = 256;                                            // no larger than twice what a row may hold
   while (slots < kLsSlots && slots / 2 < L.width + L.bias_width) slots *= 2;
   const size_t smem = (size_t)slots * 10 + bitmap_words(V) * 4;      // 224 KB at most
@@ -432,12 +513,6 @@ static int launch_logits_as(const void* x, long long ldx, int B, int V, const Lo
   if (smem > 48 * 1024) B200_CHECK(cudaFuncSetAttribute(settle, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   settle<<<B, kLsThreads, smem, st>>>((const T*)x, ldx, V, L, out, ldo, plan, bitmap, best, parts, slots);
   B200_LAUNCH_CHECK();
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   cfg.gridDim = dim3(parts, B); cfg.blockDim = dim3(kLgThreads); cfg.stream = st;
   B200_CHECK(cudaLaunchKernelEx(&cfg, logits_stream_kernel<T, GREEDY>, (const T*)x, ldx, V, L.mask, L.words, out, ldo, (const RowPlan*)plan, (const uint32_t*)bitmap, best, parts));
   if (!GREEDY) return 0;

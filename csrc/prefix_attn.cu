@@ -383,8 +383,15 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll 4
     for (int w = 0; w < warps; ++w) take(load4(of_warp(w, smem_own + (w % W) * L::kRing + (hh * LD + d) * 4)), sw[hh][w]);
     const float4* part = reinterpret_cast<const float4*>(p.part_o + ((long long)t * p.H + h0 + hh) * p.nsplit * D + d);
-#pragma unroll 8
-    for (int r = 0; r < used; ++r) take(part[(long long)r * (D / 4)], sw[hh][kPxClusterWarps + r]);
+    for (int r0 = 0; r0 < used; r0 += 8) {            // eight at a time, the last ones too: one after another each is a wait of its own
+      float4 x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r0 + r < used) x[r] = part[(long long)(r0 + r) * (D / 4)];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r0 + r < used) take(x[r], sw[hh][kPxClusterWarps + r0 + r]);
+    }
     const float inv = sinv[hh];
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + ((long long)t * p.H + h0 + hh) * D + d) =
         make_uint2(pack_pair<T>(a.x * inv, a.y * inv), pack_pair<T>(a.z * inv, a.w * inv));

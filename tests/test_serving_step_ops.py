@@ -221,6 +221,17 @@ def state_of(rows, V, max_len, device, max_bias=8):
     return st
 
 
+def both(x, st, slot=None):
+    """process_logits and greedy_tokens of a batch, and of one so large (the same rows again and again) that another kernel takes it: the same."""
+    y, ids = process_logits(x, st, slot), greedy_tokens(x, st, slot)
+    k = 801 // (x.shape[0] * -(-x.shape[1] // 4096)) + 1
+    again = (torch.arange(x.shape[0], dtype=torch.int32, device=x.device) if slot is None else slot).repeat(k)
+    ys, more = process_logits(x.repeat(k, 1), st, again).view(k, *y.shape), greedy_tokens(x.repeat(k, 1), st, again).view(k, -1)
+    assert torch.equal(torch.isnan(ys), torch.isnan(y).expand_as(ys)) and torch.equal(ys.nan_to_num(7.0), y.nan_to_num(7.0).expand_as(ys))
+    assert torch.equal(more, ids.expand_as(more))
+    return y, ids
+
+
 def check_rules(got, want, bound):
     got = got.double().cpu()
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got == -INF, want == -INF) and torch.equal(got == INF, want == INF)
@@ -242,7 +253,8 @@ def test_rules_on_logits(device, V, B, dtype):
         want, bound = exact_rules(x, rows)
         y = process_logits(x.to(device) if x.is_contiguous() else wide.to(device)[:, x.storage_offset():x.storage_offset() + V], st)
         check_rules(y, want, bound)
-        assert torch.equal(greedy_tokens(x.to(device), st).cpu(), y.argmax(1).cpu())
+        same, ids = both(x.to(device), st)
+        assert torch.equal(same, y) and torch.equal(ids.cpu(), y.argmax(1).cpu())
 
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
@@ -254,9 +266,9 @@ def test_rules_go_by_slot(device):
     slot = [8, 2, 2, -1, 9, 0, 6, 2 ** 31 - 1]
     x = torch.randn(len(slot), V) * 3
     want, bound = exact_rules(x, [rows[s] if 0 <= s < 9 else None for s in slot])
-    y = process_logits(x.to(device), st, i32(slot, device))
+    y, ids = both(x.to(device), st, i32(slot, device))
     check_rules(y, want, bound)
-    assert torch.equal(y[3].cpu(), x[3]) and torch.equal(greedy_tokens(x.to(device), st, i32(slot, device)).cpu(), y.argmax(1).cpu())
+    assert torch.equal(y[3].cpu(), x[3]) and torch.equal(ids.cpu(), y.argmax(1).cpu())
 
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
@@ -276,10 +288,11 @@ def test_nan_and_infinity_in_logits(device, dtype):
     x[6, :2] = -1.0
     rows = [dict(allowed=range(200, 5000))] + [dict(repetition_penalty=1.5, prompt=[1])] + [None] * 5
     st = state_of(rows, V, 8, device)
-    y = process_logits(x.to(device), st).cpu()
+    y, ids = both(x.to(device), st)
+    y = y.cpu()
     assert not torch.isnan(y[0]).any() and (y[0] == -INF).sum() == V - 4800 and (y[0, 200:5000] == 0).all()
     assert torch.isnan(y[1]).sum() == 1 and y[1, 50] == INF and torch.equal(y[2:], x[2:].float())
-    assert greedy_tokens(x.to(device), st).tolist() == [200, 7000, 4000, 0, 0, 0, 2] == y.argmax(1).tolist()[:4] + [0, 0, 2]
+    assert ids.tolist() == [200, 7000, 4000, 0, 0, 0, 2] == y.argmax(1).tolist()[:4] + [0, 0, 2]
 
 
 @pytest.mark.parametrize("device", CPU_AND_GPU)
@@ -287,7 +300,7 @@ def test_masked_to_nothing_and_all_allowed(device):
     V = 12345
     st = state_of([dict(allowed=[]), dict(allowed=range(V)), dict(allowed=[V - 1]), dict(allowed=[0])], V, 4, device)
     x = torch.randn(4, V)
-    y = process_logits(x.to(device), st).cpu()
+    y = both(x.to(device), st)[0].cpu()
     assert (y[0] == -INF).all() and torch.equal(y[1], x[1]) and greedy_tokens(x.to(device), st).tolist()[0] == 0
     assert greedy_tokens(x.to(device), st).tolist()[2:] == [V - 1, 0] and (y[2] == -INF).sum() == V - 1
     st.set_mask(0, None)
@@ -303,7 +316,7 @@ def test_biases_that_name_a_token_twice(device):
     st.bias_values[0, :300] = torch.arange(300, dtype=torch.float32, device=device)
     st.bias_length[0] = 300
     st.bias_ids[1, :3], st.bias_values[1, :3], st.bias_length[1] = i32([V, -1, 5], device), torch.tensor([9.0, 9.0, 2.0], device=device), 9999
-    y = process_logits(torch.zeros(2, V, device=device), st).cpu()
+    y = both(torch.zeros(2, V, device=device), st)[0].cpu()
     assert y[0, :7].tolist() == [float(max(i for i in range(300) if i % 7 == t)) for t in range(7)] and (y[0, 7:] == 0).all()
     assert y[1, 5] == 2.0 and y[1].count_nonzero() == 1          # ids outside the vocabulary are passed over, as are entries of id 0 and value 0
 
@@ -320,9 +333,9 @@ def test_long_histories(device, V, n):
     x = torch.randn(2, V, generator=g) * 3
     said = [collections.Counter(r.get("output", ())) for r in rows]
     want, bound = exact_counts(x, rows, said)
-    y = process_logits(x.to(device), st)
+    y, ids = both(x.to(device), st)
     check_rules(y, want, bound)
-    assert torch.equal(greedy_tokens(x.to(device), st).cpu(), y.argmax(1).cpu())
+    assert torch.equal(ids.cpu(), y.argmax(1).cpu())
 
 
 def exact_counts(x, rows, said):
@@ -372,6 +385,10 @@ def test_logits_in_place(device):
     y = x.clone().to(device)
     assert process_logits(y, st, out=y) is y
     check_rules(y, *exact_rules(x, rows))
+    slot = torch.arange(7, dtype=torch.int32, device=device).repeat(60)
+    many = x.repeat(60, 1).to(device)
+    process_logits(many, st, slot, out=many)
+    assert torch.equal(many.view(60, 7, V), y.expand(60, 7, V))
     assert process_logits(x[:0].to(device), st).shape == (0, V) and greedy_tokens(x[:0].to(device), st).shape == (0,)
 
 
