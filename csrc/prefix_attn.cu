@@ -513,7 +513,8 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
   if ((dtype != B200_DT_BF16 && dtype != B200_DT_FP16) || D % 16 || D < 16 || D > 128 || !(scale > 0.f)) return B200_ERR_UNSUPPORTED;
   const bool tc = plan >= kPxTc;
   const int nsplit = tc ? plan - kPxTc : plan;
-  if (H < 1 || G < 1 || H % G || n_pages < 0 || table_rows < 1 || width < 1 || n_groups < 0 || nsplit < 1 || nsplit > 32 || block_size < 1) return B200_ERR_BAD_SHAPE;
+  if (H < 1 || G < 1 || H % G || n_pages < 0 || table_rows < 1 || width < 1 || n_groups < 0 || nsplit < 1 || nsplit > 32 || block_size < 1 ||
+      q_stride < (long long)H * D) return B200_ERR_BAD_SHAPE;
   if (n_groups > 65535 || (long long)G * ceil_div64((int64_t)(longest < 1 ? 1 : longest) * (H / G), kPxRows) > 65535 || H > 65535) return B200_ERR_TOO_LARGE;
   if (q_stride % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(ck) | reinterpret_cast<uintptr_t>(cv) |
                         reinterpret_cast<uintptr_t>(part)) & 15)) return B200_ERR_BAD_ALIGN;

@@ -20,6 +20,8 @@ import torch
 from . import _native as nv
 
 vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+_PROCESS_ARGS = [vp, i64, i32, i32, vp, vp, vp, vp, i64, i32, vp]
+_GREEDY_ARGS = [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp]
 MAX_VOCAB = 1 << 19
 MAX_BIAS = 2047          # biases of one row
 MAX_HISTORY = (1 << 20) - 1      # tokens of one row's history
@@ -58,7 +60,7 @@ class LogitState:
         self.device = self.tokens.device
 
     def allow_masks(self) -> "LogitState":
-        """Room for a mask a row (all of them off)."""
+        """Room for a mask a row (all of them off). A graph captured before there is room applies no masks."""
         if self.mask is None:
             self.mask = torch.zeros(self.rows, self.words, dtype=torch.int32, device=self.device)
             self.masked = torch.zeros(self.rows, dtype=torch.bool, device=self.device)
@@ -151,15 +153,16 @@ def process_logits(logits: torch.Tensor, state: LogitState, slot: Optional[torch
     nothing is all minus infinity."""
     _check("process_logits", logits, state, slot)
     if out is None:
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-    elif out.dtype != torch.float32 or out.shape != logits.shape or out.device != logits.device or out.stride(1) != 1:
-        raise ValueError("process_logits: out must be fp32, like the logits in shape, with contiguous rows")
+        out = logits.new_empty(logits.shape, dtype=torch.float32)
+    elif (out.dtype != torch.float32 or out.shape != logits.shape or out.device != logits.device or (out.stride(1) != 1 and state.vocab > 1)
+          or (out.stride(0) < state.vocab and out.shape[0] > 1)):
+        raise ValueError("process_logits: out must be fp32, like the logits in shape, with contiguous rows, each of its own")
     if not nv.use_native(logits):
         return out.copy_(_rules_torch(logits, state, slot))
     if logits.shape[0] == 0:
         return out
     work = _workspace(state, logits.shape[0], 0)
-    fn = nv.proto("b200_process_logits", [vp, i64, i32, i32, vp, vp, vp, vp, i64, i32, vp])
+    fn = nv.proto("b200_process_logits", _PROCESS_ARGS)
     nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), logits.shape[0], state.vocab, nv.ptr(slot), state._address(),
                         work.data_ptr(), out.data_ptr(), out.stride(0), nv.dtype_code(logits.dtype)), "process_logits")
     nv.count_launch(2)
@@ -172,7 +175,7 @@ def _workspace(state, B, greedy):
         fn = nv.lib().b200_logits_workspace
         fn.argtypes, fn.restype = [i32] * 3, i64
         size = state._work[B, greedy] = fn(B, state.vocab, greedy)
-    return torch.empty(size, dtype=torch.uint8, device=state.device)
+    return state.tokens.new_empty(size, dtype=torch.uint8)
 
 
 def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -182,11 +185,11 @@ def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.
     if not nv.use_native(logits):
         return _rules_torch(logits, state, slot).argmax(1)
     B = logits.shape[0]
-    ids = torch.empty(B, dtype=torch.int64, device=logits.device)
+    ids = logits.new_empty(B, dtype=torch.int64)
     if B == 0:
         return ids
     work = _workspace(state, B, 1)
-    fn = nv.proto("b200_greedy_tokens", [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp])
+    fn = nv.proto("b200_greedy_tokens", _GREEDY_ARGS)
     nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), B, state.vocab, nv.ptr(slot), state._address(), work.data_ptr(),
                         ids.data_ptr(), nv.dtype_code(logits.dtype)), "greedy_tokens")
     nv.count_launch(3)

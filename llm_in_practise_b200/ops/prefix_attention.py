@@ -19,15 +19,16 @@ from . import _native as nv
 from .paged_attention import paged_attention
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_PLAN_ARGS = [i32] * 7
 _ARGS = [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp]
 
 
 @dataclass
 class PrefixGroups:
-    """Which tokens of a step share their first keys. ``groups`` int32 [n_groups, 4] = (first token, tokens, shared keys, 0); ``of`` int32
-    [tokens]: the group of every token, -1 for none. ``longest`` (tokens of the largest group) and ``max_shared`` (shared keys of the group with
-    the most) are bounds known on the host, ``min_shared`` what every token shares at least; a plan that a captured graph replays may be rewritten on the device within them: tokens of a
-    group behind the ``longest``-th read all their keys by themselves, and the last two only choose how the work is cut."""
+    """Which tokens of a step share their first keys. ``groups`` int32 [n_groups, 4] = (first token, tokens, shared keys, 0); ``of`` int32 [tokens]:
+    the group of every token, -1 for none. Bounds known on the host: ``longest`` (tokens of the largest group), ``max_shared`` and ``min_shared`` (shared
+    keys of the group with the most; what every token of the step shares at least). A plan that a captured graph replays may be rewritten
+    on the device: tokens of a group behind the ``longest``-th read all their keys by themselves, the other two only choose how the work is cut."""
     groups: torch.Tensor
     of: torch.Tensor
     n_groups: int
@@ -38,7 +39,8 @@ class PrefixGroups:
 
 def make_prefix_groups(groups: Sequence[Sequence[int]], tokens: int, device) -> PrefixGroups:
     """The plan of a step of ``tokens`` tokens from its groups ``(first token, tokens, shared keys)``: runs of consecutive tokens, none of them in
-    two groups, whose sequences hold the same keys and values at positions ``0 .. shared - 1`` (in the same pages, or in copies)."""
+    two groups, whose sequences hold the same keys and values at positions ``0 .. shared - 1`` (in the same pages, or in copies). They are read
+    from the pages that the group's first token lists."""
     rows, of = [], [-1] * tokens
     for first, n, shared in ([int(v) for v in g] for g in groups):
         if n < 0 or shared < 0 or first < 0 or first + n > tokens:
@@ -56,21 +58,17 @@ def make_prefix_groups(groups: Sequence[Sequence[int]], tokens: int, device) -> 
                         max((r[2] for r in rows), default=0), min((r[2] for r in rows), default=0) if -1 not in of else 0)
 
 
-def _ints(device, **tensors):
-    for name, (t, shape) in tensors.items():
-        if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-            raise ValueError(f"prefix_attention: {name} must be a contiguous int32 {list(shape)} tensor on the queries' device")
-
-
 def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, table: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
                      groups: Optional[PrefixGroups], n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                      sinks: Optional[torch.Tensor] = None, max_pos: int = 0, plan: int = 0) -> torch.Tensor:
     """Context [T, H * D] of token t over keys ``0 .. pos[t]`` of cache row ``slot[t]``, as ``paged_attention`` gives it (same arguments; no
     window), with the shared keys of ``groups`` read once. Tokens of a group whose position is before its last shared key, and tokens of no
-    group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. Caches of 16 bits with head sizes that
-    are multiples of 16 up to 128, pages of a power of two from 8 on (fewer than 2^31 - 256 rows of a pool in all) and a positive scale; others go through ``paged_attention``, as does a step without
-    groups. ``max_pos``: an upper bound of ``pos`` known on the host (0: unknown). Captured into a graph, each call keeps a workspace of its own. ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it
-    (include/b200_ops.h); 0: chosen by the sizes."""
+    group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. ``max_pos``: an upper bound of ``pos`` known on the host
+    (0: unknown). ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it (include/b200_ops.h); 0: chosen by the sizes.
+
+    For caches of 16 bits with head sizes that are multiples of 16 up to 128, pages of a power of two from 8 on (fewer than 2^31 - 256 rows of a
+    pool in all) and a positive scale; others go through ``paged_attention``, as does a step without groups. Captured into a graph, each
+    call keeps a workspace of its own."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
     BS, dt = cache_k.shape[2], q.dtype
     if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or (dt is not torch.bfloat16 and dt is not torch.float16) or D % 16 or D > 128
@@ -82,20 +80,24 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     if not cache_k.is_contiguous() or not cache_v.is_contiguous() or cache_k.device != dev or cache_v.device != dev:
         raise ValueError("prefix_attention: caches must be contiguous and on the queries' device")
     q_ptr, stride = q.data_ptr(), q.stride()
-    if H % G or len(stride) != 2 or q.shape[1] < H * D or (T and stride[1] != 1) or stride[0] % 8 or q_ptr % 16:
-        raise ValueError(f"prefix_attention: queries must be rows of {H * D} or more contiguous values that start on 16 bytes")
+    row = stride[0] if T > 1 else H * D
+    if H % G or len(stride) != 2 or q.shape[1] < H * D or (T and stride[1] != 1) or row < H * D or row % 8 or q_ptr % 16:
+        raise ValueError(f"prefix_attention: queries must be rows of {H * D} or more contiguous values that start on 16 bytes, each of its own")
     if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev or (table.stride(1) != 1 and table.shape[1] > 1):
         raise ValueError("prefix_attention: the block table is int32 [rows, blocks] with contiguous rows on the queries' device")
     if sinks is not None and (sinks.dtype is not torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous() or sinks.device != dev):
         raise ValueError(f"prefix_attention: sinks must be contiguous fp32 [{H}] on the queries' device")
-    _ints(dev, pos=(pos, (T,)), slot=(slot, (T,)), of=(groups.of, (T,)), groups=(groups.groups, (groups.n_groups, 4)))
+    of, rows, n_groups, tokens = groups.of, groups.groups, groups.n_groups, (T,)
+    for t, shape in ((pos, tokens), (slot, tokens), (of, tokens), (rows, (n_groups, 4))):
+        if t.dtype is not torch.int32 or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"prefix_attention: pos, slot and the groups' tables must be contiguous int32 tensors for {T} tokens on the queries' device")
     if not plan:
-        plan = nv.proto("b200_prefix_attn_plan", [i32] * 7)(T, groups.n_groups, groups.longest, groups.max_shared, H, G, D)
-    out = torch.empty(T, H * D, dtype=dt, device=dev)
-    part = torch.empty(T * H * (plan % 256) * (D + 2), dtype=torch.float32, device=dev)
+        plan = nv.proto("b200_prefix_attn_plan", _PLAN_ARGS)(T, n_groups, groups.longest, groups.max_shared, H, G, D)
+    out = q.new_empty((T, H * D))
+    part = q.new_empty(T * H * (plan % 256) * (D + 2), dtype=torch.float32)
     fn = nv.proto("b200_prefix_attn", _ARGS)
-    nv.check(nv.call_on(dev, fn, q_ptr, stride[0], cache_k.data_ptr(), cache_v.data_ptr(), pools[0], pos.data_ptr(), slot.data_ptr(), table.data_ptr(),
-                        table.stride(0), *table.shape, groups.groups.data_ptr(), groups.of.data_ptr(), groups.n_groups, groups.longest, nv.ptr(sinks),
+    nv.check(nv.call_on(dev, fn, q_ptr, row, cache_k.data_ptr(), cache_v.data_ptr(), pools[0], pos.data_ptr(), slot.data_ptr(), table.data_ptr(),
+                        table.stride(0), *table.shape, rows.data_ptr(), of.data_ptr(), n_groups, groups.longest, nv.ptr(sinks),
                         out.data_ptr(), part.data_ptr(), plan, max(1, max_pos + 1 - groups.min_shared) if max_pos else 0, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
     nv.count_launch(2)
     return out

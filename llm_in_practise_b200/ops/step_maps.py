@@ -19,6 +19,8 @@ import torch
 from . import _native as nv
 
 vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+_EXTEND_ARGS = [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp, i32, i32, vp]
+_MAPS_ARGS = [vp, i64, i32, i32, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
 TILE_Q = 64          # query rows per tile of the tensor-core attention kernels
 
 
@@ -48,8 +50,9 @@ def _ints(n, device, tensors) -> bool:
 
 
 def _check(what, table, rows, block_size, *lengths):
-    if table.dtype is not torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1):
-        raise ValueError(f"{what}: the block table is int32 [rows, blocks] with contiguous rows")
+    if (table.dtype is not torch.int32 or table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1)
+            or (table.stride(0) < table.shape[1] and table.shape[0] > 1)):
+        raise ValueError(f"{what}: the block table is int32 [rows, blocks] with contiguous rows, each of its own")
     if block_size < 1:
         raise ValueError(f"{what}: block_size must be positive, not {block_size}")
     if rows.dim() != 1 or not _ints(rows.shape[0], table.device, (rows, *lengths)):
@@ -67,9 +70,9 @@ def extend_block_tables(table: torch.Tensor, rows: torch.Tensor, cached: torch.T
     if blocks.dim() != 1 or not _ints(blocks.shape[0], table.device, (blocks,)):
         raise ValueError(f"extend_block_tables: blocks must be a contiguous int32 tensor on the table's device, {table.device}")
     n = rows.shape[0]
-    used = torch.empty(1, dtype=torch.int32, device=table.device)
+    used = table.new_empty(1)
     if nv.use_native(table):
-        fn = nv.proto("b200_extend_block_tables", [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp, i32, i32, vp])
+        fn = nv.proto("b200_extend_block_tables", _EXTEND_ARGS)
         nv.check(nv.call_on(table.device, fn, table.data_ptr(), table.stride(0), *table.shape, rows.data_ptr(), cached.data_ptr(), lens.data_ptr(),
                             blocks.data_ptr(), blocks.shape[0], used.data_ptr(), n, block_size), "extend_block_tables")
         nv.count_launch()
@@ -100,11 +103,11 @@ def step_maps(table: torch.Tensor, rows: torch.Tensor, cached: torch.Tensor, new
     four = 4 * n if n_tiles else 0
     # one allocation for the int32 tables (those of four columns first, so that they start on 16 bytes), one for the int64 ones
     at = 8 * n_tiles + 2 * four
-    words = torch.empty(at + 2 * total + n + 1, dtype=torch.int32, device=dev)
-    longs = torch.empty(total + n, dtype=torch.int64, device=dev)
+    words = table.new_empty(at + 2 * total + n + 1)
+    longs = table.new_empty(total + n, dtype=torch.int64)
     w, g = words.data_ptr(), longs.data_ptr()
     w_pos = w + 4 * at
-    fn = nv.proto("b200_step_maps", [vp, i64, i32, i32, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp])
+    fn = nv.proto("b200_step_maps", _MAPS_ARGS)
     nv.check(nv.call_on(dev, fn, table.data_ptr(), table.stride(0), *table.shape, rows.data_ptr(), cached.data_ptr(), new.data_ptr(), n, block_size, total,
                         n_tiles, w_pos + 8 * total, w_pos, w_pos + 4 * total, g, g + 8 * total, w, w + 16 * n_tiles, w + 32 * n_tiles,
                         w + 32 * n_tiles + 4 * four), "step_maps")

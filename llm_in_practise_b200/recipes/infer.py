@@ -89,6 +89,8 @@ def main(argv=None):
                     help="serve: ranks that share every layer (vllm serve --tensor-parallel-size; launch under torchrun)")
     ap.add_argument("--pipeline-parallel-size", "--pipeline_parallel_size", dest="pp", type=int, default=1,
                     help="serve: pipeline stages (engine_kwargs.pipeline_parallel_size of the Ray Serve recipe)")
+    ap.add_argument("--shared-prefix-attention", action="store_true",
+                    help="serve: decode requests behind one cached prompt prefix as a group (paged KV cache, by default in blocks of 16; one GPU)")
     ap.add_argument("--block-size", "--block_size", dest="block_size", type=int, default=0, help="serve: paged KV cache block (0 = one row per sequence)")
     a = ap.parse_args(argv)
     dtype = getattr(torch, a.dtype)
@@ -170,7 +172,8 @@ def main(argv=None):
     elif a.cmd == "serve":
         from ..serve import EngineArgs, LLMEngine
         from ..serve.openai_server import serve
-        eargs = EngineArgs(max_num_seqs=a.max_num_seqs or 16, max_model_len=a.max_model_len, block_size=a.block_size,
+        eargs = EngineArgs(max_num_seqs=a.max_num_seqs or 16, max_model_len=a.max_model_len, block_size=a.block_size or (16 if a.shared_prefix_attention else 0),
+                           shared_prefix_attention=a.shared_prefix_attention,
                            enable_prefix_caching=a.prefix_caching, enable_chunked_prefill=a.chunked_prefill,
                            gpu_memory_utilization=(a.gpu_mem if a.max_num_seqs is None else 0.0), warmup=not a.enforce_eager,
                            kv_offload_gb=a.kv_offload_gb)

@@ -137,7 +137,7 @@ def test_step_maps_keep_to_their_bounds(device):
 
 def test_refusals_of_tables():
     t, r = torch.zeros(4, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
-    for bad in (dict(table=t.long()), dict(rows=r.long()), dict(cached=r[:1]), dict(lens=r.view(1, 2)), dict(block_size=0), dict(table=t.t()),
+    for bad in (dict(table=t.long()), dict(rows=r.long()), dict(cached=r[:1]), dict(lens=r.view(1, 2)), dict(block_size=0), dict(table=t.t()), dict(table=t[:1].expand(4, 4)),
                 dict(blocks=torch.zeros(8, dtype=torch.int32)[::2])):
         args = dict(table=t, rows=r, cached=r, lens=r, blocks=r, block_size=16)
         args.update(bad)
@@ -400,7 +400,7 @@ def test_refusals_of_rules():
         for fn in (process_logits, greedy_tokens):
             with pytest.raises(ValueError, match=fn.__name__):
                 fn(**{**dict(logits=x, state=st), **bad})
-    for out in (x.double(), x[:2], torch.zeros(100, 4).t()):
+    for out in (x.double(), x[:2], torch.zeros(100, 4).t(), x[:1].clone().expand(4, 100)):
         with pytest.raises(ValueError, match="process_logits"):
             process_logits(x, st, out=out)
     for bad in (dict(row=4), dict(row=-1), dict(row=0, prompt=range(9)), dict(row=0, logit_bias={1: 1.0, 2: 1.0, 3: 1.0}), dict(row=0, logit_bias={100: 1.0}),
@@ -671,7 +671,7 @@ def test_refusals_of_attention():
             call({**b, **change}, "cuda")
     on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
     args = [on["q"], on["ck"], on["cv"], on["table"], on["pos"], on["slot"], make_prefix_groups(b["plan"], 5, "cuda"), 4, 2, 64, 0.125]
-    for i, bad in ((0, torch.empty(5, 516, dtype=torch.bfloat16, device="cuda")[:, 1:513]), (7, 3), (6, make_prefix_groups(b["plan"], 4, "cuda")),
+    for i, bad in ((0, torch.empty(5, 516, dtype=torch.bfloat16, device="cuda")[:, 1:513]), (0, on["q"][:1].expand(5, 512)), (0, on["q"].flatten().unfold(0, 512, 64)[:5]), (7, 3), (6, make_prefix_groups(b["plan"], 4, "cuda")),
                    (6, make_prefix_groups(b["plan"], 5, "cpu"))):
         with pytest.raises(ValueError, match="prefix_attention"):
             prefix_attention(*args[:i], bad, *args[i + 1:])
