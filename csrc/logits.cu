@@ -484,6 +484,9 @@ static long long work_bytes(int B, int V, bool greedy) {
   return (long long)B * (sizeof(RowPlan) + bitmap_words(V) * 4ll + (greedy ? (ceil_div(V, kLgTokens) + 1) * 8ll : 0));
 }
 
+// whether a call is one kernel's
+static bool small_batch(int B, int V) { return (long long)B * ceil_div(V, kLmTokens) <= kLmSlices; }
+
 template <typename T, bool GREEDY>
 static int launch_logits_as(const void* x, long long ldx, int B, int V, const LogitRules& L, float* out, long long ldo, void* work, long long* ids, cudaStream_t st) {
   RowPlan* plan = (RowPlan*)work;
@@ -498,7 +501,7 @@ static int launch_logits_as(const void* x, long long ldx, int B, int V, const Lo
   cfg.numAttrs = 1;
   // Up to so many slices one kernel is faster: 8 x 151936, histories of 1500: 7.2 us on the device against 9.6 (and a launch less for the host), 16 rows 8.2
   // against 11.1, 24 rows (912 slices) 12.4 against 13.8, but greedy 17.3 against 15.9; 48 rows 20.6 against 18.5, 128 with all rules 100 against 52
-  if ((long long)B * slices <= kLmSlices) {
+  if (small_batch(B, V)) {
     logits_small_kernel<T, GREEDY><<<dim3(slices, B), 256, 0, st>>>((const T*)x, ldx, V, L, out, ldo, best);
     B200_LAUNCH_CHECK();
     if (!GREEDY) return 0;
@@ -537,6 +540,8 @@ static int launch_logits(const void* x, long long ldx, int B, int V, const int* 
 }
 
 B200_API long long b200_logits_workspace(int B, int V, int greedy) { return B < 1 || V < 1 ? 0 : work_bytes(B, V, greedy != 0); }
+
+B200_API int b200_logits_launches(int B, int V, int greedy) { return B < 1 || V < 1 ? 0 : (small_batch(B, V) ? 1 : 2) + (greedy != 0); }
 
 B200_API int b200_process_logits(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, void* workspace, float* out, long long ldo,
                                  int dtype, void* stream) {

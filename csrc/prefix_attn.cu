@@ -520,8 +520,9 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
                         reinterpret_cast<uintptr_t>(part)) & 15)) return B200_ERR_BAD_ALIGN;
   PrefixParams p = {};
   while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
-  // a swizzled box starts on a group of eight rows, and rows of the pools are counted in 32 bits
-  if ((1 << p.bs_log2) != block_size || block_size < 8 || n_pages < 1 || (long long)n_pages * G * block_size >= 0x7fffff00LL) return B200_ERR_UNSUPPORTED;
+  // a swizzled box starts on a group of eight rows, and rows of the pools and keys of a sequence are counted in 32 bits
+  if ((1 << p.bs_log2) != block_size || block_size < 8 || n_pages < 1 || (long long)n_pages * G * block_size >= 0x7fffff00LL ||
+      (long long)width * block_size >= 0x7ffff000LL) return B200_ERR_UNSUPPORTED;
   if (n_groups > 0 && longest > 0 && !part) return B200_ERR_BAD_SHAPE;
   if (tc && prefix_tc_tokens(H, G, D) < 1) return B200_ERR_UNSUPPORTED;
   p.q = q; p.ck = ck; p.cv = cv; p.q_stride = q_stride; p.pos = pos; p.slot = slot; p.table = table; p.table_stride = table_stride;

@@ -761,7 +761,8 @@ int b200_moe_gather(const void* h, const long long* dest, const long long* tok, 
  * part in the sum. plan = b200_prefix_attn_plan(...), or any number of ranges of the shared keys (1 .. 32), plus 256
  * for the tcgen05 kernel (D 64 or 128, at most 128 heads to a KV head); part: fp32 [T * H * (plan % 256) * (D + 2)] scratch.
  * most_own: keys behind the shared ones that a token has, at most (0: not known); it only chooses how they are cut. Pools [n_pages, G, block_size, D];
- * 16-bit types, D a multiple of 16 up to 128, block_size a power of two from 8 on, n_pages * G * block_size below 2^31 - 256, scale > 0.
+ * 16-bit types, D a multiple of 16 up to 128, block_size a power of two from 8 on, n_pages * G * block_size below 2^31 - 256, width * block_size below
+ * 2^31 - 4096, scale > 0.
  * A token with pos < 0, or a slot outside the table, sees no key:
  * zero. Pages outside the pools are not read. */
 int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int H, int G, int D);
@@ -798,6 +799,7 @@ typedef struct {
 /* out fp32 [B, ldo] (x itself, if that is fp32 with the same rows): seen: y < 0 ? y r : y / r; in the output c times: y -= f c, y -= p; y += bias; y /= T;
  * not allowed: -inf. V up to 2^19. workspace: b200_logits_workspace(B, V, greedy) bytes, 16-byte aligned, of this call alone while it runs. */
 long long b200_logits_workspace(int B, int V, int greedy);
+int b200_logits_launches(int B, int V, int greedy);   /* kernels of such a call */
 int b200_process_logits(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, void* workspace, float* out, long long ldo,
                         int dtype, void* stream);
 /* The best token of each row under these rules, the lowest of equals, NaN above all. */

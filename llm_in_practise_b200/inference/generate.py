@@ -26,7 +26,7 @@ import torch
 from ..ops import _native as nv
 from ..ops import elementwise as ew
 from ..ops import fused_decode
-from ..ops.logits import MAX_BIAS, LogitState, greedy_tokens, process_logits
+from ..ops.logits import MAX_BIAS, MAX_HISTORY, MAX_VOCAB, SCALES, LogitState, greedy_tokens, process_logits
 from ..ops.paged_attention import rope_paged_store
 from ..ops.prefix_attention import PrefixGroups, make_prefix_groups, prefix_attention
 from ..ops.step_maps import extend_block_tables
@@ -64,20 +64,22 @@ class GenerationConfig:
         return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias or self.allowed_token_ids is not None
                     or self.prefix_allowed_tokens_fn is not None)
 
-    def check_rules(self, vocab: int) -> None:
-        """Refuse rules that ``vocab`` tokens have no room for, before a step is run with them."""
+    def check_rules(self, vocab: int, max_len: int = 0) -> None:
+        """Refuse rules that ``vocab`` tokens, or sequences of up to ``max_len``, have no room for, before a step is run with them."""
         if not self.has_rules():
             return
+        if vocab > MAX_VOCAB or max_len > MAX_HISTORY:
+            raise ValueError(f"rules on logits take vocabularies of up to {MAX_VOCAB} and sequences of up to {MAX_HISTORY} tokens, not {vocab} and {max_len}")
         bias = self.logit_bias or {}
         if len(bias) > MAX_BIAS:
             raise ValueError(f"logit_bias has {len(bias)} entries; at most {MAX_BIAS} are taken")
         for t in [*bias, *(self.allowed_token_ids if self.allowed_token_ids is not None else ())]:
             if not 0 <= int(t) < vocab:
                 raise ValueError(f"logit_bias and allowed_token_ids name token {t}, which is not one of the vocabulary's {vocab}")
-        if not all(math.isfinite(float(v)) for v in (*bias.values(), self.presence_penalty, self.frequency_penalty)):
-            raise ValueError("logit_bias and penalties must be finite")
-        if not self.repetition_penalty > 0 or (self.do_sample and self.temperature > 0 and not math.isfinite(self.temperature)):
-            raise ValueError("repetition_penalty must be positive and the temperature finite")
+        if not all(abs(float(v)) <= torch.finfo(torch.float32).max for v in (*bias.values(), self.presence_penalty, self.frequency_penalty)):
+            raise ValueError("logit_bias and penalties must be finite numbers of 32 bits")
+        if not all(SCALES[0] <= v <= SCALES[1] for v in (self.repetition_penalty, self.temperature if self.do_sample and self.temperature > 0 else 1.0)):
+            raise ValueError(f"repetition_penalty and temperature must be from {SCALES[0]:.2g} to {SCALES[1]:.2g}")
 
 
 def sample_next(logits: torch.Tensor, cfg: GenerationConfig, prev: Optional[torch.Tensor] = None,
@@ -115,7 +117,7 @@ class LogitRules:
     def __init__(self, rows: int, vocab: int, max_len: int, device, max_bias: int = 0):
         self.state = LogitState(rows, vocab, max_len, max_bias, device)
         self._tokens: Dict[int, List[int]] = {}          # rows whose grammar is asked before every token: what they hold
-        self._fn: Dict[int, tuple] = {}
+        self._fn: Dict[int, tuple] = {}                  # ... the grammar, the name it knows the row by, the tokens allowed in any case (None: all)
 
     def begin(self, row: int, cfg: GenerationConfig, prompt: Sequence[int], output: Sequence[int] = (), name: Optional[int] = None) -> None:
         """Row ``row`` starts a sequence (``name``: what its ``prefix_allowed_tokens_fn`` is called with, by default the row)."""
@@ -124,18 +126,23 @@ class LogitRules:
                            cfg.logit_bias, cfg.allowed_token_ids)
         self._fn.pop(row, None)
         if cfg.prefix_allowed_tokens_fn is not None:
-            self._fn[row], self._tokens[row] = (cfg, row if name is None else name), [*prompt, *output]
+            always = None if cfg.allowed_token_ids is None else set(cfg.allowed_token_ids)
+            self._fn[row], self._tokens[row] = (cfg.prefix_allowed_tokens_fn, row if name is None else name, always), [*prompt, *output]
 
-    def next(self, logits: torch.Tensor, rows: Sequence[int], cfgs: Sequence[GenerationConfig], generator: Optional[torch.Generator] = None) -> torch.Tensor:
-        """logits [B, V] of sequences ``rows`` (all different) -> next ids [B], which join the rows' histories."""
+    def ask(self, row: int) -> None:
+        """Ask the grammar of ``row``, if it has one, what may come next. An exception of the grammar's leaves the row's mask as it was."""
+        if row in self._fn:
+            fn, name, always = self._fn[row]
+            allowed = [int(t) for t in fn(name, list(self._tokens[row]))]
+            self.state.set_mask(row, [t for t in allowed if 0 <= t < self.state.vocab and (always is None or t in always)])
+
+    def next(self, logits: torch.Tensor, rows: Sequence[int], cfgs: Sequence[GenerationConfig], generator: Optional[torch.Generator] = None,
+             asked: bool = False) -> torch.Tensor:
+        """logits [B, V] of sequences ``rows`` (all different) -> next ids [B], which join the rows' histories. ``asked``: their grammars were asked
+        already."""
         st, dev = self.state, logits.device
-        for row in rows:
-            if row in self._fn:
-                cfg, name = self._fn[row]
-                allowed = cfg.prefix_allowed_tokens_fn(name, list(self._tokens[row]))
-                if cfg.allowed_token_ids is not None:
-                    allowed = [t for t in allowed if t in set(cfg.allowed_token_ids)]
-                st.set_mask(row, [t for t in allowed if 0 <= int(t) < st.vocab])
+        for row in () if asked else rows:
+            self.ask(row)
         slot = torch.tensor(list(rows), dtype=torch.int32)
         slot = slot.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else slot
         draws: Dict[tuple, List[int]] = {}
@@ -161,7 +168,7 @@ def logit_rules(cfg: GenerationConfig, prompts: torch.Tensor, vocab: int, max_le
     """Rules of ``generate`` for prompts [B, S], None where ``sample_next`` does all that ``cfg`` asks for."""
     if not cfg.has_rules():
         return None
-    cfg.check_rules(vocab)
+    cfg.check_rules(vocab, max_len)
     rules = LogitRules(prompts.shape[0], vocab, max_len, prompts.device, len(cfg.logit_bias or ()))
     for b, ids in enumerate(prompts.tolist()):
         rules.begin(b, cfg, ids)

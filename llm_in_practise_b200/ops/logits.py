@@ -25,6 +25,7 @@ _GREEDY_ARGS = [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp]
 MAX_VOCAB = 1 << 19
 MAX_BIAS = 2047          # biases of one row
 MAX_HISTORY = (1 << 20) - 1      # tokens of one row's history
+SCALES = (2.0 ** -126, 2.0 ** 126)       # repetition penalties and temperatures: numbers whose reciprocal has all its bits
 
 
 class _Rules(ctypes.Structure):
@@ -37,7 +38,7 @@ class LogitState:
     """Rules of ``rows`` sequences over a vocabulary of ``vocab`` tokens, histories of up to ``max_len`` tokens, up to ``max_bias`` biases each.
     The tensors may be filled directly (``set_row`` does it from Python values): ``tokens`` int32 [rows, max_len], of which ``length`` [rows] are
     the history and its first ``prompt_length`` [rows] the prompt; ``repetition``, ``presence``, ``frequency``, ``temperature`` fp32 [rows];
-    ``bias_ids`` int32 / ``bias_values`` fp32 [rows, max_bias] with ``bias_length`` [rows]; after ``allow_masks()`` ``mask`` int32
+    (the first and the last of these four within ``SCALES``); ``bias_ids`` int32 / ``bias_values`` fp32 [rows, max_bias] with ``bias_length`` [rows]; after ``allow_masks()`` ``mask`` int32
     [rows, ceil(vocab / 32)] (bit v % 32 of word v // 32 set: token v is allowed) and ``masked`` bool [rows]. Tokens outside 0 .. vocab - 1 are
     passed over, and of biases for one token the last one counts. Sequences, and calls on several streams, may share a state as long as
     nobody writes the rows that another call reads."""
@@ -56,7 +57,7 @@ class LogitState:
         self.bias_ids, self.bias_values = of(torch.int32, rows, max_bias), of(torch.float32, rows, max_bias)
         self.bias_length = of(torch.int32, rows)
         self.mask = self.masked = None
-        self._work = {}                                  # bytes of a workspace by batch size and form
+        self._work = {}                                  # bytes of a workspace and launches, by batch size and form
         self.device = self.tokens.device
 
     def allow_masks(self) -> "LogitState":
@@ -72,8 +73,9 @@ class LogitState:
         """The rules of ``row`` from Python values; what the row held is gone. ``allowed``: the only tokens that may come next (None: all)."""
         if not 0 <= row < self.rows:
             raise ValueError(f"LogitState: no row {row} of {self.rows}")
-        if not repetition_penalty > 0 or not temperature > 0:
-            raise ValueError(f"LogitState: repetition_penalty and temperature must be positive, not {repetition_penalty} and {temperature}")
+        if not all(SCALES[0] <= v <= SCALES[1] for v in (repetition_penalty, temperature)):
+            raise ValueError(f"LogitState: repetition_penalty and temperature must be from {SCALES[0]:.2g} to {SCALES[1]:.2g}, not {repetition_penalty} and "
+                             f"{temperature}")
         hist, bias = list(prompt) + list(output), dict(logit_bias or {})
         if len(hist) > self.max_len or len(bias) > self.max_bias:
             raise ValueError(f"LogitState: {len(hist)} tokens and {len(bias)} biases do not fit rows of {self.max_len} and {self.max_bias}")
@@ -127,9 +129,24 @@ class LogitState:
 
     def _address(self) -> int:
         if self._struct is None:
+            self._check_tensors()
             self.__dict__["_struct"] = _Rules(*(nv.ptr(getattr(self, n)) for n, _ in _Rules._fields_[:12]), self.rows, self.max_len, self.max_bias,
                                               self.words)
         return ctypes.addressof(self._struct)
+
+
+    def _check_tensors(self) -> None:
+        """Tensors that were put in place of the state's own are like them."""
+        i, f, R = torch.int32, torch.float32, (self.rows,)
+        kinds = {"tokens": (i, (self.rows, self.max_len)), "length": (i, R), "prompt_length": (i, R), "repetition": (f, R), "presence": (f, R),
+                 "frequency": (f, R), "temperature": (f, R), "bias_ids": (i, (self.rows, self.max_bias)), "bias_values": (f, (self.rows, self.max_bias)),
+                 "bias_length": (i, R), "mask": (i, (self.rows, self.words)), "masked": (torch.bool, R)}
+        for name, (dtype, shape) in kinds.items():
+            t = getattr(self, name)
+            if t is None and name in ("mask", "masked") and self.mask is self.masked:
+                continue
+            if t is None or t.dtype is not dtype or t.shape != shape or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"LogitState: {name} must be a contiguous {dtype} {list(shape)} tensor on {self.device}")
 
 
 def _check_slot(what, state, n, slot):
@@ -157,25 +174,36 @@ def process_logits(logits: torch.Tensor, state: LogitState, slot: Optional[torch
     elif (out.dtype != torch.float32 or out.shape != logits.shape or out.device != logits.device or (out.stride(1) != 1 and state.vocab > 1)
           or (out.stride(0) < state.vocab and out.shape[0] > 1)):
         raise ValueError("process_logits: out must be fp32, like the logits in shape, with contiguous rows, each of its own")
+    elif _overlap(out, logits) and (out.data_ptr(), out.dtype, out.stride(0)) != (logits.data_ptr(), logits.dtype, logits.stride(0)):
+        raise ValueError("process_logits: out and the logits overlap without being the same")
     if not nv.use_native(logits):
         return out.copy_(_rules_torch(logits, state, slot))
     if logits.shape[0] == 0:
         return out
-    work = _workspace(state, logits.shape[0], 0)
+    work, launches = _workspace(state, logits.shape[0], 0)
     fn = nv.proto("b200_process_logits", _PROCESS_ARGS)
     nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), logits.shape[0], state.vocab, nv.ptr(slot), state._address(),
                         work.data_ptr(), out.data_ptr(), out.stride(0), nv.dtype_code(logits.dtype)), "process_logits")
-    nv.count_launch(2)
+    nv.count_launch(launches)
     return out
 
 
+def _overlap(a, b) -> bool:
+    """Whether the memory from the first to the last element of one reaches into the other's."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def _workspace(state, B, greedy):
-    size = state._work.get((B, greedy))
-    if size is None:
+    """The call's scratch, and how many kernels it launches."""
+    known = state._work.get((B, greedy))
+    if known is None:
         fn = nv.lib().b200_logits_workspace
         fn.argtypes, fn.restype = [i32] * 3, i64
-        size = state._work[B, greedy] = fn(B, state.vocab, greedy)
-    return state.tokens.new_empty(size, dtype=torch.uint8)
+        known = state._work[B, greedy] = fn(B, state.vocab, greedy), nv.proto("b200_logits_launches", [i32] * 3)(B, state.vocab, greedy)
+    return state.tokens.new_empty(known[0], dtype=torch.uint8), known[1]
 
 
 def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -188,11 +216,11 @@ def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.
     ids = logits.new_empty(B, dtype=torch.int64)
     if B == 0:
         return ids
-    work = _workspace(state, B, 1)
+    work, launches = _workspace(state, B, 1)
     fn = nv.proto("b200_greedy_tokens", _GREEDY_ARGS)
     nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), B, state.vocab, nv.ptr(slot), state._address(), work.data_ptr(),
                         ids.data_ptr(), nv.dtype_code(logits.dtype)), "greedy_tokens")
-    nv.count_launch(3)
+    nv.count_launch(launches)
     return ids
 
 

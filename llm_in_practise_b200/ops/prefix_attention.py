@@ -67,12 +67,12 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     (0: unknown). ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it (include/b200_ops.h); 0: chosen by the sizes.
 
     For caches of 16 bits with head sizes that are multiples of 16 up to 128, pages of a power of two from 8 on (fewer than 2^31 - 256 rows of a
-    pool in all) and a positive scale; others go through ``paged_attention``, as does a step without groups. Captured into a graph, each
+    pool, fewer than 2^31 - 4096 places in a table row) and a positive scale; others go through ``paged_attention``, as does a step without groups. Captured into a graph, each
     call keeps a workspace of its own."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
     BS, dt = cache_k.shape[2], q.dtype
     if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or (dt is not torch.bfloat16 and dt is not torch.float16) or D % 16 or D > 128
-            or BS < 8 or BS & (BS - 1) or cache_k.shape[0] * G * BS >= 2 ** 31 - 256 or not scale > 0):
+            or BS < 8 or BS & (BS - 1) or cache_k.shape[0] * G * BS >= 2 ** 31 - 256 or table.shape[-1] * BS >= 2 ** 31 - 4096 or not scale > 0):
         return paged_attention(q, cache_k, cache_v, table.contiguous(), pos, slot, H, G, D, scale, sinks=sinks, max_pos=max_pos)
     dev, pools = q.device, cache_k.shape
     if cache_k.dtype is not dt or cache_v.dtype is not dt or cache_v.shape != pools or pools[1] != G or pools[3] != D:

@@ -254,7 +254,7 @@ class LLMEngine:
             raise ValueError("empty prompt")
         if len(ids) >= self.args.max_model_len:
             raise ValueError(f"prompt of {len(ids)} tokens does not fit max_model_len={self.args.max_model_len}")
-        cfg.check_rules(self.model.embed_tokens.shape[0])
+        cfg.check_rules(self.model.embed_tokens.shape[0], self.args.max_model_len)
         if self.paged:
             pool = len(self._block_ref) - 1
             if self._nblocks(len(ids) + 1) > pool:
@@ -566,6 +566,9 @@ class LLMEngine:
 
     def _emit(self, r: Request, tok: int) -> bool:
         """Record one sampled token; returns True when the request is finished."""
+        if r.error is not None:
+            self._finish(r, "error")
+            return True
         now = time.perf_counter()
         if r.first_token_time is None:
             r.first_token_time = now
@@ -629,7 +632,11 @@ class LLMEngine:
             if r.rules_row != r.slot:
                 r.rules_row = r.slot
                 self._rules.begin(r.slot, r.cfg, r.prompt_ids, r.output_ids, name=r.rid)
-        return self._rules.next(logits, [r.slot for r in reqs], [r.cfg for r in reqs], self._rng).tolist()
+            try:
+                self._rules.ask(r.slot)
+            except Exception as e:                           # the request's own grammar failed: it ends, the others go on
+                r.error = f"{type(e).__name__}: {e}"
+        return self._rules.next(logits, [r.slot for r in reqs], [r.cfg for r in reqs], self._rng, asked=True).tolist()
 
     def _sample(self, logits: torch.Tensor, reqs: List[Request]) -> List[int]:
         """Per-request sampling parameters: requests sharing a config are sampled together."""

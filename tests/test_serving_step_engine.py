@@ -89,6 +89,23 @@ def test_a_grammar_is_asked_before_every_token(model):
     assert {c[0] for c in calls} == {x.rid for x in r}
 
 
+def test_a_grammar_that_fails_ends_its_own_request(model):
+    """An exception of one request's prefix_allowed_tokens_fn is that request's error; what runs beside it gets what it gets alone."""
+    def fn(name, toks):
+        if len(toks) == 5:
+            raise KeyError("no such state")
+        return [20, 21]
+
+    eng = LLMEngine(model, None, EngineArgs(max_num_seqs=3, max_model_len=64))
+    cfgs = [GenerationConfig(max_new_tokens=6, prefix_allowed_tokens_fn=fn), GenerationConfig(max_new_tokens=6, presence_penalty=0.5), GenerationConfig(max_new_tokens=6)]
+    reqs = [eng.submit([1, 2, 3], c) for c in cfgs]
+    while not all(r.done.is_set() for r in reqs):
+        eng.step()
+    assert reqs[0].finish_reason == "error" and "no such state" in reqs[0].error and len(reqs[0].output_ids) == 2
+    for r, c in zip(reqs[1:], cfgs[1:]):
+        assert r.error is None and r.output_ids == Generator(model, max_len=64).generate(torch.tensor([[1, 2, 3]]), c)[0, 3:].tolist()
+
+
 def test_sampling_with_rules(model):
     """Drawn tokens keep to the rules; a row whose rules allow nothing gets token 0 and spoils nobody's draw."""
     torch.manual_seed(2)
@@ -111,6 +128,20 @@ def test_rules_that_cannot_hold_are_refused_at_submission(model):
         with pytest.raises(ValueError):
             Generator(model, max_len=64).generate(torch.tensor([[1, 2]]), max_new_tokens=2, **kw)
     assert eng.num_waiting == 0
+
+
+def test_rules_that_32_bits_or_the_tables_do_not_hold_are_refused(model):
+    eng = LLMEngine(model, None, EngineArgs(max_num_seqs=2, max_model_len=64))
+    for kw in (dict(logit_bias={1: 1e39}), dict(presence_penalty=-1e39), dict(frequency_penalty=1.0, do_sample=True, temperature=1e-39),
+               dict(frequency_penalty=1.0, repetition_penalty=1e38), dict(frequency_penalty=1.0, do_sample=True, temperature=float("inf"))):
+        with pytest.raises(ValueError):
+            eng.submit([1, 2], GenerationConfig(**kw))
+    ruled = GenerationConfig(presence_penalty=1.0)
+    ruled.check_rules(1 << 19, (1 << 20) - 1)
+    for size in ((1 << 19) + 1, 0), (300, 1 << 20):
+        with pytest.raises(ValueError):
+            ruled.check_rules(*size)
+        GenerationConfig().check_rules(*size)
 
 
 def test_server_takes_penalties_and_biases():

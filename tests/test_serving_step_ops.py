@@ -415,6 +415,71 @@ def test_refusals_of_rules():
             st.append(ids, slot)
 
 
+def test_outputs_that_overlap_their_logits_are_refused():
+    st, buf = LogitState(4, 100, 8), torch.randn(900)
+    x = buf[:400].view(4, 100)
+    for out in (buf[100:500].view(4, 100), buf[4:404].view(4, 100), buf[:800].view(4, 200)[:, :100], buf[399:799].view(4, 100)):
+        with pytest.raises(ValueError, match="overlap"):
+            process_logits(x, st, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        process_logits(buf.view(torch.bfloat16)[:400].view(4, 100), st, out=x)
+    for out in (x, buf[400:800].view(4, 100)):
+        want = x.clone()
+        assert torch.equal(process_logits(x, st, out=out), want)
+
+
+def test_tensors_in_place_of_the_state_s_own():
+    """They are looked at before their addresses are taken."""
+    for name, bad in (("tokens", torch.zeros(4, 7, dtype=torch.int32)), ("length", torch.zeros(4, dtype=torch.int64)), ("bias_values", torch.zeros(3, 2)),
+                      ("temperature", torch.ones(8)[::2]), ("mask", torch.zeros(4, 4, dtype=torch.int32)), ("rows", 5)):
+        st = LogitState(4, 100, 8, 2)
+        st._address()
+        setattr(st, name, bad)
+        with pytest.raises(ValueError, match="LogitState"):
+            st._address()
+    st = LogitState(4, 100, 8, 2)
+    st.temperature = torch.full((4,), 2.0)
+    st.mask, st.masked = torch.zeros(4, 4, dtype=torch.int32), torch.ones(4, dtype=torch.bool)
+    st._address()
+
+
+def test_scales_at_their_bounds():
+    st = LogitState(2, 8, 4)
+    for v in (2.0 ** -126, 2.0 ** 126):
+        st.set_row(0, [1], repetition_penalty=v, temperature=v)
+    for v in (2.0 ** -127, 2.0 ** 127, float("inf"), -1.0):
+        for kw in (dict(repetition_penalty=v), dict(temperature=v)):
+            with pytest.raises(ValueError, match="LogitState"):
+                st.set_row(0, [1], **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [2, 300])
+def test_launches_are_counted(B):
+    V = 12800                                                     # four slices a row: 8 and 1200 of them
+    st = LogitState(B, V, 4, device="cuda")
+    x = torch.randn(B, V, device="cuda")
+    for fn, more in ((process_logits, 0), (greedy_tokens, 1)):
+        before = nv.launch_count
+        fn(x, st)
+        assert nv.launch_count - before == (1 if B == 2 else 2) + more
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [3, 300])
+@pytest.mark.parametrize("e", [-126, -60, 0, 60, 126])
+def test_temperatures_at_their_bounds(B, e):
+    """Powers of two: the quotient is exact wherever 32 bits hold it (smaller ones are off by at most their last bit), infinite behind that."""
+    V = 12800
+    st = LogitState(B, V, 4, device="cuda")
+    st.temperature.fill_(2.0 ** e)
+    x = torch.randn(B, V, device="cuda")
+    got, want = process_logits(x, st).double(), x.double() / 2.0 ** e
+    want = torch.where(want.abs() >= 2.0 ** 128, torch.full_like(want, float("inf")).copysign(want), want)
+    off = (got - want).abs().nan_to_num(0.0)                      # infinities of one sign
+    assert torch.equal(got.isinf(), want.isinf()) and bool((off <= torch.where(want.abs() < 2.0 ** -126, 2.0 ** -149, 0.0)).all())
+
+
 # ------------------------------------------------------------------------------------------------ attention over shared keys
 def batch_of(groups, alone, own, H, G, D, BS, dtype, seed, copies=False, odd=None):
     """A decode batch on the CPU: groups (tokens, shared keys), then sequences by themselves, ``own`` keys (cyclic) behind the shared ones. Whole pages of
