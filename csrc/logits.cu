@@ -7,24 +7,27 @@
 //   b200_process_logits    y, fp32
 //   b200_greedy_tokens     the best token of each row, the lowest of equals; a NaN is above all (as in torch.argmax)
 //
-// Two kernels. The first, a CTA to a row, counts the row's history and notes its biases in a hash table in shared memory (integer atomics: any order, one
-// result) and settles the few logits that these say something of, each by one thread; a bitmap tells which. The second streams all of the logits past
-// temperature and mask, as many loads under way as registers hold, and leaves out what is settled; it starts while the first one runs and waits for
-// it when its logits are there. Nothing of a call is kept for the next one.
+// Two kernels. One, a CTA to a row, counts the row's history and notes its biases in a hash table in shared memory (integer atomics: any order, one
+// result) and settles the few logits that these say something of, each by one thread. The other streams all of the logits past temperature and mask, as many
+// loads under way as registers hold. Where logits are written elsewhere the stream goes first, and what is settled is written over it; where they stay in their
+// place, or only the best is asked for, the settling kernel goes first and leaves a bitmap of what the stream is to pass over. Either way the second starts while the
+// first ends. Nothing of a call is kept for the next one.
 //
-// Bound: memory. 128 x 151936 in 32 bits, histories of up to 6000 tokens, 300 biases, half of the rows masked (158 MB): 24 us; here 52, 30 of them the second
-// kernel (29 in all without histories) and the rest the first: 4800 single logits of a row lie in half of the memory of its 152 000. One
+// Bound: memory. 128 x 151936 in 32 bits, histories of up to 6000 tokens, 300 biases, half of the rows masked (158 MB): 24 us; here 47 (52 with the settling
+// first), 27 of them the stream (5.8 TB/s) and the rest the settling, of which a little is beside it: 3 us of table, 5 to 11 of tokens entered, 6 of single logits, 4800 of a
+// row, which lie in half of the memory of its 152 000. A stream of four CTAs to an SM that go on from tile to tile leaves room for the settling kernel beside it, but
+// each slows the other: 60 to 74 us. One
 // kernel with the counts of a slice in shared memory is kept waiting by its own steps (rules, history, counts, logits): 100 us in slices of 4096
 // tokens (which small batches keep, see kLmSlices), 69 to 78 in slices of 20480 with the history counted once for clusters of 2 to 8 CTAs (8 rows: 8.8 and 6.5 us, here 9.7). The rules applied in
-// the second kernel, from records in token order, took 64: almost every warp had a lane with one.
+// the stream, from records in token order, took 64: almost every warp had a lane with one.
 #include "common.cuh"
 #include "../include/b200_ops.h"
 
 namespace b200 {
 
-constexpr int kLgThreads = 256, kLgQuads = 2;                      // second kernel: twice four logits to a thread
+constexpr int kLgThreads = 256, kLgQuads = 2;                      // streaming kernel: twice four logits to a thread
 constexpr int kLgTokens = kLgThreads * kLgQuads * 4;
-constexpr int kLsThreads = 1024, kLsEarly = 6;                     // first kernel; tokens that a thread asks for before it knows how many there are
+constexpr int kLsThreads = 1024, kLsEarly = 6;                     // settling kernel; tokens that a thread asks for before it knows how many there are
 constexpr int kLsSlots = 16384;                                    // of its table, at most
 constexpr int kLgVocab = 1 << 19;                                  // its bitmap has room for so many tokens
 // a token's word: whether it stands in the prompt | its last bias, counted from 1 | how often it stands in the output
@@ -131,20 +134,20 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
 }
 __device__ __forceinline__ unsigned long long rank_of(float y, int v) { return ((unsigned long long)order_of(y) << 32) | (uint32_t)~(uint32_t)v; }      // of equals the lowest
 
-// what the second kernel needs of a batch row's rules
+// what a stream that comes second needs of a batch row's rules
 struct __align__(16) RowPlan { float T, inv_T; int mask_row, settled; };      // mask_row: -1 for none; settled: the bitmap has bits
 
-// x and out may be the same
-template <typename T, bool GREEDY>
+// LAST: it goes over what the streaming kernel left, and sees to the mask. Otherwise it comes first and says what is settled; x and out may then be the same
+template <typename T, bool GREEDY, bool LAST>
 __global__ void __launch_bounds__(kLsThreads, 1)
 logits_settle_kernel(const T* x, long long ldx, int V, const LogitRules L, float* out, long long ldo, RowPlan* __restrict__ plan, uint32_t* __restrict__ bitmap,
                      unsigned long long* __restrict__ best, int parts, int most_slots) {
   extern __shared__ __align__(16) uint32_t smem_ls[];         // bitmap, keys, words, places of the tokens found
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, bit_words = (V + 127) / 128 * 4;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, bit_words = LAST ? 0 : (V + 127) / 128 * 4;
   uint32_t *bits = smem_ls, *keys = bits + bit_words;
   __shared__ unsigned long long red[kLsThreads / 32];
   __shared__ int n_found;
-  pdl_launch_dependents();
+  if (!LAST) pdl_launch_dependents();
   const int row = L.slot ? L.slot[b] : b;
   const bool ruled = (unsigned)row < (unsigned)L.rows;
   // What the row's history and biases are is asked for together with how long they are: a table's row may be read to its end
@@ -161,10 +164,10 @@ logits_settle_kernel(const T* x, long long ldx, int V, const LogitRules L, float
     R = row_rules(L, row);
   }
   const bool tables = R.n_hist > 0 || R.n_bias > 0;
-  if (tid == 0) plan[b] = {R.T, R.inv_T, R.masked ? row : -1, tables ? 1 : 0};
+  if (!LAST && tid == 0) plan[b] = {R.T, R.inv_T, R.masked ? row : -1, tables ? 1 : 0};
   unsigned long long mine = 0;
   if (tables) {
-    const int* mask = GREEDY && R.masked ? L.mask + r0 * L.words : nullptr;      // else the second kernel sees to it
+    const int* mask = (GREEDY || LAST) && R.masked ? L.mask + r0 * L.words : nullptr;      // else the stream sees to it
     const float* values = L.bias_values + r0 * L.bias_width;
     const T* xr = x + (long long)b * ldx;
     int slots = min(1024, most_slots);                        // twice the tokens, if that is not too many
@@ -173,6 +176,7 @@ logits_settle_kernel(const T* x, long long ldx, int V, const LogitRules L, float
     uint16_t* found = reinterpret_cast<uint16_t*>(word + slots);
     // up to three quarters of its slots the table is one of hashes; a longer history goes by parts of the vocabulary, a slot for each token
     const bool hashed = R.n_hist + R.n_bias <= slots / 4 * 3;
+    bool waited = !LAST;
     const int turns = hashed ? 1 : (V + slots - 1) / slots;
     for (int i = tid; i < bit_words / 4; i += kLsThreads) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0, 0, 0, 0);
     for (int turn = 0; turn < turns; ++turn) {
@@ -265,20 +269,23 @@ logits_settle_kernel(const T* x, long long ldx, int V, const LogitRules L, float
           l[i] = xr[v[i]];
           if (mask) ok[i] = (uint32_t)mask[v[i] >> 5];
         }
+        if (!waited) pdl_wait();                              // these logits are read; what goes over them is written
+        waited = true;
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
           if (i0 + i * kLsThreads >= n) break;
           float y = apply_word(to_f32<T>(l[i]), R, w[i], values);
           if (mask && !(ok[i] >> (v[i] & 31) & 1)) y = -INFINITY;
-          atomicOr(bits + (v[i] >> 5), 1u << (v[i] & 31));
+          if (!LAST) atomicOr(bits + (v[i] >> 5), 1u << (v[i] & 31));
           if (GREEDY) mine = max(mine, rank_of(y, v[i]));
           else out[(long long)b * ldo + v[i]] = y;
         }
       }
     }
-    __syncthreads();
+    if (!LAST) __syncthreads();
     for (int i = tid; i < bit_words / 4; i += kLsThreads) reinterpret_cast<uint4*>(bitmap)[(long long)b * (bit_words / 4) + i] = reinterpret_cast<const uint4*>(bits)[i];
   }
+  if (LAST) pdl_wait();                                       // threads that had nothing to write too: the call ends with its stream
   if (GREEDY) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
@@ -291,10 +298,10 @@ logits_settle_kernel(const T* x, long long ldx, int V, const LogitRules L, float
   }
 }
 
-template <typename T, bool GREEDY>
+// FIRST: nothing is settled yet
+template <typename T, bool GREEDY, bool FIRST>
 __global__ void __launch_bounds__(kLgThreads)
-logits_stream_kernel(const T* x, long long ldx, int V, const int* __restrict__ masks, int words, float* out, long long ldo, const RowPlan* __restrict__ plan,
-                     const uint32_t* __restrict__ bitmap, unsigned long long* __restrict__ best, int parts) {
+logits_stream_kernel(const T* x, long long ldx, int V, const LogitRules L, float* out, long long ldo, const RowPlan* plan, const uint32_t* bitmap, unsigned long long* __restrict__ best, int parts) {
   __shared__ uint32_t red[2][kLgThreads / 32];
   const int b = blockIdx.y, tid = threadIdx.x, v0 = blockIdx.x * kLgTokens + tid * 4;
   const T* xr = x + (long long)b * ldx;
@@ -302,16 +309,26 @@ logits_stream_kernel(const T* x, long long ldx, int V, const int* __restrict__ m
   Quad<T> q[kLgQuads];
 #pragma unroll
   for (int i = 0; i < kLgQuads; ++i) q[i] = load_quad<T>(xr + v0 + i * (kLgThreads * 4), V - v0 - i * (kLgThreads * 4), whole_in);
-  if (GREEDY) pdl_launch_dependents();
-  pdl_wait();
-  const RowPlan P = plan[b];
+  if (GREEDY || FIRST) pdl_launch_dependents();
+  RowPlan P = {1.f, 1.f, -1, 0};
+  if (FIRST) {
+    const int row = L.slot ? L.slot[b] : b;
+    if ((unsigned)row < (unsigned)L.rows) {
+      P.T = L.temperature[row];
+      P.inv_T = __frcp_rn(P.T);
+      if (L.mask && L.masked[row]) P.mask_row = row;
+    }
+  } else {
+    pdl_wait();
+    P = plan[b];
+  }
   const uint32_t* known = bitmap + (long long)b * ((V + 127) / 128 * 4);
   uint32_t have[kLgQuads], allow[kLgQuads];
 #pragma unroll
   for (int i = 0; i < kLgQuads; ++i) {
     const int v = v0 + i * (kLgThreads * 4);
-    have[i] = P.settled && v < V ? known[v >> 5] >> (v & 31) & 15u : 0u;
-    allow[i] = P.mask_row >= 0 && v < V ? (uint32_t)masks[(long long)P.mask_row * words + (v >> 5)] >> (v & 31) & 15u : 15u;
+    have[i] = !FIRST && P.settled && v < V ? known[v >> 5] >> (v & 31) & 15u : 0u;
+    allow[i] = P.mask_row >= 0 && v < V ? (uint32_t)L.mask[(long long)P.mask_row * L.words + (v >> 5)] >> (v & 31) & 15u : 15u;
   }
 #pragma unroll
   for (int i = 0; i < kLgQuads; ++i)
@@ -444,7 +461,7 @@ logits_small_kernel(const T* x, long long ldx, int V, const LogitRules L, float*
 }
 
 // the best of a row's CTAs: a warp to a row
-__global__ void __launch_bounds__(128) greedy_pick_kernel(const unsigned long long* __restrict__ best, int parts, long long* __restrict__ ids, int B) {
+__global__ void __launch_bounds__(128) greedy_pick_kernel(const unsigned long long* best, int parts, long long* __restrict__ ids, int B) {
   pdl_wait();
   const int b = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (b >= B) return;
@@ -510,14 +527,24 @@ static int launch_logits_as(const void* x, long long ldx, int B, int V, const Lo
   }
   int slots = 256;                                            // no larger than twice what a row may hold
   while (slots < kLsSlots && slots / 2 < L.width + L.bias_width) slots *= 2;
+  if (!GREEDY && x != out) {
+    logits_stream_kernel<T, GREEDY, !GREEDY><<<dim3(parts, B), kLgThreads, 0, st>>>((const T*)x, ldx, V, L, out, ldo, nullptr, nullptr, nullptr, parts);
+    B200_LAUNCH_CHECK();
+    const size_t smem = (size_t)slots * 10;
+    auto settle = logits_settle_kernel<T, GREEDY, !GREEDY>;
+    // per call: the attribute belongs to the current device, and a process may use several
+    if (smem > 48 * 1024) B200_CHECK(cudaFuncSetAttribute(settle, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cfg.gridDim = dim3(B); cfg.blockDim = dim3(kLsThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    return (int)cudaLaunchKernelEx(&cfg, settle, (const T*)x, ldx, V, L, out, ldo, (RowPlan*)nullptr, (uint32_t*)nullptr, (unsigned long long*)nullptr, parts, slots);
+  }
   const size_t smem = (size_t)slots * 10 + bitmap_words(V) * 4;      // 224 KB at most
-  auto settle = logits_settle_kernel<T, GREEDY>;
+  auto settle = logits_settle_kernel<T, GREEDY, false>;
   // per call: the attribute belongs to the current device, and a process may use several
   if (smem > 48 * 1024) B200_CHECK(cudaFuncSetAttribute(settle, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   settle<<<B, kLsThreads, smem, st>>>((const T*)x, ldx, V, L, out, ldo, plan, bitmap, best, parts, slots);
   B200_LAUNCH_CHECK();
   cfg.gridDim = dim3(parts, B); cfg.blockDim = dim3(kLgThreads); cfg.stream = st;
-  B200_CHECK(cudaLaunchKernelEx(&cfg, logits_stream_kernel<T, GREEDY>, (const T*)x, ldx, V, L.mask, L.words, out, ldo, (const RowPlan*)plan, (const uint32_t*)bitmap, best, parts));
+  B200_CHECK(cudaLaunchKernelEx(&cfg, logits_stream_kernel<T, GREEDY, false>, (const T*)x, ldx, V, L, out, ldo, (const RowPlan*)plan, (const uint32_t*)bitmap, best, parts));
   if (!GREEDY) return 0;
   cfg.gridDim = dim3(ceil_div(B, 4)); cfg.blockDim = dim3(128);
   return (int)cudaLaunchKernelEx(&cfg, greedy_pick_kernel, (const unsigned long long*)best, parts + 1, ids, B);

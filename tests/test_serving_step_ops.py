@@ -392,6 +392,33 @@ def test_logits_in_place(device):
     assert process_logits(x[:0].to(device), st).shape == (0, V) and greedy_tokens(x[:0].to(device), st).shape == (0,)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,n", [(6400, 30), (40000, 20000)])
+def test_in_place_and_elsewhere_are_the_same(V, n):
+    """Batches of several kernels, which go over logits that stay in their place in another order; rows with histories longer than a table, too. Equal are
+    numbers, and any two NaN: which of its NaN an operation gives is open (IEEE 754, 6.2.3), so a row of T 1 may pass one on or divide it by 1."""
+    def same(a, b):
+        return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+    rows = some_rules(V, 7, 5, 30)
+    st = state_of(rows, V, n, "cuda")
+    if n > 30:
+        st.tokens[2] = torch.randint(0, V, (n,), dtype=torch.int32, device="cuda")
+        st.length[2], st.prompt_length[2], st.frequency[2] = n, n // 2, 0.25
+    slot = torch.arange(8, dtype=torch.int32, device="cuda").repeat(60)          # row 7 has no rules
+    x = torch.randn(480, V, device="cuda")
+    x[::3, 5], x[1::3, 9] = NAN, -INF
+    y = process_logits(x, st, slot)
+    z = x.clone()
+    process_logits(z, st, slot, out=z)
+    assert same(y, z)
+    wide = torch.empty(480, V + 3, device="cuda")                             # rows that do not start on 16 bytes
+    assert same(process_logits(x, st, slot, out=wide[:, 1:V + 1]), y)
+    few = process_logits(x[:8], st, slot[:8])                                 # by one kernel
+    assert same(few, y[:8])
+    assert torch.equal(greedy_tokens(x, st, slot), y.argmax(1))
+
+
 def test_refusals_of_rules():
     st = LogitState(4, 100, 8, 2)
     x = torch.zeros(4, 100)
