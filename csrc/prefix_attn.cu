@@ -8,13 +8,17 @@
 // 16 bits for the tensor cores' second product, as in the other attention kernels.
 //
 //   shared keys  for each group and KV head ONE product of all its rows (tokens x heads of the KV head) with the keys: they are read
-//                once for 64 rows instead of once a sequence. The keys are cut into nsplit ranges, so that few rows still
-//                fill the GPU; a range leaves (m, l, o) per row
-//   own keys     a CTA for a token and KV head, 16-byte loads, every lane with keys of its own; at its end it takes up the ranges of the
-//                shared keys and the sink, and writes the result: no third kernel
+//                once for 64 rows (mma.sync, here) or 128 (tcgen05, prefix_attn_tc.cu) instead of once a sequence. The keys are cut into nsplit
+//                ranges, so that few rows still fill the GPU; a range leaves (m, l, o) per row
+//   own keys     a CTA for a token and KV head (or a cluster, where tokens are few), whose warps have rings of 16 keys by TMA and mma.sync products; at its end
+//                it takes up the ranges of the shared keys and the sink, and writes the result: no third kernel (one beside both took 36 us where this takes 31). It
+//                starts while the first kernel runs and waits for it only there
 //
-// Bound: memory, until the rows of a group are so many that the tensor cores are. 64 tokens, 32 / 8 heads of 128, 4096 shared and 300 own keys:
-// 17 MB of shared keys and 78 MB of own ones (15 us at 6.5 TB/s), 4.6 GFLOP (3 us); read once a sequence they were 1.15 GB.
+// Bound: memory, until the rows of a group are so many that the tensor cores are. 64 tokens, 32 / 8 heads of 128, 4096 shared and 300 own keys on average:
+// 17 MB of shared keys and 78 MB of own ones (15 us at 6.5 TB/s), 4.6 GFLOP (3 us); read once a sequence they were 1.15 GB. It takes 31 us, 16 of them beside the
+// shared keys, whose CTAs leave room for one of the own keys' on an SM; then three fit one. There a CTA's own steps count: four loads one after another (row, group,
+// page numbers, keys) before the first product, five blocks to a warp, two waits to join the parts. 128 tokens, 16384 shared and 256 own keys: 68 us, 39 of them the
+// shared keys (prefix_attn_tc.cu), which fill the SMs. 4 tokens, 512 shared and 20 own keys: 6 + 5 us, of which 8 remain as the second starts early.
 #include "common.cuh"
 #include "mma_sync.cuh"
 #include "prefix_attn.cuh"
@@ -199,7 +203,8 @@ prefix_shared_mma_kernel(const PrefixParams p) {
 // ------------------------------------------------------------------------------------------------------------------
 // A CTA owns one token and up to eight query heads of one KV head; its warps take blocks of 16 keys in turn, each with a ring of its own that its
 // first lane refills by TMA (one box per page and 64 dimensions, 128-byte swizzle). On mma.sync: S^T = K Q^T, the keys the first operand and the
-// heads the eight columns, then O^T = V^T P^T with V turned by ldmatrix; P changes sides by movmatrix.
+// heads the eight columns, then O^T = V^T P^T with V turned by ldmatrix; P changes sides by movmatrix. Rings against 16-byte loads into registers: 64 tokens with
+// 300 keys of their own 33 -> 20 us. Four warps of two stages take 31 us with 4096 shared keys before them; three of two 32, three of three 37, five of two 34.
 constexpr int kPxOwn = 16, kPxStages = 2, kPxCluster = 4, kPxClusterWarps = 8 * kPxCluster;
 
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {

@@ -3,9 +3,12 @@ requests' lengths, rules on logits. Each against a statement of its own in 64 bi
 path on the CPU, the kernels on the GPU."""
 import collections
 import itertools
+import re
 
 import pytest
 import torch
+
+import test_kernel_sources_cpu as sources
 
 from llm_in_practise_b200.ops import _native as nv
 from llm_in_practise_b200.ops.logits import LogitState, greedy_tokens, process_logits
@@ -769,3 +772,9 @@ def test_refusals_of_attention():
             prefix_attention(*args[:i], bad, *args[i + 1:])
     with pytest.raises(ValueError, match="sinks"):
         prefix_attention(*args, sinks=torch.zeros(4))
+
+
+def test_lanes_meet_before_instructions_of_a_warp(monkeypatch):
+    """The tcgen05 kernel's source, read as the other ones are."""
+    monkeypatch.setattr(sources, "WHOLE", re.compile(r"\b(issue_qk|pt_mma_ss|pt_mma_ts|pt_commit|tmem_ld_32x32)\b\s*[(<]"))
+    sources.test_lanes_meet_before_instructions_of_a_warp("prefix_attn_tc.cu")
