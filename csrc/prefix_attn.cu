@@ -410,9 +410,12 @@ static int launch_shared_mma(const PrefixParams& p, dim3 grid, cudaStream_t st) 
   auto kern = prefix_shared_mma_kernel<T, DK>;
   // per call: the attribute belongs to the current device, and a process may use several
   if (smem > 48 * 1024) B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kern<<<grid, 128, smem, st>>>(p);
-  B200_LAUNCH_CHECK();
-  return 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute room = most_shared_memory();
+  cfg.gridDim = grid; cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.attrs = &room;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 // The second kernel starts while the first one ends: it waits for it (griddepcontrol.wait) before it takes up the ranges, its own keys, queries and
@@ -431,8 +434,9 @@ static int launch_own_by(const PrefixParams& p, dim3 grid, int cl, cudaStream_t 
   B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid; cfg.blockDim = dim3(32 * W); cfg.dynamicSmemBytes = L::kBytes; cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  int na = 0;
+  cudaLaunchAttribute attr[3];
+  int na = 1;
+  attr[0] = most_shared_memory();
   if (cl > 1) {
     attr[na].id = cudaLaunchAttributeClusterDimension;
     attr[na].val.clusterDim.x = cl; attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
@@ -447,13 +451,31 @@ static int launch_own_by(const PrefixParams& p, dim3 grid, int cl, cudaStream_t 
   cfg.numAttrs = na;
   return (int)cudaLaunchKernelEx(&cfg, kern, tk, tv, p, cl);
 }
+// Warps of a CTA that has a token to itself, heads of 128. Those that run beside the tcgen05 kernel end only after it, and what no SM has room for until then starts from
+// the beginning: two waves. So where four warps to a CTA leave some out, three or two, if then all have room. beside: CTAs of that kernel, one to an SM.
+// 40 tokens, 4096 shared and up to 600 own keys, four warps 25.9 us, three 22.2, two 25.8; 64 tokens (three leave some out) 30.8, 31.5, 28; with one own key 19.9, 19.2,
+// 18.2. Two warps are slower at own keys alone: up to 2400 of them 74 us, three 62, four 62; 64 tokens, 4096 shared and up to 1000 own keys 40.3, four 39.8.
+constexpr int kPxTwoWarps = 800;                      // own keys, at most, for two
+static int own_warps(long long ctas, long long beside, int most_own, bool* room = nullptr) {
+  const bool one = beside <= kNumSMs, four = one && ctas <= 3 * kNumSMs - 2 * beside, three = one && ctas <= 4 * kNumSMs - 2 * beside,
+             two = one && ctas <= 6 * kNumSMs - 3 * beside && most_own <= kPxTwoWarps;
+  if (room) *room = four || three || two;
+  return four ? 4 : three ? 3 : two ? 2 : 4;
+}
 template <typename T, int DK>
 static int launch_own(const PrefixParams& p, dim3 grid, cudaStream_t st) {
   // Where there are fewer CTAs than SMs, eight warps to each (four otherwise: then three CTAs fit an SM), and up to four CTAs to a token, while each warp has
   // two blocks. 32 / 8 heads of 128, own keys of up to 3000 for 2 tokens 37.9 -> 12.9 us (with eight CTAs to a token 21.9), of 2000 for 8 30.7 -> 21.5; 16 / 4
   // heads, 8000 keys for 4 tokens 99 -> 22; 64 tokens by eight warps 29.7 -> 37.5, 4 tokens with 40 keys 7.7 -> 7.9.
   const long long ctas = (long long)grid.x * grid.y;
-  if (ctas > kNumSMs || p.most_own <= 256) return launch_own_by<T, DK, 4>(p, grid, 1, st);
+  if (ctas > kNumSMs || p.most_own <= 256) {
+    if constexpr (DK == 8) {
+      const int w = own_warps(ctas, p.beside, p.most_own);
+      if (w == 2) return launch_own_by<T, DK, 2>(p, grid, 1, st);
+      if (w == 3) return launch_own_by<T, DK, 3>(p, grid, 1, st);
+    }
+    return launch_own_by<T, DK, 4>(p, grid, 1, st);
+  }
   int cl = 1;
   while (cl < kPxCluster && ctas * cl * 2 <= kNumSMs && p.most_own >= 256 * cl) cl *= 2;
   grid.x *= cl;
@@ -485,18 +507,23 @@ using namespace b200;
 // Which kernel: tcgen05 for the head sizes that it has, but for up to 32 rows a group and 1024 keys (32 / 8 heads of 128, one token, 600 keys: 15.4 us, 13.3 on
 // mma.sync; 4096 keys: 19.1 and 19.4, 16000: 29.7 and 37.9; 64 rows, 16000 keys: 30 and 42; 128 rows: 30 and 52).
 // How many ranges: those that a cost makes cheapest, in us: the blocks of a CTA, each of which takes longer where an SM has more CTAs (0.72 and 1.15
-// for one and two on tcgen05, 1.7 for each on mma.sync), rounds of CTAs, and the ranges' way through L2, written and read at 4 TB/s. 64 x 4096 keys with 32 / 8 heads:
-// 4, 8, 9, 18 ranges 44, 38, 39, 40 us (chosen: 8); 128 x 16384: 4, 8, 9, 12 ranges 92, 75.5, 75.3, 91 (9); 100 x 8000, 12 / 2 heads of 64: 4, 9, 12, 18 ranges
+// for one and two on tcgen05, 1.7 for each on mma.sync), rounds of CTAs, the ranges' way through L2, written and read at 4 TB/s, a wait for each eight of them where they are joined, and
+// where not all CTAs of own keys have room beside the shared ones (own_warps) their first steps once more. 64 x 4096 keys with 32 / 8 heads and up to 600 own ones:
+// 4, 6, 7, 8, 9 ranges 28, 28, 28, 31, 31 us (chosen: 7); 40 x 3000, 16 / 2 heads: 4, 8, 11, 24 ranges 17, 13, 13, 16 (8); 128 x 16384: 4, 8, 9, 12 ranges 92, 75.5, 75.3, 91 (9); 100 x 8000, 12 / 2 heads of 64: 4, 9, 12, 18 ranges
 // 36, 25.7, 23.7, 26.2 (14).
 constexpr int kPxTc = 256;
-B200_API int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int H, int G, int D) {
+// CTAs of the shared keys' kernel for one range: tiles of the longest group for each, but no more than the batch can fill
+static long long shared_items(int T, int n_groups, int longest, int rep, int G, int tc_tokens) {
+  const long long of_longest = tc_tokens > 0 ? ceil_div(longest, tc_tokens) : ceil_div64((int64_t)longest * rep, kPxRows);
+  const long long of_batch = (tc_tokens > 0 ? T / tc_tokens : (long long)T * rep / kPxRows) + n_groups;
+  return G * (n_groups * of_longest < of_batch ? n_groups * of_longest : of_batch);
+}
+B200_API int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int most_own, int H, int G, int D) {
   if (T < 1 || n_groups < 1 || longest < 1 || max_shared < 1 || H < 1 || G < 1 || H % G) return 1;
   const int rep = H / G, tokens = prefix_tc_tokens(H, G, D);
   const bool tc = tokens > 0 && !((long long)longest * rep <= 32 && max_shared <= 1024);
-  // tiles: those of the longest group for each, but no more than the batch can fill
-  const long long of_longest = tc ? ceil_div(longest, tokens) : ceil_div64((int64_t)longest * rep, kPxRows);
-  const long long of_batch = (tc ? T / tokens : (long long)T * rep / kPxRows) + n_groups;
-  const long long items = G * (n_groups * of_longest < of_batch ? n_groups * of_longest : of_batch), blocks = ceil_div64(max_shared, kPxKeys);
+  const long long items = shared_items(T, n_groups, longest, rep, G, tc ? tokens : 0), blocks = ceil_div64(max_shared, kPxKeys);
+  const long long own = (long long)T * G * ceil_div(rep, 8);
   const int resident = tc ? 2 : 3;
   const double pass = (double)T * H * D * 8 / 4e6;
   int best = 1;
@@ -504,7 +531,11 @@ B200_API int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_sha
   for (int n = 1; n <= 32 && n <= blocks; ++n) {
     const long long ctas = items * n, rounds = ceil_div64(ctas, resident * kNumSMs);
     const int beside = ctas > resident * kNumSMs ? resident : (int)ceil_div64(ctas, kNumSMs);
-    const double cost = rounds * ceil_div64(blocks, n) * (tc ? 0.29 + 0.43 * beside : 1.7 * beside) + n * pass;
+    double cost = rounds * ceil_div64(blocks, n) * (tc ? 0.29 + 0.43 * beside : 1.7 * beside) + n * pass;
+    cost += ceil_div(n, 8);
+    bool room = true;
+    if (tc && D == 128) own_warps(own, ctas, most_own > 0 ? most_own : 0x7fffffff, &room);
+    if (!room) cost += 3;
     if (n == 1 || cost < least) { best = n; least = cost; }
   }
   return best + (tc ? kPxTc : 0);
@@ -535,6 +566,7 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
   p.longest = longest; p.sinks = sinks; p.out = out; p.T = T; p.H = H; p.G = G; p.D = D; p.nsplit = nsplit;
   p.part_o = part; p.part_ml = part ? part + (long long)T * H * nsplit * D : nullptr;
   p.most_own = most_own > 0 ? most_own : 0x7fffffff;
+  p.beside = tc ? (int)(shared_items(T, n_groups, longest, H / G, G, prefix_tc_tokens(H, G, D)) * nsplit) : 0;
   p.scale_log2 = scale * kPxLog2e;
   return dtype == B200_DT_BF16 ? prefix_attn<__nv_bfloat16>(p, tc, (cudaStream_t)stream) : prefix_attn<__half>(p, tc, (cudaStream_t)stream);
 }

@@ -338,9 +338,12 @@ static int launch_shared_tc(const PrefixParams& p, cudaStream_t st) {
   auto kern = prefix_shared_tc_kernel<D, BF16>;
   // per call: the attribute belongs to the current device, and a process may use several
   B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PtSmem<D>::kBytes));
-  kern<<<dim3(p.nsplit, p.G * ceil_div(p.longest, tokens), p.n_groups), kPtThreads, PtSmem<D>::kBytes, st>>>(tq, tk, tv, p, tokens);
-  B200_LAUNCH_CHECK();
-  return 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute room = most_shared_memory();
+  cfg.gridDim = dim3(p.nsplit, p.G * ceil_div(p.longest, tokens), p.n_groups); cfg.blockDim = dim3(kPtThreads); cfg.dynamicSmemBytes = PtSmem<D>::kBytes; cfg.stream = st;
+  cfg.attrs = &room;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p, tokens);
 }
 
 int prefix_shared_tc(const PrefixParams& p, int dtype, cudaStream_t st) {

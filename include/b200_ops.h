@@ -765,7 +765,7 @@ int b200_moe_gather(const void* h, const long long* dest, const long long* tok, 
  * 2^31 - 4096, scale > 0.
  * A token with pos < 0, or a slot outside the table, sees no key:
  * zero. Pages outside the pools are not read. */
-int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int H, int G, int D);
+int b200_prefix_attn_plan(int T, int n_groups, int longest, int max_shared, int most_own, int H, int G, int D);
 int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const void* cv, int n_pages, const int* pos, const int* slot,
                      const int* table, long long table_stride, int table_rows, int width, const int* groups, const int* of, int n_groups,
                      int longest, const float* sinks, void* out, float* part, int plan, int most_own, int T, int H, int G, int D, int block_size,

@@ -19,7 +19,7 @@ from . import _native as nv
 from .paged_attention import paged_attention
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-_PLAN_ARGS = [i32] * 7
+_PLAN_ARGS = [i32] * 8
 _ARGS = [vp, i64, vp, vp, i32, vp, vp, vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, vp]
 
 
@@ -91,13 +91,14 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     for t, shape in ((pos, tokens), (slot, tokens), (of, tokens), (rows, (n_groups, 4))):
         if t.dtype is not torch.int32 or t.shape != shape or t.device != dev or not t.is_contiguous():
             raise ValueError(f"prefix_attention: pos, slot and the groups' tables must be contiguous int32 tensors for {T} tokens on the queries' device")
+    most_own = max(1, max_pos + 1 - groups.min_shared) if max_pos else 0
     if not plan:
-        plan = nv.proto("b200_prefix_attn_plan", _PLAN_ARGS)(T, n_groups, groups.longest, groups.max_shared, H, G, D)
+        plan = nv.proto("b200_prefix_attn_plan", _PLAN_ARGS)(T, n_groups, groups.longest, groups.max_shared, most_own, H, G, D)
     out = q.new_empty((T, H * D))
     part = q.new_empty(T * H * (plan % 256) * (D + 2), dtype=torch.float32)
     fn = nv.proto("b200_prefix_attn", _ARGS)
     nv.check(nv.call_on(dev, fn, q_ptr, row, cache_k.data_ptr(), cache_v.data_ptr(), pools[0], pos.data_ptr(), slot.data_ptr(), table.data_ptr(),
                         table.stride(0), *table.shape, rows.data_ptr(), of.data_ptr(), n_groups, groups.longest, nv.ptr(sinks),
-                        out.data_ptr(), part.data_ptr(), plan, max(1, max_pos + 1 - groups.min_shared) if max_pos else 0, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
+                        out.data_ptr(), part.data_ptr(), plan, most_own, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
     nv.count_launch(2)
     return out
