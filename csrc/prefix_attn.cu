@@ -11,13 +11,14 @@
 //                once for 64 rows (mma.sync, here) or 128 (tcgen05, prefix_attn_tc.cu) instead of once a sequence. The keys are cut into nsplit
 //                ranges, so that few rows still fill the GPU; a range leaves (m, l, o) per row
 //   own keys     a CTA for a token and KV head (or a cluster, where tokens are few), whose warps have rings of 16 keys by TMA and mma.sync products; at its end
-//                it takes up the ranges of the shared keys and the sink, and writes the result: no third kernel (one beside both took 36 us where this takes 31). It
+//                it takes up the ranges of the shared keys and the sink, and writes the result: no third kernel (one beside both took 36 us where this took 31). It
 //                starts while the first kernel runs and waits for it only there
 //
 // Bound: memory, until the rows of a group are so many that the tensor cores are. 64 tokens, 32 / 8 heads of 128, 4096 shared and 300 own keys on average:
-// 17 MB of shared keys and 78 MB of own ones (15 us at 6.5 TB/s), 4.6 GFLOP (3 us); read once a sequence they were 1.15 GB. It takes 31 us, 16 of them beside the
-// shared keys, whose CTAs leave room for one of the own keys' on an SM; then three fit one. There a CTA's own steps count: four loads one after another (row, group,
-// page numbers, keys) before the first product, five blocks to a warp, two waits to join the parts. 128 tokens, 16384 shared and 256 own keys: 68 us, 39 of them the
+// 17 MB of shared keys and 78 MB of own ones (15 us at 6.5 TB/s), 4.6 GFLOP (3 us); read once a sequence they were 1.15 GB. It takes 28 us, about 16 of them beside the
+// shared keys. 10 of them are there without any work: two launches, for the shared keys the way from a row number to the first product and back to memory, and the
+// joining. There a CTA's own steps count: four loads one after another (row, group, page numbers, keys), its blocks, two waits to join the parts. What finds no room
+// beside the shared keys takes these steps after them (own_warps): 31 us with four warps to each token. 128 tokens, 16384 shared and 256 own keys: 68 us, 39 of them the
 // shared keys (prefix_attn_tc.cu), which fill the SMs. 4 tokens, 512 shared and 20 own keys: 6 + 5 us, of which 8 remain as the second starts early.
 #include "common.cuh"
 #include "mma_sync.cuh"
@@ -204,7 +205,7 @@ prefix_shared_mma_kernel(const PrefixParams p) {
 // A CTA owns one token and up to eight query heads of one KV head; its warps take blocks of 16 keys in turn, each with a ring of its own that its
 // first lane refills by TMA (one box per page and 64 dimensions, 128-byte swizzle). On mma.sync: S^T = K Q^T, the keys the first operand and the
 // heads the eight columns, then O^T = V^T P^T with V turned by ldmatrix; P changes sides by movmatrix. Rings against 16-byte loads into registers: 64 tokens with
-// 300 keys of their own 33 -> 20 us. Four warps of two stages take 31 us with 4096 shared keys before them; three of two 32, three of three 37, five of two 34.
+// 300 keys of their own 33 -> 20 us. How many warps: own_warps. Rings of three blocks instead of two 37 us (three warps) against 32; five warps of two 34.
 constexpr int kPxOwn = 16, kPxStages = 2, kPxCluster = 4, kPxClusterWarps = 8 * kPxCluster;
 
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
@@ -566,7 +567,7 @@ B200_API int b200_prefix_attn(const void* q, long long q_stride, const void* ck,
   p.longest = longest; p.sinks = sinks; p.out = out; p.T = T; p.H = H; p.G = G; p.D = D; p.nsplit = nsplit;
   p.part_o = part; p.part_ml = part ? part + (long long)T * H * nsplit * D : nullptr;
   p.most_own = most_own > 0 ? most_own : 0x7fffffff;
-  p.beside = tc ? (int)(shared_items(T, n_groups, longest, H / G, G, prefix_tc_tokens(H, G, D)) * nsplit) : 0;
+  p.beside = tc ? shared_items(T, n_groups, longest, H / G, G, prefix_tc_tokens(H, G, D)) * nsplit : 0;
   p.scale_log2 = scale * kPxLog2e;
   return dtype == B200_DT_BF16 ? prefix_attn<__nv_bfloat16>(p, tc, (cudaStream_t)stream) : prefix_attn<__half>(p, tc, (cudaStream_t)stream);
 }

@@ -20,7 +20,7 @@ struct PrefixParams {
   void* out;
   float *part_o, *part_ml;                      // [T, H, nsplit, D], [T, H, nsplit, 2] (maximum in powers of two, sum)
   int T, H, G, D, bs_log2, nsplit;
-  int beside;                                   // CTAs of the tcgen05 kernel, none: 0
+  long long beside;                             // CTAs of the tcgen05 kernel, none: 0
   int most_own;                                 // keys that a token sees to by itself, at most: chooses how they are cut
   float scale_log2;
 };

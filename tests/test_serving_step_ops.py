@@ -511,7 +511,7 @@ def test_temperatures_at_their_bounds(B, e):
 
 
 # ------------------------------------------------------------------------------------------------ attention over shared keys
-def batch_of(groups, alone, own, H, G, D, BS, dtype, seed, copies=False, odd=None):
+def batch_of(groups, alone, own, H, G, D, BS, dtype, seed, copies=False):
     """A decode batch on the CPU: groups (tokens, shared keys), then sequences by themselves, ``own`` keys (cyclic) behind the shared ones. Whole pages of
     the shared part are the same page for all; the page that it ends in is each sequence's copy. All that no sequence holds is NaN."""
     g = torch.Generator().manual_seed(seed)
@@ -612,6 +612,39 @@ def test_few_and_many_rows(entries, dtype, D, groups, own):
     """Work cut into many ranges and into none, tiles that are full and all but empty; copies of the shared keys instead of the same pages."""
     b = batch_of(groups, 0, own, 8, 2, D, 16, dtype, D, copies=len(own) == 1 and groups[0][0] < 40)
     close(call(b, "cuda"), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [18, 48, 70, 120])
+@pytest.mark.parametrize("unknown", [False, True])
+def test_tokens_with_and_without_room_beside_the_shared_keys(dtype, tokens, unknown):
+    """144, 384, 560 and 960 CTAs of own keys (as many as tokens times KV heads) beside 8 to 64 of shared ones: rooms for four, three and two warps to a CTA, and for not
+    even those; two only where the number of own keys is known. A token of the group sees less than the shared part, one nothing at all."""
+    b = batch_of([(tokens, 130)], 0, [1, 40, 7, 100], 16, 8, 128, 16, dtype, tokens)
+    b["pos"][3], b["pos"][5] = 76, -1
+    if unknown:
+        plan = make_prefix_groups(b["plan"], tokens, "cuda")
+        on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
+        close(prefix_attention(on["q"], on["ck"], on["cv"], on["table"][:, :-2], on["pos"], on["slot"], plan, 16, 8, 128, 128 ** -0.5), b)
+    else:
+        close(call(b, "cuda"), b)
+
+
+@pytest.mark.skipif(not nv.lib_path().exists(), reason="no kernel library here")
+def test_plans_by_size():
+    """Which kernel has the shared keys, and in how many ranges; of any sizes, some plan that the call takes."""
+    fn = nv.proto("b200_prefix_attn_plan", [nv.ctypes.c_int] * 8)
+    assert fn(4, 1, 4, 512, 40, 16, 4, 128) < TC                      # up to 32 rows and 1024 keys: mma.sync
+    assert fn(64, 1, 64, 4096, 600, 32, 8, 96) < TC                   # a head size that tcgen05 has not
+    assert fn(64, 1, 64, 4096, 600, 32, 8, 128) == TC + 7             # 28 us; in 8 ranges 31
+    assert fn(128, 1, 128, 16384, 512, 32, 8, 128) == TC + 9          # 68 us; in 4 ranges 80, in 12 82
+    for T, n, longest, shared, own, H, G, D in itertools.product((1, 64, 4096), (1, 5, 300), (1, 4096), (1, 64, 2 ** 31 - 1), (0, 1, 2 ** 31 - 1), (128,), (1, 128), (16, 64, 128)):
+        assert 1 <= fn(T, n, longest, shared, own, H, G, D) % TC <= min(32, -(-shared // 64))
+    for bad in itertools.product((0, 1), repeat=7):
+        if not all(bad):
+            T, n, longest, shared, H, G, D = bad
+            assert fn(T, n, longest, shared, 0, H, G, 16 * D) >= 1
 
 
 TC = 256                      # plan: the tcgen05 kernel
