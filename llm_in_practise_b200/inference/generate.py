@@ -645,6 +645,8 @@ class Generator:
         epoch). Inside a capture the GEMMs run without stream-K and 4-bit weights are expanded in line. ``groups``: up to ``MAX_GROUPS`` of
         (first batch row, rows, shared keys), as for ``make_prefix_groups``: sequences of a paged cache that list the same first blocks."""
         B = tok.shape[0]
+        if groups and not cache.paged:
+            raise ValueError("groups of sequences that list the same first blocks need a paged cache")
         L = cache.len                                   # ``cache.len`` is the caller's to advance, never this method's
         tp = getattr(self.model, "tp", None)
         # under tensor parallelism the step is replayable only when its all-reduce keeps its epoch on the device

@@ -159,6 +159,8 @@ def _check_slot(what, state, n, slot):
 def _check(what, logits, state, slot):
     if logits.dim() != 2 or logits.shape[1] != state.vocab or logits.device != state.device:
         raise ValueError(f"{what}: logits must be [rows, {state.vocab}] on {state.device}, like the state")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: logits must be fp32, bf16 or fp16, not {logits.dtype}")
     if logits.stride(1) != 1 and state.vocab > 1:
         raise ValueError(f"{what}: the logits of a row must be contiguous")
     _check_slot(what, state, logits.shape[0], slot)
@@ -174,7 +176,7 @@ def process_logits(logits: torch.Tensor, state: LogitState, slot: Optional[torch
     elif (out.dtype != torch.float32 or out.shape != logits.shape or out.device != logits.device or (out.stride(1) != 1 and state.vocab > 1)
           or (out.stride(0) < state.vocab and out.shape[0] > 1)):
         raise ValueError("process_logits: out must be fp32, like the logits in shape, with contiguous rows, each of its own")
-    elif _overlap(out, logits) and (out.data_ptr(), out.dtype, out.stride(0)) != (logits.data_ptr(), logits.dtype, logits.stride(0)):
+    elif _overlap(out, logits) and (out.data_ptr(), out.dtype, out.stride(0)) != (logits.data_ptr(), logits.dtype, logits.stride(0) if out.shape[0] > 1 else out.stride(0)):
         raise ValueError("process_logits: out and the logits overlap without being the same")
     if not nv.use_native(logits):
         return out.copy_(_rules_torch(logits, state, slot))

@@ -6,7 +6,7 @@ from fastapi.testclient import TestClient
 
 from llm_in_practise_b200.data.tokenizers import ByteTokenizer
 from llm_in_practise_b200.inference import GenerationConfig, Generator
-from llm_in_practise_b200.inference.generate import MAX_GROUPS, LogitRules, PagedKVCache, group_plan, set_group_plan
+from llm_in_practise_b200.inference.generate import MAX_GROUPS, KVCache, LogitRules, PagedKVCache, group_plan, set_group_plan
 from llm_in_practise_b200.inference.ragged import RaggedGenerator, make_pieces
 from llm_in_practise_b200.models.qwen3 import Qwen3Config, Qwen3ForCausalLM
 from llm_in_practise_b200.ops import _native as nv
@@ -223,6 +223,14 @@ def test_maps_of_a_ragged_step_on_the_device():
     assert (pieces.n_tiles, pieces.n_runs, pieces.longest) == (host.n_tiles, host.n_runs, host.longest)
     for f in ("tiles", "runs", "tile_of", "run_tiles"):
         assert getattr(pieces, f).tolist() == getattr(host, f).tolist() and getattr(pieces, f).dtype == torch.int32 and getattr(pieces, f).is_contiguous()
+
+
+def test_groups_need_pages(model):
+    gen = Generator(model, max_len=64)
+    cache = KVCache(2, 2, 2, 64, 16, torch.float32, "cpu")
+    two = torch.zeros(2, dtype=torch.long)
+    with pytest.raises(ValueError, match="paged"):
+        gen.decode_graphed(two, cache, two.int(), two.int(), groups=[(0, 2, 8)])
 
 
 def test_plans_of_captured_steps():

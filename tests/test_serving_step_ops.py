@@ -426,7 +426,7 @@ def test_refusals_of_rules():
     st = LogitState(4, 100, 8, 2)
     x = torch.zeros(4, 100)
     for bad in (dict(logits=x[0]), dict(logits=x[:, :99]), dict(logits=torch.zeros(5, 100)), dict(slot=torch.zeros(4)), dict(slot=torch.zeros(3, dtype=torch.int32)),
-                dict(logits=torch.zeros(100, 4).t())):
+                dict(logits=torch.zeros(100, 4).t()), dict(logits=x.double())):
         for fn in (process_logits, greedy_tokens):
             with pytest.raises(ValueError, match=fn.__name__):
                 fn(**{**dict(logits=x, state=st), **bad})
