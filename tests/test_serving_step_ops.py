@@ -489,10 +489,26 @@ def test_launches_are_counted(B):
     V = 12800                                                     # four slices a row: 8 and 1200 of them
     st = LogitState(B, V, 4, device="cuda")
     x = torch.randn(B, V, device="cuda")
-    for fn, more in ((process_logits, 0), (greedy_tokens, 1)):
+    for fn, many in ((process_logits, 1 if B == 2 else 2), (greedy_tokens, 1 if B == 2 else 3)):
         before = nv.launch_count
         fn(x, st)
-        assert nv.launch_count - before == (1 if B == 2 else 2) + more
+        assert nv.launch_count - before == many
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1, 127, 1025, 20353, 162815, 162816, 162817])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_best_of_few_rows(V, dtype):
+    """Up to eight rows are a cluster's each, up to 162816 tokens; more rows and tokens go other ways. All of them give the first of the largest."""
+    rows = some_rules(V, 9, V, 30)
+    st = state_of(rows, V, 64, "cuda")
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(9, V, generator=g) * 4).round().div(4).to(dtype).cuda()          # many equals
+    x[1], x[2, V // 2], x[3, -1] = -INF, NAN, INF
+    for n in (1, 8, 9):
+        y = process_logits(x[:n], st)
+        first = torch.where(y.isnan().any(1, keepdim=True), y.isnan(), y == y.nan_to_num(-INF, INF, -INF).amax(1, keepdim=True)).int().argmax(1)
+        assert torch.equal(greedy_tokens(x[:n], st), first)
 
 
 @pytest.mark.gpu
