@@ -10,9 +10,9 @@
 // Bound: the launch. 64 requests read 1 KB and write 2; a step of 60 prompt pieces (60 000 tokens) writes 1 MB, 0.15 us at the memory's
 // rate. The tables take 3.4 us (of 200 requests with 800 000 tokens 4.3), the maps 3.3 (of that step 4.4), about what a kernel of two loads that
 // depend on each other takes; a call is 12 and 23 us, most of it the host's. So each of them is one launch whose CTAs ask each other nothing: a CTA
-// takes kReq requests and adds up the lengths of all requests before them by itself (n values from L2 instead of a pass over the CTAs; sums that
-// pass 2^31 wrap, and writes are checked against the tables' sizes), then its threads share out the tokens of its requests, kChunk to a CTA: a long
-// prompt is spread over the grid's second dimension.
+// takes kReq requests and adds up the lengths of all requests before them by itself (n values from L2 instead of a pass over the CTAs), then its threads
+// share out the tokens of its requests, kChunk to a CTA: a long prompt is spread over the grid's second dimension. Sums stop at 2^31 - 1: what lies that
+// far behind is behind the end of every table, and nothing is written there.
 #include "common.cuh"
 #include "../include/b200_ops.h"
 
@@ -25,20 +25,30 @@ constexpr int kMapTile = 64;        // rows of an attention tile
 
 __device__ __forceinline__ int blocks_of(int tokens, int bs) { return tokens > 0 ? (int)(((long long)tokens + bs - 1) / bs) : 0; }
 
-// Sums of value(i) over requests before this CTA's and, in cu[0 .. kReq], over its own; n requests, blockIdx.x * kReq the first
+constexpr unsigned kMost = 0x7fffffffu;
+
+// a + b of numbers that are not negative, kMost at most: in any order the same
+__device__ __forceinline__ int add_up(int a, int b) { return (int)min((unsigned)a + (unsigned)b, kMost); }
+// a warp's values, by halves of 16 bits, whose sums fit
+__device__ __forceinline__ int add_up_warp(int v) {
+  const unsigned long long lo = __reduce_add_sync(0xffffffffu, (unsigned)v & 0xffffu), hi = __reduce_add_sync(0xffffffffu, (unsigned)v >> 16);
+  return (int)min((hi << 16) + lo, (unsigned long long)kMost);
+}
+
+// Sums of value(i) >= 0 over requests before this CTA's and, in cu[0 .. kReq], over its own; n requests, blockIdx.x * kReq the first
 template <typename F>
 __device__ __forceinline__ int scan_requests(int n, int* cu, int* red, F value) {
   const int first = blockIdx.x * kReq, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int before = 0;
-  for (int i = threadIdx.x; i < first; i += kMapThreads) before += value(i);
-  before = __reduce_add_sync(0xffffffffu, before);
+  for (int i = threadIdx.x; i < first; i += kMapThreads) before = add_up(before, value(i));
+  before = add_up_warp(before);
   if (lane == 0) red[warp] = before;
   if (warp == 0) {
     int v = first + lane < n ? value(first + lane) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+      if (lane >= o) v = add_up(v, u);
     }
     cu[lane + 1] = v;
     if (lane == 0) cu[0] = 0;
@@ -46,7 +56,7 @@ __device__ __forceinline__ int scan_requests(int n, int* cu, int* red, F value) 
   __syncthreads();
   before = 0;
 #pragma unroll
-  for (int w = 0; w < kMapThreads / 32; ++w) before += red[w];
+  for (int w = 0; w < kMapThreads / 32; ++w) before = add_up(before, red[w]);
   return before;
 }
 
@@ -66,20 +76,20 @@ extend_tables_kernel(int* __restrict__ table, long long table_stride, int table_
   __shared__ int cu[kReq + 1], red[kMapThreads / 32];
   auto need = [&](int i) { return max(blocks_of(lens[i], bs) - blocks_of(cached[i], bs), 0); };
   const int before = scan_requests(n, cu, red, need);
-  const int total = cu[kReq];
-  for (int k = blockIdx.y * kChunk + threadIdx.x; k < total; k += gridDim.y * kChunk) {
+  const int total = cu[kReq], live = min(total, max(n_blocks - before, 0));      // blocks that the list still has for them
+  for (unsigned k = blockIdx.y * kChunk + threadIdx.x; k < (unsigned)live; k += gridDim.y * kChunk) {
 #pragma unroll
     for (int u = 0; u < kChunk; u += kMapThreads) {
-      const int kk = k + u;
-      if (kk >= total) break;
+      if (k + u >= (unsigned)live) break;
+      const int kk = (int)(k + u);
       const int j = owner_of(cu, kk), i = blockIdx.x * kReq + j;
       const int row = rows[i], col = blocks_of(cached[i], bs) + kk - cu[j];
-      // a list that ends too early, or a row that is too short, leaves the rest of the row as it was
-      if ((unsigned)row < (unsigned)table_rows && (unsigned)col < (unsigned)width && (unsigned)(before + kk) < (unsigned)n_blocks)
+      // a list that ended too early, or a row that is too short, leaves the rest of the row as it was
+      if ((unsigned)row < (unsigned)table_rows && (unsigned)col < (unsigned)width)
         table[row * table_stride + col] = blocks[before + kk];
     }
   }
-  if (used && blockIdx.y == 0 && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *used = before + total;
+  if (used && blockIdx.y == 0 && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *used = add_up(before, total);
 }
 
 struct StepMapsOut {
@@ -93,14 +103,14 @@ step_maps_kernel(const int* __restrict__ table, long long table_stride, int tabl
   __shared__ int cu[kReq + 1], ct[kReq + 1], red[kMapThreads / 32], red2[kMapThreads / 32];
   const int first = blockIdx.x * kReq;
   const int before = scan_requests(n, cu, red, [&](int i) { return max(fresh[i], 0); });
-  const int mine = cu[kReq];
-  for (int k0 = blockIdx.y * kChunk; k0 < mine; k0 += gridDim.y * kChunk) {
+  const int mine = cu[kReq], live = min(mine, max(total - before, 0));           // tokens that the tables have room for
+  for (unsigned k0 = blockIdx.y * kChunk; k0 < (unsigned)live; k0 += gridDim.y * kChunk) {
 #pragma unroll
     for (int u = 0; u < kChunk; u += kMapThreads) {
-      const int k = k0 + u + threadIdx.x, t = before + k;
-      if (k >= mine || (unsigned)t >= (unsigned)total) break;
+      if (k0 + u + threadIdx.x >= (unsigned)live) break;
+      const int k = (int)(k0 + u + threadIdx.x), t = before + k;
       const int j = owner_of(cu, k), i = first + j;
-      const int p = cached[i] + k - cu[j], row = rows[i];
+      const int p = (int)((unsigned)cached[i] + (unsigned)(k - cu[j])), row = rows[i];      // behind 2^31 - 1: negative, and in no table
       out.pos[t] = p;
       out.slot[t] = row;
       long long at = -1;                                   // a place that no table entry gives
@@ -109,32 +119,31 @@ step_maps_kernel(const int* __restrict__ table, long long table_stride, int tabl
     }
   }
   if (blockIdx.y == 0 && threadIdx.x < kReq && first + threadIdx.x < n) {
-    const int i = first + threadIdx.x, end = before + cu[threadIdx.x + 1];
+    const int i = first + threadIdx.x, end = add_up(before, cu[threadIdx.x + 1]);
     if (i == 0) out.cu[0] = 0;
     out.cu[i + 1] = end;
     out.last[i] = (long long)end - 1;
   }
   if (n_tiles == 0) return;
   const int tiles_before = scan_requests(n, ct, red2, [&](int i) { return blocks_of(fresh[i], kMapTile); });
-  const int my_tiles = ct[kReq];
+  const int my_tiles = ct[kReq], live_tiles = min(my_tiles, max(n_tiles - tiles_before, 0));
   int4* tiles = reinterpret_cast<int4*>(out.tiles);
   int4* tile_of = reinterpret_cast<int4*>(out.tile_of);
-  for (int k = blockIdx.y * kMapThreads + threadIdx.x; k < my_tiles; k += gridDim.y * kMapThreads) {
-    const int t = tiles_before + k;
-    if ((unsigned)t >= (unsigned)n_tiles) break;
+  for (unsigned kt = blockIdx.y * kMapThreads + threadIdx.x; kt < (unsigned)live_tiles; kt += gridDim.y * kMapThreads) {
+    const int k = (int)kt, t = tiles_before + k;
     const int j = owner_of(ct, k), i = first + j, place = k - ct[j];
-    const int row0 = place * kMapTile;
-    tiles[t] = make_int4(before + cu[j] + row0, min(kMapTile, cu[j + 1] - cu[j] - row0), cached[i] + row0, rows[i]);
-    tile_of[t] = make_int4(i, place, ct[j + 1] - ct[j], tiles_before + ct[j]);
+    const int row0 = place * kMapTile, rows_i = max(fresh[i], 0);
+    tiles[t] = make_int4(add_up(add_up(before, cu[j]), row0), min(kMapTile, rows_i - row0), (int)((unsigned)cached[i] + (unsigned)row0), rows[i]);
+    tile_of[t] = make_int4(i, place, blocks_of(rows_i, kMapTile), tiles_before + ct[j]);
   }
   if (blockIdx.y == 0 && threadIdx.x < kReq && first + threadIdx.x < n) {
     const int j = threadIdx.x, i = first + j;
-    reinterpret_cast<int4*>(out.runs)[i] = make_int4(before + cu[j], cu[j + 1] - cu[j], cached[i], rows[i]);
-    reinterpret_cast<int4*>(out.run_tiles)[i] = make_int4(tiles_before + ct[j], ct[j + 1] - ct[j], 0, 0);
+    reinterpret_cast<int4*>(out.runs)[i] = make_int4(add_up(before, cu[j]), max(fresh[i], 0), cached[i], rows[i]);
+    reinterpret_cast<int4*>(out.run_tiles)[i] = make_int4(add_up(tiles_before, ct[j]), blocks_of(fresh[i], kMapTile), 0, 0);
   }
   // tiles that the caller's bound has too many of are of no rows
   if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0)
-    for (int t = max(tiles_before + my_tiles, 0) + threadIdx.x; t < n_tiles; t += kMapThreads) tiles[t] = tile_of[t] = make_int4(0, 0, 0, 0);
+    for (unsigned t = (unsigned)add_up(tiles_before, my_tiles) + threadIdx.x; t < (unsigned)n_tiles; t += kMapThreads) tiles[t] = tile_of[t] = make_int4(0, 0, 0, 0);
 }
 
 // chunks along the second dimension: enough for kReq requests to hold all of `items`, at most 256 (the rest in turn)

@@ -774,7 +774,7 @@ int b200_prefix_attn(const void* q, long long q_stride, const void* ck, const vo
 /* Block tables and maps of a serving step (csrc/step_maps.cu), from the requests' lengths on the device: rows, cached, lens / fresh int32 [n]
  * (row of the block table, tokens in the cache, tokens after / new in the step); table int32, rows of table_stride entries of which
  * width are used. extend: row i gets blocks ceil(cached / bs) .. ceil(lens / bs) - 1 off the list `blocks` in request order; used (int32, may be
- * NULL): how many they need. Entries outside the table or beyond the list are left alone. maps: cu int32 [n + 1], pos / slot int32 [total], place
+ * NULL): how many they need. Sums of lengths stop at 2^31 - 1. Entries outside the table or beyond the list are left alone. maps: cu int32 [n + 1], pos / slot int32 [total], place
  * int64 [total] (block * bs + offset, -1 where none is listed), last int64 [n]; with n_tiles > 0 tiles / tile_of int32 [n_tiles, 4] and runs /
  * run_tiles int32 [n, 4], 16-byte aligned. */
 int b200_extend_block_tables(void* table, long long table_stride, int table_rows, int width, const void* rows, const void* cached,

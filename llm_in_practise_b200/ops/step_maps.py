@@ -21,6 +21,7 @@ from . import _native as nv
 vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 _EXTEND_ARGS = [vp, i64, i32, i32, vp, vp, vp, vp, i32, vp, i32, i32, vp]
 _MAPS_ARGS = [vp, i64, i32, i32, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+MOST = 2 ** 31 - 1   # sums of lengths stop there
 TILE_Q = 64          # query rows per tile of the tensor-core attention kernels
 
 
@@ -64,8 +65,8 @@ def extend_block_tables(table: torch.Tensor, rows: torch.Tensor, cached: torch.T
     """Give every request the blocks it lacks: row ``rows[i]`` of ``table`` (int32 [rows, max_blocks], changed in place) lists
     ``ceil(cached[i] / block_size)`` blocks and gets the next ``ceil(lens[i] / block_size) - that`` of the list ``blocks`` (int32) behind them, in the
     order of the requests (none where a length shrinks). ``rows`` are different rows. Returns the number of blocks that the requests need, int32 [1]
-    on the device: where it is more than ``blocks`` holds, entries beyond the list stay as they were, and so do those beyond the table's
-    width. With ``block_size`` 1 ``cached`` and ``lens`` count blocks."""
+    on the device (``MOST`` where it is more): where it is more than ``blocks`` holds, entries beyond the list stay as they were, and so do those beyond
+    the table's width. With ``block_size`` 1 ``cached`` and ``lens`` count blocks."""
     _check("extend_block_tables", table, rows, block_size, cached, lens)
     if blocks.dim() != 1 or not _ints(blocks.shape[0], table.device, (blocks,)):
         raise ValueError(f"extend_block_tables: blocks must be a contiguous int32 tensor on the table's device, {table.device}")
@@ -81,11 +82,11 @@ def extend_block_tables(table: torch.Tensor, rows: torch.Tensor, cached: torch.T
     free = blocks.tolist()
     for row, c, k in zip(rows.tolist(), cached.tolist(), lens.tolist()):
         have, want = -(-max(c, 0) // block_size), -(-max(k, 0) // block_size)
-        for j in range(have, want):
-            if 0 <= row < table.shape[0] and j < table.shape[1] and at < len(free):
-                table[row, j] = free[at]
-            at += 1
-    return used.fill_(at)
+        if 0 <= row < table.shape[0]:
+            for j in range(have, min(want, table.shape[1], have + len(free) - at)):
+                table[row, j] = free[at + j - have]
+        at += max(want - have, 0)
+    return used.fill_(min(at, MOST))
 
 
 def step_maps(table: torch.Tensor, rows: torch.Tensor, cached: torch.Tensor, new: torch.Tensor, block_size: int, total: int,
@@ -93,7 +94,7 @@ def step_maps(table: torch.Tensor, rows: torch.Tensor, cached: torch.Tensor, new
     """Maps of a step in which request i brings ``new[i]`` tokens from position ``cached[i]`` on (``rows``, ``cached``, ``new`` int32 [n]; ``table``
     int32 [rows, max_blocks] lists their blocks already). ``total``: the step's tokens, as known to the host: rows of the result, which where
     it is larger than the sum of ``new`` are not written behind that sum. ``n_tiles`` > 0: tables of the tiles too, so many of them; where the step
-    has fewer, the others are of no rows (where more, they are left out)."""
+    has fewer, the others are of no rows (where more, they are left out). Positions are below 2^31, and ``cu`` stops at ``MOST``."""
     _check("step_maps", table, rows, block_size, cached, new)
     n, dev = rows.shape[0], table.device
     if n < 1 or total < 0 or n_tiles < 0:
@@ -124,29 +125,31 @@ def _step_maps_torch(table, rows, cached, new, bs, total, n_tiles) -> StepMaps:
     dev, n = table.device, rows.shape[0]
     pos, slot = (torch.zeros(total, dtype=torch.int32, device=dev) for _ in range(2))
     place = torch.zeros(total, dtype=torch.int64, device=dev)
-    cu, tiles, tile_of, run_tiles = [0], [], [], []
+    cu, tiles, tile_of, run_tiles, at = [0], [], [], [], 0
     new_l = [max(0, k) for k in new.tolist()]
     for i, (row, c, k) in enumerate(zip(rows.tolist(), cached.tolist(), new_l)):
-        nt, at = -(-k // TILE_Q), len(tiles)
-        tiles += [[cu[-1] + a, min(TILE_Q, k - a), c + a, row] for a in range(0, k, TILE_Q)]
-        tile_of += [[i, j, nt, at] for j in range(nt)]
-        run_tiles.append([at, nt, 0, 0])
+        nt = -(-k // TILE_Q)
+        some = range(max(0, min(nt, n_tiles - at)))
+        tiles += [[min(cu[-1] + j * TILE_Q, MOST), min(TILE_Q, k - j * TILE_Q), c + j * TILE_Q, row] for j in some]
+        tile_of += [[i, j, nt, at] for j in some]
+        run_tiles.append([min(at, MOST), nt, 0, 0])
+        at += nt
         live = max(0, min(k, total - cu[-1]))
         p = torch.arange(c, c + live, device=dev)
         pos[cu[-1]:cu[-1] + live] = p.to(torch.int32)
         slot[cu[-1]:cu[-1] + live] = row
-        listed = (p >= 0) & (p // bs < table.shape[1])
+        listed = (p >= 0) & (p <= MOST) & (p // bs < table.shape[1])
         if 0 <= row < table.shape[0] and bool(listed.any()):
             blk = table[row, (p // bs).clamp(0, table.shape[1] - 1)].long()
             place[cu[-1]:cu[-1] + live] = torch.where(listed, blk * bs + p % bs, -1)
         else:
             place[cu[-1]:cu[-1] + live] = -1
         cu.append(cu[-1] + k)
-    cu_t = torch.tensor(cu, dtype=torch.int32, device=dev)
+    cu_t = torch.tensor([min(c, MOST) for c in cu], dtype=torch.int32, device=dev)
     maps = StepMaps(cu_t, pos, slot, place, cu_t[1:].long() - 1)
     if n_tiles:
         def table4(x, m):
-            return torch.tensor((x + [[0, 0, 0, 0]] * m)[:m], dtype=torch.int32, device=dev).view(-1, 4)
+            return torch.tensor((x + [[0, 0, 0, 0]] * m)[:m], device=dev).to(torch.int32).view(-1, 4)
         maps.tiles, maps.tile_of = table4(tiles, n_tiles), table4(tile_of, n_tiles)
         maps.run_tiles = table4(run_tiles, n)
         maps.runs = torch.stack([cu_t[:-1], torch.tensor(new_l, dtype=torch.int32, device=dev), cached, rows], 1)

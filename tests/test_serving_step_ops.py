@@ -138,6 +138,41 @@ def test_step_maps_keep_to_their_bounds(device):
     assert -1 in want["place"][70:73] and -1 in want["place"][-7:]
 
 
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("n", [4, 70])
+def test_lengths_whose_sums_pass_31_bits(device, n):
+    """Requests that need more blocks, or bring more tokens, than 32 bits count: those before them have theirs, those behind them nothing, never the first ones'
+    again; sums stop at 2^31 - 1. The last of 70 is in another CTA than the long ones."""
+    most = 2 ** 31 - 1
+    lens = [5, most, most] + [3] * (n - 3)
+    rows = list(range(n))
+    before = [[-5] * 6 for _ in range(n)]
+    zeros, blocks = [0] * n, list(range(100, 109))
+    table = i32(before, device)
+    used = extend_block_tables(table, i32(rows, device), i32(zeros, device), i32(lens, device), i32(blocks, device), 1)
+    assert used.tolist() == [most] and table[0].tolist() == [100, 101, 102, 103, 104, -5] and table[1].tolist() == [105, 106, 107, 108, -5, -5]
+    assert bool((table[2:] == -5).all())
+    used = extend_block_tables(table, i32(rows, device), i32(zeros, device), i32([most, 0, 0] + lens[3:], device), i32(list(range(7)), device), 16)
+    assert used.tolist() == [2 ** 27 + n - 3] and table[0].tolist() == [0, 1, 2, 3, 4, 5] and bool((table[2:] == -5).all())
+
+    table = torch.arange(6 * n, dtype=torch.int32).view(n, 6)
+    lens = [70] + lens[1:]
+    cached = [2, 9, most - 64] + [0] * (n - 3)
+    want = [list(range(2, 72)) + list(range(9, 39)), [0] * 70 + [1] * 30]
+    m = step_maps(table.to(device), i32(rows, device), i32(cached, device), i32(lens, device), 16, 100, n_tiles=5)
+    assert [m.pos.tolist(), m.slot.tolist()] == want
+    assert m.place.tolist() == [int(table[s, p // 16]) * 16 + p % 16 for p, s in zip(*want)]
+    assert m.cu.tolist() == [0, 70] + [most] * (n - 1) and m.last.tolist() == [69] + [most - 1] * (n - 1)
+    assert m.tiles.tolist() == [[0, 64, 2, 0], [64, 6, 66, 0], [70, 64, 9, 1], [134, 64, 73, 1], [198, 64, 137, 1]]
+    nt = 2 ** 25
+    assert m.tile_of.tolist() == [[0, 0, 2, 0], [0, 1, 2, 0], [1, 0, nt, 2], [1, 1, nt, 2], [1, 2, nt, 2]]
+    assert m.runs[:4].tolist() == [[0, 70, 2, 0], [70, most, 9, 1], [most, most, most - 64, 2], [most, 3, 0, 3]]
+    assert m.run_tiles[:4].tolist() == [[0, 2, 0, 0], [2, nt, 0, 0], [2 + nt, nt, 0, 0], [2 + 2 * nt, 1, 0, 0]]
+    # a position behind the last of 32 bits has no place
+    m = step_maps(table.to(device), i32([0], device), i32([most - 1], device), i32([4], device), 2 ** 30, 4, n_tiles=1)
+    assert m.place.tolist() == [(int(table[0, 1]) * 2 ** 30) + 2 ** 30 - 2, (int(table[0, 1]) * 2 ** 30) + 2 ** 30 - 1, -1, -1] and m.tiles.tolist() == [[0, 4, most - 1, 0]]
+
+
 def test_refusals_of_tables():
     t, r = torch.zeros(4, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
     for bad in (dict(table=t.long()), dict(rows=r.long()), dict(cached=r[:1]), dict(lens=r.view(1, 2)), dict(block_size=0), dict(table=t.t()), dict(table=t[:1].expand(4, 4)),
