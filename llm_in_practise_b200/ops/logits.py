@@ -13,6 +13,7 @@ r, f, p are HF's ``repetition_penalty`` (Quantization/GPTQModel/inference_qwen3_
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import Dict, Optional, Sequence
 
 import torch
@@ -26,6 +27,7 @@ MAX_VOCAB = 1 << 19
 MAX_BIAS = 2047          # biases of one row
 MAX_HISTORY = (1 << 20) - 1      # tokens of one row's history
 SCALES = (2.0 ** -126, 2.0 ** 126)       # repetition penalties and temperatures: numbers whose reciprocal has all its bits
+_LOCK = threading.RLock()       # held while a state's tensors are exchanged or their addresses are taken
 
 
 class _Rules(ctypes.Structure):
@@ -41,7 +43,7 @@ class LogitState:
     (the first and the last of these four within ``SCALES``); ``bias_ids`` int32 / ``bias_values`` fp32 [rows, max_bias] with ``bias_length`` [rows]; after ``allow_masks()`` ``mask`` int32
     [rows, ceil(vocab / 32)] (bit v % 32 of word v // 32 set: token v is allowed) and ``masked`` bool [rows]. Tokens outside 0 .. vocab - 1 are
     passed over, and of biases for one token the last one counts. Sequences, and calls on several streams, may share a state as long as
-    nobody writes the rows that another call reads."""
+    nobody writes the rows that another call reads; tensors put in place of others count from the next call on."""
 
     def __init__(self, rows: int, vocab: int, max_len: int, max_bias: int = 0, device=None):
         if rows < 1 or not 1 <= vocab <= MAX_VOCAB or not 1 <= max_len <= MAX_HISTORY or not 0 <= max_bias <= MAX_BIAS:
@@ -63,8 +65,11 @@ class LogitState:
     def allow_masks(self) -> "LogitState":
         """Room for a mask a row (all of them off). A graph captured before there is room applies no masks."""
         if self.mask is None:
-            self.mask = torch.zeros(self.rows, self.words, dtype=torch.int32, device=self.device)
-            self.masked = torch.zeros(self.rows, dtype=torch.bool, device=self.device)
+            mask = torch.zeros(self.rows, self.words, dtype=torch.int32, device=self.device)
+            masked = torch.zeros(self.rows, dtype=torch.bool, device=self.device)
+            with _LOCK:                                  # both at once, and not over masks that another thread made room for meanwhile
+                if self.mask is None:
+                    self.__dict__.update(mask=mask, masked=masked, _struct=None)
         return self
 
     def set_row(self, row: int, prompt: Sequence[int] = (), output: Sequence[int] = (), repetition_penalty: float = 1.0, presence_penalty: float = 0.0,
@@ -124,16 +129,22 @@ class LogitState:
                 self.length[s] = at + 1
 
     def __setattr__(self, name, value):
-        object.__setattr__(self, name, value)
-        self.__dict__["_struct"] = None                  # holds the tensors' addresses
+        with _LOCK:
+            object.__setattr__(self, name, value)
+            self.__dict__["_struct"] = None              # holds the tensors' addresses
 
-    def _address(self) -> int:
-        if self._struct is None:
-            self._check_tensors()
-            self.__dict__["_struct"] = _Rules(*(nv.ptr(getattr(self, n)) for n, _ in _Rules._fields_[:12]), self.rows, self.max_len, self.max_bias,
-                                              self.words)
-        return ctypes.addressof(self._struct)
-
+    def _address(self) -> _Rules:
+        """What a native call takes the address of. Whoever calls holds it until the call is back: it keeps the tensors that it names, and another thread
+        may have put others in their place by then."""
+        rules = self._struct
+        if rules is None:
+            with _LOCK:
+                self._check_tensors()
+                tensors = [getattr(self, n) for n, _ in _Rules._fields_[:12]]
+                rules = _Rules(*map(nv.ptr, tensors), self.rows, self.max_len, self.max_bias, self.words)
+                rules.tensors = tensors
+                self.__dict__["_struct"] = rules
+        return rules
 
     def _check_tensors(self) -> None:
         """Tensors that were put in place of the state's own are like them."""
@@ -183,8 +194,8 @@ def process_logits(logits: torch.Tensor, state: LogitState, slot: Optional[torch
     if logits.shape[0] == 0:
         return out
     work, launches = _workspace(state, logits.shape[0], 0)
-    fn = nv.proto("b200_process_logits", _PROCESS_ARGS)
-    nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), logits.shape[0], state.vocab, nv.ptr(slot), state._address(),
+    fn, rules = nv.proto("b200_process_logits", _PROCESS_ARGS), state._address()
+    nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), logits.shape[0], state.vocab, nv.ptr(slot), ctypes.addressof(rules),
                         work.data_ptr(), out.data_ptr(), out.stride(0), nv.dtype_code(logits.dtype)), "process_logits")
     nv.count_launch(launches)
     return out
@@ -219,9 +230,9 @@ def greedy_tokens(logits: torch.Tensor, state: LogitState, slot: Optional[torch.
     if B == 0:
         return ids
     work, launches = _workspace(state, B, 1)
-    fn = nv.proto("b200_greedy_tokens", _GREEDY_ARGS)
-    nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), B, state.vocab, nv.ptr(slot), state._address(), work.data_ptr(),
-                        ids.data_ptr(), nv.dtype_code(logits.dtype)), "greedy_tokens")
+    fn, rules = nv.proto("b200_greedy_tokens", _GREEDY_ARGS), state._address()
+    nv.check(nv.call_on(state.device, fn, logits.data_ptr(), logits.stride(0), B, state.vocab, nv.ptr(slot), ctypes.addressof(rules),
+                        work.data_ptr(), ids.data_ptr(), nv.dtype_code(logits.dtype)), "greedy_tokens")
     nv.count_launch(launches)
     return ids
 

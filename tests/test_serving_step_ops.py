@@ -2,8 +2,10 @@
 requests' lengths, rules on logits. Each against a statement of its own in 64 bits (or in whole numbers), token by token; the plain PyTorch
 path on the CPU, the kernels on the GPU."""
 import collections
+import gc
 import itertools
 import re
+import weakref
 
 import pytest
 import torch
@@ -11,6 +13,7 @@ import torch
 import test_kernel_sources_cpu as sources
 
 from llm_in_practise_b200.ops import _native as nv
+from llm_in_practise_b200.ops import logits as logits_module
 from llm_in_practise_b200.ops.logits import LogitState, greedy_tokens, process_logits
 from llm_in_practise_b200.ops.prefix_attention import make_prefix_groups, prefix_attention
 from llm_in_practise_b200.ops.step_maps import extend_block_tables, step_maps
@@ -506,6 +509,45 @@ def test_tensors_in_place_of_the_state_s_own():
     st.temperature = torch.full((4,), 2.0)
     st.mask, st.masked = torch.zeros(4, 4, dtype=torch.int32), torch.ones(4, dtype=torch.bool)
     st._address()
+
+
+def test_a_call_holds_what_it_was_given(monkeypatch):
+    """Another thread puts a tensor in place while a call is on its way: the struct that the call was given, and the tensors it names, live until the call
+    is back."""
+    st, x = LogitState(4, 100, 8), torch.zeros(4, 100)
+    seen = []
+
+    def entry(*args):
+        struct = weakref.ref(st._struct)
+        old = [weakref.ref(t) for t in (st.tokens, st.temperature)]
+        st.tokens, st.temperature = torch.zeros(4, 8, dtype=torch.int32), torch.ones(4)
+        gc.collect()
+        seen.append(struct() is not None and all(t() is not None for t in old))
+        return 0
+    monkeypatch.setattr(logits_module, "_workspace", lambda *a: (torch.zeros(16, dtype=torch.uint8), 1))
+    for name, fake in (("use_native", lambda *a: True), ("proto", lambda *a: entry), ("call_on", lambda dev, fn, *a: fn(*a, 0))):
+        monkeypatch.setattr(nv, name, fake)
+    process_logits(x, st)
+    greedy_tokens(x, st)
+    assert seen == [True, True]
+
+
+def test_masks_of_a_state_that_others_use(monkeypatch):
+    """Room for masks, made while other threads call with the state and set a mask of their own: a call sees both tensors or none, and no mask is lost."""
+    st, real, nested = LogitState(4, 100, 8), torch.zeros, []
+
+    def zeros(*args, **kw):
+        st._address()
+        if not nested:
+            nested.append(1)
+            st.set_mask(1, [3])
+        return real(*args, **kw)
+    monkeypatch.setattr(torch, "zeros", zeros)
+    st.allow_masks()
+    monkeypatch.undo()
+    assert st.masked.tolist() == [False, True, False, False] and int(st.mask[1, 0]) == 8
+    struct = st._address()
+    assert (struct.mask, struct.masked) == (st.mask.data_ptr(), st.masked.data_ptr())
 
 
 def test_scales_at_their_bounds():
