@@ -99,13 +99,18 @@ class LogitState:
 
     def set_mask(self, row: int, allowed: Optional[Sequence[int]]) -> None:
         """The tokens that may come next in ``row`` (None: all of them)."""
-        if allowed is None:
+        if not 0 <= row < self.rows:
+            raise ValueError(f"LogitState: no row {row} of {self.rows}")
+        ids = None if allowed is None else torch.as_tensor(list(allowed), dtype=torch.long)
+        if ids is not None and len(ids) and not 0 <= int(ids.min()) <= int(ids.max()) < self.vocab:
+            raise ValueError(f"LogitState: a mask names tokens {int(ids.min())} .. {int(ids.max())}, and the vocabulary has {self.vocab}")
+        if ids is None:
             if self.mask is not None:
                 self.masked[row] = False
             return
         self.allow_masks()
         bits = torch.zeros(self.words * 32, dtype=torch.bool)
-        bits[torch.as_tensor(list(allowed), dtype=torch.long)] = True
+        bits[ids] = True
         word = (bits.view(-1, 32).long() << torch.arange(32)).sum(1)
         self.mask[row] = torch.where(word >= 2 ** 31, word - 2 ** 32, word).to(torch.int32).to(self.device)
         self.masked[row] = True

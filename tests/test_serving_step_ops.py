@@ -511,6 +511,23 @@ def test_tensors_in_place_of_the_state_s_own():
     st._address()
 
 
+@pytest.mark.parametrize("room", [False, True])
+def test_masks_of_rows_and_tokens_that_are_not_there_are_refused(room):
+    """They are not counted from the end, and a refused mask leaves the rows as they were."""
+    st = LogitState(3, 64, 4)
+    st.set_row(2, allowed=[5])
+    if not room:
+        st.mask = st.masked = None
+    for row, allowed in ((-1, [1]), (3, [1]), (-1, None), (3, None), (0, [-1]), (0, [1, 64]), (0, torch.tensor([2, -3]))):
+        with pytest.raises(ValueError, match="LogitState"):
+            st.set_mask(row, allowed)
+    if room:
+        assert st.masked.tolist() == [False, False, True] and st.mask.tolist() == [[0, 0], [0, 0], [32, 0]]
+        st.set_mask(0, torch.tensor([0, 63]))
+        st.set_mask(1, range(0))
+        assert st.masked.all() and st.mask[:2].tolist() == [[1, -2 ** 31], [0, 0]]
+
+
 def test_a_call_holds_what_it_was_given(monkeypatch):
     """Another thread puts a tensor in place while a call is on its way: the struct that the call was given, and the tensors it names, live until the call
     is back."""
