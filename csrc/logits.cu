@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(128) greedy_pick_kernel(const unsigned long lo
   if (lane == 0) ids[b] = (long long)(uint32_t)~(uint32_t)m;
 }
 
-// tokens that have come: behind the history of their rows. A full row keeps what it has
+// tokens that have come: behind the history of their rows; one that 32 bits do not hold is none of the vocabulary, and -1. A full row keeps what it has
 __global__ void append_tokens_kernel(int* __restrict__ tokens, int rows, int width, int* __restrict__ length, const int* __restrict__ slot,
                                      const long long* __restrict__ ids, int n) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -556,7 +556,8 @@ __global__ void append_tokens_kernel(int* __restrict__ tokens, int rows, int wid
   if ((unsigned)s >= (unsigned)rows) return;
   const int at = length[s];
   if ((unsigned)at >= (unsigned)width) return;
-  tokens[(long long)s * width + at] = (int)ids[i];
+  const long long id = ids[i];
+  tokens[(long long)s * width + at] = id == (int)id ? (int)id : -1;
   length[s] = at + 1;
 }
 

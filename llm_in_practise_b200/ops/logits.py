@@ -87,14 +87,20 @@ class LogitState:
         bad = [t for t in [*bias, *(() if allowed is None else allowed)] if not 0 <= int(t) < self.vocab]
         if bad:
             raise ValueError(f"LogitState: token {bad[0]} is not one of the vocabulary's {self.vocab}")
-        for t, v in ((self.length, len(hist)), (self.prompt_length, len(prompt)), (self.repetition, repetition_penalty), (self.presence, presence_penalty),
-                     (self.frequency, frequency_penalty), (self.temperature, temperature), (self.bias_length, len(bias))):
+        # all that may fail comes before the first write
+        ids = _in_32_bits(torch.tensor(hist, dtype=torch.int64))
+        bias_ids = torch.tensor([int(k) for k in bias], dtype=torch.int32)
+        values = torch.tensor([float(v) for v in bias.values()], dtype=torch.float32)
+        numbers = [(self.length, len(hist)), (self.prompt_length, len(prompt)), (self.repetition, float(repetition_penalty)),
+                   (self.presence, float(presence_penalty)), (self.frequency, float(frequency_penalty)), (self.temperature, float(temperature)),
+                   (self.bias_length, len(bias))]
+        for t, v in numbers:
             t[row] = v
         if hist:
-            self.tokens[row, :len(hist)] = torch.tensor(hist, dtype=torch.int32).to(self.device)
+            self.tokens[row, :len(hist)] = ids.to(self.device)
         if bias:
-            self.bias_ids[row, :len(bias)] = torch.tensor([int(k) for k in bias], dtype=torch.int32).to(self.device)
-            self.bias_values[row, :len(bias)] = torch.tensor([float(v) for v in bias.values()], dtype=torch.float32).to(self.device)
+            self.bias_ids[row, :len(bias)] = bias_ids.to(self.device)
+            self.bias_values[row, :len(bias)] = values.to(self.device)
         self.set_mask(row, allowed)
 
     def set_mask(self, row: int, allowed: Optional[Sequence[int]]) -> None:
@@ -127,7 +133,7 @@ class LogitState:
             nv.count_launch()
             return
         rows = range(ids.shape[0]) if slot is None else slot.tolist()
-        for s, t in zip(rows, ids.tolist()):
+        for s, t in zip(rows, _in_32_bits(ids).tolist()):
             at = int(self.length[s]) if 0 <= s < self.rows else -1
             if 0 <= at < self.max_len:
                 self.tokens[s, at] = t
@@ -163,6 +169,11 @@ class LogitState:
                 continue
             if t is None or t.dtype is not dtype or t.shape != shape or t.device != self.device or not t.is_contiguous():
                 raise ValueError(f"LogitState: {name} must be a contiguous {dtype} {list(shape)} tensor on {self.device}")
+
+
+def _in_32_bits(ids: torch.Tensor) -> torch.Tensor:
+    """int64 tokens as int32; those that it does not hold are -1, which is no token either."""
+    return torch.where(ids == ids.to(torch.int32), ids, -1).to(torch.int32)
 
 
 def _check_slot(what, state, n, slot):

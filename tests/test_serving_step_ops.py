@@ -511,6 +511,23 @@ def test_tensors_in_place_of_the_state_s_own():
     st._address()
 
 
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+def test_tokens_that_32_bits_do_not_hold(device):
+    """They are not of the vocabulary, and passed over like others that are not: in a prompt, in an output and behind a history. A row that is refused keeps what
+    it has."""
+    V = 50
+    st = LogitState(2, V, 8, 1, device)
+    st.set_row(0, prompt=[2 ** 32 + 3, 7, -2 ** 40], output=[2 ** 32 + 5, 8], frequency_penalty=1.0, repetition_penalty=2.0)
+    st.append(torch.tensor([2 ** 32 + 6, 9], device=device), i32([0, 1], device))
+    y = process_logits(torch.ones(2, V, device=device), st).cpu()
+    assert st.length.tolist() == [6, 1] and y[0].tolist() == [{7: 0.5, 8: -0.5}.get(v, 1.0) for v in range(V)]
+    before = {n: t.clone() for n, t in vars(st).items() if isinstance(t, torch.Tensor)}
+    for bad in (dict(prompt=["a"]), dict(prompt=[1], logit_bias={3: "x"}), dict(prompt=[1], presence_penalty="x")):
+        with pytest.raises((ValueError, TypeError)):
+            st.set_row(0, **bad)
+        assert all(torch.equal(t, before[n]) for n, t in vars(st).items() if n in before)
+
+
 @pytest.mark.parametrize("room", [False, True])
 def test_masks_of_rows_and_tokens_that_are_not_there_are_refused(room):
     """They are not counted from the end, and a refused mask leaves the rows as they were."""
