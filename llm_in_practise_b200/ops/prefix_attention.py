@@ -63,7 +63,8 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
                      sinks: Optional[torch.Tensor] = None, max_pos: int = 0, plan: int = 0) -> torch.Tensor:
     """Context [T, H * D] of token t over keys ``0 .. pos[t]`` of cache row ``slot[t]``, as ``paged_attention`` gives it (same arguments; no
     window), with the shared keys of ``groups`` read once. Tokens of a group whose position is before its last shared key, and tokens of no
-    group, read all their keys by themselves. A token with ``pos`` -1 sees no key: zeros. ``max_pos``: an upper bound of ``pos`` known on the host
+    group, read all their keys by themselves. A token with ``pos`` -1, or a slot outside the table, sees no key: zeros. A table entry that names no
+    page of the pools reads nothing outside of them; what its row gets is without meaning. ``max_pos``: an upper bound of ``pos`` known on the host
     (0: unknown). ``plan``: how the shared keys are cut, as ``b200_prefix_attn`` takes it (include/b200_ops.h); 0: chosen by the sizes.
 
     For caches of 16 bits with head sizes that are multiples of 16 up to 128, pages of a power of two from 8 on (fewer than 2^31 - 256 rows of a
@@ -71,9 +72,10 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     call keeps a workspace of its own."""
     T, H, G, D = q.shape[0], n_heads, n_kv_heads, head_dim
     BS, dt = cache_k.shape[2], q.dtype
-    if (groups is None or groups.n_groups == 0 or not nv.use_native(q) or (dt is not torch.bfloat16 and dt is not torch.float16) or D % 16 or D > 128
-            or BS < 8 or BS & (BS - 1) or cache_k.shape[0] * G * BS >= 2 ** 31 - 256 or table.shape[-1] * BS >= 2 ** 31 - 4096 or not scale > 0):
-        return paged_attention(q, cache_k, cache_v, table.contiguous(), pos, slot, H, G, D, scale, sinks=sinks, max_pos=max_pos)
+    if not nv.use_native(q):
+        return _by_paged_attention(q, cache_k, cache_v, table, pos, slot, H, G, D, scale, sinks, max_pos)
+    others = (groups is None or groups.n_groups == 0 or (dt is not torch.bfloat16 and dt is not torch.float16) or D % 16 or D > 128 or BS < 8 or BS & (BS - 1)
+              or cache_k.shape[0] * G * BS >= 2 ** 31 - 256 or table.shape[-1] * BS >= 2 ** 31 - 4096 or not scale > 0)
     dev, pools = q.device, cache_k.shape
     if cache_k.dtype is not dt or cache_v.dtype is not dt or cache_v.shape != pools or pools[1] != G or pools[3] != D:
         raise ValueError(f"prefix_attention: caches must be {dt} [blocks, {G}, block_size, {D}], both of one shape")
@@ -81,16 +83,23 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
         raise ValueError("prefix_attention: caches must be contiguous and on the queries' device")
     q_ptr, stride = q.data_ptr(), q.stride()
     row = stride[0] if T > 1 else H * D
-    if H % G or len(stride) != 2 or q.shape[1] < H * D or (T and stride[1] != 1) or row < H * D or row % 8 or q_ptr % 16:
+    if H % G or len(stride) != 2 or q.shape[1] < H * D or (T and stride[1] != 1) or (not others and (row < H * D or row % 8 or q_ptr % 16)):
         raise ValueError(f"prefix_attention: queries must be rows of {H * D} or more contiguous values that start on 16 bytes, each of its own")
     if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev or (table.stride(1) != 1 and table.shape[1] > 1):
         raise ValueError("prefix_attention: the block table is int32 [rows, blocks] with contiguous rows on the queries' device")
     if sinks is not None and (sinks.dtype is not torch.float32 or sinks.shape != (H,) or not sinks.is_contiguous() or sinks.device != dev):
         raise ValueError(f"prefix_attention: sinks must be contiguous fp32 [{H}] on the queries' device")
-    of, rows, n_groups, tokens = groups.of, groups.groups, groups.n_groups, (T,)
-    for t, shape in ((pos, tokens), (slot, tokens), (of, tokens), (rows, (n_groups, 4))):
+    tokens = (T,)
+    tables = ((pos, tokens), (slot, tokens)) if others else ((pos, tokens), (slot, tokens), (groups.of, tokens), (groups.groups, (groups.n_groups, 4)))
+    for t, shape in tables:
         if t.dtype is not torch.int32 or t.shape != shape or t.device != dev or not t.is_contiguous():
             raise ValueError(f"prefix_attention: pos, slot and the groups' tables must be contiguous int32 tensors for {T} tokens on the queries' device")
+    if others:
+        if cache_k.data_ptr() % 16 or cache_v.data_ptr() % 16:
+            raise ValueError("prefix_attention: caches must start on 16 bytes")
+        with torch.cuda.device(dev):
+            return _by_paged_attention(q, cache_k, cache_v, table, pos, slot, H, G, D, scale, sinks, max_pos)
+    of, rows, n_groups = groups.of, groups.groups, groups.n_groups
     most_own = max(1, max_pos + 1 - groups.min_shared) if max_pos else 0
     if not plan:
         plan = nv.proto("b200_prefix_attn_plan", _PLAN_ARGS)(T, n_groups, groups.longest, groups.max_shared, most_own, H, G, D)
@@ -102,3 +111,13 @@ def prefix_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
                         out.data_ptr(), part.data_ptr(), plan, most_own, T, H, G, D, BS, scale, nv.dtype_code(dt)), "prefix_attn")
     nv.count_launch(2)
     return out
+
+
+def _by_paged_attention(q, cache_k, cache_v, table, pos, slot, H, G, D, scale, sinks, max_pos):
+    """``paged_attention`` takes slots, positions and pages as they are: what lies outside the table or the pools is seen to here."""
+    if q.shape[0] == 0:
+        return q.new_empty((0, H * D))
+    n, last = table.shape[0], min(table.shape[1] * cache_k.shape[2], 2 ** 31) - 1
+    row = slot.clamp(0, max(n - 1, 0))
+    pos = torch.where(row == slot, pos.clamp(max=last), -1) if n else torch.full_like(pos, -1)
+    return paged_attention(q, cache_k, cache_v, table.clamp(0, cache_k.shape[0] - 1).contiguous(), pos, row, H, G, D, scale, sinks=sinks, max_pos=max_pos)

@@ -908,6 +908,53 @@ def test_other_caches_go_through_paged_attention(entries, device):
     assert "b200_prefix_attn" not in entries
 
 
+FALLBACKS = [(torch.float32, 64, 16), (torch.bfloat16, 24, 16), (torch.bfloat16, 64, 4)]
+
+
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("dtype,D,BS", FALLBACKS)
+@pytest.mark.parametrize("grouped", [True, False])
+def test_other_caches_keep_to_the_same_bounds(device, dtype, D, BS, grouped):
+    """What goes through paged_attention: tokens without a key and slots outside the table are zeros there as well, a position behind the table's last one sees
+    all of its row, an entry that names no page of the pool reads nothing outside of it, and no row of the batch touches another's."""
+    b = batch_of([(6, 40)], 3, [10], 4, 2, D, BS, dtype, 5)
+    want, bound = exact_attention(b, D ** -0.5)
+    b["pos"][[1, 7]] = torch.tensor([-1, 2 ** 31 - 1], dtype=torch.int32)
+    b["slot"][[3, 4, 8]] = torch.tensor([-1, 9, 2 ** 31 - 1], dtype=torch.int32)
+    last = b["table"][7].clone()
+    b["table"][7, 1:] = last[0]                                       # entries behind the sequence's own: its first page again
+    b["table"][5, 40 // BS] = 2 ** 31 - 1
+    b["table"][6, 0] = -1
+    for sinks in (None, torch.zeros(4)):
+        got = call(b, device, groups=None if grouped else [], sinks=sinks)
+        assert (got[[1, 3, 4, 8]] == 0).all()
+        if sinks is None:                                             # by the bound: max_pos, another one now, chooses how the keys are cut
+            assert bool(((got.double().cpu() - want).abs() <= bound)[[0, 2]].all())
+    none = torch.empty(0, dtype=torch.int32)
+    empty = {**b, "q": b["q"][:0], "pos": none, "slot": none, "plan": []}
+    on = {k: v.to(device) for k, v in empty.items() if isinstance(v, torch.Tensor)}
+    assert prefix_attention(on["q"], on["ck"], on["cv"], on["table"], on["pos"], on["slot"], None, 4, 2, D, 0.1, max_pos=5000).shape == (0, 4 * D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D,BS", FALLBACKS)
+def test_refusals_of_other_caches(dtype, D, BS):
+    """What goes through paged_attention is looked at as well before its addresses are taken."""
+    b = batch_of([(4, 40)], 1, [3], 4, 2, D, BS, dtype, 1)
+    other = torch.float16 if dtype is torch.float32 else torch.float32
+    for change in (dict(ck=b["ck"].to(other)), dict(cv=b["cv"].to(other)), dict(cv=b["cv"][:, :1]), dict(q=b["q"][:, :20]), dict(table=b["table"].long()),
+                   dict(pos=b["pos"].long()), dict(slot=b["slot"][:2]), dict(ck=b["ck"].transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises(ValueError, match="prefix_attention"):
+            call({**b, **change}, "cuda")
+    on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
+    args = [on["q"], on["ck"], on["cv"], on["table"], on["pos"], on["slot"], None, 4, 2, D, 0.125]
+    for i, bad in ((0, on["q"].t().contiguous().t()), (3, b["table"]), (4, b["pos"]), (5, b["slot"]), (1, b["ck"]), (7, 3)):
+        with pytest.raises(ValueError, match="prefix_attention"):
+            prefix_attention(*args[:i], bad, *args[i + 1:])
+    with pytest.raises(ValueError, match="sinks"):
+        prefix_attention(*args, sinks=torch.zeros(4))
+
+
 def test_refusals_of_groups():
     for groups in ([(0, 3, 5), (2, 2, 5)], [(-1, 2, 5)], [(3, 2, 5)], [(0, -1, 5)], [(0, 1, -5)]):
         with pytest.raises(ValueError, match="make_prefix_groups"):
