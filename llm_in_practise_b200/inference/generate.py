@@ -56,7 +56,8 @@ class GenerationConfig:
     frequency_penalty: float = 0.0
     logit_bias: Optional[Dict[int, float]] = None
     allowed_token_ids: Optional[Sequence[int]] = None
-    # HF's prefix_allowed_tokens_fn(batch row or request id, its tokens so far) -> the tokens that may come next: a grammar, asked before every token
+    # HF's prefix_allowed_tokens_fn(batch row or request id, its tokens so far) -> the tokens that may come next: a grammar, asked before every token.
+    # Where it allows none of the vocabulary (and of allowed_token_ids) it is an error, as in HF
     prefix_allowed_tokens_fn: Optional[Callable[[int, List[int]], Sequence[int]]] = None
 
     def has_rules(self) -> bool:
@@ -130,11 +131,14 @@ class LogitRules:
             self._fn[row], self._tokens[row] = (cfg.prefix_allowed_tokens_fn, row if name is None else name, always), [*prompt, *output]
 
     def ask(self, row: int) -> None:
-        """Ask the grammar of ``row``, if it has one, what may come next. An exception of the grammar's leaves the row's mask as it was."""
+        """Ask the grammar of ``row``, if it has one, what may come next. Where it allows nothing that could, that is an error: any token would break it. An
+        exception, the grammar's own too, leaves the row's mask as it was."""
         if row in self._fn:
             fn, name, always = self._fn[row]
-            allowed = [int(t) for t in fn(name, list(self._tokens[row]))]
-            self.state.set_mask(row, [t for t in allowed if 0 <= t < self.state.vocab and (always is None or t in always)])
+            allowed = [t for t in map(int, fn(name, list(self._tokens[row]))) if 0 <= t < self.state.vocab and (always is None or t in always)]
+            if not allowed:
+                raise ValueError(f"prefix_allowed_tokens_fn allows no token behind {len(self._tokens[row])} tokens of {name}")
+            self.state.set_mask(row, allowed)
 
     def next(self, logits: torch.Tensor, rows: Sequence[int], cfgs: Sequence[GenerationConfig], generator: Optional[torch.Generator] = None,
              asked: bool = False) -> torch.Tensor:

@@ -119,6 +119,25 @@ def test_sampling_with_rules(model):
     assert set(reqs[0].output_ids) == {3, 4, 5} and set(reqs[1].output_ids) == {9} and set(reqs[2].output_ids) == {0}
 
 
+@pytest.mark.parametrize("sample", [False, True])
+def test_a_grammar_that_allows_nothing_ends_its_own_request(model, sample):
+    """Nothing, nothing of the vocabulary, nothing beside allowed_token_ids: an error of the request's, not a token that its grammar forbids. What runs beside
+    it goes on, and generate raises."""
+    how = dict(do_sample=sample, temperature=1.0, max_new_tokens=5)
+    cfgs = [GenerationConfig(prefix_allowed_tokens_fn=fn, allowed_token_ids=ids, **how) for fn, ids in
+            ((lambda name, toks: [20, 21] if len(toks) < 5 else [], None), (lambda name, toks: [300, -1], None), (lambda name, toks: [7], [8]))]
+    eng = LLMEngine(model, None, EngineArgs(max_num_seqs=4, max_model_len=64))
+    reqs = [eng.submit([1, 2, 3], c) for c in cfgs + [GenerationConfig(allowed_token_ids=[4], max_new_tokens=5)]]
+    while not all(r.done.is_set() for r in reqs):
+        eng.step()
+    for r, n in zip(reqs, (2, 0, 0)):
+        assert r.finish_reason == "error" and "no token" in r.error and len(r.output_ids) == n and set(r.output_ids) <= {20, 21}
+    assert reqs[3].error is None and reqs[3].output_ids == [4] * 5
+    for c in cfgs:
+        with pytest.raises(ValueError, match="no token"):
+            Generator(model, max_len=64).generate(torch.tensor([[1, 2, 3]]), c)
+
+
 def test_rules_that_cannot_hold_are_refused_at_submission(model):
     eng = LLMEngine(model, None, EngineArgs(max_num_seqs=2, max_model_len=64))
     for kw in (dict(logit_bias={300: 1.0}), dict(logit_bias={-1: 1.0}), dict(allowed_token_ids=[5, 300]), dict(presence_penalty=float("nan")),
