@@ -60,6 +60,10 @@ class GenerationConfig:
     # Where it allows none of the vocabulary (and of allowed_token_ids) it is an error, as in HF
     prefix_allowed_tokens_fn: Optional[Callable[[int, List[int]], Sequence[int]]] = None
 
+    def allows_nothing(self) -> bool:
+        """Whether ``allowed_token_ids`` is an empty list: every token would break it."""
+        return self.allowed_token_ids is not None and len(self.allowed_token_ids) == 0
+
     def has_rules(self) -> bool:
         """Whether ``LogitRules`` has anything to do for this configuration that ``sample_next`` does not."""
         return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias or self.allowed_token_ids is not None
@@ -173,6 +177,8 @@ def logit_rules(cfg: GenerationConfig, prompts: torch.Tensor, vocab: int, max_le
     if not cfg.has_rules():
         return None
     cfg.check_rules(vocab, max_len)
+    if cfg.allows_nothing():
+        raise ValueError("allowed_token_ids allows no token")
     rules = LogitRules(prompts.shape[0], vocab, max_len, prompts.device, len(cfg.logit_bias or ()))
     for b, ids in enumerate(prompts.tolist()):
         rules.begin(b, cfg, ids)
@@ -180,7 +186,7 @@ def logit_rules(cfg: GenerationConfig, prompts: torch.Tensor, vocab: int, max_le
 
 
 def _one_at_least(lg: torch.Tensor) -> torch.Tensor:
-    """Rows that allow no token at all draw token 0, as the greedy choice does, instead of failing the batch."""
+    """Rows that allow no token at all draw token 0, as the greedy choice does, instead of failing the batch; their requests end with it."""
     none = (lg == float("-inf")).all(1)
     lg[:, 0] = torch.where(none, torch.zeros_like(lg[:, 0]), lg[:, 0])
     return lg

@@ -581,6 +581,10 @@ class LLMEngine:
         r.stream.put(tok)
         with self.metrics.lock:
             self.metrics.generation_tokens += 1
+        if r.cfg.allows_nothing():                           # the batch's convention for such a row (token 0) is nothing to go on from
+            r.error = "allowed_token_ids allows no token"
+            self._finish(r, "error")
+            return True
         if len(r.output_ids) >= r.cfg.max_new_tokens or len(r.prompt_ids) + len(r.output_ids) >= self.args.max_model_len:
             self._finish(r, "length")
             return True

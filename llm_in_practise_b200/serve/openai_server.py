@@ -163,6 +163,8 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         rules = {} if req is None else {"presence_penalty": float(req.presence_penalty or 0.0), "frequency_penalty": float(req.frequency_penalty or 0.0),
                                         "logit_bias": {int(k): float(v) for k, v in (req.logit_bias or {}).items()} or None,
                                         "allowed_token_ids": req.allowed_token_ids}
+        if rules.get("allowed_token_ids") == []:
+            raise ValueError("allowed_token_ids allows no token")
         t = 0.0 if temperature is None else float(temperature)
         return GenerationConfig(max_new_tokens=int(max_tokens or 16), do_sample=t > 0.0, temperature=max(t, 1e-5),
                                 top_p=1.0 if top_p is None else float(top_p), top_k=int(top_k or 0),

@@ -138,6 +138,23 @@ def test_a_grammar_that_allows_nothing_ends_its_own_request(model, sample):
             Generator(model, max_len=64).generate(torch.tensor([[1, 2, 3]]), c)
 
 
+def test_an_empty_list_of_allowed_tokens(model):
+    """generate and the HTTP server refuse it; a request of the engine's ends with an error at its first token."""
+    with pytest.raises(ValueError, match="allowed_token_ids"):
+        Generator(model, max_len=64).generate(torch.tensor([[1, 2, 3]]), max_new_tokens=3, allowed_token_ids=[])
+    eng = LLMEngine(model, ByteTokenizer(), EngineArgs(max_num_seqs=3, max_model_len=64))
+    for how in (dict(), dict(do_sample=True, temperature=1.0)):
+        r, other = (eng.submit([1, 2, 3], GenerationConfig(max_new_tokens=6, allowed_token_ids=ids, **how)) for ids in ([], [9]))
+        while not (r.done.is_set() and other.done.is_set()):
+            eng.step()
+        assert r.finish_reason == "error" and "allowed_token_ids" in r.error and len(r.output_ids) <= 1
+        assert other.error is None and other.output_ids == [9] * 6
+    c = TestClient(build_app(eng, prompt_style="deepseek"))
+    assert c.post("/v1/chat/completions", json={"model": "m", "messages": [{"role": "user", "content": "hi"}], "allowed_token_ids": []}).status_code == 400
+    assert c.post("/v1/completions", json={"model": "m", "prompt": "hi", "allowed_token_ids": []}).status_code == 400
+    assert eng.num_waiting == 0
+
+
 def test_rules_that_cannot_hold_are_refused_at_submission(model):
     eng = LLMEngine(model, None, EngineArgs(max_num_seqs=2, max_model_len=64))
     for kw in (dict(logit_bias={300: 1.0}), dict(logit_bias={-1: 1.0}), dict(allowed_token_ids=[5, 300]), dict(presence_penalty=float("nan")),
