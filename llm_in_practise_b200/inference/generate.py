@@ -145,14 +145,19 @@ class LogitRules:
             self.state.set_mask(row, allowed)
 
     def next(self, logits: torch.Tensor, rows: Sequence[int], cfgs: Sequence[GenerationConfig], generator: Optional[torch.Generator] = None,
-             asked: bool = False) -> torch.Tensor:
+             asked: bool = False, done: Optional[torch.Tensor] = None) -> torch.Tensor:
         """logits [B, V] of sequences ``rows`` (all different) -> next ids [B], which join the rows' histories. ``asked``: their grammars were asked
-        already."""
+        already. ``done`` (bool [B]): sequences that have ended: they are not asked, and what comes for them joins nothing."""
         st, dev = self.state, logits.device
+        gone = {row for row, d in zip(rows, done.tolist()) if d} if done is not None else ()
         for row in () if asked else rows:
-            self.ask(row)
-        slot = torch.tensor(list(rows), dtype=torch.int32)
-        slot = slot.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else slot
+            if row not in gone:
+                self.ask(row)
+
+        def table(x):
+            t = torch.tensor(x, dtype=torch.int32)
+            return t.pin_memory().to(dev, non_blocking=True) if dev.type == "cuda" else t
+        slot = table(list(rows))
         draws: Dict[tuple, List[int]] = {}
         for i, c in enumerate(cfgs):
             if c.do_sample and c.temperature > 0:
@@ -164,10 +169,10 @@ class LogitRules:
             ids = y.argmax(1)
             for at in draws.values():
                 ids[at] = draw_next(_one_at_least(y[at]), cfgs[at[0]], generator)
-        st.append(ids, slot)
+        st.append(ids, table([-1 if row in gone else row for row in rows]) if gone else slot)      # no row of the state: left out
         if self._fn:
             for row, t in zip(rows, ids.tolist()):
-                if row in self._fn:
+                if row in self._fn and row not in gone:
                     self._tokens[row].append(t)
         return ids
 
@@ -726,7 +731,7 @@ class Generator:
         logprobs: List[torch.Tensor] = []
         rules = logit_rules(cfg, input_ids, logits.shape[1], total)
         for _ in range(total - S):
-            nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen)
+            nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen, done=done)
             if return_logprobs:
                 logprobs.append(logits.float().log_softmax(-1).gather(1, nxt[:, None]).squeeze(1))
             nxt = torch.where(done, torch.full_like(nxt, cfg.pad_token_id), nxt)

@@ -239,7 +239,7 @@ class RaggedGenerator(Generator):
         logprobs: List[torch.Tensor] = []
         rules = logit_rules(cfg, input_ids, logits.shape[1], total)
         for n in range(S, total):
-            nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen)
+            nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen, done=done)
             if return_logprobs:
                 logprobs.append(logits.float().log_softmax(-1).gather(1, nxt[:, None]).squeeze(1))
             nxt = torch.where(done, torch.full_like(nxt, cfg.pad_token_id), nxt)

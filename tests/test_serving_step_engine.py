@@ -138,6 +138,48 @@ def test_a_grammar_that_allows_nothing_ends_its_own_request(model, sample):
             Generator(model, max_len=64).generate(torch.tensor([[1, 2, 3]]), c)
 
 
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("sample", [False, True])
+def test_rows_of_generate_that_are_done_are_not_asked(model, tmp_path, ragged, sample):
+    """A row that has ended: its grammar is not called behind its end, and what is drawn for it and thrown away does not join its history. The other rows get what
+    they get with a grammar that says the same without an end."""
+    if ragged:
+        import gorozen_oracle as O
+        from test_gorozen import build
+        cfg = O.make_config(64, 96, [O.attn_layer(4, 2, 32, 16, 100.0, None, mlp=O.dense())])
+        gen = RaggedGenerator(build(tmp_path, cfg, O.random_weights(cfg, seed=15), "cpu", torch.float32), None, 64)
+    else:
+        gen = Generator(model, max_len=64)
+    calls, states = [], []
+
+    def fn(row, toks, strict=True):
+        calls.append((row, list(toks)))
+        if row == 0 and 20 in toks:
+            if strict:
+                raise KeyError("no state behind the end")
+            return [20, 30]
+        return [20] if row == 0 and len(toks) == 5 else [30, 31, 32]
+
+    real = LogitRules.__init__
+
+    def init(self, *a, **kw):
+        real(self, *a, **kw)
+        states.append(self)
+    kw = dict(max_new_tokens=7, eos_token_id=20, pad_token_id=9, do_sample=sample, temperature=1.0, frequency_penalty=0.5)
+    prompts = torch.tensor([[1, 2, 3], [4, 5, 6]])
+    LogitRules.__init__ = init
+    try:
+        out = gen.generate(prompts, seed=3, prefix_allowed_tokens_fn=fn, **kw)
+    finally:
+        LogitRules.__init__ = real
+    assert out[0, 5:].tolist() == [20, 9, 9, 9, 9] and [c[1] for c in calls if c[0] == 0] == [out[0, :n].tolist() for n in (3, 4, 5)]
+    assert [c[1] for c in calls if c[0] == 1] == [out[1, :n].tolist() for n in range(3, 10)]
+    st = states[0].state
+    assert st.length.tolist() == [6, 10] and st.tokens[0, :6].tolist() == out[0, :6].tolist() and st.tokens[1, :10].tolist() == out[1].tolist()
+    free = gen.generate(prompts, seed=3, prefix_allowed_tokens_fn=lambda row, toks: fn(row, toks, False), **kw)
+    assert torch.equal(out, free)
+
+
 def test_an_empty_list_of_allowed_tokens(model):
     """generate and the HTTP server refuse it; a request of the engine's ends with an error at its first token."""
     with pytest.raises(ValueError, match="allowed_token_ids"):
