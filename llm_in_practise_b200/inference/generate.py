@@ -129,10 +129,15 @@ class LogitRules:
         warm = cfg.do_sample and cfg.temperature > 0
         self.state.set_row(row, prompt, output, cfg.repetition_penalty, cfg.presence_penalty, cfg.frequency_penalty, cfg.temperature if warm else 1.0,
                            cfg.logit_bias, cfg.allowed_token_ids)
-        self._fn.pop(row, None)
+        self.end(row)
         if cfg.prefix_allowed_tokens_fn is not None:
             always = None if cfg.allowed_token_ids is None else set(cfg.allowed_token_ids)
             self._fn[row], self._tokens[row] = (cfg.prefix_allowed_tokens_fn, row if name is None else name, always), [*prompt, *output]
+
+    def end(self, row: int) -> None:
+        """The sequence of ``row`` has ended: its grammar and tokens are let go."""
+        self._fn.pop(row, None)
+        self._tokens.pop(row, None)
 
     def ask(self, row: int) -> None:
         """Ask the grammar of ``row``, if it has one, what may come next. Where it allows nothing that could, that is an error: any token would break it. An
@@ -170,7 +175,7 @@ class LogitRules:
             for at in draws.values():
                 ids[at] = draw_next(_one_at_least(y[at]), cfgs[at[0]], generator)
         st.append(ids, table([-1 if row in gone else row for row in rows]) if gone else slot)      # no row of the state: left out
-        if self._fn:
+        if any(row in self._fn for row in rows):
             for row, t in zip(rows, ids.tolist()):
                 if row in self._fn and row not in gone:
                     self._tokens[row].append(t)

@@ -557,6 +557,8 @@ class LLMEngine:
     def _finish(self, r: Request, reason: str) -> None:
         r.finish_reason = reason
         r.finish_time = time.perf_counter()
+        if r.rules_row >= 0:
+            self._rules.end(r.rules_row)
         self._release_slot(r)
         with self.metrics.lock:
             self.metrics.requests_finished[reason] = self.metrics.requests_finished.get(reason, 0) + 1

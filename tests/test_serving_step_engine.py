@@ -1,5 +1,8 @@
 """The operators of a shared serving step where the framework calls them: generation and the engine with rules on the logits, decode steps of
 sequences that share a cached prefix, block tables and maps of the ragged step built on the device."""
+import gc
+import weakref
+
 import pytest
 import torch
 from fastapi.testclient import TestClient
@@ -178,6 +181,36 @@ def test_rows_of_generate_that_are_done_are_not_asked(model, tmp_path, ragged, s
     assert st.length.tolist() == [6, 10] and st.tokens[0, :6].tolist() == out[0, :6].tolist() and st.tokens[1, :10].tolist() == out[1].tolist()
     free = gen.generate(prompts, seed=3, prefix_allowed_tokens_fn=lambda row, toks: fn(row, toks, False), **kw)
     assert torch.equal(out, free)
+
+
+def test_grammars_of_requests_that_ended_are_let_go(model):
+    """Finished, failed and aborted requests: their functions and tokens are not kept for the row, and later steps of others do not wait for their ids."""
+    class Grammar:
+        def __init__(self, fail=False):
+            self.fail = fail
+
+        def __call__(self, name, toks):
+            if self.fail:
+                raise KeyError("failed")
+            return [20, 21]
+
+    eng = LLMEngine(model, None, EngineArgs(max_num_seqs=4, max_model_len=64))
+    grammars = [Grammar(), Grammar(fail=True), Grammar()]
+    refs = [weakref.ref(g) for g in grammars]
+    reqs = [eng.submit([1, 2, 3], GenerationConfig(max_new_tokens=n, prefix_allowed_tokens_fn=g)) for g, n in zip(grammars, (3, 3, 40))]
+    other = eng.submit([1, 2, 3], GenerationConfig(max_new_tokens=30, presence_penalty=0.5))
+    for _ in range(6):
+        eng.step()
+    assert [r.finish_reason for r in reqs] == ["length", "error", None]
+    eng.abort(reqs[2])
+    eng.step()
+    assert reqs[2].finish_reason == "abort" and not other.done.is_set()
+    assert not eng._rules._fn and not eng._rules._tokens
+    del grammars, reqs
+    gc.collect()
+    assert [r() for r in refs] == [None] * 3
+    eng.abort(other)
+    eng.step()
 
 
 def test_an_empty_list_of_allowed_tokens(model):
