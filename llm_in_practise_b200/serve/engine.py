@@ -216,9 +216,10 @@ class LLMEngine:
     # ------------------------------------------------------------------ client side
     @torch.no_grad()
     def warmup(self) -> None:
-        """Capture the CUDA graphs of every prefill bucket and decode bucket up front (dummy tokens in the scratch cache
-        row), so no request pays a capture (~0.1 s each) in its time to first token."""
-        if self.device.type != "cuda" or self.ragged:       # the ragged step runs eagerly: nothing to capture
+        """Capture the CUDA graphs of every prefill bucket and decode bucket, with groups too where decode steps take them, up front (dummy
+        tokens in the scratch cache row), so no request pays a capture (~0.1 s each) in its time to first token. Ragged models capture a decode
+        graph at its first use: there is one for each batch and each context bucket."""
+        if self.device.type != "cuda" or self.ragged:
             return
         scratch = self.args.max_num_seqs
         for tb in self.gen._PREFILL_BUCKETS:
@@ -227,8 +228,10 @@ class LLMEngine:
         nb = 1
         while True:
             z = torch.zeros(nb, dtype=torch.int32, device=self.device)
-            self.gen.decode_graphed(torch.zeros(nb, dtype=torch.long, device=self.device), self.cache, z,
-                                    torch.full((nb,), scratch, dtype=torch.int32, device=self.device))
+            step = (torch.zeros(nb, dtype=torch.long, device=self.device), self.cache, z, torch.full((nb,), scratch, dtype=torch.int32, device=self.device))
+            self.gen.decode_graphed(*step)
+            if self.args.shared_prefix_attention and nb > 1:
+                self.gen.decode_graphed(*step, groups=((0, nb, 1),))        # tokens of one row share its first key
             if nb >= self.args.max_num_seqs:
                 break
             nb *= 2

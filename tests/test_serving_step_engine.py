@@ -429,6 +429,26 @@ def test_engine_with_a_shared_prompt(entries, D, H, Hkv, bs):
 
 
 @gpu
+def test_no_request_pays_for_a_capture():
+    """warmup captures the decode steps with groups too: requests behind one system prompt, in batches of every bucket, add none."""
+    m = qwen("cuda", torch.bfloat16, 64, 8, 2)
+    eng = LLMEngine(m, None, EngineArgs(max_num_seqs=6, max_model_len=256, block_size=16, shared_prefix_attention=True, shared_prefix_min=32))
+    eng.warmup()
+    captured = set(eng.gen._graphs)
+    assert {k[0] for k in captured if k[-1] == "groups"} == {2, 4, 8}
+    torch.manual_seed(4)
+    system = torch.randint(0, 300, (64,)).tolist()
+    first = eng.submit(system + [1], GenerationConfig(max_new_tokens=12, ignore_eos=True))
+    eng.step()
+    reqs = [first] + [eng.submit(system + [i], GenerationConfig(max_new_tokens=3 * i, ignore_eos=True)) for i in range(1, 6)]
+    grouped = 0
+    while not all(r.done.is_set() for r in reqs):
+        eng.step()
+        grouped += bool(eng._shared_groups(eng.running)[1])
+    assert grouped > 5 and set(eng.gen._graphs) == captured
+
+
+@gpu
 def test_gorozen_decodes_groups(tmp_path, entries):
     """The ragged step's decode graph with groups (sinks, keys as values): logits against the oracle, as near as without groups; groups change from replay
     to replay."""
