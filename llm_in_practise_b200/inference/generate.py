@@ -18,6 +18,7 @@ import ctypes
 import math
 import queue
 import threading
+import weakref
 from dataclasses import dataclass
 from typing import Callable, Dict, Iterator, List, Optional, Sequence
 
@@ -547,7 +548,7 @@ class Generator:
             return self._prefill_packed_core(ids_h.to(dev), pos_h.to(dev), row_h.to(dev), cu_h.to(dev), last_h.to(dev),
                                              max(lens), cache)
         key = ("prefill", Tb, id(cache))
-        g = self._graphs.get(key)
+        g = self._graph_of(key, cache)
         if g is None:
             st = {"ids": ids_h.to(dev), "pos": pos_h.to(dev), "row": row_h.to(dev), "cu": cu_h.to(dev), "last": last_h.to(dev)}
             ensure_graph_workspace(dev)
@@ -556,8 +557,8 @@ class Generator:
             graph = torch.cuda.CUDAGraph()
             with no_gc(), torch.cuda.graph(graph):
                 st["logits"] = self._prefill_packed_core(st["ids"], st["pos"], st["row"], st["cu"], st["last"], Tb, cache)
-            g = self._graphs[key] = (graph, st)
-        graph, st = g
+            g = self._graphs[key] = (graph, st, weakref.ref(cache))
+        graph, st, _ = g
         st["ids"].copy_(ids_h, non_blocking=True)
         st["pos"].copy_(pos_h, non_blocking=True)
         st["row"].copy_(row_h, non_blocking=True)
@@ -565,6 +566,11 @@ class Generator:
         st["last"].copy_(last_h, non_blocking=True)
         graph.replay()
         return st["logits"][:n]
+
+    def _graph_of(self, key, cache: KVCache):
+        """What was captured under ``key`` with this very cache: a graph holds its cache's addresses, and another cache may get the id of one that is gone."""
+        g = self._graphs.get(key)
+        return g if g is not None and g[2]() is cache else None
 
     def _fused_tail(self, x: torch.Tensor):
         """The fused-tail context (staging buffer + device state) when every o_proj / down_proj of the model can take the
@@ -677,7 +683,7 @@ class Generator:
             cache.len = L
             return out
         key = (B, id(cache), "groups") if groups else (B, id(cache))
-        g = self._graphs.get(key)
+        g = self._graph_of(key, cache)
         if g is None:
             st = {"tok": tok.clone(), "pos": pos.clone(), "slots": slots.clone(), "plan": group_plan(B, cache.max_len, tok.device) if groups else None}
             ensure_graph_workspace(tok.device)                              # stream-K scratch of captured GEMMs
@@ -686,9 +692,9 @@ class Generator:
             graph = torch.cuda.CUDAGraph()
             with no_gc(), torch.cuda.graph(graph):
                 st["logits"] = self._decode(st["tok"], cache, st["pos"], st["slots"], st["plan"])
-            g = self._graphs[key] = (graph, st)
+            g = self._graphs[key] = (graph, st, weakref.ref(cache))
             cache.len = L
-        graph, st = g
+        graph, st, _ = g
         st["tok"].copy_(tok)
         st["pos"].copy_(pos)
         st["slots"].copy_(slots)

@@ -429,6 +429,33 @@ def test_engine_with_a_shared_prompt(entries, D, H, Hkv, bs):
 
 
 @gpu
+@pytest.mark.parametrize("groups", [(), ((0, 2, 16),)])
+def test_a_cache_that_gets_a_dead_ones_id(groups):
+    """A captured step is replayed for the cache that it was captured with, and for no other that is known by the same number: its keys go where they belong."""
+    gen = Generator(qwen("cuda", torch.bfloat16, 64, 8, 2), max_len=128)
+    tok, pos, slots = torch.tensor([5, 6], device="cuda"), torch.full((2,), 40, dtype=torch.int32, device="cuda"), torch.arange(2, dtype=torch.int32, device="cuda")
+
+    def make():
+        cache = PagedKVCache(2, 20, 2, 16, 64, torch.bfloat16, "cuda", 3, 128)
+        for row, blocks in enumerate(([1, 2, 3], [1, 4, 5])):
+            cache.set_row(row, blocks)
+        return cache
+    old = make()
+    gen.decode_graphed(tok, old, pos, slots, groups=groups)
+    new = make()
+    for key in list(gen._graphs):
+        gen._graphs[tuple(id(new) if k == id(old) else k for k in key)] = gen._graphs.pop(key)
+    for c in (old, new):
+        for pool in c.k + c.v:
+            pool.zero_()
+    logits = gen.decode_graphed(tok, new, pos, slots, groups=groups).clone()
+    again = gen.decode_graphed(tok, new, pos, slots, groups=groups)
+    assert torch.equal(logits, again) and len(gen._graphs) == 1
+    assert not any(bool(pool.any()) for pool in old.k + old.v)
+    assert all(bool((pool[[3, 5], :, 8] != 0).any(2).all()) and int(pool.count_nonzero()) <= 2 * 2 * 64 for pool in new.k + new.v)
+
+
+@gpu
 def test_no_request_pays_for_a_capture():
     """warmup captures the decode steps with groups too: requests behind one system prompt, in batches of every bucket, add none."""
     m = qwen("cuda", torch.bfloat16, 64, 8, 2)
