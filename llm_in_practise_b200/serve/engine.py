@@ -381,14 +381,15 @@ class LLMEngine:
         self._grow_all([(r, n_tokens)])
 
     def _grow_all(self, wanted: Sequence[Tuple[Request, int]]) -> None:
-        """``_grow`` for several requests; the blocks of all of them reach the table in one update."""
+        """``_grow`` for several requests; the blocks of all of them reach the table in one update. Where the pool has too few, none is taken."""
         updates = []
-        for r, n_tokens in wanted:
+        need = [(r, self._nblocks(n_tokens)) for r, n_tokens in wanted]
+        if sum(max(0, want - len(self._slot_blocks.get(r.slot, ()))) for r, want in need) > len(self._free_blocks):
+            raise RuntimeError("KV block pool exhausted (reservation accounting is broken)")
+        for r, want in need:
             blocks = self._slot_blocks.setdefault(r.slot, [])
-            want, first_new = self._nblocks(n_tokens), len(blocks)
+            first_new = len(blocks)
             while len(blocks) < want:
-                if not self._free_blocks:
-                    raise RuntimeError("KV block pool exhausted (reservation accounting is broken)")
                 b = self._free_blocks.pop()
                 self._block_ref[b] = 1
                 blocks.append(b)

@@ -14,6 +14,7 @@ from llm_in_practise_b200.inference.ragged import RaggedGenerator, make_pieces
 from llm_in_practise_b200.models.qwen3 import Qwen3Config, Qwen3ForCausalLM
 from llm_in_practise_b200.ops import _native as nv
 from llm_in_practise_b200.serve import EngineArgs, LLMEngine
+from llm_in_practise_b200.serve.engine import Request
 from llm_in_practise_b200.serve.openai_server import build_app
 from test_serving_step_ops import entries  # noqa: F401
 
@@ -353,6 +354,24 @@ def test_plans_of_captured_steps():
     assert plan.of.tolist() == [-1, 0, 0, 0, 0, 0] and (plan.groups[1:] == 0).all()
     with pytest.raises(ValueError):
         set_group_plan(plan, [(i, 1, 5) for i in range(MAX_GROUPS + 1)])
+
+
+def test_blocks_that_a_step_cannot_have_are_not_booked(model):
+    """Where the pool runs out at one of several requests, none of them has blocks that its row of the table does not list."""
+    eng = LLMEngine(model, None, EngineArgs(max_num_seqs=3, max_model_len=64, block_size=8, num_kv_blocks=7))
+    reqs = [Request(i, [1], GenerationConfig()) for i in range(3)]
+    for i, r in enumerate(reqs):
+        r.slot = i
+    eng._grow_all([(reqs[0], 1)])
+    before = eng.cache.table.clone(), {k: list(v) for k, v in eng._slot_blocks.items()}, list(eng._free_blocks), list(eng._block_ref)
+    with pytest.raises(RuntimeError, match="exhausted"):
+        eng._grow_all([(reqs[0], 9), (reqs[1], 9), (reqs[2], 40)])
+    after = eng.cache.table, {k: v for k, v in eng._slot_blocks.items() if v}, eng._free_blocks, eng._block_ref
+    assert torch.equal(before[0], after[0]) and before[1:] == after[1:]
+    eng._grow_all([(reqs[0], 9), (reqs[1], 9)])
+    for i in (0, 1):
+        blocks = eng._slot_blocks[i]
+        assert eng.cache.table[i, :len(blocks)].tolist() == blocks and all(eng._block_ref[b] == 1 for b in blocks)
 
 
 def test_groups_are_found_among_running_requests(model):
