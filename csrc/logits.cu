@@ -68,10 +68,13 @@ __device__ __forceinline__ RowRules row_rules(const LogitRules& L, int s) {
 }
 
 // y / d: the product with 1 / d, corrected once by what is left of y (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor",
-// 1990), which leaves no more than a division's rounding but in the last of the smallest numbers. Infinities have nothing left over.
+// 1990), which leaves no more than a division's rounding but in the last of the smallest numbers. The product may pass the largest number where the quotient
+// does not: that one goes by halves, which are exact there. An infinite half has nothing left over.
 __device__ __forceinline__ float quotient(float y, float d, float inv) {
-  const float q = __fmul_rn(y, inv), c = __fmaf_rn(__fmaf_rn(-q, d, y), inv, q);
-  return fabsf(q) < INFINITY ? c : q;
+  const float q = __fmul_rn(y, inv);
+  if (fabsf(q) < INFINITY) return __fmaf_rn(__fmaf_rn(-q, d, y), inv, q);
+  const float h = __fmul_rn(0.5f, y), p = __fmul_rn(h, inv);
+  return fabsf(p) < INFINITY ? __fmul_rn(2.f, __fmaf_rn(__fmaf_rn(-p, d, h), inv, p)) : p;
 }
 // four at once, two to an instruction
 __device__ __forceinline__ void over_temperature(float (&y)[4], float T, float inv_T) {

@@ -637,6 +637,32 @@ def test_temperatures_at_their_bounds(B, e):
     assert torch.equal(got.isinf(), want.isinf()) and bool((off <= torch.where(want.abs() < 2.0 ** -126, 2.0 ** -149, 0.0)).all())
 
 
+@pytest.mark.parametrize("device", CPU_AND_GPU)
+@pytest.mark.parametrize("B", [3, 300])
+def test_quotients_next_to_the_largest_number(device, B):
+    """By temperatures and repetition penalties below 1: infinite where the quotient is, and nowhere else. Off by a rounding, and by the correction's own of a
+    remainder, 2^-24 of half a step."""
+    V, top = 12800, torch.finfo(torch.float32).max
+    g = torch.Generator().manual_seed(B)
+    d = 1 - torch.randint(1, 2 ** 23, (B,), generator=g) * 2.0 ** -24
+    x = (top * d.double()[:, None] * (1 - torch.randint(0, 6, (B, V), generator=g) * 2.0 ** -24)).float()
+    x[:, ::2] *= -1
+    want = x.double() / d.double()[:, None]
+    for name in ("temperature", "repetition"):
+        if name == "repetition":
+            x, want = x.abs(), want.abs()
+        st = LogitState(B, V, V, device=device)
+        getattr(st, name).copy_(d)
+        if name == "repetition":
+            st.tokens.copy_(torch.arange(V, dtype=torch.int32).expand(B, V))
+            st.length.fill_(V)
+            st.prompt_length.fill_(V)
+        got = process_logits(x.to(device), st).double().cpu()
+        assert torch.equal(got.isinf(), want.abs() >= 2.0 ** 128 * (1 - 2.0 ** -25))
+        fin = got.isfinite()
+        assert bool(((got - want).abs()[fin] <= want.abs()[fin] * 2.0 ** -24 * (1 + 2.0 ** -20)).all())
+
+
 # ------------------------------------------------------------------------------------------------ attention over shared keys
 def batch_of(groups, alone, own, H, G, D, BS, dtype, seed, copies=False):
     """A decode batch on the CPU: groups (tokens, shared keys), then sequences by themselves, ``own`` keys (cyclic) behind the shared ones. Whole pages of
