@@ -637,6 +637,84 @@ def test_temperatures_at_their_bounds(B, e):
     assert torch.equal(got.isinf(), want.isinf()) and bool((off <= torch.where(want.abs() < 2.0 ** -126, 2.0 ** -149, 0.0)).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 30, 300])
+def test_rules_captured_and_replayed(B):
+    """Each way through the kernels in one graph of a decode step (elsewhere, in place, the best token, which joins the history): the same as eager calls with a
+    state of their own, step after step; rows whose rules change between replays have the new ones."""
+    V = 30522
+    rows = some_rules(V, B, B, 60)
+    st, eager = (state_of(rows, V, 100, "cuda").allow_masks() for _ in range(2))
+    slot = torch.arange(B, dtype=torch.int32, device="cuda").flip(0)
+    x = torch.randn(B, V, device="cuda")
+    place, stream, graph = x.clone(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        y = process_logits(x, st, slot)
+        process_logits(place, st, slot, out=place)
+        ids = greedy_tokens(x, st, slot)
+        st.append(ids, slot)
+    for i in range(6):
+        x.copy_(torch.randn(B, V, device="cuda") * 3)
+        place.copy_(x)
+        if i == 3:
+            for s in (st, eager):
+                s.set_row(0, [1, 2, 3], [4, 4], frequency_penalty=2.0, temperature=0.5, allowed=range(1, V, 3))
+        graph.replay()
+        want, best = process_logits(x, eager, slot), greedy_tokens(x, eager, slot)
+        eager.append(best, slot)
+        assert torch.equal(y, want) and torch.equal(place, want) and torch.equal(ids, best) and torch.equal(best, want.argmax(1))
+    assert torch.equal(st.tokens, eager.tokens) and torch.equal(st.length, eager.length)
+
+
+@pytest.mark.gpu
+def test_a_state_on_two_streams_at_once():
+    """Calls of several sizes on two streams, each with scratch of its own, and of one state that nobody writes."""
+    V = 32768
+    rows = some_rules(V, 40, 7, 60)
+    st = state_of(rows, V, 100, "cuda")
+    xs = [torch.randn(n, V, device="cuda") for n in (2, 40, 300, 9)]
+    slots = [torch.arange(x.shape[0], dtype=torch.int32, device="cuda") % 40 for x in xs]
+    want = [(process_logits(x, st, s), greedy_tokens(x, st, s)) for x, s in zip(xs, slots)]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                for x, s, w in zip(xs, slots, want):
+                    got.append((process_logits(x, st, s), greedy_tokens(x, st, s), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w[0]) and torch.equal(ids, w[1]) for y, ids, w in got)
+
+
+@pytest.mark.gpu
+def test_tables_and_maps_captured_and_replayed():
+    """A decode step's tables and maps in one graph, whose requests' lengths change on the device from replay to replay."""
+    n, bs, width = 70, 16, 20
+    table = torch.zeros(n + 2, width, dtype=torch.int32, device="cuda")
+    rows = torch.randperm(n + 2, generator=torch.Generator().manual_seed(1))[:n].to(torch.int32).cuda()
+    cached, lens, new = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(3))
+    blocks = torch.zeros(n * width, dtype=torch.int32, device="cuda")
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        used = extend_block_tables(table, rows, cached, lens, blocks, bs)
+        m = step_maps(table, rows, cached, new, bs, 1000, n_tiles=80)
+    want, have, free = table.tolist(), [0] * n, list(range(1, n * width + 1))
+    for step in range(5):
+        k = torch.randint(1, 14, (n,), generator=torch.Generator().manual_seed(step)).tolist()
+        for t, v in ((cached, have), (new, k), (lens, [a + b for a, b in zip(have, k)])):
+            t.copy_(torch.tensor(v, dtype=torch.int32))
+        blocks[:len(free)].copy_(torch.tensor(free, dtype=torch.int32))
+        graph.replay()
+        want, at = grown(want, rows.tolist(), have, lens.tolist(), free, bs)
+        assert table.tolist() == want and used.tolist() == [at]
+        maps, T = maps_of(want, rows.tolist(), have, k, bs), sum(k)
+        assert all(getattr(m, f)[:T].tolist() == maps[f] for f in ("pos", "slot", "place")) and m.cu.tolist() == maps["cu"] and m.last.tolist() == maps["last"]
+        assert m.tiles.tolist() == maps["tiles"] + [[0, 0, 0, 0]] * 10 and m.runs.tolist() == maps["runs"]
+        free, have = free[at:], lens.tolist()
+
+
 @pytest.mark.parametrize("device", CPU_AND_GPU)
 @pytest.mark.parametrize("B", [3, 300])
 def test_quotients_next_to_the_largest_number(device, B):
@@ -891,6 +969,27 @@ def test_a_pool_that_32_bits_do_not_address():
     ck[-used:], cv[-used:] = on["ck"], on["cv"]
     out = prefix_attention(on["q"], ck, cv, on["table"] + (n_pages - used), on["pos"], on["slot"], make_prefix_groups(b["plan"], 6, "cuda"), 8, 8, 128, 128 ** -0.5)
     assert torch.equal(out, call(b, "cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups,own,D", [([(64, 4096)], [300, 12], 128), ([(3, 700)], [5], 64), ([(20, 900), (9, 50)], [600, 3, 90], 96), ([(2, 4096)], [3000], 128)])
+def test_calls_repeat_themselves(groups, own, D):
+    """Bit for bit, on two streams at once as well: no sum depends on what is done first."""
+    b = batch_of(groups, 1, own, 8, 2, D, 16, torch.bfloat16, 17)
+    on = {k: v.cuda() for k, v in b.items() if isinstance(v, torch.Tensor)}
+    T = b["q"].shape[0]
+    plan, most = make_prefix_groups(b["plan"], T, "cuda"), int(b["pos"].max())
+
+    def once():
+        return prefix_attention(on["q"], on["ck"], on["cv"], on["table"], on["pos"], on["slot"], plan, 8, 2, D, D ** -0.5, max_pos=most)
+    first, outs, streams = once(), [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                outs.append(once())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
 
 
 @pytest.mark.gpu
