@@ -3,7 +3,7 @@
 // Batch row b follows the rules in row slot[b] of the tables of a LogitState. With l a logit in 32 bits, c(v) how often v stands in the
 // row's output and seen(v) whether it stands in its prompt or output:
 //   y = l;  seen: y < 0 ? y r : y / r;  c > 0: y -= f c, y -= p;  y += bias(v);  y /= T;  not allowed: -inf
-// in this order, each step rounded once to 32 bits. A masked place is minus infinity whatever stood there, NaN included.
+// in this order, each step rounded once to 32 bits. So r scales what the model says and not the bias (where a bias is added first, r scales it too). A masked place is minus infinity whatever stood there, NaN included.
 //   b200_process_logits    y, fp32
 //   b200_greedy_tokens     the best token of each row, the lowest of equals; a NaN is above all (as in torch.argmax)
 //
@@ -18,8 +18,9 @@
 // row, which lie in half of the memory of its 152 000. A stream of four CTAs to an SM that go on from tile to tile leaves room for the settling kernel beside it, but
 // each slows the other: 60 to 74 us. One
 // kernel with the counts of a slice in shared memory is kept waiting by its own steps (rules, history, counts, logits): 100 us in slices of 4096
-// tokens (which small batches keep, see kLmSlices), 69 to 78 in slices of 20480 with the history counted once for clusters of 2 to 8 CTAs (8 rows: 8.8 and 6.5 us, here 9.7). The rules applied in
-// the stream, from records in token order, took 64: almost every warp had a lane with one.
+// tokens (which small batches keep, see kLmSlices), 69 to 78 in slices of 20480 with the history counted once for clusters of 2 to 8 CTAs (8 rows: 8.8 and
+// 6.5 us; by these two kernels 9.7, by the one of small batches 7.2). The rules applied in the stream, from records in token order, took 64: almost every warp
+// had a lane with one.
 #include "common.cuh"
 #include "../include/b200_ops.h"
 

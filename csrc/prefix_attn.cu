@@ -505,13 +505,16 @@ static int prefix_attn(const PrefixParams& p, bool tc, cudaStream_t st) {
 using namespace b200;
 
 // How the shared keys of a call are worked on: the number of ranges (1 .. 32), plus kPxTc where tcgen05 does it.
-// Which kernel: tcgen05 for the head sizes that it has, but for up to 32 rows a group and 1024 keys (32 / 8 heads of 128, one token, 600 keys: 15.4 us, 13.3 on
-// mma.sync; 4096 keys: 19.1 and 19.4, 16000: 29.7 and 37.9; 64 rows, 16000 keys: 30 and 42; 128 rows: 30 and 52).
+// Which kernel: tcgen05 for the head sizes that it has, but for up to 32 rows a group and 1024 keys (device time with up to 20 own keys, each kernel at its best number
+// of ranges; 32 / 8 heads of 128, one token, 600 keys: 9.6 us, 7.6 on mma.sync; 4096 keys: 12.1 and 13.4, 16000: 21.9 and 32; 32 rows, 1024 keys: 9.9 and 9.6, 2048:
+// 10.8 and 11.4; 64 rows, 16000 keys: 22.6 and 37; 128 rows: 24 and 60).
 // How many ranges: those that a cost makes cheapest, in us: the blocks of a CTA, each of which takes longer where an SM has more CTAs (0.72 and 1.15
 // for one and two on tcgen05, 1.7 for each on mma.sync), rounds of CTAs, the ranges' way through L2, written and read at 4 TB/s, a wait for each eight of them where they are joined, and
 // where not all CTAs of own keys have room beside the shared ones (own_warps) their first steps once more. 64 x 4096 keys with 32 / 8 heads and up to 600 own ones:
-// 4, 6, 7, 8, 9 ranges 28, 28, 28, 31, 31 us (chosen: 7); 40 x 3000, 16 / 2 heads: 4, 8, 11, 24 ranges 17, 13, 13, 16 (8); 128 x 16384: 4, 8, 9, 12 ranges 92, 75.5, 75.3, 91 (9); 100 x 8000, 12 / 2 heads of 64: 4, 9, 12, 18 ranges
-// 36, 25.7, 23.7, 26.2 (14).
+// 4, 6, 7, 8, 9 ranges 28, 28, 28, 31, 31 us (chosen: 7); 40 x 3000 and up to 512, 16 / 2 heads: 4, 8, 11, 24 ranges 17, 13.3, 13, 17 (8); 128 x 16384 and up to 512: 4, 8,
+// 9, 12 ranges 80, 68, 69, 83 (9); 100 x 8000 and up to 512, 12 / 2 heads of 64: 4, 9, 12, 14, 18 ranges 30, 19.5, 18, 17.2, 17.5 (14).
+// These are plans of the batch as it is. A captured step has to plan for every batch that it may replay: up to four groups as long as the batch, the cache's longest
+// sequences, own keys unknown. 64 x 4096 and up to 600: 32 instead of 28 us; 40 x 4096: 26.6 and 22.9; 128 x 16384: 78 and 69; 4 x 512 and up to 40 (on tcgen05): 11.3 and 7.9.
 constexpr int kPxTc = 256;
 // CTAs of the shared keys' kernel for one range: tiles of the longest group for each, but no more than the batch can fill
 static long long shared_items(int T, int n_groups, int longest, int rep, int G, int tc_tokens) {

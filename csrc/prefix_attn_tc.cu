@@ -11,7 +11,7 @@
 //
 // Bound: the softmax warps' chain for a block (TMEM load, maximum, exponentials and conversions, TMEM store) beside the tensor pipe, as in the flash forward
 // (flash_tc.cu). 128 tokens x 16384 keys, 32 / 8 heads of 128 (34 GFLOP, 21 us at the 1638 TFLOP/s of a GEMM): 39 us in 9 ranges, 288 CTAs, 0.9 PFLOP/s; the
-// exponentials' unit is busy for 49 % of it, tensor memory for 53. 64 tokens x 4096 keys: 16 us (mma.sync 33), mostly the first loads and the joining.
+// exponentials' unit is busy for 47 % of it, the tensor pipe for 46. 64 tokens x 4096 keys: 16 us (mma.sync 33), mostly the first loads and the joining.
 #include "common.cuh"
 #include "prefix_attn.cuh"
 #include "tma_host.h"
@@ -22,8 +22,8 @@ namespace b200 {
 constexpr int kPtRows = 128, kPtThreads = 192;
 constexpr uint32_t kPtCols = 256, kPtO = 128;
 // How far a row's maximum may run ahead of the number that its weights refer to before O is scaled (an exponent of two). With 32 rows to a warp one of
-// them has a new maximum in almost every block: with no slack 128 x 16384 keys, 32 / 8 heads of 128, take 88 us, with 2^8 75. A weight of up to 256 is rounded
-// like one of up to 1, relative to itself, and sums are in 32 bits.
+// them has a new maximum in almost every block: with no slack 128 x 16384 keys, 32 / 8 heads of 128, and up to 512 own ones take 79 us, with 2^8 69. A weight of
+// up to 256 is rounded like one of up to 1, relative to itself, and sums are in 32 bits.
 constexpr float kPtSlack = 8.f;
 
 template <int D> struct PtSmem {

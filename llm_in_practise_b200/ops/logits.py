@@ -9,6 +9,9 @@ each row without writing the logits out, ``LogitState.append`` puts the tokens t
 
 r, f, p are HF's ``repetition_penalty`` (Quantization/GPTQModel/inference_qwen3_4b_gptq.py:58-68) and the OpenAI API's
 ``frequency_penalty`` and ``presence_penalty``, the bias its ``logit_bias``; the mask is what structured output hands a vLLM server.
+The bias comes behind the repetition penalty, which scales what the model says and not what the caller adds. HF and vLLM add it first and scale
+the sum: for a seen token with both (and r not 1) they give another value, (l + bias) r or (l + bias) / r. All other rules commute or stand in
+one place only.
 """
 from __future__ import annotations
 

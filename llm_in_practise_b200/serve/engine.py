@@ -53,8 +53,9 @@ class EngineArgs:
     # memory (LRU) and copies them back on a later prefix hit instead of recomputing the prompt
     kv_offload_gb: float = 0.0
     # decode steps read the K/V blocks that running sequences share (their cached prefix) once for all of them instead of once each; a paged
-    # cache with prefix caching, one GPU. Sums are then in another order: a logit may differ in its last bits. Groups of at least two
-    # sequences and shared_prefix_min keys count
+    # cache with prefix caching, one GPU. Sums are then in another order, and in a step with groups attention weights, of every sequence and of its own keys
+    # too, are rounded to 16 bits before their product with the values (32 without): about a third more rounding error in attention (ops/prefix_attention.py).
+    # Groups of at least two sequences and shared_prefix_min keys count
     shared_prefix_attention: bool = False
     shared_prefix_min: int = 256
 
