@@ -580,7 +580,7 @@ class LLMEngine:
         if r.first_token_time is None:
             r.first_token_time = now
             self.metrics.observe_ttft(now - r.arrival)
-        if tok in self._eos(r.cfg):
+        if tok in self._eos(r.cfg) and not r.cfg.allows_nothing():
             self._finish(r, "stop")
             return True
         r.output_ids.append(tok)

@@ -225,6 +225,10 @@ def test_an_empty_list_of_allowed_tokens(model):
             eng.step()
         assert r.finish_reason == "error" and "allowed_token_ids" in r.error and len(r.output_ids) <= 1
         assert other.error is None and other.output_ids == [9] * 6
+    r = eng.submit([1, 2, 3], GenerationConfig(max_new_tokens=6, allowed_token_ids=[], eos_token_id=0))          # an end that is not allowed either
+    while not r.done.is_set():
+        eng.step()
+    assert r.finish_reason == "error"
     c = TestClient(build_app(eng, prompt_style="deepseek"))
     assert c.post("/v1/chat/completions", json={"model": "m", "messages": [{"role": "user", "content": "hi"}], "allowed_token_ids": []}).status_code == 400
     assert c.post("/v1/completions", json={"model": "m", "prompt": "hi", "allowed_token_ids": []}).status_code == 400
