@@ -805,7 +805,8 @@ int b200_process_logits(const void* x, long long ldx, int B, int V, const int* s
 /* The best token of each row under these rules, the lowest of equals, NaN above all. */
 int b200_greedy_tokens(const void* x, long long ldx, int B, int V, const int* slot, const b200_logit_rules* rules, void* workspace, long long* ids, int dtype,
                        void* stream);
-/* ids int64 [n] behind the histories of rows slot[i] (NULL: i), whose lengths go up by one; full rows and slots outside the table keep theirs. */
+/* ids int64 [n] behind the histories of rows slot[i] (NULL: i), whose lengths go up by one; full rows and slots outside the table keep theirs. An
+ * id that 32 bits do not hold is noted as -1. */
 int b200_append_tokens(int* tokens, int rows, int width, int* length, const int* slot, const long long* ids, int n, void* stream);
 
 #ifdef __cplusplus
