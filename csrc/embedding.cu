@@ -1,0 +1,300 @@
+// The gradient of an embedding lookup y[t] = s W[id_t], by sorted tokens:
+//     dW[v] = s * sum over t with id_t = v, in the order of t, of dy[t]
+// dense, a row of zeros where a token does not occur; every sum in 32 bits, in an order that is the same in every call (atomics into the
+// table would add in the order in which they arrive). Tokens outside 0 .. V - 1 and the padding token have no gradient.
+//
+//   embed_sort   (token, place) pairs by token, places of a token in order: a radix sort by one cluster of eight CTAs, which hold the counts of
+//                a digit in shared memory and read each other's totals there. T ids make 8 T bytes a pass: the sort is bound by its steps'
+//                latencies, and stands beside the next kernel
+//   embed_fill   zeros, the bulk of what is written for a large vocabulary (V D against T D): bound by HBM
+//   embed_sum    a CTA takes L sorted pairs and a slice of the columns, reads their rows of dy once, and writes each token's sum. A token whose
+//                pairs lie in several CTAs leaves a partial sum in each
+//   embed_join   adds the partial sums of such a token, in order
+#include "common.cuh"
+#include "../include/b200_ops.h"
+
+namespace b200 {
+
+constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 1024, kSortBits = 10;
+constexpr int kSortSmem = (kSortWarps + 3) * kSortBins * 4;
+
+__device__ __forceinline__ uint32_t es_remote(const uint32_t* p, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+
+// Exclusive prefix sums of n <= 1024 numbers in shared memory, in place, by the whole CTA.
+__device__ __forceinline__ void es_scan(uint32_t* a, int n, uint32_t* warp_total) {
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  uint32_t own = t < n ? a[t] : 0, sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 31) warp_total[w] = sum;
+  __syncthreads();
+  if (w == 0) {
+    uint32_t x = warp_total[lane], s = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    warp_total[lane] = s - x;
+  }
+  __syncthreads();
+  if (t < n) a[t] = warp_total[w] + sum - own;
+  __syncthreads();
+}
+
+// ids [T] -> pairs (token, place), ascending by token, then place; ids without a gradient have token V and come last. `a` and `b` hold T
+// pairs each; the last of `passes` passes over `bits` bits writes `a`.
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
+embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint2* __restrict__ b, int T, int V, long long pad, int bits,
+                  int passes) {
+  pdl_launch_dependents();
+  extern __shared__ uint32_t sm[];
+  uint32_t* count = sm;                                     // [warps][bins]: pairs of the warp with a digit, then the places before them
+  uint32_t* total = sm + kSortWarps * kSortBins;            // [bins]: pairs of this CTA with a digit
+  uint32_t* start = total + kSortBins;                      // [bins]: where this CTA's pairs with a digit begin
+  uint32_t* warp_total = start + kSortBins;
+  const uint32_t rank = cluster_ctarank();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, bins = 1 << bits;
+  const long long per_warp = ((T + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32ll;
+  const long long lo = min((long long)T, (rank * kSortWarps + w) * per_warp), hi = min((long long)T, lo + per_warp);
+  uint32_t* mine = count + w * bins;
+
+  for (int pass = 0; pass < passes; ++pass) {
+    const uint2* src = (passes - pass) & 1 ? b : a;         // what this pass reads (the first one reads ids)
+    uint2* dst = (passes - pass) & 1 ? a : b;
+    const int shift = pass * bits;
+    auto pair = [&](long long i) -> uint2 {
+      if (pass == 0) {
+        const long long id = ids[i];
+        return make_uint2(id >= 0 && id < V && id != pad ? uint32_t(id) : uint32_t(V), uint32_t(i));
+      }
+      return __ldcg(src + i);                               // written by other SMs in the pass before
+    };
+    for (int i = threadIdx.x; i < kSortWarps * bins; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+    for (long long i0 = lo; i0 < hi; i0 += 32) {
+      const bool has = i0 + lane < hi;
+      const uint32_t d = has ? (pair(i0 + lane).x >> shift) & (bins - 1) : 0xffffffffu;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (has && lane == __ffs(same) - 1) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kSortThreads) {
+      uint32_t sum = 0;
+      for (int x = 0; x < kSortWarps; ++x) {
+        const uint32_t c = count[x * bins + d];
+        count[x * bins + d] = sum;
+        sum += c;
+      }
+      total[d] = sum;
+    }
+    cluster_sync_all();
+    uint32_t before = 0;
+    if (threadIdx.x < bins) {
+      uint32_t all = 0;
+      for (uint32_t r = 0; r < kSortCtas; ++r) {
+        const uint32_t c = es_remote(total + threadIdx.x, r);
+        if (r < rank) before += c;
+        all += c;
+      }
+      start[threadIdx.x] = all;
+    }
+    __syncthreads();
+    es_scan(start, bins, warp_total);
+    if (threadIdx.x < bins) start[threadIdx.x] += before;
+    __syncthreads();
+    for (long long i0 = lo; i0 < hi; i0 += 32) {
+      const bool has = i0 + lane < hi;
+      const uint2 p = has ? pair(i0 + lane) : make_uint2(0, 0);
+      const uint32_t d = has ? (p.x >> shift) & (bins - 1) : 0xffffffffu;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (has) dst[start[d] + mine[d] + __popc(same & ((1u << lane) - 1))] = p;
+      __syncwarp();
+      if (has && lane == __ffs(same) - 1) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    cluster_sync_all();                                     // the pass is written, and nobody reads this CTA's totals any more
+  }
+}
+
+// n 16-byte zeros, then the last `rest` bytes. Stands beside the sort: it waits for it only at its end, so that what follows finds both done.
+__global__ void __launch_bounds__(256) embed_fill_kernel(uint4* __restrict__ out, long long n, int rest) {
+  const long long step = (long long)gridDim.x * 256;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += step) out[i] = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == 0 && threadIdx.x < rest) reinterpret_cast<uint8_t*>(out + n)[threadIdx.x] = 0;
+  pdl_wait();
+}
+
+template <typename TO, int N>
+__device__ __forceinline__ void es_write(TO* __restrict__ p, const float (&acc)[N], float scale) {
+  alignas(16) TO raw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) raw[i] = from_f32<TO>(acc[i] * scale);
+  if constexpr (N * sizeof(TO) >= 16) {
+#pragma unroll
+    for (int i = 0; i < N; i += 16 / sizeof(TO)) *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<uint4*>(raw + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = raw[i];
+  }
+}
+
+// Pairs [L tile, L (tile + 1)) of the sorted ones, N columns a thread. `part` [tiles][2][D]: sums of a token that began before the tile, and of
+// one that begins in it and goes on behind it.
+constexpr int kSumAhead = 8;            // rows under way at a time
+template <typename TI, typename TO, int N>
+__global__ void __launch_bounds__(256)
+embed_sum_kernel(const uint2* __restrict__ pairs, const TI* __restrict__ dy, long long rs, TO* __restrict__ out, float* __restrict__ part, int T,
+                 int V, int D, int L, float scale) {
+  const int tile = blockIdx.x, col = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  const int lo = tile * L, hi = min(T, lo + L);
+  if (col >= D || pairs[lo].x >= uint32_t(V)) return;
+  const uint32_t before = lo > 0 ? pairs[lo - 1].x : 0xffffffffu, behind = hi < T ? pairs[hi].x : 0xffffffffu;
+  uint32_t token = pairs[lo].x;
+  bool inside = token != before;        // the token's pairs begin in this tile
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  auto done = [&](bool goes_on) {
+    if (inside && !goes_on) { es_write<TO, N>(out + (long long)token * D + col, acc, scale); return; }
+    float* p = part + ((long long)tile * 2 + inside) * D + col;
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = acc[i];
+  };
+  for (int i0 = lo; i0 < hi; i0 += kSumAhead) {
+    alignas(16) TI raw[kSumAhead][N];
+    uint32_t tok[kSumAhead];
+#pragma unroll
+    for (int j = 0; j < kSumAhead; ++j) {
+      const uint2 p = i0 + j < hi ? pairs[i0 + j] : make_uint2(V, 0);
+      tok[j] = p.x;
+      const TI* src = dy + (long long)p.y * rs + col;
+      if (p.x < uint32_t(V)) {
+        if constexpr (N * sizeof(TI) == 16) *reinterpret_cast<uint4*>(raw[j]) = __ldg(reinterpret_cast<const uint4*>(src));
+        else
+#pragma unroll
+          for (int i = 0; i < N; ++i) raw[j][i] = src[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kSumAhead; ++j) {
+      if (tok[j] >= uint32_t(V)) break;
+      if (tok[j] != token) {
+        done(false);
+        token = tok[j];
+        inside = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += to_f32<TI>(raw[j][i]);
+    }
+  }
+  done(token == behind);
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(256)
+embed_join_kernel(const uint2* __restrict__ pairs, TO* __restrict__ out, const float* __restrict__ part, int T, int V, int D, int L, float scale) {
+  const int tile = blockIdx.x, tiles = gridDim.x, lo = tile * L, hi = lo + L;
+  if (hi >= T) return;
+  const uint32_t token = pairs[hi].x;
+  if (token >= uint32_t(V) || pairs[hi - 1].x != token || (pairs[lo].x == token && lo > 0 && pairs[lo - 1].x == token)) return;
+  int more = 0;                         // tiles behind this one that begin with the token
+  for (int n = blockDim.x; n == blockDim.x;) {
+    const long long at = tile + 1ll + more + threadIdx.x;
+    n = __syncthreads_count(at < tiles && pairs[at * L].x == token);
+    more += n;
+  }
+  for (int col = blockIdx.y * blockDim.x + threadIdx.x; col < D; col += gridDim.y * blockDim.x) {
+    float acc = part[((long long)tile * 2 + 1) * D + col];
+    const float* p = part + (long long)(tile + 1) * 2 * D + col;
+#pragma unroll 8
+    for (int j = 0; j < more; ++j) acc += p[(long long)j * 2 * D];
+    out[(long long)token * D + col] = from_f32<TO>(acc * scale);
+  }
+}
+
+static int es_tile(long long T) {       // pairs of a CTA: 32, and more from 2^15 tokens on, so that partial sums stay a small part of the work
+  long long L = 32;
+  while (L * 1024 < T) L *= 2;
+  return int(L);
+}
+static int es_bits(int V) {
+  int n = 1;
+  while (n < 31 && (1u << n) <= unsigned(V)) ++n;
+  return n;
+}
+
+}  // namespace b200
+using namespace b200;
+
+B200_API long long b200_embedding_grad_workspace(long long T, int D) {
+  if (T <= 0 || D <= 0) return 16;
+  const long long tiles = ceil_div64(T, es_tile(T));
+  return 2 * ((T * 8 + 15) / 16 * 16) + tiles * 2 * D * 4;
+}
+
+template <typename TI, typename TO, int N>
+static void es_sum(const uint2* a, const void* dy, long long rs, void* out, float* part, int T, int V, int D, int L, float scale, cudaStream_t st) {
+  const int lanes = (D + N - 1) / N, threads = lanes >= 128 ? 128 : (lanes + 31) / 32 * 32;
+  const dim3 grid((T + L - 1) / L, (lanes + threads - 1) / threads);
+  embed_sum_kernel<TI, TO, N><<<grid, threads, 0, st>>>(a, (const TI*)dy, rs, (TO*)out, part, T, V, D, L, scale);
+}
+
+B200_API int b200_embedding_grad(const long long* ids, const void* dy, long long rs, void* out, long long T, int V, int D, float scale,
+                                 long long padding, int dtype, int out_dtype, void* workspace, void* stream) {
+  if (T < 0 || V <= 0 || D <= 0 || V == 0x7fffffff) return B200_ERR_BAD_SHAPE;
+  if (T > 0x3fffffff) return B200_ERR_TOO_LARGE;
+  if ((uintptr_t)out % 16 || (uintptr_t)workspace % 16) return B200_ERR_BAD_ALIGN;
+  if (out_dtype != dtype && out_dtype != B200_DT_FP32) return B200_ERR_UNSUPPORTED;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int es = dtype == B200_DT_FP32 ? 4 : 2, os = out_dtype == B200_DT_FP32 ? 4 : 2;
+  const long long bytes = (long long)V * D * os, n16 = bytes / 16;
+  uint2* a = (uint2*)workspace;
+  uint2* b = (uint2*)((char*)workspace + (T * 8 + 15) / 16 * 16);
+  float* part = (float*)((char*)workspace + 2 * ((T * 8 + 15) / 16 * 16));
+  if (T > 0) {
+    const int all = es_bits(V), passes = (all + kSortBits - 1) / kSortBits, bits = (all + passes - 1) / passes;
+    B200_CHECK(cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem));
+    embed_sort_kernel<<<kSortCtas, kSortThreads, kSortSmem, st>>>(ids, a, b, int(T), V, padding, bits, passes);
+    B200_LAUNCH_CHECK();
+  }
+  {
+    cudaLaunchConfig_t cfg = {};
+    long long grid = (n16 + 255) / 256;
+    if (grid > kNumSMs * 8) grid = kNumSMs * 8;
+    cfg.gridDim = dim3(unsigned(grid < 1 ? 1 : grid)); cfg.blockDim = dim3(256); cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = T > 0 ? 1 : 0;
+    B200_CHECK(cudaLaunchKernelEx(&cfg, embed_fill_kernel, (uint4*)out, n16, int(bytes - n16 * 16)));
+  }
+  if (T == 0) return 0;
+  const int L = es_tile(T);
+  const int V16 = 16 / es;
+  const bool vec = D % V16 == 0 && (rs * es) % 16 == 0 && (uintptr_t)dy % 16 == 0;
+#define ES_SUM(TI, TO) vec ? es_sum<TI, TO, 16 / sizeof(TI)>(a, dy, rs, out, part, int(T), V, D, L, scale, st) : es_sum<TI, TO, 1>(a, dy, rs, out, part, int(T), V, D, L, scale, st)
+  if (dtype == B200_DT_FP32) ES_SUM(float, float);
+  else if (dtype == B200_DT_BF16 && out_dtype == B200_DT_BF16) ES_SUM(__nv_bfloat16, __nv_bfloat16);
+  else if (dtype == B200_DT_BF16) ES_SUM(__nv_bfloat16, float);
+  else if (dtype == B200_DT_FP16 && out_dtype == B200_DT_FP16) ES_SUM(__half, __half);
+  else if (dtype == B200_DT_FP16) ES_SUM(__half, float);
+  else return B200_ERR_UNSUPPORTED;
+  B200_LAUNCH_CHECK();
+  const dim3 grid(unsigned((T + L - 1) / L), unsigned((D + 255) / 256));
+  if (out_dtype == B200_DT_FP32) embed_join_kernel<float><<<grid, 256, 0, st>>>(a, (float*)out, part, int(T), V, D, L, scale);
+  else if (out_dtype == B200_DT_BF16) embed_join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, (__nv_bfloat16*)out, part, int(T), V, D, L, scale);
+  else embed_join_kernel<__half><<<grid, 256, 0, st>>>(a, (__half*)out, part, int(T), V, D, L, scale);
+  B200_LAUNCH_CHECK();
+  return 0;
+}

@@ -809,6 +809,40 @@ int b200_greedy_tokens(const void* x, long long ldx, int B, int V, const int* sl
  * id that 32 bits do not hold is noted as -1. */
 int b200_append_tokens(int* tokens, int rows, int width, int* length, const int* slot, const long long* ids, int n, void* stream);
 
+/* Log probabilities of given tokens (csrc/logprobs.cu). logits [rows, V] with row stride rs (elements, any alignment), tokens int64 [rows] (NULL: none are
+ * given, lp and rank must be NULL). Outputs that are NULL are not computed: lp, ent fp32 [rows], rank int64 [rows], top_ids int64 / top_lp fp32 [rows, top]
+ * (top up to 32), stats fp32 [rows, 4] for the gradient. inv_t = 1 / temperature. A token outside 0 .. V - 1: zeros, alternatives -1. */
+int b200_token_logprobs(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp, float* ent,
+                        long long* rank, long long* top_ids, float* top_lp, void* stats, int dtype, void* stream);
+/* out [rows, V] (row stride os) = gradient of the logits for gradients g of lp and h of ent (fp32 [rows], NULL: zeros). */
+int b200_token_logprobs_grad(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, const void* stats,
+                             const float* g, const float* h, void* out, long long os, int dtype, void* stream);
+/* The same from fp32 logits of columns c0 .. c0 + C, chunk after chunk: run fp32 [rows, 4] is made by the chunk with c0 = 0 and carried on by the others. */
+int b200_logprob_chunk(const float* lg, long long rs, long long rows, int C, int c0, const long long* tokens, float inv_t, void* run, int entropy, void* stream);
+int b200_logprob_finish(const void* run, long long rows, int V, const long long* tokens, float inv_t, float* lp, float* ent, void* stats, void* stream);
+/* scale [2]: a power of two that brings gradients into fp16's range, and its reciprocal. */
+int b200_logprob_scale(const float* g, const float* h, long long rows, float inv_t, int V, float* scale, void* stream);
+/* out (16 bits, row stride os) = gradient of a chunk's logits, times scale[0]; rows of lg and out have room for whole groups of four columns. */
+int b200_logprob_chunk_grad(const float* lg, long long rs, long long rows, int C, int c0, int V, const long long* tokens, float inv_t, const void* stats,
+                            const float* g, const float* h, const float* scale, void* out, long long os, int dtype, void* stream);
+/* y (16 bits) = x * scale[1] (scale NULL: x). */
+int b200_logprob_cast(const float* x, void* y, long long n, const float* scale, int dtype, void* stream);
+
+/* Gradient of an embedding table by sorted tokens (csrc/embedding.cu): out [V, D] (dtype or fp32, 16-byte aligned) = scale * sum of dy[t] over ids[t] = row, in the
+ * order of t, zeros elsewhere. dy [T, D] with row stride rs. Ids outside 0 .. V - 1 and `padding` (-1: none) add nothing. workspace: this many bytes, 16-byte
+ * aligned, of this call alone while it runs. */
+long long b200_embedding_grad_workspace(long long T, int D);
+int b200_embedding_grad(const long long* ids, const void* dy, long long rs, void* out, long long T, int V, int D, float scale, long long padding, int dtype,
+                        int out_dtype, void* workspace, void* stream);
+
+/* Activations in 8 bits (csrc/act8.cu): blocks of 32 neighbours share a power of two. q int8 [rows, 32 nb] (8-byte aligned), e uint8 [rows, nb], nb = ceil(D / 32);
+ * a value is q * 2^(e - 127), q = -128 is NaN. x, add, gu with row strides, y and dgu dense. add (NULL: none) joins x, rounded to dtype. */
+int b200_pack8(const void* x, long long x_rs, const void* add, long long add_rs, void* q, void* e, long long rows, int D, int dtype, void* stream);
+int b200_unpack8(const void* q, const void* e, void* y, long long rows, int D, int dtype, void* stream);
+/* gu [rows, 2F] = [g | u], y = silu(g) u; q [rows, 64 nb], e [rows, 2 nb] (both NULL: not kept): g's blocks, then u's. */
+int b200_swiglu8_fwd(const void* gu, long long rs, void* y, void* q, void* e, long long rows, int F, int dtype, void* stream);
+int b200_swiglu8_bwd(const void* dy, const void* q, const void* e, void* dgu, long long rows, int F, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,7 +4,8 @@
   on a slice of the fused qkv projection, rotate-half (Qwen3) or interleaved (DeepSeekLike) layout.
 * ``swiglu``       — ``silu(gate) * up`` on the fused gate|up projection (HF ``Qwen3MLP``).
 * ``gelu``         — exact erf GELU (``nn.GELU`` in GPTLike).
-* ``embedding``    — token gather (+ learned / sinusoidal positions), scatter-add backward.
+* ``embedding``    — token gather (+ learned / sinusoidal positions); the table's gradient by sorted tokens (``embedding_grad``,
+  ``csrc/embedding.cu``), the same bits in every call.
 * ``dropout``      — Philox mask regenerated in backward from (seed), never stored.
 
 Reference: Fine-Tuning/*.py (HF Qwen3 modules), LLM_Distributed_Trainning/PyTorch/ddp_basics/
@@ -286,9 +287,37 @@ def dropout(x: torch.Tensor, p: float, training: bool = True, seed: Optional[int
 # ------------------------------------------------------------------------------------------------
 # embedding
 # ------------------------------------------------------------------------------------------------
+def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
+                   dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """[rows, D] = ``scale * sum of dout[t] over the t with ids[t] = row``, in the order of t: the gradient of ``embedding``'s table. ``ids`` int64 [...], ``dout``
+    [..., D] (fp32, bf16 or fp16), ``dtype`` its own type or fp32. Sums in 32 bits, rounded once. Tokens outside 0 .. rows - 1 and ``padding_idx`` add nothing."""
+    if ids.dtype != torch.int64 or dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.device != ids.device:
+        raise ValueError("embedding_grad: ids must be int64 [...] and dout [..., D] on the same device")
+    D, T = dout.shape[-1], ids.numel()
+    dtype = dtype or dout.dtype
+    if D < 1 or not 1 <= rows < 2 ** 31 - 1 or T >= 2 ** 30 or dout.dtype not in (torch.float32, torch.bfloat16, torch.float16) or dtype not in (dout.dtype, torch.float32):
+        raise ValueError(f"embedding_grad: {T} tokens of {dout.dtype} [{D}] into {rows} rows of {dtype} are not taken")
+    flat, d2 = ids.reshape(-1).contiguous(), dout.reshape(T, D)
+    if not nv.use_native(dout):
+        keep = (flat >= 0) & (flat < rows) & (flat != (-1 if padding_idx is None else padding_idx))
+        out = torch.zeros(rows, D, dtype=torch.float32, device=dout.device)
+        return out.index_add_(0, flat[keep], d2[keep].float()).mul_(scale).to(dtype)
+    if D > 1 and d2.stride(1) != 1:
+        d2 = d2.contiguous()
+    out = torch.empty(rows, D, dtype=dtype, device=dout.device)
+    size = nv.lib().b200_embedding_grad_workspace
+    size.argtypes, size.restype = [i64, i32], i64
+    work = torch.empty(size(T, D), dtype=torch.uint8, device=dout.device)
+    fn = nv.proto("b200_embedding_grad", [vp, vp, i64, vp, i64, i32, i32, f32, i64, i32, i32, vp, vp])
+    nv.check(nv.call_on(dout.device, fn, flat.data_ptr(), d2.data_ptr(), d2.stride(0) if T > 1 else D, out.data_ptr(), T, rows, D, float(scale),
+                        -1 if padding_idx is None else padding_idx, nv.dtype_code(dout.dtype), nv.dtype_code(dtype), work.data_ptr()), "embedding_grad")
+    nv.count_launch(4 if T else 1)
+    return out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, pos_table, period, scale):
+    def forward(ctx, ids, table, pos_table, period, scale, padding_idx):
         flat = ids.reshape(-1).contiguous()
         out = torch.empty(flat.numel(), table.shape[1], dtype=table.dtype, device=table.device)
         fn = nv.proto("b200_embedding_fwd", [vp, vp, vp, vp, i64, i32, i32, f32, i32, vp])
@@ -300,39 +329,33 @@ class _EmbeddingFn(torch.autograd.Function):
             note_use(table, False)              # its gradient arrives through autograd (possibly after a tied head's)
         ctx.save_for_backward(flat)
         ctx.meta = (table.shape, table.dtype, pos_table is not None, period, scale,
-                    None if pos_table is None else pos_table.shape)
+                    None if pos_table is None else pos_table.shape, padding_idx)
         return out.view(*ids.shape, table.shape[1])
 
     @staticmethod
     def backward(ctx, dout):
         (flat,) = ctx.saved_tensors
-        tshape, tdtype, has_pos, period, scale, pshape = ctx.meta
-        dout2 = dout.reshape(-1, tshape[1]).contiguous()
-        dtable = None
-        if ctx.needs_input_grad[1]:
-            acc = torch.zeros(tshape, dtype=torch.float32, device=dout.device)
-            fn = nv.proto("b200_embedding_bwd", [vp, vp, vp, i64, i32, f32, i32, vp])
-            nv.check(fn(nv.ptr(flat), nv.ptr(dout2), nv.ptr(acc), flat.numel(), tshape[1], scale,
-                        nv.dtype_code(dout2.dtype), nv.stream()), "embedding_bwd")
-            nv.count_launch()
-            dtable = acc.to(tdtype)
+        tshape, tdtype, has_pos, period, scale, pshape, padding_idx = ctx.meta
+        dout2 = dout.reshape(-1, tshape[1])
+        dtable = embedding_grad(flat, dout2, tshape[0], scale, padding_idx) if ctx.needs_input_grad[1] else None
         dpos = None
         if has_pos and ctx.needs_input_grad[2]:
             g = dout2.float().view(-1, period, tshape[1]).sum(0)
             dpos = torch.zeros(pshape, dtype=torch.float32, device=dout.device)
             dpos[:period] = g
             dpos = dpos.to(tdtype)
-        return None, dtable, dpos, None, None
+        return None, dtable, dpos, None, None, None
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, pos_table: Optional[torch.Tensor] = None,
-              scale: float = 1.0) -> torch.Tensor:
-    """``table[ids] * scale (+ pos_table[position])``; ids [..., L], position = index along the last dim."""
+              scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``table[ids] * scale (+ pos_table[position])``; ids [..., L], position = index along the last dim. ``padding_idx``: a token
+    whose row gets no gradient."""
     period = ids.shape[-1]
     vec = 4 if table.dtype == torch.float32 else 8
     if nv.use_native(table) and table.shape[1] % vec == 0:
-        return _EmbeddingFn.apply(ids, table, pos_table, period, float(scale))
-    out = F.embedding(ids, table) * scale if scale != 1.0 else F.embedding(ids, table)
+        return _EmbeddingFn.apply(ids, table, pos_table, period, float(scale), padding_idx)
+    out = F.embedding(ids, table, padding_idx) * scale if scale != 1.0 else F.embedding(ids, table, padding_idx)
     if pos_table is not None:
         out = out + pos_table[:period]
     return out

@@ -1,0 +1,311 @@
+"""Log probabilities of given tokens (``csrc/logprobs.cu``): what scoring, an API's ``logprobs`` and training on answers need of a model's logits.
+
+``token_logprobs(logits, tokens)``            from logits: log probabilities, and where asked entropies, ranks and the most probable alternatives.
+``linear_token_logprobs(x, w, tokens)``       from hidden states and the output projection, without a [tokens, vocab] tensor.
+
+With y = logits / temperature and p = softmax(y): ``logprob = log p[token]``, ``entropy = -sum p log p``, ``rank = 1 +`` the number of larger logits.
+Log probabilities and entropies have gradients, formed where autograd delivers the weights of the rows (a policy gradient, a preference loss, a
+distillation): a mean cross entropy whose gradient is known in the forward is ``ops.loss``. A row whose token is not one of the vocabulary (-100,
+say) is passed over: zeros, rank 0, alternatives -1, no gradient.
+
+Reference: perplexities and answers scored in Quantization/LLM-Compressor/AWQ/eval_qwen3_4b_awq.py through vLLM, whose server gives ``logprobs``.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as nv
+from .gemm import gemm, gemv16
+
+vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+MAX_TOP = 32             # alternatives of a row
+_ROWS_ARGS = [vp, i64, i64, i32, vp, f32, i32, vp, vp, vp, vp, vp, vp, i32, vp]
+_GRAD_ARGS = [vp, i64, i64, i32, vp, f32, vp, vp, vp, vp, i64, i32, vp]
+
+
+class TokenLogprobs(NamedTuple):
+    """What was not asked for is None. Shapes are the tokens' (``top_ids`` and ``top_logprobs`` have one dimension more)."""
+    logprob: Optional[torch.Tensor]           # fp32
+    entropy: Optional[torch.Tensor] = None    # fp32
+    rank: Optional[torch.Tensor] = None       # int64: 1 = no logit is larger
+    top_ids: Optional[torch.Tensor] = None    # int64, the most probable first, the lowest id first among equals
+    top_logprobs: Optional[torch.Tensor] = None
+
+
+def _check(what, tokens, shape, device, temperature):
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.shape != shape or tokens.device != device):
+        raise ValueError(f"{what}: tokens must be int64 {list(shape)} on {device}")
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+        raise ValueError(f"{what}: temperature must be from 2^-60 to 2^60, not {temperature}")
+
+
+def _as_rows(x: torch.Tensor) -> torch.Tensor:
+    """[rows, last] with contiguous rows; a view where there is one."""
+    x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def _rows(logits, tokens, temperature, top, entropy, rank, save):
+    """(lp, H, rank, ids, lps, stats) of logits [B, V]; ``stats`` fp32 [B, 4] is what the gradient needs."""
+    B, V = logits.shape
+    if not nv.use_native(logits):
+        return _rows_torch(logits, tokens, temperature, top, entropy, rank)
+    def new(*size, dtype=torch.float32):
+        return logits.new_empty(size, dtype=dtype)
+    lp, H, r = new(B) if tokens is not None else None, new(B) if entropy else None, new(B, dtype=torch.int64) if rank else None
+    ids, lps = (new(B, top, dtype=torch.int64), new(B, top)) if top else (None, None)
+    stats = new(B, 4) if save else None
+    if B:
+        fn = nv.proto("b200_token_logprobs", _ROWS_ARGS)
+        nv.check(nv.call_on(logits.device, fn, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, nv.ptr(tokens), 1.0 / temperature, top, nv.ptr(lp),
+                            nv.ptr(H), nv.ptr(r), nv.ptr(ids), nv.ptr(lps), nv.ptr(stats), nv.dtype_code(logits.dtype)), "token_logprobs")
+        nv.count_launch()
+    return lp, H, r, ids, lps, stats
+
+
+def _rows_torch(logits, tokens, temperature, top, entropy, rank):
+    B, V = logits.shape
+    ok = torch.ones(B, dtype=torch.bool, device=logits.device) if tokens is None else (tokens >= 0) & (tokens < V)
+    m = logits.float().amax(1, keepdim=True)
+    d = (logits.float() - m) / temperature
+    e = torch.exp(d)
+    s = e.sum(1, keepdim=True)
+    ls = torch.log(s)
+    zero = torch.zeros(B, device=logits.device)
+    lp = H = r = ids = lps = None
+    if tokens is not None:
+        at = tokens.clamp(0, V - 1)[:, None]
+        lp = torch.where(ok, (d.gather(1, at) - ls)[:, 0], zero)
+    if entropy:
+        H = torch.where(ok, (ls - (e * d.clamp_min(-150.0)).sum(1, keepdim=True) / s)[:, 0], zero)
+    if rank:
+        r = torch.where(ok, 1 + (logits > logits.gather(1, at)).sum(1), 0)
+    if top:
+        ids = _order(logits)[:, :top]
+        lps = torch.where(ok[:, None], d.gather(1, ids) - ls, zero[:, None])
+        ids = torch.where(ok[:, None], ids, -1)
+    stats = torch.cat([m, 1 / s, ls, torch.zeros_like(ls) if H is None else H[:, None]], 1)
+    return lp, H, r, ids, lps, stats
+
+
+def _order(logits):
+    """Ids by logit, the largest first, the lowest id first among equals; NaN above all."""
+    x = logits.float()
+    return torch.sort(torch.where(x.isnan(), torch.full_like(x, float("nan")), x), dim=1, descending=True, stable=True)[1]
+
+
+def _rows_grad(logits, tokens, temperature, stats, g, h):
+    B, V = logits.shape
+    if not nv.use_native(logits):
+        return _grad_torch(logits.float(), tokens, temperature, stats, g, h, 0, V).to(logits.dtype)
+    out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
+    if B:
+        fn = nv.proto("b200_token_logprobs_grad", _GRAD_ARGS)
+        nv.check(nv.call_on(logits.device, fn, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, nv.ptr(tokens), 1.0 / temperature, nv.ptr(stats),
+                            nv.ptr(g), nv.ptr(h), nv.ptr(out), V, nv.dtype_code(logits.dtype)), "token_logprobs_grad")
+        nv.count_launch()
+    return out
+
+
+def _grad_torch(l, tokens, temperature, stats, g, h, c0, vocab):
+    """fp32 gradient of columns c0 .. of the logits, whose fp32 values are l."""
+    m, inv_s, ls, H = stats.unsqueeze(2).unbind(1)
+    zero = torch.zeros_like(m)
+    g, h = (zero if x is None else x.reshape(-1, 1).float() for x in (g, h))
+    d = ((l - m) / temperature)
+    p = torch.exp(d) * inv_s                         # zero below -150, where d would be no factor beside it
+    out = -p * (g + h * (d.clamp_min(-150.0) - ls + H))
+    if tokens is not None:
+        t = tokens[:, None] - c0
+        here = (t >= 0) & (t < l.shape[1])
+        out = out + torch.zeros_like(out).scatter_(1, t.clamp(0, l.shape[1] - 1), torch.where(here, g, zero))
+        out = torch.where((tokens >= 0)[:, None] & (tokens < vocab)[:, None], out, torch.zeros_like(out))
+    return out / temperature
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, top, entropy, rank):
+        lp, H, r, ids, lps, stats = _rows(logits, tokens, temperature, top, entropy, rank, True)
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(t for t in (r, ids, lps) if t is not None))
+        return lp, H, r, ids, lps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, h, *_):
+        if g is None and h is None:
+            return (None,) * 6
+        logits, tokens, stats = ctx.saved_tensors
+        g, h = (None if x is None else x.to(torch.float32).contiguous() for x in (g, h))
+        return (_rows_grad(logits, tokens, ctx.temperature, stats, g, h),) + (None,) * 5
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top: int = 0, entropy: bool = False, rank: bool = False,
+                   temperature: float = 1.0) -> TokenLogprobs:
+    """``logits`` [..., vocab] (fp32, bf16 or fp16; rows may be strided), ``tokens`` int64 [...] (None: no tokens are given, for entropies and
+    alternatives alone). ``top``: how many alternatives, up to ``MAX_TOP``. Sums in 32 bits. A row of minus infinities alone, or with a NaN or plus infinity,
+    gives NaN, as log_softmax does. Ranks and alternatives are those of the logits as they are given."""
+    if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("token_logprobs: logits must be [..., vocab] in fp32, bf16 or fp16")
+    _check("token_logprobs", tokens, logits.shape[:-1], logits.device, temperature)
+    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top must be from 0 to {min(MAX_TOP, logits.shape[-1])}, not {top}")
+    if tokens is None and (rank or not (entropy or top)):
+        raise ValueError("token_logprobs: without tokens there are entropies and alternatives only")
+    shape, rows = logits.shape[:-1], _as_rows(logits)
+    flat = None if tokens is None else tokens.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        got = _TokenLogprobsFn.apply(rows, flat, temperature, top, entropy, rank)
+    else:
+        got = _rows(rows, flat, temperature, top, entropy, rank, False)[:5]
+    if len(shape) == 1:
+        return TokenLogprobs(*got)
+    lp, H, r, ids, lps = got
+    one, many = (lambda t: None if t is None else t.view(shape)), (lambda t: None if t is None else t.view(*shape, top))
+    return TokenLogprobs(one(lp), one(H), one(r), many(ids), many(lps))
+
+
+# ------------------------------------------------------------------------------------------------
+# from hidden states
+# ------------------------------------------------------------------------------------------------
+_CHUNK_BYTES = 64 << 20          # fp32 logits that exist at a time: they stay in the 126 MB L2 between the product and what reads them
+
+
+def _chunks(T: int, V: int):
+    """Columns of the vocabulary that are taken at a time."""
+    C = max(_CHUNK_BYTES // (4 * max(T, 1)), 2048) // 256 * 256
+    n = -(-V // min(C, V))
+    C = min((-(-V // n) + 255) // 256 * 256, V)                       # chunks of about the same size
+    return [(a, min(V, a + C)) for a in range(0, V, C)], C
+
+
+def _chunk_logits(x, w, buf, c0, c1):
+    """fp32 logits of columns c0 .. c1, as rows of ``buf``."""
+    y = gemv16(x, w[c0:c1], out_dtype=torch.float32) if x.shape[0] <= 16 else None
+    return y if y is not None else gemm(x, w[c0:c1], out=buf[:, :c1 - c0])
+
+
+def _linear_forward(x, w, tokens, temperature, entropy, save):
+    T, V = x.shape[0], w.shape[0]
+    lp = x.new_empty(T, dtype=torch.float32) if tokens is not None else None
+    H = x.new_empty(T, dtype=torch.float32) if entropy else None
+    stats = x.new_empty(T, 4, dtype=torch.float32) if save else None
+    if T == 0:
+        return lp, H, stats
+    inv_t = 1.0 / temperature
+    if not nv.use_native(x):
+        lp, H, _, _, _, stats = _rows_torch(x.float() @ w.float().t(), tokens, temperature, 0, entropy, False)
+        return lp, H, stats
+    chunks, C = _chunks(T, V)
+    buf = torch.empty(T, (C + 7) // 8 * 8, dtype=torch.float32, device=x.device)
+    run = torch.empty(T, 4, dtype=torch.float32, device=x.device)
+    fn = nv.proto("b200_logprob_chunk", [vp, i64, i64, i32, i32, vp, f32, vp, i32, vp])
+    for c0, c1 in chunks:
+        y = _chunk_logits(x, w, buf, c0, c1)
+        nv.check(fn(nv.ptr(y), y.stride(0), T, c1 - c0, c0, nv.ptr(tokens), inv_t, nv.ptr(run), int(entropy), nv.stream()), "logprob_chunk")
+    fin = nv.proto("b200_logprob_finish", [vp, i64, i32, vp, f32, vp, vp, vp, vp])
+    nv.check(fin(nv.ptr(run), T, V, nv.ptr(tokens), inv_t, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), nv.stream()), "logprob_finish")
+    nv.count_launch(len(chunks) + 1)
+    return lp, H, stats
+
+
+def _linear_backward(x, w, tokens, temperature, stats, g, h, need_dx, need_dw):
+    T, K = x.shape
+    V = w.shape[0]
+    if not nv.use_native(x):
+        d = _grad_torch(x.float() @ w.float().t(), tokens, temperature, stats, g, h, 0, V)
+        return (d @ w.float()).to(x.dtype) if need_dx else None, (d.t() @ x.float()).to(w.dtype) if need_dw else None
+    dev, dt, inv_t = x.device, nv.dtype_code(x.dtype), 1.0 / temperature
+    dw = torch.empty(V, K, dtype=w.dtype, device=dev) if need_dw else None
+    if T == 0:
+        return (torch.empty_like(x) if need_dx else None), (None if dw is None else dw.zero_())
+    chunks, C = _chunks(T, V)
+    ld = (C + 7) // 8 * 8
+    buf = torch.empty(T, ld, dtype=torch.float32, device=dev)
+    dl = torch.empty(T, ld, dtype=x.dtype, device=dev)
+    acc = torch.empty(T, K, dtype=torch.float32, device=dev) if need_dx else None
+    half = x.dtype == torch.float16
+    scale = part = None
+    if half:             # gradients of single logits lie below fp16's numbers: they are brought up by a power of two, the results back down
+        scale = torch.empty(2, dtype=torch.float32, device=dev)
+        fs = nv.proto("b200_logprob_scale", [vp, vp, i64, f32, i32, vp, vp])
+        nv.check(fs(nv.ptr(g), nv.ptr(h), T, inv_t, V, nv.ptr(scale), nv.stream()), "logprob_scale")
+        part = torch.empty(C, K, dtype=torch.float32, device=dev) if need_dw else None
+    fg = nv.proto("b200_logprob_chunk_grad", [vp, i64, i64, i32, i32, i32, vp, f32, vp, vp, vp, vp, vp, i64, i32, vp])
+    fc = nv.proto("b200_logprob_cast", [vp, vp, i64, vp, i32, vp])
+    for c0, c1 in chunks:
+        n = c1 - c0
+        gemm(x, w[c0:c1], out=buf[:, :n])
+        nv.check(fg(nv.ptr(buf), ld, T, n, c0, V, nv.ptr(tokens), inv_t, nv.ptr(stats), nv.ptr(g), nv.ptr(h), nv.ptr(scale), nv.ptr(dl), ld, dt, nv.stream()),
+                 "logprob_chunk_grad")
+        if need_dx:
+            gemm(dl[:, :n], w[c0:c1], b_mn=True, out=acc, beta=1.0 if c0 else 0.0)
+        if need_dw and not half:
+            gemm(dl[:, :n], x, a_mn=True, b_mn=True, out=dw[c0:c1])
+        elif need_dw:
+            gemm(dl[:, :n], x, a_mn=True, b_mn=True, out=part[:n])
+            nv.check(fc(nv.ptr(part), nv.ptr(dw[c0:c1]), n * K, nv.ptr(scale), dt, nv.stream()), "logprob_cast")
+    dx = None
+    if need_dx:
+        dx = torch.empty_like(x)
+        nv.check(fc(nv.ptr(acc), nv.ptr(dx), T * K, nv.ptr(scale), dt, nv.stream()), "logprob_cast")
+    nv.count_launch(len(chunks) * (2 if half and need_dw else 1) + bool(need_dx) + half)
+    return dx, dw
+
+
+class _LinearLogprobsFn(torch.autograd.Function):
+    """Saves nothing of the size of the logits: the backward pass computes them again, a chunk at a time."""
+
+    @staticmethod
+    def forward(ctx, x, w, tokens, temperature, entropy):
+        with torch.cuda.device_of(x):
+            lp, H, stats = _linear_forward(x, w, tokens, temperature, entropy, True)
+        if w.requires_grad:
+            from ..utils.arena import note_use
+            note_use(w, False)                   # its gradient arrives through autograd
+        ctx.save_for_backward(x, w, tokens, stats)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        return lp, H
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, h):
+        if g is None and h is None:
+            return (None,) * 5
+        x, w, tokens, stats = ctx.saved_tensors
+        g, h = (None if t is None else t.to(torch.float32).contiguous() for t in (g, h))
+        with torch.cuda.device_of(x):
+            dx, dw = _linear_backward(x, w, tokens, ctx.temperature, stats, g, h, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor], *, entropy: bool = False, temperature: float = 1.0) -> TokenLogprobs:
+    """``token_logprobs(x @ w.T, tokens)`` for hidden states ``x`` [..., K] and an output projection ``w`` [vocab, K] (bf16 or fp16, K a multiple of 8),
+    with fp32 logits that exist a chunk of the vocabulary at a time, in the forward and again in the backward pass. Gradients for ``x`` and ``w``."""
+    if w.dim() != 2 or w.shape[0] < 1 or x.dim() < 1 or x.shape[-1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
+        raise ValueError("linear_token_logprobs: x [..., K] and w [vocab, K] must agree in K, type and device")
+    if x.dtype not in ((torch.bfloat16, torch.float16) if nv.use_native(x) else (torch.bfloat16, torch.float16, torch.float32)):
+        raise TypeError(f"linear_token_logprobs: x and w must be bf16 or fp16, not {x.dtype}; token_logprobs takes logits of 32 bits")
+    if nv.use_native(x) and (x.shape[-1] % 8 or w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16):
+        raise ValueError("linear_token_logprobs: rows of w must be contiguous, start at multiples of 16 bytes and have a multiple of 8 values")
+    _check("linear_token_logprobs", tokens, x.shape[:-1], x.device, temperature)
+    if tokens is None and not entropy:
+        raise ValueError("linear_token_logprobs: without tokens there are entropies only")
+    shape, rows = x.shape[:-1], _as_rows(x)
+    if nv.use_native(rows) and (rows.data_ptr() % 16 or rows.stride(0) % 8):
+        rows = rows.contiguous() if rows.stride(0) % 8 else rows.clone()
+    flat = None if tokens is None else tokens.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        lp, H = _LinearLogprobsFn.apply(rows, w, flat, temperature, entropy)
+    else:
+        with torch.cuda.device_of(rows):
+            lp, H, _ = _linear_forward(rows, w, flat, temperature, entropy, False)
+    return TokenLogprobs(None if lp is None else lp.view(shape), None if H is None else H.view(shape))
