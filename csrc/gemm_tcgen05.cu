@@ -23,6 +23,7 @@
 // Replaces: cuBLAS/cuBLASLt behind every nn.Linear in the reference, e.g.
 // LLM_Distributed_Trainning/PyTorch/ddp_basics/ddp_gpt_wikitext2.py:86-165.
 #include "common.cuh"
+#include "logprob_math.cuh"
 #include "tma_host.h"
 #include "../include/b200_ops.h"
 
@@ -100,6 +101,23 @@ struct W4Params {
   int raw_stages, is_bf16;
   int lut_bytes;
   int debug;  // B200_W4_DEBUG bit mask; only read when the library is built with -DB200_W4_EXPERIMENT (timing experiments)
+};
+
+// Epilogues of an output projection whose result, fp32 logits, is not stored (ops/logprobs.py). A row of the accumulator is one thread's, so what
+// it needs of a row stays in that thread.
+//   kHeadSums   the 256 logits of a row and tile become (m, s, u) of logprob_math.cuh in part[tile column][row]; the given token's logit goes to lt[row]
+//   kHeadGrads  a logit becomes its gradient, which is stored in 16 bits as D
+enum { kHeadNone = 0, kHeadSums = 1, kHeadGrads = 2 };
+struct HeadParams {
+  const long long* tokens;   // [M] or null
+  int V, c0;                 // the vocabulary; the first column of this product in it
+  float inv_t;
+  int entropy;
+  float4* part;              // [num_n][M]
+  float* lt;                 // [M]
+  const float4* stats;       // [M] (m, 1 / s, log s, H)
+  const float *g, *h;        // [M] or null
+  const float* scale;        // scale[0] times the gradient, or null
 };
 
 constexpr int kW4Threads = 480;      // + 8 dequant warps + 1 packed-tile TMA warp
@@ -291,6 +309,14 @@ __device__ __forceinline__ void epilogue_store(const GemmKernelParams& p, OutT* 
   }
 }
 
+template <bool ENT>
+__device__ __forceinline__ void head_sums(LpSum& a, const uint32_t (&r)[32], int inside, float c) {
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = j < inside ? __uint_as_float(r[j]) : -INFINITY;    // columns behind the last: no weight
+  lp_join<ENT>(a, v, c);
+}
+
 // ---- K-C5: the all-reduce half of the fused row-parallel GEMM (called by the four epilogue warps, 128 threads) ----
 // A reduction item is a slab of kArSlabRows rows of a tile this rank owns (tile % world == rank); item i of the rank goes
 // to CTA i % gridDim.x. An item can be summed once every rank has announced the tile (both CTAs of a pair). With
@@ -401,9 +427,9 @@ __device__ __noinline__ int ar_reduce(const GemmKernelParams& p, int next, int n
   return next;
 }
 
-template <int ES, int CTAS, bool W4>
+template <int ES, int CTAS, bool W4, int HEAD = kHeadNone>
 __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmA2,
-                                          const CUtensorMap& tmB2, const GemmKernelParams& p, const W4Params* w4) {
+                                          const CUtensorMap& tmB2, const GemmKernelParams& p, const W4Params* w4, const HeadParams* head = nullptr) {
   constexpr int EPR = 128 / ES;  // elements per 128-byte swizzle row = k-block depth
   constexpr int UK = 32 / ES;    // elements per UMMA k-step
 
@@ -814,7 +840,46 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const int col_limit = min(p.N, n0 + p.bn);
       const int nchunks = (p.bn + 31) / 32;
       const float beta = (p.beta_rows != nullptr && row_ok) ? p.beta_rows[row] : p.beta;
-      if (sg.kb0 > 0) {
+      if constexpr (HEAD != kHeadNone) {
+        // ---- whole tiles of logits: sums or gradients of this thread's row ----
+        const float c2 = head->inv_t * kLog2e;
+        const long long t = row_ok && head->tokens ? head->tokens[row] : -1;
+        const bool skip = !row_ok || (head->tokens && (t < 0 || t >= head->V));
+        const long long at = t - head->c0;                       // the token's column, if it is in this product
+        LpSum sum{-INFINITY, 0.f, 0.f};
+        LpGrad grad{};
+        if (HEAD == kHeadGrads && !skip)
+          grad = lp_grad_of(head->stats[row], head->g ? head->g[row] : 0.f, head->h ? head->h[row] : 0.f, head->inv_t, at, head->scale ? head->scale[0] : 1.f);
+        for (int c = 0; c < nchunks; ++c) {
+          const int col0 = n0 + c * 32;
+          if (col0 >= col_limit) break;
+          __syncwarp();                                // lanes went ways of their own in the group before
+          uint32_t r[32];
+          tmem_ld_32x32(t0 + c * 32, r);
+          tmem_ld_wait();
+          if constexpr (HEAD == kHeadSums) {
+            if (at >= col0 && at < col0 + 32) {
+              float lt = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) lt = at == col0 + j ? __uint_as_float(r[j]) : lt;
+              head->lt[row] = lt;
+            }
+            if (head->entropy) head_sums<true>(sum, r, col_limit - col0, c2);
+            else head_sums<false>(sum, r, col_limit - col0, c2);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float d = lp_grad_at(__uint_as_float(r[j]), grad, c2) + (col0 + j == grad.t ? grad.g : 0.f);
+              r[j] = skip ? 0u : __float_as_uint(d);
+            }
+            if (p.out_dtype == B200_DT_BF16)
+              epilogue_store<__nv_bfloat16>(p, reinterpret_cast<__nv_bfloat16*>(p.D) + doff, col0, col_limit, r, row_ok, 0.f, 0);
+            else
+              epilogue_store<__half>(p, reinterpret_cast<__half*>(p.D) + doff, col0, col_limit, r, row_ok, 0.f, 0);
+          }
+        }
+        if (HEAD == kHeadSums && row_ok) head->part[(long long)n_blk * p.M + row] = make_float4(sum.m, sum.s, sum.u, 0.f);
+      } else if (sg.kb0 > 0) {
         // ---- stream-K contributor: publish this CTA's fp32 partial, the tile's owner finishes it ----
         // laid out [16-byte piece][row], so that a warp's store or load is whole lines (a row to a lane is 32 lines an instruction:
         // 2048 x 5120 x 34816 625 us, now 596; 490 x 4096 x 12288 76, now 68)
@@ -941,6 +1006,13 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
                     const __grid_constant__ GemmKernelParams p) {
   gemm_body<ES, CTAS, false>(tmA, tmB, tmA2, tmB2, p, nullptr);
+}
+
+template <int CTAS, int HEAD>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_head_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ HeadParams head,
+                 const __grid_constant__ GemmKernelParams p) {
+  gemm_body<2, CTAS, false, HEAD>(tmA, tmB, tmA, tmB, p, nullptr, &head);
 }
 
 // Same pipeline with the B operand expanded from 4-bit codes inside the kernel (NF4 / GPTQ / AWQ weights, optionally
@@ -1295,6 +1367,90 @@ B200_API int b200_gemm_2d(const void* A, const void* B, void* D, const void* bia
   a.a_mn = a_mn; a.b_mn = b_mn; a.in_dtype = in_dtype; a.out_dtype = out_dtype; a.bias_dtype = bias_dtype;
   a.alpha = alpha; a.beta = beta; a.workspace = workspace; a.workspace_bytes = workspace_bytes;
   return b200_gemm(&a, stream);
+}
+
+// ---- logits of an output projection, x [M, K] times w [N, K]^T, that are not stored ----
+template <int CTAS, int HEAD>
+static int launch_head(const CUtensorMap& tmA, const CUtensorMap& tmB, const HeadParams& h, const GemmKernelParams& p, int grid, int smem, cudaStream_t stream) {
+  B200_CHECK(cudaFuncSetAttribute(gemm_head_kernel<CTAS, HEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, g_max_smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kGemmThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  B200_CHECK(cudaLaunchKernelEx(&cfg, gemm_head_kernel<CTAS, HEAD>, tmA, tmB, h, p));
+  return 0;
+}
+
+static GemmConfig head_config(int M, int N, int K) { return pick_config(M, N, 1, ceil_div(K, 64), 0, 64, g_num_sms, false); }
+
+static int gemm_head(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, void* out, long long out_rs, HeadParams h, int mode,
+                     cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0) return B200_ERR_BAD_SHAPE;
+  if (dtype != B200_DT_BF16 && dtype != B200_DT_FP16) return B200_ERR_UNSUPPORTED;
+  if (((uintptr_t)x | (uintptr_t)w) & 15 || x_rs % 8 || w_rs % 8) return B200_ERR_BAD_ALIGN;
+  int rc = device_props();
+  if (rc) return rc;
+  const GemmConfig cfg = head_config(M, N, K);
+  const int ctas = cfg.ctas, bn_cta = cfg.bn / ctas;
+  GemmKernelParams p = {};
+  p.D = out; p.M = M; p.N = N; p.K = K; p.batch = p.nb0 = p.b_div = p.nb0_b = 1;
+  p.d_rs = out_rs; p.alpha = 1.f; p.out_dtype = dtype;
+  p.num_k = ceil_div(K, 64); p.bn = cfg.bn; p.sk_group = 1;
+  p.num_m = ceil_div(M, kBM * ctas); p.num_n = ceil_div(N, p.bn);
+  const int stage_bytes = kStageABytes + bn_cta * 128;
+  p.stages = (g_max_smem - 2048) / stage_bytes;
+  if (p.stages > 6) p.stages = 6;
+  if (p.stages < 2) return B200_ERR_UNSUPPORTED;
+  const uint32_t fmt = dtype == B200_DT_BF16 ? 1u : 0u;
+  p.idesc_main = p.idesc_lora = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM * ctas >> 4) << 24);
+  p.vec_ok = out && ((uintptr_t)out & 15) == 0 && out_rs % 8 == 0;
+  CUtensorMap tmA, tmB;
+  {
+    uint64_t dims[4] = {(uint64_t)K, (uint64_t)M, 1, 1}, str[3] = {(uint64_t)x_rs * 2, 0, 0};
+    uint32_t box[4] = {64, kBM, 1, 1};
+    rc = make_tensor_map(&tmA, x, 2, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  {
+    uint64_t dims[4] = {(uint64_t)K, (uint64_t)N, 1, 1}, str[3] = {(uint64_t)w_rs * 2, 0, 0};
+    uint32_t box[4] = {64, (uint32_t)bn_cta, 1, 1};
+    rc = make_tensor_map(&tmB, w, 2, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  const int units = g_num_sms / ctas;
+  const long long tiles = (long long)p.num_m * p.num_n;
+  if (tiles > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  const int grid = (int)(tiles < units ? tiles : units) * ctas;
+  const int smem = p.stages * stage_bytes + 8 * (2 * p.stages + 6) + 1024;
+  if (mode == kHeadSums) rc = ctas == 2 ? launch_head<2, kHeadSums>(tmA, tmB, h, p, grid, smem, stream) : launch_head<1, kHeadSums>(tmA, tmB, h, p, grid, smem, stream);
+  else rc = ctas == 2 ? launch_head<2, kHeadGrads>(tmA, tmB, h, p, grid, smem, stream) : launch_head<1, kHeadGrads>(tmA, tmB, h, p, grid, smem, stream);
+  if (rc) return rc;
+  B200_LAUNCH_CHECK();
+  return 0;
+}
+
+// Columns of tiles, for which b200_gemm_head_sums writes a partial result each.
+B200_API int b200_gemm_head_tiles(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return -B200_ERR_BAD_SHAPE;
+  const int rc = device_props();
+  if (rc) return -rc;
+  return ceil_div(N, head_config(M, N, K).bn);
+}
+
+B200_API int b200_gemm_head_sums(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, float inv_t,
+                                 int entropy, void* part, float* lt, void* stream) {
+  HeadParams h = {};
+  h.tokens = tokens; h.V = N; h.inv_t = inv_t; h.entropy = entropy; h.part = (float4*)part; h.lt = lt;
+  return gemm_head(x, x_rs, w, w_rs, M, N, K, dtype, nullptr, 0, h, kHeadSums, (cudaStream_t)stream);
+}
+
+B200_API int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, int V, int c0,
+                                  float inv_t, const void* stats, const float* g, const float* h, const float* scale, void* out, long long out_rs, void* stream) {
+  HeadParams hp = {};
+  hp.tokens = tokens; hp.V = V; hp.c0 = c0; hp.inv_t = inv_t; hp.stats = (const float4*)stats; hp.g = g; hp.h = h; hp.scale = scale;
+  return gemm_head(x, x_rs, w, w_rs, M, N, K, dtype, out, out_rs, hp, kHeadGrads, (cudaStream_t)stream);
 }
 
 B200_API int b200_gemm_w4(const b200_gemm_args* a, const b200_w4_desc* w, void* stream_) {

@@ -8,170 +8,114 @@
 // without a token of the vocabulary is passed over: zeros, no alternatives, no gradient. A row of minus infinities alone, or with a NaN or
 // plus infinity, gives NaN as log_softmax does.
 //
-//   lp_rows        logits [B, V] -> lp, H, rank, alternatives, and (m, 1 / s, log s, H) for the backward pass; a CTA a row
+//   lp_rows        logits [B, V] -> lp, H, rank, alternatives, and (m, 1 / s, log s, H) for the backward pass; a CTA or a cluster a row
 //   lp_rows_grad   logits, (m, 1 / s, log s, H), g, h -> dl, in one pass
-// and for logits x w^T that are never there as a whole, a chunk of the vocabulary at a time (products by gemm_tcgen05.cu):
-//   lp_chunk       a chunk's logits (fp32) join m, s, u and l_t of their rows
-//   lp_finish      lp, H and what the backward pass needs
-//   lp_chunk_grad  a chunk's logits, computed again, -> dl in 16 bits, the operand of the products dl w and dl^T x
+// and for logits x w^T that are never stored (gemm_tcgen05.cu: sums and gradients in the epilogues of the product):
+//   lp_finish      lp, H and what the backward pass needs, from the sums of a row's tiles
+//   lp_scale, lp_cast   a power of two for fp16's gradients of single logits, and back
 // Rows of logits are bound by HBM; a 16-bit logit has eight operations beside its exponential.
-#include "common.cuh"
+#include "logprob_math.cuh"
 #include "../include/b200_ops.h"
+#include <type_traits>
 
 namespace b200 {
 
-constexpr int kLpThreads = 512;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpMaxTop = 32, kLpMaxCluster = 8;
 
-struct LpSum { float m, s, u; };
+// What a CTA knows of its slice of a row, where the others of its cluster read it.
+struct LpShared {
+  float red[3][kLpWarps];
+  int redi[kLpWarps];
+  float4 sums;                                   // m, s, u, logits above the token's
+  unsigned long long best[kLpMaxTop];            // the slice's alternatives in order
+  unsigned long long list[1024];
+  uint32_t group[64];
+  int chosen[kLpMaxTop];
+  unsigned long long bound;
+  int n;
+};
 
-__device__ __forceinline__ float lp_exp2(float x) { return exp2f(x); }
-// x where it is a factor beside 2^x: below -200 that is zero, and zero times minus infinity would not be.
-__device__ __forceinline__ float lp_factor(float x) { return fmaxf(x, -200.f); }
+template <typename T> struct LpVec { static constexpr int N = 16 / sizeof(T); };
 
-// What lies in two parts of a row as if it were one. c = log2(e) / T.
-template <bool ENT>
-__device__ __forceinline__ LpSum lp_both(LpSum a, LpSum b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.u + b.u};               // nothing yet (or a NaN in s)
-  const float xa = (a.m - m) * c, xb = (b.m - m) * c, fa = lp_exp2(xa), fb = lp_exp2(xb);
-  LpSum r{m, a.s * fa + b.s * fb, 0.f};
-  if constexpr (ENT) r.u = fa * (a.u + a.s * lp_factor(xa)) + fb * (b.u + b.s * lp_factor(xb));
-  return r;
-}
-
-template <bool ENT>
-__device__ __forceinline__ LpSum lp_block(LpSum a, float c, float* red) {      // red: 96 floats
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = lp_both<ENT>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
-  __syncthreads();
-  if (lane == 0) { red[w] = a.m; red[32 + w] = a.s; red[64 + w] = a.u; }
-  __syncthreads();
-  a = lane < nw ? LpSum{red[lane], red[32 + lane], red[64 + lane]} : LpSum{-INFINITY, 0.f, 0.f};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = lp_both<ENT>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
-  return a;
-}
-
-__device__ __forceinline__ int lp_block_count(int v, int* red) {               // red: 32 ints
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0);
-}
-
-// n values join the sums: the largest first, so that a group rescales at most once.
-template <bool ENT, int N>
-__device__ __forceinline__ void lp_join(LpSum& a, const float (&v)[N], float c) {
-  float m = v[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-  if (m > a.m) {
-    const float x = (a.m - m) * c, f = lp_exp2(x);
-    if constexpr (ENT) a.u = f * (a.u + a.s * lp_factor(x));
-    a.s *= f;
-    a.m = m;
-  }
-  const float base = a.m == -INFINITY ? 0.f : a.m;                    // minus infinities alone: their weights are zeros
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = (v[i] - base) * c, e = lp_exp2(x);
-    a.s += e;
-    if constexpr (ENT) a.u = fmaf(e, lp_factor(x), a.u);
-  }
-}
-
-// f(index of the first, values) for groups of N neighbours of p[0 .. n) and f1 for single ones at its unaligned ends, over the CTA's threads.
-template <typename T, typename F, typename F1>
-__device__ __forceinline__ void lp_walk(const T* __restrict__ p, int n, F f, F1 f1) {
-  constexpr int V = 16 / sizeof(T), G = 4, N = V * G;
-  const int head = min(n, int((16 - ((uintptr_t)p & 15)) & 15) / int(sizeof(T)));
-  if (threadIdx.x < head) f1(threadIdx.x, to_f32<T>(p[threadIdx.x]));
-  const int nvec = (n - head) / V;
-  const uint4* q = reinterpret_cast<const uint4*>(p + head);
-  int i = threadIdx.x;
-  for (; i + (G - 1) * blockDim.x < nvec; i += G * blockDim.x) {
-    uint4 raw[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) raw[g] = __ldg(q + i + g * blockDim.x);
-    float v[N];
+// The values of G vectors, and the largest of them (NaN aside).
+template <typename T, int G>
+__device__ __forceinline__ float lp_values(const uint4 (&raw)[G], float (&v)[G * LpVec<T>::N]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -INFINITY;
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[g * V + j] = to_f32<T>(reinterpret_cast<const T*>(&raw[g])[j]);
-    f(v);
-  }
-  for (; i < nvec; i += blockDim.x) {
-    const uint4 raw = __ldg(q + i);
-    float v[V];
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, v[g * 4 + j] = __uint_as_float((&raw[g].x)[j]));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m = *reinterpret_cast<const T2*>(&raw[0].x);
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = to_f32<T>(reinterpret_cast<const T*>(&raw)[j]);
-    f(v);
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T2 p = *reinterpret_cast<const T2*>(&(&raw[g].x)[j]);
+        m = __hmax2(m, p);
+        v[(g * 4 + j) * 2] = to_f32<T>(p.x);
+        v[(g * 4 + j) * 2 + 1] = to_f32<T>(p.y);
+      }
+    return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
   }
-  for (int j = head + nvec * V + threadIdx.x; j < n; j += blockDim.x) f1(j, to_f32<T>(p[j]));
 }
+
+// How a CTA walks over p[0 .. n): single values up to the first multiple of 16 bytes, vectors i = thread, thread + threads .. in groups of kLpGroup
+// and then one by one, single values behind the last.
+constexpr int kLpGroup = 4;
+struct LpWalk { int head, nvec, tail; };
+template <typename T> __device__ __forceinline__ LpWalk lp_walk(const T* p, int n) {
+  const int head = min(n, int((16 - ((uintptr_t)p & 15)) & 15) / int(sizeof(T))), nvec = (n - head) / LpVec<T>::N;
+  return {head, nvec, head + nvec * LpVec<T>::N};
+}
+// vectors in the group that begins with vector i
+__device__ __forceinline__ int lp_group(int i, int nvec) { return i + (kLpGroup - 1) * kLpThreads < nvec ? kLpGroup : 1; }
 
 // Order of logits as whole numbers: NaN above all, -0 as 0; ties by the lower id.
-__device__ __forceinline__ unsigned long long lp_key(float v, uint32_t id) {
+__device__ __forceinline__ uint32_t lp_order(float v) {
   const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
-  const uint32_t o = v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return (unsigned long long)o << 32 | uint32_t(~id);
+  return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long lp_key(float v, uint32_t id) { return (unsigned long long)lp_order(v) << 32 | uint32_t(~id); }
+__device__ __forceinline__ uint32_t lp_id(unsigned long long key) { return ~uint32_t(key); }
+__device__ __forceinline__ float lp_of_key(unsigned long long key) {
+  const uint32_t o = uint32_t(key >> 32);
+  return o == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
 }
 
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads)
-lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, const long long* __restrict__ tokens, float inv_t, int top, float* __restrict__ lp,
-               float* __restrict__ ent, long long* __restrict__ rank, long long* __restrict__ top_ids, float* __restrict__ top_lp,
-               float4* __restrict__ stats) {
-  __shared__ float red[96];
-  __shared__ int redi[32];
-  __shared__ unsigned long long redk[32];
-  const long long row = blockIdx.x;
-  const long long t = tokens ? tokens[row] : 0;
-  if (t < 0 || t >= V) {
-    if (threadIdx.x == 0) {
-      if (lp) lp[row] = 0.f;
-      if (ENT) ent[row] = 0.f;
-      if (rank) rank[row] = 0;
-      if (stats) stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    for (int i = threadIdx.x; i < top; i += blockDim.x) { top_ids[row * top + i] = -1; top_lp[row * top + i] = 0.f; }
-    return;
+__device__ __forceinline__ unsigned long long lp_remote(const unsigned long long* p, uint32_t rank) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lp_cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+
+// out[0 .. k) = the k largest of n distinct keys in order; a key's place is the number of larger ones. All threads of the CTA.
+__device__ __forceinline__ void lp_sort(const unsigned long long* keys, int n, int k, unsigned long long* out) {
+  for (int i = threadIdx.x; i < n; i += kLpThreads) {
+    const unsigned long long key = keys[i];
+    int larger = 0;
+    for (int j = 0; j < n; ++j) larger += keys[j] > key;
+    if (larger < k) out[larger] = key;
   }
-  const T* p = logits + row * rs;
-  const float c = inv_t * kLog2e, lt = to_f32<T>(p[t]);
-  LpSum a{-INFINITY, 0.f, 0.f};
-  int above = 0;
-  lp_walk<T>(p, V, [&](const auto& v) {
-    lp_join<ENT>(a, v, c);
-    if (rank) {
-#pragma unroll
-      for (int i = 0; i < int(sizeof(v) / 4); ++i) above += v[i] > lt;
-    }
-  }, [&](int, float x) {
-    const float v[1] = {x};
-    lp_join<ENT>(a, v, c);
-    above += x > lt;
-  });
-  a = lp_block<ENT>(a, c, red);
-  if (rank) above = lp_block_count(above, redi);
-  const float ls = logf(a.s);
-  const float H = ENT ? ls - kLn2 * a.u / a.s : 0.f;
-  if (threadIdx.x == 0) {
-    if (lp) lp[row] = (lt - a.m) * inv_t - ls;
-    if (ENT) ent[row] = H;
-    if (rank) rank[row] = 1 + above;
-    if (stats) stats[row] = make_float4(a.m, 1.f / a.s, ls, H);
-  }
-  unsigned long long last = ~0ull;                                     // above every key: a NaN's has ids below 2^31
-  for (int k = 0; k < top; ++k) {
+  __syncthreads();
+}
+
+// The k largest keys of p[0 .. n) (ids from id0 on) into sh.best, one pass a key: for what the shorter way below does not take.
+template <typename T>
+__device__ __noinline__ void lp_top_by_passes(const T* __restrict__ p, int n, int id0, int k, LpShared& sh) {
+  unsigned long long last = ~0ull;
+  for (int i = 0; i < k; ++i) {
     unsigned long long best = 0;
-    for (int j = threadIdx.x; j < V; j += blockDim.x) {
-      const unsigned long long key = lp_key(to_f32<T>(p[j]), j);
+    for (int j = threadIdx.x; j < n; j += kLpThreads) {
+      const unsigned long long key = lp_key(to_f32<T>(p[j]), id0 + j);
       if (key < last && key > best) best = key;
     }
 #pragma unroll
@@ -180,92 +124,296 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, const long lon
       best = x > best ? x : best;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) redk[threadIdx.x >> 5] = best;
+    if ((threadIdx.x & 31) == 0) sh.list[threadIdx.x >> 5] = best;
     __syncthreads();
-    for (int w = 0; w < kLpThreads / 32; ++w) best = redk[w] > best ? redk[w] : best;
+    for (int w = 0; w < kLpWarps; ++w) best = sh.list[w] > best ? sh.list[w] : best;
+    if (threadIdx.x == 0) sh.best[i] = best;
     last = best;
-    if (threadIdx.x == 0) {
-      const int id = int(~uint32_t(best));
-      top_ids[row * top + k] = id;
-      top_lp[row * top + k] = (to_f32<T>(p[id]) - a.m) * inv_t - ls;
+  }
+  __syncthreads();
+}
+
+// The k largest of p[0 .. n), from what each thread noted on its way: the largest value among its vectors and the group that first had it.
+// The k threads with the largest of those values (lowest ids first) have all k of them: a value that is none of these threads' is smaller than
+// each of their largest. So only their vectors are looked at again, about k values in all are not below the last of those, and they are ordered.
+template <typename T>
+__device__ __forceinline__ void lp_top(const T* __restrict__ p, int n, int id0, int k, LpWalk at, float most, int group, LpShared& sh) {
+  constexpr int N = LpVec<T>::N;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
+  // 1. a bound by values alone, so that few threads look up where their largest is: the k-th of 64 groups of four threads
+  const uint32_t own = group < 0 ? 0u : lp_order(most);
+  uint32_t g = max(own, __shfl_xor_sync(0xffffffffu, own, 1));
+  g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+  if ((lane & 3) == 0) sh.group[threadIdx.x >> 2] = g;
+  if (threadIdx.x == 0) { sh.n = 0; sh.bound = 0; }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const uint32_t v = sh.group[threadIdx.x];
+    int before = 0;
+    for (int j = 0; j < 64; ++j) before += sh.group[j] > v || (sh.group[j] == v && j < int(threadIdx.x));
+    if (before == k - 1) sh.bound = v;
+  }
+  __syncthreads();
+  // 2. those threads' largest with their ids, and which of them are the k largest
+  const uint32_t least = max(uint32_t(sh.bound), 1u);
+  unsigned long long mine = 0;
+  if (own >= least) {
+    const int vecs = lp_group(group, at.nvec);
+    for (int x = 0; x < vecs; ++x) {
+      const int i = group + x * kLpThreads;
+      const uint4 raw = __ldg(q + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const unsigned long long key = lp_key(to_f32<T>(reinterpret_cast<const T*>(&raw)[j]), id0 + at.head + i * N + j);
+        mine = key > mine ? key : mine;
+      }
+    }
+    sh.list[atomicAdd(&sh.n, 1)] = mine;
+  }
+  __syncthreads();
+  const int found = sh.n;
+  int larger = kLpThreads;
+  if (mine) {
+    larger = 0;
+    for (int j = 0; j < found; ++j) larger += sh.list[j] > mine;
+    if (larger < k) sh.chosen[larger] = threadIdx.x;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) { sh.n = 0; if (found < k) sh.bound = 0; }
+  if (larger == k - 1) sh.bound = mine;
+  __syncthreads();
+  // 3. the chosen threads' vectors again, a warp each, and the single values at the ends
+  const unsigned long long bound = sh.bound;
+  auto offer = [&](float v, int j) {
+    const unsigned long long key = lp_key(v, id0 + j);
+    if (key >= bound) {
+      const int i = atomicAdd(&sh.n, 1);
+      if (i < 1024) sh.list[i] = key;
+    }
+  };
+  for (int b = w; b < min(found, k); b += kLpWarps) {
+    const int t = sh.chosen[b];
+    for (int i = t + lane * kLpThreads; i < at.nvec; i += 32 * kLpThreads) {
+      const uint4 raw = __ldg(q + i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) offer(to_f32<T>(reinterpret_cast<const T*>(&raw)[j]), at.head + i * N + j);
     }
   }
+  if (threadIdx.x < at.head) offer(to_f32<T>(p[threadIdx.x]), threadIdx.x);
+  if (threadIdx.x < n - at.tail) offer(to_f32<T>(p[at.tail + threadIdx.x]), at.tail + threadIdx.x);
+  __syncthreads();
+  const int m = sh.n;
+  if (m > 1024 || m < min(k, n)) lp_top_by_passes<T>(p, n, id0, k, sh);      // large values close together in few threads, or NaN
+  else lp_sort(sh.list, m, k, sh.best);
 }
 
-// dl_j = 2^x_j (A + B x_j) + [j = t] g / T with A = -(g + h (H - log s)) / T, B = -h log(2) / T, both with 1 / s in them.
-struct LpGrad { float m, A, B, g; long long t; };
-__device__ __forceinline__ LpGrad lp_grad_of(float4 st, float g, float h, float inv_t, long long t, float scale) {
-  return {st.x, -(g + h * (st.w - st.z)) * inv_t * st.y * scale, -h * kLn2 * inv_t * st.y * scale, g * inv_t * scale, t};
-}
-__device__ __forceinline__ float lp_grad_at(float l, const LpGrad& q, float c) {
-  const float x = (l - q.m) * c;
-  return lp_exp2(x) * fmaf(q.B, lp_factor(x), q.A);
+// A row by a cluster of CTAs (of one, where there are rows enough), a slice each.
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kLpThreads, 4)
+lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, const long long* __restrict__ tokens, float inv_t, int top, float* __restrict__ lp,
+               float* __restrict__ ent, long long* __restrict__ rank, long long* __restrict__ top_ids, float* __restrict__ top_lp,
+               float4* __restrict__ stats) {
+  constexpr int N = LpVec<T>::N;
+  __shared__ LpShared sh;
+  const uint32_t parts = lp_cluster_size(), part = cluster_ctarank();
+  const long long row = blockIdx.x / parts;
+  const long long t = tokens ? tokens[row] : 0;
+  if (t < 0 || t >= V) {                                                // all CTAs of the cluster go
+    if (part == 0 && threadIdx.x == 0) {
+      if (lp) lp[row] = 0.f;
+      if (ENT) ent[row] = 0.f;
+      if (rank) rank[row] = 0;
+      if (stats) stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (part == 0)
+      for (int i = threadIdx.x; i < top; i += kLpThreads) { top_ids[row * top + i] = -1; top_lp[row * top + i] = 0.f; }
+    return;
+  }
+  const int id0 = part * slice, n = max(0, min(slice, V - id0));
+  const T* p = logits + row * rs + id0;
+  const float c = inv_t * kLog2e, lt = to_f32<T>(logits[row * rs + t]);
+  LpSum a{-INFINITY, 0.f, 0.f};
+  int above = 0, group = -1;
+  float most = -INFINITY;
+  const LpWalk at = lp_walk<T>(p, n);
+  auto single = [&](int j) {
+    const float v[1] = {to_f32<T>(p[j])};
+    lp_join<ENT>(a, v, v[0], c);
+    above += v[0] > lt;
+  };
+  auto vectors = [&](auto& raw, int i) {
+    constexpr int G = sizeof(raw) / 16;
+    float v[G * N];
+    const float m = lp_values<T, G>(raw, v);
+    lp_join<ENT>(a, v, m, c);
+    if (rank && m > lt) {
+#pragma unroll
+      for (int j = 0; j < G * N; ++j) above += v[j] > lt;
+    }
+    if (m > most || group < 0) { most = m; group = i; }
+  };
+  if (threadIdx.x < at.head) single(threadIdx.x);
+  {
+    const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
+    int i = threadIdx.x;
+    for (; i + (kLpGroup - 1) * kLpThreads < at.nvec; i += kLpGroup * kLpThreads) {
+      uint4 raw[kLpGroup];
+#pragma unroll
+      for (int g = 0; g < kLpGroup; ++g) raw[g] = __ldg(q + i + g * kLpThreads);
+      vectors(raw, i);
+    }
+    for (; i < at.nvec; i += kLpThreads) {
+      uint4 raw[1] = {__ldg(q + i)};
+      vectors(raw, i);
+    }
+  }
+  if (threadIdx.x < n - at.tail) single(at.tail + threadIdx.x);
+  // the CTA's threads
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = lp_both<ENT>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
+  above = __reduce_add_sync(0xffffffffu, above);
+  if (lane == 0) { sh.red[0][w] = a.m; sh.red[1][w] = a.s; sh.red[2][w] = a.u; sh.redi[w] = above; }
+  __syncthreads();
+  a = {sh.red[0][0], sh.red[1][0], sh.red[2][0]};
+  above = sh.redi[0];
+  for (int x = 1; x < kLpWarps; ++x) {
+    a = lp_both<ENT>(a, {sh.red[0][x], sh.red[1][x], sh.red[2][x]}, c);
+    above += sh.redi[x];
+  }
+  const int k = min(top, n);
+  if (k > 0) {
+    if (a.s == a.s) lp_top<T>(p, n, id0, k, at, most, group, sh);
+    else lp_top_by_passes<T>(p, n, id0, k, sh);                          // a NaN or plus infinity, which the maxima on the way do not count
+  }
+  // the cluster's CTAs
+  if (parts > 1) {
+    if (threadIdx.x == 0) sh.sums = make_float4(a.m, a.s, a.u, __int_as_float(above));
+    __syncthreads();
+    cluster_sync_all();
+    if (part == 0) {
+      for (uint32_t x = 1; x < parts; ++x) {
+        const unsigned long long *s0 = reinterpret_cast<const unsigned long long*>(&sh.sums), lo = lp_remote(s0, x), hi = lp_remote(s0 + 1, x);
+        a = lp_both<ENT>(a, {__uint_as_float(uint32_t(lo)), __uint_as_float(uint32_t(lo >> 32)), __uint_as_float(uint32_t(hi))}, c);
+        above += int(uint32_t(hi >> 32));
+      }
+      if (top > 0) {
+        int all = 0;                                                     // slices have top alternatives each, the last one maybe fewer
+        for (uint32_t x = 0; x < parts; ++x) {
+          const int kx = min(top, max(0, min(slice, V - int(x) * slice)));
+          if (int(threadIdx.x) < kx) sh.list[all + threadIdx.x] = lp_remote(sh.best + threadIdx.x, x);
+          all += kx;
+        }
+        __syncthreads();
+        lp_sort(sh.list, all, top, sh.best);
+      }
+    }
+  }
+  if (part == 0) {
+    const float ls = logf(a.s), H = ENT ? ls - kLn2 * a.u / a.s : 0.f;
+    if (threadIdx.x == 0) {
+      if (lp) lp[row] = (lt - a.m) * inv_t - ls;
+      if (ENT) ent[row] = H;
+      if (rank) rank[row] = 1 + above;
+      if (stats) stats[row] = make_float4(a.m, 1.f / a.s, ls, H);
+    }
+    if (int(threadIdx.x) < top) {
+      const unsigned long long key = sh.best[threadIdx.x];
+      top_ids[row * top + threadIdx.x] = lp_id(key);
+      top_lp[row * top + threadIdx.x] = (lp_of_key(key) - a.m) * inv_t - ls;
+    }
+  }
+  if (parts > 1) {                                                       // nobody leaves while its memory is read
+    __syncthreads();
+    cluster_sync_all();
+  }
 }
 
-template <typename T>
+template <typename T, bool HASH>
 __global__ void __launch_bounds__(kLpThreads)
-lp_rows_grad_kernel(const T* __restrict__ logits, long long rs, int V, const long long* __restrict__ tokens, float inv_t, const float4* __restrict__ stats,
+lp_rows_grad_kernel(const T* __restrict__ logits, long long rs, int V, int slice, const long long* __restrict__ tokens, float inv_t, const float4* __restrict__ stats,
                     const float* __restrict__ g, const float* __restrict__ h, T* __restrict__ out, long long os) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = LpVec<T>::N, G = 2;
   const long long row = blockIdx.x;
+  const int id0 = blockIdx.y * slice, n = min(slice, V - id0);
   const long long t = tokens ? tokens[row] : 0;
   const bool skip = t < 0 || t >= V;
-  const T* p = logits + row * rs;
-  T* o = out + row * os;
+  const T* p = logits + row * rs + id0;
+  T* o = out + row * os + id0;
   const float c = inv_t * kLog2e;
-  const LpGrad q = lp_grad_of(stats[row], g ? g[row] : 0.f, h ? h[row] : 0.f, inv_t, tokens ? t : -1, 1.f);
-  const bool same = (((uintptr_t)p ^ (uintptr_t)o) & 15) == 0;          // both aligned at the same elements
-  const int head = min(V, int((16 - ((uintptr_t)p & 15)) & 15) / int(sizeof(T)));
-  const int nvec = (V - head) / N;
-  auto one = [&](int j) { o[j] = from_f32<T>(skip ? 0.f : lp_grad_at(to_f32<T>(p[j]), q, c) + (j == q.t ? q.g : 0.f)); };
-  if (threadIdx.x < head) one(threadIdx.x);
-  for (int i = threadIdx.x; i < nvec; i += blockDim.x) {
-    const int j0 = head + i * N;
-    alignas(16) T in[N];
-    alignas(16) T r[N];
-    if (!skip) *reinterpret_cast<uint4*>(in) = __ldg(reinterpret_cast<const uint4*>(p + j0));
+  const LpGrad r = lp_grad_of(stats[row], g ? g[row] : 0.f, HASH && h ? h[row] : 0.f, inv_t, (tokens ? t : -1) - id0, 1.f);
+  const LpWalk at = lp_walk<T>(p, n);
+  const bool same = (((uintptr_t)p ^ (uintptr_t)o) & 15) == 0;          // both have their multiples of 16 bytes at the same elements
+  auto single = [&](int j) { o[j] = from_f32<T>(skip ? 0.f : lp_grad_at(to_f32<T>(p[j]), r, c)); };
+  auto vector = [&](const uint4& raw, int i) {
+    alignas(16) T y[N];
+    float v[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) r[j] = from_f32<T>(skip ? 0.f : lp_grad_at(to_f32<T>(in[j]), q, c) + (j0 + j == q.t ? q.g : 0.f));
-    if (same) *reinterpret_cast<uint4*>(o + j0) = *reinterpret_cast<uint4*>(r);
+    for (int j = 0; j < N; ++j) v[j] = to_f32<T>(reinterpret_cast<const T*>(&raw)[j]);
+    const unsigned long long nm = lp_pair(-r.m, -r.m), cc = lp_pair(c, c), A = lp_pair(r.A, r.A), B = lp_pair(r.B, r.B);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const unsigned long long x = lp_mul2(lp_add2(lp_pair(v[j], v[j + 1]), nm), cc);
+      const float2 xs = lp_split(x);
+      const unsigned long long e = lp_pair(lp_exp2(xs.x), lp_exp2(xs.y));
+      const float2 d = lp_split(lp_mul2(e, HASH ? lp_fma2(B, lp_pair(lp_factor(xs.x), lp_factor(xs.y)), A) : A));
+      y[j] = from_f32<T>(d.x);
+      y[j + 1] = from_f32<T>(d.y);
+    }
+    uint4 w = skip ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<uint4*>(y);
+    T* to = o + at.head + i * N;
+    if (same) *reinterpret_cast<uint4*>(to) = w;
     else
 #pragma unroll
-      for (int j = 0; j < N; ++j) o[j0 + j] = r[j];
+      for (int j = 0; j < N; ++j) to[j] = reinterpret_cast<const T*>(&w)[j];
+  };
+  if (threadIdx.x < at.head) single(threadIdx.x);
+  const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
+  int i = threadIdx.x;
+  for (; i + (G - 1) * kLpThreads < at.nvec; i += G * kLpThreads) {
+    uint4 raw[G];
+#pragma unroll
+    for (int x = 0; x < G; ++x) raw[x] = skip ? make_uint4(0, 0, 0, 0) : __ldg(q + i + x * kLpThreads);
+#pragma unroll
+    for (int x = 0; x < G; ++x) vector(raw[x], i + x * kLpThreads);
   }
-  for (int j = head + nvec * N + threadIdx.x; j < V; j += blockDim.x) one(j);
+  for (; i < at.nvec; i += kLpThreads) vector(skip ? make_uint4(0, 0, 0, 0) : __ldg(q + i), i);
+  if (threadIdx.x < n - at.tail) single(at.tail + threadIdx.x);
+  if (!skip && r.t >= 0 && r.t < n) {                                    // the token's own term, over what its vector's thread wrote
+    __syncthreads();
+    if (threadIdx.x == 0) o[r.t] = from_f32<T>(lp_grad_at(to_f32<T>(p[r.t]), r, c) + r.g);
+  }
 }
 
-// ---- logits a chunk of the vocabulary at a time ----
-// run [rows] = (m, s, u, l_t) of what came before columns c0 .. c0 + C of the vocabulary; the first chunk makes it.
-template <bool ENT>
+// ---- logits that are not stored ----
+// part [n][rows] = (m, s, u) of n parts of each row, lt [rows] its token's logit. 32 rows a CTA, 8 threads a row.
 __global__ void __launch_bounds__(256)
-lp_chunk_kernel(const float* __restrict__ lg, long long rs, int C, int c0, const long long* __restrict__ tokens, float inv_t, float4* __restrict__ run) {
-  __shared__ float red[96];
-  const long long row = blockIdx.x;
+lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, const long long* __restrict__ tokens, const float* __restrict__ lt, float inv_t,
+                 float* __restrict__ lp, float* __restrict__ ent, float4* __restrict__ stats) {
+  __shared__ float red[3][8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long row = blockIdx.x * 32ll + lane;
   const float c = inv_t * kLog2e;
-  const float* p = lg + row * rs;
   LpSum a{-INFINITY, 0.f, 0.f};
-  lp_walk<float>(p, C, [&](const auto& v) { lp_join<ENT>(a, v, c); }, [&](int, float x) { const float v[1] = {x}; lp_join<ENT>(a, v, c); });
-  a = lp_block<ENT>(a, c, red);
-  if (threadIdx.x == 0) {
-    float4 r = c0 == 0 ? make_float4(-INFINITY, 0.f, 0.f, 0.f) : run[row];
-    const LpSum b = lp_both<ENT>({r.x, r.y, r.z}, a, c);
-    const long long t = tokens ? tokens[row] - c0 : -1;
-    run[row] = make_float4(b.m, b.s, b.u, t >= 0 && t < C ? p[t] : r.w);
+  if (row < rows) {
+#pragma unroll 8
+    for (int i = w; i < n; i += 8) {
+      const float4 x = __ldg(part + i * rows + row);
+      a = lp_both<true>(a, {x.x, x.y, x.z}, c);
+    }
   }
-}
-
-__global__ void __launch_bounds__(256)
-lp_finish_kernel(const float4* __restrict__ run, long long rows, int V, const long long* __restrict__ tokens, float inv_t, float* __restrict__ lp,
-                 float* __restrict__ ent, float4* __restrict__ stats) {
-  const long long row = blockIdx.x * 256ll + threadIdx.x;
-  if (row >= rows) return;
+  red[0][w][lane] = a.m; red[1][w][lane] = a.s; red[2][w][lane] = a.u;
+  __syncthreads();
+  if (w || row >= rows) return;
+  for (int i = 1; i < 8; ++i) a = lp_both<true>(a, {red[0][i][lane], red[1][i][lane], red[2][i][lane]}, c);
   const long long t = tokens ? tokens[row] : 0;
   const bool skip = t < 0 || t >= V;
-  const float4 r = run[row];
-  const float ls = logf(r.y), H = ls - kLn2 * r.z / r.y;
-  if (lp) lp[row] = skip ? 0.f : (r.w - r.x) * inv_t - ls;
+  const float ls = logf(a.s), H = ls - kLn2 * a.u / a.s;
+  if (lp) lp[row] = skip ? 0.f : (lt[row] - a.m) * inv_t - ls;
   if (ent) ent[row] = skip ? 0.f : H;
-  if (stats) stats[row] = make_float4(r.x, 1.f / r.y, ls, H);
+  if (stats) stats[row] = make_float4(a.m, 1.f / a.s, ls, H);
 }
 
 // A power of two that brings the largest gradient of a logit to 2^13 .. 2^14, so that fp16 holds the small ones too, and its reciprocal.
@@ -280,28 +428,6 @@ lp_scale_kernel(const float* __restrict__ g, const float* __restrict__ h, long l
   const int e = m > 0.f && m < INFINITY ? min(max(14 - (ilogbf(m) + 1), -100), 100) : 0;
   scale[0] = ldexpf(1.f, e);
   scale[1] = ldexpf(1.f, -e);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-lp_chunk_grad_kernel(const float* __restrict__ lg, long long rs, int C, int c0, int V, const long long* __restrict__ tokens, float inv_t,
-                     const float4* __restrict__ stats, const float* __restrict__ g, const float* __restrict__ h, const float* __restrict__ scale,
-                     T* __restrict__ out, long long os) {
-  const long long row = blockIdx.x;
-  const long long t = tokens ? tokens[row] : 0;
-  const bool skip = t < 0 || t >= V;
-  const float* p = lg + row * rs;
-  T* o = out + row * os;
-  const float c = inv_t * kLog2e;
-  const LpGrad q = lp_grad_of(stats[row], g ? g[row] : 0.f, h ? h[row] : 0.f, inv_t, tokens ? t - c0 : -1, scale ? scale[0] : 1.f);
-  for (int j0 = threadIdx.x * 4; j0 < C; j0 += blockDim.x * 4) {        // rows of both are padded to whole groups of four
-    const float4 in = *reinterpret_cast<const float4*>(p + j0);
-    const float v[4] = {in.x, in.y, in.z, in.w};
-    alignas(8) T r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = from_f32<T>(skip || j0 + j >= C ? 0.f : lp_grad_at(v[j], q, c) + (j0 + j == q.t ? q.g : 0.f));
-    *reinterpret_cast<uint2*>(o + j0) = *reinterpret_cast<uint2*>(r);
-  }
 }
 
 // y = x * scale[1] in the type of the gradients.
@@ -333,14 +459,36 @@ using namespace b200;
 
 static bool lp_bad(long long rows, int V) { return rows < 0 || rows > 0x7fffffffll || V <= 0; }
 
+// Rows of few: a cluster of up to eight CTAs a row, as long as each has 4096 logits or more and the GPU's SMs are not all busy.
+static int lp_parts(long long rows, int V) {
+  int parts = 1;
+  while (parts < kLpMaxCluster && rows * parts * 2 <= 2 * kNumSMs && V / (parts * 2) >= 4096) parts *= 2;
+  return parts;
+}
+static int lp_slice(int V, int parts) { return ((V + parts - 1) / parts + 31) / 32 * 32; }
+
+template <typename T, bool ENT>
+static cudaError_t lp_rows_launch(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp, float* ent,
+                                  long long* rank, long long* top_ids, float* top_lp, void* stats, cudaStream_t st) {
+  const int parts = lp_parts(rows, V);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows * parts)); cfg.blockDim = dim3(kLpThreads); cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, lp_rows_kernel<T, ENT>, (const T*)logits, rs, V, parts > 1 ? lp_slice(V, parts) : V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp,
+                            (float4*)stats);
+}
+
 B200_API int b200_token_logprobs(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp,
                                  float* ent, long long* rank, long long* top_ids, float* top_lp, void* stats, int dtype, void* stream) {
-  if (lp_bad(rows, V) || top < 0 || top > 32 || top > V) return B200_ERR_BAD_SHAPE;
+  if (lp_bad(rows, V) || top < 0 || top > kLpMaxTop || top > V) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
   cudaStream_t st = (cudaStream_t)stream;
   LP_TYPES(dtype, {
-    if (ent) lp_rows_kernel<T, true><<<(unsigned)rows, kLpThreads, 0, st>>>((const T*)logits, rs, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, (float4*)stats);
-    else lp_rows_kernel<T, false><<<(unsigned)rows, kLpThreads, 0, st>>>((const T*)logits, rs, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, (float4*)stats);
+    if (ent) B200_CHECK((lp_rows_launch<T, true>(logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)));
+    else B200_CHECK((lp_rows_launch<T, false>(logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)));
   });
   B200_LAUNCH_CHECK();
   return 0;
@@ -351,28 +499,24 @@ B200_API int b200_token_logprobs_grad(const void* logits, long long rs, long lon
   if (lp_bad(rows, V)) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
   cudaStream_t st = (cudaStream_t)stream;
-  LP_TYPES(dtype, lp_rows_grad_kernel<T><<<(unsigned)rows, kLpThreads, 0, st>>>((const T*)logits, rs, V, tokens, inv_t, (const float4*)stats, g, h,
-                                                                             (T*)out, os));
+  // few rows: slices of 4096 logits, CTAs of their own
+  int parts = 1;
+  while (parts < 64 && rows * parts * 2 <= 8 * kNumSMs && V / (parts * 2) >= 2048) parts *= 2;
+  const int slice = parts > 1 ? lp_slice(V, parts) : V;
+  const dim3 grid((unsigned)rows, (unsigned)((V + slice - 1) / slice));
+  LP_TYPES(dtype, {
+    if (h) lp_rows_grad_kernel<T, true><<<grid, kLpThreads, 0, st>>>((const T*)logits, rs, V, slice, tokens, inv_t, (const float4*)stats, g, h, (T*)out, os);
+    else lp_rows_grad_kernel<T, false><<<grid, kLpThreads, 0, st>>>((const T*)logits, rs, V, slice, tokens, inv_t, (const float4*)stats, g, h, (T*)out, os);
+  });
   B200_LAUNCH_CHECK();
   return 0;
 }
 
-B200_API int b200_logprob_chunk(const float* lg, long long rs, long long rows, int C, int c0, const long long* tokens, float inv_t, void* run, int entropy,
-                                void* stream) {
-  if (lp_bad(rows, C) || c0 < 0) return B200_ERR_BAD_SHAPE;
+B200_API int b200_logprob_finish(const void* part, int parts, long long rows, int V, const long long* tokens, const float* lt, float inv_t, float* lp, float* ent,
+                                 void* stats, void* stream) {
+  if (lp_bad(rows, V) || parts < 1) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (entropy) lp_chunk_kernel<true><<<(unsigned)rows, 256, 0, st>>>(lg, rs, C, c0, tokens, inv_t, (float4*)run);
-  else lp_chunk_kernel<false><<<(unsigned)rows, 256, 0, st>>>(lg, rs, C, c0, tokens, inv_t, (float4*)run);
-  B200_LAUNCH_CHECK();
-  return 0;
-}
-
-B200_API int b200_logprob_finish(const void* run, long long rows, int V, const long long* tokens, float inv_t, float* lp, float* ent, void* stats,
-                                 void* stream) {
-  if (lp_bad(rows, V)) return B200_ERR_BAD_SHAPE;
-  if (rows == 0) return 0;
-  lp_finish_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const float4*)run, rows, V, tokens, inv_t, lp, ent, (float4*)stats);
+  lp_finish_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, (cudaStream_t)stream>>>((const float4*)part, parts, rows, V, tokens, lt, inv_t, lp, ent, (float4*)stats);
   B200_LAUNCH_CHECK();
   return 0;
 }
@@ -380,17 +524,6 @@ B200_API int b200_logprob_finish(const void* run, long long rows, int V, const l
 B200_API int b200_logprob_scale(const float* g, const float* h, long long rows, float inv_t, int V, float* scale, void* stream) {
   if (lp_bad(rows, V)) return B200_ERR_BAD_SHAPE;
   lp_scale_kernel<<<1, 256, 0, (cudaStream_t)stream>>>(g, h, rows, inv_t, logf((float)V), scale);
-  B200_LAUNCH_CHECK();
-  return 0;
-}
-
-B200_API int b200_logprob_chunk_grad(const float* lg, long long rs, long long rows, int C, int c0, int V, const long long* tokens, float inv_t,
-                                     const void* stats, const float* g, const float* h, const float* scale, void* out, long long os, int dtype, void* stream) {
-  if (lp_bad(rows, C) || c0 < 0 || rs < (C + 3) / 4 * 4 || os < (C + 3) / 4 * 4) return B200_ERR_BAD_SHAPE;
-  if (rs % 4 || os % 4 || (uintptr_t)lg % 16 || (uintptr_t)out % 8) return B200_ERR_BAD_ALIGN;
-  if (rows == 0) return 0;
-  LP_TYPES16(dtype, lp_chunk_grad_kernel<T><<<(unsigned)rows, 256, 0, (cudaStream_t)stream>>>(lg, rs, C, c0, V, tokens, inv_t, (const float4*)stats, g, h,
-                                                                                          scale, (T*)out, os));
   B200_LAUNCH_CHECK();
   return 0;
 }

@@ -817,14 +817,18 @@ int b200_token_logprobs(const void* logits, long long rs, long long rows, int V,
 /* out [rows, V] (row stride os) = gradient of the logits for gradients g of lp and h of ent (fp32 [rows], NULL: zeros). */
 int b200_token_logprobs_grad(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, const void* stats,
                              const float* g, const float* h, void* out, long long os, int dtype, void* stream);
-/* The same from fp32 logits of columns c0 .. c0 + C, chunk after chunk: run fp32 [rows, 4] is made by the chunk with c0 = 0 and carried on by the others. */
-int b200_logprob_chunk(const float* lg, long long rs, long long rows, int C, int c0, const long long* tokens, float inv_t, void* run, int entropy, void* stream);
-int b200_logprob_finish(const void* run, long long rows, int V, const long long* tokens, float inv_t, float* lp, float* ent, void* stats, void* stream);
+/* The same from x [M, K] and w [N, K] (bf16 or fp16, rows at multiples of 16 bytes): sums of each row's logits in a tile's columns into part fp32
+ * [b200_gemm_head_tiles(M, N, K), M, 4], the tokens' logits into lt fp32 [M] (csrc/gemm_tcgen05.cu), then what token_logprobs gives. */
+int b200_gemm_head_tiles(int M, int N, int K);   /* below zero: minus a status */
+int b200_gemm_head_sums(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, float inv_t,
+                        int entropy, void* part, float* lt, void* stream);
+int b200_logprob_finish(const void* part, int parts, long long rows, int V, const long long* tokens, const float* lt, float inv_t, float* lp, float* ent, void* stats,
+                        void* stream);
 /* scale [2]: a power of two that brings gradients into fp16's range, and its reciprocal. */
 int b200_logprob_scale(const float* g, const float* h, long long rows, float inv_t, int V, float* scale, void* stream);
-/* out (16 bits, row stride os) = gradient of a chunk's logits, times scale[0]; rows of lg and out have room for whole groups of four columns. */
-int b200_logprob_chunk_grad(const float* lg, long long rs, long long rows, int C, int c0, int V, const long long* tokens, float inv_t, const void* stats,
-                            const float* g, const float* h, const float* scale, void* out, long long os, int dtype, void* stream);
+/* out [M, N] (row stride out_rs) = gradient, in 16 bits, of the logits of columns c0 .. c0 + N of a vocabulary of V (w: those rows), times scale[0] (NULL: 1). */
+int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, int V, int c0,
+                         float inv_t, const void* stats, const float* g, const float* h, const float* scale, void* out, long long out_rs, void* stream);
 /* y (16 bits) = x * scale[1] (scale NULL: x). */
 int b200_logprob_cast(const float* x, void* y, long long n, const float* scale, int dtype, void* stream);
 
@@ -835,7 +839,7 @@ long long b200_embedding_grad_workspace(long long T, int D);
 int b200_embedding_grad(const long long* ids, const void* dy, long long rs, void* out, long long T, int V, int D, float scale, long long padding, int dtype,
                         int out_dtype, void* workspace, void* stream);
 
-/* Activations in 8 bits (csrc/act8.cu): blocks of 32 neighbours share a power of two. q int8 [rows, 32 nb] (8-byte aligned), e uint8 [rows, nb], nb = ceil(D / 32);
+/* Activations in 8 bits (csrc/act8.cu): blocks of 32 neighbours share a power of two. q int8 [rows, 32 nb] (16-byte aligned), e uint8 [rows, nb], nb = ceil(D / 32);
  * a value is q * 2^(e - 127), q = -128 is NaN. x, add, gu with row strides, y and dgu dense. add (NULL: none) joins x, rounded to dtype. */
 int b200_pack8(const void* x, long long x_rs, const void* add, long long add_rs, void* q, void* e, long long rows, int D, int dtype, void* stream);
 int b200_unpack8(const void* q, const void* e, void* y, long long rows, int D, int dtype, void* stream);

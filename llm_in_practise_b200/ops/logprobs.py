@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nv
-from .gemm import gemm, gemv16
+from .gemm import gemm
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 MAX_TOP = 32             # alternatives of a row
@@ -175,44 +175,39 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 # ------------------------------------------------------------------------------------------------
 # from hidden states
 # ------------------------------------------------------------------------------------------------
-_CHUNK_BYTES = 64 << 20          # fp32 logits that exist at a time: they stay in the 126 MB L2 between the product and what reads them
+_CHUNK_BYTES = 128 << 20         # 16-bit gradients of logits that exist at a time in the backward pass
+_HEAD = [vp, i64, vp, i64, i32, i32, i32, i32, vp]
 
 
 def _chunks(T: int, V: int):
-    """Columns of the vocabulary that are taken at a time."""
-    C = max(_CHUNK_BYTES // (4 * max(T, 1)), 2048) // 256 * 256
-    n = -(-V // min(C, V))
-    C = min((-(-V // n) + 255) // 256 * 256, V)                       # chunks of about the same size
-    return [(a, min(V, a + C)) for a in range(0, V, C)], C
-
-
-def _chunk_logits(x, w, buf, c0, c1):
-    """fp32 logits of columns c0 .. c1, as rows of ``buf``."""
-    y = gemv16(x, w[c0:c1], out_dtype=torch.float32) if x.shape[0] <= 16 else None
-    return y if y is not None else gemm(x, w[c0:c1], out=buf[:, :c1 - c0])
+    """Columns of the vocabulary whose gradients exist at a time: chunks of about the same size."""
+    n = -(-V // min(max(_CHUNK_BYTES // (2 * max(T, 1)), 4096), V))
+    C = (-(-V // n) + 255) // 256 * 256
+    return [(a, min(V, a + C)) for a in range(0, V, C)], min(C, V)
 
 
 def _linear_forward(x, w, tokens, temperature, entropy, save):
-    T, V = x.shape[0], w.shape[0]
+    T, K = x.shape
+    V = w.shape[0]
+    if not nv.use_native(x):
+        lp, H, _, _, _, stats = _rows_torch(x.float() @ w.float().t(), tokens, temperature, 0, entropy, False)
+        return lp, H, stats
     lp = x.new_empty(T, dtype=torch.float32) if tokens is not None else None
     H = x.new_empty(T, dtype=torch.float32) if entropy else None
     stats = x.new_empty(T, 4, dtype=torch.float32) if save else None
     if T == 0:
         return lp, H, stats
-    inv_t = 1.0 / temperature
-    if not nv.use_native(x):
-        lp, H, _, _, _, stats = _rows_torch(x.float() @ w.float().t(), tokens, temperature, 0, entropy, False)
-        return lp, H, stats
-    chunks, C = _chunks(T, V)
-    buf = torch.empty(T, (C + 7) // 8 * 8, dtype=torch.float32, device=x.device)
-    run = torch.empty(T, 4, dtype=torch.float32, device=x.device)
-    fn = nv.proto("b200_logprob_chunk", [vp, i64, i64, i32, i32, vp, f32, vp, i32, vp])
-    for c0, c1 in chunks:
-        y = _chunk_logits(x, w, buf, c0, c1)
-        nv.check(fn(nv.ptr(y), y.stride(0), T, c1 - c0, c0, nv.ptr(tokens), inv_t, nv.ptr(run), int(entropy), nv.stream()), "logprob_chunk")
-    fin = nv.proto("b200_logprob_finish", [vp, i64, i32, vp, f32, vp, vp, vp, vp])
-    nv.check(fin(nv.ptr(run), T, V, nv.ptr(tokens), inv_t, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), nv.stream()), "logprob_finish")
-    nv.count_launch(len(chunks) + 1)
+    tiles = nv.proto("b200_gemm_head_tiles", [i32] * 3)(T, V, K)
+    if tiles < 0:
+        nv.check(-tiles, "gemm_head_tiles")
+    part = torch.empty(tiles, T, 4, dtype=torch.float32, device=x.device)
+    lt = torch.empty(T, dtype=torch.float32, device=x.device)
+    fn = nv.proto("b200_gemm_head_sums", _HEAD + [f32, i32, vp, vp, vp])
+    nv.check(fn(nv.ptr(x), x.stride(0), nv.ptr(w), w.stride(0), T, V, K, nv.dtype_code(x.dtype), nv.ptr(tokens), 1.0 / temperature, int(entropy), nv.ptr(part),
+                nv.ptr(lt), nv.stream()), "gemm_head_sums")
+    fin = nv.proto("b200_logprob_finish", [vp, i32, i64, i32, vp, vp, f32, vp, vp, vp, vp])
+    nv.check(fin(nv.ptr(part), tiles, T, V, nv.ptr(tokens), nv.ptr(lt), 1.0 / temperature, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), nv.stream()), "logprob_finish")
+    nv.count_launch(2)
     return lp, H, stats
 
 
@@ -228,9 +223,7 @@ def _linear_backward(x, w, tokens, temperature, stats, g, h, need_dx, need_dw):
         return (torch.empty_like(x) if need_dx else None), (None if dw is None else dw.zero_())
     chunks, C = _chunks(T, V)
     ld = (C + 7) // 8 * 8
-    buf = torch.empty(T, ld, dtype=torch.float32, device=dev)
     dl = torch.empty(T, ld, dtype=x.dtype, device=dev)
-    acc = torch.empty(T, K, dtype=torch.float32, device=dev) if need_dx else None
     half = x.dtype == torch.float16
     scale = part = None
     if half:             # gradients of single logits lie below fp16's numbers: they are brought up by a power of two, the results back down
@@ -238,25 +231,25 @@ def _linear_backward(x, w, tokens, temperature, stats, g, h, need_dx, need_dw):
         fs = nv.proto("b200_logprob_scale", [vp, vp, i64, f32, i32, vp, vp])
         nv.check(fs(nv.ptr(g), nv.ptr(h), T, inv_t, V, nv.ptr(scale), nv.stream()), "logprob_scale")
         part = torch.empty(C, K, dtype=torch.float32, device=dev) if need_dw else None
-    fg = nv.proto("b200_logprob_chunk_grad", [vp, i64, i64, i32, i32, i32, vp, f32, vp, vp, vp, vp, vp, i64, i32, vp])
+    dx = torch.empty(T, K, dtype=x.dtype, device=dev) if need_dx else None
+    direct = len(chunks) == 1 and not half                # one product gives dx: no sums in 32 bits between chunks
+    acc = dx if direct else torch.empty(T, K, dtype=torch.float32, device=dev) if need_dx else None
+    fg = nv.proto("b200_gemm_head_grads", _HEAD + [i32, i32, f32, vp, vp, vp, vp, vp, i64, vp])
     fc = nv.proto("b200_logprob_cast", [vp, vp, i64, vp, i32, vp])
     for c0, c1 in chunks:
-        n = c1 - c0
-        gemm(x, w[c0:c1], out=buf[:, :n])
-        nv.check(fg(nv.ptr(buf), ld, T, n, c0, V, nv.ptr(tokens), inv_t, nv.ptr(stats), nv.ptr(g), nv.ptr(h), nv.ptr(scale), nv.ptr(dl), ld, dt, nv.stream()),
-                 "logprob_chunk_grad")
+        n, wc = c1 - c0, w[c0:c1]
+        nv.check(fg(nv.ptr(x), x.stride(0), nv.ptr(wc), w.stride(0), T, n, K, dt, nv.ptr(tokens), V, c0, inv_t, nv.ptr(stats), nv.ptr(g), nv.ptr(h), nv.ptr(scale),
+                    nv.ptr(dl), ld, nv.stream()), "gemm_head_grads")
         if need_dx:
-            gemm(dl[:, :n], w[c0:c1], b_mn=True, out=acc, beta=1.0 if c0 else 0.0)
+            gemm(dl[:, :n], wc, b_mn=True, out=acc, beta=1.0 if c0 else 0.0)
         if need_dw and not half:
             gemm(dl[:, :n], x, a_mn=True, b_mn=True, out=dw[c0:c1])
         elif need_dw:
             gemm(dl[:, :n], x, a_mn=True, b_mn=True, out=part[:n])
             nv.check(fc(nv.ptr(part), nv.ptr(dw[c0:c1]), n * K, nv.ptr(scale), dt, nv.stream()), "logprob_cast")
-    dx = None
-    if need_dx:
-        dx = torch.empty_like(x)
+    if need_dx and not direct:
         nv.check(fc(nv.ptr(acc), nv.ptr(dx), T * K, nv.ptr(scale), dt, nv.stream()), "logprob_cast")
-    nv.count_launch(len(chunks) * (2 if half and need_dw else 1) + bool(need_dx) + half)
+    nv.count_launch(len(chunks) * (2 if half and need_dw else 1) + bool(need_dx and not direct) + half)
     return dx, dw
 
 
@@ -289,7 +282,8 @@ class _LinearLogprobsFn(torch.autograd.Function):
 
 def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor], *, entropy: bool = False, temperature: float = 1.0) -> TokenLogprobs:
     """``token_logprobs(x @ w.T, tokens)`` for hidden states ``x`` [..., K] and an output projection ``w`` [vocab, K] (bf16 or fp16, K a multiple of 8),
-    with fp32 logits that exist a chunk of the vocabulary at a time, in the forward and again in the backward pass. Gradients for ``x`` and ``w``."""
+    without the logits: their sums are taken from the product's accumulators (fp32), and in the backward pass, where the product is computed again, their
+    gradients, which exist in 16 bits a chunk of the vocabulary at a time. Gradients for ``x`` and ``w``."""
     if w.dim() != 2 or w.shape[0] < 1 or x.dim() < 1 or x.shape[-1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
         raise ValueError("linear_token_logprobs: x [..., K] and w [vocab, K] must agree in K, type and device")
     if x.dtype not in ((torch.bfloat16, torch.float16) if nv.use_native(x) else (torch.bfloat16, torch.float16, torch.float32)):

@@ -251,7 +251,7 @@ def test_what_log_probabilities_refuse():
 @pytest.mark.parametrize("T,K,V", [(1, 64, 37), (5, 128, 1001), (17, 64, 4099), (130, 72, 20011), (300, 128, 9000)])
 def test_from_hidden_states(T, K, V, dtype, device, monkeypatch):
     """Chunks of the vocabulary, odd sizes, rows that are passed over; the gradients of both operands, small ones too (weights of 1e-6)."""
-    monkeypatch.setattr(lpm, "_CHUNK_BYTES", 4 * T * 2560)             # several chunks, the last one short
+    monkeypatch.setattr(lpm, "_CHUNK_BYTES", 0)                         # chunks of 4096 columns at most, the last one short
     dt, tau = DT[dtype], 0.8
     r = torch.Generator().manual_seed(T)
     x, w = torch.randn(T, K, generator=r).to(dt), (torch.randn(V, K, generator=r) * 3 / K ** 0.5).to(dt)
