@@ -139,11 +139,11 @@ template <typename T> __device__ __forceinline__ void a8_add(A8Raw<T>& r, const 
 // The largest byte e + 127 of a type.
 template <typename T> __device__ __forceinline__ constexpr int a8_top() { return std::is_same<T, __half>::value ? 9 + 127 : 121 + 127; }
 
-// Sixteen values of a block whose other half is with the neighbouring lane: their q as bytes, and the block's byte of e. All lanes of the warp call it.
-// Where all are finite and no e was cut, q is the low byte of x 2^-e + 1.5 (2^23), one operation that rounds as rint does (with conversions,
-// tests for infinities and bounds for each value pack8 took 84 us of 16384 x 4096 + 16384 x 4096, bound by its instructions).
+// The power of two of a block, of which this thread has half and the neighbouring lane the other: its byte, 2^-e, and whether all values are finite
+// and no e was cut. All lanes of the warp call it.
+struct A8Scale { int eb; float inv; bool plain; };
 template <typename T>
-__device__ __forceinline__ uint4 a8_encode(const A8Raw<T>& r, int& eb) {
+__device__ __forceinline__ A8Scale a8_scale(const A8Raw<T>& r) {
   constexpr int TOP = a8_top<T>();
   uint32_t most = 0;
   if constexpr (sizeof(T) == 4) {
@@ -155,24 +155,18 @@ __device__ __forceinline__ uint4 a8_encode(const A8Raw<T>& r, int& eb) {
     most = max(most & 0xffffu, most >> 16);
   }
   most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-  bool plain;
+  A8Scale s;
   if constexpr (std::is_same<T, __half>::value) {
-    plain = most < 0x7c00u;
+    s.plain = most < 0x7c00u;
     most = __float_as_uint(__half2float(__ushort_as_half(uint16_t(most))));
   } else {
     if constexpr (sizeof(T) == 2) most <<= 16;
-    plain = most < 0x7f800000u;
+    s.plain = most < 0x7f800000u;
   }
   // max = 2^(E - 127) * 1.f: 128 * 2^-1 * 1.f is below 127.5 unless the first seven bits of f are all ones
-  eb = int(most >> 23) - 6 + ((most & 0x7f0000u) == 0x7f0000u);
-  plain = plain && eb <= TOP;
-  uint32_t q[kA8Each];
-  if (plain) {
-    eb = max(eb, 0);
-    const float inv = __uint_as_float(uint32_t(254 - eb) << 23);
-#pragma unroll
-    for (int i = 0; i < kA8Each; ++i) q[i] = __float_as_uint(fmaf(a8_at<T>(r, i), inv, 12582912.f));
-  } else {
+  s.eb = int(most >> 23) - 6 + ((most & 0x7f0000u) == 0x7f0000u);
+  s.plain = s.plain && s.eb <= TOP;
+  if (!s.plain) {
     uint32_t fin = 0;                                            // the largest finite magnitude
 #pragma unroll
     for (int i = 0; i < kA8Each; ++i) {
@@ -180,19 +174,28 @@ __device__ __forceinline__ uint4 a8_encode(const A8Raw<T>& r, int& eb) {
       fin = max(fin, a < 0x7f800000u ? a : 0u);
     }
     fin = max(fin, __shfl_xor_sync(3u << (threadIdx.x & 30), fin, 1));      // both lanes of a block come here
-    eb = min(max(int(fin >> 23) - 6 + ((fin & 0x7f0000u) == 0x7f0000u), 0), TOP);
-    const float inv = __uint_as_float(uint32_t(254 - eb) << 23);
-#pragma unroll
-    for (int i = 0; i < kA8Each; ++i) {
-      const float v = a8_at<T>(r, i);
-      q[i] = uint32_t((__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? min(max(__float2int_rn(v * inv), -127), 127) : -128);
-    }
+    s.eb = min(int(fin >> 23) - 6 + ((fin & 0x7f0000u) == 0x7f0000u), TOP);
   }
+  s.eb = max(s.eb, 0);
+  s.inv = __uint_as_float(uint32_t(254 - s.eb) << 23);
+  return s;
+}
+// Four values as bytes. Plain ones: q is the low byte of x 2^-e + 1.5 (2^23), one operation that rounds as rint does (with conversions, tests
+// for infinities and bounds for each value pack8 took 84 us of 16384 x 4096 + 16384 x 4096, bound by its instructions; now 46).
+template <bool PLAIN>
+__device__ __forceinline__ uint32_t a8_bytes(float a, float b, float c, float d, float inv) {
+  auto q = [&](float v) -> uint32_t {
+    if constexpr (PLAIN) return __float_as_uint(fmaf(v, inv, 12582912.f));
+    else return uint32_t((__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? min(max(__float2int_rn(v * inv), -127), 127) : -128);
+  };
+  return __byte_perm(__byte_perm(q(a), q(b), 0x0040), __byte_perm(q(c), q(d), 0x0040), 0x5410);
+}
+template <typename T, bool PLAIN>
+__device__ __forceinline__ uint4 a8_encode(const A8Raw<T>& r, float inv) {
   uint4 o;
-  uint32_t* w = &o.x;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+    (&o.x)[i] = a8_bytes<PLAIN>(a8_at<T>(r, 4 * i), a8_at<T>(r, 4 * i + 1), a8_at<T>(r, 4 * i + 2), a8_at<T>(r, 4 * i + 3), inv);
   return o;
 }
 
@@ -238,11 +241,10 @@ pack8_kernel(const T* __restrict__ x, long long x_rs, const T* __restrict__ add,
     a8_load<T, W>(add + max(at.row, 0ll) * add_rs + at.col, inside, a);
     a8_add<T>(v, a);
   }
-  int eb;
-  const uint4 r = a8_encode<T>(v, eb);
+  const A8Scale s = a8_scale<T>(v);
   if (at.row < 0) return;
-  *reinterpret_cast<uint4*>(q + (at.row * nb * 32 + at.col)) = r;
-  if ((threadIdx.x & 1) == 0) e[at.row * nb + at.blk] = uint8_t(eb);
+  *reinterpret_cast<uint4*>(q + (at.row * nb * 32 + at.col)) = s.plain ? a8_encode<T, true>(v, s.inv) : a8_encode<T, false>(v, s.inv);
+  if ((threadIdx.x & 1) == 0) e[at.row * nb + at.blk] = uint8_t(s.eb);
 }
 
 template <typename T, int W>
@@ -262,6 +264,25 @@ unpack8_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ e, T* 
 template <typename T> __device__ __forceinline__ float a8_sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 template <> __device__ __forceinline__ float a8_sigmoid<float>(float g) { return 1.f / (1.f + expf(-g)); }
 
+// Four columns at a time from here on: what a value needs is unpacked once and nothing of sixteen values but the operands and results is held.
+template <typename T, bool PLAIN>
+__device__ __forceinline__ void swiglu8_row(const A8Raw<T>& g, const A8Raw<T>& u, float gi, float ui, A8Raw<T>& o, uint4& gq, uint4& uq) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a[4], b[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = a8_at<T>(g, 4 * i + j);
+      b[j] = a8_at<T>(u, 4 * i + j);
+      y[j] = a[j] * a8_sigmoid<T>(a[j]) * b[j];
+    }
+    a8_set<T>(o, 2 * i, y[0], y[1]);
+    a8_set<T>(o, 2 * i + 1, y[2], y[3]);
+    (&gq.x)[i] = a8_bytes<PLAIN>(a[0], a[1], a[2], a[3], gi);
+    (&uq.x)[i] = a8_bytes<PLAIN>(b[0], b[1], b[2], b[3], ui);
+  }
+}
+
 template <typename T, int W>
 __global__ void __launch_bounds__(kA8Threads)
 swiglu8_fwd_kernel(const T* __restrict__ gu, long long rs, T* __restrict__ y, uint8_t* __restrict__ q, uint8_t* __restrict__ e, unsigned n,
@@ -272,22 +293,18 @@ swiglu8_fwd_kernel(const T* __restrict__ gu, long long rs, T* __restrict__ y, ui
   const T* row = gu + max(at.row, 0ll) * rs + at.col;
   a8_load<T, W>(row, inside, g);
   a8_load<T, W>(row + F, inside, u);
-#pragma unroll
-  for (int i = 0; i < kA8Each / 2; ++i) {
-    const float g0 = a8_at<T>(g, 2 * i), g1 = a8_at<T>(g, 2 * i + 1);
-    a8_set<T>(o, i, g0 * a8_sigmoid<T>(g0) * a8_at<T>(u, 2 * i), g1 * a8_sigmoid<T>(g1) * a8_at<T>(u, 2 * i + 1));
-  }
+  uint4 gq, uq;
+  const A8Scale gs = a8_scale<T>(g), us = a8_scale<T>(u);
+  if (gs.plain && us.plain) swiglu8_row<T, true>(g, u, gs.inv, us.inv, o, gq, uq);
+  else swiglu8_row<T, false>(g, u, gs.inv, us.inv, o, gq, uq);
   if (inside > 0) a8_store<T, W>(y + at.row * F + at.col, inside, o);
-  if (q == nullptr) return;                                        // nobody asks for a gradient
-  int ge, ue;
-  const uint4 gq = a8_encode<T>(g, ge), uq = a8_encode<T>(u, ue);
-  if (at.row < 0) return;
+  if (q == nullptr || at.row < 0) return;                          // nobody asks for a gradient
   uint8_t* qr = q + (at.row * 2 * nb * 32 + at.col);
   *reinterpret_cast<uint4*>(qr) = gq;
   *reinterpret_cast<uint4*>(qr + nb * 32) = uq;
   if ((threadIdx.x & 1) == 0) {
-    e[at.row * 2 * nb + at.blk] = uint8_t(ge);
-    e[at.row * 2 * nb + nb + at.blk] = uint8_t(ue);
+    e[at.row * 2 * nb + at.blk] = uint8_t(gs.eb);
+    e[at.row * 2 * nb + nb + at.blk] = uint8_t(us.eb);
   }
 }
 

@@ -127,6 +127,7 @@ embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint
 
 // n 16-byte zeros, then the last `rest` bytes. Stands beside the sort: it waits for it only at its end, so that what follows finds both done.
 __global__ void __launch_bounds__(256) embed_fill_kernel(uint4* __restrict__ out, long long n, int rest) {
+  pdl_launch_dependents();
   const long long step = (long long)gridDim.x * 256;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += step) out[i] = make_uint4(0, 0, 0, 0);
   if (blockIdx.x == 0 && threadIdx.x < rest) reinterpret_cast<uint8_t*>(out + n)[threadIdx.x] = 0;
@@ -154,6 +155,8 @@ template <typename TI, typename TO, int N>
 __global__ void __launch_bounds__(256)
 embed_sum_kernel(const uint2* __restrict__ pairs, const TI* __restrict__ dy, long long rs, TO* __restrict__ out, float* __restrict__ part, int T,
                  int V, int D, int L, float scale) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int tile = blockIdx.x, col = (blockIdx.y * blockDim.x + threadIdx.x) * N;
   const int lo = tile * L, hi = min(T, lo + L);
   if (col >= D || pairs[lo].x >= uint32_t(V)) return;
@@ -201,9 +204,10 @@ embed_sum_kernel(const uint2* __restrict__ pairs, const TI* __restrict__ dy, lon
   done(token == behind);
 }
 
-template <typename TO>
+template <typename TO, int N>
 __global__ void __launch_bounds__(256)
 embed_join_kernel(const uint2* __restrict__ pairs, TO* __restrict__ out, const float* __restrict__ part, int T, int V, int D, int L, float scale) {
+  pdl_wait();
   const int tile = blockIdx.x, tiles = gridDim.x, lo = tile * L, hi = lo + L;
   if (hi >= T) return;
   const uint32_t token = pairs[hi].x;
@@ -214,13 +218,25 @@ embed_join_kernel(const uint2* __restrict__ pairs, TO* __restrict__ out, const f
     n = __syncthreads_count(at < tiles && pairs[at * L].x == token);
     more += n;
   }
-  for (int col = blockIdx.y * blockDim.x + threadIdx.x; col < D; col += gridDim.y * blockDim.x) {
-    float acc = part[((long long)tile * 2 + 1) * D + col];
-    const float* p = part + (long long)(tile + 1) * 2 * D + col;
+  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  if (col >= D) return;
+  float acc[N];
+  const float* p = part + ((long long)tile * 2 + 1) * D + col;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = p[i];
+  p += D;                               // the next tile's first
 #pragma unroll 8
-    for (int j = 0; j < more; ++j) acc += p[(long long)j * 2 * D];
-    out[(long long)token * D + col] = from_f32<TO>(acc * scale);
+  for (int j = 0; j < more; ++j, p += 2ll * D) {
+    if constexpr (N == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
+    } else {
+      acc[0] += p[0];
+    }
   }
+  TO* o = out + (long long)token * D + col;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = from_f32<TO>(acc[i] * scale);
 }
 
 static int es_tile(long long T) {       // pairs of a CTA: 32, and more from 2^15 tokens on, so that partial sums stay a small part of the work
@@ -243,11 +259,24 @@ B200_API long long b200_embedding_grad_workspace(long long T, int D) {
   return 2 * ((T * 8 + 15) / 16 * 16) + tiles * 2 * D * 4;
 }
 
+// A launch that may begin while the one before ends: each of these kernels waits for that one before it reads or writes (embed_fill, which has nothing to
+// wait for, at its end).
+template <typename... K, typename... A>
+static cudaError_t es_next(cudaStream_t st, dim3 grid, int threads, void (*kernel)(K...), A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+}
+
 template <typename TI, typename TO, int N>
-static void es_sum(const uint2* a, const void* dy, long long rs, void* out, float* part, int T, int V, int D, int L, float scale, cudaStream_t st) {
+static cudaError_t es_sum(const uint2* a, const void* dy, long long rs, void* out, float* part, int T, int V, int D, int L, float scale, cudaStream_t st) {
   const int lanes = (D + N - 1) / N, threads = lanes >= 128 ? 128 : (lanes + 31) / 32 * 32;
   const dim3 grid((T + L - 1) / L, (lanes + threads - 1) / threads);
-  embed_sum_kernel<TI, TO, N><<<grid, threads, 0, st>>>(a, (const TI*)dy, rs, (TO*)out, part, T, V, D, L, scale);
+  return es_next(st, grid, threads, embed_sum_kernel<TI, TO, N>, a, (const TI*)dy, rs, (TO*)out, part, T, V, D, L, scale);
 }
 
 B200_API int b200_embedding_grad(const long long* ids, const void* dy, long long rs, void* out, long long T, int V, int D, float scale,
@@ -269,21 +298,17 @@ B200_API int b200_embedding_grad(const long long* ids, const void* dy, long long
     B200_LAUNCH_CHECK();
   }
   {
-    cudaLaunchConfig_t cfg = {};
     long long grid = (n16 + 255) / 256;
     if (grid > kNumSMs * 8) grid = kNumSMs * 8;
-    cfg.gridDim = dim3(unsigned(grid < 1 ? 1 : grid)); cfg.blockDim = dim3(256); cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = T > 0 ? 1 : 0;
-    B200_CHECK(cudaLaunchKernelEx(&cfg, embed_fill_kernel, (uint4*)out, n16, int(bytes - n16 * 16)));
+    if (grid < 1) grid = 1;
+    if (T > 0) B200_CHECK(es_next(st, dim3(unsigned(grid)), 256, embed_fill_kernel, (uint4*)out, n16, int(bytes - n16 * 16)));
+    else embed_fill_kernel<<<unsigned(grid), 256, 0, st>>>((uint4*)out, n16, int(bytes - n16 * 16));
   }
   if (T == 0) return 0;
   const int L = es_tile(T);
   const int V16 = 16 / es;
   const bool vec = D % V16 == 0 && (rs * es) % 16 == 0 && (uintptr_t)dy % 16 == 0;
-#define ES_SUM(TI, TO) vec ? es_sum<TI, TO, 16 / sizeof(TI)>(a, dy, rs, out, part, int(T), V, D, L, scale, st) : es_sum<TI, TO, 1>(a, dy, rs, out, part, int(T), V, D, L, scale, st)
+#define ES_SUM(TI, TO) B200_CHECK((vec ? es_sum<TI, TO, 16 / sizeof(TI)>(a, dy, rs, out, part, int(T), V, D, L, scale, st) : es_sum<TI, TO, 1>(a, dy, rs, out, part, int(T), V, D, L, scale, st)))
   if (dtype == B200_DT_FP32) ES_SUM(float, float);
   else if (dtype == B200_DT_BF16 && out_dtype == B200_DT_BF16) ES_SUM(__nv_bfloat16, __nv_bfloat16);
   else if (dtype == B200_DT_BF16) ES_SUM(__nv_bfloat16, float);
@@ -291,10 +316,11 @@ B200_API int b200_embedding_grad(const long long* ids, const void* dy, long long
   else if (dtype == B200_DT_FP16) ES_SUM(__half, float);
   else return B200_ERR_UNSUPPORTED;
   B200_LAUNCH_CHECK();
-  const dim3 grid(unsigned((T + L - 1) / L), unsigned((D + 255) / 256));
-  if (out_dtype == B200_DT_FP32) embed_join_kernel<float><<<grid, 256, 0, st>>>(a, (float*)out, part, int(T), V, D, L, scale);
-  else if (out_dtype == B200_DT_BF16) embed_join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, (__nv_bfloat16*)out, part, int(T), V, D, L, scale);
-  else embed_join_kernel<__half><<<grid, 256, 0, st>>>(a, (__half*)out, part, int(T), V, D, L, scale);
-  B200_LAUNCH_CHECK();
+  const int n = D % 4 == 0 ? 4 : 1, threads = D / n >= 256 ? 256 : (D / n + 31) / 32 * 32;
+  const dim3 grid(unsigned((T + L - 1) / L), unsigned((D / n + threads - 1) / threads));
+#define ES_JOIN(TO) es_next(st, grid, threads, n == 4 ? embed_join_kernel<TO, 4> : embed_join_kernel<TO, 1>, (const uint2*)a, (TO*)out, (const float*)part, int(T), V, D, L, scale)
+  if (out_dtype == B200_DT_FP32) B200_CHECK(ES_JOIN(float));
+  else if (out_dtype == B200_DT_BF16) B200_CHECK(ES_JOIN(__nv_bfloat16));
+  else B200_CHECK(ES_JOIN(__half));
   return 0;
 }

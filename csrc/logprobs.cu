@@ -63,6 +63,27 @@ __device__ __forceinline__ float lp_values(const uint4 (&raw)[G], float (&v)[G *
   }
 }
 
+// How many of a group's values are above lt: 16-bit types two to an instruction, whose counts of ones a group's sixteen pairs do not exhaust.
+template <typename T, int G>
+__device__ __forceinline__ int lp_above(const uint4 (&raw)[G], const float (&v)[G * LpVec<T>::N], float lt) {
+  int n = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < G * 4; ++j) n += v[j] > lt;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 one, sum;
+    one.x = one.y = from_f32<T>(lt);
+    sum.x = sum.y = from_f32<T>(0.f);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = __hadd2(sum, __hgt2(*reinterpret_cast<const T2*>(&(&raw[g].x)[j]), one));
+    n = int(to_f32<T>(sum.x) + to_f32<T>(sum.y));
+  }
+  return n;
+}
+
 // How a CTA walks over p[0 .. n): single values up to the first multiple of 16 bytes, vectors i = thread, thread + threads .. in groups of kLpGroup
 // and then one by one, single values behind the last.
 constexpr int kLpGroup = 4;
@@ -247,10 +268,7 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     float v[G * N];
     const float m = lp_values<T, G>(raw, v);
     lp_join<ENT>(a, v, m, c);
-    if (rank && m > lt) {
-#pragma unroll
-      for (int j = 0; j < G * N; ++j) above += v[j] > lt;
-    }
+    if (rank && m > lt) above += lp_above<T, G>(raw, v, lt);
     if (m > most || group < 0) { most = m; group = i; }
   };
   if (threadIdx.x < at.head) single(threadIdx.x);
@@ -294,20 +312,25 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     __syncthreads();
     cluster_sync_all();
     if (part == 0) {
-      for (uint32_t x = 1; x < parts; ++x) {
-        const unsigned long long *s0 = reinterpret_cast<const unsigned long long*>(&sh.sums), lo = lp_remote(s0, x), hi = lp_remote(s0 + 1, x);
-        a = lp_both<ENT>(a, {__uint_as_float(uint32_t(lo)), __uint_as_float(uint32_t(lo >> 32)), __uint_as_float(uint32_t(hi))}, c);
-        above += int(uint32_t(hi >> 32));
+      LpSum b{-INFINITY, 0.f, 0.f};
+      int more = 0;
+      if (uint32_t(lane) < parts) {
+        const unsigned long long *s0 = reinterpret_cast<const unsigned long long*>(&sh.sums), lo = lp_remote(s0, lane), hi = lp_remote(s0 + 1, lane);
+        b = {__uint_as_float(uint32_t(lo)), __uint_as_float(uint32_t(lo >> 32)), __uint_as_float(uint32_t(hi))};
+        more = int(uint32_t(hi >> 32));
       }
+#pragma unroll
+      for (int o = kLpMaxCluster / 2; o > 0; o >>= 1)
+        b = lp_both<ENT>(b, {__shfl_xor_sync(0xffffffffu, b.m, o), __shfl_xor_sync(0xffffffffu, b.s, o), __shfl_xor_sync(0xffffffffu, b.u, o)}, c);
+      a = {__shfl_sync(0xffffffffu, b.m, 0), __shfl_sync(0xffffffffu, b.s, 0), __shfl_sync(0xffffffffu, b.u, 0)};
+      above = __reduce_add_sync(0xffffffffu, more);
       if (top > 0) {
-        int all = 0;                                                     // slices have top alternatives each, the last one maybe fewer
-        for (uint32_t x = 0; x < parts; ++x) {
-          const int kx = min(top, max(0, min(slice, V - int(x) * slice)));
-          if (int(threadIdx.x) < kx) sh.list[all + threadIdx.x] = lp_remote(sh.best + threadIdx.x, x);
-          all += kx;
+        if (int(threadIdx.x) < int(parts) * top) {                       // a slice has top alternatives, a short last one fewer: keys of zero, below all
+          const int x = threadIdx.x / top, j = threadIdx.x - x * top;
+          sh.list[threadIdx.x] = j < min(top, max(0, min(slice, V - x * slice))) ? lp_remote(sh.best + j, x) : 0;
         }
         __syncthreads();
-        lp_sort(sh.list, all, top, sh.best);
+        lp_sort(sh.list, parts * top, top, sh.best);
       }
     }
   }
@@ -388,26 +411,29 @@ lp_rows_grad_kernel(const T* __restrict__ logits, long long rs, int V, int slice
 }
 
 // ---- logits that are not stored ----
-// part [n][rows] = (m, s, u) of n parts of each row, lt [rows] its token's logit. 32 rows a CTA, 8 threads a row.
+// part [n][rows] = (m, s, u) of n parts of each row, lt [rows] its token's logit. 8 rows a CTA, 32 threads a row (32 rows a CTA and 8 threads a row took
+// 41 us of 2048 x 594 parts, the loads' latency).
 __global__ void __launch_bounds__(256)
 lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, const long long* __restrict__ tokens, const float* __restrict__ lt, float inv_t,
                  float* __restrict__ lp, float* __restrict__ ent, float4* __restrict__ stats) {
-  __shared__ float red[3][8][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const long long row = blockIdx.x * 32ll + lane;
+  __shared__ float4 red[32][8];
+  const int r = threadIdx.x & 7, slice = threadIdx.x >> 3;
+  const long long row = blockIdx.x * 8ll + r;
   const float c = inv_t * kLog2e;
   LpSum a{-INFINITY, 0.f, 0.f};
   if (row < rows) {
-#pragma unroll 8
-    for (int i = w; i < n; i += 8) {
-      const float4 x = __ldg(part + i * rows + row);
-      a = lp_both<true>(a, {x.x, x.y, x.z}, c);
+    for (int i0 = slice; i0 < n; i0 += 32 * 8) {
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = i0 + j * 32 < n ? __ldg(part + (long long)(i0 + j * 32) * rows + row) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a = lp_both<true>(a, {x[j].x, x[j].y, x[j].z}, c);
     }
   }
-  red[0][w][lane] = a.m; red[1][w][lane] = a.s; red[2][w][lane] = a.u;
+  red[slice][r] = make_float4(a.m, a.s, a.u, 0.f);
   __syncthreads();
-  if (w || row >= rows) return;
-  for (int i = 1; i < 8; ++i) a = lp_both<true>(a, {red[0][i][lane], red[1][i][lane], red[2][i][lane]}, c);
+  if (threadIdx.x >= 8 || row >= rows) return;
+  for (int i = 1; i < 32; ++i) a = lp_both<true>(a, {red[i][r].x, red[i][r].y, red[i][r].z}, c);
   const long long t = tokens ? tokens[row] : 0;
   const bool skip = t < 0 || t >= V;
   const float ls = logf(a.s), H = ls - kLn2 * a.u / a.s;
@@ -516,7 +542,7 @@ B200_API int b200_logprob_finish(const void* part, int parts, long long rows, in
                                  void* stats, void* stream) {
   if (lp_bad(rows, V) || parts < 1) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
-  lp_finish_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, (cudaStream_t)stream>>>((const float4*)part, parts, rows, V, tokens, lt, inv_t, lp, ent, (float4*)stats);
+  lp_finish_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, (cudaStream_t)stream>>>((const float4*)part, parts, rows, V, tokens, lt, inv_t, lp, ent, (float4*)stats);
   B200_LAUNCH_CHECK();
   return 0;
 }

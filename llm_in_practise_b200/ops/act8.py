@@ -14,13 +14,16 @@ import ctypes
 from typing import Callable, NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nv
 
 vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 BLOCK = 32
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_SWIGLU_FWD = [vp, i64, vp, vp, vp, i64, i32, i32, vp]
+_SWIGLU_BWD = [vp, vp, vp, vp, i64, i32, i32, vp]
+_PACK = [vp, i64, vp, i64, vp, vp, i64, i32, i32, vp]
+_UNPACK = [vp, vp, vp, i64, i32, i32, vp]
 
 
 class Packed8(NamedTuple):
@@ -47,22 +50,24 @@ def _stride(x):
 
 def _room(x, rows, D, parts=1):
     nb = -(-D // BLOCK)
-    return torch.empty(rows, parts * nb * BLOCK, dtype=torch.int8, device=x.device), torch.empty(rows, parts * nb, dtype=torch.uint8, device=x.device)
+    return x.new_empty((rows, parts * nb * BLOCK), dtype=torch.int8), x.new_empty((rows, parts * nb), dtype=torch.uint8)
 
 
 def pack8(x: torch.Tensor, add: Optional[torch.Tensor] = None) -> Packed8:
     """``x`` [..., columns], or ``x + add`` rounded to their type, in 8 bits. No gradient."""
     if add is not None and (add.shape != x.shape or add.dtype != x.dtype or add.device != x.device):
         raise ValueError("pack8: add must be like x in shape, type and device")
-    shape, x = tuple(x.shape), _rows_of("pack8", x.detach())
-    add = None if add is None else _rows_of("pack8", add.detach())
+    shape, x = tuple(x.shape), _rows_of("pack8", x)
+    if add is not None:
+        add = _rows_of("pack8", add)
     rows, D = x.shape
     if not nv.use_native(x):
-        q, e = _pack_torch(x if add is None else x + add)
+        with torch.no_grad():
+            q, e = _pack_torch(x if add is None else x + add)
         return Packed8(q, e, shape, x.dtype)
     q, e = _room(x, rows, D)
     if rows:
-        fn = nv.proto("b200_pack8", [vp, i64, vp, i64, vp, vp, i64, i32, i32, vp])
+        fn = nv.proto("b200_pack8", _PACK)
         nv.check(nv.call_on(x.device, fn, x.data_ptr(), _stride(x), nv.ptr(add), 0 if add is None else _stride(add), q.data_ptr(), e.data_ptr(), rows, D,
                             nv.dtype_code(x.dtype)), "pack8")
         nv.count_launch()
@@ -82,7 +87,7 @@ def unpack8(p: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return _unpack_torch(p.q, p.e, D).to(dtype).view(p.shape)
     y = torch.empty(p.shape, dtype=dtype, device=p.q.device)
     if rows:
-        fn = nv.proto("b200_unpack8", [vp, vp, vp, i64, i32, i32, vp])
+        fn = nv.proto("b200_unpack8", _UNPACK)
         nv.check(nv.call_on(y.device, fn, p.q.data_ptr(), p.e.data_ptr(), y.data_ptr(), rows, D, nv.dtype_code(dtype)), "unpack8")
         nv.count_launch()
     return y
@@ -112,54 +117,75 @@ def _unpack_torch(q, e, D):
     return y.flatten(1)[:, :D]
 
 
+def _first_order_only(what):
+    """In a backward pass: gradients are being recorded for a second one only where it was asked for."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative (create_graph)")
+
+
+def _swiglu8(gate_up, keep):
+    """(y, q, e) of gate_up [..., 2F]; q and e None without ``keep``."""
+    gu = _rows_of("swiglu8", gate_up)
+    rows, F = gu.shape[0], gu.shape[1] // 2
+    shape = (rows, F) if gate_up.dim() == 2 else (*gate_up.shape[:-1], F)
+    q = e = None
+    if not nv.use_native(gu):
+        g, u = gu[:, :F].float(), gu[:, F:].float()
+        y = (g * torch.sigmoid(g) * u).to(gu.dtype).view(shape)
+        if keep:
+            (gq, ge), (uq, ue) = _pack_torch(gu[:, :F]), _pack_torch(gu[:, F:])
+            q, e = torch.cat([gq, uq], 1), torch.cat([ge, ue], 1)
+        return y, q, e
+    y = gu.new_empty(shape)
+    if keep:
+        q, e = _room(gu, rows, F, 2)
+    if rows:
+        rc = nv.call_on(gu.device, nv.proto("b200_swiglu8_fwd", _SWIGLU_FWD), gu.data_ptr(), _stride(gu), y.data_ptr(), nv.ptr(q), nv.ptr(e), rows, F,
+                        nv.dtype_code(gu.dtype))
+        if rc:
+            nv.check(rc, "swiglu8_fwd")
+        nv.count_launch()
+    return y, q, e
+
+
 class _SwiGLU8Fn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gu, keep):
-        rows, F = gu.shape[0], gu.shape[1] // 2
-        q = e = None
-        if not nv.use_native(gu):
-            g, u = gu[:, :F].float(), gu[:, F:].float()
-            y = (g * torch.sigmoid(g) * u).to(gu.dtype)
-            if keep:
-                (gq, ge), (uq, ue) = _pack_torch(gu[:, :F]), _pack_torch(gu[:, F:])
-                q, e = torch.cat([gq, uq], 1), torch.cat([ge, ue], 1)
-        else:
-            y = torch.empty(rows, F, dtype=gu.dtype, device=gu.device)
-            if keep:
-                q, e = _room(gu, rows, F, 2)
-            if rows:
-                fn = nv.proto("b200_swiglu8_fwd", [vp, i64, vp, vp, vp, i64, i32, i32, vp])
-                nv.check(nv.call_on(gu.device, fn, gu.data_ptr(), _stride(gu), y.data_ptr(), nv.ptr(q), nv.ptr(e), rows, F, nv.dtype_code(gu.dtype)), "swiglu8_fwd")
-                nv.count_launch()
+    def forward(ctx, gate_up):
+        y, q, e = _swiglu8(gate_up, True)
         ctx.save_for_backward(q, e)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _first_order_only("swiglu8")
         q, e = ctx.saved_tensors
-        rows, F = dy.shape
+        shape, rows = dy.shape, q.shape[0]
+        F = shape[-1]
         if not nv.use_native(dy):
             n = q.shape[1] // 2
-            g, u, d = _unpack_torch(q[:, :n], e[:, :n // BLOCK], F), _unpack_torch(q[:, n:], e[:, n // BLOCK:], F), dy.float()
+            g, u, d = _unpack_torch(q[:, :n], e[:, :n // BLOCK], F), _unpack_torch(q[:, n:], e[:, n // BLOCK:], F), dy.reshape(rows, F).float()
             s = torch.sigmoid(g)
-            return torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], 1).to(dy.dtype), None
+            return torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], 1).to(dy.dtype).view(*shape[:-1], 2 * F)
         dy = dy.contiguous()
-        dgu = torch.empty(rows, 2 * F, dtype=dy.dtype, device=dy.device)
+        dgu = dy.new_empty((*shape[:-1], 2 * F))
         if rows:
-            fn = nv.proto("b200_swiglu8_bwd", [vp, vp, vp, vp, i64, i32, i32, vp])
-            nv.check(nv.call_on(dy.device, fn, dy.data_ptr(), q.data_ptr(), e.data_ptr(), dgu.data_ptr(), rows, F, nv.dtype_code(dy.dtype)), "swiglu8_bwd")
+            rc = nv.call_on(dy.device, nv.proto("b200_swiglu8_bwd", _SWIGLU_BWD), dy.data_ptr(), q.data_ptr(), e.data_ptr(), dgu.data_ptr(), rows, F,
+                            nv.dtype_code(dy.dtype))
+            if rc:
+                nv.check(rc, "swiglu8_bwd")
             nv.count_launch()
-        return dgu, None
+        return dgu
 
 
 def swiglu8(gate_up: torch.Tensor) -> torch.Tensor:
     """``silu(gate) * up`` for ``gate_up`` = [..., 2F] (gate in the first F columns, any F), rounded once. Where a gradient is asked for, gate and up are kept
     in 8 bits, and it is taken there."""
-    if gate_up.dim() < 1 or gate_up.shape[-1] < 2 or gate_up.shape[-1] % 2:
-        raise ValueError(f"swiglu8: needs [..., 2F], not {list(gate_up.shape)}")
-    x = _rows_of("swiglu8", gate_up)
-    return _SwiGLU8Fn.apply(x, torch.is_grad_enabled() and x.requires_grad).view(*gate_up.shape[:-1], gate_up.shape[-1] // 2)
+    n = gate_up.shape[-1] if gate_up.dim() else 0
+    if n < 2 or n % 2 or gate_up.dtype not in _TYPES:
+        raise ValueError(f"swiglu8: needs [..., 2F] in fp32, bf16 or fp16, not {gate_up.dtype} {list(gate_up.shape)}")
+    if gate_up.requires_grad and torch.is_grad_enabled():
+        return _SwiGLU8Fn.apply(gate_up)
+    return _swiglu8(gate_up, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------
@@ -179,8 +205,8 @@ class _Checkpoint8Fn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
+        _first_order_only("checkpoint8")
         x = unpack8(Packed8(*ctx.saved_tensors, *ctx.kept)).requires_grad_(True)
         now = _draws(x)
         try:                                             # dropout masks of the layer are those of its forward

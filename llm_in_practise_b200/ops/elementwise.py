@@ -287,6 +287,10 @@ def dropout(x: torch.Tensor, p: float, training: bool = True, seed: Optional[int
 # ------------------------------------------------------------------------------------------------
 # embedding
 # ------------------------------------------------------------------------------------------------
+_EMBEDDING_GRAD = [vp, vp, i64, vp, i64, i32, i32, f32, i64, i32, i32, vp, vp]
+_embedding_work = {}                 # bytes of a workspace by tokens and columns
+
+
 def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
                    dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """[rows, D] = ``scale * sum of dout[t] over the t with ids[t] = row``, in the order of t: the gradient of ``embedding``'s table. ``ids`` int64 [...], ``dout``
@@ -304,13 +308,17 @@ def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: floa
         return out.index_add_(0, flat[keep], d2[keep].float()).mul_(scale).to(dtype)
     if D > 1 and d2.stride(1) != 1:
         d2 = d2.contiguous()
-    out = torch.empty(rows, D, dtype=dtype, device=dout.device)
-    size = nv.lib().b200_embedding_grad_workspace
-    size.argtypes, size.restype = [i64, i32], i64
-    work = torch.empty(size(T, D), dtype=torch.uint8, device=dout.device)
-    fn = nv.proto("b200_embedding_grad", [vp, vp, i64, vp, i64, i32, i32, f32, i64, i32, i32, vp, vp])
-    nv.check(nv.call_on(dout.device, fn, flat.data_ptr(), d2.data_ptr(), d2.stride(0) if T > 1 else D, out.data_ptr(), T, rows, D, float(scale),
-                        -1 if padding_idx is None else padding_idx, nv.dtype_code(dout.dtype), nv.dtype_code(dtype), work.data_ptr()), "embedding_grad")
+    out = d2.new_empty((rows, D), dtype=dtype)
+    size = _embedding_work.get((T, D))
+    if size is None:
+        fn = nv.lib().b200_embedding_grad_workspace
+        fn.argtypes, fn.restype = [i64, i32], i64
+        size = _embedding_work[T, D] = fn(T, D)
+    work = d2.new_empty((size,), dtype=torch.uint8)
+    rc = nv.call_on(dout.device, nv.proto("b200_embedding_grad", _EMBEDDING_GRAD), flat.data_ptr(), d2.data_ptr(), d2.stride(0) if T > 1 else D, out.data_ptr(), T,
+                    rows, D, float(scale), -1 if padding_idx is None else padding_idx, nv.dtype_code(dout.dtype), nv.dtype_code(dtype), work.data_ptr())
+    if rc:
+        nv.check(rc, "embedding_grad")
     nv.count_launch(4 if T else 1)
     return out
 

@@ -16,7 +16,6 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nv
 from .gemm import gemm
@@ -36,9 +35,15 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[torch.Tensor] = None
 
 
-def _check(what, tokens, shape, device, temperature):
-    if tokens is not None and (tokens.dtype != torch.int64 or tokens.shape != shape or tokens.device != device):
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _check(what, tokens, shape, device):
+    if tokens.dtype is not torch.int64 or tokens.shape != shape or tokens.device != device:
         raise ValueError(f"{what}: tokens must be int64 {list(shape)} on {device}")
+
+
+def _check_temperature(what, temperature):
     if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
         raise ValueError(f"{what}: temperature must be from 2^-60 to 2^60, not {temperature}")
 
@@ -49,20 +54,32 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
-def _rows(logits, tokens, temperature, top, entropy, rank, save):
-    """(lp, H, rank, ids, lps, stats) of logits [B, V]; ``stats`` fp32 [B, 4] is what the gradient needs."""
-    B, V = logits.shape
+def _rows(logits, tokens, temperature, top, entropy, rank, save, shape=None):
+    """(lp, H, rank, ids, lps, stats) of logits [B, V], with leading dimensions ``shape`` (None: [B]); ``stats`` fp32 [B, 4] is what the gradient needs."""
     if not nv.use_native(logits):
-        return _rows_torch(logits, tokens, temperature, top, entropy, rank)
-    def new(*size, dtype=torch.float32):
-        return logits.new_empty(size, dtype=dtype)
-    lp, H, r = new(B) if tokens is not None else None, new(B) if entropy else None, new(B, dtype=torch.int64) if rank else None
-    ids, lps = (new(B, top, dtype=torch.int64), new(B, top)) if top else (None, None)
-    stats = new(B, 4) if save else None
+        got = _rows_torch(logits, tokens, temperature, top, entropy, rank)
+        if shape is None:
+            return got
+        return (*(t if t is None else t.view(shape) for t in got[:3]), *(t if t is None else t.view(*shape, top) for t in got[3:5]), got[5])
+    B, V = logits.shape
+    new, one = logits.new_empty, (B,) if shape is None else shape
+    lp = H = r = ids = lps = stats = None
+    if tokens is not None:
+        lp = new(one, dtype=torch.float32)
+    if entropy:
+        H = new(one, dtype=torch.float32)
+    if rank:
+        r = new(one, dtype=torch.int64)
+    if top:
+        ids, lps = new((*one, top), dtype=torch.int64), new((*one, top), dtype=torch.float32)
+    if save:
+        stats = new((B, 4), dtype=torch.float32)
     if B:
-        fn = nv.proto("b200_token_logprobs", _ROWS_ARGS)
-        nv.check(nv.call_on(logits.device, fn, logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, nv.ptr(tokens), 1.0 / temperature, top, nv.ptr(lp),
-                            nv.ptr(H), nv.ptr(r), nv.ptr(ids), nv.ptr(lps), nv.ptr(stats), nv.dtype_code(logits.dtype)), "token_logprobs")
+        ptr = nv.ptr
+        rc = nv.call_on(logits.device, nv.proto("b200_token_logprobs", _ROWS_ARGS), logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, ptr(tokens),
+                        1.0 / temperature, top, ptr(lp), ptr(H), ptr(r), ptr(ids), ptr(lps), ptr(stats), nv.dtype_code(logits.dtype))
+        if rc:
+            nv.check(rc, "token_logprobs")
         nv.count_launch()
     return lp, H, r, ids, lps, stats
 
@@ -127,24 +144,34 @@ def _grad_torch(l, tokens, temperature, stats, g, h, c0, vocab):
     return out / temperature
 
 
+def _first_order_only(what):
+    """In a backward pass: gradients are being recorded for a second one only where it was asked for."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no second derivative (create_graph)")
+
+
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature, top, entropy, rank):
-        lp, H, r, ids, lps, stats = _rows(logits, tokens, temperature, top, entropy, rank, True)
+        shape = logits.shape[:-1]
+        rows = _as_rows(logits)
+        lp, H, r, ids, lps, stats = _rows(rows, tokens, temperature, top, entropy, rank, True, None if len(shape) == 1 else shape)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (r, ids, lps) if t is not None))
+        if rank or top:
+            ctx.mark_non_differentiable(*(t for t in (r, ids, lps) if t is not None))
         return lp, H, r, ids, lps
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, h, *_):
+        _first_order_only("token_logprobs")
         if g is None and h is None:
             return (None,) * 6
         logits, tokens, stats = ctx.saved_tensors
-        g, h = (None if x is None else x.to(torch.float32).contiguous() for x in (g, h))
-        return (_rows_grad(logits, tokens, ctx.temperature, stats, g, h),) + (None,) * 5
+        g, h = (None if x is None else x.to(torch.float32).reshape(-1).contiguous() for x in (g, h))
+        d = _rows_grad(_as_rows(logits), tokens, ctx.temperature, stats, g, h)
+        return (d if logits.dim() == 2 else d.view(logits.shape)), None, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top: int = 0, entropy: bool = False, rank: bool = False,
@@ -152,24 +179,20 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """``logits`` [..., vocab] (fp32, bf16 or fp16; rows may be strided), ``tokens`` int64 [...] (None: no tokens are given, for entropies and
     alternatives alone). ``top``: how many alternatives, up to ``MAX_TOP``. Sums in 32 bits. A row of minus infinities alone, or with a NaN or plus infinity,
     gives NaN, as log_softmax does. Ranks and alternatives are those of the logits as they are given."""
-    if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    shape = logits.shape
+    if not shape or shape[-1] < 1 or logits.dtype not in _TYPES:
         raise ValueError("token_logprobs: logits must be [..., vocab] in fp32, bf16 or fp16")
-    _check("token_logprobs", tokens, logits.shape[:-1], logits.device, temperature)
-    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
-        raise ValueError(f"token_logprobs: top must be from 0 to {min(MAX_TOP, logits.shape[-1])}, not {top}")
-    if tokens is None and (rank or not (entropy or top)):
+    if tokens is not None:
+        _check("token_logprobs", tokens, shape[:-1], logits.device)
+        tokens = tokens if len(shape) == 2 and tokens.is_contiguous() else tokens.reshape(-1).contiguous()
+    elif rank or not (entropy or top):
         raise ValueError("token_logprobs: without tokens there are entropies and alternatives only")
-    shape, rows = logits.shape[:-1], _as_rows(logits)
-    flat = None if tokens is None else tokens.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        got = _TokenLogprobsFn.apply(rows, flat, temperature, top, entropy, rank)
-    else:
-        got = _rows(rows, flat, temperature, top, entropy, rank, False)[:5]
-    if len(shape) == 1:
-        return TokenLogprobs(*got)
-    lp, H, r, ids, lps = got
-    one, many = (lambda t: None if t is None else t.view(shape)), (lambda t: None if t is None else t.view(*shape, top))
-    return TokenLogprobs(one(lp), one(H), one(r), many(ids), many(lps))
+    _check_temperature("token_logprobs", temperature)
+    if not 0 <= top <= min(MAX_TOP, shape[-1]):
+        raise ValueError(f"token_logprobs: top must be from 0 to {min(MAX_TOP, shape[-1])}, not {top}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, tokens, temperature, top, entropy, rank))
+    return TokenLogprobs(*_rows(_as_rows(logits), tokens, temperature, top, entropy, rank, False, None if len(shape) == 2 else shape[:-1])[:5])
 
 
 # ------------------------------------------------------------------------------------------------
@@ -269,8 +292,8 @@ class _LinearLogprobsFn(torch.autograd.Function):
         return lp, H
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, h):
+        _first_order_only("linear_token_logprobs")
         if g is None and h is None:
             return (None,) * 5
         x, w, tokens, stats = ctx.saved_tensors
@@ -290,7 +313,9 @@ def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[tor
         raise TypeError(f"linear_token_logprobs: x and w must be bf16 or fp16, not {x.dtype}; token_logprobs takes logits of 32 bits")
     if nv.use_native(x) and (x.shape[-1] % 8 or w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16):
         raise ValueError("linear_token_logprobs: rows of w must be contiguous, start at multiples of 16 bytes and have a multiple of 8 values")
-    _check("linear_token_logprobs", tokens, x.shape[:-1], x.device, temperature)
+    if tokens is not None:
+        _check("linear_token_logprobs", tokens, x.shape[:-1], x.device)
+    _check_temperature("linear_token_logprobs", temperature)
     if tokens is None and not entropy:
         raise ValueError("linear_token_logprobs: without tokens there are entropies only")
     shape, rows = x.shape[:-1], _as_rows(x)
