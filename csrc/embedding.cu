@@ -239,8 +239,8 @@ embed_join_kernel(const uint2* __restrict__ pairs, TO* __restrict__ out, const f
   for (int i = 0; i < N; ++i) o[i] = from_f32<TO>(acc[i] * scale);
 }
 
-static int es_tile(long long T) {       // pairs of a CTA: 32, and more from 2^15 tokens on, so that partial sums stay a small part of the work
-  long long L = 32;
+static int es_tile(long long T) {       // pairs of a CTA: 8, and more from 8192 tokens on, so that partial sums stay a small part of the work
+  long long L = kSumAhead;
   while (L * 1024 < T) L *= 2;
   return int(L);
 }

@@ -20,15 +20,19 @@
 
 namespace b200 {
 
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32, kLpMaxTop = 32, kLpMaxCluster = 8;
+constexpr int kLpThreads = 256, kLpMaxTop = 32, kLpMaxCluster = 8;
 
-// What a CTA knows of its slice of a row, where the others of its cluster read it.
-struct LpShared {
-  float red[3][kLpWarps];
-  int redi[kLpWarps];
+// What a CTA of NT threads knows of its slice of a row, where the others of its cluster read it.
+template <int NT> struct LpSums {
+  float red[3][NT / 32];
+  int redi[NT / 32];
   float4 sums;                                   // m, s, u, logits above the token's
+};
+template <int NT> struct LpShared : LpSums<NT> {
+  static constexpr int kList = NT == 64 ? 512 : 1280, kSegments = NT == 64 ? 1 : 2048;
   unsigned long long best[kLpMaxTop];            // the slice's alternatives in order
-  unsigned long long list[1024];
+  unsigned long long list[kList];
+  float segment[kSegments];                      // the largest of each 32 vectors
   uint32_t group[64];
   int chosen[kLpMaxTop];
   unsigned long long bound;
@@ -37,39 +41,71 @@ struct LpShared {
 
 template <typename T> struct LpVec { static constexpr int N = 16 / sizeof(T); };
 
-// The values of G vectors, and the largest of them (NaN aside).
-template <typename T, int G>
-__device__ __forceinline__ float lp_values(const uint4 (&raw)[G], float (&v)[G * LpVec<T>::N]) {
+// Two values of a vector's word (one of 32 bits).
+template <typename T> __device__ __forceinline__ float2 lp_word(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// The largest of G vectors' values, from vector G0 on (NaN aside).
+template <typename T, int G0, int G, int ALL>
+__device__ __forceinline__ float lp_largest(const uint4 (&raw)[ALL]) {
   if constexpr (sizeof(T) == 4) {
     float m = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = G0; g < G0 + G; ++g)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m = fmaxf(m, v[g * 4 + j] = __uint_as_float((&raw[g].x)[j]));
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, __uint_as_float((&raw[g].x)[j]));
     return m;
   } else {
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    T2 m = *reinterpret_cast<const T2*>(&raw[0].x);
+    T2 m = *reinterpret_cast<const T2*>(&raw[G0].x);
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = G0; g < G0 + G; ++g)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const T2 p = *reinterpret_cast<const T2*>(&(&raw[g].x)[j]);
-        m = __hmax2(m, p);
-        v[(g * 4 + j) * 2] = to_f32<T>(p.x);
-        v[(g * 4 + j) * 2 + 1] = to_f32<T>(p.y);
-      }
+      for (int j = 0; j < 4; ++j) m = __hmax2(m, *reinterpret_cast<const T2*>(&(&raw[g].x)[j]));
     return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
+  }
+}
+// lp_join of G vectors, of which m is the largest value: unpacked two at a time as they are used, so that a thread holds the vectors and little else.
+template <typename T, bool ENT, int G>
+__device__ __forceinline__ void lp_join_vectors(LpSum& a, const uint4 (&raw)[G], float m, float c) {
+  if (m > a.m) {
+    const float x = (a.m - m) * c, f = lp_exp2(x);
+    if constexpr (ENT) a.u = f * (a.u + a.s * lp_factor(x));
+    a.s *= f;
+    a.m = m;
+  }
+  const float base = a.m == -INFINITY ? 0.f : a.m;
+  const unsigned long long nb = lp_pair(-base, -base), cc = lp_pair(c, c);
+  unsigned long long s = 0, u = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < (sizeof(T) == 4 ? 2 : 4); ++j) {
+      const float2 v = sizeof(T) == 4 ? make_float2(__uint_as_float((&raw[g].x)[2 * j]), __uint_as_float((&raw[g].x)[2 * j + 1])) : lp_word<T>((&raw[g].x)[j & 3]);
+      const unsigned long long x = lp_mul2(lp_add2(lp_pair(v.x, v.y), nb), cc);
+      const float2 xs = lp_split(x);
+      const unsigned long long e = lp_pair(lp_exp2(xs.x), lp_exp2(xs.y));
+      s = lp_add2(s, e);
+      if constexpr (ENT) u = lp_fma2(e, lp_pair(lp_factor(xs.x), lp_factor(xs.y)), u);
+    }
+  const float2 s2 = lp_split(s);
+  a.s += s2.x + s2.y;
+  if constexpr (ENT) {
+    const float2 u2 = lp_split(u);
+    a.u += u2.x + u2.y;
   }
 }
 
 // How many of a group's values are above lt: 16-bit types two to an instruction, whose counts of ones a group's sixteen pairs do not exhaust.
 template <typename T, int G>
-__device__ __forceinline__ int lp_above(const uint4 (&raw)[G], const float (&v)[G * LpVec<T>::N], float lt) {
+__device__ __forceinline__ int lp_above(const uint4 (&raw)[G], float lt) {
   int n = 0;
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < G * 4; ++j) n += v[j] > lt;
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) n += __uint_as_float((&raw[g].x)[j]) > lt;
   } else {
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     T2 one, sum;
@@ -84,16 +120,12 @@ __device__ __forceinline__ int lp_above(const uint4 (&raw)[G], const float (&v)[
   return n;
 }
 
-// How a CTA walks over p[0 .. n): single values up to the first multiple of 16 bytes, vectors i = thread, thread + threads .. in groups of kLpGroup
-// and then one by one, single values behind the last.
-constexpr int kLpGroup = 4;
+// How NT threads walk over p[0 .. n): single values up to the first multiple of 16 bytes, vectors i = thread, thread + NT .. by fours, single values behind the last.
 struct LpWalk { int head, nvec, tail; };
 template <typename T> __device__ __forceinline__ LpWalk lp_walk(const T* p, int n) {
   const int head = min(n, int((16 - ((uintptr_t)p & 15)) & 15) / int(sizeof(T))), nvec = (n - head) / LpVec<T>::N;
   return {head, nvec, head + nvec * LpVec<T>::N};
 }
-// vectors in the group that begins with vector i
-__device__ __forceinline__ int lp_group(int i, int nvec) { return i + (kLpGroup - 1) * kLpThreads < nvec ? kLpGroup : 1; }
 
 // Order of logits as whole numbers: NaN above all, -0 as 0; ties by the lower id.
 __device__ __forceinline__ uint32_t lp_order(float v) {
@@ -119,8 +151,9 @@ __device__ __forceinline__ uint32_t lp_cluster_size() {
 }
 
 // out[0 .. k) = the k largest of n distinct keys in order; a key's place is the number of larger ones. All threads of the CTA.
+template <int NT>
 __device__ __forceinline__ void lp_sort(const unsigned long long* keys, int n, int k, unsigned long long* out) {
-  for (int i = threadIdx.x; i < n; i += kLpThreads) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const unsigned long long key = keys[i];
     int larger = 0;
     for (int j = 0; j < n; ++j) larger += keys[j] > key;
@@ -130,12 +163,12 @@ __device__ __forceinline__ void lp_sort(const unsigned long long* keys, int n, i
 }
 
 // The k largest keys of p[0 .. n) (ids from id0 on) into sh.best, one pass a key: for what the shorter way below does not take.
-template <typename T>
-__device__ __noinline__ void lp_top_by_passes(const T* __restrict__ p, int n, int id0, int k, LpShared& sh) {
+template <typename T, int NT>
+__device__ __noinline__ void lp_top_by_passes(const T* __restrict__ p, int n, int id0, int k, LpShared<NT>& sh) {
   unsigned long long last = ~0ull;
   for (int i = 0; i < k; ++i) {
     unsigned long long best = 0;
-    for (int j = threadIdx.x; j < n; j += kLpThreads) {
+    for (int j = threadIdx.x; j < n; j += NT) {
       const unsigned long long key = lp_key(to_f32<T>(p[j]), id0 + j);
       if (key < last && key > best) best = key;
     }
@@ -147,7 +180,7 @@ __device__ __noinline__ void lp_top_by_passes(const T* __restrict__ p, int n, in
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh.list[threadIdx.x >> 5] = best;
     __syncthreads();
-    for (int w = 0; w < kLpWarps; ++w) best = sh.list[w] > best ? sh.list[w] : best;
+    for (int w = 0; w < NT / 32; ++w) best = sh.list[w] > best ? sh.list[w] : best;
     if (threadIdx.x == 0) sh.best[i] = best;
     last = best;
   }
@@ -157,21 +190,21 @@ __device__ __noinline__ void lp_top_by_passes(const T* __restrict__ p, int n, in
 // The k largest of p[0 .. n), from what each thread noted on its way: the largest value among its vectors and the group that first had it.
 // The k threads with the largest of those values (lowest ids first) have all k of them: a value that is none of these threads' is smaller than
 // each of their largest. So only their vectors are looked at again, about k values in all are not below the last of those, and they are ordered.
-template <typename T>
-__device__ __forceinline__ void lp_top(const T* __restrict__ p, int n, int id0, int k, LpWalk at, float most, int group, LpShared& sh) {
-  constexpr int N = LpVec<T>::N;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// For short rows: a CTA of 64 threads.
+template <typename T, int NT>
+__device__ __forceinline__ void lp_top_of_threads(const T* __restrict__ p, int n, int id0, int k, LpWalk at, float most, int group, LpShared<NT>& sh) {
+  constexpr int N = LpVec<T>::N, CAP = LpShared<NT>::kList;
+  static_assert(NT == 64, "one thread to each of the 64 groups");
   const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
-  // 1. a bound by values alone, so that few threads look up where their largest is: the k-th of 64 groups of four threads
+  // 1. a bound by values alone, so that few threads look up where their largest is: the k-th of the threads'
   const uint32_t own = group < 0 ? 0u : lp_order(most);
-  uint32_t g = max(own, __shfl_xor_sync(0xffffffffu, own, 1));
-  g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-  if ((lane & 3) == 0) sh.group[threadIdx.x >> 2] = g;
+  sh.group[threadIdx.x] = own;
   if (threadIdx.x == 0) { sh.n = 0; sh.bound = 0; }
   __syncthreads();
-  if (threadIdx.x < 64) {
+  {
     const uint32_t v = sh.group[threadIdx.x];
     int before = 0;
+#pragma unroll 16
     for (int j = 0; j < 64; ++j) before += sh.group[j] > v || (sh.group[j] == v && j < int(threadIdx.x));
     if (before == k - 1) sh.bound = v;
   }
@@ -180,23 +213,25 @@ __device__ __forceinline__ void lp_top(const T* __restrict__ p, int n, int id0, 
   const uint32_t least = max(uint32_t(sh.bound), 1u);
   unsigned long long mine = 0;
   if (own >= least) {
-    const int vecs = lp_group(group, at.nvec);
-    for (int x = 0; x < vecs; ++x) {
-      const int i = group + x * kLpThreads;
-      const uint4 raw = __ldg(q + i);
+    // (a group of one vector is a thread's last: there is none behind it)
+    uint4 raw[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) raw[x] = __ldg(q + (group + x * NT < at.nvec ? group + x * NT : group));
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const unsigned long long key = lp_key(to_f32<T>(reinterpret_cast<const T*>(&raw)[j]), id0 + at.head + i * N + j);
+        const unsigned long long key = lp_key(to_f32<T>(reinterpret_cast<const T*>(&raw[x])[j]), id0 + at.head + (group + x * NT < at.nvec ? group + x * NT : group) * N + j);
         mine = key > mine ? key : mine;
       }
-    }
     sh.list[atomicAdd(&sh.n, 1)] = mine;
   }
   __syncthreads();
   const int found = sh.n;
-  int larger = kLpThreads;
+  int larger = NT;
   if (mine) {
     larger = 0;
+#pragma unroll 4
     for (int j = 0; j < found; ++j) larger += sh.list[j] > mine;
     if (larger < k) sh.chosen[larger] = threadIdx.x;
   }
@@ -204,39 +239,146 @@ __device__ __forceinline__ void lp_top(const T* __restrict__ p, int n, int id0, 
   if (threadIdx.x == 0) { sh.n = 0; if (found < k) sh.bound = 0; }
   if (larger == k - 1) sh.bound = mine;
   __syncthreads();
-  // 3. the chosen threads' vectors again, a warp each, and the single values at the ends
+  // 3. the chosen threads' vectors again, dealt to all threads, and the single values at the ends
   const unsigned long long bound = sh.bound;
+  const float value = bound ? lp_of_key(bound) : -INFINITY;
   auto offer = [&](float v, int j) {
-    const unsigned long long key = lp_key(v, id0 + j);
-    if (key >= bound) {
-      const int i = atomicAdd(&sh.n, 1);
-      if (i < 1024) sh.list[i] = key;
+    if (v >= value) {
+      const unsigned long long key = lp_key(v, id0 + j);
+      if (key >= bound) {
+        const int i = atomicAdd(&sh.n, 1);
+        if (i < CAP) sh.list[i] = key;
+      }
     }
   };
-  for (int b = w; b < min(found, k); b += kLpWarps) {
-    const int t = sh.chosen[b];
-    for (int i = t + lane * kLpThreads; i < at.nvec; i += 32 * kLpThreads) {
-      const uint4 raw = __ldg(q + i);
+  const int each = (at.nvec + NT - 1) / NT, all = min(found, k) * each;
+  for (int x0 = threadIdx.x; x0 < all; x0 += 4 * NT) {
+    uint4 raw[4];
+    int i[4];
 #pragma unroll
-      for (int j = 0; j < N; ++j) offer(to_f32<T>(reinterpret_cast<const T*>(&raw)[j]), at.head + i * N + j);
+    for (int x = 0; x < 4; ++x) {
+      const int e = x0 + x * NT, b = e / each;
+      i[x] = e < all ? sh.chosen[b] + (e - b * each) * NT : at.nvec;
+      if (i[x] < at.nvec) raw[x] = __ldg(q + i[x]);
     }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (i[x] < at.nvec) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) offer(to_f32<T>(reinterpret_cast<const T*>(&raw[x])[j]), at.head + i[x] * N + j);
+      }
   }
   if (threadIdx.x < at.head) offer(to_f32<T>(p[threadIdx.x]), threadIdx.x);
   if (threadIdx.x < n - at.tail) offer(to_f32<T>(p[at.tail + threadIdx.x]), at.tail + threadIdx.x);
   __syncthreads();
   const int m = sh.n;
-  if (m > 1024 || m < min(k, n)) lp_top_by_passes<T>(p, n, id0, k, sh);      // large values close together in few threads, or NaN
-  else lp_sort(sh.list, m, k, sh.best);
+  if (m > CAP || m < min(k, n)) lp_top_by_passes<T, NT>(p, n, id0, k, sh);      // large values close together in few threads, or NaN
+  else lp_sort<NT>(sh.list, m, k, sh.best);
+}
+
+// The same for long rows, from the largest value of each segment of 32 vectors, 512 bytes in a row. The k segments with the largest of those (the first
+// ones among equals) have all k of them: whatever stands in another segment comes behind the largest of each of these. They are read again as whole
+// lines (what 20 threads had seen, a sector here and there, was a third of a row of 16 bits: 3000 x 151936 with 20 alternatives 239 us).
+template <typename T, int NT>
+__device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int n, int id0, int k, LpWalk at, LpShared<NT>& sh) {
+  constexpr int N = LpVec<T>::N, CAP = LpShared<NT>::kList, EACH = NT / 64;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, segments = (at.nvec + 31) / 32;
+  const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
+  if (segments < k || segments > LpShared<NT>::kSegments) { lp_top_by_passes<T, NT>(p, n, id0, k, sh); return; }
+  // 1. a bound, the k-th of 64 groups of segments
+  uint32_t own = 0;
+  for (int i = threadIdx.x; i < segments; i += NT) own = max(own, lp_order(sh.segment[i]));
+#pragma unroll
+  for (int o = 1; o < EACH; o *= 2) own = max(own, __shfl_xor_sync(0xffffffffu, own, o));
+  if (lane % EACH == 0) sh.group[threadIdx.x / EACH] = own;
+  if (threadIdx.x == 0) { sh.n = 0; sh.bound = 0; }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const uint32_t v = sh.group[threadIdx.x];
+    int before = 0;
+#pragma unroll 16
+    for (int j = 0; j < 64; ++j) before += sh.group[j] > v || (sh.group[j] == v && j < int(threadIdx.x));
+    if (before == k - 1) sh.bound = v;
+  }
+  __syncthreads();
+  // 2. the segments not below it, in order: the first k are chosen
+  const uint32_t least = uint32_t(sh.bound);
+  for (int i = threadIdx.x; i < segments; i += NT) {
+    const uint32_t v = lp_order(sh.segment[i]);
+    if (v >= least) {
+      const int at_list = atomicAdd(&sh.n, 1);
+      if (at_list < CAP) sh.list[at_list] = (unsigned long long)v << 32 | uint32_t(~i);
+    }
+  }
+  __syncthreads();
+  const int found = sh.n;
+  if (found > CAP) { lp_top_by_passes<T, NT>(p, n, id0, k, sh); return; }
+  for (int i = threadIdx.x; i < found; i += NT) {
+    const unsigned long long key = sh.list[i];
+    int larger = 0;
+#pragma unroll 4
+    for (int j = 0; j < found; ++j) larger += sh.list[j] > key;
+    if (larger < k) sh.chosen[larger] = int(~uint32_t(key));
+  }
+  __syncthreads();
+  const float value = sh.segment[sh.chosen[k - 1]];
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  // 3. their values that are not below the last one's largest, of those equal to it no more than k a segment, a warp a segment
+  auto offer = [&](float v, int j) {
+    const int i = atomicAdd(&sh.n, 1);
+    if (i < CAP) sh.list[i] = lp_key(v, id0 + j);
+  };
+  for (int b = w; b < k; b += NT / 32) {
+    const int i = sh.chosen[b] * 32 + lane;
+    const bool has = i < at.nvec;
+    const uint4 raw = __ldg(q + (has ? i : 0));
+    float v[N];
+    int equal = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      v[j] = to_f32<T>(reinterpret_cast<const T*>(&raw)[j]);
+      equal += v[j] == value;
+    }
+    if (!has) equal = 0;
+    int before = equal;                                                  // equal ones in the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    before -= equal;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const bool same = v[j] == value;
+      if (has && (v[j] > value || (same && before < k))) offer(v[j], at.head + i * N + j);
+      before += same;
+    }
+  }
+  if (threadIdx.x < at.head && to_f32<T>(p[threadIdx.x]) >= value) offer(to_f32<T>(p[threadIdx.x]), threadIdx.x);
+  if (threadIdx.x < n - at.tail && to_f32<T>(p[at.tail + threadIdx.x]) >= value) offer(to_f32<T>(p[at.tail + threadIdx.x]), at.tail + threadIdx.x);
+  __syncthreads();
+  const int m = sh.n;
+  if (m > CAP || m < k) lp_top_by_passes<T, NT>(p, n, id0, k, sh);       // more than a thousand large values in a few segments
+  else lp_sort<NT>(sh.list, m, k, sh.best);
+}
+
+// The largest of a warp's values.
+__device__ __forceinline__ float lp_warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
 // A row by a cluster of CTAs (of one, where there are rows enough), a slice each.
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(kLpThreads, 4)
+// NT: 64 threads a CTA for short rows, 256 for long ones; TOP (256): with alternatives.
+template <typename T, bool ENT, int NT, bool TOP>
+__global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 1280) / NT)
 lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, const long long* __restrict__ tokens, float inv_t, int top, float* __restrict__ lp,
                float* __restrict__ ent, long long* __restrict__ rank, long long* __restrict__ top_ids, float* __restrict__ top_lp,
                float4* __restrict__ stats) {
   constexpr int N = LpVec<T>::N;
-  __shared__ LpShared sh;
+  __shared__ typename std::conditional<TOP, LpShared<NT>, LpSums<NT>>::type sh;
   const uint32_t parts = lp_cluster_size(), part = cluster_ctarank();
   const long long row = blockIdx.x / parts;
   const long long t = tokens ? tokens[row] : 0;
@@ -248,7 +390,7 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
       if (stats) stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (part == 0)
-      for (int i = threadIdx.x; i < top; i += kLpThreads) { top_ids[row * top + i] = -1; top_lp[row * top + i] = 0.f; }
+      for (int i = threadIdx.x; i < top; i += NT) { top_ids[row * top + i] = -1; top_lp[row * top + i] = 0.f; }
     return;
   }
   const int id0 = part * slice, n = max(0, min(slice, V - id0));
@@ -263,32 +405,53 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     lp_join<ENT>(a, v, v[0], c);
     above += v[0] > lt;
   };
+  const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   auto vectors = [&](auto& raw, int i) {
     constexpr int G = sizeof(raw) / 16;
-    float v[G * N];
-    const float m = lp_values<T, G>(raw, v);
-    lp_join<ENT>(a, v, m, c);
-    if (rank && m > lt) above += lp_above<T, G>(raw, v, lt);
-    if (m > most || group < 0) { most = m; group = i; }
+    float m;
+    if constexpr (TOP && NT > 64) {
+      float each[G];
+      each[0] = m = lp_largest<T, 0, 1>(raw);
+      if constexpr (G == 4) {
+        each[1] = lp_largest<T, 1, 1>(raw);
+        each[2] = lp_largest<T, 2, 1>(raw);
+        each[3] = lp_largest<T, 3, 1>(raw);
+        m = fmaxf(fmaxf(m, each[1]), fmaxf(each[2], each[3]));
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float s = lp_warp_max(each[g]);
+        const int at_segment = (i - lane + g * NT) >> 5;
+        if (lane == 0 && i + g * NT < at.nvec && at_segment < LpShared<NT>::kSegments) sh.segment[at_segment] = s;
+      }
+    } else {
+      m = lp_largest<T, 0, G>(raw);
+    }
+    lp_join_vectors<T, ENT, G>(a, raw, m, c);
+    if (rank && m > lt) above += lp_above<T, G>(raw, lt);
+    if constexpr (TOP && NT == 64)
+      if (m > most || group < 0) { most = m; group = i; }
   };
   if (threadIdx.x < at.head) single(threadIdx.x);
-  {
-    const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
-    int i = threadIdx.x;
-    for (; i + (kLpGroup - 1) * kLpThreads < at.nvec; i += kLpGroup * kLpThreads) {
-      uint4 raw[kLpGroup];
+  int i = threadIdx.x;
+  for (; i - lane + 31 + 3 * NT < at.nvec; i += 4 * NT) {
+    const uint4 raw[4] = {__ldg(q + i), __ldg(q + i + NT), __ldg(q + i + 2 * NT), __ldg(q + i + 3 * NT)};
+    vectors(raw, i);
+  }
+  // a warp's last vectors, all of them under way at once: what lies behind the row's end counts as minus infinities
+  constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  if (i - lane + NT < at.nvec) {
+    uint4 raw[4];
 #pragma unroll
-      for (int g = 0; g < kLpGroup; ++g) raw[g] = __ldg(q + i + g * kLpThreads);
-      vectors(raw, i);
-    }
-    for (; i < at.nvec; i += kLpThreads) {
-      uint4 raw[1] = {__ldg(q + i)};
-      vectors(raw, i);
-    }
+    for (int g = 0; g < 4; ++g) raw[g] = i + g * NT < at.nvec ? __ldg(q + i + g * NT) : make_uint4(none, none, none, none);
+    vectors(raw, i);
+  } else if (i - lane < at.nvec) {
+    const uint4 raw[1] = {i < at.nvec ? __ldg(q + i) : make_uint4(none, none, none, none)};
+    vectors(raw, i);
   }
   if (threadIdx.x < n - at.tail) single(at.tail + threadIdx.x);
   // the CTA's threads
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     a = lp_both<ENT>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
@@ -297,14 +460,17 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
   __syncthreads();
   a = {sh.red[0][0], sh.red[1][0], sh.red[2][0]};
   above = sh.redi[0];
-  for (int x = 1; x < kLpWarps; ++x) {
+  for (int x = 1; x < NT / 32; ++x) {
     a = lp_both<ENT>(a, {sh.red[0][x], sh.red[1][x], sh.red[2][x]}, c);
     above += sh.redi[x];
   }
-  const int k = min(top, n);
-  if (k > 0) {
-    if (a.s == a.s) lp_top<T>(p, n, id0, k, at, most, group, sh);
-    else lp_top_by_passes<T>(p, n, id0, k, sh);                          // a NaN or plus infinity, which the maxima on the way do not count
+  if constexpr (TOP) {
+    const int k = min(top, n);
+    if (k > 0) {
+      if (!(a.s == a.s)) lp_top_by_passes<T, NT>(p, n, id0, k, sh);      // a NaN or plus infinity, which the maxima on the way do not count
+      else if constexpr (NT == 64) lp_top_of_threads<T, NT>(p, n, id0, k, at, most, group, sh);
+      else lp_top_of_segments<T, NT>(p, n, id0, k, at, sh);
+    }
   }
   // the cluster's CTAs
   if (parts > 1) {
@@ -324,13 +490,13 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
         b = lp_both<ENT>(b, {__shfl_xor_sync(0xffffffffu, b.m, o), __shfl_xor_sync(0xffffffffu, b.s, o), __shfl_xor_sync(0xffffffffu, b.u, o)}, c);
       a = {__shfl_sync(0xffffffffu, b.m, 0), __shfl_sync(0xffffffffu, b.s, 0), __shfl_sync(0xffffffffu, b.u, 0)};
       above = __reduce_add_sync(0xffffffffu, more);
-      if (top > 0) {
-        if (int(threadIdx.x) < int(parts) * top) {                       // a slice has top alternatives, a short last one fewer: keys of zero, below all
-          const int x = threadIdx.x / top, j = threadIdx.x - x * top;
-          sh.list[threadIdx.x] = j < min(top, max(0, min(slice, V - x * slice))) ? lp_remote(sh.best + j, x) : 0;
+      if constexpr (TOP) {
+        for (int e = threadIdx.x; e < int(parts) * top; e += NT) {       // a slice has top alternatives, a short last one fewer: keys of zero, below all
+          const int x = e / top, j = e - x * top;
+          sh.list[e] = j < min(top, max(0, min(slice, V - x * slice))) ? lp_remote(sh.best + j, x) : 0;
         }
         __syncthreads();
-        lp_sort(sh.list, parts * top, top, sh.best);
+        lp_sort<NT>(sh.list, parts * top, top, sh.best);
       }
     }
   }
@@ -342,10 +508,12 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
       if (rank) rank[row] = 1 + above;
       if (stats) stats[row] = make_float4(a.m, 1.f / a.s, ls, H);
     }
-    if (int(threadIdx.x) < top) {
-      const unsigned long long key = sh.best[threadIdx.x];
-      top_ids[row * top + threadIdx.x] = lp_id(key);
-      top_lp[row * top + threadIdx.x] = (lp_of_key(key) - a.m) * inv_t - ls;
+    if constexpr (TOP) {
+      if (int(threadIdx.x) < top) {
+        const unsigned long long key = sh.best[threadIdx.x];
+        top_ids[row * top + threadIdx.x] = lp_id(key);
+        top_lp[row * top + threadIdx.x] = (lp_of_key(key) - a.m) * inv_t - ls;
+      }
     }
   }
   if (parts > 1) {                                                       // nobody leaves while its memory is read
@@ -485,26 +653,26 @@ using namespace b200;
 
 static bool lp_bad(long long rows, int V) { return rows < 0 || rows > 0x7fffffffll || V <= 0; }
 
-// Rows of few: a cluster of up to eight CTAs a row, as long as each has 4096 logits or more and the GPU's SMs are not all busy.
-static int lp_parts(long long rows, int V) {
+// CTAs of a row: where rows are few, a cluster of up to eight, as long as each has 32 KB or more and the SMs are not all busy.
+static int lp_parts(long long rows, long long bytes) {
   int parts = 1;
-  while (parts < kLpMaxCluster && rows * parts * 2 <= 2 * kNumSMs && V / (parts * 2) >= 4096) parts *= 2;
+  while (parts < kLpMaxCluster && rows * parts * 2 <= 2 * kNumSMs && bytes / (parts * 2) >= 32768) parts *= 2;
   return parts;
 }
+constexpr long long kLpSmallRow = 32768;
 static int lp_slice(int V, int parts) { return ((V + parts - 1) / parts + 31) / 32 * 32; }
 
-template <typename T, bool ENT>
-static cudaError_t lp_rows_launch(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp, float* ent,
+template <typename T, bool ENT, int NT, bool TOP>
+static cudaError_t lp_rows_launch(int parts, const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp, float* ent,
                                   long long* rank, long long* top_ids, float* top_lp, void* stats, cudaStream_t st) {
-  const int parts = lp_parts(rows, V);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(rows * parts)); cfg.blockDim = dim3(kLpThreads); cfg.stream = st;
+  cfg.gridDim = dim3(unsigned(rows * parts)); cfg.blockDim = dim3(NT); cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, lp_rows_kernel<T, ENT>, (const T*)logits, rs, V, parts > 1 ? lp_slice(V, parts) : V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp,
-                            (float4*)stats);
+  cfg.attrs = attr; cfg.numAttrs = parts > 1;
+  return cudaLaunchKernelEx(&cfg, lp_rows_kernel<T, ENT, NT, TOP>, (const T*)logits, rs, V, parts > 1 ? lp_slice(V, parts) : V, tokens, inv_t, top, lp, ent, rank, top_ids,
+                            top_lp, (float4*)stats);
 }
 
 B200_API int b200_token_logprobs(const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp,
@@ -512,9 +680,16 @@ B200_API int b200_token_logprobs(const void* logits, long long rs, long long row
   if (lp_bad(rows, V) || top < 0 || top > kLpMaxTop || top > V) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
   cudaStream_t st = (cudaStream_t)stream;
+  const long long bytes = (long long)V * (dtype == B200_DT_FP32 ? 4 : 2);
+  const int parts = lp_parts(rows, bytes);
+  // Short rows take CTAs of two warps: what a row costs beside its logits (its token, the meeting of its threads) is then one of many on an SM
+  // (20000 x 6400 in bf16: 147 us with 256 threads a row, 95 with 64).
+  const bool small = parts == 1 && bytes <= kLpSmallRow;
+#define LP_ROWS(ENT, NT, TOP) B200_CHECK((lp_rows_launch<T, ENT, NT, TOP>(parts, logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)))
   LP_TYPES(dtype, {
-    if (ent) B200_CHECK((lp_rows_launch<T, true>(logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)));
-    else B200_CHECK((lp_rows_launch<T, false>(logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)));
+    if (small) { if (ent) LP_ROWS(true, 64, true); else LP_ROWS(false, 64, true); }
+    else if (top) { if (ent) LP_ROWS(true, 256, true); else LP_ROWS(false, 256, true); }
+    else { if (ent) LP_ROWS(true, 256, false); else LP_ROWS(false, 256, false); }
   });
   B200_LAUNCH_CHECK();
   return 0;

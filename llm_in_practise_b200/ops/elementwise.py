@@ -302,10 +302,15 @@ def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: floa
     if D < 1 or not 1 <= rows < 2 ** 31 - 1 or T >= 2 ** 30 or dout.dtype not in (torch.float32, torch.bfloat16, torch.float16) or dtype not in (dout.dtype, torch.float32):
         raise ValueError(f"embedding_grad: {T} tokens of {dout.dtype} [{D}] into {rows} rows of {dtype} are not taken")
     flat, d2 = ids.reshape(-1).contiguous(), dout.reshape(T, D)
-    if not nv.use_native(dout):
-        keep = (flat >= 0) & (flat < rows) & (flat != (-1 if padding_idx is None else padding_idx))
-        out = torch.zeros(rows, D, dtype=torch.float32, device=dout.device)
-        return out.index_add_(0, flat[keep], d2[keep].float()).mul_(scale).to(dtype)
+    if nv.use_native(dout):
+        return _embedding_grad(flat, d2, rows, scale, padding_idx, dtype)
+    keep = (flat >= 0) & (flat < rows) & (flat != (-1 if padding_idx is None else padding_idx))
+    out = torch.zeros(rows, D, dtype=torch.float32, device=dout.device)
+    return out.index_add_(0, flat[keep], d2[keep].float()).mul_(scale).to(dtype)
+
+
+def _embedding_grad(flat, d2, rows, scale, padding_idx, dtype):
+    T, D = d2.shape
     if D > 1 and d2.stride(1) != 1:
         d2 = d2.contiguous()
     out = d2.new_empty((rows, D), dtype=dtype)
@@ -315,37 +320,49 @@ def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: floa
         fn.argtypes, fn.restype = [i64, i32], i64
         size = _embedding_work[T, D] = fn(T, D)
     work = d2.new_empty((size,), dtype=torch.uint8)
-    rc = nv.call_on(dout.device, nv.proto("b200_embedding_grad", _EMBEDDING_GRAD), flat.data_ptr(), d2.data_ptr(), d2.stride(0) if T > 1 else D, out.data_ptr(), T,
-                    rows, D, float(scale), -1 if padding_idx is None else padding_idx, nv.dtype_code(dout.dtype), nv.dtype_code(dtype), work.data_ptr())
+    rc = nv.call_on(d2.device, nv.proto("b200_embedding_grad", _EMBEDDING_GRAD), flat.data_ptr(), d2.data_ptr(), d2.stride(0) if T > 1 else D, out.data_ptr(), T,
+                    rows, D, float(scale), -1 if padding_idx is None else padding_idx, nv.dtype_code(d2.dtype), nv.dtype_code(dtype), work.data_ptr())
     if rc:
         nv.check(rc, "embedding_grad")
     nv.count_launch(4 if T else 1)
     return out
 
 
+_EMBEDDING_FWD = [vp, vp, vp, vp, i64, i32, i32, f32, i32, vp]
+
+
+def _embedding_fwd(ids, table, pos_table, period, scale):
+    flat = ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
+    if flat.dtype is not torch.int64:
+        flat = flat.to(torch.int64)
+    out = table.new_empty((*ids.shape, table.shape[1]))
+    if flat.numel():
+        rc = nv.call_on(table.device, nv.proto("b200_embedding_fwd", _EMBEDDING_FWD), flat.data_ptr(), table.data_ptr(), nv.ptr(pos_table), out.data_ptr(),
+                        flat.numel(), table.shape[1], period, scale, nv.dtype_code(table.dtype))
+        if rc:
+            nv.check(rc, "embedding_fwd")
+        nv.count_launch()
+    return flat, out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, pos_table, period, scale, padding_idx):
-        flat = ids.reshape(-1).contiguous()
-        out = torch.empty(flat.numel(), table.shape[1], dtype=table.dtype, device=table.device)
-        fn = nv.proto("b200_embedding_fwd", [vp, vp, vp, vp, i64, i32, i32, f32, i32, vp])
-        nv.check(fn(nv.ptr(flat), nv.ptr(table), nv.ptr(pos_table), nv.ptr(out), flat.numel(), table.shape[1], period,
-                    scale, nv.dtype_code(table.dtype), nv.stream()), "embedding_fwd")
-        nv.count_launch()
+        flat, out = _embedding_fwd(ids, table, pos_table, period, scale)
         if table.requires_grad:
             from ..utils.arena import note_use
             note_use(table, False)              # its gradient arrives through autograd (possibly after a tied head's)
         ctx.save_for_backward(flat)
         ctx.meta = (table.shape, table.dtype, pos_table is not None, period, scale,
                     None if pos_table is None else pos_table.shape, padding_idx)
-        return out.view(*ids.shape, table.shape[1])
+        return out
 
     @staticmethod
     def backward(ctx, dout):
         (flat,) = ctx.saved_tensors
         tshape, tdtype, has_pos, period, scale, pshape, padding_idx = ctx.meta
-        dout2 = dout.reshape(-1, tshape[1])
-        dtable = embedding_grad(flat, dout2, tshape[0], scale, padding_idx) if ctx.needs_input_grad[1] else None
+        dout2 = dout if dout.dim() == 2 else dout.reshape(-1, tshape[1])
+        dtable = _embedding_grad(flat, dout2, tshape[0], scale, padding_idx, tdtype) if ctx.needs_input_grad[1] else None
         dpos = None
         if has_pos and ctx.needs_input_grad[2]:
             g = dout2.float().view(-1, period, tshape[1]).sum(0)
@@ -362,7 +379,9 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, pos_table: Optional[torch.
     period = ids.shape[-1]
     vec = 4 if table.dtype == torch.float32 else 8
     if nv.use_native(table) and table.shape[1] % vec == 0:
-        return _EmbeddingFn.apply(ids, table, pos_table, period, float(scale), padding_idx)
+        if torch.is_grad_enabled() and (table.requires_grad or (pos_table is not None and pos_table.requires_grad)):
+            return _EmbeddingFn.apply(ids, table, pos_table, period, float(scale), padding_idx)
+        return _embedding_fwd(ids, table, pos_table, period, float(scale))[1]
     out = F.embedding(ids, table, padding_idx) * scale if scale != 1.0 else F.embedding(ids, table, padding_idx)
     if pos_table is not None:
         out = out + pos_table[:period]
