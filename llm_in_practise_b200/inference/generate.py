@@ -28,6 +28,7 @@ from ..ops import _native as nv
 from ..ops import elementwise as ew
 from ..ops import fused_decode
 from ..ops.logits import MAX_BIAS, MAX_HISTORY, MAX_VOCAB, SCALES, LogitState, greedy_tokens, process_logits
+from ..ops.logprobs import MAX_TOP, token_logprobs
 from ..ops.paged_attention import rope_paged_store
 from ..ops.prefix_attention import PrefixGroups, make_prefix_groups, prefix_attention
 from ..ops.step_maps import extend_block_tables
@@ -60,6 +61,9 @@ class GenerationConfig:
     # HF's prefix_allowed_tokens_fn(batch row or request id, its tokens so far) -> the tokens that may come next: a grammar, asked before every token.
     # Where it allows none of the vocabulary (and of allowed_token_ids) it is an error, as in HF
     prefix_allowed_tokens_fn: Optional[Callable[[int, List[int]], Sequence[int]]] = None
+    # the serving engine's requests: log probabilities of what is generated, with this many alternatives (0: of the tokens alone), under the logits
+    # as the model gives them, before penalties and temperature (vLLM's ``logprobs``). ``generate`` has ``return_logprobs``
+    logprobs: Optional[int] = None
 
     def allows_nothing(self) -> bool:
         """Whether ``allowed_token_ids`` is an empty list: every token would break it."""
@@ -72,6 +76,8 @@ class GenerationConfig:
 
     def check_rules(self, vocab: int, max_len: int = 0) -> None:
         """Refuse rules that ``vocab`` tokens, or sequences of up to ``max_len``, have no room for, before a step is run with them."""
+        if self.logprobs is not None and not 0 <= self.logprobs <= min(MAX_TOP, vocab):
+            raise ValueError(f"logprobs must be from 0 to {min(MAX_TOP, vocab)}, not {self.logprobs}")
         if not self.has_rules():
             return
         if vocab > MAX_VOCAB or max_len > MAX_HISTORY:
@@ -744,7 +750,7 @@ class Generator:
         for _ in range(total - S):
             nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen, done=done)
             if return_logprobs:
-                logprobs.append(logits.float().log_softmax(-1).gather(1, nxt[:, None]).squeeze(1))
+                logprobs.append(token_logprobs(logits, nxt).logprob)
             nxt = torch.where(done, torch.full_like(nxt, cfg.pad_token_id), nxt)
             out = torch.cat([out, nxt[:, None]], 1)
             if streamer is not None:

@@ -20,6 +20,7 @@ import numpy as np
 import torch
 
 from ..ops.gemm import ensure_graph_workspace
+from ..ops.logprobs import token_logprobs
 from ..ops.step_maps import step_maps
 from ..utils.graph_step import no_gc
 
@@ -241,7 +242,7 @@ class RaggedGenerator(Generator):
         for n in range(S, total):
             nxt = sample_next(logits, cfg, out, gen) if rules is None else rules.next(logits, range(B), [cfg] * B, gen, done=done)
             if return_logprobs:
-                logprobs.append(logits.float().log_softmax(-1).gather(1, nxt[:, None]).squeeze(1))
+                logprobs.append(token_logprobs(logits, nxt).logprob)
             nxt = torch.where(done, torch.full_like(nxt, cfg.pad_token_id), nxt)
             out = torch.cat([out, nxt[:, None]], 1)
             if streamer is not None:

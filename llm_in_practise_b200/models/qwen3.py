@@ -21,8 +21,11 @@ from torch import nn
 from torch.utils.checkpoint import checkpoint
 
 from ..ops import elementwise as ew
+from ..ops.act8 import checkpoint8, swiglu8
 from ..ops.attention import attention
+from ..ops.functional import linear
 from ..ops.linear import FusedLinear
+from ..ops.logprobs import TokenLogprobs, linear_token_logprobs, token_logprobs
 from ..ops.loss import linear_cross_entropy, micro_batch_row_scale
 from ..ops.norm import rms_norm
 from ..ops.gemm import gemm
@@ -89,6 +92,7 @@ class Qwen3DecoderLayer(nn.Module):
         self.down_proj = FusedLinear(F, [("down_proj", h)], dtype=dtype, device=device)
         for j, lin in enumerate((self.qkv_proj, self.o_proj, self.gate_up_proj, self.down_proj)):
             lin.layer_uid = idx * 4 + j
+        self.activation_bits = 16          # of what the gated unit keeps for its backward pass
 
     def fused_linears(self):
         return {"qkv_proj": self.qkv_proj, "o_proj": self.o_proj, "gate_up_proj": self.gate_up_proj,
@@ -104,7 +108,7 @@ class Qwen3DecoderLayer(nn.Module):
         a = self.o_proj(ctx)
         x, residual = rms_norm(a, self.post_attention_layernorm, cfg.rms_norm_eps, residual)
         gu = self.gate_up_proj(x)
-        hmid = ew.swiglu(gu)
+        hmid = swiglu8(gu) if self.activation_bits == 8 and gu.requires_grad else ew.swiglu(gu)
         return self.down_proj(hmid), residual
 
 
@@ -125,6 +129,7 @@ class Qwen3ForCausalLM(nn.Module):
             self.lm_head = nn.Parameter(torch.empty(cfg.vocab_size, cfg.hidden_size, dtype=dtype, device=device))
             nn.init.normal_(self.lm_head, std=init_std)
         self.gradient_checkpointing = False
+        self.checkpoint_bits = 16
         self._rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
         self.ce_chunk_tokens = 4096
 
@@ -132,11 +137,22 @@ class Qwen3ForCausalLM(nn.Module):
     def head_weight(self) -> torch.Tensor:
         return self.embed_tokens if self.lm_head is None else self.lm_head
 
-    def gradient_checkpointing_enable(self, **_):
-        self.gradient_checkpointing = True
+    def gradient_checkpointing_enable(self, activation_bits: int = 16, **_):
+        """``activation_bits`` 8: a layer's input, stream and branch added, is kept in 8 bits (``ops.act8.checkpoint8``) instead of 16 of each; as
+        ``gradient_checkpointing_kwargs={"activation_bits": 8}`` of the trainer's arguments."""
+        if activation_bits not in (8, 16):
+            raise ValueError(f"activation_bits must be 8 or 16, not {activation_bits}")
+        self.gradient_checkpointing, self.checkpoint_bits = True, activation_bits
 
     def gradient_checkpointing_disable(self):
         self.gradient_checkpointing = False
+
+    def set_activation_bits(self, bits: int) -> None:
+        """8: training without checkpoints keeps the gated units' inputs, the largest of a layer's activations, in 8 bits (``ops.act8.swiglu8``)."""
+        if bits not in (8, 16):
+            raise ValueError(f"activation bits must be 8 or 16, not {bits}")
+        for layer in self.layers:
+            layer.activation_bits = bits
 
     # ---- the rest of the transformers call surface the reference's scripts use on a model -------------------------------
     @property
@@ -206,7 +222,9 @@ class Qwen3ForCausalLM(nn.Module):
         delta = ew.embedding(input_ids.reshape(-1), self.embed_tokens)
         residual = None
         for layer in self.layers:
-            if self.gradient_checkpointing and self.training and torch.is_grad_enabled():
+            if self.gradient_checkpointing and self.training and torch.is_grad_enabled() and self.checkpoint_bits == 8:
+                delta, residual = checkpoint8(layer, delta, residual, cos, sin, pos, B, S)
+            elif self.gradient_checkpointing and self.training and torch.is_grad_enabled():
                 delta, residual = checkpoint(layer, delta, residual, cos, sin, pos, B, S, use_reentrant=False)
             else:
                 delta, residual = layer(delta, residual, cos, sin, pos, B, S)
@@ -231,6 +249,19 @@ class Qwen3ForCausalLM(nn.Module):
         loss = linear_cross_entropy(hidden, self.head_weight(), targets.reshape(-1), -100, n_valid,
                                     self.ce_chunk_tokens, row_scale=rs)
         return {"loss": loss}
+
+    def log_probs(self, input_ids: torch.Tensor, labels: Optional[torch.Tensor] = None, entropy: bool = False, temperature: float = 1.0,
+                  position_ids: Optional[torch.Tensor] = None) -> TokenLogprobs:
+        """Log probabilities (and entropies of what they were chosen from) of the tokens behind each position, [B, S - 1], with gradients: what a policy gradient, a
+        preference loss or a perplexity takes. ``labels`` (input_ids where not given) [B, S]: tokens that are -100 are passed over, zeros."""
+        B, S = input_ids.shape
+        labels = input_ids if labels is None else labels
+        hidden = self.hidden_states(input_ids, position_ids).view(B, S, -1)[:, :-1]
+        w, targets = self.head_weight(), labels[:, 1:].contiguous()
+        if hidden.dtype == torch.float32 and hidden.is_cuda:         # products of 32 bits have no such epilogue
+            logits = linear(hidden.reshape(-1, hidden.shape[-1]), w)
+            return token_logprobs(logits.view(B, S - 1, -1), targets, entropy=entropy, temperature=temperature)
+        return linear_token_logprobs(hidden, w, targets, entropy=entropy, temperature=temperature)
 
     # -------------------------------------------------------------------------------------
     def num_parameters(self, only_trainable: bool = False) -> int:

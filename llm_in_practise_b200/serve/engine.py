@@ -22,12 +22,13 @@ import threading
 import time
 from collections import OrderedDict, deque
 from dataclasses import dataclass, field
-from typing import Deque, Dict, Iterator, List, Optional, Sequence, Tuple
+from typing import Deque, Dict, Iterator, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
 from ..inference.generate import MAX_GROUPS, GenerationConfig, Generator, KVCache, LogitRules, PagedKVCache, sample_next
 from ..ops.logits import MAX_BIAS
+from ..ops.logprobs import token_logprobs
 
 
 @dataclass
@@ -60,6 +61,15 @@ class EngineArgs:
     shared_prefix_min: int = 256
 
 
+class TokenLogprob(NamedTuple):
+    """What ``GenerationConfig.logprobs`` asks for, of one generated token: its log probability, its rank (1: the most probable) and the alternatives,
+    (token, log probability), the most probable first."""
+    token: int
+    logprob: float
+    rank: int
+    top: Tuple[Tuple[int, float], ...]
+
+
 @dataclass
 class Request:
     rid: int
@@ -80,6 +90,8 @@ class Request:
     aborted: bool = False                                    # set by LLMEngine.abort(): dropped at the next scheduler iteration
     reserved_blocks: int = 0                                 # paged cache: blocks promised to this request but not handed out yet
     rules_row: int = -1                                      # row of the engine's logit rules that was set up for this request
+    logprobs: List[TokenLogprob] = field(default_factory=list)   # one to a token of output_ids, where the request asks for them
+    sampled: Optional[TokenLogprob] = None                   # that of the token that was sampled last
 
     @property
     def ttft(self) -> Optional[float]:
@@ -583,6 +595,9 @@ class LLMEngine:
         if tok in self._eos(r.cfg) and not r.cfg.allows_nothing():
             self._finish(r, "stop")
             return True
+        if r.sampled is not None:                            # in the list before the token is in the stream
+            r.logprobs.append(r.sampled)
+            r.sampled = None
         r.output_ids.append(tok)
         r.token_times.append(now)
         r.stream.put(tok)
@@ -672,7 +687,19 @@ class LLMEngine:
             ids = sample_next(logits[idx], cfg, prev, self._rng)
             for i, t in zip(idx, ids.tolist()):
                 out[i] = t
+        asked = [i for i, r in enumerate(reqs) if r.cfg.logprobs is not None]
+        if asked:
+            self._note_logprobs(logits if len(asked) == len(reqs) else logits[asked], [reqs[i] for i in asked], [out[i] for i in asked])
         return out
+
+    def _note_logprobs(self, logits: torch.Tensor, reqs: List[Request], tokens: List[int]) -> None:
+        """Log probabilities of the tokens that were sampled, and alternatives, for the requests that ask for them: one launch and one copy."""
+        top = max(r.cfg.logprobs for r in reqs)
+        got = token_logprobs(logits, torch.tensor(tokens, device=logits.device), top=top, rank=True)
+        parts = [got.logprob.unsqueeze(1), got.rank.unsqueeze(1)] + ([got.top_ids, got.top_logprobs] if top else [])
+        for r, t, row in zip(reqs, tokens, torch.cat([x.double() for x in parts], 1).tolist()):
+            n = r.cfg.logprobs
+            r.sampled = TokenLogprob(t, row[0], int(row[1]), tuple((int(i), p) for i, p in zip(row[2:2 + n], row[2 + top:2 + top + n])))
 
     def _start_running(self, r: Request) -> None:
         self.running.append(r)

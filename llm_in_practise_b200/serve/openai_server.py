@@ -49,6 +49,8 @@ class ChatCompletionRequest(BaseModel):
     allowed_token_ids: Optional[List[int]] = None   # vLLM: the only tokens that may be generated
     stop: Optional[Union[str, List[str]]] = None    # vLLM / OpenAI stop strings (not in the reference's FastAPI schema)
     ignore_eos: Optional[bool] = False              # vLLM extension (``vllm bench serve --ignore-eos``)
+    logprobs: Optional[bool] = False                # OpenAI: log probabilities of the generated tokens ...
+    top_logprobs: Optional[int] = Field(None, ge=0, le=20)      # ... and of this many alternatives to each
     stream_options: Optional[Dict[str, Any]] = None  # {"include_usage": true}: one more chunk with the token counts
 
 
@@ -65,6 +67,7 @@ class CompletionRequest(BaseModel):
     allowed_token_ids: Optional[List[int]] = None
     stop: Optional[Union[str, List[str]]] = None
     ignore_eos: Optional[bool] = False
+    logprobs: Optional[int] = Field(None, ge=0, le=20)          # OpenAI: log probabilities of the tokens and of this many alternatives
     stream_options: Optional[Dict[str, Any]] = None
 
 
@@ -96,6 +99,29 @@ def cut_at_stop(text: str, stops: List[str]):
     """(text truncated at the earliest stop string, True if one matched)."""
     cut = min((i for i in (text.find(x) for x in stops) if i >= 0), default=-1)
     return (text, False) if cut < 0 else (text[:cut], True)
+
+
+def _finite(lp: float) -> float:
+    """JSON has no infinities: what cannot happen is as improbable as vLLM says it."""
+    return max(lp, -9999.0) if lp == lp else -9999.0
+
+
+def chat_logprobs(entries, text_of) -> Dict[str, Any]:
+    """``choices[].logprobs`` of a chat completion for ``TokenLogprob`` s; ``text_of``: token id -> text."""
+    def one(i, lp):
+        t = text_of(i)
+        return {"token": t, "logprob": _finite(lp), "bytes": list(t.encode("utf-8", "replace"))}
+    return {"content": [{**one(e.token, e.logprob), "top_logprobs": [one(i, lp) for i, lp in e.top]} for e in entries]}
+
+
+def completion_logprobs(entries, text_of, offset: int = 0) -> Dict[str, Any]:
+    """The same of a text completion; ``offset``: characters in front of the first token."""
+    tokens, offsets = [text_of(e.token) for e in entries], []
+    for t in tokens:
+        offsets.append(offset)
+        offset += len(t)
+    return {"tokens": tokens, "token_logprobs": [_finite(e.logprob) for e in entries], "text_offset": offsets,
+            "top_logprobs": [{text_of(i): _finite(lp) for i, lp in reversed(e.top)} for e in entries]}
 
 
 def render_metrics(engine: LLMEngine) -> str:
@@ -158,11 +184,29 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         except TypeError:
             return eng.tokenizer.decode(ids)
 
+    def asked_logprobs(req) -> Optional[int]:
+        """Alternatives to a token (0: none), None where log probabilities are not asked for."""
+        if isinstance(req, CompletionRequest):
+            return req.logprobs
+        if req.top_logprobs and not req.logprobs:
+            raise ValueError("top_logprobs needs logprobs")
+        return int(req.top_logprobs or 0) if req.logprobs else None
+
+    def said(eng: LLMEngine, r, n, form, *at):
+        """``choices[].logprobs`` of the tokens of ``r`` from ``n[0]`` to ``n[1]``."""
+        return None if r.cfg.logprobs is None else form(r.logprobs[n[0]:n[1]], lambda i: decode(eng, [i]), *at)
+
+    def tokens_of(eng: LLMEngine, ids: List[int], stops: List[str]) -> int:
+        """How many tokens the text up to a stop string takes."""
+        if not stops:
+            return len(ids)
+        return next((n for n in range(1, len(ids) + 1) if cut_at_stop(decode(eng, ids[:n]), stops)[1]), len(ids))
+
     def gen_cfg(temperature, top_p, max_tokens, top_k=0, rep=1.0, ignore_eos=False, req=None) -> GenerationConfig:
         """``req``: the request that rules on logits are taken from (OpenAI's penalties and logit_bias, vLLM's allowed_token_ids)."""
         rules = {} if req is None else {"presence_penalty": float(req.presence_penalty or 0.0), "frequency_penalty": float(req.frequency_penalty or 0.0),
                                         "logit_bias": {int(k): float(v) for k, v in (req.logit_bias or {}).items()} or None,
-                                        "allowed_token_ids": req.allowed_token_ids}
+                                        "allowed_token_ids": req.allowed_token_ids, "logprobs": asked_logprobs(req)}
         if rules.get("allowed_token_ids") == []:
             raise ValueError("allowed_token_ids allows no token")
         t = 0.0 if temperature is None else float(temperature)
@@ -206,8 +250,15 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
             def events():
                 head = {"id": cid, "object": "chat.completion.chunk", "created": created, "model": req.model}
                 yield "data: " + json.dumps({**head, "choices": [{"index": 0, "delta": {"role": "assistant"}, "finish_reason": None}]}) + "\n\n"
-                sent, acc, stops, hit = "", [], _stops(req.stop), False
+                sent, acc, stops, hit, told = "", [], _stops(req.stop), False, 0
                 hold = max((len(x) for x in stops), default=1) - 1     # characters that could still become a stop string
+
+                def with_logprobs(choice):                 # those of the tokens since the last chunk
+                    nonlocal told
+                    if r.cfg.logprobs is not None:
+                        choice["logprobs"] = said(eng, r, (told, len(acc)), chat_logprobs)
+                        told = len(acc)
+                    return choice
                 for tok in r.tokens():
                     acc.append(tok)
                     text = decode(eng, acc)
@@ -217,15 +268,16 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
                     safe = text if hit else text[:max(len(text) - hold, len(sent))]
                     delta, sent = safe[len(sent):], safe
                     if delta:
-                        yield "data: " + json.dumps({**head, "choices": [{"index": 0, "delta": {"content": delta}, "finish_reason": None}]}, ensure_ascii=False) + "\n\n"
+                        yield "data: " + json.dumps({**head, "choices": [with_logprobs({"index": 0, "delta": {"content": delta}, "finish_reason": None})]}, ensure_ascii=False) + "\n\n"
                     if hit:
                         eng.abort(r)
                         break
                 if not hit:
                     tail = cut_at_stop(decode(eng, acc), stops)[0][len(sent):]
                     if tail:
-                        yield "data: " + json.dumps({**head, "choices": [{"index": 0, "delta": {"content": tail}, "finish_reason": None}]}, ensure_ascii=False) + "\n\n"
-                yield "data: " + json.dumps({**head, "choices": [{"index": 0, "delta": {}, "finish_reason": "stop" if hit else r.finish_reason}]}) + "\n\n"
+                        yield "data: " + json.dumps({**head, "choices": [with_logprobs({"index": 0, "delta": {"content": tail}, "finish_reason": None})]}, ensure_ascii=False) + "\n\n"
+                last = {"index": 0, "delta": {}, "finish_reason": "stop" if hit else r.finish_reason}
+                yield "data: " + json.dumps({**head, "choices": [with_logprobs(last) if told < len(acc) else last]}) + "\n\n"
                 if (req.stream_options or {}).get("include_usage"):
                     yield usage_chunk(head, len(ids), len(acc))
                 yield "data: [DONE]\n\n"
@@ -237,7 +289,8 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         text, hit = cut_at_stop(text, _stops(req.stop))
         n_p, n_c = len(ids), len(r.output_ids)
         return {"id": cid, "object": "chat.completion", "created": created, "model": req.model,
-                "choices": [{"index": 0, "message": {"role": "assistant", "content": text}, "finish_reason": "stop" if hit else r.finish_reason}],
+                "choices": [{"index": 0, "message": {"role": "assistant", "content": text}, "finish_reason": "stop" if hit else r.finish_reason,
+                             **({} if r.cfg.logprobs is None else {"logprobs": said(eng, r, (0, tokens_of(eng, r.output_ids, _stops(req.stop))), chat_logprobs)})}],
                 "usage": {"prompt_tokens": n_p, "completion_tokens": n_c, "total_tokens": n_p + n_c}}
 
     @app.post("/v1/completions")
@@ -259,8 +312,13 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
             head = {"id": f"cmpl-{uuid.uuid4().hex}", "object": "text_completion", "created": int(time.time()), "model": req.model}
 
             def events():
-                sent, acc, stops, hit = "", [], _stops(req.stop), False
+                sent, acc, stops, hit, told = "", [], _stops(req.stop), False, 0
                 hold = max((len(x) for x in stops), default=1) - 1
+
+                def logprobs():                            # those of the tokens since the last chunk
+                    nonlocal told
+                    a, told = told, len(acc)
+                    return said(eng, r, (a, told), completion_logprobs, len(decode(eng, acc[:a])))
                 for tok in r.tokens():
                     acc.append(tok)
                     text = decode(eng, acc)
@@ -270,13 +328,13 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
                     safe = text if hit else text[:max(len(text) - hold, len(sent))]
                     delta, sent = safe[len(sent):], safe
                     if delta:
-                        yield "data: " + json.dumps({**head, "choices": [{"index": 0, "text": delta, "finish_reason": None, "logprobs": None}]},
+                        yield "data: " + json.dumps({**head, "choices": [{"index": 0, "text": delta, "finish_reason": None, "logprobs": logprobs()}]},
                                                     ensure_ascii=False) + "\n\n"
                     if hit:
                         eng.abort(r)
                         break
                 tail = "" if hit else cut_at_stop(decode(eng, acc), stops)[0][len(sent):]
-                yield "data: " + json.dumps({**head, "choices": [{"index": 0, "text": tail, "logprobs": None,
+                yield "data: " + json.dumps({**head, "choices": [{"index": 0, "text": tail, "logprobs": logprobs(),
                                                                   "finish_reason": "stop" if hit else r.finish_reason}]},
                                             ensure_ascii=False) + "\n\n"
                 if (req.stream_options or {}).get("include_usage"):
@@ -289,7 +347,8 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
             if r.error:
                 raise HTTPException(status_code=500, detail=r.error)
             text, hit = cut_at_stop(decode(eng, r.output_ids), _stops(req.stop))
-            choices.append({"index": i, "text": text, "finish_reason": "stop" if hit else r.finish_reason, "logprobs": None})
+            choices.append({"index": i, "text": text, "finish_reason": "stop" if hit else r.finish_reason,
+                            "logprobs": said(eng, r, (0, tokens_of(eng, r.output_ids, _stops(req.stop))), completion_logprobs)})
             n_p += len(r.prompt_ids)
             n_c += len(r.output_ids)
         return {"id": f"cmpl-{uuid.uuid4().hex}", "object": "text_completion", "created": int(time.time()), "model": req.model,
