@@ -1,8 +1,10 @@
-// The gradient of an embedding lookup y[t] = s W[id_t], by sorted tokens:
+// An embedding lookup y[t] = s W[id_t] (+ P[t mod period]) and its gradient by sorted tokens:
 //     dW[v] = s * sum over t with id_t = v, in the order of t, of dy[t]
 // dense, a row of zeros where a token does not occur; every sum in 32 bits, in an order that is the same in every call (atomics into the
 // table would add in the order in which they arrive). Tokens outside 0 .. V - 1 and the padding token have no gradient.
 //
+//   embed_lookup the rows of W, eight values of 16 bits or four of 32 a thread, four such pieces under way; bound by HBM (with a CTA a token 16384 rows of
+//                64 values took 21 us, the CTAs' launches). A token outside the table gives zeros
 //   embed_sort   (token, place) pairs by token, places of a token in order: a radix sort by one cluster of eight CTAs, which hold the counts of
 //                a digit in shared memory and read each other's totals there. T ids make 8 T bytes a pass: the sort is bound by its steps'
 //                latencies, and stands beside the next kernel
@@ -15,12 +17,12 @@
 
 namespace b200 {
 
-constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 1024, kSortBits = 10;
+constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 1024, kSortBits = 10, kSortHeld = 4;
 constexpr int kSortSmem = (kSortWarps + 3) * kSortBins * 4;
 
 __device__ __forceinline__ uint32_t es_remote(const uint32_t* p, uint32_t rank) {
   uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)));
   return v;
 }
 
@@ -66,6 +68,7 @@ embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint
   const long long lo = min((long long)T, (rank * kSortWarps + w) * per_warp), hi = min((long long)T, lo + per_warp);
   uint32_t* mine = count + w * bins;
 
+  const int steps = int((hi - lo + 31) / 32);
   for (int pass = 0; pass < passes; ++pass) {
     const uint2* src = (passes - pass) & 1 ? b : a;         // what this pass reads (the first one reads ids)
     uint2* dst = (passes - pass) & 1 ? a : b;
@@ -77,11 +80,22 @@ embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint
       }
       return __ldcg(src + i);                               // written by other SMs in the pass before
     };
+    uint2 held[kSortHeld];                                  // a warp's first pairs stay where both walks over them find them
+#pragma unroll
+    for (int x = 0; x < kSortHeld; ++x) held[x] = lo + x * 32 + lane < hi ? pair(lo + x * 32 + lane) : make_uint2(0, 0);
+    auto at = [&](int x) -> uint2 {                         // the lane's pair of step x
+      uint2 p = make_uint2(0, 0);
+#pragma unroll
+      for (int y = 0; y < kSortHeld; ++y)
+        if (x == y) p = held[y];
+      if (x >= kSortHeld && lo + x * 32ll + lane < hi) p = pair(lo + x * 32ll + lane);
+      return p;
+    };
     for (int i = threadIdx.x; i < kSortWarps * bins; i += kSortThreads) count[i] = 0;
     __syncthreads();
-    for (long long i0 = lo; i0 < hi; i0 += 32) {
-      const bool has = i0 + lane < hi;
-      const uint32_t d = has ? (pair(i0 + lane).x >> shift) & (bins - 1) : 0xffffffffu;
+    for (int x = 0; x < steps; ++x) {
+      const bool has = lo + x * 32ll + lane < hi;
+      const uint32_t d = has ? (at(x).x >> shift) & (bins - 1) : 0xffffffffu;
       const uint32_t same = __match_any_sync(0xffffffffu, d);
       if (has && lane == __ffs(same) - 1) mine[d] += __popc(same);
       __syncwarp();
@@ -89,6 +103,7 @@ embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += kSortThreads) {
       uint32_t sum = 0;
+#pragma unroll 8
       for (int x = 0; x < kSortWarps; ++x) {
         const uint32_t c = count[x * bins + d];
         count[x * bins + d] = sum;
@@ -99,11 +114,13 @@ embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint
     cluster_sync_all();
     uint32_t before = 0;
     if (threadIdx.x < bins) {
-      uint32_t all = 0;
+      uint32_t all = 0, c[kSortCtas];
+#pragma unroll
+      for (uint32_t r = 0; r < kSortCtas; ++r) c[r] = es_remote(total + threadIdx.x, r);
+#pragma unroll
       for (uint32_t r = 0; r < kSortCtas; ++r) {
-        const uint32_t c = es_remote(total + threadIdx.x, r);
-        if (r < rank) before += c;
-        all += c;
+        if (r < rank) before += c[r];
+        all += c[r];
       }
       start[threadIdx.x] = all;
     }
@@ -111,9 +128,9 @@ embed_sort_kernel(const long long* __restrict__ ids, uint2* __restrict__ a, uint
     es_scan(start, bins, warp_total);
     if (threadIdx.x < bins) start[threadIdx.x] += before;
     __syncthreads();
-    for (long long i0 = lo; i0 < hi; i0 += 32) {
-      const bool has = i0 + lane < hi;
-      const uint2 p = has ? pair(i0 + lane) : make_uint2(0, 0);
+    for (int x = 0; x < steps; ++x) {
+      const bool has = lo + x * 32ll + lane < hi;
+      const uint2 p = at(x);
       const uint32_t d = has ? (p.x >> shift) & (bins - 1) : 0xffffffffu;
       const uint32_t same = __match_any_sync(0xffffffffu, d);
       if (has) dst[start[d] + mine[d] + __popc(same & ((1u << lane) - 1))] = p;
@@ -148,57 +165,63 @@ __device__ __forceinline__ void es_write(TO* __restrict__ p, const float (&acc)[
   }
 }
 
-// Pairs [L tile, L (tile + 1)) of the sorted ones, N columns a thread. `part` [tiles][2][D]: sums of a token that began before the tile, and of
-// one that begins in it and goes on behind it.
+// Pairs [L tile, L (tile + 1)) of the sorted ones (L a multiple of 32), N columns a thread. `part` [tiles][2][D]: sums of a token that began before the tile, and of
+// one that begins in it and goes on behind it. A lane holds one of 32 pairs, so that rows are asked for without waiting for their places.
 constexpr int kSumAhead = 8;            // rows under way at a time
 template <typename TI, typename TO, int N>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 embed_sum_kernel(const uint2* __restrict__ pairs, const TI* __restrict__ dy, long long rs, TO* __restrict__ out, float* __restrict__ part, int T,
                  int V, int D, int L, float scale) {
   pdl_launch_dependents();
   pdl_wait();
-  const int tile = blockIdx.x, col = (blockIdx.y * blockDim.x + threadIdx.x) * N;
+  const int tile = blockIdx.x, col = (blockIdx.y * blockDim.x + threadIdx.x) * N, lane = threadIdx.x & 31;
   const int lo = tile * L, hi = min(T, lo + L);
-  if (col >= D || pairs[lo].x >= uint32_t(V)) return;
-  const uint32_t before = lo > 0 ? pairs[lo - 1].x : 0xffffffffu, behind = hi < T ? pairs[hi].x : 0xffffffffu;
+  const bool has = col < D;
   uint32_t token = pairs[lo].x;
+  if (token >= uint32_t(V)) return;
+  const uint32_t before = lo > 0 ? pairs[lo - 1].x : 0xffffffffu, behind = hi < T ? pairs[hi].x : 0xffffffffu;
   bool inside = token != before;        // the token's pairs begin in this tile
   float acc[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
   auto done = [&](bool goes_on) {
+    if (!has) return;
     if (inside && !goes_on) { es_write<TO, N>(out + (long long)token * D + col, acc, scale); return; }
     float* p = part + ((long long)tile * 2 + inside) * D + col;
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = acc[i];
   };
-  for (int i0 = lo; i0 < hi; i0 += kSumAhead) {
-    alignas(16) TI raw[kSumAhead][N];
-    uint32_t tok[kSumAhead];
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const uint2 mine = i0 + lane < hi ? pairs[i0 + lane] : make_uint2(V, 0);
 #pragma unroll
-    for (int j = 0; j < kSumAhead; ++j) {
-      const uint2 p = i0 + j < hi ? pairs[i0 + j] : make_uint2(V, 0);
-      tok[j] = p.x;
-      const TI* src = dy + (long long)p.y * rs + col;
-      if (p.x < uint32_t(V)) {
-        if constexpr (N * sizeof(TI) == 16) *reinterpret_cast<uint4*>(raw[j]) = __ldg(reinterpret_cast<const uint4*>(src));
-        else
+    for (int b = 0; b < 32; b += kSumAhead) {
+      alignas(16) TI raw[kSumAhead][N];
+      uint32_t tok[kSumAhead];
 #pragma unroll
-          for (int i = 0; i < N; ++i) raw[j][i] = src[i];
-      }
-    }
+      for (int j = 0; j < kSumAhead; ++j) {
+        tok[j] = __shfl_sync(0xffffffffu, mine.x, b + j);
+        const uint32_t place = __shfl_sync(0xffffffffu, mine.y, b + j);
+        const TI* src = dy + (long long)place * rs + col;
+        if (has && tok[j] < uint32_t(V)) {
+          if constexpr (N * sizeof(TI) == 16) *reinterpret_cast<uint4*>(raw[j]) = __ldg(reinterpret_cast<const uint4*>(src));
+          else
 #pragma unroll
-    for (int j = 0; j < kSumAhead; ++j) {
-      if (tok[j] >= uint32_t(V)) break;
-      if (tok[j] != token) {
-        done(false);
-        token = tok[j];
-        inside = true;
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+            for (int i = 0; i < N; ++i) raw[j][i] = src[i];
+        }
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += to_f32<TI>(raw[j][i]);
+      for (int j = 0; j < kSumAhead; ++j) {
+        if (tok[j] >= uint32_t(V)) break;
+        if (tok[j] != token) {
+          done(false);
+          token = tok[j];
+          inside = true;
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += to_f32<TI>(raw[j][i]);
+      }
     }
   }
   done(token == behind);
@@ -239,8 +262,44 @@ embed_join_kernel(const uint2* __restrict__ pairs, TO* __restrict__ out, const f
   for (int i = 0; i < N; ++i) o[i] = from_f32<TO>(acc[i] * scale);
 }
 
-static int es_tile(long long T) {       // pairs of a CTA: 8, and more from 8192 tokens on, so that partial sums stay a small part of the work
-  long long L = kSumAhead;
+// Piece i of T tokens' `each` pieces: token i / each. 1024 pieces a CTA.
+template <typename T>
+__global__ void __launch_bounds__(256)
+embed_lookup_kernel(const long long* __restrict__ ids, const T* __restrict__ table, const T* __restrict__ pos, T* __restrict__ out, unsigned n, unsigned each,
+                    long long V, unsigned period, float scale) {
+  constexpr int N = 16 / sizeof(T), U = 4;
+  unsigned t[U], at[U];
+  long long id[U];
+  uint4 raw[U], p[U];
+#pragma unroll
+  for (int x = 0; x < U; ++x) {
+    const unsigned i = blockIdx.x * 1024u + x * 256u + threadIdx.x;
+    t[x] = i / each;
+    at[x] = i - t[x] * each;
+    id[x] = i < n ? ids[t[x]] : -1;
+    if (i >= n) t[x] = 0xffffffffu;
+  }
+#pragma unroll
+  for (int x = 0; x < U; ++x) {
+    raw[x] = id[x] >= 0 && id[x] < V ? __ldg(reinterpret_cast<const uint4*>(table) + id[x] * each + at[x]) : make_uint4(0, 0, 0, 0);
+    if (pos && t[x] != 0xffffffffu) p[x] = __ldg(reinterpret_cast<const uint4*>(pos) + (long long)(t[x] % period) * each + at[x]);
+  }
+#pragma unroll
+  for (int x = 0; x < U; ++x) {
+    if (t[x] == 0xffffffffu) continue;
+    alignas(16) T o[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float v = to_f32<T>(reinterpret_cast<const T*>(&raw[x])[j]) * scale;
+      if (pos) v += to_f32<T>(reinterpret_cast<const T*>(&p[x])[j]);
+      o[j] = from_f32<T>(v);
+    }
+    *(reinterpret_cast<uint4*>(out) + (long long)t[x] * each + at[x]) = *reinterpret_cast<uint4*>(o);
+  }
+}
+
+static int es_tile(long long T) {       // pairs of a CTA: 32, and more from 2^15 tokens on, so that partial sums stay a small part of the work (8 at 4096
+  long long L = 32;                     // tokens of 768 columns: sums 11 -> 8 us, joins 5 -> 12)
   while (L * 1024 < T) L *= 2;
   return int(L);
 }
@@ -252,6 +311,29 @@ static int es_bits(int V) {
 
 }  // namespace b200
 using namespace b200;
+
+B200_API int b200_embedding_lookup(const long long* ids, const void* table, const void* pos_table, void* out, long long T, int V, int D, int period, float scale,
+                                   int dtype, void* stream) {
+  const int N = dtype == B200_DT_FP32 ? 4 : 8;
+  if (T < 0 || V <= 0 || D <= 0 || D % N || (pos_table && period <= 0)) return B200_ERR_BAD_SHAPE;
+  if (((uintptr_t)table | (uintptr_t)out | (uintptr_t)pos_table) & 15) return B200_ERR_BAD_ALIGN;
+  cudaStream_t st = (cudaStream_t)stream;
+  const unsigned each = unsigned(D / N);
+  // pieces are counted in 32 bits: more tokens go in several launches, each with whole periods of positions
+  long long most = 0x7fff0000ll / each;
+  if (pos_table) most = most / period * period;
+  if (most < 1) return B200_ERR_TOO_LARGE;
+  for (long long t = 0; t < T; t += most) {
+    const unsigned n = unsigned((T - t < most ? T - t : most) * each), grid = (n + 1023) / 1024;
+#define ES_LOOKUP(TT) embed_lookup_kernel<TT><<<grid, 256, 0, st>>>(ids + t, (const TT*)table, (const TT*)pos_table, (TT*)out + t * D, n, each, V, unsigned(period), scale)
+    if (dtype == B200_DT_FP32) ES_LOOKUP(float);
+    else if (dtype == B200_DT_BF16) ES_LOOKUP(__nv_bfloat16);
+    else if (dtype == B200_DT_FP16) ES_LOOKUP(__half);
+    else return B200_ERR_UNSUPPORTED;
+  }
+  B200_LAUNCH_CHECK();
+  return 0;
+}
 
 B200_API long long b200_embedding_grad_workspace(long long T, int D) {
   if (T <= 0 || D <= 0) return 16;

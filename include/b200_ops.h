@@ -832,6 +832,10 @@ int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long
 /* y (16 bits) = x * scale[1] (scale NULL: x). */
 int b200_logprob_cast(const float* x, void* y, long long n, const float* scale, int dtype, void* stream);
 
+/* out [T, D] = table[ids] * scale (+ pos_table[t % period]) (csrc/embedding.cu): D a multiple of 16 bytes, V rows; a token outside 0 .. V - 1 gives zeros for its
+ * row of the table. */
+int b200_embedding_lookup(const long long* ids, const void* table, const void* pos_table, void* out, long long T, int V, int D, int period, float scale, int dtype,
+                          void* stream);
 /* Gradient of an embedding table by sorted tokens (csrc/embedding.cu): out [V, D] (dtype or fp32, 16-byte aligned) = scale * sum of dy[t] over ids[t] = row, in the
  * order of t, zeros elsewhere. dy [T, D] with row stride rs. Ids outside 0 .. V - 1 and `padding` (-1: none) add nothing. workspace: this many bytes, 16-byte
  * aligned, of this call alone while it runs. */

@@ -328,7 +328,7 @@ def _embedding_grad(flat, d2, rows, scale, padding_idx, dtype):
     return out
 
 
-_EMBEDDING_FWD = [vp, vp, vp, vp, i64, i32, i32, f32, i32, vp]
+_EMBEDDING_FWD = [vp, vp, vp, vp, i64, i32, i32, i32, f32, i32, vp]
 
 
 def _embedding_fwd(ids, table, pos_table, period, scale):
@@ -337,10 +337,11 @@ def _embedding_fwd(ids, table, pos_table, period, scale):
         flat = flat.to(torch.int64)
     out = table.new_empty((*ids.shape, table.shape[1]))
     if flat.numel():
-        rc = nv.call_on(table.device, nv.proto("b200_embedding_fwd", _EMBEDDING_FWD), flat.data_ptr(), table.data_ptr(), nv.ptr(pos_table), out.data_ptr(),
-                        flat.numel(), table.shape[1], period, scale, nv.dtype_code(table.dtype))
+        rows, D = table.shape
+        rc = nv.call_on(table.device, nv.proto("b200_embedding_lookup", _EMBEDDING_FWD), flat.data_ptr(), table.data_ptr(), nv.ptr(pos_table), out.data_ptr(),
+                        flat.numel(), rows, D, period, scale, nv.dtype_code(table.dtype))
         if rc:
-            nv.check(rc, "embedding_fwd")
+            nv.check(rc, "embedding_lookup")
         nv.count_launch()
     return flat, out
 
@@ -375,10 +376,13 @@ class _EmbeddingFn(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, pos_table: Optional[torch.Tensor] = None,
               scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``table[ids] * scale (+ pos_table[position])``; ids [..., L], position = index along the last dim. ``padding_idx``: a token
-    whose row gets no gradient."""
-    period = ids.shape[-1]
+    whose row gets no gradient. A token outside the table is an error on the CPU and a row of zeros (before positions) on a GPU."""
+    period = ids.shape[-1] if ids.dim() else 1
     vec = 4 if table.dtype == torch.float32 else 8
-    if nv.use_native(table) and table.shape[1] % vec == 0:
+    if pos_table is not None and pos_table.shape[0] < period:
+        raise ValueError(f"embedding: {period} positions, and the table has {pos_table.shape[0]}")
+    if (nv.use_native(table) and table.shape[1] % vec == 0 and table.is_contiguous()
+            and (pos_table is None or (pos_table.dtype == table.dtype and pos_table.is_contiguous()))):
         if torch.is_grad_enabled() and (table.requires_grad or (pos_table is not None and pos_table.requires_grad)):
             return _EmbeddingFn.apply(ids, table, pos_table, period, float(scale), padding_idx)
         return _embedding_fwd(ids, table, pos_table, period, float(scale))[1]

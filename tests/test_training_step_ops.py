@@ -348,6 +348,33 @@ def test_embedding_and_its_gradient(scale, device):
     assert torch.allclose(b, dout.sum(0), rtol=0, atol=1e-5)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("T,D", [(1, 8), (3, 64), (257, 40), (1025, 16), (300, 4096)])
+def test_embedding_lookup(T, D, dtype):
+    """Values are rounded to 32 bits and to the type; without a scale they are the table's. Tokens outside the table give zeros, ids of 32 bits and other shapes
+    are taken."""
+    dt = DT[dtype]
+    table, pos = torch.randn(77, D, device="cuda").to(dt), torch.randn(T, D, device="cuda").to(dt)
+    ids = torch.randint(0, 77, (T,), device="cuda")
+    for scale in (1.0, 3.7):
+        s32 = float(torch.tensor(scale))
+        for p in (None, pos):
+            want = table.double()[ids] * s32 + (0 if p is None else p.double())
+            half, least = half_step(dt)
+            # product and sum are one operation of 32 bits (2^-24 of the result), then the type's half step
+            assert ((embedding(ids, table, p, scale).double() - want).abs() <= (half + 2.0 ** -24) * want.abs() * (1 + 2.0 ** -20) + least).all()
+    assert torch.equal(embedding(ids, table), table[ids]) and torch.equal(embedding(ids, table, pos), (table.float()[ids] + pos.float()).to(dt))
+    assert torch.equal(embedding(ids.int(), table), table[ids]) and torch.equal(embedding(ids.view(1, 1, T), table), table[ids].view(1, 1, T, D))
+    bad = ids.clone()
+    bad[0], bad[-1] = -100, 77
+    y = embedding(bad, table)
+    assert not y[0].any() and not y[-1].any() and torch.equal(y[1:-1], table[ids[1:-1]])
+    assert embedding(ids[:0], table).shape == (0, D) and embedding(ids[0], table).shape == (D,)
+    wide = torch.randn(77, 2 * D, device="cuda").to(dt)
+    assert torch.equal(embedding(ids, wide[:, :D]), wide[:, :D][ids])
+
+
 def test_what_embedding_gradients_refuse():
     ids, d = torch.zeros(3, dtype=torch.int64), torch.randn(3, 4)
     for bad in (lambda: embedding_grad(ids.int(), d, 5), lambda: embedding_grad(ids[:2], d, 5), lambda: embedding_grad(ids, d.double(), 5), lambda: embedding_grad(ids, d, 0),
