@@ -586,10 +586,9 @@ lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, 
                  float* __restrict__ lp, float* __restrict__ ent, float4* __restrict__ stats) {
   __shared__ float4 red[32][8];
   const int r = threadIdx.x & 7, slice = threadIdx.x >> 3;
-  const long long row = blockIdx.x * 8ll + r;
   const float c = inv_t * kLog2e;
   LpSum a{-INFINITY, 0.f, 0.f};
-  if (row < rows) {
+  if (const long long row = blockIdx.x * 8ll + r; row < rows) {
     for (int i0 = slice; i0 < n; i0 += 32 * 8) {
       float4 x[8];
 #pragma unroll
@@ -600,8 +599,13 @@ lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, 
   }
   red[slice][r] = make_float4(a.m, a.s, a.u, 0.f);
   __syncthreads();
-  if (threadIdx.x >= 8 || row >= rows) return;
-  for (int i = 1; i < 32; ++i) a = lp_both<true>(a, {red[i][r].x, red[i][r].y, red[i][r].z}, c);
+  const float4 x = red[threadIdx.x & 31][threadIdx.x >> 5];              // a warp to each row
+  a = {x.x, x.y, x.z};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = lp_both<true>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
+  const long long row = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if ((threadIdx.x & 31) || row >= rows) return;
   const long long t = tokens ? tokens[row] : 0;
   const bool skip = t < 0 || t >= V;
   const float ls = logf(a.s), H = ls - kLn2 * a.u / a.s;

@@ -12,6 +12,7 @@ Reference: perplexities and answers scored in Quantization/LLM-Compressor/AWQ/ev
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import NamedTuple, Optional
 
@@ -22,6 +23,7 @@ from .gemm import gemm
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 MAX_TOP = 32             # alternatives of a row
+_HERE = contextlib.nullcontext()
 _ROWS_ARGS = [vp, i64, i64, i32, vp, f32, i32, vp, vp, vp, vp, vp, vp, i32, vp]
 _GRAD_ARGS = [vp, i64, i64, i32, vp, f32, vp, vp, vp, vp, i64, i32, vp]
 
@@ -200,6 +202,14 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 # ------------------------------------------------------------------------------------------------
 _CHUNK_BYTES = 128 << 20         # 16-bit gradients of logits that exist at a time in the backward pass
 _HEAD = [vp, i64, vp, i64, i32, i32, i32, i32, vp]
+_HEAD_SUMS = _HEAD + [f32, i32, vp, vp, vp]
+_HEAD_GRADS = _HEAD + [i32, i32, f32, vp, vp, vp, vp, vp, i64, vp]
+_FINISH = [vp, i32, i64, i32, vp, vp, f32, vp, vp, vp, vp]
+
+
+def _on(x: torch.Tensor):
+    """x's device as the current one; nothing to enter where it is."""
+    return _HERE if not x.is_cuda or x.device.index == torch._C._cuda_getDevice() else torch.cuda.device(x.device)
 
 
 def _chunks(T: int, V: int):
@@ -215,21 +225,23 @@ def _linear_forward(x, w, tokens, temperature, entropy, save):
     if not nv.use_native(x):
         lp, H, _, _, _, stats = _rows_torch(x.float() @ w.float().t(), tokens, temperature, 0, entropy, False)
         return lp, H, stats
-    lp = x.new_empty(T, dtype=torch.float32) if tokens is not None else None
-    H = x.new_empty(T, dtype=torch.float32) if entropy else None
-    stats = x.new_empty(T, 4, dtype=torch.float32) if save else None
+    new, dt = x.new_empty, torch.float32
+    lp, H, stats = new((T,), dtype=dt) if tokens is not None else None, new((T,), dtype=dt) if entropy else None, new((T, 4), dtype=dt) if save else None
     if T == 0:
         return lp, H, stats
     tiles = nv.proto("b200_gemm_head_tiles", [i32] * 3)(T, V, K)
     if tiles < 0:
         nv.check(-tiles, "gemm_head_tiles")
-    part = torch.empty(tiles, T, 4, dtype=torch.float32, device=x.device)
-    lt = torch.empty(T, dtype=torch.float32, device=x.device)
-    fn = nv.proto("b200_gemm_head_sums", _HEAD + [f32, i32, vp, vp, vp])
-    nv.check(fn(nv.ptr(x), x.stride(0), nv.ptr(w), w.stride(0), T, V, K, nv.dtype_code(x.dtype), nv.ptr(tokens), 1.0 / temperature, int(entropy), nv.ptr(part),
-                nv.ptr(lt), nv.stream()), "gemm_head_sums")
-    fin = nv.proto("b200_logprob_finish", [vp, i32, i64, i32, vp, vp, f32, vp, vp, vp, vp])
-    nv.check(fin(nv.ptr(part), tiles, T, V, nv.ptr(tokens), nv.ptr(lt), 1.0 / temperature, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), nv.stream()), "logprob_finish")
+    work = new((tiles * T * 4 + T,), dtype=dt)                           # sums of tiles, then the tokens' logits
+    part, inv_t, st, tok = work.data_ptr(), 1.0 / temperature, nv.stream(), nv.ptr(tokens)
+    lt = part + tiles * T * 16
+    rc = nv.proto("b200_gemm_head_sums", _HEAD_SUMS)(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), T, V, K, nv.dtype_code(x.dtype), tok, inv_t,
+                                                     int(entropy), part, lt, st)
+    if rc:
+        nv.check(rc, "gemm_head_sums")
+    rc = nv.proto("b200_logprob_finish", _FINISH)(part, tiles, T, V, tok, lt, inv_t, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), st)
+    if rc:
+        nv.check(rc, "logprob_finish")
     nv.count_launch(2)
     return lp, H, stats
 
@@ -257,7 +269,7 @@ def _linear_backward(x, w, tokens, temperature, stats, g, h, need_dx, need_dw):
     dx = torch.empty(T, K, dtype=x.dtype, device=dev) if need_dx else None
     direct = len(chunks) == 1 and not half                # one product gives dx: no sums in 32 bits between chunks
     acc = dx if direct else torch.empty(T, K, dtype=torch.float32, device=dev) if need_dx else None
-    fg = nv.proto("b200_gemm_head_grads", _HEAD + [i32, i32, f32, vp, vp, vp, vp, vp, i64, vp])
+    fg = nv.proto("b200_gemm_head_grads", _HEAD_GRADS)
     fc = nv.proto("b200_logprob_cast", [vp, vp, i64, vp, i32, vp])
     for c0, c1 in chunks:
         n, wc = c1 - c0, w[c0:c1]
@@ -281,7 +293,7 @@ class _LinearLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, tokens, temperature, entropy):
-        with torch.cuda.device_of(x):
+        with _on(x):
             lp, H, stats = _linear_forward(x, w, tokens, temperature, entropy, True)
         if w.requires_grad:
             from ..utils.arena import note_use
@@ -298,7 +310,7 @@ class _LinearLogprobsFn(torch.autograd.Function):
             return (None,) * 5
         x, w, tokens, stats = ctx.saved_tensors
         g, h = (None if t is None else t.to(torch.float32).contiguous() for t in (g, h))
-        with torch.cuda.device_of(x):
+        with _on(x):
             dx, dw = _linear_backward(x, w, tokens, ctx.temperature, stats, g, h, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dx, dw, None, None, None
 
@@ -307,24 +319,28 @@ def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[tor
     """``token_logprobs(x @ w.T, tokens)`` for hidden states ``x`` [..., K] and an output projection ``w`` [vocab, K] (bf16 or fp16, K a multiple of 8),
     without the logits: their sums are taken from the product's accumulators (fp32), and in the backward pass, where the product is computed again, their
     gradients, which exist in 16 bits a chunk of the vocabulary at a time. Gradients for ``x`` and ``w``."""
-    if w.dim() != 2 or w.shape[0] < 1 or x.dim() < 1 or x.shape[-1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
+    shape, native = x.shape, nv.use_native(x)
+    if w.dim() != 2 or w.shape[0] < 1 or not shape or shape[-1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
         raise ValueError("linear_token_logprobs: x [..., K] and w [vocab, K] must agree in K, type and device")
-    if x.dtype not in ((torch.bfloat16, torch.float16) if nv.use_native(x) else (torch.bfloat16, torch.float16, torch.float32)):
+    if x.dtype not in (_TYPES[1:] if native else _TYPES):
         raise TypeError(f"linear_token_logprobs: x and w must be bf16 or fp16, not {x.dtype}; token_logprobs takes logits of 32 bits")
-    if nv.use_native(x) and (x.shape[-1] % 8 or w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16):
+    if native and (shape[-1] % 8 or w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16):
         raise ValueError("linear_token_logprobs: rows of w must be contiguous, start at multiples of 16 bytes and have a multiple of 8 values")
+    shape = shape[:-1]
     if tokens is not None:
-        _check("linear_token_logprobs", tokens, x.shape[:-1], x.device)
+        _check("linear_token_logprobs", tokens, shape, x.device)
     _check_temperature("linear_token_logprobs", temperature)
     if tokens is None and not entropy:
         raise ValueError("linear_token_logprobs: without tokens there are entropies only")
-    shape, rows = x.shape[:-1], _as_rows(x)
-    if nv.use_native(rows) and (rows.data_ptr() % 16 or rows.stride(0) % 8):
+    rows = _as_rows(x)
+    if native and (rows.data_ptr() % 16 or rows.stride(0) % 8):
         rows = rows.contiguous() if rows.stride(0) % 8 else rows.clone()
     flat = None if tokens is None else tokens.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         lp, H = _LinearLogprobsFn.apply(rows, w, flat, temperature, entropy)
     else:
-        with torch.cuda.device_of(rows):
+        with _on(rows):
             lp, H, _ = _linear_forward(rows, w, flat, temperature, entropy, False)
+    if len(shape) == 1:
+        return TokenLogprobs(lp, H)
     return TokenLogprobs(None if lp is None else lp.view(shape), None if H is None else H.view(shape))
