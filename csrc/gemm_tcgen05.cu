@@ -106,17 +106,21 @@ struct W4Params {
 // Epilogues of an output projection whose result, fp32 logits, is not stored (ops/logprobs.py). A row of the accumulator is one thread's, so what
 // it needs of a row stays in that thread.
 //   kHeadSums   the 256 logits of a row and tile become (m, s, u) of logprob_math.cuh in part[tile column][row]; the given token's logit goes to lt[row]
-//   kHeadGrads  a logit becomes its gradient, which is stored in 16 bits as D
-enum { kHeadNone = 0, kHeadSums = 1, kHeadGrads = 2 };
+//   kHeadGrads  a logit becomes its gradient, which is stored in 16 bits as D; rows behind the last of `active` become zeros
+//   kHeadRows, kHeadDepth   plain products whose rows, or whose depth, end where `active` says
+// Tokens that are passed over cost nothing so: the others' rows stand first, and how many they are the host need not know.
+enum { kHeadNone = 0, kHeadSums = 1, kHeadGrads = 2, kHeadRows = 3, kHeadDepth = 4 };
 struct HeadParams {
+  const int* active;         // how many of the M rows (kHeadDepth: of K) count, at least 1; null: all
+  const int* rows;           // [M] which of the caller's rows each is, for stats, g and h; null: the same
   const long long* tokens;   // [M] or null
   int V, c0;                 // the vocabulary; the first column of this product in it
   float inv_t;
   int entropy;
   float4* part;              // [num_n][M]
   float* lt;                 // [M]
-  const float4* stats;       // [M] (m, 1 / s, log s, H)
-  const float *g, *h;        // [M] or null
+  const float4* stats;       // (m, 1 / s, log s, H) by the caller's rows
+  const float *g, *h;        // the same, or null
   const float* scale;        // scale[0] times the gradient, or null
 };
 
@@ -432,6 +436,10 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
                                           const CUtensorMap& tmB2, const GemmKernelParams& p, const W4Params* w4, const HeadParams* head = nullptr) {
   constexpr int EPR = 128 / ES;  // elements per 128-byte swizzle row = k-block depth
   constexpr int UK = 32 / ES;    // elements per UMMA k-step
+  // the rows, or for kHeadDepth the depth, of a product that ends at a count which is on the device
+  const int live = HEAD != kHeadNone && head->active ? *head->active : HEAD == kHeadDepth ? p.K : p.M;
+  const int num_m = HEAD == kHeadNone || HEAD == kHeadDepth ? p.num_m : (live + kBM * CTAS - 1) / (kBM * CTAS);
+  const int num_k = HEAD == kHeadDepth ? (live + EPR - 1) / EPR : p.num_k;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -527,9 +535,9 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     else asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(unit), "=r"(sk_epoch_v) : "r"(mapa_shared(sk_unit_slot, 0)) : "memory");
   }
 
-  const int tiles_per_batch = p.num_m * p.num_n;
+  const int tiles_per_batch = num_m * p.num_n;
   const int total_tiles = tiles_per_batch * p.batch;
-  const int num_k_total = p.num_k + (p.K2 > 0 ? 1 : 0);
+  const int num_k_total = num_k + (p.K2 > 0 ? 1 : 0);
 
   // ================= TMA producers (every CTA: its own rows of A and its share of B) =========
   // A warp for each operand: one warp for both took 90 cycles to see that a stage is free, 200 for A's box and 120 to 180 for each box of B, 530 a
@@ -553,8 +561,8 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const int tile = sg.tile;
       const int bt = tile / tiles_per_batch;
       const int rem = tile - bt * tiles_per_batch;
-      const int n_blk = rem / p.num_m;
-      const int m_blk = rem - n_blk * p.num_m;
+      const int n_blk = rem / num_m;
+      const int m_blk = rem - n_blk * num_m;
       const int m0 = m_blk * (kBM * CTAS) + (int)rank * kBM;
       const int n0 = n_blk * p.bn + (int)rank * bn_cta;
       const int ab0 = bt % p.nb0, ab1 = bt / p.nb0;
@@ -569,8 +577,8 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         const uint32_t sb = sB0 + (uint32_t)stage * stage_b_bytes;
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         free = mbar_test_wait(empty_bar(stage), phase ^ 1u);
-        if (A && leader) mbar_expect_tx_elected(fb, (W4 && kb < p.num_k) ? tx_a_only : tx_full);
-        if (kb < p.num_k) {
+        if (A && leader) mbar_expect_tx_elected(fb, (W4 && kb < num_k) ? tx_a_only : tx_full);
+        if (kb < num_k) {
           const int k0 = kb * EPR;
           if constexpr (A) {
             if (!p.a_mn) {
@@ -638,7 +646,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           const int cur = stage;
           if (++stage == p.stages) { stage = 0; phase ^= 1u; }
           full = mbar_test_wait(full_bar(stage), phase);
-          if (kb < p.num_k) {
+          if (kb < num_k) {
             const uint32_t a_lo = a_lo_main + (uint32_t)cur * a_stage16;
             const uint32_t b_lo = b_lo_main + (uint32_t)cur * b_stage16;
             umma_kblock<ES, CTAS>(d_tmem, desc(a_lo), desc(b_lo), p.idesc_main, kb != sg.kb0 ? 1u : 0u, a_step_main, b_step_main);
@@ -667,9 +675,9 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       Segment sg;
       while (it.next(sg)) {
         const int rem = sg.tile % tiles_per_batch;
-        const int n_blk = rem / p.num_m;
+        const int n_blk = rem / num_m;
         const int n0 = n_blk * p.bn + (int)rank * bn_cta;
-        for (int kb = sg.kb0; kb < sg.kb1 && kb < p.num_k; ++kb) {
+        for (int kb = sg.kb0; kb < sg.kb1 && kb < num_k; ++kb) {
           mbar_wait(rempty_bar(rs), rphase ^ 1u);
           if (W4DBG(32)) {   // timing experiment: no packed-tile traffic
             mbar_arrive(rfull_bar(rs));
@@ -703,7 +711,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       Segment sg;
       while (it.next(sg)) {
         const int rem = sg.tile % tiles_per_batch;
-        const int n_blk = rem / p.num_m;
+        const int n_blk = rem / num_m;
         const int n0 = n_blk * p.bn + (int)rank * bn_cta;
         // K-major: B row n0 + t/2, k half t&1 of the block. MN-major: k row t/4, column half (t>>1)&1, 32-column part t&1.
         const int r_loc = p.b_mn ? (t >> 2) : (t >> 1);
@@ -731,13 +739,13 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
         float scq[3] = {0.f, 0.f, 0.f}, zsq[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-          if (sg.kb0 + j < sg.kb1 && sg.kb0 + j < p.num_k) scale_at(sg.kb0 + j, scq[j], zsq[j]);
+          if (sg.kb0 + j < sg.kb1 && sg.kb0 + j < num_k) scale_at(sg.kb0 + j, scq[j], zsq[j]);
         for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
           const uint32_t fb_local = full_bar(stage);
-          if (kb < p.num_k) {
+          if (kb < num_k) {
             const float sc = scq[0], zs = zsq[0];
             scq[0] = scq[1]; scq[1] = scq[2]; zsq[0] = zsq[1]; zsq[1] = zsq[2];
-            if (kb + 3 < sg.kb1 && kb + 3 < p.num_k) scale_at(kb + 3, scq[2], zsq[2]);
+            if (kb + 3 < sg.kb1 && kb + 3 < num_k) scale_at(kb + 3, scq[2], zsq[2]);
             uint32_t sc2, nz2;
             if (w4->is_bf16) { sc2 = pack_bf16x2(sc, sc); nz2 = pack_bf16x2(-zs, -zs); }
             else {
@@ -823,8 +831,8 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const int tile = sg.tile;
       const int bt = tile / tiles_per_batch;
       const int rem = tile - bt * tiles_per_batch;
-      const int n_blk = rem / p.num_m;
-      const int m_blk = rem - n_blk * p.num_m;
+      const int n_blk = rem / num_m;
+      const int m_blk = rem - n_blk * num_m;
       const int m0 = m_blk * (kBM * CTAS) + (int)rank * kBM, n0 = n_blk * p.bn;
       const int ab0 = bt % p.nb0, ab1 = bt / p.nb0;
       const int bsel = p.b_map ? p.b_map[bt] : 0;
@@ -834,22 +842,25 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       __syncwarp();                                  // each lane has looked for itself, tcgen05.ld takes them together
       tc_fence_after();
       const int row = m0 + q * 32 + lane;
-      const bool row_ok = row < p.M;
+      const bool row_ok = row < (HEAD == kHeadRows ? live : p.M);
       const long long doff = (long long)ab0 * p.d_bs0 + (long long)ab1 * p.d_bs1 + (long long)row * p.d_rs;
       const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * kAccStride;
       const int col_limit = min(p.N, n0 + p.bn);
       const int nchunks = (p.bn + 31) / 32;
       const float beta = (p.beta_rows != nullptr && row_ok) ? p.beta_rows[row] : p.beta;
-      if constexpr (HEAD != kHeadNone) {
+      if constexpr (HEAD == kHeadSums || HEAD == kHeadGrads) {
         // ---- whole tiles of logits: sums or gradients of this thread's row ----
         const float c2 = head->inv_t * kLog2e;
-        const long long t = row_ok && head->tokens ? head->tokens[row] : -1;
-        const bool skip = !row_ok || (head->tokens && (t < 0 || t >= head->V));
+        const bool lives = row < live;
+        const long long t = lives && head->tokens ? head->tokens[row] : -1;
+        const bool skip = !lives || (head->tokens && (t < 0 || t >= head->V));
         const long long at = t - head->c0;                       // the token's column, if it is in this product
         LpSum sum{-INFINITY, 0.f, 0.f};
         LpGrad grad{};
-        if (HEAD == kHeadGrads && !skip)
-          grad = lp_grad_of(head->stats[row], head->g ? head->g[row] : 0.f, head->h ? head->h[row] : 0.f, head->inv_t, at, head->scale ? head->scale[0] : 1.f);
+        if (HEAD == kHeadGrads && !skip) {
+          const int from = head->rows ? head->rows[row] : row;
+          grad = lp_grad_of(head->stats[from], head->g ? head->g[from] : 0.f, head->h ? head->h[from] : 0.f, head->inv_t, at, head->scale ? head->scale[0] : 1.f);
+        }
         for (int c = 0; c < nchunks; ++c) {
           const int col0 = n0 + c * 32;
           if (col0 >= col_limit) break;
@@ -1385,47 +1396,45 @@ static int launch_head(const CUtensorMap& tmA, const CUtensorMap& tmB, const Hea
 
 static GemmConfig head_config(int M, int N, int K) { return pick_config(M, N, 1, ceil_div(K, 64), 0, 64, g_num_sms, false); }
 
-static int gemm_head(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, void* out, long long out_rs, HeadParams h, int mode,
-                     cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0) return B200_ERR_BAD_SHAPE;
-  if (dtype != B200_DT_BF16 && dtype != B200_DT_FP16) return B200_ERR_UNSUPPORTED;
-  if (((uintptr_t)x | (uintptr_t)w) & 15 || x_rs % 8 || w_rs % 8) return B200_ERR_BAD_ALIGN;
+struct HeadOperands { const void *a, *b; long long a_rs, b_rs; int a_mn, b_mn, M, N, K, dtype; void* out; long long out_rs; int out_dtype; float beta; };
+
+static int gemm_head(const HeadOperands& o, HeadParams h, int mode, cudaStream_t stream) {
+  if (o.M <= 0 || o.N <= 0 || o.K <= 0) return B200_ERR_BAD_SHAPE;
+  if (o.dtype != B200_DT_BF16 && o.dtype != B200_DT_FP16) return B200_ERR_UNSUPPORTED;
+  if (((uintptr_t)o.a | (uintptr_t)o.b) & 15 || o.a_rs % 8 || o.b_rs % 8) return B200_ERR_BAD_ALIGN;
   int rc = device_props();
   if (rc) return rc;
-  const GemmConfig cfg = head_config(M, N, K);
+  const GemmConfig cfg = pick_config(o.M, o.N, 1, ceil_div(o.K, 64), o.b_mn, 64, g_num_sms, false);
   const int ctas = cfg.ctas, bn_cta = cfg.bn / ctas;
   GemmKernelParams p = {};
-  p.D = out; p.M = M; p.N = N; p.K = K; p.batch = p.nb0 = p.b_div = p.nb0_b = 1;
-  p.d_rs = out_rs; p.alpha = 1.f; p.out_dtype = dtype;
-  p.num_k = ceil_div(K, 64); p.bn = cfg.bn; p.sk_group = 1;
-  p.num_m = ceil_div(M, kBM * ctas); p.num_n = ceil_div(N, p.bn);
+  p.D = o.out; p.M = o.M; p.N = o.N; p.K = o.K; p.batch = p.nb0 = p.b_div = p.nb0_b = 1;
+  p.d_rs = o.out_rs; p.alpha = 1.f; p.beta = o.beta; p.out_dtype = o.out_dtype;
+  p.a_mn = o.a_mn; p.b_mn = o.b_mn;
+  p.num_k = ceil_div(o.K, 64); p.bn = cfg.bn; p.sk_group = 1;
+  p.num_m = ceil_div(o.M, kBM * ctas); p.num_n = ceil_div(o.N, p.bn);
   const int stage_bytes = kStageABytes + bn_cta * 128;
   p.stages = (g_max_smem - 2048) / stage_bytes;
   if (p.stages > 6) p.stages = 6;
   if (p.stages < 2) return B200_ERR_UNSUPPORTED;
-  const uint32_t fmt = dtype == B200_DT_BF16 ? 1u : 0u;
-  p.idesc_main = p.idesc_lora = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM * ctas >> 4) << 24);
-  p.vec_ok = out && ((uintptr_t)out & 15) == 0 && out_rs % 8 == 0;
+  const uint32_t fmt = o.dtype == B200_DT_BF16 ? 1u : 0u;
+  p.idesc_lora = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM * ctas >> 4) << 24);
+  p.idesc_main = p.idesc_lora | ((uint32_t)o.a_mn << 15) | ((uint32_t)o.b_mn << 16);
+  p.vec_ok = o.out && ((uintptr_t)o.out & 15) == 0 && o.out_rs % (o.out_dtype == B200_DT_FP32 ? 4 : 8) == 0;
   CUtensorMap tmA, tmB;
-  {
-    uint64_t dims[4] = {(uint64_t)K, (uint64_t)M, 1, 1}, str[3] = {(uint64_t)x_rs * 2, 0, 0};
-    uint32_t box[4] = {64, kBM, 1, 1};
-    rc = make_tensor_map(&tmA, x, 2, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-  }
-  {
-    uint64_t dims[4] = {(uint64_t)K, (uint64_t)N, 1, 1}, str[3] = {(uint64_t)w_rs * 2, 0, 0};
-    uint32_t box[4] = {64, (uint32_t)bn_cta, 1, 1};
-    rc = make_tensor_map(&tmB, w, 2, 4, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-  }
+  const uint64_t str[3] = {(uint64_t)o.a_rs * 2, 0, 0}, strb[3] = {(uint64_t)o.b_rs * 2, 0, 0};
+  const uint64_t da[4] = {(uint64_t)(o.a_mn ? o.M : o.K), (uint64_t)(o.a_mn ? o.K : o.M), 1, 1}, db[4] = {(uint64_t)(o.b_mn ? o.N : o.K), (uint64_t)(o.b_mn ? o.K : o.N), 1, 1};
+  const uint32_t ba[4] = {64, o.a_mn ? 64u : (uint32_t)kBM, 1, 1}, bb[4] = {64, o.b_mn ? 64u : (uint32_t)bn_cta, 1, 1};
+  rc = make_tensor_map(&tmA, o.a, 2, 4, da, str, ba, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  rc = make_tensor_map(&tmB, o.b, 2, 4, db, strb, bb, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
   const int units = g_num_sms / ctas;
   const long long tiles = (long long)p.num_m * p.num_n;
   if (tiles > 0x7fffffff) return B200_ERR_TOO_LARGE;
   const int grid = (int)(tiles < units ? tiles : units) * ctas;
   const int smem = p.stages * stage_bytes + 8 * (2 * p.stages + 6) + 1024;
-  if (mode == kHeadSums) rc = ctas == 2 ? launch_head<2, kHeadSums>(tmA, tmB, h, p, grid, smem, stream) : launch_head<1, kHeadSums>(tmA, tmB, h, p, grid, smem, stream);
-  else rc = ctas == 2 ? launch_head<2, kHeadGrads>(tmA, tmB, h, p, grid, smem, stream) : launch_head<1, kHeadGrads>(tmA, tmB, h, p, grid, smem, stream);
+#define HEAD_LAUNCH(MODE) (ctas == 2 ? launch_head<2, MODE>(tmA, tmB, h, p, grid, smem, stream) : launch_head<1, MODE>(tmA, tmB, h, p, grid, smem, stream))
+  rc = mode == kHeadSums ? HEAD_LAUNCH(kHeadSums) : mode == kHeadGrads ? HEAD_LAUNCH(kHeadGrads) : mode == kHeadRows ? HEAD_LAUNCH(kHeadRows) : HEAD_LAUNCH(kHeadDepth);
   if (rc) return rc;
   B200_LAUNCH_CHECK();
   return 0;
@@ -1439,18 +1448,28 @@ B200_API int b200_gemm_head_tiles(int M, int N, int K) {
   return ceil_div(N, head_config(M, N, K).bn);
 }
 
-B200_API int b200_gemm_head_sums(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, float inv_t,
-                                 int entropy, void* part, float* lt, void* stream) {
+B200_API int b200_gemm_head_sums(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const int* active, const long long* tokens,
+                                 float inv_t, int entropy, void* part, float* lt, void* stream) {
   HeadParams h = {};
-  h.tokens = tokens; h.V = N; h.inv_t = inv_t; h.entropy = entropy; h.part = (float4*)part; h.lt = lt;
-  return gemm_head(x, x_rs, w, w_rs, M, N, K, dtype, nullptr, 0, h, kHeadSums, (cudaStream_t)stream);
+  h.active = active; h.tokens = tokens; h.V = N; h.inv_t = inv_t; h.entropy = entropy; h.part = (float4*)part; h.lt = lt;
+  return gemm_head({x, w, x_rs, w_rs, 0, 0, M, N, K, dtype, nullptr, 0, dtype, 0.f}, h, kHeadSums, (cudaStream_t)stream);
 }
 
-B200_API int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, int V, int c0,
-                                  float inv_t, const void* stats, const float* g, const float* h, const float* scale, void* out, long long out_rs, void* stream) {
+B200_API int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const int* active, const int* rows,
+                                  const long long* tokens, int V, int c0, float inv_t, const void* stats, const float* g, const float* h, const float* scale, void* out,
+                                  long long out_rs, void* stream) {
   HeadParams hp = {};
+  hp.active = active; hp.rows = rows;
   hp.tokens = tokens; hp.V = V; hp.c0 = c0; hp.inv_t = inv_t; hp.stats = (const float4*)stats; hp.g = g; hp.h = h; hp.scale = scale;
-  return gemm_head(x, x_rs, w, w_rs, M, N, K, dtype, out, out_rs, hp, kHeadGrads, (cudaStream_t)stream);
+  return gemm_head({x, w, x_rs, w_rs, 0, 0, M, N, K, dtype, out, out_rs, dtype, 0.f}, hp, kHeadGrads, (cudaStream_t)stream);
+}
+
+B200_API int b200_gemm_active(const void* a, long long a_rs, int a_mn, const void* b, long long b_rs, int b_mn, int M, int N, int K, int dtype, const int* active,
+                              int depth, void* out, long long out_rs, int out_dtype, float beta, void* stream) {
+  if (!active) return B200_ERR_BAD_SHAPE;
+  HeadParams h = {};
+  h.active = active;
+  return gemm_head({a, b, a_rs, b_rs, a_mn ? 1 : 0, b_mn ? 1 : 0, M, N, K, dtype, out, out_rs, out_dtype, beta}, h, depth ? kHeadDepth : kHeadRows, (cudaStream_t)stream);
 }
 
 B200_API int b200_gemm_w4(const b200_gemm_args* a, const b200_w4_desc* w, void* stream_) {

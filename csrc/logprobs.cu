@@ -12,6 +12,7 @@
 //   lp_rows_grad   logits, (m, 1 / s, log s, H), g, h -> dl, in one pass
 // and for logits x w^T that are never stored (gemm_tcgen05.cu: sums and gradients in the epilogues of the product):
 //   lp_finish      lp, H and what the backward pass needs, from the sums of a row's tiles
+//   lp_active, lp_gather, lp_return   rows whose tokens are not passed over, side by side, and their gradients back where they belong
 //   lp_scale, lp_cast   a power of two for fp16's gradients of single logits, and back
 // Rows of logits are bound by HBM; a 16-bit logit has eight operations beside its exponential.
 #include "logprob_math.cuh"
@@ -582,13 +583,16 @@ lp_rows_grad_kernel(const T* __restrict__ logits, long long rs, int V, int slice
 // part [n][rows] = (m, s, u) of n parts of each row, lt [rows] its token's logit. 8 rows a CTA, 32 threads a row (32 rows a CTA and 8 threads a row took
 // 41 us of 2048 x 594 parts, the loads' latency).
 __global__ void __launch_bounds__(256)
-lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, const long long* __restrict__ tokens, const float* __restrict__ lt, float inv_t,
-                 float* __restrict__ lp, float* __restrict__ ent, float4* __restrict__ stats) {
+lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, const int* __restrict__ active, const int* __restrict__ from,
+                 const long long* __restrict__ tokens, const float* __restrict__ lt, float inv_t, float* __restrict__ lp, float* __restrict__ ent,
+                 float4* __restrict__ stats) {
   __shared__ float4 red[32][8];
   const int r = threadIdx.x & 7, slice = threadIdx.x >> 3;
   const float c = inv_t * kLog2e;
   LpSum a{-INFINITY, 0.f, 0.f};
-  if (const long long row = blockIdx.x * 8ll + r; row < rows) {
+  const long long live = active ? *active : rows;
+  if (blockIdx.x * 8ll >= live) return;
+  if (const long long row = blockIdx.x * 8ll + r; row < live) {
     for (int i0 = slice; i0 < n; i0 += 32 * 8) {
       float4 x[8];
 #pragma unroll
@@ -605,27 +609,107 @@ lp_finish_kernel(const float4* __restrict__ part, int n, long long rows, int V, 
   for (int o = 16; o > 0; o >>= 1)
     a = lp_both<true>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
   const long long row = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  if ((threadIdx.x & 31) || row >= rows) return;
-  const long long t = tokens ? tokens[row] : 0;
+  if ((threadIdx.x & 31) || row >= live) return;
+  const long long t = tokens ? tokens[row] : 0, to = from ? from[row] : row;
   const bool skip = t < 0 || t >= V;
   const float ls = logf(a.s), H = ls - kLn2 * a.u / a.s;
-  if (lp) lp[row] = skip ? 0.f : (lt[row] - a.m) * inv_t - ls;
-  if (ent) ent[row] = skip ? 0.f : H;
-  if (stats) stats[row] = make_float4(a.m, 1.f / a.s, ls, H);
+  if (lp) lp[to] = skip ? 0.f : (lt[row] - a.m) * inv_t - ls;
+  if (ent) ent[to] = skip ? 0.f : H;
+  if (stats) stats[to] = make_float4(a.m, 1.f / a.s, ls, H);
 }
 
 // A power of two that brings the largest gradient of a logit to 2^13 .. 2^14, so that fp16 holds the small ones too, and its reciprocal.
 // |dl| <= (|g| + |h| (log V + 1)) / T.
 __global__ void __launch_bounds__(256)
-lp_scale_kernel(const float* __restrict__ g, const float* __restrict__ h, long long rows, float inv_t, float log_v, float* __restrict__ scale) {
+lp_scale_kernel(const float* __restrict__ g, const float* __restrict__ h, const long long* __restrict__ tokens, long long rows, int V, float inv_t,
+                float log_v, float* __restrict__ scale) {
   __shared__ float red[32];
   float m = 0.f;
-  for (long long i = threadIdx.x; i < rows; i += 256) m = fmaxf(m, ((g ? fabsf(g[i]) : 0.f) + (h ? fabsf(h[i]) : 0.f) * (log_v + 1.f)) * inv_t);
+  for (long long i = threadIdx.x; i < rows; i += 256)
+    if (!tokens || (tokens[i] >= 0 && tokens[i] < V)) m = fmaxf(m, ((g ? fabsf(g[i]) : 0.f) + (h ? fabsf(h[i]) : 0.f) * (log_v + 1.f)) * inv_t);
   m = block_max(m, red);
   if (threadIdx.x) return;
   const int e = m > 0.f && m < INFINITY ? min(max(14 - (ilogbf(m) + 1), -100), 100) : 0;
   scale[0] = ldexpf(1.f, e);
   scale[1] = ldexpf(1.f, -e);
+}
+
+// The rows whose tokens are not passed over, in order: from[i] is the i-th of them, place[t] where row t went (-1: passed over), mine[i] its token, *active how
+// many (at least one: of tokens that are all passed over the first one stands for itself, as a token of -1). Rows that are passed over get their zeros here. One CTA.
+__global__ void __launch_bounds__(1024)
+lp_active_kernel(const long long* __restrict__ tokens, int rows, int V, int* __restrict__ from, int* __restrict__ place, long long* __restrict__ mine,
+                 int* __restrict__ active, float* __restrict__ lp, float* __restrict__ ent) {
+  __shared__ int warps[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int base = 0;
+  for (int r0 = 0; r0 < rows; r0 += 4096) {
+    long long t[4];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = r0 + threadIdx.x * 4 + j;
+      t[j] = r < rows ? tokens[r] : -1;
+      n += t[j] >= 0 && t[j] < V;
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    if (lane == 31) warps[w] = sum;
+    __syncthreads();
+    int own = lane < w ? warps[lane] : 0;
+    const int before = __reduce_add_sync(0xffffffffu, own), all = __reduce_add_sync(0xffffffffu, warps[lane]);
+    int at = base + before + sum - n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = r0 + threadIdx.x * 4 + j;
+      if (r >= rows) break;
+      if (t[j] >= 0 && t[j] < V) {
+        from[at] = r;
+        mine[at] = t[j];
+        place[r] = at++;
+      } else {
+        place[r] = -1;
+        if (lp) lp[r] = 0.f;
+        if (ent) ent[r] = 0.f;
+      }
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    *active = base > 0 ? base : 1;
+    if (base == 0) { from[0] = 0; mine[0] = -1; }
+  }
+}
+
+// Those rows of x, and zeros up to the next multiple of 256 rows: what stands in one k-block or tile with them. (The row that stands for itself is zeros,
+// too.)
+__global__ void __launch_bounds__(128)
+lp_gather_kernel(const uint4* __restrict__ x, long long rs, int vecs, int rows, const int* __restrict__ from, const long long* __restrict__ mine,
+                 const int* __restrict__ active, uint4* __restrict__ out) {
+  const int r = blockIdx.x, live = *active;
+  if (r >= min(rows, (live + 255) / 256 * 256)) return;
+  const bool has = r < live && mine[r] >= 0;
+  const uint4* p = x + (has ? from[r] : 0) * rs;
+  for (int i = threadIdx.x; i < vecs; i += 128) out[(long long)r * vecs + i] = has ? __ldg(p + i) : make_uint4(0, 0, 0, 0);
+}
+
+// y[t] = x[place[t]] * scale[1], zeros for rows that were passed over.
+template <typename TI, typename T>
+__global__ void __launch_bounds__(256)
+lp_return_kernel(const TI* __restrict__ x, T* __restrict__ y, int K, const int* __restrict__ place, const float* __restrict__ scale) {
+  const int at = place[blockIdx.x];
+  const float f = scale ? scale[1] : 1.f;
+  for (int k = threadIdx.x * 4; k < K; k += 1024) {                      // K is a multiple of 8
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = at < 0 ? 0.f : to_f32<TI>(x[(long long)at * K + k + j]) * f;
+    alignas(8) T r[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+    *reinterpret_cast<uint2*>(y + (long long)blockIdx.x * K + k) = *reinterpret_cast<uint2*>(r);
+  }
 }
 
 // y = x * scale[1] in the type of the gradients.
@@ -717,18 +801,43 @@ B200_API int b200_token_logprobs_grad(const void* logits, long long rs, long lon
   return 0;
 }
 
-B200_API int b200_logprob_finish(const void* part, int parts, long long rows, int V, const long long* tokens, const float* lt, float inv_t, float* lp, float* ent,
-                                 void* stats, void* stream) {
+B200_API int b200_logprob_finish(const void* part, int parts, long long rows, int V, const int* active, const int* from, const long long* tokens, const float* lt,
+                                 float inv_t, float* lp, float* ent, void* stats, void* stream) {
   if (lp_bad(rows, V) || parts < 1) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
-  lp_finish_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, (cudaStream_t)stream>>>((const float4*)part, parts, rows, V, tokens, lt, inv_t, lp, ent, (float4*)stats);
+  lp_finish_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, (cudaStream_t)stream>>>((const float4*)part, parts, rows, V, active, from, tokens, lt, inv_t, lp, ent,
+                                                                                (float4*)stats);
   B200_LAUNCH_CHECK();
   return 0;
 }
 
-B200_API int b200_logprob_scale(const float* g, const float* h, long long rows, float inv_t, int V, float* scale, void* stream) {
+B200_API int b200_logprob_active(const long long* tokens, const void* x, long long x_rs, int rows, int K, int V, int* from, int* place, long long* mine, int* active,
+                                 float* lp, float* ent, void* out, void* stream) {
+  if (rows <= 0 || V <= 0 || K <= 0 || K % 8) return B200_ERR_BAD_SHAPE;
+  if (((uintptr_t)x | (uintptr_t)out) & 15 || x_rs % 8) return B200_ERR_BAD_ALIGN;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (tokens) lp_active_kernel<<<1, 1024, 0, st>>>(tokens, rows, V, from, place, mine, active, lp, ent);      // null: the maps are there already
+  lp_gather_kernel<<<rows, 128, 0, st>>>((const uint4*)x, x_rs / 8, K / 8, rows, from, mine, active, (uint4*)out);
+  B200_LAUNCH_CHECK();
+  return 0;
+}
+
+B200_API int b200_logprob_return(const void* x, int x_dtype, void* y, int rows, int K, const int* place, const float* scale, int dtype, void* stream) {
+  if (rows <= 0 || K <= 0 || K % 8) return B200_ERR_BAD_SHAPE;
+  if (((uintptr_t)x | (uintptr_t)y) & 15) return B200_ERR_BAD_ALIGN;
+  if (x_dtype != dtype && x_dtype != B200_DT_FP32) return B200_ERR_UNSUPPORTED;
+  cudaStream_t st = (cudaStream_t)stream;
+  LP_TYPES16(dtype, {
+    if (x_dtype == B200_DT_FP32) lp_return_kernel<float, T><<<rows, 256, 0, st>>>((const float*)x, (T*)y, K, place, scale);
+    else lp_return_kernel<T, T><<<rows, 256, 0, st>>>((const T*)x, (T*)y, K, place, scale);
+  });
+  B200_LAUNCH_CHECK();
+  return 0;
+}
+
+B200_API int b200_logprob_scale(const float* g, const float* h, const long long* tokens, long long rows, float inv_t, int V, float* scale, void* stream) {
   if (lp_bad(rows, V)) return B200_ERR_BAD_SHAPE;
-  lp_scale_kernel<<<1, 256, 0, (cudaStream_t)stream>>>(g, h, rows, inv_t, logf((float)V), scale);
+  lp_scale_kernel<<<1, 256, 0, (cudaStream_t)stream>>>(g, h, tokens, rows, V, inv_t, logf((float)V), scale);
   B200_LAUNCH_CHECK();
   return 0;
 }

@@ -820,15 +820,29 @@ int b200_token_logprobs_grad(const void* logits, long long rs, long long rows, i
 /* The same from x [M, K] and w [N, K] (bf16 or fp16, rows at multiples of 16 bytes): sums of each row's logits in a tile's columns into part fp32
  * [b200_gemm_head_tiles(M, N, K), M, 4], the tokens' logits into lt fp32 [M] (csrc/gemm_tcgen05.cu), then what token_logprobs gives. */
 int b200_gemm_head_tiles(int M, int N, int K);   /* below zero: minus a status */
-int b200_gemm_head_sums(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, float inv_t,
-                        int entropy, void* part, float* lt, void* stream);
-int b200_logprob_finish(const void* part, int parts, long long rows, int V, const long long* tokens, const float* lt, float inv_t, float* lp, float* ent, void* stats,
-                        void* stream);
-/* scale [2]: a power of two that brings gradients into fp16's range, and its reciprocal. */
-int b200_logprob_scale(const float* g, const float* h, long long rows, float inv_t, int V, float* scale, void* stream);
-/* out [M, N] (row stride out_rs) = gradient, in 16 bits, of the logits of columns c0 .. c0 + N of a vocabulary of V (w: those rows), times scale[0] (NULL: 1). */
-int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const long long* tokens, int V, int c0,
-                         float inv_t, const void* stats, const float* g, const float* h, const float* scale, void* out, long long out_rs, void* stream);
+/* active (NULL: all): int32 on the device, how many of the M rows count, at least 1; the products' work ends there. */
+int b200_gemm_head_sums(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const int* active, const long long* tokens,
+                        float inv_t, int entropy, void* part, float* lt, void* stream);
+/* from (NULL: the same): which row of lp, ent and stats each one is. */
+int b200_logprob_finish(const void* part, int parts, long long rows, int V, const int* active, const int* from, const long long* tokens, const float* lt, float inv_t,
+                        float* lp, float* ent, void* stats, void* stream);
+/* The rows of x (16 bits, K a multiple of 8) whose tokens are in 0 .. V - 1, in order, into out [rows, K] (zeros behind them up to a multiple of 256 rows): from int32
+ * [rows], place int32 [rows] (-1: passed over, zeros in lp and ent), mine int64 [rows] their tokens, active int32 [1]. tokens NULL: from, mine and active are given. */
+int b200_logprob_active(const long long* tokens, const void* x, long long x_rs, int rows, int K, int V, int* from, int* place, long long* mine, int* active,
+                        float* lp, float* ent, void* out, void* stream);
+/* y [rows, K] (16 bits) = x[place] * scale[1] (NULL: 1), zeros where place is -1; x in y's type or fp32. */
+int b200_logprob_return(const void* x, int x_dtype, void* y, int rows, int K, const int* place, const float* scale, int dtype, void* stream);
+/* scale [2]: a power of two that brings gradients into fp16's range, and its reciprocal; rows whose tokens (NULL: all count) are passed over do not count. */
+int b200_logprob_scale(const float* g, const float* h, const long long* tokens, long long rows, float inv_t, int V, float* scale, void* stream);
+/* out [M, N] (row stride out_rs) = gradient, in 16 bits, of the logits of columns c0 .. c0 + N of a vocabulary of V (w: those rows), times scale[0] (NULL: 1); rows from
+ * active on (up to the end of their tile of 256) are zeros. rows (NULL: the same): which of stats, g and h is each row's. */
+int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long w_rs, int M, int N, int K, int dtype, const int* active, const int* rows,
+                         const long long* tokens, int V, int c0, float inv_t, const void* stats, const float* g, const float* h, const float* scale, void* out,
+                         long long out_rs, void* stream);
+/* out [M, N] = a b^T + beta out (16-bit operands, stored transposed where a_mn / b_mn), for the first `active` rows, or where `depth` for the first `active` of K (what
+ * stands behind them in a block of 64 must be zeros). */
+int b200_gemm_active(const void* a, long long a_rs, int a_mn, const void* b, long long b_rs, int b_mn, int M, int N, int K, int dtype, const int* active, int depth,
+                     void* out, long long out_rs, int out_dtype, float beta, void* stream);
 /* y (16 bits) = x * scale[1] (scale NULL: x). */
 int b200_logprob_cast(const float* x, void* y, long long n, const float* scale, int dtype, void* stream);
 

@@ -201,10 +201,28 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 # from hidden states
 # ------------------------------------------------------------------------------------------------
 _CHUNK_BYTES = 128 << 20         # 16-bit gradients of logits that exist at a time in the backward pass
+_COMPACT_ROWS = 256              # more rows than one tile of the products has: those that are passed over leave them
 _HEAD = [vp, i64, vp, i64, i32, i32, i32, i32, vp]
-_HEAD_SUMS = _HEAD + [f32, i32, vp, vp, vp]
-_HEAD_GRADS = _HEAD + [i32, i32, f32, vp, vp, vp, vp, vp, i64, vp]
-_FINISH = [vp, i32, i64, i32, vp, vp, f32, vp, vp, vp, vp]
+_HEAD_SUMS = _HEAD + [vp, f32, i32, vp, vp, vp]
+_HEAD_GRADS = _HEAD + [vp, vp, i32, i32, f32, vp, vp, vp, vp, vp, i64, vp]
+_ACTIVE_GEMM = [vp, i64, i32, vp, i64, i32, i32, i32, i32, i32, vp, i32, vp, i64, i32, f32, vp]
+_FINISH = [vp, i32, i64, i32, vp, vp, vp, vp, f32, vp, vp, vp, vp]
+_ACTIVE = [vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
+
+
+class _Active:
+    """Rows whose tokens are not passed over, side by side in ``x`` [T, K]; their number stays on the device. ``maps`` int32 [2 T + 1]: which row each is, where each
+    row went, how many; ``tokens`` int64 [T]: theirs."""
+
+    def __init__(self, x, tokens, V, maps, mine, lp=None, H=None):
+        T, K = x.shape
+        self.x, self.maps, self.mine = torch.empty(T, K, dtype=x.dtype, device=x.device), maps, mine
+        self.rows, self.place, self.count = maps.data_ptr(), maps.data_ptr() + 4 * T, maps.data_ptr() + 8 * T
+        rc = nv.proto("b200_logprob_active", _ACTIVE)(nv.ptr(tokens), x.data_ptr(), x.stride(0), T, K, V, self.rows, self.place, nv.ptr(mine), self.count, nv.ptr(lp),
+                                                      nv.ptr(H), self.x.data_ptr(), nv.stream())
+        if rc:
+            nv.check(rc, "logprob_active")
+        nv.count_launch(1 + (tokens is not None))
 
 
 def _on(x: torch.Tensor):
@@ -224,35 +242,42 @@ def _linear_forward(x, w, tokens, temperature, entropy, save):
     V = w.shape[0]
     if not nv.use_native(x):
         lp, H, _, _, _, stats = _rows_torch(x.float() @ w.float().t(), tokens, temperature, 0, entropy, False)
-        return lp, H, stats
+        return lp, H, (stats, None, None)
     new, dt = x.new_empty, torch.float32
     lp, H, stats = new((T,), dtype=dt) if tokens is not None else None, new((T,), dtype=dt) if entropy else None, new((T, 4), dtype=dt) if save else None
     if T == 0:
-        return lp, H, stats
+        return lp, H, (stats, None, None)
+    maps = mine = None
+    rows = count = 0
+    if tokens is not None and T > _COMPACT_ROWS:
+        maps, mine = new((2 * T + 1,), dtype=torch.int32), new((T,), dtype=torch.int64)
+        act = _Active(x, tokens, V, maps, mine, lp, H)
+        x, rows, count, tokens = act.x, act.rows, act.count, mine
     tiles = nv.proto("b200_gemm_head_tiles", [i32] * 3)(T, V, K)
     if tiles < 0:
         nv.check(-tiles, "gemm_head_tiles")
     work = new((tiles * T * 4 + T,), dtype=dt)                           # sums of tiles, then the tokens' logits
     part, inv_t, st, tok = work.data_ptr(), 1.0 / temperature, nv.stream(), nv.ptr(tokens)
     lt = part + tiles * T * 16
-    rc = nv.proto("b200_gemm_head_sums", _HEAD_SUMS)(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), T, V, K, nv.dtype_code(x.dtype), tok, inv_t,
+    rc = nv.proto("b200_gemm_head_sums", _HEAD_SUMS)(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), T, V, K, nv.dtype_code(x.dtype), count, tok, inv_t,
                                                      int(entropy), part, lt, st)
     if rc:
         nv.check(rc, "gemm_head_sums")
-    rc = nv.proto("b200_logprob_finish", _FINISH)(part, tiles, T, V, tok, lt, inv_t, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), st)
+    rc = nv.proto("b200_logprob_finish", _FINISH)(part, tiles, T, V, count, rows, tok, lt, inv_t, nv.ptr(lp), nv.ptr(H), nv.ptr(stats), st)
     if rc:
         nv.check(rc, "logprob_finish")
     nv.count_launch(2)
-    return lp, H, stats
+    return lp, H, (stats, maps, mine)
 
 
-def _linear_backward(x, w, tokens, temperature, stats, g, h, need_dx, need_dw):
+def _linear_backward(x, w, tokens, temperature, saved, g, h, need_dx, need_dw):
     T, K = x.shape
     V = w.shape[0]
+    stats, maps, mine = saved
     if not nv.use_native(x):
         d = _grad_torch(x.float() @ w.float().t(), tokens, temperature, stats, g, h, 0, V)
         return (d @ w.float()).to(x.dtype) if need_dx else None, (d.t() @ x.float()).to(w.dtype) if need_dw else None
-    dev, dt, inv_t = x.device, nv.dtype_code(x.dtype), 1.0 / temperature
+    dev, dt, inv_t, f32_ = x.device, nv.dtype_code(x.dtype), 1.0 / temperature, torch.float32
     dw = torch.empty(V, K, dtype=w.dtype, device=dev) if need_dw else None
     if T == 0:
         return (torch.empty_like(x) if need_dx else None), (None if dw is None else dw.zero_())
@@ -262,29 +287,62 @@ def _linear_backward(x, w, tokens, temperature, stats, g, h, need_dx, need_dw):
     half = x.dtype == torch.float16
     scale = part = None
     if half:             # gradients of single logits lie below fp16's numbers: they are brought up by a power of two, the results back down
-        scale = torch.empty(2, dtype=torch.float32, device=dev)
-        fs = nv.proto("b200_logprob_scale", [vp, vp, i64, f32, i32, vp, vp])
-        nv.check(fs(nv.ptr(g), nv.ptr(h), T, inv_t, V, nv.ptr(scale), nv.stream()), "logprob_scale")
-        part = torch.empty(C, K, dtype=torch.float32, device=dev) if need_dw else None
-    dx = torch.empty(T, K, dtype=x.dtype, device=dev) if need_dx else None
+        scale = torch.empty(2, dtype=f32_, device=dev)
+        fs = nv.proto("b200_logprob_scale", [vp, vp, vp, i64, f32, i32, vp, vp])
+        nv.check(fs(nv.ptr(g), nv.ptr(h), nv.ptr(tokens), T, inv_t, V, nv.ptr(scale), nv.stream()), "logprob_scale")
+        part = torch.empty(C, K, dtype=f32_, device=dev) if need_dw else None
+    act, rows, count = None, 0, 0
+    if maps is not None:
+        act = _Active(x, None, V, maps, mine)
+    elif tokens is not None and need_dw:                  # zeros times what stands in a row that is passed over would not do: it may be no number
+        mine = x.new_empty((T,), dtype=torch.int64)
+        act = _Active(x, tokens, V, x.new_empty((2 * T + 1,), dtype=torch.int32), mine)
+    if act is not None:
+        x, rows, count, tokens = act.x, act.rows, act.count, mine
     direct = len(chunks) == 1 and not half                # one product gives dx: no sums in 32 bits between chunks
-    acc = dx if direct else torch.empty(T, K, dtype=torch.float32, device=dev) if need_dx else None
+    dx = torch.empty(T, K, dtype=x.dtype, device=dev) if need_dx else None
+    acc = None
+    if need_dx:
+        acc = dx if direct and act is None else torch.empty(T, K, dtype=x.dtype if direct else f32_, device=dev)
     fg = nv.proto("b200_gemm_head_grads", _HEAD_GRADS)
     fc = nv.proto("b200_logprob_cast", [vp, vp, i64, vp, i32, vp])
+    fa = nv.proto("b200_gemm_active", _ACTIVE_GEMM)
+    st = nv.stream()
+    # dx has few tiles where tokens are few: cut along the vocabulary (which the products that end at a count are not) all rows take less time than those that
+    # count (1001 x 2560, 751 rows that count, chunks of 50688: 185 us and 248)
+    plan = (i32 * 4)()
+    if act is not None and need_dx:
+        nv.check(nv.proto("b200_gemm_plan", [i32] * 7 + [vp])(T, K, C, 1, 1, dt, nv.sm_count(dev), ctypes.addressof(plan)), "gemm_plan")
+
+    def product(n, depth, c0, out, beta):
+        """dl w of the chunk (rows), or dl^T x (depth)."""
+        d, wc = dl[:, :n], w[c0:c0 + n]
+        if act is None or (not depth and plan[2]):
+            gemm(d, x, a_mn=True, b_mn=True, out=out) if depth else gemm(d, wc, b_mn=True, out=out, beta=beta)
+            return
+        o = (x.data_ptr(), x.stride(0)) if depth else (wc.data_ptr(), w.stride(0))
+        rc = fa(dl.data_ptr(), ld, int(depth), *o, 1, n if depth else T, K, T if depth else n, dt, count, int(depth), out.data_ptr(), out.stride(0),
+                nv.dtype_code(out.dtype), beta, st)
+        if rc:
+            nv.check(rc, "gemm_active")
+        nv.count_launch()
     for c0, c1 in chunks:
-        n, wc = c1 - c0, w[c0:c1]
-        nv.check(fg(nv.ptr(x), x.stride(0), nv.ptr(wc), w.stride(0), T, n, K, dt, nv.ptr(tokens), V, c0, inv_t, nv.ptr(stats), nv.ptr(g), nv.ptr(h), nv.ptr(scale),
-                    nv.ptr(dl), ld, nv.stream()), "gemm_head_grads")
+        n = c1 - c0
+        nv.check(fg(nv.ptr(x), x.stride(0), nv.ptr(w[c0:c1]), w.stride(0), T, n, K, dt, count, rows, nv.ptr(tokens), V, c0, inv_t, nv.ptr(stats), nv.ptr(g), nv.ptr(h),
+                    nv.ptr(scale), nv.ptr(dl), ld, st), "gemm_head_grads")
         if need_dx:
-            gemm(dl[:, :n], wc, b_mn=True, out=acc, beta=1.0 if c0 else 0.0)
+            product(n, False, c0, acc, 1.0 if c0 else 0.0)
         if need_dw and not half:
-            gemm(dl[:, :n], x, a_mn=True, b_mn=True, out=dw[c0:c1])
+            product(n, True, c0, dw[c0:c1], 0.0)
         elif need_dw:
-            gemm(dl[:, :n], x, a_mn=True, b_mn=True, out=part[:n])
-            nv.check(fc(nv.ptr(part), nv.ptr(dw[c0:c1]), n * K, nv.ptr(scale), dt, nv.stream()), "logprob_cast")
-    if need_dx and not direct:
-        nv.check(fc(nv.ptr(acc), nv.ptr(dx), T * K, nv.ptr(scale), dt, nv.stream()), "logprob_cast")
-    nv.count_launch(len(chunks) * (2 if half and need_dw else 1) + bool(need_dx and not direct) + half)
+            product(n, True, c0, part[:n], 0.0)
+            nv.check(fc(nv.ptr(part), nv.ptr(dw[c0:c1]), n * K, nv.ptr(scale), dt, st), "logprob_cast")
+    if need_dx and act is not None:
+        fr = nv.proto("b200_logprob_return", [vp, i32, vp, i32, i32, vp, vp, i32, vp])
+        nv.check(fr(nv.ptr(acc), nv.dtype_code(acc.dtype), nv.ptr(dx), T, K, act.place, nv.ptr(scale), dt, st), "logprob_return")
+    elif need_dx and not direct:
+        nv.check(fc(nv.ptr(acc), nv.ptr(dx), T * K, nv.ptr(scale), dt, st), "logprob_cast")
+    nv.count_launch(len(chunks) * (2 if half and need_dw else 1) + bool(need_dx and acc is not dx) + half)
     return dx, dw
 
 
@@ -294,11 +352,11 @@ class _LinearLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, tokens, temperature, entropy):
         with _on(x):
-            lp, H, stats = _linear_forward(x, w, tokens, temperature, entropy, True)
+            lp, H, saved = _linear_forward(x, w, tokens, temperature, entropy, True)
         if w.requires_grad:
             from ..utils.arena import note_use
             note_use(w, False)                   # its gradient arrives through autograd
-        ctx.save_for_backward(x, w, tokens, stats)
+        ctx.save_for_backward(x, w, tokens, *saved)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         return lp, H
@@ -308,17 +366,19 @@ class _LinearLogprobsFn(torch.autograd.Function):
         _first_order_only("linear_token_logprobs")
         if g is None and h is None:
             return (None,) * 5
-        x, w, tokens, stats = ctx.saved_tensors
+        x, w, tokens, *saved = ctx.saved_tensors
         g, h = (None if t is None else t.to(torch.float32).contiguous() for t in (g, h))
         with _on(x):
-            dx, dw = _linear_backward(x, w, tokens, ctx.temperature, stats, g, h, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+            dx, dw = _linear_backward(x, w, tokens, ctx.temperature, saved, g, h, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dx, dw, None, None, None
 
 
 def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor], *, entropy: bool = False, temperature: float = 1.0) -> TokenLogprobs:
     """``token_logprobs(x @ w.T, tokens)`` for hidden states ``x`` [..., K] and an output projection ``w`` [vocab, K] (bf16 or fp16, K a multiple of 8),
     without the logits: their sums are taken from the product's accumulators (fp32), and in the backward pass, where the product is computed again, their
-    gradients, which exist in 16 bits a chunk of the vocabulary at a time. Gradients for ``x`` and ``w``."""
+    gradients, which exist in 16 bits a chunk of the vocabulary at a time. Rows whose tokens are passed over leave the products before they begin (how many stays
+    on the device) and may hold anything. Gradients for ``x`` and ``w``. Tensor cores add up a logit's K products with an error of about K * 2^-30 of it (4.6e-6 of a log
+    probability at K = 4096, where ``token_logprobs`` has 6e-8 of the logits it is given)."""
     shape, native = x.shape, nv.use_native(x)
     if w.dim() != 2 or w.shape[0] < 1 or not shape or shape[-1] != w.shape[1] or x.dtype != w.dtype or x.device != w.device:
         raise ValueError("linear_token_logprobs: x [..., K] and w [vocab, K] must agree in K, type and device")

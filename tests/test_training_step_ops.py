@@ -248,9 +248,11 @@ def test_what_log_probabilities_refuse():
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-@pytest.mark.parametrize("T,K,V", [(1, 64, 37), (5, 128, 1001), (17, 64, 4099), (130, 72, 20011), (300, 128, 9000)])
-def test_from_hidden_states(T, K, V, dtype, device, monkeypatch):
-    """Chunks of the vocabulary, odd sizes, rows that are passed over; the gradients of both operands, small ones too (weights of 1e-6)."""
+@pytest.mark.parametrize("T,K,V,passed", [(1, 64, 37, 0), (5, 128, 1001, 0), (17, 64, 4099, 0.5), (130, 72, 20011, 0), (256, 64, 5000, 0.5), (257, 64, 5000, 0.5),
+                                          (300, 128, 9000, 0), (700, 64, 3000, 0.9), (600, 64, 600, 0.572), (513, 64, 600, 1)])
+def test_from_hidden_states(T, K, V, passed, dtype, device, monkeypatch):
+    """Chunks of the vocabulary, odd sizes; few, many and only rows that are passed over, up to the ends of tiles (256 of 600 count), whose states and weights may be
+    anything; the gradients of both operands, small ones too (weights of 1e-6)."""
     monkeypatch.setattr(lpm, "_CHUNK_BYTES", 0)                         # chunks of 4096 columns at most, the last one short
     dt, tau = DT[dtype], 0.8
     r = torch.Generator().manual_seed(T)
@@ -258,26 +260,40 @@ def test_from_hidden_states(T, K, V, dtype, device, monkeypatch):
     tokens = torch.randint(0, V, (T,), generator=r)
     if T > 3:
         tokens[2] = -100
+    tokens[torch.randperm(T, generator=r)[:round(T * passed)]] = V + 3
+    if T == 600:
+        counting = ((tokens >= 0) & (tokens < V)).nonzero()[:, 0]
+        tokens[counting[256:]] = -1
     g, h = torch.randn(T, generator=r) * 1e-6, torch.randn(T, generator=r) * 1e-6
-    logits = x.double() @ w.double().t()
+    bad = (tokens < 0) | (tokens >= V)
+    x[bad] = float("nan")
+    g[bad], h[bad] = 1e20, float("inf")
+    if device == "cpu":
+        x[bad] = 0
+    a, b = x.clone(), w                                    # what counts; a row that is passed over has no part in anything
+    a[bad] = 0
+    logits = a.double() @ b.double().t()
     e = exact_rows(logits, tokens, tau, g, h)
+    live, keep = a.double(), (~bad).double()
+    g, h = g.clone(), h.clone()
     a, b = x.to(device).requires_grad_(True), w.to(device).requires_grad_(True)
     got = linear_token_logprobs(a, b, tokens.to(device), entropy=True, temperature=tau)
     dx, dw = torch.autograd.grad([got.logprob, got.entropy], [a, b], [g.to(device), h.to(device)])
     # a logit is a sum of K exact products in 32 bits (K + 8 roundings of the sum of magnitudes); row sums as above
-    logit = (K + 8) * 2.0 ** -24 * float((x.double().abs() @ w.double().abs().t()).max()) / tau
+    logit = (K + 8) * 2.0 ** -24 * float((live.abs() @ w.double().abs().t()).max()) / tau
     tol = lp_tolerance(e, V, tau, float((logits.amax(1, keepdim=True) - logits).max()) / tau) + 2 * logit
     assert ((got.logprob.detach().cpu().double() - e["lp"]).abs() <= tol).all()
     assert ((got.entropy.detach().cpu().double() - e["H"]).abs() <= tol + 2 * (sum_error(V) + 2 * logit) * (math.log(V) + 2)).all()
-    assert not got.logprob[2:3].any() if T > 3 else True
+    assert not got.logprob[bad.to(device)].any() and not got.entropy[bad.to(device)].any() and not dx[bad.to(device)].any()
     # gradients of logits are rounded to 16 bits before the products (half a step of each term), the results once more; sums in 32 bits
     half, least = half_step(dt)
     rel = half + 2 * logit + 8 * sum_error(V) + 2.0 ** -19
-    size = e["p"] * (g.abs()[:, None] + h.abs()[:, None] * ((e["p"].clamp_min(1e-30).log()).abs() + e["H"][:, None] + 1)) / tau + e["grad"].abs()
+    gs, hs = torch.where(bad, 0, g).abs(), torch.where(bad, 0, h).abs()
+    size = e["p"] * (gs[:, None] + hs[:, None] * ((e["p"].clamp_min(1e-30).log()).abs() + e["H"][:, None] + 1)) / tau + e["grad"].abs()
     # fp16 brings the largest gradient to 2^13 or more, so that the smallest number, 2^-24, is 2^-37 of it
-    tiny = 2.0 ** -37 * float(((g.abs() + h.abs() * (math.log(V) + 1)) / tau).max()) if dt == torch.float16 else 0.0
+    tiny = 2.0 ** -37 * float(((gs + hs * (math.log(V) + 1)) / tau).max()) * keep[:, None] if dt == torch.float16 else 0.0
     for name, u, v, want, terms in (("dx", dx, None, e["grad"] @ w.double(), (size * rel + tiny) @ w.double().abs()),
-                                    ("dw", dw, None, e["grad"].t() @ x.double(), (size * rel + tiny).t() @ x.double().abs())):
+                                    ("dw", dw, None, e["grad"].t() @ live, (size * rel + tiny).t() @ live.abs())):
         assert u.dtype == dt
         assert ((u.cpu().double() - want).abs() <= terms + half * want.abs() + least + max(T, V) * 2.0 ** -24 * terms).all(), name
     frozen = linear_token_logprobs(a, w.to(device), tokens.to(device), temperature=tau)
