@@ -195,10 +195,12 @@ class _Checkpoint8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, anchor, run, delta, residual):
         ctx.run, ctx.n_in = run, 1 + (residual is not None)
-        ctx.draws = _draws(delta)
+        ctx.draws, ctx.autocast = _draws(delta), _autocast(delta.device.type)
         p = pack8(delta, residual)
         with torch.no_grad():
             out = run(delta, residual)
+        if not isinstance(out, tuple) or not all(isinstance(t, torch.Tensor) for t in out):
+            raise TypeError("checkpoint8: the layer must return a tuple of tensors")
         ctx.kept = p.shape, p.dtype
         ctx.save_for_backward(p.q, p.e)
         ctx.set_materialize_grads(False)
@@ -211,7 +213,7 @@ class _Checkpoint8Fn(torch.autograd.Function):
         now = _draws(x)
         try:                                             # dropout masks of the layer are those of its forward
             _set_draws(ctx.draws)
-            with torch.enable_grad():
+            with torch.enable_grad(), torch.autocast(x.device.type, **ctx.autocast):
                 out = ctx.run(x, None)
         finally:
             _set_draws(now)
@@ -219,6 +221,10 @@ class _Checkpoint8Fn(torch.autograd.Function):
         if pairs:
             torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
         return None, None, x.grad if ctx.needs_input_grad[2] else None, x.grad if ctx.n_in == 2 and ctx.needs_input_grad[3] else None
+
+
+def _autocast(device):
+    return {"enabled": torch.is_autocast_enabled(device), "dtype": torch.get_autocast_dtype(device), "cache_enabled": torch.is_autocast_cache_enabled()}
 
 
 def _draws(x):

@@ -348,7 +348,7 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
                 raise HTTPException(status_code=500, detail=r.error)
             text, hit = cut_at_stop(decode(eng, r.output_ids), _stops(req.stop))
             choices.append({"index": i, "text": text, "finish_reason": "stop" if hit else r.finish_reason,
-                            "logprobs": said(eng, r, (0, tokens_of(eng, r.output_ids, _stops(req.stop))), completion_logprobs)})
+                            "logprobs": None if r.cfg.logprobs is None else said(eng, r, (0, tokens_of(eng, r.output_ids, _stops(req.stop))), completion_logprobs)})
             n_p += len(r.prompt_ids)
             n_c += len(r.output_ids)
         return {"id": f"cmpl-{uuid.uuid4().hex}", "object": "text_completion", "created": int(time.time()), "model": req.model,

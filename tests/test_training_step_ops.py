@@ -584,6 +584,30 @@ def test_checkpoints_in_8_bits(p, device):
     assert torch.equal(got[0], kept.grad) and torch.equal(got[1], kept.grad) and torch.equal(got[2], layer.w.grad)
 
 
+def test_checkpoints_take_layers_that_return_tuples_and_keep_autocast():
+    x = torch.randn(3, 32, requires_grad=True)
+    with pytest.raises(TypeError):
+        checkpoint8(lambda d, r: d * 2, x, None)
+    layer, seen = Layer(32), []
+
+    def watched(d, r):
+        y = layer(d, r)
+        seen.append(y[0].dtype)
+        return y
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = checkpoint8(watched, x, None)
+    y[0].float().sum().backward()
+    assert seen == [torch.bfloat16, torch.bfloat16] and x.grad is not None
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(3, 64, requires_grad=True)
+    for f in (lambda: token_logprobs(x, torch.tensor([0, 1, 2])).logprob, lambda: linear_token_logprobs(x, torch.randn(9, 64), torch.tensor([0, 1, 2])).logprob,
+              lambda: swiglu8(x), lambda: checkpoint8(Layer(64), x, None)[0]):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(f().sum(), x, create_graph=True)
+
+
 def test_checkpoints_behind_a_frozen_input_and_without_gradients():
     layer = Layer(32)
     x = torch.randn(3, 32)
