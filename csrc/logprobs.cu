@@ -523,59 +523,67 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
   }
 }
 
+// A thread has kGradSteps times 32 bytes of a row: 4096 x 151936 of 16 bits with entropies 385 us (one 438, two 410, eight 382; by CTAs that go over a whole row,
+// 16 bytes a load, 411), 1000 x 151936 of 32 bits 190 (187, 189, 192; 213).
+constexpr int kGradSteps = 4;
 template <typename T, bool HASH>
 __global__ void __launch_bounds__(kLpThreads)
-lp_rows_grad_kernel(const T* __restrict__ logits, long long rs, int V, int slice, const long long* __restrict__ tokens, float inv_t, const float4* __restrict__ stats,
+lp_rows_grad_kernel(const T* __restrict__ logits, long long rs, int V, const long long* __restrict__ tokens, float inv_t, const float4* __restrict__ stats,
                     const float* __restrict__ g, const float* __restrict__ h, T* __restrict__ out, long long os) {
-  constexpr int N = LpVec<T>::N, G = 2;
+  constexpr int N = 32 / sizeof(T);
   const long long row = blockIdx.x;
-  const int id0 = blockIdx.y * slice, n = min(slice, V - id0);
-  const long long t = tokens ? tokens[row] : 0;
-  const bool skip = t < 0 || t >= V;
-  const T* p = logits + row * rs + id0;
-  T* o = out + row * os + id0;
+  const T* p = logits + row * rs;
+  T* o = out + row * os;
+  const int head = min(V, int((32 - ((uintptr_t)p & 31)) & 31) / int(sizeof(T))), nvec = (V - head) / N;
+  const bool same = (((uintptr_t)p ^ (uintptr_t)o) & 31) == 0;          // both have their multiples of 32 bytes at the same elements
+  const int i0 = blockIdx.y * (kGradSteps * kLpThreads) + threadIdx.x;
+  const long long t = tokens ? tokens[row] : -1;
+  const bool skip = tokens && (t < 0 || t >= V);
   const float c = inv_t * kLog2e;
-  const LpGrad r = lp_grad_of(stats[row], g ? g[row] : 0.f, HASH && h ? h[row] : 0.f, inv_t, (tokens ? t : -1) - id0, 1.f);
-  const LpWalk at = lp_walk<T>(p, n);
-  const bool same = (((uintptr_t)p ^ (uintptr_t)o) & 15) == 0;          // both have their multiples of 16 bytes at the same elements
-  auto single = [&](int j) { o[j] = from_f32<T>(skip ? 0.f : lp_grad_at(to_f32<T>(p[j]), r, c)); };
-  auto vector = [&](const uint4& raw, int i) {
-    alignas(16) T y[N];
-    float v[N];
+  const LpGrad r = lp_grad_of(stats[row], g ? g[row] : 0.f, HASH && h ? h[row] : 0.f, inv_t, t, 1.f);
+  auto single = [&](int j) { o[j] = from_f32<T>(skip ? 0.f : lp_grad_at(to_f32<T>(p[j]), r, c) + (j == r.t ? r.g : 0.f)); };
+  const unsigned long long nm = lp_pair(-r.m, -r.m), cc = lp_pair(c, c), A = lp_pair(r.A, r.A), B = lp_pair(r.B, r.B);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = to_f32<T>(reinterpret_cast<const T*>(&raw)[j]);
-    const unsigned long long nm = lp_pair(-r.m, -r.m), cc = lp_pair(c, c), A = lp_pair(r.A, r.A), B = lp_pair(r.B, r.B);
+  for (int x = 0; x < kGradSteps; ++x) {
+    const int i = i0 + x * kLpThreads;
+    if (i >= nvec) break;
+    uint32_t w[8];
+    if (skip) {
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const unsigned long long x = lp_mul2(lp_add2(lp_pair(v[j], v[j + 1]), nm), cc);
-      const float2 xs = lp_split(x);
-      const unsigned long long e = lp_pair(lp_exp2(xs.x), lp_exp2(xs.y));
-      const float2 d = lp_split(lp_mul2(e, HASH ? lp_fma2(B, lp_pair(lp_factor(xs.x), lp_factor(xs.y)), A) : A));
-      y[j] = from_f32<T>(d.x);
-      y[j + 1] = from_f32<T>(d.y);
+      for (int j = 0; j < 8; ++j) w[j] = 0;
+    } else {
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+                   "=r"(w[7]) : "l"(p + head + (long long)i * N));
+      const long long at = r.t - head - (long long)i * N;               // the token's place among these
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        const float2 v = sizeof(T) == 4 ? make_float2(__uint_as_float(w[j & 7]), __uint_as_float(w[(j + 1) & 7])) : lp_word<T>(w[(j / 2) & 7]);
+        const unsigned long long y = lp_mul2(lp_add2(lp_pair(v.x, v.y), nm), cc);
+        const float2 ys = lp_split(y);
+        const unsigned long long e = lp_pair(lp_exp2(ys.x), lp_exp2(ys.y));
+        float2 d = lp_split(lp_mul2(e, HASH ? lp_fma2(B, lp_pair(lp_factor(ys.x), lp_factor(ys.y)), A) : A));
+        if (at == j) d.x += r.g;
+        if (at == j + 1) d.y += r.g;
+        if constexpr (sizeof(T) == 4) { w[j] = __float_as_uint(d.x); w[j + 1] = __float_as_uint(d.y); }
+        else {
+          alignas(4) T q[2] = {from_f32<T>(d.x), from_f32<T>(d.y)};
+          w[j / 2] = *reinterpret_cast<uint32_t*>(q);
+        }
+      }
     }
-    uint4 w = skip ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<uint4*>(y);
-    T* to = o + at.head + i * N;
-    if (same) *reinterpret_cast<uint4*>(to) = w;
-    else
+    T* to = o + head + (long long)i * N;
+    if (same) {
+      asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" :: "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]),
+                   "l"(to) : "memory");
+    } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) to[j] = reinterpret_cast<const T*>(&w)[j];
-  };
-  if (threadIdx.x < at.head) single(threadIdx.x);
-  const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
-  int i = threadIdx.x;
-  for (; i + (G - 1) * kLpThreads < at.nvec; i += G * kLpThreads) {
-    uint4 raw[G];
-#pragma unroll
-    for (int x = 0; x < G; ++x) raw[x] = skip ? make_uint4(0, 0, 0, 0) : __ldg(q + i + x * kLpThreads);
-#pragma unroll
-    for (int x = 0; x < G; ++x) vector(raw[x], i + x * kLpThreads);
+      for (int j = 0; j < N; ++j) to[j] = reinterpret_cast<const T*>(w)[j];
+    }
   }
-  for (; i < at.nvec; i += kLpThreads) vector(skip ? make_uint4(0, 0, 0, 0) : __ldg(q + i), i);
-  if (threadIdx.x < n - at.tail) single(at.tail + threadIdx.x);
-  if (!skip && r.t >= 0 && r.t < n) {                                    // the token's own term, over what its vector's thread wrote
-    __syncthreads();
-    if (threadIdx.x == 0) o[r.t] = from_f32<T>(lp_grad_at(to_f32<T>(p[r.t]), r, c) + r.g);
+  if (blockIdx.y == 0) {                                                 // the row's unaligned ends
+    if (threadIdx.x < head) single(threadIdx.x);
+    const int tail = head + nvec * N + threadIdx.x;
+    if (tail < V) single(tail);
   }
 }
 
@@ -788,14 +796,13 @@ B200_API int b200_token_logprobs_grad(const void* logits, long long rs, long lon
   if (lp_bad(rows, V)) return B200_ERR_BAD_SHAPE;
   if (rows == 0) return 0;
   cudaStream_t st = (cudaStream_t)stream;
-  // few rows: slices of 4096 logits, CTAs of their own
-  int parts = 1;
-  while (parts < 64 && rows * parts * 2 <= 8 * kNumSMs && V / (parts * 2) >= 2048) parts *= 2;
-  const int slice = parts > 1 ? lp_slice(V, parts) : V;
-  const dim3 grid((unsigned)rows, (unsigned)((V + slice - 1) / slice));
+  const long long vecs = ((long long)V * (dtype == B200_DT_FP32 ? 4 : 2)) / 32;
+  const long long steps = (vecs + kGradSteps * kLpThreads - 1) / (kGradSteps * kLpThreads);
+  if (steps > 65535) return B200_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)rows, (unsigned)(steps > 0 ? steps : 1));
   LP_TYPES(dtype, {
-    if (h) lp_rows_grad_kernel<T, true><<<grid, kLpThreads, 0, st>>>((const T*)logits, rs, V, slice, tokens, inv_t, (const float4*)stats, g, h, (T*)out, os);
-    else lp_rows_grad_kernel<T, false><<<grid, kLpThreads, 0, st>>>((const T*)logits, rs, V, slice, tokens, inv_t, (const float4*)stats, g, h, (T*)out, os);
+    if (h) lp_rows_grad_kernel<T, true><<<grid, kLpThreads, 0, st>>>((const T*)logits, rs, V, tokens, inv_t, (const float4*)stats, g, h, (T*)out, os);
+    else lp_rows_grad_kernel<T, false><<<grid, kLpThreads, 0, st>>>((const T*)logits, rs, V, tokens, inv_t, (const float4*)stats, g, h, (T*)out, os);
   });
   B200_LAUNCH_CHECK();
   return 0;
