@@ -137,12 +137,15 @@ class Qwen3ForCausalLM(nn.Module):
     def head_weight(self) -> torch.Tensor:
         return self.embed_tokens if self.lm_head is None else self.lm_head
 
-    def gradient_checkpointing_enable(self, activation_bits: int = 16, **_):
+    def gradient_checkpointing_enable(self, activation_bits: Optional[int] = None, gradient_checkpointing_kwargs: Optional[dict] = None, **_):
         """``activation_bits`` 8: a layer's input, stream and branch added, is kept in 8 bits (``ops.act8.checkpoint8``) instead of 16 of each; as
-        ``gradient_checkpointing_kwargs={"activation_bits": 8}`` of the trainer's arguments."""
-        if activation_bits not in (8, 16):
-            raise ValueError(f"activation_bits must be 8 or 16, not {activation_bits}")
-        self.gradient_checkpointing, self.checkpoint_bits = True, activation_bits
+        ``gradient_checkpointing_kwargs={"activation_bits": 8}`` of the trainer's arguments, or of this call as transformers spells it. None: as it was set
+        last (16 at first), so that a trainer that enables checkpoints once more leaves it."""
+        bits = (gradient_checkpointing_kwargs or {}).get("activation_bits") if activation_bits is None else activation_bits
+        bits = self.checkpoint_bits if bits is None else bits
+        if bits not in (8, 16):
+            raise ValueError(f"activation_bits must be 8 or 16, not {bits}")
+        self.gradient_checkpointing, self.checkpoint_bits = True, bits
 
     def gradient_checkpointing_disable(self):
         self.gradient_checkpointing = False

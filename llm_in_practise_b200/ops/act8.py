@@ -20,6 +20,7 @@ from . import _native as nv
 vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 BLOCK = 32
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MOST = 2 ** 28          # columns: a row's are counted in 32 bits
 _SWIGLU_FWD = [vp, i64, vp, vp, vp, i64, i32, i32, vp]
 _SWIGLU_BWD = [vp, vp, vp, vp, i64, i32, i32, vp]
 _PACK = [vp, i64, vp, i64, vp, vp, i64, i32, i32, vp]
@@ -38,8 +39,8 @@ class Packed8(NamedTuple):
 
 
 def _rows_of(what, x):
-    if x.dim() < 1 or x.shape[-1] < 1 or x.dtype not in _TYPES:
-        raise ValueError(f"{what}: needs [..., columns] in fp32, bf16 or fp16, not {x.dtype} {list(x.shape)}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _MOST or x.dtype not in _TYPES:
+        raise ValueError(f"{what}: needs [..., columns] in fp32, bf16 or fp16, up to {_MOST} columns, not {x.dtype} {list(x.shape)}")
     x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 

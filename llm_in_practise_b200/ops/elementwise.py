@@ -301,12 +301,20 @@ def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: floa
     dtype = dtype or dout.dtype
     if D < 1 or not 1 <= rows < 2 ** 31 - 1 or T >= 2 ** 30 or dout.dtype not in (torch.float32, torch.bfloat16, torch.float16) or dtype not in (dout.dtype, torch.float32):
         raise ValueError(f"embedding_grad: {T} tokens of {dout.dtype} [{D}] into {rows} rows of {dtype} are not taken")
+    padding_idx = _padding("embedding_grad", padding_idx, rows)
     flat, d2 = ids.reshape(-1).contiguous(), dout.reshape(T, D)
     if nv.use_native(dout):
         return _embedding_grad(flat, d2, rows, scale, padding_idx, dtype)
     keep = (flat >= 0) & (flat < rows) & (flat != (-1 if padding_idx is None else padding_idx))
     out = torch.zeros(rows, D, dtype=torch.float32, device=dout.device)
     return out.index_add_(0, flat[keep], d2[keep].float()).mul_(scale).to(dtype)
+
+
+def _padding(what, padding_idx, rows):
+    """As torch counts it: from the end where it is negative."""
+    if padding_idx is not None and not -rows <= padding_idx < rows:
+        raise ValueError(f"{what}: padding_idx must be from {-rows} to {rows - 1}, not {padding_idx}")
+    return padding_idx % rows if padding_idx is not None else None
 
 
 def _embedding_grad(flat, d2, rows, scale, padding_idx, dtype):
@@ -377,11 +385,17 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, pos_table: Optional[torch.
               scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``table[ids] * scale (+ pos_table[position])``; ids [..., L], position = index along the last dim. ``padding_idx``: a token
     whose row gets no gradient. A token outside the table is an error on the CPU and a row of zeros (before positions) on a GPU."""
+    if ids.device != table.device or (pos_table is not None and pos_table.device != table.device):
+        raise ValueError(f"embedding: ids and tables must be on the same device, not {ids.device} and {table.device}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"embedding: ids must be int64 or int32, not {ids.dtype}")
+    if padding_idx is not None:
+        padding_idx = _padding("embedding", padding_idx, table.shape[0])
     period = ids.shape[-1] if ids.dim() else 1
     vec = 4 if table.dtype == torch.float32 else 8
     if pos_table is not None and pos_table.shape[0] < period:
         raise ValueError(f"embedding: {period} positions, and the table has {pos_table.shape[0]}")
-    if (nv.use_native(table) and table.shape[1] % vec == 0 and table.is_contiguous()
+    if (nv.use_native(table) and table.shape[1] % vec == 0 and table.is_contiguous() and table.shape[0] < 2 ** 31 - 1
             and (pos_table is None or (pos_table.dtype == table.dtype and pos_table.is_contiguous()))):
         if torch.is_grad_enabled() and (table.requires_grad or (pos_table is not None and pos_table.requires_grad)):
             return _EmbeddingFn.apply(ids, table, pos_table, period, float(scale), padding_idx)

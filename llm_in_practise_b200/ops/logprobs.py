@@ -38,6 +38,7 @@ class TokenLogprobs(NamedTuple):
 
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MOST = 2 ** 30          # columns, and tokens from hidden states, are counted in 32 bits
 
 
 def _check(what, tokens, shape, device):
@@ -190,6 +191,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     elif rank or not (entropy or top):
         raise ValueError("token_logprobs: without tokens there are entropies and alternatives only")
     _check_temperature("token_logprobs", temperature)
+    if shape[-1] >= _MOST:
+        raise ValueError(f"token_logprobs: a row of {shape[-1]} logits; there is room for {_MOST - 1}")
     if not 0 <= top <= min(MAX_TOP, shape[-1]):
         raise ValueError(f"token_logprobs: top must be from 0 to {min(MAX_TOP, shape[-1])}, not {top}")
     if logits.requires_grad and torch.is_grad_enabled():
@@ -384,7 +387,7 @@ def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[tor
         raise ValueError("linear_token_logprobs: x [..., K] and w [vocab, K] must agree in K, type and device")
     if x.dtype not in (_TYPES[1:] if native else _TYPES):
         raise TypeError(f"linear_token_logprobs: x and w must be bf16 or fp16, not {x.dtype}; token_logprobs takes logits of 32 bits")
-    if native and (shape[-1] % 8 or w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16):
+    if native and (shape[-1] % 8 or w.stride(1) != 1 or w.stride(0) % 8 or w.stride(0) < shape[-1] or w.data_ptr() % 16):
         raise ValueError("linear_token_logprobs: rows of w must be contiguous, start at multiples of 16 bytes and have a multiple of 8 values")
     shape = shape[:-1]
     if tokens is not None:
@@ -393,8 +396,14 @@ def linear_token_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[tor
     if tokens is None and not entropy:
         raise ValueError("linear_token_logprobs: without tokens there are entropies only")
     rows = _as_rows(x)
-    if native and (rows.data_ptr() % 16 or rows.stride(0) % 8):
-        rows = rows.contiguous() if rows.stride(0) % 8 else rows.clone()
+    if max(rows.shape[0], *w.shape) >= _MOST:
+        raise ValueError(f"linear_token_logprobs: {rows.shape[0]} tokens, a vocabulary of {w.shape[0]}; there is room for {_MOST - 1}")
+    if native:
+        K = rows.shape[1]
+        if rows.data_ptr() % 16 or rows.stride(0) % 8 or rows.stride(0) < K:     # a row to a multiple of 16 bytes, none upon another
+            rows = rows.clone(memory_format=torch.contiguous_format)
+        if rows.shape[0] == 1 and rows.stride(0) != K:                           # one row is contiguous, whatever its stride says
+            rows = rows.view(K).unsqueeze(0)
     flat = None if tokens is None else tokens.reshape(-1).contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         lp, H = _LinearLogprobsFn.apply(rows, w, flat, temperature, entropy)

@@ -206,6 +206,19 @@ def test_trainer_arguments_reach_the_model():
     assert m.gradient_checkpointing and m.checkpoint_bits == 8
 
 
+def test_checkpoints_keep_the_bits_that_were_set():
+    from llm_in_practise_b200.trainer import Trainer, TrainingArguments
+    m = build("cpu")
+    m.gradient_checkpointing_enable()
+    assert m.checkpoint_bits == 16
+    m.gradient_checkpointing_enable(gradient_checkpointing_kwargs={"use_reentrant": False, "activation_bits": 8})
+    assert m.checkpoint_bits == 8
+    Trainer(model=m, args=TrainingArguments(output_dir="out", gradient_checkpointing=True, report_to="none"))
+    assert m.checkpoint_bits == 8
+    m.gradient_checkpointing_enable(16)
+    assert m.checkpoint_bits == 16
+
+
 def test_lora_behind_8_bit_checkpoints():
     """A frozen base: nothing in front of the first layer needs a gradient, and the adapters still get theirs."""
     from llm_in_practise_b200.peft import LoraConfig, get_peft_model

@@ -399,6 +399,63 @@ def test_what_embedding_gradients_refuse():
             bad()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_padding_tokens_count_as_torch_counts_them(device):
+    table, ids = torch.randn(20, 16, device=device, requires_grad=True), torch.tensor([3, 19, 7, 19], device=device)
+    dout = torch.randn(4, 16, device=device)
+    for pad in (19, -1):
+        (a,) = torch.autograd.grad(embedding(ids, table, padding_idx=pad), table, dout)
+        (b,) = torch.autograd.grad(torch.nn.functional.embedding(ids, table, pad), table, dout)
+        assert torch.equal(a, b) and torch.equal(a, embedding_grad(ids, dout, 20, padding_idx=pad)) and not a[19].any()
+    for pad in (20, -21):
+        for call in (lambda: embedding(ids, table, padding_idx=pad), lambda: embedding_grad(ids, dout, 20, padding_idx=pad)):
+            with pytest.raises(ValueError):
+                call()
+
+
+def test_what_embeddings_refuse():
+    table, ids = torch.randn(20, 16), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        embedding(ids.to("meta"), table)
+    with pytest.raises(ValueError):
+        embedding(ids, table, torch.randn(4, 16, device="meta"))
+    with pytest.raises(ValueError):
+        embedding(ids, table, torch.randn(3, 16))
+    for dt in (torch.float32, torch.bool, torch.int16):
+        with pytest.raises(TypeError):
+            embedding(ids.to(dt), table)
+
+
+def test_sizes_that_32_bits_do_not_count_are_refused():
+    """On a device without memory: nothing but the check runs."""
+    row, t = torch.empty(1, 2 ** 32 + 5, dtype=torch.bfloat16, device="meta"), torch.empty(1, dtype=torch.int64, device="meta")
+    for bad in (lambda: token_logprobs(row, t), lambda: pack8(row), lambda: swiglu8(row[:, 1:]),
+                lambda: linear_token_logprobs(row[:, :8], torch.empty(2 ** 31, 8, dtype=torch.bfloat16, device="meta"), t),
+                lambda: linear_token_logprobs(torch.empty(2 ** 31, 8, device="meta"), torch.empty(9, 8, device="meta"), t.expand(2 ** 31))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@gpu
+def test_log_probabilities_of_one_row_and_of_rows_upon_one_another():
+    """A single row may have any stride, and rows may share memory."""
+    w = torch.randn(100, 64, device="cuda").bfloat16()
+    one = torch.randn(1, 67, device="cuda").bfloat16()[:, :64]
+    same = torch.randn(64, device="cuda").bfloat16().expand(5, 64)
+    over = torch.randn(200, device="cuda").bfloat16().as_strided((5, 64), (8, 1))
+    aside = torch.randn(1, 80, device="cuda").bfloat16()[:, 3:67]
+    for x in (one, same, over, aside):
+        t = torch.arange(x.shape[0], device="cuda")
+        plain = x.clone(memory_format=torch.contiguous_format)
+        a, b = x.detach().requires_grad_(True), plain.detach().requires_grad_(True)
+        la, lb = linear_token_logprobs(a, w, t).logprob, linear_token_logprobs(b, w, t).logprob
+        assert torch.equal(la, lb) and torch.equal(linear_token_logprobs(x, w, t).logprob, lb)
+        g = torch.randn_like(la)
+        assert torch.equal(torch.autograd.grad(la, a, g)[0], torch.autograd.grad(lb, b, g)[0])
+    with pytest.raises(ValueError):
+        linear_token_logprobs(plain, w[0].expand(100, 64), t)
+
+
 @gpu
 @pytest.mark.parametrize("T", [100000, 70000])
 def test_embedding_gradient_of_many_tokens(T):
