@@ -33,7 +33,7 @@ template <int NT> struct LpShared : LpSums<NT> {
   static constexpr int kList = NT == 64 ? 512 : 1280, kSegments = NT == 64 ? 1 : 2048;
   unsigned long long best[kLpMaxTop];            // the slice's alternatives in order
   unsigned long long list[kList];
-  float segment[kSegments];                      // the largest of each 32 vectors
+  float segment[kSegments];                      // the largest of each 128 vectors, or 32
   uint32_t group[64];
   int chosen[kLpMaxTop];
   unsigned long long bound;
@@ -47,21 +47,21 @@ template <typename T> __device__ __forceinline__ float2 lp_word(uint32_t w) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-// The largest of G vectors' values, from vector G0 on (NaN aside).
-template <typename T, int G0, int G, int ALL>
-__device__ __forceinline__ float lp_largest(const uint4 (&raw)[ALL]) {
+// The largest of G vectors' values (NaN aside).
+template <typename T, int G>
+__device__ __forceinline__ float lp_largest(const uint4 (&raw)[G]) {
   if constexpr (sizeof(T) == 4) {
     float m = -INFINITY;
 #pragma unroll
-    for (int g = G0; g < G0 + G; ++g)
+    for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int j = 0; j < 4; ++j) m = fmaxf(m, __uint_as_float((&raw[g].x)[j]));
     return m;
   } else {
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    T2 m = *reinterpret_cast<const T2*>(&raw[G0].x);
+    T2 m = *reinterpret_cast<const T2*>(&raw[0].x);
 #pragma unroll
-    for (int g = G0; g < G0 + G; ++g)
+    for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int j = 0; j < 4; ++j) m = __hmax2(m, *reinterpret_cast<const T2*>(&(&raw[g].x)[j]));
     return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
@@ -121,7 +121,8 @@ __device__ __forceinline__ int lp_above(const uint4 (&raw)[G], float lt) {
   return n;
 }
 
-// How NT threads walk over p[0 .. n): single values up to the first multiple of 16 bytes, vectors i = thread, thread + NT .. by fours, single values behind the last.
+// How NT threads walk over p[0 .. n): single values up to the first multiple of 16 bytes, vectors by fours, single values behind the last. A warp's four are 128
+// vectors in a row (in CTAs of 64 threads: thread, thread + NT ..).
 struct LpWalk { int head, nvec, tail; };
 template <typename T> __device__ __forceinline__ LpWalk lp_walk(const T* p, int n) {
   const int head = min(n, int((16 - ((uintptr_t)p & 15)) & 15) / int(sizeof(T))), nvec = (n - head) / LpVec<T>::N;
@@ -277,13 +278,13 @@ __device__ __forceinline__ void lp_top_of_threads(const T* __restrict__ p, int n
   else lp_sort<NT>(sh.list, m, k, sh.best);
 }
 
-// The same for long rows, from the largest value of each segment of 32 vectors, 512 bytes in a row. The k segments with the largest of those (the first
-// ones among equals) have all k of them: whatever stands in another segment comes behind the largest of each of these. They are read again as whole
-// lines (what 20 threads had seen, a sector here and there, was a third of a row of 16 bits: 3000 x 151936 with 20 alternatives 239 us).
-template <typename T, int NT>
+// The same for long rows, from the largest value of each segment of 2^SEG vectors. The k segments with the largest of those (the first ones among equals) have all k of them:
+// whatever stands in another segment comes behind the largest of each of these. They are read again as whole lines (what 20 threads had seen, a sector
+// here and there, was a third of a row of 16 bits: 3000 x 151936 with 20 alternatives 239 us, now 184).
+template <typename T, int NT, int SEG>
 __device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int n, int id0, int k, LpWalk at, LpShared<NT>& sh) {
   constexpr int N = LpVec<T>::N, CAP = LpShared<NT>::kList, EACH = NT / 64;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, segments = (at.nvec + 31) / 32;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, segments = (at.nvec + (1 << SEG) - 1) >> SEG;
   const uint4* q = reinterpret_cast<const uint4*>(p + at.head);
   if (segments < k || segments > LpShared<NT>::kSegments) { lp_top_by_passes<T, NT>(p, n, id0, k, sh); return; }
   // 1. a bound, the k-th of 64 groups of segments
@@ -331,29 +332,42 @@ __device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int 
     if (i < CAP) sh.list[i] = lp_key(v, id0 + j);
   };
   for (int b = w; b < k; b += NT / 32) {
-    const int i = sh.chosen[b] * 32 + lane;
-    const bool has = i < at.nvec;
-    const uint4 raw = __ldg(q + (has ? i : 0));
-    float v[N];
-    int equal = 0;
+    const int i0 = (sh.chosen[b] << SEG) + lane;
+    constexpr int P = 1 << (SEG - 5);
+    uint4 raw[P];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      v[j] = to_f32<T>(reinterpret_cast<const T*>(&raw)[j]);
-      equal += v[j] == value;
-    }
-    if (!has) equal = 0;
-    int before = equal;                                                  // equal ones in the lanes up to this one
+    for (int g = 0; g < P; ++g) raw[g] = __ldg(q + (i0 + g * 32 < at.nvec ? i0 + g * 32 : 0));
+    int seen = 0;                                                        // equal ones in the pieces before
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int x = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += x;
-    }
-    before -= equal;
+    for (int g = 0; g < P; ++g) {
+      const int i = i0 + g * 32;
+      const uint4 one[1] = {raw[g]};
+      const float largest = i < at.nvec ? lp_largest<T, 1>(one) : -INFINITY;
+      if (!__any_sync(0xffffffffu, i < at.nvec && largest >= value)) continue;        // most pieces of a segment, which has one alternative or two
+      int equal = 0;
+      if (i < at.nvec && largest >= value) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const bool same = v[j] == value;
-      if (has && (v[j] > value || (same && before < k))) offer(v[j], at.head + i * N + j);
-      before += same;
+        for (int j = 0; j < N; ++j) {
+          const float v = to_f32<T>(reinterpret_cast<const T*>(&raw[g])[j]);
+          if (v > value) offer(v, at.head + i * N + j);
+          equal += v == value;
+        }
+      }
+      if (!__any_sync(0xffffffffu, equal)) continue;
+      int before = equal;                                                // equal ones in the lanes up to this one
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+      }
+      const int all = __shfl_sync(0xffffffffu, before, 31);
+      before += seen - equal;
+      seen += all;
+      if (equal && before < k) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (to_f32<T>(reinterpret_cast<const T*>(&raw[g])[j]) == value && before++ < k) offer(value, at.head + i * N + j);
+      }
     }
   }
   if (threadIdx.x < at.head && to_f32<T>(p[threadIdx.x]) >= value) offer(to_f32<T>(p[threadIdx.x]), threadIdx.x);
@@ -372,13 +386,13 @@ __device__ __forceinline__ float lp_warp_max(float v) {
 }
 
 // A row by a cluster of CTAs (of one, where there are rows enough), a slice each.
-// NT: 64 threads a CTA for short rows, 256 for long ones; TOP (256): with alternatives.
-template <typename T, bool ENT, int NT, bool TOP>
+// NT: 64 threads a CTA for short rows, 256 for long ones; SEG: 0 without alternatives, else 5 or 7, the segments whose largest values are noted (64 threads: theirs).
+template <typename T, bool ENT, int NT, int SEG>
 __global__ void __launch_bounds__(NT, (sizeof(T) == 4 ? 1024 : 1280) / NT)
 lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, const long long* __restrict__ tokens, float inv_t, int top, float* __restrict__ lp,
                float* __restrict__ ent, long long* __restrict__ rank, long long* __restrict__ top_ids, float* __restrict__ top_lp,
                float4* __restrict__ stats) {
-  constexpr int N = LpVec<T>::N;
+  constexpr bool TOP = SEG != 0;
   __shared__ typename std::conditional<TOP, LpShared<NT>, LpSums<NT>>::type sh;
   const uint32_t parts = lp_cluster_size(), part = cluster_ctarank();
   const long long row = blockIdx.x / parts;
@@ -412,22 +426,27 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     constexpr int G = sizeof(raw) / 16;
     float m;
     if constexpr (TOP && NT > 64) {
-      float each[G];
-      each[0] = m = lp_largest<T, 0, 1>(raw);
-      if constexpr (G == 4) {
-        each[1] = lp_largest<T, 1, 1>(raw);
-        each[2] = lp_largest<T, 2, 1>(raw);
-        each[3] = lp_largest<T, 3, 1>(raw);
-        m = fmaxf(fmaxf(m, each[1]), fmaxf(each[2], each[3]));
-      }
+      auto note = [&](float v, int first) {                                // the largest of the warp's vectors from `first` on
+        const float s = lp_warp_max(v);
+        const int segment = first >> SEG;
+        if (lane == 0 && first < at.nvec && segment < LpShared<NT>::kSegments) sh.segment[segment] = s;
+      };
+      if constexpr (SEG == 7) {
+        m = lp_largest<T, G>(raw);
+        note(m, i - lane);
+      } else {
+        float each[G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const float s = lp_warp_max(each[g]);
-        const int at_segment = (i - lane + g * NT) >> 5;
-        if (lane == 0 && i + g * NT < at.nvec && at_segment < LpShared<NT>::kSegments) sh.segment[at_segment] = s;
+        for (int g = 0; g < G; ++g) {
+          const uint4 one[1] = {raw[g]};
+          each[g] = lp_largest<T, 1>(one);
+          m = g ? fmaxf(m, each[g]) : each[0];
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) note(each[g], i - lane + g * 32);
       }
     } else {
-      m = lp_largest<T, 0, G>(raw);
+      m = lp_largest<T, G>(raw);
     }
     lp_join_vectors<T, ENT, G>(a, raw, m, c);
     if (rank && m > lt) above += lp_above<T, G>(raw, lt);
@@ -435,17 +454,18 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
       if (m > most || group < 0) { most = m; group = i; }
   };
   if (threadIdx.x < at.head) single(threadIdx.x);
-  int i = threadIdx.x;
-  for (; i - lane + 31 + 3 * NT < at.nvec; i += 4 * NT) {
-    const uint4 raw[4] = {__ldg(q + i), __ldg(q + i + NT), __ldg(q + i + 2 * NT), __ldg(q + i + 3 * NT)};
+  constexpr int NEXT = NT == 64 ? NT : 32;                                // from one of a thread's four vectors to the next
+  int i = NT == 64 ? threadIdx.x : w * 128 + lane;
+  for (; i - lane + 31 + 3 * NEXT < at.nvec; i += 4 * NT) {
+    const uint4 raw[4] = {__ldg(q + i), __ldg(q + i + NEXT), __ldg(q + i + 2 * NEXT), __ldg(q + i + 3 * NEXT)};
     vectors(raw, i);
   }
   // a warp's last vectors, all of them under way at once: what lies behind the row's end counts as minus infinities
   constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-  if (i - lane + NT < at.nvec) {
+  if (i - lane + NEXT < at.nvec) {
     uint4 raw[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) raw[g] = i + g * NT < at.nvec ? __ldg(q + i + g * NT) : make_uint4(none, none, none, none);
+    for (int g = 0; g < 4; ++g) raw[g] = i + g * NEXT < at.nvec ? __ldg(q + i + g * NEXT) : make_uint4(none, none, none, none);
     vectors(raw, i);
   } else if (i - lane < at.nvec) {
     const uint4 raw[1] = {i < at.nvec ? __ldg(q + i) : make_uint4(none, none, none, none)};
@@ -470,7 +490,7 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     if (k > 0) {
       if (!(a.s == a.s)) lp_top_by_passes<T, NT>(p, n, id0, k, sh);      // a NaN or plus infinity, which the maxima on the way do not count
       else if constexpr (NT == 64) lp_top_of_threads<T, NT>(p, n, id0, k, at, most, group, sh);
-      else lp_top_of_segments<T, NT>(p, n, id0, k, at, sh);
+      else lp_top_of_segments<T, NT, SEG>(p, n, id0, k, at, sh);
     }
   }
   // the cluster's CTAs
@@ -758,7 +778,7 @@ static int lp_parts(long long rows, long long bytes) {
 constexpr long long kLpSmallRow = 32768;
 static int lp_slice(int V, int parts) { return ((V + parts - 1) / parts + 31) / 32 * 32; }
 
-template <typename T, bool ENT, int NT, bool TOP>
+template <typename T, bool ENT, int NT, int SEG>
 static cudaError_t lp_rows_launch(int parts, const void* logits, long long rs, long long rows, int V, const long long* tokens, float inv_t, int top, float* lp, float* ent,
                                   long long* rank, long long* top_ids, float* top_lp, void* stats, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
@@ -767,7 +787,7 @@ static cudaError_t lp_rows_launch(int parts, const void* logits, long long rs, l
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = parts > 1;
-  return cudaLaunchKernelEx(&cfg, lp_rows_kernel<T, ENT, NT, TOP>, (const T*)logits, rs, V, parts > 1 ? lp_slice(V, parts) : V, tokens, inv_t, top, lp, ent, rank, top_ids,
+  return cudaLaunchKernelEx(&cfg, lp_rows_kernel<T, ENT, NT, SEG>, (const T*)logits, rs, V, parts > 1 ? lp_slice(V, parts) : V, tokens, inv_t, top, lp, ent, rank, top_ids,
                             top_lp, (float4*)stats);
 }
 
@@ -781,11 +801,16 @@ B200_API int b200_token_logprobs(const void* logits, long long rs, long long row
   // Short rows take CTAs of two warps: what a row costs beside its logits (its token, the meeting of its threads) is then one of many on an SM
   // (20000 x 6400 in bf16: 147 us with 256 threads a row, 95 with 64).
   const bool small = parts == 1 && bytes <= kLpSmallRow;
-#define LP_ROWS(ENT, NT, TOP) B200_CHECK((lp_rows_launch<T, ENT, NT, TOP>(parts, logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)))
+  // A warp notes the largest value of the 128 vectors that it reads at a time where rows have 256 KB or more and reading a segment again for each alternative is a
+  // sixteenth of one at most, else of 32: one maximum of a warp instead of four is what rows of 16 bits with entropies and ranks wait for (3000 x 151936 with
+  // five alternatives 191 us and 203, with 20 of them 231 and 215; 3000 x 131080 with four 169 and 178, 2000 x 65600 80 and 74).
+  const bool wide = (parts > 1 ? lp_slice(V, parts) : V) * (bytes / V) / 16 >= max(2048 * top, 128 * 128);
+#define LP_ROWS(ENT, NT, SEG) B200_CHECK((lp_rows_launch<T, ENT, NT, SEG>(parts, logits, rs, rows, V, tokens, inv_t, top, lp, ent, rank, top_ids, top_lp, stats, st)))
   LP_TYPES(dtype, {
-    if (small) { if (ent) LP_ROWS(true, 64, true); else LP_ROWS(false, 64, true); }
-    else if (top) { if (ent) LP_ROWS(true, 256, true); else LP_ROWS(false, 256, true); }
-    else { if (ent) LP_ROWS(true, 256, false); else LP_ROWS(false, 256, false); }
+    if (small) { if (ent) LP_ROWS(true, 64, 5); else LP_ROWS(false, 64, 5); }
+    else if (!top) { if (ent) LP_ROWS(true, 256, 0); else LP_ROWS(false, 256, 0); }
+    else if (wide) { if (ent) LP_ROWS(true, 256, 7); else LP_ROWS(false, 256, 7); }
+    else { if (ent) LP_ROWS(true, 256, 5); else LP_ROWS(false, 256, 5); }
   });
   B200_LAUNCH_CHECK();
   return 0;

@@ -234,6 +234,45 @@ def test_only_one_gradient_and_none():
         assert not token_logprobs(x, tokens).logprob.requires_grad
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,V", [(150, 140001), (150, 131080), (3, 1100001), (150, 65544), (2, 300000)])
+def test_alternatives_of_long_rows(rows, V, dtype):
+    """Segments of either length, rows at odd addresses, a CTA or a cluster a row: values that are far apart, equal ones across segments and their pieces, rows with few
+    values that are not the lowest, of one value alone, and with more large values than a list holds."""
+    dt = DT[dtype]
+    l = torch.randn(rows, V, device="cuda") * 3
+    r = torch.Generator().manual_seed(V)
+    for i in range(rows):
+        kind = i % 6
+        if kind == 1:
+            l[i] = l[i].clamp_max(0) - 1
+            l[i, torch.randint(0, V, (12,), generator=r).cuda()] = 5.0                       # twelve equal ones, anywhere
+        elif kind == 2:
+            l[i] = -INF
+            l[i, torch.randint(0, V, (3,), generator=r).cuda()] = torch.tensor([1.0, 2.0, 1.0], device="cuda")
+        elif kind == 3:
+            l[i] = -1.5
+        elif kind == 4:
+            l[i] = torch.randint(-3, 3, (V,), generator=r).float().cuda()                    # a sixth of the row is the largest
+        elif kind == 5:
+            at = int(torch.randint(0, V - 4000, (1,), generator=r))
+            l[i, at:at + 4000] = 50 + torch.rand(4000, device="cuda")                        # close together
+    l = l.to(dt)
+    tokens = torch.randint(0, V, (rows,), device="cuda")
+    order = torch.sort(l.float(), dim=1, descending=True, stable=True)[1]
+    lp = torch.log_softmax(l.double(), 1)
+    for top in (1, 5, 8, 9, 32):
+        for more in ({}, {"entropy": True, "rank": True}):
+            got = token_logprobs(l, tokens, top=top, **more)
+            assert torch.equal(got.top_ids, order[:, :top])
+            want = lp.gather(1, got.top_ids)
+            # the sum's error and that of a difference of up to |log p| (2^-22 of it, in 32 bits), as for the token itself
+            bound = sum_error(V) + want.abs().clamp_max(1e4) * 2.0 ** -22 + 2.0 ** -22
+            fine = (got.top_logprobs.double() - want).abs() <= bound
+            assert (fine | (want == -INF) & (got.top_logprobs == -INF)).all()
+
+
 def test_what_log_probabilities_refuse():
     l, t = torch.randn(2, 5), torch.tensor([0, 1])
     for bad in (lambda: token_logprobs(l.double(), t), lambda: token_logprobs(l, t.int()), lambda: token_logprobs(l, t[:1]), lambda: token_logprobs(l, t, top=6),
