@@ -7,11 +7,12 @@
 //                64 values took 21 us, the CTAs' launches). A token outside the table gives zeros
 //   embed_sort   (token, place) pairs by token, places of a token in order: a radix sort by one cluster of eight CTAs, which hold the counts of
 //                a digit in shared memory and read each other's totals there. T ids make 8 T bytes a pass: the sort is bound by its steps'
-//                latencies, and stands beside the next kernel
-//   embed_fill   zeros, the bulk of what is written for a large vocabulary (V D against T D): bound by HBM
+//                latencies (16384 ids in two passes 19 us, 4096 13), and stands beside the next kernel
+//   embed_fill   zeros, the bulk of what is written for a large vocabulary (V D against T D): bound by HBM (151936 x 4096 of 16 bits 164 us, 7.5 TB/s)
 //   embed_sum    a CTA takes L sorted pairs and a slice of the columns, reads their rows of dy once, and writes each token's sum. A token whose
-//                pairs lie in several CTAs leaves a partial sum in each
-//   embed_join   adds the partial sums of such a token, in order
+//                pairs lie in several CTAs leaves a partial sum in each (16384 x 4096 of 16 bits 26 us)
+//   embed_join   adds the partial sums of such a token, in order (8 us)
+// Together, captured: 16384 tokens into 151936 x 4096 in bf16 224 us, 4096 into 30522 x 768 in fp32 27; the lookup of 16384 rows of 4096 in bf16 43 us (6.2 TB/s).
 #include "common.cuh"
 #include "../include/b200_ops.h"
 

@@ -109,6 +109,9 @@ struct W4Params {
 //   kHeadGrads  a logit becomes its gradient, which is stored in 16 bits as D; rows behind the last of `active` become zeros
 //   kHeadRows, kHeadDepth   plain products whose rows, or whose depth, end where `active` says
 // Tokens that are passed over cost nothing so: the others' rows stand first, and how many they are the host need not know.
+// The products stay bound by the tensor cores: sums of 2048 x 4096 x 151936 1.63 ms (1.57 PFLOP/s, the tensor pipe 85 % busy in a smaller one), gradients of 751 rows x 2560 x
+// 50688 152 us (73 %). An accumulator's error is the tensor cores' (4.6e-6 of a log
+// probability at K = 4096); gradients are rounded to 16 bits since the products behind take those.
 enum { kHeadNone = 0, kHeadSums = 1, kHeadGrads = 2, kHeadRows = 3, kHeadDepth = 4 };
 struct HeadParams {
   const int* active;         // how many of the M rows (kHeadDepth: of K) count, at least 1; null: all

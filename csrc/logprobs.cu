@@ -14,7 +14,9 @@
 //   lp_finish      lp, H and what the backward pass needs, from the sums of a row's tiles
 //   lp_active, lp_gather, lp_return   rows whose tokens are not passed over, side by side, and their gradients back where they belong
 //   lp_scale, lp_cast   a power of two for fp16's gradients of single logits, and back
-// Rows of logits are bound by HBM; a 16-bit logit has eight operations beside its exponential.
+// Rows of logits are bound by HBM where log probabilities alone are asked for (3000 x 151936 in bf16 144 us, 6.3 TB/s; gradients of 4096 rows 385, 6.5 TB/s): 6.8 instructions
+// and an exponential a 16-bit logit are just behind it (issue slots 55 % busy, exponential unit 72 %). With entropies, ranks and alternatives instructions
+// bound 16-bit rows (191 us), while rows of 32 bits stay near HBM (1000 x 151936 96 us, with all of them 110).
 #include "logprob_math.cuh"
 #include "../include/b200_ops.h"
 #include <type_traits>

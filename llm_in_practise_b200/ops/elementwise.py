@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _native as nv
 
@@ -368,17 +369,24 @@ class _EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        (flat,) = ctx.saved_tensors
-        tshape, tdtype, has_pos, period, scale, pshape, padding_idx = ctx.meta
-        dout2 = dout if dout.dim() == 2 else dout.reshape(-1, tshape[1])
-        dtable = _embedding_grad(flat, dout2, tshape[0], scale, padding_idx, tdtype) if ctx.needs_input_grad[1] else None
-        dpos = None
-        if has_pos and ctx.needs_input_grad[2]:
-            g = dout2.float().view(-1, period, tshape[1]).sum(0)
-            dpos = torch.zeros(pshape, dtype=torch.float32, device=dout.device)
-            dpos[:period] = g
-            dpos = dpos.to(tdtype)
-        return None, dtable, dpos, None, None, None
+        return (_embedding_backward_once if torch.is_grad_enabled() else _embedding_backward)(ctx, dout)
+
+
+def _embedding_backward(ctx, dout):
+    (flat,) = ctx.saved_tensors
+    tshape, tdtype, has_pos, period, scale, pshape, padding_idx = ctx.meta
+    dout2 = dout if dout.dim() == 2 else dout.reshape(-1, tshape[1])
+    dtable = _embedding_grad(flat, dout2, tshape[0], scale, padding_idx, tdtype) if ctx.needs_input_grad[1] else None
+    dpos = None
+    if has_pos and ctx.needs_input_grad[2]:
+        g = dout2.float().view(-1, period, tshape[1]).sum(0)
+        dpos = torch.zeros(pshape, dtype=torch.float32, device=dout.device)
+        dpos[:period] = g
+        dpos = dpos.to(tdtype)
+    return None, dtable, dpos, None, None, None
+
+
+_embedding_backward_once = once_differentiable(_embedding_backward)          # a second derivative is an error when it is asked for
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, pos_table: Optional[torch.Tensor] = None,

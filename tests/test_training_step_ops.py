@@ -452,6 +452,18 @@ def test_padding_tokens_count_as_torch_counts_them(device):
                 call()
 
 
+@gpu
+def test_embedding_gradient_has_no_derivative():
+    """A graph of the gradient may be asked for; what is refused is to go through it."""
+    table, f = torch.randn(20, 16, device="cuda", requires_grad=True), torch.randn(4, 16, device="cuda", requires_grad=True)
+    ids = torch.tensor([3, 19, 7, 19], device="cuda")
+    (plain,) = torch.autograd.grad((embedding(ids, table) * f).sum(), table)
+    (g,) = torch.autograd.grad((embedding(ids, table) * f).sum(), table, create_graph=True)
+    assert torch.equal(g, plain)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_what_embeddings_refuse():
     table, ids = torch.randn(20, 16), torch.zeros(4, dtype=torch.int64)
     with pytest.raises(ValueError):
