@@ -14,9 +14,9 @@
 //   lp_finish      lp, H and what the backward pass needs, from the sums of a row's tiles
 //   lp_active, lp_gather, lp_return   rows whose tokens are not passed over, side by side, and their gradients back where they belong
 //   lp_scale, lp_cast   a power of two for fp16's gradients of single logits, and back
-// Rows of logits are bound by HBM where log probabilities alone are asked for (3000 x 151936 in bf16 144 us, 6.3 TB/s; gradients of 4096 rows 385, 6.5 TB/s): 6.8 instructions
+// Rows of logits are bound by HBM where log probabilities alone are asked for (3000 x 151936 in bf16 141 us, 6.5 TB/s; gradients of 4096 rows 385, 6.5 TB/s): 6.8 instructions
 // and an exponential a 16-bit logit are just behind it (issue slots 55 % busy, exponential unit 72 %). With entropies, ranks and alternatives instructions
-// bound 16-bit rows (191 us), while rows of 32 bits stay near HBM (1000 x 151936 96 us, with all of them 110).
+// bound 16-bit rows (187 us), while rows of 32 bits stay near HBM (1000 x 151936 95 us, with all of them 107).
 #include "logprob_math.cuh"
 #include "../include/b200_ops.h"
 #include <type_traits>
@@ -39,7 +39,7 @@ template <int NT> struct LpShared : LpSums<NT> {
   uint32_t group[64];
   int chosen[kLpMaxTop];
   unsigned long long bound;
-  int n;
+  int n, more;
 };
 
 template <typename T> struct LpVec { static constexpr int N = 16 / sizeof(T); };
@@ -154,6 +154,38 @@ __device__ __forceinline__ uint32_t lp_cluster_size() {
   return n;
 }
 
+// The largest of a warp's values.
+__device__ __forceinline__ float lp_warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+// The parts that the first LANES lanes hold (the others: nothing, {-inf, 0, 0}) as one: to the largest of all at once, then plain sums.
+template <bool ENT, int LANES>
+__device__ __forceinline__ LpSum lp_warp_sum(LpSum a, float c) {
+  const float m = lp_warp_max(a.m), x = (a.m - (m == -INFINITY ? 0.f : m)) * c, f = lp_exp2(x);
+  if constexpr (ENT) a.u = f * (a.u + a.s * lp_factor(x));
+  a.s *= f;
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    if constexpr (ENT) a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  a.m = m;
+  return a;
+}
+// The k-th largest of 64 numbers, by one warp.
+__device__ __forceinline__ uint32_t lp_kth(const uint32_t* v, int k) {
+  const int lane = threadIdx.x & 31;
+  uint32_t a = v[lane], b = v[lane + 32], most = 0;
+  if (a < b) { const uint32_t x = a; a = b; b = x; }
+  for (int i = 0; i < k; ++i) {
+    most = __reduce_max_sync(0xffffffffu, a);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, a == most)) - 1) { a = b; b = 0; }
+  }
+  return most;
+}
+
 // out[0 .. k) = the k largest of n distinct keys in order; a key's place is the number of larger ones. All threads of the CTA.
 template <int NT>
 __device__ __forceinline__ void lp_sort(const unsigned long long* keys, int n, int k, unsigned long long* out) {
@@ -203,14 +235,11 @@ __device__ __forceinline__ void lp_top_of_threads(const T* __restrict__ p, int n
   // 1. a bound by values alone, so that few threads look up where their largest is: the k-th of the threads'
   const uint32_t own = group < 0 ? 0u : lp_order(most);
   sh.group[threadIdx.x] = own;
-  if (threadIdx.x == 0) { sh.n = 0; sh.bound = 0; }
+  if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  {
-    const uint32_t v = sh.group[threadIdx.x];
-    int before = 0;
-#pragma unroll 16
-    for (int j = 0; j < 64; ++j) before += sh.group[j] > v || (sh.group[j] == v && j < int(threadIdx.x));
-    if (before == k - 1) sh.bound = v;
+  if (threadIdx.x < 32) {
+    const uint32_t v = lp_kth(sh.group, k);
+    if (threadIdx.x == 0) sh.bound = v;
   }
   __syncthreads();
   // 2. those threads' largest with their ids, and which of them are the k largest
@@ -295,14 +324,11 @@ __device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int 
 #pragma unroll
   for (int o = 1; o < EACH; o *= 2) own = max(own, __shfl_xor_sync(0xffffffffu, own, o));
   if (lane % EACH == 0) sh.group[threadIdx.x / EACH] = own;
-  if (threadIdx.x == 0) { sh.n = 0; sh.bound = 0; }
+  if (threadIdx.x == 0) sh.n = sh.more = 0;
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const uint32_t v = sh.group[threadIdx.x];
-    int before = 0;
-#pragma unroll 16
-    for (int j = 0; j < 64; ++j) before += sh.group[j] > v || (sh.group[j] == v && j < int(threadIdx.x));
-    if (before == k - 1) sh.bound = v;
+  if (w == 0) {
+    const uint32_t v = lp_kth(sh.group, k);
+    if (lane == 0) sh.bound = v;
   }
   __syncthreads();
   // 2. the segments not below it, in order: the first k are chosen
@@ -326,11 +352,9 @@ __device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int 
   }
   __syncthreads();
   const float value = sh.segment[sh.chosen[k - 1]];
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
   // 3. their values that are not below the last one's largest, of those equal to it no more than k a segment, a warp a segment
   auto offer = [&](float v, int j) {
-    const int i = atomicAdd(&sh.n, 1);
+    const int i = atomicAdd(&sh.more, 1);
     if (i < CAP) sh.list[i] = lp_key(v, id0 + j);
   };
   for (int b = w; b < k; b += NT / 32) {
@@ -375,16 +399,9 @@ __device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int 
   if (threadIdx.x < at.head && to_f32<T>(p[threadIdx.x]) >= value) offer(to_f32<T>(p[threadIdx.x]), threadIdx.x);
   if (threadIdx.x < n - at.tail && to_f32<T>(p[at.tail + threadIdx.x]) >= value) offer(to_f32<T>(p[at.tail + threadIdx.x]), at.tail + threadIdx.x);
   __syncthreads();
-  const int m = sh.n;
+  const int m = sh.more;
   if (m > CAP || m < k) lp_top_by_passes<T, NT>(p, n, id0, k, sh);       // more than a thousand large values in a few segments
   else lp_sort<NT>(sh.list, m, k, sh.best);
-}
-
-// The largest of a warp's values.
-__device__ __forceinline__ float lp_warp_max(float v) {
-  float m;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-  return m;
 }
 
 // A row by a cluster of CTAs (of one, where there are rows enough), a slice each.
@@ -474,23 +491,22 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     vectors(raw, i);
   }
   if (threadIdx.x < n - at.tail) single(at.tail + threadIdx.x);
-  // the CTA's threads
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = lp_both<ENT>(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)}, c);
+  // the CTA's threads: a warp each, then the first warp for all of them (no other needs what comes out)
+  a = lp_warp_sum<ENT, 32>(a, c);
   above = __reduce_add_sync(0xffffffffu, above);
   if (lane == 0) { sh.red[0][w] = a.m; sh.red[1][w] = a.s; sh.red[2][w] = a.u; sh.redi[w] = above; }
-  __syncthreads();
-  a = {sh.red[0][0], sh.red[1][0], sh.red[2][0]};
-  above = sh.redi[0];
-  for (int x = 1; x < NT / 32; ++x) {
-    a = lp_both<ENT>(a, {sh.red[0][x], sh.red[1][x], sh.red[2][x]}, c);
-    above += sh.redi[x];
+  const bool no_number = __syncthreads_or(a.s != a.s);                    // a NaN or plus infinity, which the maxima on the way do not count
+  if (w == 0) {
+    constexpr int W = NT / 32;
+    a = lane < W ? LpSum{sh.red[0][lane], sh.red[1][lane], sh.red[2][lane]} : LpSum{-INFINITY, 0.f, 0.f};
+    a = lp_warp_sum<ENT, W>(a, c);
+    a = {a.m, __shfl_sync(0xffffffffu, a.s, 0), __shfl_sync(0xffffffffu, a.u, 0)};
+    above = __reduce_add_sync(0xffffffffu, lane < W ? sh.redi[lane] : 0);
   }
   if constexpr (TOP) {
     const int k = min(top, n);
     if (k > 0) {
-      if (!(a.s == a.s)) lp_top_by_passes<T, NT>(p, n, id0, k, sh);      // a NaN or plus infinity, which the maxima on the way do not count
+      if (no_number) lp_top_by_passes<T, NT>(p, n, id0, k, sh);
       else if constexpr (NT == 64) lp_top_of_threads<T, NT>(p, n, id0, k, at, most, group, sh);
       else lp_top_of_segments<T, NT, SEG>(p, n, id0, k, at, sh);
     }
@@ -508,10 +524,8 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
         b = {__uint_as_float(uint32_t(lo)), __uint_as_float(uint32_t(lo >> 32)), __uint_as_float(uint32_t(hi))};
         more = int(uint32_t(hi >> 32));
       }
-#pragma unroll
-      for (int o = kLpMaxCluster / 2; o > 0; o >>= 1)
-        b = lp_both<ENT>(b, {__shfl_xor_sync(0xffffffffu, b.m, o), __shfl_xor_sync(0xffffffffu, b.s, o), __shfl_xor_sync(0xffffffffu, b.u, o)}, c);
-      a = {__shfl_sync(0xffffffffu, b.m, 0), __shfl_sync(0xffffffffu, b.s, 0), __shfl_sync(0xffffffffu, b.u, 0)};
+      b = lp_warp_sum<ENT, kLpMaxCluster>(b, c);
+      a = {b.m, __shfl_sync(0xffffffffu, b.s, 0), __shfl_sync(0xffffffffu, b.u, 0)};
       above = __reduce_add_sync(0xffffffffu, more);
       if constexpr (TOP) {
         for (int e = threadIdx.x; e < int(parts) * top; e += NT) {       // a slice has top alternatives, a short last one fewer: keys of zero, below all
@@ -801,7 +815,7 @@ B200_API int b200_token_logprobs(const void* logits, long long rs, long long row
   const long long bytes = (long long)V * (dtype == B200_DT_FP32 ? 4 : 2);
   const int parts = lp_parts(rows, bytes);
   // Short rows take CTAs of two warps: what a row costs beside its logits (its token, the meeting of its threads) is then one of many on an SM
-  // (20000 x 6400 in bf16: 147 us with 256 threads a row, 95 with 64).
+  // (20000 x 6400 in bf16: 147 us with 256 threads a row, 95 with 64; 51 by now).
   const bool small = parts == 1 && bytes <= kLpSmallRow;
   // A warp notes the largest value of the 128 vectors that it reads at a time where rows have 256 KB or more and reading a segment again for each alternative is a
   // sixteenth of one at most, else of 32: one maximum of a warp instead of four is what rows of 16 bits with entropies and ranks wait for (3000 x 151936 with
