@@ -107,7 +107,7 @@ struct W4Params {
 // it needs of a row stays in that thread.
 //   kHeadSums   the 256 logits of a row and tile become (m, s, u) of logprob_math.cuh in part[tile column][row]; the given token's logit goes to lt[row]
 //   kHeadGrads  a logit becomes its gradient, which is stored in 16 bits as D; rows behind the last of `active` become zeros
-//   kHeadRows, kHeadDepth   plain products whose rows, or whose depth, end where `active` says
+//   kHeadRows, kHeadDepth   plain products whose rows, or whose depth, end where `active` says (kHeadRows also cut along k)
 // Tokens that are passed over cost nothing so: the others' rows stand first, and how many they are the host need not know.
 // The products stay bound by the tensor cores: sums of 2048 x 4096 x 151936 1.63 ms (1.57 PFLOP/s, the tensor pipe 85 % busy in a smaller one), gradients of 751 rows x 2560 x
 // 50688 152 us (73 %). An accumulator's error is the tensor cores' (4.6e-6 of a log
@@ -148,7 +148,7 @@ struct SegmentIter {
   long long item, end;  // stream-K: current / last work item of this unit
   int tile, stride, total_tiles, nkt, grp_size, member;
   bool stream_k;
-  __host__ __device__ SegmentIter(const GemmKernelParams& p, int unit, int nunits, int total_tiles_, int nkt_) {
+  __host__ __device__ SegmentIter(const GemmKernelParams& p, int unit, int nunits, int total_tiles_, int nkt_, int sk_group) {
     stream_k = p.stream_k != 0;
     total_tiles = total_tiles_;
     nkt = nkt_;
@@ -158,7 +158,7 @@ struct SegmentIter {
     // form groups of sk_group members: a group walks one contiguous (panel, k) range and member j computes M-tile j
     // of it, so the members read the same B tiles at the same time (one DRAM fetch, sk_group - 1 L2 hits). With
     // sk_group = 1 this is plain per-tile stream-K.
-    grp_size = p.stream_k ? p.sk_group : 1;
+    grp_size = p.stream_k ? sk_group : 1;
     member = unit % grp_size;
     const int ngroups = nunits / grp_size, grp = unit / grp_size;
     const long long total = (long long)(total_tiles_ / grp_size) * nkt_;
@@ -186,6 +186,9 @@ struct SegmentIter {
     return true;
   }
 };
+
+// stream-K in lock-step groups when the M-tiles of a panel fit a group and at most ~5 % of the units are left without one
+__host__ __device__ __forceinline__ int sk_group_fit(int num_m, int units) { return num_m > 1 && num_m <= units && (units % num_m) * 20 <= units ? num_m : 1; }
 
 // A tile's owner waits for units of higher numbers, which hold its later k-blocks. So the n-th unit to START takes the n-th number from the end: what it
 // waits for has been on an SM before it, waits in its turn only for what started earlier still, and the first one waits for nobody. Whatever else is
@@ -541,6 +544,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
   const int tiles_per_batch = num_m * p.num_n;
   const int total_tiles = tiles_per_batch * p.batch;
   const int num_k_total = num_k + (p.K2 > 0 ? 1 : 0);
+  const int sk_group = HEAD == kHeadRows ? sk_group_fit(num_m, nunits) : p.sk_group;
 
   // ================= TMA producers (every CTA: its own rows of A and its share of B) =========
   // A warp for each operand: one warp for both took 90 cycles to see that a stage is free, 200 for A's box and 120 to 180 for each box of B, 530 a
@@ -558,7 +562,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     const uint32_t box_bytes = EPR * 128;  // MN-major operands: one box = EPR k-rows x 128 B
     const uint32_t fb0 = leader ? full_bar(0) : mapa_shared(full_bar(0), 0);   // the leader's barriers
     bool free = false;
-    SegmentIter it(p, unit, nunits, total_tiles, num_k_total);
+    SegmentIter it(p, unit, nunits, total_tiles, num_k_total, sk_group);
     Segment sg;
     while (it.next(sg)) {
       const int tile = sg.tile;
@@ -635,7 +639,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const int lora_ksteps = (p.K2 + UK - 1) / UK;
       auto desc = [](uint32_t lo) { return ((uint64_t)kDescHi << 32) | (uint64_t)lo; };
       bool full = false;   // whether the stage that comes next was seen full, a k-block ahead
-      SegmentIter it(p, unit, nunits, total_tiles, num_k_total);
+      SegmentIter it(p, unit, nunits, total_tiles, num_k_total, sk_group);
       Segment sg;
       while (it.next(sg)) {
         if (p.b_map && p.b_map[sg.tile / tiles_per_batch] < 0) continue;   // grouped GEMM: unused row tile
@@ -674,7 +678,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     if constexpr (W4) if (lane == 0) {
       int rs = 0;
       uint32_t rphase = 0;
-      SegmentIter it(p, unit, nunits, total_tiles, num_k_total);
+      SegmentIter it(p, unit, nunits, total_tiles, num_k_total, sk_group);
       Segment sg;
       while (it.next(sg)) {
         const int rem = sg.tile % tiles_per_batch;
@@ -710,7 +714,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
       const int gpr = w4->kw / w4->group;     // scale groups per stored row of W
       const uint32_t lut_lane = lut0 + 4u * lane;
       const bool bf = w4->is_bf16 != 0;
-      SegmentIter it(p, unit, nunits, total_tiles, num_k_total);
+      SegmentIter it(p, unit, nunits, total_tiles, num_k_total, sk_group);
       Segment sg;
       while (it.next(sg)) {
         const int rem = sg.tile % tiles_per_batch;
@@ -820,9 +824,9 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
     const int q = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
-    SegmentIter it(p, unit, nunits, total_tiles, num_k_total);
+    SegmentIter it(p, unit, nunits, total_tiles, num_k_total, sk_group);
     Segment sg;
-    const int sk_g = p.stream_k ? p.sk_group : 1;
+    const int sk_g = p.stream_k ? sk_group : 1;
     const int sk_groups = nunits / sk_g, sk_grp = unit / sk_g;
     const long long sk_total = (long long)(total_tiles / sk_g) * num_k_total;
     // fused all-reduce: this CTA's reduction items are ar_next, ar_next + gridDim.x, ... < ar_items (see ar_reduce)
@@ -1118,10 +1122,9 @@ static GemmConfig pick_config(int M, int N, int batch, int nkt, int b_mn, int EP
   return cut.stream_k ? cut : best;
 }
 
-// stream-K in lock-step groups when the M-tiles of a panel fit a group and at most ~5 % of the units are left without one
 static int sk_group_of(int num_m, int units) {
   static const bool sk_flat = getenv("B200_GEMM_SK_FLAT") != nullptr;
-  return num_m > 1 && num_m <= units && (units % num_m) * 20 <= units && !sk_flat ? num_m : 1;
+  return sk_flat ? 1 : sk_group_fit(num_m, units);
 }
 
 template <int ES, int CTAS>
@@ -1184,7 +1187,7 @@ B200_API int b200_gemm_streamk_waits(int M, int N, int K, int batch, int b_mn, i
   int n = 0;
   for (int started = 0; started < nunits; ++started) {
     const int unit = sk_unit_of(started, nunits);
-    SegmentIter it(p, unit, nunits, tiles, nkt);
+    SegmentIter it(p, unit, nunits, tiles, nkt, p.sk_group);
     Segment sg;
     while (it.next(sg)) {
       if (sg.kb0 > 0 || sg.kb1 == nkt) continue;
@@ -1401,13 +1404,21 @@ static GemmConfig head_config(int M, int N, int K) { return pick_config(M, N, 1,
 
 struct HeadOperands { const void *a, *b; long long a_rs, b_rs; int a_mn, b_mn, M, N, K, dtype; void* out; long long out_rs; int out_dtype; float beta; };
 
-static int gemm_head(const HeadOperands& o, HeadParams h, int mode, cudaStream_t stream) {
+// `ws`: a workspace of b200_gemm, or null. With one, products of few rows are cut along k as b200_gemm's are, by the rows that count: each unit then has
+// k-blocks of its own whatever their number (num_n * num_k of them are left with one tile of rows), as an owner waits for every unit between its tile's first and last.
+// 751 of 1001 rows, 2560 x 50688 a product: 160 us, not cut 248, all rows cut 195; both gradients of 2800 of 4000 tokens 8.2 ms, with all rows in dx 9.8.
+static int gemm_head(const HeadOperands& o, HeadParams h, int mode, cudaStream_t stream, void* ws = nullptr, long long ws_bytes = 0) {
   if (o.M <= 0 || o.N <= 0 || o.K <= 0) return B200_ERR_BAD_SHAPE;
   if (o.dtype != B200_DT_BF16 && o.dtype != B200_DT_FP16) return B200_ERR_UNSUPPORTED;
   if (((uintptr_t)o.a | (uintptr_t)o.b) & 15 || o.a_rs % 8 || o.b_rs % 8) return B200_ERR_BAD_ALIGN;
   int rc = device_props();
   if (rc) return rc;
-  const GemmConfig cfg = pick_config(o.M, o.N, 1, ceil_div(o.K, 64), o.b_mn, 64, g_num_sms, false);
+  b200_gemm_args sk = {};
+  sk.workspace = ws; sk.workspace_bytes = ws_bytes;
+  unsigned int* const sk_state = mode == kHeadRows && ws ? sk_state_of(&sk) : nullptr;
+  GemmConfig cfg = pick_config(o.M, o.N, 1, ceil_div(o.K, 64), o.b_mn, 64, g_num_sms, sk_state != nullptr);
+  if (cfg.stream_k && (long long)ceil_div(o.N, cfg.bn) * ceil_div(o.K, 64) < g_num_sms / cfg.ctas)
+    cfg = pick_config(o.M, o.N, 1, ceil_div(o.K, 64), o.b_mn, 64, g_num_sms, false);
   const int ctas = cfg.ctas, bn_cta = cfg.bn / ctas;
   GemmKernelParams p = {};
   p.D = o.out; p.M = o.M; p.N = o.N; p.K = o.K; p.batch = p.nb0 = p.b_div = p.nb0_b = 1;
@@ -1415,6 +1426,12 @@ static int gemm_head(const HeadOperands& o, HeadParams h, int mode, cudaStream_t
   p.a_mn = o.a_mn; p.b_mn = o.b_mn;
   p.num_k = ceil_div(o.K, 64); p.bn = cfg.bn; p.sk_group = 1;
   p.num_m = ceil_div(o.M, kBM * ctas); p.num_n = ceil_div(o.N, p.bn);
+  if (cfg.stream_k) {
+    p.stream_k = 1;
+    p.sk_ws = reinterpret_cast<float*>(ws);
+    p.sk_flags = reinterpret_cast<unsigned int*>(reinterpret_cast<char*>(ws) + (long long)g_num_sms * kBM * kAccStride * 4);
+    p.sk_state = sk_state;
+  }
   const int stage_bytes = kStageABytes + bn_cta * 128;
   p.stages = (g_max_smem - 2048) / stage_bytes;
   if (p.stages > 6) p.stages = 6;
@@ -1434,7 +1451,7 @@ static int gemm_head(const HeadOperands& o, HeadParams h, int mode, cudaStream_t
   const int units = g_num_sms / ctas;
   const long long tiles = (long long)p.num_m * p.num_n;
   if (tiles > 0x7fffffff) return B200_ERR_TOO_LARGE;
-  const int grid = (int)(tiles < units ? tiles : units) * ctas;
+  const int grid = (int)(tiles < units && !p.stream_k ? tiles : units) * ctas;
   const int smem = p.stages * stage_bytes + 8 * (2 * p.stages + 6) + 1024;
 #define HEAD_LAUNCH(MODE) (ctas == 2 ? launch_head<2, MODE>(tmA, tmB, h, p, grid, smem, stream) : launch_head<1, MODE>(tmA, tmB, h, p, grid, smem, stream))
   rc = mode == kHeadSums ? HEAD_LAUNCH(kHeadSums) : mode == kHeadGrads ? HEAD_LAUNCH(kHeadGrads) : mode == kHeadRows ? HEAD_LAUNCH(kHeadRows) : HEAD_LAUNCH(kHeadDepth);
@@ -1468,11 +1485,12 @@ B200_API int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, 
 }
 
 B200_API int b200_gemm_active(const void* a, long long a_rs, int a_mn, const void* b, long long b_rs, int b_mn, int M, int N, int K, int dtype, const int* active,
-                              int depth, void* out, long long out_rs, int out_dtype, float beta, void* stream) {
+                              int depth, void* out, long long out_rs, int out_dtype, float beta, void* workspace, long long workspace_bytes, void* stream) {
   if (!active) return B200_ERR_BAD_SHAPE;
   HeadParams h = {};
   h.active = active;
-  return gemm_head({a, b, a_rs, b_rs, a_mn ? 1 : 0, b_mn ? 1 : 0, M, N, K, dtype, out, out_rs, out_dtype, beta}, h, depth ? kHeadDepth : kHeadRows, (cudaStream_t)stream);
+  return gemm_head({a, b, a_rs, b_rs, a_mn ? 1 : 0, b_mn ? 1 : 0, M, N, K, dtype, out, out_rs, out_dtype, beta}, h, depth ? kHeadDepth : kHeadRows, (cudaStream_t)stream,
+                   workspace, workspace_bytes);
 }
 
 B200_API int b200_gemm_w4(const b200_gemm_args* a, const b200_w4_desc* w, void* stream_) {

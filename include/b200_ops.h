@@ -842,7 +842,7 @@ int b200_gemm_head_grads(const void* x, long long x_rs, const void* w, long long
 /* out [M, N] = a b^T + beta out (16-bit operands, stored transposed where a_mn / b_mn), for the first `active` rows, or where `depth` for the first `active` of K (what
  * stands behind them in a block of 64 must be zeros). */
 int b200_gemm_active(const void* a, long long a_rs, int a_mn, const void* b, long long b_rs, int b_mn, int M, int N, int K, int dtype, const int* active, int depth,
-                     void* out, long long out_rs, int out_dtype, float beta, void* stream);
+                     void* out, long long out_rs, int out_dtype, float beta, void* workspace, long long workspace_bytes, void* stream);
 /* y (16 bits) = x * scale[1] (scale NULL: x). */
 int b200_logprob_cast(const float* x, void* y, long long n, const float* scale, int dtype, void* stream);
 

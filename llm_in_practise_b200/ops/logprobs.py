@@ -19,7 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as nv
-from .gemm import gemm
+from .gemm import _stream_k_workspace, gemm
 
 vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 MAX_TOP = 32             # alternatives of a row
@@ -208,7 +208,7 @@ _COMPACT_ROWS = 256              # more rows than one tile of the products has: 
 _HEAD = [vp, i64, vp, i64, i32, i32, i32, i32, vp]
 _HEAD_SUMS = _HEAD + [vp, f32, i32, vp, vp, vp]
 _HEAD_GRADS = _HEAD + [vp, vp, i32, i32, f32, vp, vp, vp, vp, vp, i64, vp]
-_ACTIVE_GEMM = [vp, i64, i32, vp, i64, i32, i32, i32, i32, i32, vp, i32, vp, i64, i32, f32, vp]
+_ACTIVE_GEMM = [vp, i64, i32, vp, i64, i32, i32, i32, i32, i32, vp, i32, vp, i64, i32, f32, vp, i64, vp]
 _FINISH = [vp, i32, i64, i32, vp, vp, vp, vp, f32, vp, vp, vp, vp]
 _ACTIVE = [vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]
 
@@ -311,21 +311,18 @@ def _linear_backward(x, w, tokens, temperature, saved, g, h, need_dx, need_dw):
     fc = nv.proto("b200_logprob_cast", [vp, vp, i64, vp, i32, vp])
     fa = nv.proto("b200_gemm_active", _ACTIVE_GEMM)
     st = nv.stream()
-    # dx has few tiles where tokens are few: cut along the vocabulary (which the products that end at a count are not) all rows take less time than those that
-    # count (1001 x 2560, 751 rows that count, chunks of 50688: 185 us and 248)
-    plan = (i32 * 4)()
-    if act is not None and need_dx:
-        nv.check(nv.proto("b200_gemm_plan", [i32] * 7 + [vp])(T, K, C, 1, 1, dt, nv.sm_count(dev), ctypes.addressof(plan)), "gemm_plan")
+    ws = _stream_k_workspace(dev) if act is not None else None      # dx has few tiles where tokens are few: it is cut along the vocabulary
+    ws = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
 
     def product(n, depth, c0, out, beta):
         """dl w of the chunk (rows), or dl^T x (depth)."""
         d, wc = dl[:, :n], w[c0:c0 + n]
-        if act is None or (not depth and plan[2]):
+        if act is None:
             gemm(d, x, a_mn=True, b_mn=True, out=out) if depth else gemm(d, wc, b_mn=True, out=out, beta=beta)
             return
         o = (x.data_ptr(), x.stride(0)) if depth else (wc.data_ptr(), w.stride(0))
         rc = fa(dl.data_ptr(), ld, int(depth), *o, 1, n if depth else T, K, T if depth else n, dt, count, int(depth), out.data_ptr(), out.stride(0),
-                nv.dtype_code(out.dtype), beta, st)
+                nv.dtype_code(out.dtype), beta, *ws, st)
         if rc:
             nv.check(rc, "gemm_active")
         nv.count_launch()

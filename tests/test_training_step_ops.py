@@ -341,6 +341,50 @@ def test_from_hidden_states(T, K, V, passed, dtype, device, monkeypatch):
         assert torch.equal(linear_token_logprobs(a, b, tokens.to(device), temperature=tau).logprob, got.logprob)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,K,V", [(1001, 64, 20011), (700, 256, 9000), (1001, 640, 30522), (300, 128, 151936)])
+def test_gradient_of_hidden_states_cut_along_the_vocabulary(T, K, V, dtype):
+    """Few tiles, whose products are cut into parts by the rows that count, from all of them to one and none; the same bits in every call, in a captured one too that
+    is replayed with other rows."""
+    from llm_in_practise_b200.ops.gemm import ensure_graph_workspace
+    dt, tau = DT[dtype], 0.8
+    half, least = half_step(dt)
+    w = (torch.randn(V, K, device="cuda") * 3 / K ** 0.5).to(dt)
+    x = torch.randn(T, K, device="cuda").to(dt).requires_grad_(True)
+    g = torch.randn(T, device="cuda")
+    tokens = torch.randint(0, V, (T,), device="cuda")
+    ensure_graph_workspace(x.device)
+    torch.autograd.grad(linear_token_logprobs(x, w, tokens, temperature=tau).logprob, x, g)          # what a capture needs is there
+    held, graph = tokens.clone(), torch.cuda.CUDAGraph()
+    leaf = x.detach().requires_grad_(True)                 # one that no eager graph holds
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        (replayed,) = torch.autograd.grad(linear_token_logprobs(leaf, w, held, temperature=tau).logprob, leaf, g)
+    logits = x.detach().double() @ w.double().t()
+    logit = (K + 8) * 2.0 ** -24 * float((x.detach().double().abs() @ w.double().abs().t()).max()) / tau
+    p = torch.softmax(logits / tau, 1)
+    del logits
+    # dl: half a step, the logit's error twice (its own and the sum's), the sum's; then V additions in 32 bits
+    rel = half + 2 * logit + 8 * sum_error(V) + V * 2.0 ** -24
+    for passed in (0, T // 4, T * 9 // 10, T - 257, T - 256, T - 1, T):
+        t = tokens.clone()
+        t[torch.randperm(T, device="cuda")[:passed]] = -1
+        keep = (t >= 0).double()[:, None]
+        one = torch.nn.functional.one_hot(t.clamp_min(0), V).double()
+        scale = g.double()[:, None] * keep / tau
+        want, terms = ((one - p) * scale) @ w.double(), ((one + p) * scale.abs()) @ w.double().abs()
+        tiny = 2.0 ** -37 * float(scale.abs().max()) * (keep * w.double().abs().sum(0)) if dt == torch.float16 else 0.0
+        del one
+        (dx,) = torch.autograd.grad(linear_token_logprobs(x, w, t, temperature=tau).logprob, x, g)
+        assert ((dx.double() - want).abs() <= terms * rel + tiny + half * want.abs() + least).all(), passed
+        assert torch.equal(torch.autograd.grad(linear_token_logprobs(x, w, t, temperature=tau).logprob, x, g)[0], dx)
+        held.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, dx) or ((replayed.double() - want).abs() <= terms * rel + tiny + half * want.abs() + least).all(), passed
+
+
 # ------------------------------------------------------------------------------------------------ embedding gradients
 def exact_embedding(ids, dout, rows, scale, pad):
     out = torch.zeros(rows, dout.shape[-1], dtype=torch.float64)
