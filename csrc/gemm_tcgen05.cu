@@ -876,7 +876,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmA, const CUtensor
           tmem_ld_32x32(t0 + c * 32, r);
           tmem_ld_wait();
           if constexpr (HEAD == kHeadSums) {
-            if (at >= col0 && at < col0 + 32) {
+            if (at >= col0 && at < min(col0 + 32, col_limit)) {       // a tile that is an odd number of 16 columns wide ends inside a chunk
               float lt = 0.f;
 #pragma unroll
               for (int j = 0; j < 32; ++j) lt = at == col0 + j ? __uint_as_float(r[j]) : lt;

@@ -385,6 +385,31 @@ def test_gradient_of_hidden_states_cut_along_the_vocabulary(T, K, V, dtype):
         assert torch.equal(replayed, dx) or ((replayed.double() - want).abs() <= terms * rel + tiny + half * want.abs() + least).all(), passed
 
 
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,K,V,width", [(128, 2048, 151936, 208), (1, 2560, 151936, 208), (64, 4096, 50257, 176), (100, 8192, 6400, 48), (37, 8192, 1001, 16)])
+def test_tokens_at_the_ends_of_tiles_of_odd_width(T, K, V, width, dtype):
+    """Tiles of an odd number of 16 columns end inside 32 that are read at a time: the log probability of the next tile's first tokens is that tile's to give."""
+    from llm_in_practise_b200.ops import _native as nv
+    tiles = nv.proto("b200_gemm_head_tiles", [lpm.i32] * 3)(T, V, K)
+    assert [n for n in range(16, 257, 16) if -(-V // n) == tiles] == [width] and width % 32 == 16
+    dt, r = DT[dtype], torch.Generator().manual_seed(V)
+    x, w = torch.randn(T, K, generator=r).to(dt).cuda(), (torch.randn(V, K, generator=r) * 3 / K ** 0.5).to(dt).cuda()
+    logits = x.double() @ w.double().t()
+    want = torch.log_softmax(logits, 1)
+    # as above: the logit's sum in 32 bits (its own and those of the row's sum), the row's sum, the logarithm
+    logit = (K + 8) * 2.0 ** -24 * float((x.double().abs() @ w.double().abs().t()).max())
+    spread = float((logits.amax(1, keepdim=True) - logits).max())
+    for at in range(4):                                     # every row has each of the places
+        places = torch.randint(0, V // width, (T,), generator=r) * width + torch.tensor([0, 15, 16 % width, width - 1])[(torch.arange(T) + at) % 4]
+        tokens = places.clamp_max(V - 1).cuda()
+        e = want.gather(1, tokens[:, None])[:, 0]
+        got = linear_token_logprobs(x, w, tokens).logprob
+        assert ((got.double() - e).abs() <= lp_tolerance({"lp": e}, V, 1.0, spread) + 2 * logit).all()
+        for _ in range(5):
+            assert torch.equal(linear_token_logprobs(x, w, tokens).logprob, got)
+
+
 # ------------------------------------------------------------------------------------------------ embedding gradients
 def exact_embedding(ids, dout, rows, scale, pad):
     out = torch.zeros(rows, dout.shape[-1], dtype=torch.float64)
