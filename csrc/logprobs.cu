@@ -470,7 +470,7 @@ lp_rows_kernel(const T* __restrict__ logits, long long rs, int V, int slice, con
     lp_join_vectors<T, ENT, G>(a, raw, m, c);
     if (rank && m > lt) above += lp_above<T, G>(raw, lt);
     if constexpr (TOP && NT == 64)
-      if (m > most || group < 0) { most = m; group = i; }
+      if (i < at.nvec && (m > most || group < 0)) { most = m; group = i; }      // (a warp's last lanes may have no vector: what they would note lies behind the row)
   };
   if (threadIdx.x < at.head) single(threadIdx.x);
   constexpr int NEXT = NT == 64 ? NT : 32;                                // from one of a thread's four vectors to the next
