@@ -198,15 +198,16 @@ __device__ __forceinline__ void lp_sort(const unsigned long long* keys, int n, i
   __syncthreads();
 }
 
-// The k largest keys of p[0 .. n) (ids from id0 on) into sh.best, one pass a key: for what the shorter way below does not take.
+// The k largest keys of p[0 .. n) (ids from id0 on) into sh.best, one pass a key: for what the shorter way below does not take. (The first pass has no key to stay
+// below: that of a NaN at id 0 has all bits set, so no start value is above it.)
 template <typename T, int NT>
 __device__ __noinline__ void lp_top_by_passes(const T* __restrict__ p, int n, int id0, int k, LpShared<NT>& sh) {
-  unsigned long long last = ~0ull;
+  unsigned long long last = 0;
   for (int i = 0; i < k; ++i) {
     unsigned long long best = 0;
     for (int j = threadIdx.x; j < n; j += NT) {
       const unsigned long long key = lp_key(to_f32<T>(p[j]), id0 + j);
-      if (key < last && key > best) best = key;
+      if ((i == 0 || key < last) && key > best) best = key;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {

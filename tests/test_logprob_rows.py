@@ -85,3 +85,37 @@ def test_alternatives_of_short_rows(V, dtype, device):
             bound = 2.0 ** -22 + (72 + V / 64 + 64) * 2.0 ** -24 + want.abs().clamp_max(1e4) * 2.0 ** -22 + 2.0 ** -22
             same = (want == -INF) & (seen == -INF) | want.isnan() & seen.isnan()
             assert (((seen - want).abs() <= bound) | same).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,V", [(6, 1), (6, 5), (6, 32), (6, 33), (6, 1001), (330, 20000), (6, 50257), (2, 151936)])
+def test_nan_comes_before_all_others(rows, V, dtype, device):
+    """A NaN at token 0, in a few places, at the end, and a row of NaN alone, up to as many alternatives as there are tokens: in rows by 64 threads, by 256 and by clusters of
+    CTAs. Every log probability is NaN."""
+    if device == "cpu" and rows * V > 400000:
+        pytest.skip("the kernels' sizes")
+    r = torch.Generator().manual_seed(V)
+    nan = float("nan")
+    l = torch.randn(rows, V, generator=r)
+    for i in range(rows):
+        kind = (i + 4 * (rows == 2)) % 6
+        if kind == 0:
+            l[i, 0] = nan
+        elif kind == 1:
+            l[i, V - 1] = nan
+        elif kind == 2:
+            l[i, ::max(1, V // 3)] = nan
+        elif kind == 3:
+            l[i] = -INF
+            l[i, 0] = nan
+        elif kind == 4:
+            l[i] = nan
+        else:
+            l[i, 0] = -nan
+    l = l.to(DT[dtype]).to(device)
+    x = l.float()
+    order = torch.sort(torch.where(x.isnan(), torch.full_like(x, nan), x), dim=1, descending=True, stable=True)[1]        # NaN above all, the lowest id first
+    for top in sorted({1, min(2, V), min(5, V), min(32, V)}):
+        got = token_logprobs(l, top=top)
+        assert torch.equal(got.top_ids, order[:, :top]) and got.top_logprobs.isnan().all()
