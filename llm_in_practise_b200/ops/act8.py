@@ -10,10 +10,12 @@ The reference's scripts train with ``gradient_checkpointing=True`` (Fine-Tuning/
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Callable, NamedTuple, Optional, Tuple
 
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from . import _native as nv
 
@@ -198,7 +200,7 @@ class _Checkpoint8Fn(torch.autograd.Function):
         ctx.run, ctx.n_in = run, 1 + (residual is not None)
         ctx.draws, ctx.autocast = _draws(delta), _autocast(delta.device.type)
         p = pack8(delta, residual)
-        with torch.no_grad():
+        with torch.no_grad(), _no_draws(delta):
             out = run(delta, residual)
         if not isinstance(out, tuple) or not all(isinstance(t, torch.Tensor) for t in out):
             raise TypeError("checkpoint8: the layer must return a tuple of tensors")
@@ -214,7 +216,7 @@ class _Checkpoint8Fn(torch.autograd.Function):
         now = _draws(x)
         try:                                             # dropout masks of the layer are those of its forward
             _set_draws(ctx.draws)
-            with torch.enable_grad(), torch.autocast(x.device.type, **ctx.autocast):
+            with torch.enable_grad(), torch.autocast(x.device.type, **ctx.autocast), _no_draws(x):
                 out = ctx.run(x, None)
         finally:
             _set_draws(now)
@@ -228,10 +230,43 @@ def _autocast(device):
     return {"enabled": torch.is_autocast_enabled(device), "dtype": torch.get_autocast_dtype(device), "cache_enabled": torch.is_autocast_cache_enabled()}
 
 
+def _capturing(x):
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+class _NoDraws(TorchDispatchMode):
+    """Torch's operators that draw random numbers on a device are errors."""
+
+    def __init__(self, device):
+        super().__init__()
+        self.device = device
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if torch.Tag.nondeterministic_seeded in func.tags and self._drew(func, args, kwargs or {}):
+            if any(isinstance(t, torch.Tensor) and t.device == self.device for t in (out if isinstance(out, (tuple, list)) else [out])):
+                raise RuntimeError(f"checkpoint8: while a graph is captured the layer may not draw from torch's generator ({func}): what its forward drew could not "
+                                   "be drawn again for the gradients; ops.elementwise.dropout can")
+        return out
+
+    @staticmethod
+    def _drew(func, args, kwargs):
+        """Attention counts as drawing, whatever its dropout."""
+        for i, a in enumerate(func._schema.arguments):
+            if a.name == "dropout_p":
+                return bool(args[i] if i < len(args) else kwargs.get(a.name, a.default_value))
+        return True
+
+
+def _no_draws(x):
+    """Torch's generator on x's device can neither be asked nor set where a capture is under way; so nothing may draw from it there."""
+    return _NoDraws(x.device) if _capturing(x) else contextlib.nullcontext()
+
+
 def _draws(x):
-    """Where the streams of random numbers stand: the package's own, torch's on the host and on x's device (which a capture forbids to ask)."""
+    """Where the streams of random numbers stand: the package's own, torch's on the host and on x's device (None in a capture, ``_no_draws``)."""
     from . import elementwise as ew
-    cuda = torch.cuda.get_rng_state(x.device) if x.is_cuda and not torch.cuda.is_current_stream_capturing() else None
+    cuda = torch.cuda.get_rng_state(x.device) if x.is_cuda and not _capturing(x) else None
     return dict(ew._seed_state), torch.get_rng_state(), cuda, x.device
 
 
@@ -247,7 +282,8 @@ def _set_draws(state):
 def checkpoint8(layer: Callable, delta: torch.Tensor, residual: Optional[torch.Tensor], *args) -> Tuple[torch.Tensor, ...]:
     """``layer(delta, residual, *args)`` -> tuple of tensors, where the layer needs its first two arguments only as ``delta + residual`` (a branch and the stream
     it is added to; ``residual`` None: delta is the stream). Keeps that sum in 8 bits and runs the layer again on it for the gradients: results are those of a
-    plain call, gradients those of the layer at what was kept. ``args`` get no gradients; parameters of the layer do, in place, as by ``backward()``."""
+    plain call, gradients those of the layer at what was kept. ``args`` get no gradients; parameters of the layer do, in place, as by ``backward()``. In a captured step the layer
+    may draw random numbers from ``ops.elementwise.dropout`` and on the host, but not from torch's generator on the device: that is an error."""
     if not torch.is_grad_enabled():
         return layer(delta, residual, *args)
     anchor = delta.new_empty(0, dtype=torch.float32).requires_grad_(True)      # so that a frozen input layer does not end the graph here

@@ -777,6 +777,64 @@ def test_checkpoints_take_layers_that_return_tuples_and_keep_autocast():
     assert seen == [torch.bfloat16, torch.bfloat16] and x.grad is not None
 
 
+@pytest.mark.parametrize("name", ["dropout", "bernoulli", "rand_like", "attention with dropout"])
+def test_checkpoints_in_a_capture_refuse_torchs_random_numbers(name, monkeypatch):
+    """In the forward and, where the forward ran before the capture, in the backward pass; a layer that draws nothing, or from another device's stream, is taken."""
+    F = torch.nn.functional
+    draw = {"dropout": lambda x: F.dropout(x, 0.5), "bernoulli": lambda x: x * torch.bernoulli(torch.full_like(x, 0.5)), "rand_like": lambda x: x * torch.rand_like(x),
+            "attention with dropout": lambda x: F.scaled_dot_product_attention(x[None], x[None], x[None], dropout_p=0.5)[0]}[name]
+    x = torch.randn(4, 32, requires_grad=True)
+    still = lambda d, r: (F.scaled_dot_product_attention(d[None], d[None], d[None])[0] + F.dropout(d, 0.5, training=False), d)  # noqa: E731
+    y = checkpoint8(lambda d, r: (draw(d), d), x, None)[0]
+    monkeypatch.setattr(act8, "_capturing", lambda t: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="captured"):
+        checkpoint8(lambda d, r: (draw(d), d), x, None)
+    checkpoint8(still, x, None)[0].sum().backward()
+    assert torch.isfinite(x.grad).all()
+    monkeypatch.setattr(act8, "_no_draws", lambda t: act8._NoDraws(torch.device("meta")))
+    checkpoint8(lambda d, r: (draw(d), d), x, None)[0].sum().backward()
+
+
+@gpu
+def test_captured_checkpoints():
+    """A captured step gives the gradients of an eager one, whose dropout is the package's; one that draws from torch's generator is an error, and the capture after it is
+    as any other."""
+    D = 64
+    layer, ga = Layer(D, 0.5).cuda(), torch.randn(5, D, device="cuda")
+    x = torch.randn(5, D, device="cuda")
+
+    def step(x):
+        ew.manual_seed(3)
+        leaf = x.detach().requires_grad_(True)
+        y = checkpoint8(layer, leaf, None)[0]
+        y.backward(ga)
+        return y.detach(), leaf.grad
+    want = [t.clone() for t in step(x)]
+    dw = layer.w.grad.clone()
+    layer.w.grad = None
+    y = checkpoint8(lambda d, r: (torch.nn.functional.dropout(d, 0.5), d), x.requires_grad_(True), None)[0]     # eagerly: under the same mask
+    y.sum().backward()
+    kept = unpack8(pack8(x.detach()))
+    assert torch.equal(x.grad != 0, y.detach() != 0) and torch.equal(x.grad[x.grad != 0], torch.full_like(kept, 2.0)[x.grad != 0])
+    x = x.detach()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            checkpoint8(lambda d, r: (torch.nn.functional.dropout(d, 0.5), d), x.detach().requires_grad_(True), None)
+    graph = torch.cuda.CUDAGraph()
+    layer.w.grad = torch.zeros_like(layer.w)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step(x)
+    for _ in range(2):
+        layer.w.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(layer.w.grad, dw)
+
+
 def test_second_derivatives_are_refused():
     x = torch.randn(3, 64, requires_grad=True)
     for f in (lambda: token_logprobs(x, torch.tensor([0, 1, 2])).logprob, lambda: linear_token_logprobs(x, torch.randn(9, 64), torch.tensor([0, 1, 2])).logprob,
