@@ -317,6 +317,8 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
 
                 def logprobs():                            # those of the tokens since the last chunk
                     nonlocal told
+                    if r.cfg.logprobs is None:             # nobody asks: nothing is decoded for them
+                        return None
                     a, told = told, len(acc)
                     return said(eng, r, (a, told), completion_logprobs, len(decode(eng, acc[:a])))
                 for tok in r.tokens():

@@ -120,6 +120,30 @@ def test_server_streams_logprobs(client):
     assert [t for p in parts for t in p["tokens"]] == whole["tokens"]
 
 
+class Counting(ByteTokenizer):
+    """How often it was asked for text."""
+
+    def decode(self, *args, **kw):
+        self.decoded = getattr(self, "decoded", 0) + 1
+        return super().decode(*args, **kw)
+
+
+@pytest.fixture(scope="module")
+def counting(model):
+    eng = LLMEngine(model, Counting(), EngineArgs(max_num_seqs=2, max_model_len=128)).start()
+    yield TestClient(build_app(eng)), eng.tokenizer
+    eng.shutdown()
+
+
+def test_streams_without_logprobs_decode_a_token_once(counting):
+    """The text behind each token, and the whole once more at the end, in both forms of a stream."""
+    client, tok = counting
+    for path, body in (("/v1/completions", {"prompt": "ab"}), ("/v1/chat/completions", {"messages": [{"role": "user", "content": "hi"}]})):
+        tok.decoded = 0
+        r = client.post(path, json={"model": "m", "max_tokens": 40, "temperature": 0, "ignore_eos": True, "stream": True, **body})
+        assert r.status_code == 200 and tok.decoded == 41
+
+
 def test_server_logprobs_end_at_a_stop_string(client):
     body = {"model": "m", "prompt": "ab", "max_tokens": 9, "temperature": 0, "ignore_eos": True, "logprobs": 0}
     free = client.post("/v1/completions", json=body).json()["choices"][0]
