@@ -18,6 +18,7 @@ from __future__ import annotations
 import json
 import time
 import uuid
+from bisect import bisect_left
 from typing import Any, Dict, List, Optional, Union
 
 from fastapi import FastAPI, HTTPException
@@ -197,10 +198,12 @@ def build_app(engine: Optional[LLMEngine], prompt_style: str = "chatml", allow_s
         return None if r.cfg.logprobs is None else form(r.logprobs[n[0]:n[1]], lambda i: decode(eng, [i]), *at)
 
     def tokens_of(eng: LLMEngine, ids: List[int], stops: List[str]) -> int:
-        """How many tokens the text up to a stop string takes."""
-        if not stops:
+        """How many tokens the text up to a stop string takes; all of them where none is in it. What a text has it still has with more tokens, so halves are tried."""
+        def stopped(n):
+            return cut_at_stop(decode(eng, ids[:n]), stops)[1]
+        if not stops or not stopped(len(ids)):
             return len(ids)
-        return next((n for n in range(1, len(ids) + 1) if cut_at_stop(decode(eng, ids[:n]), stops)[1]), len(ids))
+        return 1 + bisect_left(range(1, len(ids) + 1), True, key=stopped)
 
     def gen_cfg(temperature, top_p, max_tokens, top_k=0, rep=1.0, ignore_eos=False, req=None) -> GenerationConfig:
         """``req``: the request that rules on logits are taken from (OpenAI's penalties and logit_bias, vLLM's allowed_token_ids)."""

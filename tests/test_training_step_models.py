@@ -131,13 +131,13 @@ class Counting(ByteTokenizer):
 @pytest.fixture(scope="module")
 def counting(model):
     eng = LLMEngine(model, Counting(), EngineArgs(max_num_seqs=2, max_model_len=128)).start()
-    yield TestClient(build_app(eng)), eng.tokenizer
+    yield TestClient(build_app(eng)), eng.tokenizer, eng
     eng.shutdown()
 
 
 def test_streams_without_logprobs_decode_a_token_once(counting):
     """The text behind each token, and the whole once more at the end, in both forms of a stream."""
-    client, tok = counting
+    client, tok, _ = counting
     for path, body in (("/v1/completions", {"prompt": "ab"}), ("/v1/chat/completions", {"messages": [{"role": "user", "content": "hi"}]})):
         tok.decoded = 0
         r = client.post(path, json={"model": "m", "max_tokens": 40, "temperature": 0, "ignore_eos": True, "stream": True, **body})
@@ -152,6 +152,27 @@ def test_server_logprobs_end_at_a_stop_string(client):
         pytest.skip("no token of this model is text by itself")
     c = client.post("/v1/completions", json={**body, "stop": free["logprobs"]["tokens"][at]}).json()["choices"][0]
     assert c["finish_reason"] == "stop" and len(c["logprobs"]["tokens"]) <= at + 1
+
+
+def test_the_token_of_a_stop_string_is_found_by_halves(counting, monkeypatch):
+    """As many tokens as a walk from the first one on takes, wherever the stop string is, with some ten decodes beside those of the tokens' own texts."""
+    client, tok, eng = counting
+    submit, reqs = eng.submit, []
+    monkeypatch.setattr(eng, "submit", lambda *a, **k: reqs.append(submit(*a, **k)) or reqs[-1])
+    body = {"model": "m", "prompt": "ab", "max_tokens": 100, "temperature": 0, "ignore_eos": True, "logprobs": 0}
+    free = client.post("/v1/completions", json=body).json()["choices"][0]
+    text, tokens = free["text"], free["logprobs"]["tokens"]
+    assert len(tokens) == 100
+    places = [at for at in range(0, len(text), 7) if "\ufffd" not in text[at:at + 2]] + [None]
+    assert len(places) > 3
+    for at in places:
+        stop = "not in it" if at is None else text[at:at + 2]
+        tok.decoded = 0
+        c = client.post("/v1/completions", json={**body, "stop": stop}).json()["choices"][0]
+        n = len(c["logprobs"]["tokens"])
+        assert c["text"] == text[:text.index(stop) if at is not None else None] and c["finish_reason"] == ("length" if at is None else "stop")
+        assert tok.decoded <= 2 + 7 + n                      # 100 places are halved 7 times
+        assert n == next((i for i in range(1, 101) if stop in ByteTokenizer().decode(reqs[-1].output_ids[:i], skip_special_tokens=True)), 100)
 
 
 def test_generate_returns_log_probabilities(model):
