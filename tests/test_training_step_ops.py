@@ -499,6 +499,16 @@ def test_embedding_lookup(T, D, dtype):
     assert torch.equal(embedding(ids, wide[:, :D]), wide[:, :D][ids])
 
 
+@gpu
+@pytest.mark.parametrize("L", [1, 2, 3, 5, 7, 64, 100, 255, 256, 257, 1000, 4097, 20011])
+def test_positions_of_any_period(L):
+    """Each row has its own position's: a sum of two numbers of 32 bits, rounded once."""
+    for dt in (torch.float32, torch.bfloat16):
+        table, pos = torch.randn(50, 8, device="cuda").to(dt), torch.randn(L + 3, 8, device="cuda").to(dt)
+        ids = torch.randint(0, 50, (-(-40000 // L), L), device="cuda")
+        assert torch.equal(embedding(ids, table, pos), (table.float()[ids] + pos[:L].float()).to(dt))
+
+
 def test_what_embedding_gradients_refuse():
     ids, d = torch.zeros(3, dtype=torch.int64), torch.randn(3, 4)
     for bad in (lambda: embedding_grad(ids.int(), d, 5), lambda: embedding_grad(ids[:2], d, 5), lambda: embedding_grad(ids, d.double(), 5), lambda: embedding_grad(ids, d, 0),
