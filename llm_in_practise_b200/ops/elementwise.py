@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -289,7 +290,14 @@ def dropout(x: torch.Tensor, p: float, training: bool = True, seed: Optional[int
 # embedding
 # ------------------------------------------------------------------------------------------------
 _EMBEDDING_GRAD = [vp, vp, i64, vp, i64, i32, i32, f32, i64, i32, i32, vp, vp]
-_embedding_work = {}                 # bytes of a workspace by tokens and columns
+
+
+@lru_cache(maxsize=128)
+def _embedding_work(tokens: int, columns: int) -> int:
+    """Bytes of a gradient's workspace."""
+    fn = nv.lib().b200_embedding_grad_workspace
+    fn.argtypes, fn.restype = [i64, i32], i64
+    return fn(tokens, columns)
 
 
 def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -323,12 +331,7 @@ def _embedding_grad(flat, d2, rows, scale, padding_idx, dtype):
     if D > 1 and d2.stride(1) != 1:
         d2 = d2.contiguous()
     out = d2.new_empty((rows, D), dtype=dtype)
-    size = _embedding_work.get((T, D))
-    if size is None:
-        fn = nv.lib().b200_embedding_grad_workspace
-        fn.argtypes, fn.restype = [i64, i32], i64
-        size = _embedding_work[T, D] = fn(T, D)
-    work = d2.new_empty((size,), dtype=torch.uint8)
+    work = d2.new_empty((_embedding_work(T, D),), dtype=torch.uint8)
     rc = nv.call_on(d2.device, nv.proto("b200_embedding_grad", _EMBEDDING_GRAD), flat.data_ptr(), d2.data_ptr(), d2.stride(0) if T > 1 else D, out.data_ptr(), T,
                     rows, D, float(scale), -1 if padding_idx is None else padding_idx, nv.dtype_code(d2.dtype), nv.dtype_code(dtype), work.data_ptr())
     if rc:

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from llm_in_practise_b200.ops import act8, elementwise as ew, logprobs as lpm
+from llm_in_practise_b200.ops import _native as nv, act8, elementwise as ew, logprobs as lpm
 from llm_in_practise_b200.ops.act8 import Packed8, checkpoint8, pack8, swiglu8, unpack8
 from llm_in_practise_b200.ops.elementwise import embedding, embedding_grad
 from llm_in_practise_b200.ops.logprobs import linear_token_logprobs, token_logprobs
@@ -390,7 +390,6 @@ def test_gradient_of_hidden_states_cut_along_the_vocabulary(T, K, V, dtype):
 @pytest.mark.parametrize("T,K,V,width", [(128, 2048, 151936, 208), (1, 2560, 151936, 208), (64, 4096, 50257, 176), (100, 8192, 6400, 48), (37, 8192, 1001, 16)])
 def test_tokens_at_the_ends_of_tiles_of_odd_width(T, K, V, width, dtype):
     """Tiles of an odd number of 16 columns end inside 32 that are read at a time: the log probability of the next tile's first tokens is that tile's to give."""
-    from llm_in_practise_b200.ops import _native as nv
     tiles = nv.proto("b200_gemm_head_tiles", [lpm.i32] * 3)(T, V, K)
     assert [n for n in range(16, 257, 16) if -(-V // n) == tiles] == [width] and width % 32 == 16
     dt, r = DT[dtype], torch.Generator().manual_seed(V)
@@ -529,6 +528,15 @@ def test_padding_tokens_count_as_torch_counts_them(device):
         for call in (lambda: embedding(ids, table, padding_idx=pad), lambda: embedding_grad(ids, dout, 20, padding_idx=pad)):
             with pytest.raises(ValueError):
                 call()
+
+
+@pytest.mark.skipif(not nv.lib_path().exists(), reason="no kernel library here")
+def test_sizes_of_workspaces_are_not_kept_for_ever():
+    """Batches of other lengths every step; pairs of ids twice and two partial sums a tile, of 32 pairs at least, are what a workspace holds."""
+    for T in range(1, 1000):
+        n = ew._embedding_work(T, 40)
+        assert 2 * 8 * T + 2 * 4 * 40 * -(-T // 32) <= n < 2 * (8 * T + 16) + 2 * 4 * 40 * -(-T // 32) + 1
+    assert ew._embedding_work.cache_info().currsize <= 128 and ew._embedding_work(0, 40) >= 16
 
 
 @gpu
