@@ -436,38 +436,8 @@ __global__ void gelu_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------------
-// Embedding: out[t, :] = table[ids[t], :] (+ pos_table[t % period, :]); grad scatter-add (fp32 atomics)
+// Sums of rows into an fp32 table by atomics, for callers of the C interface that add into a gradient they have (embedding.cu: a whole gradient, the same bits every time)
 // ---------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void embedding_fwd_kernel(const long long* __restrict__ ids, const T* __restrict__ table,
-                                     const T* __restrict__ pos_table, T* __restrict__ out, long long tokens, int dim,
-                                     int period, float scale) {
-  pdl_launch_dependents();
-  pdl_wait();
-  constexpr int V = 16 / sizeof(T);
-  const long long t = blockIdx.x;
-  const long long id = ids[t];
-  const T* src = table + id * dim;
-  const T* ps = pos_table ? pos_table + (t % period) * dim : nullptr;
-  for (int i = threadIdx.x * V; i < dim; i += blockDim.x * V) {
-    float v[V];
-    uint4 raw = *reinterpret_cast<const uint4*>(src + i);
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = to_f32<T>(e[j]) * scale;
-    if (ps) {
-      uint4 pr = *reinterpret_cast<const uint4*>(ps + i);
-      const T* pe = reinterpret_cast<const T*>(&pr);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] += to_f32<T>(pe[j]);
-    }
-    uint4 o;
-    T* oe = reinterpret_cast<T*>(&o);
-#pragma unroll
-    for (int j = 0; j < V; ++j) oe[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<uint4*>(out + t * dim + i) = o;
-  }
-}
 template <typename T>
 __global__ void embedding_bwd_kernel(const long long* __restrict__ ids, const T* __restrict__ dout,
                                      float* __restrict__ dtable, long long tokens, int dim, float scale) {
@@ -618,17 +588,6 @@ B200_API int b200_gelu_bwd(const void* dy, const void* x, void* dx, long long n,
   return 0;
 }
 
-B200_API int b200_embedding_fwd(const long long* ids, const void* table, const void* pos_table, void* out,
-                                long long tokens, int dim, int period, float scale, int dtype, void* stream) {
-  const int V = dtype == B200_DT_FP32 ? 4 : 8;
-  if (dim % V || tokens <= 0) return B200_ERR_BAD_SHAPE;
-  int tb = dim / V;
-  tb = tb > 256 ? 256 : (tb < 32 ? 32 : (tb + 31) / 32 * 32);
-  B200_DISPATCH_T(dtype, launch_pdl(embedding_fwd_kernel<T>, (unsigned)tokens, tb, 0, (cudaStream_t)stream, 
-      ids, (const T*)table, (const T*)pos_table, (T*)out, tokens, dim, period > 0 ? period : 1, scale));
-  B200_LAUNCH_CHECK();
-  return 0;
-}
 namespace b200 {
 // out[t, c] = table[ids[t], c] * scale + pos_table[pos[t], c]: embedding rows entering an fp32 stream with an additive
 // position table (fp32, built on the host) indexed by every token's own position, or without one (NULL)

@@ -351,6 +351,13 @@ B200_API int b200_embedding_lookup(const long long* ids, const void* table, cons
   return 0;
 }
 
+// The same without the table's number of rows: every id that is not below zero is taken for one of them.
+B200_API int b200_embedding_fwd(const long long* ids, const void* table, const void* pos_table, void* out, long long T, int D, int period, float scale, int dtype,
+                                void* stream) {
+  if (T <= 0) return B200_ERR_BAD_SHAPE;
+  return b200_embedding_lookup(ids, table, pos_table, out, T, 0x7fffffff, D, period > 0 ? period : 1, scale, dtype, stream);
+}
+
 B200_API long long b200_embedding_grad_workspace(long long T, int D) {
   if (T <= 0 || D <= 0) return 16;
   const long long tiles = ceil_div64(T, es_tile(T));

@@ -191,11 +191,14 @@ int b200_swiglu_fwd(const void* gu, void* h, long long rows, int F, int dtype, v
 int b200_swiglu_bwd(const void* dh, const void* gu, void* dgu, long long rows, int F, int dtype, void* stream);
 int b200_gelu_fwd(const void* x, void* y, long long n, int dtype, void* stream);
 int b200_gelu_bwd(const void* dy, const void* x, void* dx, long long n, int dtype, void* stream);
+/* b200_embedding_lookup (below) without the number of rows: ids from 0 to 2^31 - 2 are taken to be in the table. */
 int b200_embedding_fwd(const long long* ids, const void* table, const void* pos_table, void* out, long long tokens,
                        int dim, int period, float scale, int dtype, void* stream);
 /* out fp32 [tokens, dim] = table[ids[t]] * scale + pos_table[pos[t]] (pos_table fp32 [positions, dim]). */
 int b200_embedding_pos(const long long* ids, const void* table, float scale, const int* pos, const float* pos_table, float* out,
                        long long tokens, int dim, int dtype, void* stream);
+/* dtable fp32 [rows, dim] += scale * dout [tokens, dim] by ids, all of which are in the table, in the order in which atomics arrive (b200_embedding_grad: a gradient as a
+ * whole, the same bits in every call). */
 int b200_embedding_bwd(const long long* ids, const void* dout, float* dtable, long long tokens, int dim, float scale,
                        int dtype, void* stream);
 int b200_dropout(const void* x, void* y, long long n, unsigned long long seed, float p, int dtype, void* stream);

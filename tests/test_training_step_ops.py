@@ -540,6 +540,24 @@ def test_sizes_of_workspaces_are_not_kept_for_ever():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DT)
+def test_embeddings_of_the_c_interface(dtype):
+    """What a C caller has had: rows without the table's number of rows, sums that are added to an fp32 table."""
+    dt, T, D = DT[dtype], 300, 72
+    table, pos, ids = torch.randn(50, D, device="cuda").to(dt), torch.randn(100, D, device="cuda").to(dt), torch.randint(0, 50, (T,), device="cuda")
+    out, vp, i64, i32, f32 = torch.empty(T, D, dtype=dt, device="cuda"), lpm.vp, lpm.i64, lpm.i32, lpm.f32
+    fwd, bwd = nv.proto("b200_embedding_fwd", [vp, vp, vp, vp, i64, i32, i32, f32, i32, vp]), nv.proto("b200_embedding_bwd", [vp, vp, vp, i64, i32, f32, i32, vp])
+    for p in (None, pos):
+        assert fwd(ids.data_ptr(), table.data_ptr(), nv.ptr(p), out.data_ptr(), T, D, 100, 1.0, nv.dtype_code(dt), nv.stream()) == 0
+        assert torch.equal(out, embedding(ids.view(3, 100), table, p).view(T, D))
+    start, dout = torch.randn(50, D, device="cuda"), torch.randn(T, D, device="cuda").to(dt)
+    got, (want, size, n) = start.clone(), exact_embedding(ids, dout.cpu(), 50, 1.5, -1)
+    assert bwd(ids.data_ptr(), dout.data_ptr(), got.data_ptr(), T, D, 1.5, nv.dtype_code(dt), nv.stream()) == 0
+    want, size = want + start.cpu().double(), size + start.cpu().double().abs()
+    assert ((got.cpu().double() - want).abs() <= (n + 2) * 2.0 ** -24 * size).all()          # n products and sums in 32 bits
+
+
+@gpu
 def test_embedding_gradient_has_no_derivative():
     """A graph of the gradient may be asked for; what is refused is to go through it."""
     table, f = torch.randn(20, 16, device="cuda", requires_grad=True), torch.randn(4, 16, device="cuda", requires_grad=True)
