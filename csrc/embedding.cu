@@ -1,9 +1,9 @@
 // An embedding lookup y[t] = s W[id_t] (+ P[t mod period]) and its gradient by sorted tokens:
-//     dW[v] = s * sum over t with id_t = v, in the order of t, of dy[t]
-// dense, a row of zeros where a token does not occur; every sum in 32 bits, in an order that is the same in every call (atomics into the
+//     dW[v] = s * sum over t with id_t = v of dy[t]
+// dense, a row of zeros where a token does not occur; every sum in 32 bits, in an order that the ids alone decide: by t within a tile of sorted pairs, then the tiles' sums in order (atomics into the
 // table would add in the order in which they arrive). Tokens outside 0 .. V - 1 and the padding token have no gradient.
 //
-//   embed_lookup the rows of W, eight values of 16 bits or four of 32 a thread, four such pieces under way; bound by HBM (with a CTA a token 16384 rows of
+//   embed_lookup the rows of W, eight values of 16 bits or four of 32 at a time, two such pieces a thread under way; bound by HBM (with a CTA a token 16384 rows of
 //                64 values took 21 us, the CTAs' launches). A token outside the table gives zeros
 //   embed_sort   (token, place) pairs by token, places of a token in order: a radix sort by one cluster of eight CTAs, which hold the counts of
 //                a digit in shared memory and read each other's totals there. T ids make 8 T bytes a pass: the sort is bound by its steps'
@@ -12,7 +12,9 @@
 //   embed_sum    a CTA takes L sorted pairs and a slice of the columns, reads their rows of dy once, and writes each token's sum. A token whose
 //                pairs lie in several CTAs leaves a partial sum in each (16384 x 4096 of 16 bits 26 us)
 //   embed_join   adds the partial sums of such a token, in order (8 us)
-// Together, captured: 16384 tokens into 151936 x 4096 in bf16 224 us, 4096 into 30522 x 768 in fp32 27; the lookup of 16384 rows of 4096 in bf16 43 us (6.2 TB/s).
+// Together, captured: 16384 tokens into 151936 x 4096 in bf16 224 us, 4096 into 30522 x 768 in fp32 27; the lookup of 16384 rows of 4096 in bf16 42 us (6.3 TB/s).
+// The order has its price where little is written: the lookup and the gradient of 1024 tokens into 6400 x 512 in bf16 take 20 us in a graph (zeros and atomics 10), of 64 tokens into
+// 1000 x 64 in fp32 13.6 (3.6), of 4096 into 6400 x 512 in bf16 24 (17): four launches that wait for one another, the sort's steps 7 to 13 us of it by themselves. Outside a graph the two are alike.
 #include "common.cuh"
 #include "../include/b200_ops.h"
 

@@ -14,9 +14,9 @@
 //   lp_finish      lp, H and what the backward pass needs, from the sums of a row's tiles
 //   lp_active, lp_gather, lp_return   rows whose tokens are not passed over, side by side, and their gradients back where they belong
 //   lp_scale, lp_cast   a power of two for fp16's gradients of single logits, and back
-// Rows of logits are bound by HBM where log probabilities alone are asked for (3000 x 151936 in bf16 141 us, 6.5 TB/s; gradients of 4096 rows 385, 6.5 TB/s): 6.8 instructions
-// and an exponential a 16-bit logit are just behind it (issue slots 55 % busy, exponential unit 72 %). With entropies, ranks and alternatives instructions
-// bound 16-bit rows (187 us), while rows of 32 bits stay near HBM (1000 x 151936 95 us, with all of them 107).
+// Rows of logits are bound by HBM where log probabilities alone are asked for (3000 x 151936 in bf16 139 us, 6.6 TB/s; gradients of 4096 rows 385, 6.5 TB/s): 5.1 instructions
+// and an exponential a 16-bit logit are just behind it (issue slots 43 % busy, exponential unit 76 %). With entropies, ranks and alternatives it is 9.2 instructions
+// and a row's last steps that 16-bit rows wait for (187 us), while rows of 32 bits stay near HBM (1000 x 151936 93 us, with all of them 106).
 #include "logprob_math.cuh"
 #include "../include/b200_ops.h"
 #include <type_traits>
@@ -312,7 +312,7 @@ __device__ __forceinline__ void lp_top_of_threads(const T* __restrict__ p, int n
 
 // The same for long rows, from the largest value of each segment of 2^SEG vectors. The k segments with the largest of those (the first ones among equals) have all k of them:
 // whatever stands in another segment comes behind the largest of each of these. They are read again as whole lines (what 20 threads had seen, a sector
-// here and there, was a third of a row of 16 bits: 3000 x 151936 with 20 alternatives 239 us, now 184).
+// here and there, was a third of a row of 16 bits: 3000 x 151936 with 20 alternatives 239 us, now 168).
 template <typename T, int NT, int SEG>
 __device__ __forceinline__ void lp_top_of_segments(const T* __restrict__ p, int n, int id0, int k, LpWalk at, LpShared<NT>& sh) {
   constexpr int N = LpVec<T>::N, CAP = LpShared<NT>::kList, EACH = NT / 64;

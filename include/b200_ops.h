@@ -853,8 +853,8 @@ int b200_logprob_cast(const float* x, void* y, long long n, const float* scale, 
  * row of the table. */
 int b200_embedding_lookup(const long long* ids, const void* table, const void* pos_table, void* out, long long T, int V, int D, int period, float scale, int dtype,
                           void* stream);
-/* Gradient of an embedding table by sorted tokens (csrc/embedding.cu): out [V, D] (dtype or fp32, 32-byte aligned) = scale * sum of dy[t] over ids[t] = row, in the
- * order of t, zeros elsewhere. dy [T, D] with row stride rs. Ids outside 0 .. V - 1 and `padding` (-1: none) add nothing. workspace: this many bytes, 16-byte
+/* Gradient of an embedding table by sorted tokens (csrc/embedding.cu): out [V, D] (dtype or fp32, 32-byte aligned) = scale * sum of dy[t] over ids[t] = row, in an
+ * order that the ids alone decide, zeros elsewhere. dy [T, D] with row stride rs. Ids outside 0 .. V - 1 and `padding` (-1: none) add nothing. workspace: this many bytes, 16-byte
  * aligned, of this call alone while it runs. */
 long long b200_embedding_grad_workspace(long long T, int D);
 int b200_embedding_grad(const long long* ids, const void* dy, long long rs, void* out, long long T, int V, int D, float scale, long long padding, int dtype,

@@ -302,7 +302,8 @@ def _embedding_work(tokens: int, columns: int) -> int:
 
 def embedding_grad(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
                    dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """[rows, D] = ``scale * sum of dout[t] over the t with ids[t] = row``, in the order of t: the gradient of ``embedding``'s table. ``ids`` int64 [...], ``dout``
+    """[rows, D] = ``scale * sum of dout[t] over the t with ids[t] = row``, the same bits in every call (the order of the sums is
+    that of t within tiles of the sorted tokens, then of the tiles): the gradient of ``embedding``'s table. ``ids`` int64 [...], ``dout``
     [..., D] (fp32, bf16 or fp16), ``dtype`` its own type or fp32. Sums in 32 bits, rounded once. Tokens outside 0 .. rows - 1 and ``padding_idx`` add nothing."""
     if ids.dtype != torch.int64 or dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.device != ids.device:
         raise ValueError("embedding_grad: ids must be int64 [...] and dout [..., D] on the same device")

@@ -179,7 +179,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top: int = 0, entropy: bool = False, rank: bool = False,
                    temperature: float = 1.0) -> TokenLogprobs:
-    """``logits`` [..., vocab] (fp32, bf16 or fp16; rows may be strided), ``tokens`` int64 [...] (None: no tokens are given, for entropies and
+    """``logits`` [..., vocab] (fp32, bf16 or fp16; rows an equal distance apart are read where they are, others, as of ``logits[:, :-1]`` of several sequences, are copied
+    first, in the backward pass too), ``tokens`` int64 [...] (None: no tokens are given, for entropies and
     alternatives alone). ``top``: how many alternatives, up to ``MAX_TOP``. Sums in 32 bits. A row of minus infinities alone, or with a NaN or plus infinity,
     gives NaN, as log_softmax does. Ranks and alternatives are those of the logits as they are given."""
     shape = logits.shape
