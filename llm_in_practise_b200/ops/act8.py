@@ -251,9 +251,9 @@ class _NoDraws(TorchDispatchMode):
 
     @staticmethod
     def _drew(func, args, kwargs):
-        """Attention counts as drawing, whatever its dropout."""
+        """Attention and recurrent layers count as drawing, whatever their dropout."""
         for i, a in enumerate(func._schema.arguments):
-            if a.name == "dropout_p":
+            if a.name in ("dropout_p", "dropout"):
                 return bool(args[i] if i < len(args) else kwargs.get(a.name, a.default_value))
         return True
 

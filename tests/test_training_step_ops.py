@@ -833,6 +833,15 @@ def test_checkpoints_in_a_capture_refuse_torchs_random_numbers(name, monkeypatch
     checkpoint8(lambda d, r: (draw(d), d), x, None)[0].sum().backward()
 
 
+def test_which_operators_draw():
+    ops, x = torch.ops.aten, torch.zeros(2)
+    for op, args, kw, draws in ((ops.native_dropout.default, (x, 0.5, True), {}, True), (ops.uniform_.default, (x,), {}, True),
+                                (ops._scaled_dot_product_flash_attention.default, (x, x, x), {}, False), (ops._scaled_dot_product_flash_attention.default, (x, x, x, 0.1), {}, True),
+                                (ops._scaled_dot_product_flash_attention.default, (x, x, x), {"dropout_p": 0.1}, True),
+                                (ops._cudnn_rnn.default, (x, [x], 4, None, x, None, 2, 4, 0, 1, False, 0.0, True, False, [], None), {}, False)):
+        assert torch.Tag.nondeterministic_seeded in op.tags and act8._NoDraws._drew(op, args, kw) == draws
+
+
 @gpu
 def test_captured_checkpoints():
     """A captured step gives the gradients of an eager one, whose dropout is the package's; one that draws from torch's generator is an error, and the capture after it is
